@@ -65,6 +65,10 @@ LIBRARIES: Dict[str, Sequence[str]] = {
     "routed": ("routed.cu",),
     # residuals of several streams that every sublayer reads and writes through small matrices
     "streams": ("stream_norm.cu",),
+    # the gated delta rule over per-request state, and the convolution and gates in front of it
+    "delta": ("delta_rule.cu", "delta_prep.cu"),
+    # blocks copied inside pools of pages and of states: forked requests, compaction
+    "blocks": ("copy_blocks.cu",),
 }
 # specialisations compiled by build_all() beside the default form of every library
 DEFAULT_SPECIALISATIONS = {"attn_mma": [("-DHEAD_DIM=128",)],

@@ -1,0 +1,16 @@
+// Arguments shared by the two forms of the gated delta rule (delta_rule.cu has the formulas).
+#pragma once
+
+namespace fsie {
+
+struct DeltaParams {
+    const void* qkv; int ld, q_off, k_off, v_off;          // [tokens, ld]; heads / share q and k columns of dim, heads of vdim
+    const float* log_decay; const float* beta;             // [tokens, heads]
+    const int* item_qstart; const int* item_qlen; const int* item_slots;   // [items]
+    float* state; long long state_stride;                  // [slots], S [heads, dim, vdim] in front of each
+    float* out;                                            // [tokens, heads * vdim]
+    int heads, dim, vdim, share;
+    float scale, eps;
+};
+
+}  // namespace fsie

@@ -2279,3 +2279,158 @@ def stream_norm(x: torch.Tensor, start: Optional[torch.Tensor], delta: Optional[
                                           float(eps), int(write_x), int(centred), _tag(dtype), int(early), _stream()),
            "stream_norm")
     return out
+
+
+# ------------------------------------------------------------------ the gated delta rule
+_delta = None
+
+
+def delta():
+    """The gated delta rule and what stands in front of it."""
+    global _delta
+    if _delta is None:
+        lib = build.load_library("delta")
+        i, f, ll, p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
+        lib.fsie_delta_prep.argtypes = [p, i, i, i, i, p, p, p, p, p, i, i, p, ll, ll, p, i, i, p, p, i, p, p, p, i, i, p]
+        lib.fsie_delta_prep_max_taps.argtypes = []
+        lib.fsie_delta_rule.argtypes = [i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, i, p]
+        lib.fsie_delta_max_dim.argtypes = []
+        for name in ("fsie_delta_prep", "fsie_delta_prep_max_taps", "fsie_delta_rule", "fsie_delta_max_dim"):
+            getattr(lib, name).restype = i
+        _delta = build.fast_calls(lib)
+    return _delta
+
+
+def delta_prep_max_taps() -> int:
+    return int(delta().fsie_delta_prep_max_taps())
+
+
+def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_qstart: torch.Tensor,
+               item_qlen: torch.Tensor, item_slots: torch.Tensor, items: int, seg_item: torch.Tensor,
+               seg_row0: torch.Tensor, num_segs: int, seg_tokens: int, state: Optional[torch.Tensor], tail_off: int,
+               conv_wt: torch.Tensor, a_log: torch.Tensor, dt_bias: torch.Tensor, act: torch.Tensor,
+               log_decay: torch.Tensor, beta: torch.Tensor, early: bool = False) -> None:
+    """What `gated_delta_rule` reads, per token of proj [tokens, ld] (the stored projection): act [tokens, channels] of its
+    type = silu(causal convolution of the columns from conv_off on), log_decay [tokens, heads] = -exp(a_log) *
+    softplus(proj[:, a_off + h] + dt_bias), beta [tokens, heads] = sigmoid(proj[:, b_off + h]), both float32.  conv_wt
+    float32 [taps, channels], the last row the current token's weights; the inputs of the taps - 1 tokens before a step's
+    first live in the request's slot of `state` [slots, n] (float32) from float tail_off on, oldest first, and are moved on.
+    seg_item / seg_row0 (int32): the tiles of `seg_tokens` tokens (at least taps - 1), listed request by request.
+    `early`: see the module's first lines; the slots are read behind the wait."""
+    _need(proj, None, "proj")
+    _need(act, proj.dtype, "act")
+    for name, t in (("conv_wt", conv_wt), ("a_log", a_log), ("dt_bias", dt_bias), ("log_decay", log_decay), ("beta", beta)):
+        _need(t, torch.float32, name)
+    for name, t in (("item_qstart", item_qstart), ("item_qlen", item_qlen), ("item_slots", item_slots),
+                    ("seg_item", seg_item), ("seg_row0", seg_row0)):
+        _need(t, torch.int32, name)
+    tokens, ld = proj.shape
+    taps, channels = conv_wt.shape
+    heads = a_log.numel()
+    if min(conv_off, a_off, b_off, tail_off) < 0 or conv_off + channels > ld or max(a_off, b_off) + heads > ld or \
+            act.numel() < tokens * channels or min(log_decay.numel(), beta.numel()) < tokens * heads or dt_bias.numel() != heads:
+        raise KernelError("delta_prep: shapes do not fit")
+    if min(item_qstart.numel(), item_qlen.numel(), item_slots.numel()) < items or min(seg_item.numel(), seg_row0.numel()) < num_segs:
+        raise KernelError("delta_prep: the lists are shorter than the requests or tiles")
+    stride = 0
+    if taps > 1:
+        _need(state, torch.float32, "state", contiguous=False)
+        stride = state.stride(0)
+        if tail_off + (taps - 1) * channels > stride:
+            raise KernelError("delta_prep: the state slots do not hold the convolution's inputs")
+    _check(delta().fsie_delta_prep(proj, ld, conv_off, a_off, b_off, item_qstart, item_qlen, item_slots, seg_item, seg_row0,
+                                   num_segs, seg_tokens, state, stride, tail_off, conv_wt, taps, channels, a_log, dt_bias,
+                                   heads, act, log_decay, beta, _tag(proj.dtype), int(early), _stream()), "delta_prep")
+
+
+def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_decay: torch.Tensor, beta: torch.Tensor,
+                     item_qstart: torch.Tensor, item_qlen: torch.Tensor, item_slots: torch.Tensor, items: int,
+                     state: torch.Tensor, out: torch.Tensor, heads: int, dim: int, vdim: int, share: int = 1,
+                     scale: Optional[float] = None, eps: float = 1e-6, longest: int = 0, early: bool = False) -> torch.Tensor:
+    """Per request and head, token by token, with q and k divided by sqrt(their squared length + eps) and
+    a = exp(log_decay):
+
+        u = beta (v - a S^T k)      S = a S + k u^T      o = scale S^T q
+
+    qkv [tokens, ld] (either storage type) holds q, k and v at the given column offsets; `share` heads in a row read the
+    same q and k columns (q and k then hold heads / share column groups of `dim`).  log_decay (at most 0) and beta
+    (0 to 2) are float32 [tokens, heads]; state [slots, n] float32 with the heads' matrices [heads, dim, vdim] in the first
+    heads * dim * vdim floats of a slot is read and left updated; out [tokens, heads * vdim] float32.  A request with a
+    negative slot is passed over, its rows of `out` stay as they are.  `scale`: dim ** -0.5 unless given.  `longest`: the
+    tokens of the step's longest request, which choose the kernel (0: not known to the caller).  dim is 256 at most.
+    `early`: the state and the lists are older than the stream's last kernel, see the module's first lines."""
+    _need(qkv, None, "qkv")
+    for name, t in (("log_decay", log_decay), ("beta", beta), ("out", out)):
+        _need(t, torch.float32, name)
+    _need(state, torch.float32, "state", contiguous=False)
+    for name, t in (("item_qstart", item_qstart), ("item_qlen", item_qlen), ("item_slots", item_slots)):
+        _need(t, torch.int32, name)
+    tokens, ld = qkv.shape
+    if min(heads, dim, vdim, share) <= 0 or heads % share:
+        raise KernelError("gated_delta_rule: sizes must be positive and heads a multiple of share")
+    narrow = heads // share * dim
+    if min(q_off, k_off, v_off) < 0 or max(q_off, k_off) + narrow > ld or v_off + heads * vdim > ld:
+        raise KernelError("gated_delta_rule: the rows are narrower than q, k and v")
+    if min(log_decay.numel(), beta.numel()) < tokens * heads or out.numel() < tokens * heads * vdim:
+        raise KernelError("gated_delta_rule: log_decay, beta or out is too small")
+    stride = state.stride(0)
+    if stride < heads * dim * vdim or state[0].numel() < heads * dim * vdim or not state[0].is_contiguous():
+        raise KernelError("gated_delta_rule: the state slots do not hold the heads' matrices")
+    if min(item_qstart.numel(), item_qlen.numel(), item_slots.numel()) < items:
+        raise KernelError("gated_delta_rule: the lists are shorter than the requests")
+    if not eps > 0:
+        raise KernelError("gated_delta_rule: eps must be positive")
+    if dim > delta().fsie_delta_max_dim():
+        raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {delta().fsie_delta_max_dim()}")
+    _check(delta().fsie_delta_rule(0, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots, items,
+                                   state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
+                                   float(eps), _tag(qkv.dtype), int(early), _stream()), "gated_delta_rule")
+    return out
+
+
+# ------------------------------------------------------------------ copies inside pools of blocks
+_blocks = None
+
+
+def blocks_lib():
+    """Copies of blocks inside pools of equal blocks."""
+    global _blocks
+    if _blocks is None:
+        lib = build.load_library("blocks")
+        i, ll, p = ctypes.c_int, ctypes.c_longlong, ctypes.c_void_p
+        lib.fsie_copy_blocks.argtypes = [p, i, ll, i, p, i, p, p]
+        lib.fsie_copy_max_buffers.argtypes = []
+        lib.fsie_copy_blocks.restype = lib.fsie_copy_max_buffers.restype = i
+        _blocks = build.fast_calls(lib)
+    return _blocks
+
+
+def copy_blocks(buffers, moves: torch.Tensor, error: torch.Tensor) -> None:
+    """buffer[dst] = buffer[src] for every buffer of the list `buffers` and every row (src, dst) of moves (int32 [n, 2], on the
+    device).  The buffers are contiguous, of any types, with equally many blocks (their first dimension) of equally many
+    bytes.  No block may be a destination twice, or a source and a destination: all pairs are copied side by side.  A pair
+    outside the pool is left out and sets error[0] (int32)."""
+    _need(moves, torch.int32, "moves")
+    _need(error, torch.int32, "error")
+    if moves.dim() != 2 or moves.shape[1] != 2:
+        raise KernelError("copy_blocks: moves must be [n, 2]")
+    buffers = list(buffers)
+    if not buffers:
+        return
+    blocks, size = None, None
+    for buffer in buffers:
+        _need(buffer, None, "buffers")
+        if buffer.dim() < 1:
+            raise KernelError("copy_blocks: a buffer needs a dimension of blocks")
+        mine = (buffer.shape[0], buffer.numel() // max(1, buffer.shape[0]) * buffer.element_size())
+        if blocks is None:
+            blocks, size = mine
+        elif mine != (blocks, size):
+            raise KernelError("copy_blocks: the buffers differ in blocks or bytes per block")
+    lib = blocks_lib()
+    most = lib.fsie_copy_max_buffers()
+    for first in range(0, len(buffers), most):
+        part = buffers[first:first + most]
+        bases = (ctypes.c_longlong * len(part))(*[b.data_ptr() for b in part])
+        _check(lib.fsie_copy_blocks(ctypes.addressof(bases), len(part), size, blocks, moves, moves.shape[0], error, _stream()),
+               "copy_blocks")
