@@ -66,7 +66,7 @@ LIBRARIES: Dict[str, Sequence[str]] = {
     # residuals of several streams that every sublayer reads and writes through small matrices
     "streams": ("stream_norm.cu",),
     # the gated delta rule over per-request state, and the convolution and gates in front of it
-    "delta": ("delta_rule.cu", "delta_prep.cu"),
+    "delta": ("delta_rule.cu", "delta_chunk.cu", "delta_prep.cu"),
     # blocks copied inside pools of pages and of states: forked requests, compaction
     "blocks": ("copy_blocks.cu",),
 }

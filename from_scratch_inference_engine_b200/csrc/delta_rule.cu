@@ -8,7 +8,7 @@
 // value goes in, so - other than in the scans of lightning.cu - a chunk's tokens depend on one another through a
 // triangular system and not only through sums.
 //
-// This file: the recurrent form, for steps of few tokens per request and for any sizes.
+// This file: the recurrent form, for steps of few tokens per request and for any sizes.  delta_chunk.cu: the chunked form.
 #include "common.cuh"
 #include "delta_rule.cuh"
 #include <math.h>
@@ -160,6 +160,8 @@ static int launch_step(const DeltaParams& p, int items, int early, cudaStream_t 
     return launch_dependent_if(early, kernel, grid, dim3(STEP_THREADS), 0, stream, p);
 }
 
+int delta_chunk(const DeltaParams& p, int items, int dtype, int early, cudaStream_t stream);       // delta_chunk.cu
+
 }  // namespace fsie
 
 using namespace fsie;
@@ -181,6 +183,7 @@ int fsie_delta_rule(int form, const void* qkv, int ld, int q_off, int k_off, int
     p.state = state; p.state_stride = state_stride; p.out = out;
     p.heads = heads; p.dim = dim; p.vdim = vdim; p.share = share; p.scale = scale; p.eps = eps;
     if (dtype != DTYPE_F32 && dtype != DTYPE_BF16) return ERR_BAD_ARGUMENT;
+    if (form == 1) return delta_chunk(p, items, dtype, early, stream);
     return dtype == DTYPE_F32 ? launch_step<float>(p, items, early, stream) : launch_step<bf16>(p, items, early, stream);
 }
 

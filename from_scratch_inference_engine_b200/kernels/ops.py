@@ -2294,8 +2294,9 @@ def delta():
         lib.fsie_delta_prep.argtypes = [p, i, i, i, i, p, p, p, p, p, i, i, p, ll, ll, p, i, i, p, p, i, p, p, p, i, i, p]
         lib.fsie_delta_prep_max_taps.argtypes = []
         lib.fsie_delta_rule.argtypes = [i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, i, p]
-        lib.fsie_delta_max_dim.argtypes = []
-        for name in ("fsie_delta_prep", "fsie_delta_prep_max_taps", "fsie_delta_rule", "fsie_delta_max_dim"):
+        lib.fsie_delta_max_dim.argtypes = lib.fsie_delta_chunk_max_dim.argtypes = []
+        for name in ("fsie_delta_prep", "fsie_delta_prep_max_taps", "fsie_delta_rule", "fsie_delta_max_dim",
+                     "fsie_delta_chunk_max_dim"):
             getattr(lib, name).restype = i
         _delta = build.fast_calls(lib)
     return _delta
@@ -2343,6 +2344,9 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
                                    heads, act, log_decay, beta, _tag(proj.dtype), int(early), _stream()), "delta_prep")
 
 
+DELTA_FEW_TOKENS = 16      # up to so many tokens of a request the recurrent form walks them one by one
+
+
 def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_decay: torch.Tensor, beta: torch.Tensor,
                      item_qstart: torch.Tensor, item_qlen: torch.Tensor, item_slots: torch.Tensor, items: int,
                      state: torch.Tensor, out: torch.Tensor, heads: int, dim: int, vdim: int, share: int = 1,
@@ -2382,7 +2386,8 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
         raise KernelError("gated_delta_rule: eps must be positive")
     if dim > delta().fsie_delta_max_dim():
         raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {delta().fsie_delta_max_dim()}")
-    _check(delta().fsie_delta_rule(0, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots, items,
+    chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= delta().fsie_delta_chunk_max_dim()
+    _check(delta().fsie_delta_rule(int(chunked), qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots, items,
                                    state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
                                    float(eps), _tag(qkv.dtype), int(early), _stream()), "gated_delta_rule")
     return out
