@@ -15,21 +15,26 @@
 // scaled by a power of two to a length of about one are exact in half precision; what is 32-bit - the state, R, U, T and the
 // weights of u_j - goes into the instructions as the sum of two half-precision numbers (22 bits), products of two low parts left
 // out.  Half precision has little range: every column of the state (a row of the transposed tiles below) has a power of
-// two, `sigma`, that keeps a bound on the column, its R and its U below 2^13; the bound follows the recurrence (a token
-// adds at most beta |v|) and is taken anew from the state itself every 32 chunks.  The state itself stays in 32-bit registers
+// two, `sigma`, chosen from the column's and the chunk's own largest numbers every 8 chunks, and anew, with the chunk's
+// sums taken again, whenever a number of R leaves the range in between.  The state itself stays in 32-bit registers
 // and the instructions only ever sum up one chunk (their running sums are truncated, not rounded).  float32 storage: q and k
 // are two parts as well.
 //
-// Layout.  A warp owns 16 value columns x 64 rows of S, transposed: S^T is the 16-row operand of S0^T k and S0^T q, the
-// accumulator of S0^T k is (after R) the operand of the next product in the registers where it lies, and the new sums end up
-// where S lies.  Heads of more than 64 rows take two warps per 16 columns, which swap their halves' sums through shared memory
-// once per chunk.  Four more warps ("makers") prepare the chunks that the others walk: warp m makes chunks m, m + 4, ... in its
-// own stage of a ring of four - q and k in half precision, T by substitution, the weights, the chunk's v.  Named barriers
-// hand stages over; nothing spins.
+// Two kernels.  The first prepares all chunks side by side, a warp per chunk and q/k head: q and k in half precision, T by
+// substitution, the weights of u_j, the gates' factors, as records in the workspace that lie as the second kernel's shared
+// memory holds them.  The second walks a head's chunks, a block for every 16 GROUPS value columns, its fifth warp copying the
+// records and the chunk's v into a ring of stages; named barriers hand the stages over, nothing spins.  (One kernel in which
+// four more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads: every block of value columns
+// prepared them again, and the two roles' code did not fit the instruction cache together.)
+//
+// Layout.  A warp of the second kernel owns 16 value columns x 64 rows of S, transposed: S^T is the 16-row operand of S0^T k
+// and S0^T q, the accumulator of S0^T k is (after R) the operand of the next product in the registers where it lies, and the
+// new sums end up where S lies.  Heads of more than 64 rows take two warps per 16 columns, which swap their halves' sums
+// through shared memory once per chunk.
 //
 // Values that are not finite: they spoil their column from their token on and nothing else, as in the recurrence - a product
-// with a zero of T would spoil the tokens before.  Such chunks are noticed after U and redone with those values left out, and
-// what they reach is set to NaN.
+// with a zero of T would spoil the tokens before.  Such chunks are noticed by R and by a mark in their record, redone with those
+// values left out, and what they reach is set to NaN.
 #include "common.cuh"
 #include "delta_rule.cuh"
 #include <cuda_fp16.h>
@@ -38,12 +43,17 @@
 namespace fsie {
 
 constexpr int DC_TOKENS = 16;              // tokens of a chunk
-constexpr int DC_STAGES = 4;               // stages of the ring = makers
+constexpr int DC_STAGES = 5;               // stages of the ring
+constexpr int DC_AHEAD = 2;                // chunks whose copies are under way
+constexpr int DC_WALKERS = 4;              // warps that walk a block's chunks
 constexpr int DC_SLICE = 64;               // rows of S (columns of k) per warp
 constexpr int DC_MAX_DIM = 128;
-constexpr int DC_REFRESH = 32;             // chunks between two looks at the state's size
+constexpr int DC_REFRESH = 8;              // chunks between two looks at the state's size
+constexpr int DC_SIZE = 4;                 // ... which brings the largest number of a column to 2^4 .. 2^5
 constexpr int DC_TLD = DC_TOKENS + 8;      // padded rows: ldmatrix without bank conflicts
-constexpr float DC_MOST = 8192.f;          // sigma times a column's bound stays below this
+// A number of R, times sigma, is below this: a row of T has at most 16 numbers of at most beta^2 <= 4 (what a token's value
+// still does to a later token's u passes through contractions), so that u, and u with a factor of at most 2, fit half precision.
+constexpr float DC_MOST = 500.f;
 
 __device__ __forceinline__ unsigned dc_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void dc_ldmatrix(unsigned (&r)[4], const void* p) {
@@ -129,161 +139,214 @@ __device__ __forceinline__ void dc_store8(float* p, const Raw8<float>& r) {
     *reinterpret_cast<float4*>(p) = r.x; *reinterpret_cast<float4*>(p + 4) = r.y;
 }
 
-template <typename T, int DK, int WALKERS>
+template <typename T, int DK>
 struct DcShape {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;       // half-precision numbers that hold a stored one
     static constexpr int SLICES = DK / DC_SLICE;               // warps that share 16 value columns
-    static constexpr int GROUPS = WALKERS / SLICES;            // groups of 16 value columns
+    static constexpr int GROUPS = DC_WALKERS / SLICES;         // groups of 16 value columns
     static constexpr int COLS = 16 * GROUPS;                   // value columns of a block
     static constexpr int KLD = DK + 8;                         // padded row of q and k
     static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 8);
-    static constexpr int THREADS = 32 * (WALKERS + DC_STAGES);
-    struct Stage {
-        __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD];
+    static constexpr int THREADS = 32 * (DC_WALKERS + 1);
+    struct alignas(16) Keys { __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD]; };
+    struct alignas(16) Gates {
         __half t[2][DC_TOKENS][DC_TLD], p[2][DC_TOKENS][DC_TLD];     // T and the weights of u_j, two parts each
-        T v[DC_TOKENS][VLD];
         float before[DC_TOKENS];          // on S0^T k: e^(G_i), the key's length, the power of two
         float after[DC_TOKENS];           // on u_j in the new state: e^(G_15 - G_j), ...
         float query[DC_TOKENS];           // on an output: scale, the query's length, the power of two
         float fade[DC_TOKENS];            // e^(G_i)
-        float v_most[COLS];               // largest |v| per column
+        float odd[4];                     // NaN where T has a number that is not finite, else 0
     };
-    struct Scratch { float a[DC_TOKENS][DC_TOKENS + 4]; double g[DC_TOKENS]; float f[DC_TOKENS], beta[DC_TOKENS]; };
+    struct alignas(16) Stage { Keys keys; Gates gates; T v[DC_TOKENS][VLD]; };
     struct Shared {
         Stage stage[DC_STAGES];
-        Scratch scratch[DC_STAGES];
-        float4 swap[2][WALKERS][3][32];
-        float norm[WALKERS][16];
+        float4 swap[2][DC_WALKERS][3][32];
+        float most[DC_WALKERS][16];
     };
 };
 
-enum { DC_FULL = 1, DC_EMPTY = DC_FULL + DC_STAGES, DC_PAIR = DC_EMPTY + DC_STAGES };       // named barriers
+// What the two kernels share beside the rule's arguments: the records, [chunk][q/k head] and [chunk][head].  Chunks are
+// numbered request after request, those of a request from its first token on; `chunks` is what the workspace has room for.
+struct DcRecords { unsigned char* keys; unsigned char* gates; int items, chunks; };
 
-template <typename T, int DK, int WALKERS, bool WIDE>
-__device__ __forceinline__ void dc_make(const DeltaParams& p, typename DcShape<T, DK, WALKERS>::Shared& sm, int maker, int lane,
-                                        int head, int col0, int t0, int count, int chunks) {
-    using Sh = DcShape<T, DK, WALKERS>;
+// The number of chunks in front of request `item`, by all lanes of a warp.
+__device__ __forceinline__ int dc_chunks_before(const int* __restrict__ item_qlen, int item, int lane) {
+    int sum = 0;
+    for (int i = lane; i < item; i += 32) sum += (max(item_qlen[i], 0) + DC_TOKENS - 1) / DC_TOKENS;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
+constexpr int DC_MAKERS = 4;               // warps of a preparing block
+
+// a warp per chunk and q/k head
+template <typename T, int DK, bool WIDE>
+__global__ void __launch_bounds__(32 * DC_MAKERS)
+delta_records_kernel(const DeltaParams p, const DcRecords records) {
+    using Sh = DcShape<T, DK>;
     constexpr int PARTS = Sh::PARTS, FOURS = DK / 32;          // 32 columns are a quad's eight each
-    auto& st = sm.stage[maker];
-    auto& own = sm.scratch[maker];
+    struct Scratch { float a[DC_TOKENS][DC_TOKENS + 4]; double g[DC_TOKENS]; float f[DC_TOKENS], beta[DC_TOKENS]; };
+    __shared__ Scratch scratch[DC_MAKERS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
+    auto& own = scratch[warp];
+    const int narrow_heads = p.heads / p.share;
+    const long long unit = (long long)blockIdx.x * DC_MAKERS + warp;
+    const int chunk = (int)(unit / narrow_heads), narrow = (int)(unit - (long long)chunk * narrow_heads);
+    // the chunk's request and first token: 32 requests at a time
+    int item = -1, place = 0;
+    for (int i0 = 0, before = 0; i0 < records.items && item < 0; i0 += 32) {
+        const int i = i0 + lane, have = i < records.items ? (max(p.item_qlen[i], 0) + DC_TOKENS - 1) / DC_TOKENS : 0;
+        int upto = have;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int left = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += left;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, before + upto > chunk && before + upto - have <= chunk);
+        if (here) {
+            const int at = __ffs(here) - 1;
+            item = i0 + at;
+            place = chunk - __shfl_sync(0xffffffffu, before + upto - have, at);
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const int slot = item >= 0 ? p.item_slots[item] : -1, count = item >= 0 ? p.item_qlen[item] : 0;
+    const int first = item >= 0 ? p.item_qstart[item] + place * DC_TOKENS : 0, n = min(DC_TOKENS, count - place * DC_TOKENS);
+    grid_dependency_wait();
+    grid_dependents_go();
+    if (slot < 0 || chunk >= records.chunks) return;           // beyond the step's chunks, or a padding entry
     const T* qkv = (const T*)p.qkv;
-    const int narrow = head / p.share * p.dim;
-    for (int c = maker; c < chunks; c += DC_STAGES) {
-        const int first = t0 + c * DC_TOKENS, n = min(DC_TOKENS, count - c * DC_TOKENS);
-        // ---- q, k, v and gates on their way
-        Raw8<T> kr[2][FOURS], qr[2][FOURS];
+    // ---- q, k and the first head's gates on their way
+    Raw8<T> kr[2][FOURS], qr[2][FOURS];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = g + 8 * h;
-            const T* row = qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + narrow;
-#pragma unroll
-            for (int f = 0; f < FOURS; ++f) {
-                const int d = f * 32 + t * 8, have = r < n ? p.dim - d : 0;
-                kr[h][f] = dc_load8<WIDE>(row + p.k_off + d, have);
-                qr[h][f] = dc_load8<WIDE>(row + p.q_off + d, have);
-            }
-        }
-        constexpr int EIGHTS = Sh::COLS / 8, VLOADS = (DC_TOKENS * EIGHTS + 31) / 32;
-        Raw8<T> vr[VLOADS];
-#pragma unroll
-        for (int i = 0; i < VLOADS; ++i) {
-            const int e = lane + 32 * i, r = e / EIGHTS, d = col0 + (e % EIGHTS) * 8;
-            vr[i] = dc_load8<WIDE>(qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + p.v_off + head * p.vdim + d,
-                                   r < n ? p.vdim - d : 0);
-        }
-        float decay = 0.f, beta = 0.f;
-        if ((lane & 15) < n) {
-            decay = p.log_decay[(size_t)(first + (lane & 15)) * p.heads + head];
-            beta = p.beta[(size_t)(first + (lane & 15)) * p.heads + head];
-        }
-        // ---- lengths of q and k, a power of two that brings each below one, both in half precision
-        float kk[2], qq[2];
-        unsigned kh[PARTS][2][FOURS][4], qh[PARTS][2][FOURS][4];
-        float kf[2], qf[2];                                    // length and power of two as one factor
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            kk[h] = qq[h] = 0.f;
-            float x[8];
-#pragma unroll
-            for (int f = 0; f < FOURS; ++f) {
-                dc_widen(kr[h][f], x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) kk[h] = fmaf(x[i], x[i], kk[h]);
-                dc_widen(qr[h][f], x);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) qq[h] = fmaf(x[i], x[i], qq[h]);
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                kk[h] += __shfl_xor_sync(0xffffffffu, kk[h], o);
-                qq[h] += __shfl_xor_sync(0xffffffffu, qq[h], o);
-            }
-            const int ke = (((__float_as_int(kk[h]) >> 23) & 255) - 125) >> 1, qe = (((__float_as_int(qq[h]) >> 23) & 255) - 125) >> 1;
-            const float ks = dc_power(-ke), qs = dc_power(-qe);
-            kf[h] = dc_power(ke) / sqrtf(kk[h] + p.eps);
-            qf[h] = p.scale * (dc_power(qe) / sqrtf(qq[h] + p.eps));
-#pragma unroll
-            for (int f = 0; f < FOURS; ++f) {
-                dc_widen(kr[h][f], x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (PARTS == 2) dc_split(x[2 * i] * ks, x[2 * i + 1] * ks, kh[0][h][f][i], kh[PARTS - 1][h][f][i]);
-                    else kh[0][h][f][i] = dc_bits(__floats2half2_rn(x[2 * i] * ks, x[2 * i + 1] * ks));
-                }
-                dc_widen(qr[h][f], x);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (PARTS == 2) dc_split(x[2 * i] * qs, x[2 * i + 1] * qs, qh[0][h][f][i], qh[PARTS - 1][h][f][i]);
-                    else qh[0][h][f][i] = dc_bits(__floats2half2_rn(x[2 * i] * qs, x[2 * i + 1] * qs));
-                }
-            }
-        }
-        // ---- K K^T and Q K^T: a lane's eight neighbouring values are operand registers as they are, because both operands
-        // take their inner index in the same order
-        float kkt[2][2][4], qkt[2][2][4];                      // [two chains][columns 0-7, 8-15]
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) kkt[i][j][e] = qkt[i][j][e] = 0.f;
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h;
+        const T* row = qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + narrow * p.dim;
 #pragma unroll
         for (int f = 0; f < FOURS; ++f) {
+            const int d = f * 32 + t * 8, have = r < n ? p.dim - d : 0;
+            kr[h][f] = dc_load8<WIDE>(row + p.k_off + d, have);
+            qr[h][f] = dc_load8<WIDE>(row + p.q_off + d, have);
+        }
+    }
+    const int i = lane & 15;                                   // the lane's token (twice per warp)
+    float decay = 0.f, beta = 0.f;
+    if (i < n) {
+        decay = p.log_decay[(size_t)(first + i) * p.heads + narrow * p.share];
+        beta = p.beta[(size_t)(first + i) * p.heads + narrow * p.share];
+    }
+    // ---- lengths of q and k, a power of two that brings each below one, both in half precision
+    float kk[2], qq[2];
+    unsigned kh[PARTS][2][FOURS][4], qh[PARTS][2][FOURS][4];
+    float kf[2], qf[2];                                    // length and power of two as one factor
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {                      // inner 16 of the 32 columns
+    for (int h = 0; h < 2; ++h) {
+        kk[h] = qq[h] = 0.f;
+        float x[8];
 #pragma unroll
-                for (int pa = 0; pa < PARTS; ++pa) {
+        for (int f = 0; f < FOURS; ++f) {
+            dc_widen(kr[h][f], x);
 #pragma unroll
-                    for (int pb = 0; pb + pa < PARTS; ++pb) {
-                        const unsigned ka[4] = {kh[pa][0][f][2 * i], kh[pa][1][f][2 * i], kh[pa][0][f][2 * i + 1], kh[pa][1][f][2 * i + 1]};
-                        const unsigned qa[4] = {qh[pa][0][f][2 * i], qh[pa][1][f][2 * i], qh[pa][0][f][2 * i + 1], qh[pa][1][f][2 * i + 1]};
+            for (int i = 0; i < 8; ++i) kk[h] = fmaf(x[i], x[i], kk[h]);
+            dc_widen(qr[h][f], x);
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            dc_mma(kkt[i][j], ka, kh[pb][j][f][2 * i], kh[pb][j][f][2 * i + 1]);
-                            dc_mma(qkt[i][j], qa, kh[pb][j][f][2 * i], kh[pb][j][f][2 * i + 1]);
-                        }
+            for (int i = 0; i < 8; ++i) qq[h] = fmaf(x[i], x[i], qq[h]);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            kk[h] += __shfl_xor_sync(0xffffffffu, kk[h], o);
+            qq[h] += __shfl_xor_sync(0xffffffffu, qq[h], o);
+        }
+        const int ke = (((__float_as_int(kk[h]) >> 23) & 255) - 125) >> 1, qe = (((__float_as_int(qq[h]) >> 23) & 255) - 125) >> 1;
+        const float ks = dc_power(-ke), qs = dc_power(-qe);
+        kf[h] = dc_power(ke) / sqrtf(kk[h] + p.eps);
+        qf[h] = p.scale * (dc_power(qe) / sqrtf(qq[h] + p.eps));
+#pragma unroll
+        for (int f = 0; f < FOURS; ++f) {
+            dc_widen(kr[h][f], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (PARTS == 2) dc_split(x[2 * i] * ks, x[2 * i + 1] * ks, kh[0][h][f][i], kh[PARTS - 1][h][f][i]);
+                else kh[0][h][f][i] = dc_bits(__floats2half2_rn(x[2 * i] * ks, x[2 * i + 1] * ks));
+            }
+            dc_widen(qr[h][f], x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (PARTS == 2) dc_split(x[2 * i] * qs, x[2 * i + 1] * qs, qh[0][h][f][i], qh[PARTS - 1][h][f][i]);
+                else qh[0][h][f][i] = dc_bits(__floats2half2_rn(x[2 * i] * qs, x[2 * i + 1] * qs));
+            }
+        }
+    }
+    // ---- K K^T and Q K^T: a lane's eight neighbouring values are operand registers as they are, because both operands
+    // take their inner index in the same order
+    float kkt[2][2][4], qkt[2][2][4];                      // [two chains][columns 0-7, 8-15]
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kkt[i][j][e] = qkt[i][j][e] = 0.f;
+#pragma unroll
+    for (int f = 0; f < FOURS; ++f) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                      // inner 16 of the 32 columns
+#pragma unroll
+            for (int pa = 0; pa < PARTS; ++pa) {
+#pragma unroll
+                for (int pb = 0; pb + pa < PARTS; ++pb) {
+                    const unsigned ka[4] = {kh[pa][0][f][2 * i], kh[pa][1][f][2 * i], kh[pa][0][f][2 * i + 1], kh[pa][1][f][2 * i + 1]};
+                    const unsigned qa[4] = {qh[pa][0][f][2 * i], qh[pa][1][f][2 * i], qh[pa][0][f][2 * i + 1], qh[pa][1][f][2 * i + 1]};
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        dc_mma(kkt[i][j], ka, kh[pb][j][f][2 * i], kh[pb][j][f][2 * i + 1]);
+                        dc_mma(qkt[i][j], qa, kh[pb][j][f][2 * i], kh[pb][j][f][2 * i + 1]);
                     }
                 }
             }
         }
-        // ---- gates: sums of log_decay in 64 bits, so that a difference of two of them is as exact as its own terms
+    }
+    auto* keys = reinterpret_cast<typename Sh::Keys*>(records.keys) + ((size_t)chunk * narrow_heads + narrow);
+#pragma unroll
+    for (int part = 0; part < PARTS; ++part)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int f = 0; f < FOURS; ++f) {
+                const unsigned(&a)[4] = kh[part][h][f];
+                const unsigned(&b)[4] = qh[part][h][f];
+                *reinterpret_cast<uint4*>(&keys->k[part][g + 8 * h][f * 32 + t * 8]) = make_uint4(a[0], a[1], a[2], a[3]);
+                *reinterpret_cast<uint4*>(&keys->q[part][g + 8 * h][f * 32 + t * 8]) = make_uint4(b[0], b[1], b[2], b[3]);
+            }
+    const int from = (lane & 7) * 4;                           // a lane of the quad that holds row lane & 7
+    const float kf0 = __shfl_sync(0xffffffffu, kf[0], from), kf1 = __shfl_sync(0xffffffffu, kf[1], from);
+    const float qf0 = __shfl_sync(0xffffffffu, qf[0], from), qf1 = __shfl_sync(0xffffffffu, qf[1], from);
+    const float kfi = (lane & 8) ? kf1 : kf0, qfi = (lane & 8) ? qf1 : qf0;        // of token i
+    if (lane < DC_TOKENS) own.f[lane] = kfi;
+    // ---- the gates of every head that reads these q and k
+#pragma unroll 1
+    for (int z = 0; z < p.share; ++z) {
+        const int head = narrow * p.share + z;
+        auto* to = reinterpret_cast<typename Sh::Gates*>(records.gates) + ((size_t)chunk * p.heads + head);
+        // sums of log_decay in 64 bits, so that a difference of two of them is as exact as its own terms
         double sum = decay < -1e4f ? -1e4 : (double)decay;     // (e^-10000 is zero)
 #pragma unroll
         for (int o = 1; o < DC_TOKENS; o <<= 1) {
             const double left = __shfl_up_sync(0xffffffffu, sum, o, DC_TOKENS);
-            if ((lane & 15) >= o) sum += left;
+            if (i >= o) sum += left;
         }
         const double all = __shfl_sync(0xffffffffu, sum, DC_TOKENS - 1, DC_TOKENS);
-        const int from = (lane & 7) * 4;                       // a lane of the quad that holds row lane & 7
-        const float kf0 = __shfl_sync(0xffffffffu, kf[0], from), kf1 = __shfl_sync(0xffffffffu, kf[1], from);
-        const float qf0 = __shfl_sync(0xffffffffu, qf[0], from), qf1 = __shfl_sync(0xffffffffu, qf[1], from);
-        const float kfi = (lane & 8) ? kf1 : kf0, qfi = (lane & 8) ? qf1 : qf0;        // of token lane & 15
-        const float fade = expf((float)sum), after = expf((float)(all - sum)) * kfi;
-        __syncwarp();                                          // the last chunk's scratch has been read
-        if (lane < DC_TOKENS) { own.g[lane] = sum; own.f[lane] = kfi; own.beta[lane] = beta; }
+        if (lane < DC_TOKENS) { own.g[lane] = sum; own.beta[lane] = beta; }
+        const float fade = expf((float)sum);
+        if (lane < DC_TOKENS) {
+            to->before[lane] = fade * kfi; to->after[lane] = expf((float)(all - sum)) * kfi; to->query[lane] = qfi; to->fade[lane] = fade;
+        }
+        if (z + 1 < p.share && i < n) {                        // the next head's
+            decay = p.log_decay[(size_t)(first + i) * p.heads + head + 1];
+            beta = p.beta[(size_t)(first + i) * p.heads + head + 1];
+        }
         __syncwarp();
-        float weight[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int col = 8 * j + 2 * t;
@@ -294,16 +357,19 @@ __device__ __forceinline__ void dc_make(const DeltaParams& p, typename DcShape<T
                 const int row = g + 8 * h;
                 const double gr = own.g[row];
                 const float mine = own.beta[row] * own.f[row];
-                const float e0 = expf((float)(gr - g0)), e1 = expf((float)(gr - g1));
-                weight[j][2 * h] = row >= col ? (qkt[0][j][2 * h] + qkt[1][j][2 * h]) * f0 * e0 : 0.f;
-                weight[j][2 * h + 1] = row > col ? (qkt[0][j][2 * h + 1] + qkt[1][j][2 * h + 1]) * f1 * e1 : 0.f;
-                own.a[row][col] = row > col ? mine * f0 * (kkt[0][j][2 * h] + kkt[1][j][2 * h]) * e0 : 0.f;
-                own.a[row][col + 1] = row > col + 1 ? mine * f1 * (kkt[0][j][2 * h + 1] + kkt[1][j][2 * h + 1]) * e1 : 0.f;
+                const float e0 = expf((float)(gr - g0)) * f0, e1 = expf((float)(gr - g1)) * f1;
+                const float w0 = row >= col ? (qkt[0][j][2 * h] + qkt[1][j][2 * h]) * e0 : 0.f;
+                const float w1 = row > col ? (qkt[0][j][2 * h + 1] + qkt[1][j][2 * h + 1]) * e1 : 0.f;
+                unsigned high, low;
+                dc_split(w0, w1, high, low);
+                *reinterpret_cast<unsigned*>(&to->p[0][row][col]) = high;
+                *reinterpret_cast<unsigned*>(&to->p[1][row][col]) = low;
+                own.a[row][col] = row > col ? mine * (kkt[0][j][2 * h] + kkt[1][j][2 * h]) * e0 : 0.f;
+                own.a[row][col + 1] = row > col + 1 ? mine * (kkt[0][j][2 * h + 1] + kkt[1][j][2 * h + 1]) * e1 : 0.f;
             }
         }
         __syncwarp();
-        // ---- row i of (I + A)^-1 in lane i (and again in lane i + 16): from x (I + A) = e_i, last column first
-        const int i = lane & 15;
+        // row i of (I + A)^-1 in lane i (and again in lane i + 16): from x (I + A) = e_i, last column first
         float x[DC_TOKENS];
 #pragma unroll
         for (int j = 0; j < DC_TOKENS; ++j) x[j] = i == j ? 1.f : 0.f;
@@ -314,65 +380,77 @@ __device__ __forceinline__ void dc_make(const DeltaParams& p, typename DcShape<T
                 for (int j = 0; j < l; ++j) x[j] = fmaf(-x[l], own.a[l][j], x[j]);
             }
         }
+        bool finite = true;
 #pragma unroll
-        for (int j = 0; j < DC_TOKENS; ++j) x[j] = j <= i ? x[j] * own.beta[j] : 0.f;
-        // ---- into the stage, once its last chunk has been walked
-        if (c >= DC_STAGES) dc_sync(DC_EMPTY + maker, 32 * (WALKERS + 1));
+        for (int j = 0; j < DC_TOKENS; ++j) {
+            x[j] = j <= i ? x[j] * own.beta[j] : 0.f;
+            finite = finite && fabsf(x[j]) < INFINITY;
+        }
+        const bool odd = !__all_sync(0xffffffffu, finite);
+        if (lane == 0) to->odd[0] = odd ? __int_as_float(0x7fffffff) : 0.f;
+        unsigned high[DC_TOKENS / 2], low[DC_TOKENS / 2];
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
+        for (int j = 0; j < DC_TOKENS / 2; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
+        // the two lanes that hold a row write one part each
+        uint4* row = reinterpret_cast<uint4*>(&to->t[lane >> 4][i][0]);
+        const bool second = lane >= 16;
+        row[0] = second ? make_uint4(low[0], low[1], low[2], low[3]) : make_uint4(high[0], high[1], high[2], high[3]);
+        row[1] = second ? make_uint4(low[4], low[5], low[6], low[7]) : make_uint4(high[4], high[5], high[6], high[7]);
+        __syncwarp();
+    }
+}
+
+__device__ __forceinline__ void dc_copy16(void* dst, const void* src, bool there) {
+    const int bytes = there ? 16 : 0;                          // 0 source bytes: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dc_smem(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+enum { DC_FULL = 1, DC_EMPTY = DC_FULL + DC_STAGES, DC_PAIR = DC_EMPTY + DC_STAGES };       // named barriers
+static_assert(DC_PAIR + DC_WALKERS / 2 <= 16, "a block has 16 named barriers");
+
+// The fifth warp: records and v of one chunk after the other into the ring.
+template <typename T, int DK, bool WIDE>
+__device__ __forceinline__ void dc_fetch(const DeltaParams& p, const DcRecords& records, typename DcShape<T, DK>::Shared& sm, int lane,
+                                         int head, int col0, int t0, int count, int chunk0, int chunks) {
+    using Sh = DcShape<T, DK>;
+    const int narrow_heads = p.heads / p.share;
+    const auto* keys = reinterpret_cast<const typename Sh::Keys*>(records.keys) + ((size_t)chunk0 * narrow_heads + head / p.share);
+    const auto* gates = reinterpret_cast<const typename Sh::Gates*>(records.gates) + ((size_t)chunk0 * p.heads + head);
+    const T* v = (const T*)p.qkv + (size_t)t0 * p.ld + p.v_off + (size_t)head * p.vdim + col0;
+    for (int c = 0; c <= chunks + DC_AHEAD; ++c) {             // (the walkers' last meeting is for a stage that nobody fills)
+        if (c < chunks) {
+            auto& st = sm.stage[c % DC_STAGES];
+            if (c >= DC_STAGES) dc_sync(DC_EMPTY + c % DC_STAGES, 32 * (DC_WALKERS + 1));
+            const int n = min(DC_TOKENS, count - c * DC_TOKENS);
+            constexpr int PER = 16 / sizeof(T), ACROSS = Sh::COLS / PER;          // 16-byte pieces of a row of v
+#pragma unroll 4
+            for (int e = lane; e < (int)(sizeof(st.keys) / 16); e += 32)
+                dc_copy16(reinterpret_cast<uint4*>(&st.keys) + e, reinterpret_cast<const uint4*>(keys) + e, true);
+#pragma unroll 4
+            for (int e = lane; e < (int)(sizeof(st.gates) / 16); e += 32)
+                dc_copy16(reinterpret_cast<uint4*>(&st.gates) + e, reinterpret_cast<const uint4*>(gates) + e, true);
+            if constexpr (WIDE) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int f = 0; f < FOURS; ++f) {
-                    const unsigned(&a)[4] = kh[part][h][f];
-                    const unsigned(&b)[4] = qh[part][h][f];
-                    *reinterpret_cast<uint4*>(&st.k[part][g + 8 * h][f * 32 + t * 8]) = make_uint4(a[0], a[1], a[2], a[3]);
-                    *reinterpret_cast<uint4*>(&st.q[part][g + 8 * h][f * 32 + t * 8]) = make_uint4(b[0], b[1], b[2], b[3]);
+                for (int e = lane; e < DC_TOKENS * ACROSS; e += 32) {
+                    const int r = e / ACROSS, d = (e % ACROSS) * PER;
+                    const bool there = r < n && col0 + d < p.vdim;
+                    dc_copy16(&st.v[r][d], v + (there ? (size_t)r * p.ld + d : 0), there);
                 }
-        {
-            unsigned high[DC_TOKENS / 2], low[DC_TOKENS / 2];
-#pragma unroll
-            for (int j = 0; j < DC_TOKENS / 2; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
-            // the two lanes that hold a row write one part each
-            uint4* to = reinterpret_cast<uint4*>(&st.t[lane >> 4][i][0]);
-            const bool second = lane >= 16;
-            to[0] = second ? make_uint4(low[0], low[1], low[2], low[3]) : make_uint4(high[0], high[1], high[2], high[3]);
-            to[1] = second ? make_uint4(low[4], low[5], low[6], low[7]) : make_uint4(high[4], high[5], high[6], high[7]);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                unsigned high, low;
-                dc_split(weight[j][2 * h], weight[j][2 * h + 1], high, low);
-                *reinterpret_cast<unsigned*>(&st.p[0][g + 8 * h][8 * j + 2 * t]) = high;
-                *reinterpret_cast<unsigned*>(&st.p[1][g + 8 * h][8 * j + 2 * t]) = low;
+            } else {
+                for (int e = lane; e < DC_TOKENS * Sh::COLS; e += 32) {
+                    const int r = e / Sh::COLS, d = e % Sh::COLS;
+                    st.v[r][d] = r < n && col0 + d < p.vdim ? v[(size_t)r * p.ld + d] : from_float<T>(0.f);
+                }
             }
-        float most[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) most[k] = 0.f;
-#pragma unroll
-        for (int k = 0; k < VLOADS; ++k) {
-            const int e = lane + 32 * k;
-            if (e < DC_TOKENS * EIGHTS) dc_store8(&st.v[e / EIGHTS][(e % EIGHTS) * 8], vr[k]);
-            float y[8];
-            dc_widen(vr[k], y);
-#pragma unroll
-            for (int z = 0; z < 8; ++z)                        // (one that is not finite must not move its column's power)
-                most[z] = fmaxf(most[z], fabsf(y[z]) < INFINITY ? fabsf(y[z]) : 0.f);
+            keys += narrow_heads;
+            gates += p.heads;
+            v += (size_t)DC_TOKENS * p.ld;
         }
-#pragma unroll
-        for (int o = EIGHTS; o < 32; o <<= 1)
-#pragma unroll
-            for (int z = 0; z < 8; ++z) most[z] = fmaxf(most[z], __shfl_xor_sync(0xffffffffu, most[z], o));
-        if (lane < EIGHTS) {
-#pragma unroll
-            for (int z = 0; z < 8; ++z) st.v_most[lane * 8 + z] = most[z];
+        asm volatile("cp.async.commit_group;\n" ::: "memory");
+        if (c >= DC_AHEAD) {
+            asm volatile("cp.async.wait_group %0;\n" ::"n"(DC_AHEAD) : "memory");
+            dc_arrive(DC_FULL + (c - DC_AHEAD) % DC_STAGES, 32 * (DC_WALKERS + 1));
         }
-        if (lane < DC_TOKENS) {
-            st.before[lane] = fade * kfi; st.after[lane] = after; st.query[lane] = qfi; st.fade[lane] = fade;
-        }
-        dc_arrive(DC_FULL + maker, 32 * (WALKERS + 1));
     }
 }
 
@@ -413,10 +491,10 @@ __device__ __forceinline__ void dc_leave_out(float (&x)[2][4], int t, const int 
             if (8 * j + 2 * t + (e & 1) >= first[e >> 1]) x[j][e] = 0.f;
 }
 
-template <typename T, int DK, int WALKERS, bool WIDE>
-__global__ void __launch_bounds__(32 * (WALKERS + DC_STAGES), 1)
-delta_chunk_kernel(const DeltaParams p) {
-    using Sh = DcShape<T, DK, WALKERS>;
+template <typename T, int DK, bool WIDE>
+__global__ void __launch_bounds__(32 * (DC_WALKERS + 1), 2)
+delta_walk_kernel(const DeltaParams p, const DcRecords records) {
+    using Sh = DcShape<T, DK>;
     constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16;
     extern __shared__ __align__(16) unsigned char dc_raw[];
     auto& sm = *reinterpret_cast<typename Sh::Shared*>(dc_raw);
@@ -425,10 +503,12 @@ delta_chunk_kernel(const DeltaParams p) {
     const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
     if (slot < 0 || count <= 0) return;                        // a padding entry of a fixed-size batch
     const int chunks = (count + DC_TOKENS - 1) / DC_TOKENS;
-    if (warp >= WALKERS) {
+    const int chunk0 = dc_chunks_before(p.item_qlen, item, lane);
+    if (chunk0 + chunks > records.chunks) return;              // lists that name more tokens than there are
+    if (warp >= DC_WALKERS) {
         grid_dependency_wait();
         grid_dependents_go();
-        dc_make<T, DK, WALKERS, WIDE>(p, sm, warp - WALKERS, lane, head, col0, t0, count, chunks);
+        dc_fetch<T, DK, WIDE>(p, records, sm, lane, head, col0, t0, count, chunk0, chunks);
         return;
     }
     const int g = lane >> 2, t = lane & 3;
@@ -447,136 +527,21 @@ delta_chunk_kernel(const DeltaParams p) {
         }
     grid_dependency_wait();
     grid_dependents_go();
-    float sigma[2] = {1.f, 1.f}, bound[2] = {0.f, 0.f};        // of columns col and col + 8
+    float sigma[2] = {1.f, 1.f}, back[2] = {1.f, 1.f};         // of columns col and col + 8, and one over it
     unsigned sh[STEPS][4], sl[STEPS][4];
 #pragma unroll
     for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
     const int b_row = (lane & 7) + 8 * (lane >> 4), b_col = 8 * ((lane >> 3) & 1);      // ldmatrix, operand stored [n][k]
     const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);    // ... and [k][n]
+    // two warps per 16 columns: each finishes the outputs of eight of the chunk's tokens
+    constexpr int FINISH = SLICES > 1 ? 1 : 2;                 // tiles of eight tokens that a warp finishes
+    const int tile0 = SLICES > 1 ? slice : 0;
     float* out = p.out + (size_t)t0 * p.heads * p.vdim + (size_t)head * p.vdim + col;
+    dc_sync(DC_FULL, 32 * (DC_WALKERS + 1));                   // stage 0 is there
 
     for (int c = 0; c < chunks; ++c) {
         auto& st = sm.stage[c % DC_STAGES];
-        dc_sync(DC_FULL + c % DC_STAGES, 32 * (WALKERS + 1));
-        // ---- the columns' powers of two
-        if (c % DC_REFRESH == 0) {                             // the bounds from the columns themselves
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float sum = 0.f;
-                const float back = 1.f / sigma[h];             // (a power of two)
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) sum = fmaxf(sum, fmaxf(fabsf(s[n][2 * h]), fabsf(s[n][2 * h + 1])));
-                sum *= back;
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) sum = fmaxf(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-                if (SLICES > 1) {
-                    if (t == 0) sm.norm[warp][g + 8 * h] = sum;
-                } else {
-                    bound[h] = sum * 8.f;                      // 2-norm of 64 numbers, at most 8 times the largest
-                }
-            }
-            if (SLICES > 1) {
-                dc_sync(DC_PAIR + group, 64);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    bound[h] = fmaxf(sm.norm[group * SLICES][g + 8 * h], sm.norm[group * SLICES + SLICES - 1][g + 8 * h]) * 12.f;
-            }
-        }
-        const float add[2] = {32.f * st.v_most[group * 16 + g], 32.f * st.v_most[group * 16 + g + 8]};
-        float factor[2];
-        bool moved = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const float most = (bound[h] + add[h]) * sigma[h];
-            factor[h] = 1.f;
-            if (most > DC_MOST || (most < DC_MOST / 256.f && most > 0.f)) {
-                // 2^12 <= most * factor < 2^13; sigma itself stays within 2^-100 .. 2^100
-                int e = 12 - (((__float_as_int(most) >> 23) & 255) - 127);
-                const int have = ((__float_as_int(sigma[h]) >> 23) & 255) - 127;
-                e = min(max(e, -100 - have), 100 - have);
-                factor[h] = dc_power(min(max(e, -126), 127));
-                moved = moved || factor[h] != 1.f;
-            }
-        }
-        if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sigma[h] *= factor[h];
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= factor[h]; s[n][2 * h + 1] *= factor[h]; }
-            }
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
-        }
-        // ---- S0^T k and S0^T q of the warp's rows: 16 columns x 16 tokens
-        float wk[2][4], wq[2][4];
-        {
-            float low_k[2][4], low_q[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wk[j][e] = wq[j][e] = low_k[j][e] = low_q[j][e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                unsigned b[4];
-                dc_ldmatrix(b, &st.k[0][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    dc_mma(wk[j], sh[k], b[2 * j], b[2 * j + 1]);
-                    dc_mma(low_k[j], sl[k], b[2 * j], b[2 * j + 1]);
-                }
-                if (PARTS == 2) {
-                    dc_ldmatrix(b, &st.k[PARTS - 1][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) dc_mma(low_k[j], sh[k], b[2 * j], b[2 * j + 1]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wk[j][e] += low_k[j][e];
-            if (SLICES > 1) {
-                sm.swap[c & 1][warp][0][lane] = make_float4(wk[0][0], wk[0][1], wk[0][2], wk[0][3]);
-                sm.swap[c & 1][warp][1][lane] = make_float4(wk[1][0], wk[1][1], wk[1][2], wk[1][3]);
-            }
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                unsigned b[4];
-                dc_ldmatrix(b, &st.q[0][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    dc_mma(wq[j], sh[k], b[2 * j], b[2 * j + 1]);
-                    dc_mma(low_q[j], sl[k], b[2 * j], b[2 * j + 1]);
-                }
-                if (PARTS == 2) {
-                    dc_ldmatrix(b, &st.q[PARTS - 1][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) dc_mma(low_q[j], sh[k], b[2 * j], b[2 * j + 1]);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wq[j][e] += low_q[j][e];
-        }
-        // ---- with two warps per 16 columns: all of S0^T k for both, of S0^T q the half of the tokens that a warp finishes
-        if (SLICES > 1) {
-            const int other = slice ^ 1;
-            sm.swap[c & 1][warp][2][lane] = other ? make_float4(wq[1][0], wq[1][1], wq[1][2], wq[1][3])
-                                                  : make_float4(wq[0][0], wq[0][1], wq[0][2], wq[0][3]);
-            dc_sync(DC_PAIR + group, 64);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float4 x = sm.swap[c & 1][warp ^ 1][j][lane];
-                wk[j][0] += x.x; wk[j][1] += x.y; wk[j][2] += x.z; wk[j][3] += x.w;
-            }
-            const float4 x = sm.swap[c & 1][warp ^ 1][2][lane];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-                if (slice == j) { wq[j][0] += x.x; wq[j][1] += x.y; wq[j][2] += x.z; wq[j][3] += x.w; }
-        }
-        // ---- R, U
-        float r[2][4], u[2][4];
+        float raw[2][4];                                       // the chunk's v, laid out as a tile of U
         if constexpr (sizeof(T) == 2) {
             unsigned v[4];                                     // tokens 0-7 of col, col + 8; tokens 8-15 of both
             dc_ldmatrix_trans(v, &st.v[(lane & 7) + 8 * (lane >> 4)][group * 16 + 8 * ((lane >> 3) & 1)]);
@@ -584,83 +549,181 @@ delta_chunk_kernel(const DeltaParams p) {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    r[j][2 * h] = __uint_as_float(v[2 * j + h] << 16);
-                    r[j][2 * h + 1] = __uint_as_float(v[2 * j + h] & 0xffff0000u);
+                    raw[j][2 * h] = __uint_as_float(v[2 * j + h] << 16);
+                    raw[j][2 * h + 1] = __uint_as_float(v[2 * j + h] & 0xffff0000u);
                 }
         } else {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[j][e] = to_float(st.v[8 * j + 2 * t + (e & 1)][group * 16 + g + 8 * (e >> 1)]);
+                for (int e = 0; e < 4; ++e) raw[j][e] = to_float(st.v[8 * j + 2 * t + (e & 1)][group * 16 + g + 8 * (e >> 1)]);
         }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float2 before = *reinterpret_cast<const float2*>(&st.before[8 * j + 2 * t]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                r[j][2 * h] = fmaf(-before.x, wk[j][2 * h], r[j][2 * h] * sigma[h]);
-                r[j][2 * h + 1] = fmaf(-before.y, wk[j][2 * h + 1], r[j][2 * h + 1] * sigma[h]);
-            }
-        }
-        unsigned rh[4], rl[4], th[4], tl[4];
-        dc_ldmatrix(th, &st.t[0][b_row][b_col]);
-        dc_ldmatrix(tl, &st.t[1][b_row][b_col]);
-        dc_split_tiles(r[0], r[1], rh, rl);
-        dc_solve(u, rh, rl, th, tl);
+        bool look = c % DC_REFRESH == 0;
         int bad[2] = {DC_TOKENS, DC_TOKENS};
-        {
-            float probe = 0.f;
+        float u[2][4], wq[FINISH][4];
+        for (int tries = 0;; ++tries) {
+            if (look) {                                        // the columns' powers of two from the columns themselves
+                float most[2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+                for (int h = 0; h < 2; ++h) {
+                    most[h] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) probe = fmaf(u[j][e], 0.f, probe);
-            if (__any_sync(0xffffffffu, probe != 0.f)) {       // (NaN: something is not finite)
-                dc_first_bad(r, t, bad);
-                dc_leave_out(r, t, bad);
-                dc_split_tiles(r[0], r[1], rh, rl);
-                dc_solve(u, rh, rl, th, tl);
-                dc_first_bad(u, t, bad);
-                dc_leave_out(u, t, bad);
+                    for (int n = 0; n < TILES; ++n) most[h] = fmaxf(most[h], fmaxf(fabsf(s[n][2 * h]), fabsf(s[n][2 * h + 1])));
+                    most[h] *= back[h];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 2 * h; e < 2 * h + 2; ++e)        // (an infinite value must not move its column's power)
+                            if (fabsf(raw[j][e]) < INFINITY) most[h] = fmaxf(most[h], fabsf(raw[j][e]));
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], o));
+                }
+                if (SLICES > 1) {
+                    if (t == 0) { sm.most[warp][g] = most[0]; sm.most[warp][g + 8] = most[1]; }
+                    dc_sync(DC_PAIR + group, 64);
+                    most[0] = fmaxf(most[0], sm.most[warp ^ 1][g]);
+                    most[1] = fmaxf(most[1], sm.most[warp ^ 1][g + 8]);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int e = DC_SIZE - (((__float_as_int(most[h]) >> 23) & 255) - 127);
+                    const float next = most[h] > 0.f ? dc_power(min(max(e, -100), 100)) : sigma[h];
+                    const float factor = next * back[h];
+                    sigma[h] = next;
+                    back[h] = 1.f / next;
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= factor; s[n][2 * h + 1] *= factor; }
+                }
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
             }
-        }
-        // ---- outputs: the chunk's start and its own tokens
-        unsigned uh[4], ul[4], ph[4], pl[4];
-        dc_ldmatrix(ph, &st.p[0][b_row][b_col]);
-        dc_ldmatrix(pl, &st.p[1][b_row][b_col]);
-        dc_split_tiles(u[0], u[1], uh, ul);
-        const float back[2] = {1.f / sigma[0], 1.f / sigma[1]};
+            // ---- S0^T k and S0^T q of the warp's rows: 16 columns x 16 tokens
+            float wk[2][4];
+            {
+                float low[2][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (SLICES > 1 && slice != j) continue;
-            float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-            dc_mma(b, ul, ph[2 * j], ph[2 * j + 1]);
-            dc_mma(a, uh, ph[2 * j], ph[2 * j + 1]);
-            dc_mma(b, uh, pl[2 * j], pl[2 * j + 1]);
-            const float2 fade = *reinterpret_cast<const float2*>(&st.fade[8 * j + 2 * t]);
-            const float2 query = *reinterpret_cast<const float2*>(&st.query[8 * j + 2 * t]);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int token = 8 * j + 2 * t + (e & 1);
-                float o = fmaf((e & 1) ? fade.y : fade.x, wq[j][e], a[e] + b[e]) * ((e & 1) ? query.y : query.x) * back[e >> 1];
-                if (token >= bad[e >> 1]) o = __int_as_float(0x7fffffff);
-                if (c * DC_TOKENS + token < count && col + 8 * (e >> 1) < p.vdim)
-                    out[(size_t)(c * DC_TOKENS + token) * p.heads * p.vdim + 8 * (e >> 1)] = o;
+                    for (int e = 0; e < 4; ++e) wk[j][e] = low[j][e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    unsigned b[4];
+                    dc_ldmatrix(b, &st.keys.k[0][b_row][row0 + 16 * k + b_col]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        dc_mma(wk[j], sh[k], b[2 * j], b[2 * j + 1]);
+                        dc_mma(low[j], sl[k], b[2 * j], b[2 * j + 1]);
+                    }
+                    if (PARTS == 2) {
+                        dc_ldmatrix(b, &st.keys.k[PARTS - 1][b_row][row0 + 16 * k + b_col]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) dc_mma(low[j], sh[k], b[2 * j], b[2 * j + 1]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) wk[j][e] += low[j][e];
             }
+            if (SLICES > 1) {
+                sm.swap[c & 1][warp][0][lane] = make_float4(wk[0][0], wk[0][1], wk[0][2], wk[0][3]);
+                sm.swap[c & 1][warp][1][lane] = make_float4(wk[1][0], wk[1][1], wk[1][2], wk[1][3]);
+            }
+            {
+                float both[2][4], low[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) both[j][e] = low[j][e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    unsigned b[4];
+                    dc_ldmatrix(b, &st.keys.q[0][b_row][row0 + 16 * k + b_col]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        dc_mma(both[j], sh[k], b[2 * j], b[2 * j + 1]);
+                        dc_mma(low[j], sl[k], b[2 * j], b[2 * j + 1]);
+                    }
+                    if (PARTS == 2) {
+                        dc_ldmatrix(b, &st.keys.q[PARTS - 1][b_row][row0 + 16 * k + b_col]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) dc_mma(low[j], sh[k], b[2 * j], b[2 * j + 1]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) both[j][e] += low[j][e];
+                if constexpr (SLICES > 1) {
+                    float4 theirs;
+                    theirs.x = slice ? both[0][0] : both[1][0]; theirs.y = slice ? both[0][1] : both[1][1];
+                    theirs.z = slice ? both[0][2] : both[1][2]; theirs.w = slice ? both[0][3] : both[1][3];
+                    sm.swap[c & 1][warp][2][lane] = theirs;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) wq[0][e] = slice ? both[1][e] : both[0][e];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) wq[j % FINISH][e] = both[j][e];
+                }
+            }
+            // ---- one meeting per chunk: the halves' sums are there, and so is the next stage
+            if (tries == 0) dc_sync(DC_FULL + (c + 1) % DC_STAGES, 32 * (DC_WALKERS + 1));
+            else if (SLICES > 1) dc_sync(DC_PAIR + group, 64);
+            if (SLICES > 1) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float4 x = sm.swap[c & 1][warp ^ 1][j][lane];
+                    wk[j][0] += x.x; wk[j][1] += x.y; wk[j][2] += x.z; wk[j][3] += x.w;
+                }
+                const float4 x = sm.swap[c & 1][warp ^ 1][2][lane];
+                wq[0][0] += x.x; wq[0][1] += x.y; wq[0][2] += x.z; wq[0][3] += x.w;
+            }
+            // ---- R, U
+            float r[2][4];
+            float size = st.gates.odd[0];                      // NaN where T is not finite
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float2 before = *reinterpret_cast<const float2*>(&st.gates.before[8 * j + 2 * t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    r[j][e] = fmaf((e & 1) ? -before.y : -before.x, wk[j][e], raw[j][e] * sigma[e >> 1]);
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(size) : "f"(fabsf(r[j][e])));
+                }
+            }
+            unsigned rh[4], rl[4], th[4], tl[4];
+            dc_ldmatrix(th, &st.gates.t[0][b_row][b_col]);
+            dc_ldmatrix(tl, &st.gates.t[1][b_row][b_col]);
+            dc_split_tiles(r[0], r[1], rh, rl);
+            dc_solve(u, rh, rl, th, tl);
+            if (!__any_sync(0xffffffffu, !(size < DC_MOST))) break;
+            if (tries == 0) { look = true; continue; }         // (both warps of a pair have the same R and T)
+            // not a matter of size: something is not finite
+            dc_first_bad(r, t, bad);
+            dc_leave_out(r, t, bad);
+            dc_split_tiles(r[0], r[1], rh, rl);
+            dc_solve(u, rh, rl, th, tl);
+            dc_first_bad(u, t, bad);
+            dc_leave_out(u, t, bad);
+            break;
         }
         // ---- the new state
+        unsigned uh[4], ul[4], zh[4], zl[4];
+        dc_split_tiles(u[0], u[1], zh, zl);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float2 after = *reinterpret_cast<const float2*>(&st.after[8 * j + 2 * t]);
+            const float2 after = *reinterpret_cast<const float2*>(&st.gates.after[8 * j + 2 * t]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) u[j][e] *= (e & 1) ? after.y : after.x;
         }
         dc_split_tiles(u[0], u[1], uh, ul);
-        const float decay = st.fade[DC_TOKENS - 1];
+        const float decay = st.gates.fade[DC_TOKENS - 1];
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
             unsigned b[4], b2[4];
-            dc_ldmatrix_trans(b, &st.k[0][bt_row][row0 + 16 * k + bt_col]);
-            if (PARTS == 2) dc_ldmatrix_trans(b2, &st.k[PARTS - 1][bt_row][row0 + 16 * k + bt_col]);
+            dc_ldmatrix_trans(b, &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
+            if (PARTS == 2) dc_ldmatrix_trans(b2, &st.keys.k[PARTS - 1][bt_row][row0 + 16 * k + bt_col]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float a[4] = {0.f, 0.f, 0.f, 0.f};
@@ -670,59 +733,121 @@ delta_chunk_kernel(const DeltaParams p) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[2 * k + j][e] = fmaf(s[2 * k + j][e], decay, a[e]);
             }
+            dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
         }
-        if (c + DC_STAGES < chunks) dc_arrive(DC_EMPTY + c % DC_STAGES, 32 * (WALKERS + 1));
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            bound[h] = fmaf(bound[h], decay, add[h]);
-            if (bad[h] < DC_TOKENS) {
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) s[n][2 * h] = s[n][2 * h + 1] = __int_as_float(0x7fffffff);
+        // ---- outputs: the chunk's start and its own tokens
+        {
+            unsigned ph[4], pl[4];
+            if constexpr (SLICES > 1) {                        // the lanes' rows are the eight tokens, first and second inner half
+                const __half* from = &st.gates.p[lane >> 4][8 * slice + (lane & 7)][b_col];
+                dc_ldmatrix(ph, from);
+                pl[0] = ph[2]; pl[1] = ph[3];
+            } else {
+                dc_ldmatrix(ph, &st.gates.p[0][b_row][b_col]);
+                dc_ldmatrix(pl, &st.gates.p[1][b_row][b_col]);
             }
-        }
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
+            for (int j = 0; j < FINISH; ++j) {
+                float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
+                dc_mma(b, zl, ph[2 * j], ph[2 * j + 1]);
+                dc_mma(a, zh, ph[2 * j], ph[2 * j + 1]);
+                dc_mma(b, zh, pl[2 * j], pl[2 * j + 1]);
+                const int first = 8 * (tile0 + j) + 2 * t;
+                const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[first]);
+                const float2 query = *reinterpret_cast<const float2*>(&st.gates.query[first]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int token = first + (e & 1);
+                    float o = fmaf((e & 1) ? fade.y : fade.x, wq[j][e], a[e] + b[e]) * ((e & 1) ? query.y : query.x) * back[e >> 1];
+                    if (token >= bad[e >> 1]) o = __int_as_float(0x7fffffff);
+                    if (c * DC_TOKENS + token < count && col + 8 * (e >> 1) < p.vdim)
+                        out[(size_t)token * p.heads * p.vdim + 8 * (e >> 1)] = o;
+                }
+            }
+            out += (size_t)DC_TOKENS * p.heads * p.vdim;
+        }
+        if (c + DC_STAGES < chunks) dc_arrive(DC_EMPTY + c % DC_STAGES, 32 * (DC_WALKERS + 1));
+        if (__any_sync(0xffffffffu, min(bad[0], bad[1]) < DC_TOKENS)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (bad[h] < DC_TOKENS) {
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) s[n][2 * h] = s[n][2 * h + 1] = __int_as_float(0x7fffffff);
+                }
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
+        }
     }
 #pragma unroll
     for (int n = 0; n < TILES; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int d = row0 + 8 * n + 2 * t + (e & 1), v = col + 8 * (e >> 1);
-            if (d < p.dim && v < p.vdim) state[(size_t)d * p.vdim + v] = s[n][e] * (1.f / sigma[e >> 1]);
+            if (d < p.dim && v < p.vdim) state[(size_t)d * p.vdim + v] = s[n][e] * back[e >> 1];
         }
 }
 
-template <typename T, int DK, int WALKERS, bool WIDE>
-static int launch_chunk(const DeltaParams& p, int items, int early, cudaStream_t stream) {
-    using Sh = DcShape<T, DK, WALKERS>;
-    auto kernel = delta_chunk_kernel<T, DK, WALKERS, WIDE>;
+template <typename T, int DK, bool WIDE>
+static int launch_chunk(const DeltaParams& p, const DcRecords& records, int early, cudaStream_t stream) {
+    using Sh = DcShape<T, DK>;
+    auto kernel = delta_walk_kernel<T, DK, WIDE>;
     static bool configured = false;            // per process and kernel; harmless if repeated
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename Sh::Shared));
         if (e != cudaSuccess) return (int)e;
         configured = true;
     }
-    const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, items);
-    if (grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
-    return launch_dependent_if(early, kernel, grid, dim3(Sh::THREADS), sizeof(typename Sh::Shared), stream, p);
+    const long long units = (long long)records.chunks * (p.heads / p.share);
+    const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.items);
+    if (grid.y > 65535 || grid.z > 65535 || units > 0x7fffffffLL) return ERR_UNSUPPORTED;
+    const int rc = launch_dependent_if(early, delta_records_kernel<T, DK, WIDE>, dim3((unsigned)((units + DC_MAKERS - 1) / DC_MAKERS)),
+                                       dim3(32 * DC_MAKERS), 0, stream, p, records);
+    if (rc != 0) return rc;
+    // the state is older than the records' kernel, which waits for whatever may have written it
+    return launch_dependent(kernel, grid, dim3(Sh::THREADS), sizeof(typename Sh::Shared), stream, p, records);
 }
 
 template <typename T, int DK>
-static int launch_chunk_any(const DeltaParams& p, int items, int early, cudaStream_t stream) {
+static int launch_chunk_any(const DeltaParams& p, int items, long long chunks, unsigned char* room, int early, cudaStream_t stream) {
+    using Sh = DcShape<T, DK>;
+    DcRecords records;
+    records.keys = room;
+    records.gates = room + (size_t)chunks * (p.heads / p.share) * sizeof(typename Sh::Keys);
+    records.items = items;
+    records.chunks = (int)chunks;
     const bool wide = p.ld % 8 == 0 && p.q_off % 8 == 0 && p.k_off % 8 == 0 && p.v_off % 8 == 0 && p.dim % 8 == 0 &&
                       p.vdim % 8 == 0 && (uintptr_t)p.qkv % 16 == 0;
-    if (wide) return launch_chunk<T, DK, 4, true>(p, items, early, stream);
-    return launch_chunk<T, DK, 4, false>(p, items, early, stream);
+    return wide ? launch_chunk<T, DK, true>(p, records, early, stream) : launch_chunk<T, DK, false>(p, records, early, stream);
 }
 
-// The chunked form; ERR_UNSUPPORTED where a head has more rows than it holds.
-int delta_chunk(const DeltaParams& p, int items, int dtype, int early, cudaStream_t stream) {
+static long long chunk_bytes(int heads, int share, int dim, int dtype) {
+    const long long gates = (long long)heads * sizeof(DcShape<bf16, 64>::Gates), narrow = heads / share;
+    if (dtype == DTYPE_F32) return gates + narrow * (dim <= 64 ? sizeof(DcShape<float, 64>::Keys) : sizeof(DcShape<float, 128>::Keys));
+    return gates + narrow * (dim <= 64 ? sizeof(DcShape<bf16, 64>::Keys) : sizeof(DcShape<bf16, 128>::Keys));
+}
+
+// The chunked form; ERR_UNSUPPORTED where a head has more rows than it holds.  `room`: 16-byte aligned memory.
+int delta_chunk(const DeltaParams& p, int items, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (p.dim > DC_MAX_DIM) return ERR_UNSUPPORTED;
+    const long long chunks = room_bytes / chunk_bytes(p.heads, p.share, p.dim, dtype);
+    if (!room || (uintptr_t)room % 16 != 0 || chunks <= 0 || chunks > 0x7fffffffLL) return ERR_BAD_ARGUMENT;
+    unsigned char* at = (unsigned char*)room;
     if (dtype == DTYPE_F32)
-        return p.dim <= 64 ? launch_chunk_any<float, 64>(p, items, early, stream) : launch_chunk_any<float, 128>(p, items, early, stream);
-    return p.dim <= 64 ? launch_chunk_any<bf16, 64>(p, items, early, stream) : launch_chunk_any<bf16, 128>(p, items, early, stream);
+        return p.dim <= 64 ? launch_chunk_any<float, 64>(p, items, chunks, at, early, stream)
+                           : launch_chunk_any<float, 128>(p, items, chunks, at, early, stream);
+    return p.dim <= 64 ? launch_chunk_any<bf16, 64>(p, items, chunks, at, early, stream)
+                       : launch_chunk_any<bf16, 128>(p, items, chunks, at, early, stream);
 }
 
 }  // namespace fsie
 
-extern "C" int fsie_delta_chunk_max_dim() { return fsie::DC_MAX_DIM; }
+extern "C" {
+
+int fsie_delta_chunk_max_dim() { return fsie::DC_MAX_DIM; }
+
+int fsie_delta_chunk_tokens() { return fsie::DC_TOKENS; }
+
+// bytes of the workspace per chunk
+int fsie_delta_chunk_bytes(int heads, int share, int dim, int dtype) { return (int)fsie::chunk_bytes(heads, share, dim, dtype); }
+
+}  // extern "C"

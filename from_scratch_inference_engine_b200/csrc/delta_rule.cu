@@ -160,7 +160,8 @@ static int launch_step(const DeltaParams& p, int items, int early, cudaStream_t 
     return launch_dependent_if(early, kernel, grid, dim3(STEP_THREADS), 0, stream, p);
 }
 
-int delta_chunk(const DeltaParams& p, int items, int dtype, int early, cudaStream_t stream);       // delta_chunk.cu
+// delta_chunk.cu
+int delta_chunk(const DeltaParams& p, int items, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream);
 
 }  // namespace fsie
 
@@ -170,11 +171,12 @@ extern "C" {
 
 int fsie_delta_max_dim() { return STEP_MAX_DIM; }
 
-// `form`: 0 the recurrent form, 1 the chunked one
+// `form`: 0 the recurrent form, 1 the chunked one, with a workspace `room` of fsie_delta_chunk_bytes() for every chunk
+// (of fsie_delta_chunk_tokens() tokens of a request, its last one begun)
 int fsie_delta_rule(int form, const void* qkv, int ld, int q_off, int k_off, int v_off, const float* log_decay, const float* beta,
                     const int* item_qstart, const int* item_qlen, const int* item_slots, int items, float* state,
                     long long state_stride, float* out, int heads, int dim, int vdim, int share, float scale, float eps,
-                    int dtype, int early, cudaStream_t stream) {
+                    int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (items <= 0) return 0;
     if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 1) return ERR_BAD_ARGUMENT;
     DeltaParams p;
@@ -183,7 +185,7 @@ int fsie_delta_rule(int form, const void* qkv, int ld, int q_off, int k_off, int
     p.state = state; p.state_stride = state_stride; p.out = out;
     p.heads = heads; p.dim = dim; p.vdim = vdim; p.share = share; p.scale = scale; p.eps = eps;
     if (dtype != DTYPE_F32 && dtype != DTYPE_BF16) return ERR_BAD_ARGUMENT;
-    if (form == 1) return delta_chunk(p, items, dtype, early, stream);
+    if (form == 1) return delta_chunk(p, items, dtype, room, room_bytes, early, stream);
     return dtype == DTYPE_F32 ? launch_step<float>(p, items, early, stream) : launch_step<bf16>(p, items, early, stream);
 }
 

@@ -2293,10 +2293,11 @@ def delta():
         i, f, ll, p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
         lib.fsie_delta_prep.argtypes = [p, i, i, i, i, p, p, p, p, p, i, i, p, ll, ll, p, i, i, p, p, i, p, p, p, i, i, p]
         lib.fsie_delta_prep_max_taps.argtypes = []
-        lib.fsie_delta_rule.argtypes = [i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, i, p]
-        lib.fsie_delta_max_dim.argtypes = lib.fsie_delta_chunk_max_dim.argtypes = []
+        lib.fsie_delta_rule.argtypes = [i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, p, ll, i, p]
+        lib.fsie_delta_max_dim.argtypes = lib.fsie_delta_chunk_max_dim.argtypes = lib.fsie_delta_chunk_tokens.argtypes = []
+        lib.fsie_delta_chunk_bytes.argtypes = [i, i, i, i]
         for name in ("fsie_delta_prep", "fsie_delta_prep_max_taps", "fsie_delta_rule", "fsie_delta_max_dim",
-                     "fsie_delta_chunk_max_dim"):
+                     "fsie_delta_chunk_max_dim", "fsie_delta_chunk_tokens", "fsie_delta_chunk_bytes"):
             getattr(lib, name).restype = i
         _delta = build.fast_calls(lib)
     return _delta
@@ -2386,10 +2387,15 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
         raise KernelError("gated_delta_rule: eps must be positive")
     if dim > delta().fsie_delta_max_dim():
         raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {delta().fsie_delta_max_dim()}")
-    chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= delta().fsie_delta_chunk_max_dim()
-    _check(delta().fsie_delta_rule(int(chunked), qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots, items,
-                                   state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
-                                   float(eps), _tag(qkv.dtype), int(early), _stream()), "gated_delta_rule")
+    lib, tag, room = delta(), _tag(qkv.dtype), None
+    chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= lib.fsie_delta_chunk_max_dim()
+    if chunked:
+        chunks = tokens // lib.fsie_delta_chunk_tokens() + items
+        room = torch.empty(chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag), dtype=torch.uint8, device=qkv.device)
+    _check(lib.fsie_delta_rule(int(chunked), qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
+                               items, state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
+                               float(eps), tag, room, 0 if room is None else room.numel(), int(early), _stream()),
+           "gated_delta_rule")
     return out
 
 
