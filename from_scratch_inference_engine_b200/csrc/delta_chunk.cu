@@ -15,15 +15,15 @@
 // scaled by a power of two to a length of about one are exact in half precision; what is 32-bit - the state, R, U, T and the
 // weights of u_j - goes into the instructions as the sum of two half-precision numbers (22 bits), products of two low parts left
 // out.  Half precision has little range: every column of the state (a row of the transposed tiles below) has a power of
-// two, `sigma`, chosen from the column's and the chunk's own largest numbers every 8 chunks, and anew, with the chunk's
+// two, `sigma`, chosen from the column's and the chunk's own largest numbers every 32 chunks, and anew, with the chunk's
 // sums taken again, whenever a number of R leaves the range in between.  The state itself stays in 32-bit registers
 // and the instructions only ever sum up one chunk (their running sums are truncated, not rounded).  float32 storage: q and k
 // are two parts as well.
 //
 // Two kernels.  The first prepares all chunks side by side, a warp per chunk and q/k head: q and k in half precision, T by
 // substitution, the weights of u_j, the gates' factors, as records in the workspace that lie as the second kernel's shared
-// memory holds them.  The second walks a head's chunks, a block for every 16 GROUPS value columns, its fifth warp copying the
-// records and the chunk's v into a ring of stages; named barriers hand the stages over, nothing spins.  (One kernel in which
+// memory holds them.  The second walks a head's chunks, a block for every 16 GROUPS value columns, four more warps
+// keeping the records and v of the next chunks on their way into a ring of stages; all meet once per chunk and nothing spins.  (One kernel in which
 // four more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads: every block of value columns
 // prepared them again, and the two roles' code did not fit the instruction cache together.)
 //
@@ -43,12 +43,11 @@
 namespace fsie {
 
 constexpr int DC_TOKENS = 16;              // tokens of a chunk
-constexpr int DC_STAGES = 5;               // stages of the ring
-constexpr int DC_AHEAD = 2;                // chunks whose copies are under way
+constexpr int DC_STAGES = 4;               // stages of the ring: the chunk's, the next one's and two on their way
 constexpr int DC_WALKERS = 4;              // warps that walk a block's chunks
 constexpr int DC_SLICE = 64;               // rows of S (columns of k) per warp
 constexpr int DC_MAX_DIM = 128;
-constexpr int DC_REFRESH = 8;              // chunks between two looks at the state's size
+constexpr int DC_REFRESH = 32;             // chunks between two looks at the state's size
 constexpr int DC_SIZE = 4;                 // ... which brings the largest number of a column to 2^4 .. 2^5
 constexpr int DC_TLD = DC_TOKENS + 8;      // padded rows: ldmatrix without bank conflicts
 // A number of R, times sigma, is below this: a row of T has at most 16 numbers of at most beta^2 <= 4 (what a token's value
@@ -73,16 +72,40 @@ __device__ __forceinline__ void dc_mma(float (&d)[4], const unsigned (&a)[4], un
 __device__ __forceinline__ void dc_sync(int barrier, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 }
-__device__ __forceinline__ void dc_arrive(int barrier, int threads) {
-    asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
-}
 __device__ __forceinline__ unsigned dc_bits(__half2 h) { return *reinterpret_cast<unsigned*>(&h); }
-// x, y as half-precision numbers, and what that rounding lost
+// two floats in one register pair: the packed instructions of sm_100 work on both at once
+__device__ __forceinline__ unsigned long long dc_pair(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void dc_unpair(unsigned long long p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ void dc_fma2(float& x, float& y, float ax, float ay, float bx, float by, float cx, float cy) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(dc_pair(ax, ay)), "l"(dc_pair(bx, by)), "l"(dc_pair(cx, cy)));
+    dc_unpair(r, x, y);
+}
+__device__ __forceinline__ void dc_mul2(float& x, float& y, float ax, float ay, float bx, float by) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(dc_pair(ax, ay)), "l"(dc_pair(bx, by)));
+    dc_unpair(r, x, y);
+}
+__device__ __forceinline__ void dc_add2(float& x, float& y, float ax, float ay, float bx, float by) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(dc_pair(ax, ay)), "l"(dc_pair(bx, by)));
+    dc_unpair(r, x, y);
+}
+// x, y as half-precision numbers, and what that rounding lost (cutting x and y off instead would save an instruction, but
+// products of two lows, which are left out, would then all have the same sign)
 __device__ __forceinline__ void dc_split(float x, float y, unsigned& high, unsigned& low) {
     const __half2 h = __floats2half2_rn(x, y);
     const float2 f = __half22float2(h);
     high = dc_bits(h);
-    low = dc_bits(__floats2half2_rn(x - f.x, y - f.y));
+    float lx, ly;
+    dc_add2(lx, ly, x, y, -f.x, -f.y);
+    low = dc_bits(__floats2half2_rn(lx, ly));
 }
 // the 16 x 16 operand of two neighbouring accumulator tiles, in two parts
 __device__ __forceinline__ void dc_split_tiles(const float (&x)[4], const float (&y)[4], unsigned (&high)[4], unsigned (&low)[4]) {
@@ -147,7 +170,7 @@ struct DcShape {
     static constexpr int COLS = 16 * GROUPS;                   // value columns of a block
     static constexpr int KLD = DK + 8;                         // padded row of q and k
     static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 8);
-    static constexpr int THREADS = 32 * (DC_WALKERS + 1);
+    static constexpr int THREADS = 2 * 32 * DC_WALKERS;        // the walkers' and the fetchers'
     struct alignas(16) Keys { __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD]; };
     struct alignas(16) Gates {
         __half t[2][DC_TOKENS][DC_TLD], p[2][DC_TOKENS][DC_TLD];     // T and the weights of u_j, two parts each
@@ -405,54 +428,113 @@ __device__ __forceinline__ void dc_copy16(void* dst, const void* src, bool there
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dc_smem(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
-enum { DC_FULL = 1, DC_EMPTY = DC_FULL + DC_STAGES, DC_PAIR = DC_EMPTY + DC_STAGES };       // named barriers
-static_assert(DC_PAIR + DC_WALKERS / 2 <= 16, "a block has 16 named barriers");
+enum { DC_MEET = 1, DC_PAIR = 2 };         // named barriers: all warps, and from DC_PAIR on the pairs'
 
-// The fifth warp: records and v of one chunk after the other into the ring.
+// A fetching thread's share of the copies into the ring, chunk after chunk: the addresses move on by a chunk with every call.
+// (Copied by the walkers themselves a chunk takes them 800 cycles more: their own reads of shared memory queue behind.)
 template <typename T, int DK, bool WIDE>
-__device__ __forceinline__ void dc_fetch(const DeltaParams& p, const DcRecords& records, typename DcShape<T, DK>::Shared& sm, int lane,
-                                         int head, int col0, int t0, int count, int chunk0, int chunks) {
+struct DcFetch {
     using Sh = DcShape<T, DK>;
-    const int narrow_heads = p.heads / p.share;
-    const auto* keys = reinterpret_cast<const typename Sh::Keys*>(records.keys) + ((size_t)chunk0 * narrow_heads + head / p.share);
-    const auto* gates = reinterpret_cast<const typename Sh::Gates*>(records.gates) + ((size_t)chunk0 * p.heads + head);
-    const T* v = (const T*)p.qkv + (size_t)t0 * p.ld + p.v_off + (size_t)head * p.vdim + col0;
-    for (int c = 0; c <= chunks + DC_AHEAD; ++c) {             // (the walkers' last meeting is for a stage that nobody fills)
-        if (c < chunks) {
-            auto& st = sm.stage[c % DC_STAGES];
-            if (c >= DC_STAGES) dc_sync(DC_EMPTY + c % DC_STAGES, 32 * (DC_WALKERS + 1));
-            const int n = min(DC_TOKENS, count - c * DC_TOKENS);
-            constexpr int PER = 16 / sizeof(T), ACROSS = Sh::COLS / PER;          // 16-byte pieces of a row of v
-#pragma unroll 4
-            for (int e = lane; e < (int)(sizeof(st.keys) / 16); e += 32)
-                dc_copy16(reinterpret_cast<uint4*>(&st.keys) + e, reinterpret_cast<const uint4*>(keys) + e, true);
-#pragma unroll 4
-            for (int e = lane; e < (int)(sizeof(st.gates) / 16); e += 32)
-                dc_copy16(reinterpret_cast<uint4*>(&st.gates) + e, reinterpret_cast<const uint4*>(gates) + e, true);
-            if constexpr (WIDE) {
+    using Stage = typename Sh::Stage;
+    static constexpr int FETCHERS = 32 * DC_WALKERS;
+    static constexpr int PER = 16 / sizeof(T), ACROSS = Sh::COLS / PER;          // 16-byte pieces of a row of v
+    static constexpr int KEYS = sizeof(typename Sh::Keys) / 16, GATES = sizeof(typename Sh::Gates) / 16;
+    const unsigned char* keys;
+    const unsigned char* gates;
+    const T* v;
+    size_t keys_step, gates_step, v_step;
+    int left, row, have;                                       // tokens from the next chunk on; the thread's row of v, its columns there
+
+    __device__ __forceinline__ DcFetch(const DeltaParams& p, const DcRecords& records, int head, int col0, int t0, int count, int chunk0) {
+        const int narrow_heads = p.heads / p.share, tid = threadIdx.x - FETCHERS;
+        keys_step = (size_t)narrow_heads * sizeof(typename Sh::Keys);
+        gates_step = (size_t)p.heads * sizeof(typename Sh::Gates);
+        v_step = (size_t)DC_TOKENS * p.ld;
+        keys = records.keys + chunk0 * keys_step + (size_t)(head / p.share) * sizeof(typename Sh::Keys) + tid * 16;
+        gates = records.gates + chunk0 * gates_step + (size_t)head * sizeof(typename Sh::Gates) + tid * 16;
+        row = WIDE ? tid / ACROSS : 0;
+        const int d = WIDE ? (tid % ACROSS) * PER : 0;
+        have = p.vdim - col0 - d;
+        v = (const T*)p.qkv + (size_t)t0 * p.ld + p.v_off + (size_t)head * p.vdim + col0 + (WIDE && have > 0 ? d : 0);
+        left = count;
+    }
+    __device__ __forceinline__ void next(const DeltaParams& p, Stage& st) {
+        const int tid = threadIdx.x - FETCHERS;
+        if (left > 0) {
 #pragma unroll
-                for (int e = lane; e < DC_TOKENS * ACROSS; e += 32) {
-                    const int r = e / ACROSS, d = (e % ACROSS) * PER;
-                    const bool there = r < n && col0 + d < p.vdim;
-                    dc_copy16(&st.v[r][d], v + (there ? (size_t)r * p.ld + d : 0), there);
+            for (int i = 0; i < (KEYS + FETCHERS - 1) / FETCHERS; ++i)
+                if ((i + 1) * FETCHERS <= KEYS || tid + i * FETCHERS < KEYS)
+                    dc_copy16(reinterpret_cast<uint4*>(&st.keys) + tid + i * FETCHERS, keys + i * FETCHERS * 16, true);
+#pragma unroll
+            for (int i = 0; i < (GATES + FETCHERS - 1) / FETCHERS; ++i)
+                if ((i + 1) * FETCHERS <= GATES || tid + i * FETCHERS < GATES)
+                    dc_copy16(reinterpret_cast<uint4*>(&st.gates) + tid + i * FETCHERS, gates + i * FETCHERS * 16, true);
+            if constexpr (WIDE) {
+                constexpr int ROWS = FETCHERS / ACROSS;     // rows of v that the block's threads copy at once
+#pragma unroll
+                for (int r = 0; r < DC_TOKENS; r += ROWS) {
+                    const bool there = r + row < left && have > 0;
+                    if (r + row < DC_TOKENS)
+                        dc_copy16(&st.v[r + row][(tid % ACROSS) * PER], v + (there ? (size_t)(r + row) * p.ld : 0), there);
                 }
             } else {
-                for (int e = lane; e < DC_TOKENS * Sh::COLS; e += 32) {
+                for (int e = tid; e < DC_TOKENS * Sh::COLS; e += FETCHERS) {
                     const int r = e / Sh::COLS, d = e % Sh::COLS;
-                    st.v[r][d] = r < n && col0 + d < p.vdim ? v[(size_t)r * p.ld + d] : from_float<T>(0.f);
+                    st.v[r][d] = r < left && d < have ? v[(size_t)r * p.ld + d] : from_float<T>(0.f);
                 }
             }
-            keys += narrow_heads;
-            gates += p.heads;
-            v += (size_t)DC_TOKENS * p.ld;
+            keys += keys_step;
+            gates += gates_step;
+            left -= DC_TOKENS;
+            if (left > 0) v += v_step;
         }
         asm volatile("cp.async.commit_group;\n" ::: "memory");
-        if (c >= DC_AHEAD) {
-            asm volatile("cp.async.wait_group %0;\n" ::"n"(DC_AHEAD) : "memory");
-            dc_arrive(DC_FULL + (c - DC_AHEAD) % DC_STAGES, 32 * (DC_WALKERS + 1));
-        }
     }
+};
+
+// S0^T times a chunk's keys or queries, the state in two parts (in sums of their own: low parts are lost beside high ones)
+template <int STEPS>
+__device__ __forceinline__ void dc_state_product(float (&sum)[2][4], const unsigned (&high)[STEPS][4], const unsigned (&low)[STEPS][4],
+                                                 const unsigned (&b)[STEPS][4]) {
+    float lows[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[j][e] = lows[j][e] = 0.f;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            dc_mma(sum[j], high[k], b[k][2 * j], b[k][2 * j + 1]);
+            dc_mma(lows[j], low[k], b[k][2 * j], b[k][2 * j + 1]);
+        }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) dc_add2(sum[j][e], sum[j][e + 1], sum[j][e], sum[j][e + 1], lows[j][e], lows[j][e + 1]);
 }
+
+// a thread's v of one chunk as it is stored
+template <typename T> struct DcValues;
+template <> struct DcValues<bf16> {
+    unsigned x[4];
+    __device__ __forceinline__ void widen(float (&r)[2][4]) const {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                r[j][2 * h] = __uint_as_float(x[2 * j + h] << 16);
+                r[j][2 * h + 1] = __uint_as_float(x[2 * j + h] & 0xffff0000u);
+            }
+    }
+};
+template <> struct DcValues<float> {
+    float x[8];
+    __device__ __forceinline__ void widen(float (&r)[2][4]) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) r[e >> 2][e & 3] = x[e];
+    }
+};
 
 // U = T R (both in two parts): operands R (high, low), T's parts as they lie in the stage
 __device__ __forceinline__ void dc_solve(float (&u)[2][4], const unsigned (&rh)[4], const unsigned (&rl)[4], const unsigned (&th)[4],
@@ -464,7 +546,7 @@ __device__ __forceinline__ void dc_solve(float (&u)[2][4], const unsigned (&rh)[
         dc_mma(a, rh, th[2 * j], th[2 * j + 1]);
         dc_mma(b, rh, tl[2 * j], tl[2 * j + 1]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[j][e] = a[e] + b[e];
+        for (int e = 0; e < 4; e += 2) dc_add2(u[j][e], u[j][e + 1], a[e], a[e + 1], b[e], b[e + 1]);
     }
 }
 
@@ -492,7 +574,7 @@ __device__ __forceinline__ void dc_leave_out(float (&x)[2][4], int t, const int 
 }
 
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(32 * (DC_WALKERS + 1), 2)
+__global__ void __launch_bounds__(2 * 32 * DC_WALKERS, 2)
 delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     using Sh = DcShape<T, DK>;
     constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16;
@@ -505,12 +587,22 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     const int chunks = (count + DC_TOKENS - 1) / DC_TOKENS;
     const int chunk0 = dc_chunks_before(p.item_qlen, item, lane);
     if (chunk0 + chunks > records.chunks) return;              // lists that name more tokens than there are
+    // registers: two blocks of 256 threads have 128 each; the walkers' four warps take over most of the fetchers' (216 + 40)
     if (warp >= DC_WALKERS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
         grid_dependency_wait();
         grid_dependents_go();
-        dc_fetch<T, DK, WIDE>(p, records, sm, lane, head, col0, t0, count, chunk0, chunks);
+        DcFetch<T, DK, WIDE> fetch(p, records, head, col0, t0, count, chunk0);
+        fetch.next(p, sm.stage[0]);
+        fetch.next(p, sm.stage[1]);
+        for (int c = 0; c <= chunks; ++c) {                    // (the last meeting is for a chunk that is not there)
+            asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+            dc_sync(DC_MEET, Sh::THREADS);                     // chunk c is there, and everybody is through with chunk c - 2:
+            fetch.next(p, sm.stage[(c + 2) % DC_STAGES]);      // its stage takes chunk c + 2
+        }
         return;
     }
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
     const int g = lane >> 2, t = lane & 3;
     const int group = warp / SLICES, slice = warp % SLICES;
     const int row0 = slice * DC_SLICE;                         // the warp's rows of S
@@ -537,33 +629,38 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     constexpr int FINISH = SLICES > 1 ? 1 : 2;                 // tiles of eight tokens that a warp finishes
     const int tile0 = SLICES > 1 ? slice : 0;
     float* out = p.out + (size_t)t0 * p.heads * p.vdim + (size_t)head * p.vdim + col;
-    dc_sync(DC_FULL, 32 * (DC_WALKERS + 1));                   // stage 0 is there
-
-    for (int c = 0; c < chunks; ++c) {
-        auto& st = sm.stage[c % DC_STAGES];
-        float raw[2][4];                                       // the chunk's v, laid out as a tile of U
-        if constexpr (sizeof(T) == 2) {
-            unsigned v[4];                                     // tokens 0-7 of col, col + 8; tokens 8-15 of both
-            dc_ldmatrix_trans(v, &st.v[(lane & 7) + 8 * (lane >> 4)][group * 16 + 8 * ((lane >> 3) & 1)]);
+    const size_t width = (size_t)p.heads * p.vdim;
+    const int left = p.vdim - col;                             // columns col and col + 8 are there
+    // Operands of the next products are read well ahead of them, and sums that do not depend on one another are asked for
+    // together: a warp has its scheduler nearly to itself, so what one instruction waits for, all wait for.
+    unsigned bk[STEPS][4];                                     // K of the chunk (the first part), operand of S0^T k
+    DcValues<T> v;                                             // its v, laid out as a tile of U
+    auto ask = [&](const typename Sh::Stage& st) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    raw[j][2 * h] = __uint_as_float(v[2 * j + h] << 16);
-                    raw[j][2 * h + 1] = __uint_as_float(v[2 * j + h] & 0xffff0000u);
-                }
+        for (int k = 0; k < STEPS; ++k) dc_ldmatrix(bk[k], &st.keys.k[0][b_row][row0 + 16 * k + b_col]);
+        if constexpr (sizeof(T) == 2) {                        // tokens 0-7 of col, col + 8; tokens 8-15 of both
+            dc_ldmatrix_trans(v.x, &st.v[(lane & 7) + 8 * (lane >> 4)][group * 16 + 8 * ((lane >> 3) & 1)]);
         } else {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) raw[j][e] = to_float(st.v[8 * j + 2 * t + (e & 1)][group * 16 + g + 8 * (e >> 1)]);
+                for (int e = 0; e < 4; ++e) v.x[4 * j + e] = st.v[8 * j + 2 * t + (e & 1)][group * 16 + g + 8 * (e >> 1)];
         }
-        bool look = c % DC_REFRESH == 0;
+    };
+    dc_sync(DC_MEET, Sh::THREADS);                             // stage 0 is there
+    ask(sm.stage[0]);
+
+    for (int c = 0; c < chunks; ++c) {
+        const auto& st = sm.stage[c % DC_STAGES];
+        const int here = count - c * DC_TOKENS;                // tokens from the chunk's first on
+        bool look = c % DC_REFRESH == 0, spoiled = false;
         int bad[2] = {DC_TOKENS, DC_TOKENS};
         float u[2][4], wq[FINISH][4];
+        unsigned kt[STEPS][4];                                 // K again, operand of the new state
         for (int tries = 0;; ++tries) {
             if (look) {                                        // the columns' powers of two from the columns themselves
-                float most[2];
+                float most[2], raw[2][4];
+                v.widen(raw);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     most[h] = 0.f;
@@ -598,108 +695,88 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
             }
             // ---- S0^T k and S0^T q of the warp's rows: 16 columns x 16 tokens
-            float wk[2][4];
-            {
-                float low[2][4];
+            unsigned bq[STEPS][4], th[4], tl[4];
+            float wk[2][4], both[2][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wk[j][e] = low[j][e] = 0.f;
+            for (int k = 0; k < STEPS; ++k) dc_ldmatrix(bq[k], &st.keys.q[0][b_row][row0 + 16 * k + b_col]);
+            dc_state_product<STEPS>(wk, sh, sl, bk);
+            if (PARTS == 2) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
-                    unsigned b[4];
-                    dc_ldmatrix(b, &st.keys.k[0][b_row][row0 + 16 * k + b_col]);
+                    dc_ldmatrix(kt[k], &st.keys.k[PARTS - 1][b_row][row0 + 16 * k + b_col]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        dc_mma(wk[j], sh[k], b[2 * j], b[2 * j + 1]);
-                        dc_mma(low[j], sl[k], b[2 * j], b[2 * j + 1]);
-                    }
-                    if (PARTS == 2) {
-                        dc_ldmatrix(b, &st.keys.k[PARTS - 1][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) dc_mma(low[j], sh[k], b[2 * j], b[2 * j + 1]);
-                    }
+                    for (int j = 0; j < 2; ++j) dc_mma(wk[j], sh[k], kt[k][2 * j], kt[k][2 * j + 1]);
                 }
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wk[j][e] += low[j][e];
             }
             if (SLICES > 1) {
                 sm.swap[c & 1][warp][0][lane] = make_float4(wk[0][0], wk[0][1], wk[0][2], wk[0][3]);
                 sm.swap[c & 1][warp][1][lane] = make_float4(wk[1][0], wk[1][1], wk[1][2], wk[1][3]);
             }
-            {
-                float both[2][4], low[2][4];
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) both[j][e] = low[j][e] = 0.f;
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    unsigned b[4];
-                    dc_ldmatrix(b, &st.keys.q[0][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        dc_mma(both[j], sh[k], b[2 * j], b[2 * j + 1]);
-                        dc_mma(low[j], sl[k], b[2 * j], b[2 * j + 1]);
-                    }
-                    if (PARTS == 2) {
-                        dc_ldmatrix(b, &st.keys.q[PARTS - 1][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) dc_mma(low[j], sh[k], b[2 * j], b[2 * j + 1]);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) both[j][e] += low[j][e];
-                if constexpr (SLICES > 1) {
-                    float4 theirs;
-                    theirs.x = slice ? both[0][0] : both[1][0]; theirs.y = slice ? both[0][1] : both[1][1];
-                    theirs.z = slice ? both[0][2] : both[1][2]; theirs.w = slice ? both[0][3] : both[1][3];
-                    sm.swap[c & 1][warp][2][lane] = theirs;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wq[0][e] = slice ? both[1][e] : both[0][e];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) wq[j % FINISH][e] = both[j][e];
-                }
-            }
-            // ---- one meeting per chunk: the halves' sums are there, and so is the next stage
-            if (tries == 0) dc_sync(DC_FULL + (c + 1) % DC_STAGES, 32 * (DC_WALKERS + 1));
-            else if (SLICES > 1) dc_sync(DC_PAIR + group, 64);
-            if (SLICES > 1) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const float4 x = sm.swap[c & 1][warp ^ 1][j][lane];
-                    wk[j][0] += x.x; wk[j][1] += x.y; wk[j][2] += x.z; wk[j][3] += x.w;
-                }
-                const float4 x = sm.swap[c & 1][warp ^ 1][2][lane];
-                wq[0][0] += x.x; wq[0][1] += x.y; wq[0][2] += x.z; wq[0][3] += x.w;
-            }
-            // ---- R, U
-            float r[2][4];
-            float size = st.gates.odd[0];                      // NaN where T is not finite
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float2 before = *reinterpret_cast<const float2*>(&st.gates.before[8 * j + 2 * t]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    r[j][e] = fmaf((e & 1) ? -before.y : -before.x, wk[j][e], raw[j][e] * sigma[e >> 1]);
-                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(size) : "f"(fabsf(r[j][e])));
-                }
-            }
-            unsigned rh[4], rl[4], th[4], tl[4];
             dc_ldmatrix(th, &st.gates.t[0][b_row][b_col]);
             dc_ldmatrix(tl, &st.gates.t[1][b_row][b_col]);
+            const float2 before0 = *reinterpret_cast<const float2*>(&st.gates.before[2 * t]);
+            const float2 before1 = *reinterpret_cast<const float2*>(&st.gates.before[8 + 2 * t]);
+            float size = st.gates.odd[0];                      // NaN where T is not finite
+            dc_state_product<STEPS>(both, sh, sl, bq);
+            if (PARTS == 2) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    dc_ldmatrix(kt[k], &st.keys.q[PARTS - 1][b_row][row0 + 16 * k + b_col]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) dc_mma(both[j], sh[k], kt[k][2 * j], kt[k][2 * j + 1]);
+                }
+            }
+            if constexpr (SLICES > 1) {
+                sm.swap[c & 1][warp][2][lane] = make_float4(slice ? both[0][0] : both[1][0], slice ? both[0][1] : both[1][1],
+                                                            slice ? both[0][2] : both[1][2], slice ? both[0][3] : both[1][3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) wq[0][e] = slice ? both[1][e] : both[0][e];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) wq[j % FINISH][e] = both[j][e];
+            }
+            // ---- one meeting per chunk: the halves' sums are there, and so is the next stage
+            if (tries == 0) dc_sync(DC_MEET, Sh::THREADS);
+            else if (SLICES > 1) dc_sync(DC_PAIR + group, 64);
+            if (SLICES > 1) {
+                float4 x[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) x[j] = sm.swap[c & 1][warp ^ 1][j][lane];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    dc_add2(wk[j][0], wk[j][1], wk[j][0], wk[j][1], x[j].x, x[j].y);
+                    dc_add2(wk[j][2], wk[j][3], wk[j][2], wk[j][3], x[j].z, x[j].w);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
+            // ---- R, U
+            float r[2][4];
+            v.widen(r);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float2 before = j ? before1 : before0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float x, y;
+                    dc_mul2(x, y, r[j][2 * h], r[j][2 * h + 1], sigma[h], sigma[h]);
+                    dc_fma2(r[j][2 * h], r[j][2 * h + 1], -before.x, -before.y, wk[j][2 * h], wk[j][2 * h + 1], x, y);
+                    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(size) : "f"(fabsf(r[j][2 * h])), "f"(fabsf(r[j][2 * h + 1])));
+                }
+            }
+            unsigned rh[4], rl[4];
             dc_split_tiles(r[0], r[1], rh, rl);
             dc_solve(u, rh, rl, th, tl);
             if (!__any_sync(0xffffffffu, !(size < DC_MOST))) break;
-            if (tries == 0) { look = true; continue; }         // (both warps of a pair have the same R and T)
+            if (tries == 0) {                                  // (both warps of a pair have the same R and T)
+                look = true;
+                ask(st);
+                continue;
+            }
             // not a matter of size: something is not finite
+            spoiled = true;
             dc_first_bad(r, t, bad);
             dc_leave_out(r, t, bad);
             dc_split_tiles(r[0], r[1], rh, rl);
@@ -710,64 +787,91 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
         // ---- the new state
         unsigned uh[4], ul[4], zh[4], zl[4];
-        dc_split_tiles(u[0], u[1], zh, zl);
+        const float2 after0 = *reinterpret_cast<const float2*>(&st.gates.after[2 * t]);
+        const float2 after1 = *reinterpret_cast<const float2*>(&st.gates.after[8 + 2 * t]);
+        const float decay = st.gates.fade[DC_TOKENS - 1];
+        float faded[2][4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            const float2 after = *reinterpret_cast<const float2*>(&st.gates.after[8 * j + 2 * t]);
+            const float2 after = j ? after1 : after0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) u[j][e] *= (e & 1) ? after.y : after.x;
+            for (int e = 0; e < 4; e += 2) dc_mul2(faded[j][e], faded[j][e + 1], u[j][e], u[j][e + 1], after.x, after.y);
         }
-        dc_split_tiles(u[0], u[1], uh, ul);
-        const float decay = st.gates.fade[DC_TOKENS - 1];
+        dc_split_tiles(faded[0], faded[1], uh, ul);
+        float add[TILES][4];
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add[n][e] = 0.f;
+            dc_mma(add[n], ul, kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+        }
+        if (PARTS == 2) {
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                unsigned b[4];
+                dc_ldmatrix_trans(b, &st.keys.k[PARTS - 1][bt_row][row0 + 16 * k + bt_col]);
+                dc_mma(add[2 * k], uh, b[0], b[1]);
+                dc_mma(add[2 * k + 1], uh, b[2], b[3]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) dc_mma(add[n], uh, kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+        dc_split_tiles(u[0], u[1], zh, zl);
+        unsigned ph[4], pl[4];
+        if constexpr (SLICES > 1) {                            // the eight tokens' rows: both inner halves, both parts
+            dc_ldmatrix(ph, &st.gates.p[lane >> 4][8 * slice + (lane & 7)][b_col]);
+            pl[0] = ph[2]; pl[1] = ph[3];
+        } else {
+            dc_ldmatrix(ph, &st.gates.p[0][b_row][b_col]);
+            dc_ldmatrix(pl, &st.gates.p[1][b_row][b_col]);
+        }
+        if (SLICES > 1) {
+            const float4 x = sm.swap[c & 1][warp ^ 1][2][lane];
+            dc_add2(wq[0][0], wq[0][1], wq[0][0], wq[0][1], x.x, x.y);
+            dc_add2(wq[0][2], wq[0][3], wq[0][2], wq[0][3], x.z, x.w);
+        }
+        float oa[FINISH][4], ob[FINISH][4];
+#pragma unroll
+        for (int j = 0; j < FINISH; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) oa[j][e] = ob[j][e] = 0.f;
+            dc_mma(ob[j], zl, ph[2 * j], ph[2 * j + 1]);
+            dc_mma(oa[j], zh, ph[2 * j], ph[2 * j + 1]);
+            dc_mma(ob[j], zh, pl[2 * j], pl[2 * j + 1]);
+        }
+        if (c + 1 < chunks) ask(sm.stage[(c + 1) % DC_STAGES]);
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) {
-            unsigned b[4], b2[4];
-            dc_ldmatrix_trans(b, &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
-            if (PARTS == 2) dc_ldmatrix_trans(b2, &st.keys.k[PARTS - 1][bt_row][row0 + 16 * k + bt_col]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float a[4] = {0.f, 0.f, 0.f, 0.f};
-                dc_mma(a, ul, b[2 * j], b[2 * j + 1]);
-                if (PARTS == 2) dc_mma(a, uh, b2[2 * j], b2[2 * j + 1]);
-                dc_mma(a, uh, b[2 * j], b[2 * j + 1]);
+            for (int n = 2 * k; n < 2 * k + 2; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[2 * k + j][e] = fmaf(s[2 * k + j][e], decay, a[e]);
-            }
+                for (int e = 0; e < 4; e += 2)
+                    dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
             dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
         }
         // ---- outputs: the chunk's start and its own tokens
-        {
-            unsigned ph[4], pl[4];
-            if constexpr (SLICES > 1) {                        // the lanes' rows are the eight tokens, first and second inner half
-                const __half* from = &st.gates.p[lane >> 4][8 * slice + (lane & 7)][b_col];
-                dc_ldmatrix(ph, from);
-                pl[0] = ph[2]; pl[1] = ph[3];
-            } else {
-                dc_ldmatrix(ph, &st.gates.p[0][b_row][b_col]);
-                dc_ldmatrix(pl, &st.gates.p[1][b_row][b_col]);
-            }
 #pragma unroll
-            for (int j = 0; j < FINISH; ++j) {
-                float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-                dc_mma(b, zl, ph[2 * j], ph[2 * j + 1]);
-                dc_mma(a, zh, ph[2 * j], ph[2 * j + 1]);
-                dc_mma(b, zh, pl[2 * j], pl[2 * j + 1]);
-                const int first = 8 * (tile0 + j) + 2 * t;
-                const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[first]);
-                const float2 query = *reinterpret_cast<const float2*>(&st.gates.query[first]);
+        for (int j = 0; j < FINISH; ++j) {
+            const int first = 8 * (tile0 + j) + 2 * t;
+            const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[first]);
+            const float2 query = *reinterpret_cast<const float2*>(&st.gates.query[first]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int token = first + (e & 1);
-                    float o = fmaf((e & 1) ? fade.y : fade.x, wq[j][e], a[e] + b[e]) * ((e & 1) ? query.y : query.x) * back[e >> 1];
-                    if (token >= bad[e >> 1]) o = __int_as_float(0x7fffffff);
-                    if (c * DC_TOKENS + token < count && col + 8 * (e >> 1) < p.vdim)
-                        out[(size_t)token * p.heads * p.vdim + 8 * (e >> 1)] = o;
+            for (int h = 0; h < 2; ++h) {
+                float x, y, fx, fy;
+                dc_add2(x, y, oa[j][2 * h], oa[j][2 * h + 1], ob[j][2 * h], ob[j][2 * h + 1]);
+                dc_fma2(x, y, fade.x, fade.y, wq[j][2 * h], wq[j][2 * h + 1], x, y);
+                dc_mul2(fx, fy, query.x, query.y, back[h], back[h]);
+                dc_mul2(x, y, x, y, fx, fy);
+                if (spoiled) {
+                    if (first >= bad[h]) x = __int_as_float(0x7fffffff);
+                    if (first + 1 >= bad[h]) y = __int_as_float(0x7fffffff);
                 }
+                if (first < here && 8 * h < left) out[(size_t)first * width + 8 * h] = x;
+                if (first + 1 < here && 8 * h < left) out[(size_t)(first + 1) * width + 8 * h] = y;
             }
-            out += (size_t)DC_TOKENS * p.heads * p.vdim;
         }
-        if (c + DC_STAGES < chunks) dc_arrive(DC_EMPTY + c % DC_STAGES, 32 * (DC_WALKERS + 1));
-        if (__any_sync(0xffffffffu, min(bad[0], bad[1]) < DC_TOKENS)) {
+        out += (size_t)DC_TOKENS * width;
+        if (spoiled) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 if (bad[h] < DC_TOKENS) {
@@ -787,15 +891,21 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
 }
 
+constexpr int DC_ALONE_BYTES = 120 * 1024;     // more than half of an SM's shared memory
+static_assert(sizeof(DcShape<float, 128>::Shared) <= DC_ALONE_BYTES, "the largest shape");
+
 template <typename T, int DK, bool WIDE>
 static int launch_chunk(const DeltaParams& p, const DcRecords& records, int early, cudaStream_t stream) {
     using Sh = DcShape<T, DK>;
     auto kernel = delta_walk_kernel<T, DK, WIDE>;
-    static bool configured = false;            // per process and kernel; harmless if repeated
-    if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(typename Sh::Shared));
+    static int sms = 0;                        // per process and kernel; harmless if repeated
+    if (sms == 0) {
+        int device = 0, count = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_ALONE_BYTES);
         if (e != cudaSuccess) return (int)e;
-        configured = true;
+        sms = count;
     }
     const long long units = (long long)records.chunks * (p.heads / p.share);
     const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.items);
@@ -803,8 +913,11 @@ static int launch_chunk(const DeltaParams& p, const DcRecords& records, int earl
     const int rc = launch_dependent_if(early, delta_records_kernel<T, DK, WIDE>, dim3((unsigned)((units + DC_MAKERS - 1) / DC_MAKERS)),
                                        dim3(32 * DC_MAKERS), 0, stream, p, records);
     if (rc != 0) return rc;
+    // Two blocks on an SM take 2,200 cycles for a chunk of each, one alone 1,530: as many blocks as SMs had better not share any,
+    // which they do if they start while the records' blocks still hold some (ask for more than half of the shared memory).
+    const size_t smem = (long long)grid.x * grid.y * grid.z <= sms ? DC_ALONE_BYTES : sizeof(typename Sh::Shared);
     // the state is older than the records' kernel, which waits for whatever may have written it
-    return launch_dependent(kernel, grid, dim3(Sh::THREADS), sizeof(typename Sh::Shared), stream, p, records);
+    return launch_dependent(kernel, grid, dim3(Sh::THREADS), smem, stream, p, records);
 }
 
 template <typename T, int DK>
