@@ -1,4 +1,4 @@
-// The gated delta rule (formulas in delta_rule.cu) for prompts: chunks of 16 tokens on the tensor cores, 32-bit results.
+// The gated delta rule (formulas in delta_rule.cu) for prompts: chunks of 32 tokens on the tensor cores, 32-bit results.
 //
 // Inside a chunk that starts from state S0, with G_i = sum of log_decay over the chunk's tokens up to i and k, q divided by
 // their lengths,
@@ -6,31 +6,33 @@
 //   R_i = v_i - e^(G_i) S0^T k_i                      what the chunk's start leaves to be stored
 //   U   = T R,  T = (I + A)^-1 diag(beta)             A_ij = beta_i (k_i.k_j) e^(G_i - G_j) for j < i, else 0
 //   o_i = scale (e^(G_i) S0^T q_i + sum_(j <= i) (q_i.k_j) e^(G_i - G_j) u_j)
-//   S   = e^(G_15) S0 + sum_j e^(G_15 - G_j) k_j u_j^T
+//   S   = e^(G_31) S0 + sum_j e^(G_31 - G_j) k_j u_j^T
 //
-// 16 tokens are what one matrix instruction takes along its inner dimension: a longer chunk only adds to the two products
-// whose size grows with the chunk (T R and the sum over u_j).
+// A chunk is a chain - S0^T k, R, U, S - whose steps wait for one another, and a request's heads give a warp of its own to every
+// 16 columns and 64 rows of S only, so what bounds a prompt is the chain's latency.  A longer chunk puts more independent
+// instructions into every step; it adds to the two products that grow with the chunk (T R and the sum over u_j), by halves only
+// where the blocks of T above the diagonal are left out.  DC_MEASURED
 //
 // Precision.  States and outputs are 32-bit results, so no operand may be rounded to 11 bits.  q and k (bfloat16, 8 bits)
 // scaled by a power of two to a length of about one are exact in half precision; what is 32-bit - the state, R, U, T and the
 // weights of u_j - goes into the instructions as the sum of two half-precision numbers (22 bits), products of two low parts left
 // out.  Half precision has little range: every column of the state (a row of the transposed tiles below) has a power of
-// two, `sigma`, chosen from the column's and the chunk's own largest numbers every 32 chunks, and anew, with the chunk's
+// two, `sigma`, chosen from the column's and the chunk's own largest numbers every 16 chunks, and anew, with the chunk's
 // sums taken again, whenever a number of R leaves the range in between.  The state itself stays in 32-bit registers
 // and the instructions only ever sum up one chunk (their running sums are truncated, not rounded).  float32 storage: q and k
 // are two parts as well.
 //
 // Two kernels.  The first prepares all chunks side by side, a warp per chunk and q/k head: q and k in half precision, T by
 // substitution, the weights of u_j, the gates' factors, as records in the workspace that lie as the second kernel's shared
-// memory holds them.  The second walks a head's chunks, a block for every 16 GROUPS value columns, four more warps
-// keeping the records and v of the next chunks on their way into a ring of stages; all meet once per chunk and nothing spins.  (One kernel in which
-// four more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads: every block of value columns
-// prepared them again, and the two roles' code did not fit the instruction cache together.)
+// memory holds them.  The second walks a head's chunks, a block for every 16 GROUPS value columns, four more warps keeping
+// the records and v of the next chunks on their way into a ring of stages; all meet once per chunk and nothing spins.  (One
+// kernel in which four more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads: every block of
+// value columns prepared them again, and the two roles' code did not fit the instruction cache together.)
 //
 // Layout.  A warp of the second kernel owns 16 value columns x 64 rows of S, transposed: S^T is the 16-row operand of S0^T k
 // and S0^T q, the accumulator of S0^T k is (after R) the operand of the next product in the registers where it lies, and the
 // new sums end up where S lies.  Heads of more than 64 rows take two warps per 16 columns, which swap their halves' sums
-// through shared memory once per chunk.
+// through shared memory: of S0^T k in the chunk's one meeting, of S0^T q in the next chunk's.
 //
 // Values that are not finite: they spoil their column from their token on and nothing else, as in the recurrence - a product
 // with a zero of T would spoil the tokens before.  Such chunks are noticed by R and by a mark in their record, redone with those
@@ -42,17 +44,20 @@
 
 namespace fsie {
 
-constexpr int DC_TOKENS = 16;              // tokens of a chunk
-constexpr int DC_STAGES = 4;               // stages of the ring: the chunk's, the next one's and two on their way
+constexpr int DC_TOKENS = 32;              // tokens of a chunk
+constexpr int DC_TILES = DC_TOKENS / 8;    // ... in tiles of eight
+constexpr int DC_STAGES = 3;               // stages of the ring: the chunk's, the next one's and one on its way
 constexpr int DC_WALKERS = 4;              // warps that walk a block's chunks
+constexpr int DC_FETCHERS = 128;           // threads that copy
 constexpr int DC_SLICE = 64;               // rows of S (columns of k) per warp
 constexpr int DC_MAX_DIM = 128;
-constexpr int DC_REFRESH = 32;             // chunks between two looks at the state's size
-constexpr int DC_SIZE = 4;                 // ... which brings the largest number of a column to 2^4 .. 2^5
-constexpr int DC_TLD = DC_TOKENS + 8;      // padded rows: ldmatrix without bank conflicts
-// A number of R, times sigma, is below this: a row of T has at most 16 numbers of at most beta^2 <= 4 (what a token's value
-// still does to a later token's u passes through contractions), so that u, and u with a factor of at most 2, fit half precision.
-constexpr float DC_MOST = 500.f;
+constexpr int DC_REFRESH = 16;             // chunks between two looks at the state's size
+constexpr int DC_SIZE = 3;                 // ... which brings the largest number of a column to 2^3 .. 2^4
+constexpr int DC_TLD = 16 + 8;             // padded rows of a 16 x 16 block: ldmatrix without bank conflicts
+// A number of R, times sigma, is below this: right behind a look it is at most 2^4 (1 + sqrt(128)).  A row of T has 32 numbers
+// of at most beta^2 <= 4 (what a token's value still does to a later token's u passes through contractions), so that u, and
+// u with a factor of at most 2, fit half precision.
+constexpr float DC_MOST = 250.f;
 
 __device__ __forceinline__ unsigned dc_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void dc_ldmatrix(unsigned (&r)[4], const void* p) {
@@ -65,7 +70,7 @@ __device__ __forceinline__ void dc_ldmatrix_trans(unsigned (&r)[4], const void* 
 }
 // d += a(16x16, row) * b(16x8, col), half-precision operands, float accumulators
 __device__ __forceinline__ void dc_mma(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -162,28 +167,35 @@ __device__ __forceinline__ void dc_store8(float* p, const Raw8<float>& r) {
     *reinterpret_cast<float4*>(p) = r.x; *reinterpret_cast<float4*>(p + 4) = r.y;
 }
 
+// T and the weights of u_j are lower triangular: of their four 16 x 16 blocks those at (0, 0), (1, 0) and (1, 1) are kept.
 template <typename T, int DK>
-struct DcShape {
+struct DcRecord {
     static constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;       // half-precision numbers that hold a stored one
-    static constexpr int SLICES = DK / DC_SLICE;               // warps that share 16 value columns
-    static constexpr int GROUPS = DC_WALKERS / SLICES;         // groups of 16 value columns
-    static constexpr int COLS = 16 * GROUPS;                   // value columns of a block
     static constexpr int KLD = DK + 8;                         // padded row of q and k
-    static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 8);
-    static constexpr int THREADS = 2 * 32 * DC_WALKERS;        // the walkers' and the fetchers'
     struct alignas(16) Keys { __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD]; };
     struct alignas(16) Gates {
-        __half t[2][DC_TOKENS][DC_TLD], p[2][DC_TOKENS][DC_TLD];     // T and the weights of u_j, two parts each
+        __half t[2][3][16][DC_TLD], p[2][3][16][DC_TLD];       // T and the weights of u_j, two parts each
         float before[DC_TOKENS];          // on S0^T k: e^(G_i), the key's length, the power of two
-        float after[DC_TOKENS];           // on u_j in the new state: e^(G_15 - G_j), ...
+        float after[DC_TOKENS];           // on u_j in the new state: e^(G_31 - G_j), ...
         float query[DC_TOKENS];           // on an output: scale, the query's length, the power of two
         float fade[DC_TOKENS];            // e^(G_i)
         float odd[4];                     // NaN where T has a number that is not finite, else 0
     };
-    struct alignas(16) Stage { Keys keys; Gates gates; T v[DC_TOKENS][VLD]; };
+};
+
+template <typename T, int DK>
+struct DcShape : DcRecord<T, DK> {
+    static constexpr int SLICES = DK / DC_SLICE;               // warps that share 16 value columns
+    static constexpr int GROUPS = DC_WALKERS / SLICES;         // groups of 16 value columns
+    static constexpr int COLS = 16 * GROUPS;                   // value columns of a block
+    static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 8);
+    static constexpr int THREADS = 32 * DC_WALKERS + DC_FETCHERS;
+    static constexpr int FINISH = SLICES > 1 ? DC_TILES / 2 : DC_TILES;     // tiles of eight tokens whose outputs a warp finishes
+    static constexpr int SWAPS = SLICES > 1 ? DC_TILES + FINISH : 1;        // pieces of 16 bytes that a thread hands over
+    struct alignas(16) Stage { typename DcRecord<T, DK>::Keys keys; typename DcRecord<T, DK>::Gates gates; T v[DC_TOKENS][VLD]; };
     struct Shared {
         Stage stage[DC_STAGES];
-        float4 swap[2][DC_WALKERS][3][32];
+        float4 swap[2][DC_WALKERS][SWAPS][32];
         float most[DC_WALKERS][16];
     };
 };
@@ -201,22 +213,51 @@ __device__ __forceinline__ int dc_chunks_before(const int* __restrict__ item_qle
     return sum;
 }
 
-constexpr int DC_MAKERS = 4;               // warps of a preparing block
+// A product of two 16 x 16 matrices in two parts each: sum += a b, b's operand registers as ldmatrix gives them.
+__device__ __forceinline__ void dc_product(float (&sum)[2][4], const unsigned (&ah)[4], const unsigned (&al)[4], const unsigned (&bh)[4],
+                                           const unsigned (&bl)[4]) {
+    float low[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) low[j][e] = 0.f;
+        dc_mma(low[j], al, bh[2 * j], bh[2 * j + 1]);
+        dc_mma(sum[j], ah, bh[2 * j], bh[2 * j + 1]);
+        dc_mma(low[j], ah, bl[2 * j], bl[2 * j + 1]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[j][e] += low[j][e];
+}
 
-// a warp per chunk and q/k head
+template <typename T, int DK>
+struct DcMaker {                           // a preparing warp's shared memory: the records as they go out, and scratch
+    typename DcRecord<T, DK>::Keys keys;
+    typename DcRecord<T, DK>::Gates gates;
+    float a[2][16][16 + 4];                // A's blocks on the diagonal
+    __half w[2][16][DC_TLD];
+    double g[DC_TOKENS];
+    float kf[DC_TOKENS], qf[DC_TOKENS], beta[DC_TOKENS];
+};
+
+__device__ __forceinline__ void dc_copy_out(void* to, const void* from, int bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(to), "r"(dc_smem(from)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+}
+
+// a block of one warp per chunk and q/k head
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(32 * DC_MAKERS)
+__global__ void __launch_bounds__(32)
 delta_records_kernel(const DeltaParams p, const DcRecords records) {
-    using Sh = DcShape<T, DK>;
+    using Sh = DcRecord<T, DK>;
     constexpr int PARTS = Sh::PARTS, FOURS = DK / 32;          // 32 columns are a quad's eight each
-    struct Scratch { float a[DC_TOKENS][DC_TOKENS + 4]; double g[DC_TOKENS]; float f[DC_TOKENS], beta[DC_TOKENS]; };
-    __shared__ Scratch scratch[DC_MAKERS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    extern __shared__ __align__(16) unsigned char dc_raw[];
+    auto& own = *reinterpret_cast<DcMaker<T, DK>*>(dc_raw);
+    const int lane = threadIdx.x;
     const int g = lane >> 2, t = lane & 3;
-    auto& own = scratch[warp];
     const int narrow_heads = p.heads / p.share;
-    const long long unit = (long long)blockIdx.x * DC_MAKERS + warp;
-    const int chunk = (int)(unit / narrow_heads), narrow = (int)(unit - (long long)chunk * narrow_heads);
+    const int chunk = blockIdx.x / narrow_heads, narrow = blockIdx.x - chunk * narrow_heads;
     // the chunk's request and first token: 32 requests at a time
     int item = -1, place = 0;
     for (int i0 = 0, before = 0; i0 < records.items && item < 0; i0 += 32) {
@@ -241,186 +282,260 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
     grid_dependents_go();
     if (slot < 0 || chunk >= records.chunks) return;           // beyond the step's chunks, or a padding entry
     const T* qkv = (const T*)p.qkv;
-    // ---- q, k and the first head's gates on their way
-    Raw8<T> kr[2][FOURS], qr[2][FOURS];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = g + 8 * h;
-        const T* row = qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + narrow * p.dim;
-#pragma unroll
-        for (int f = 0; f < FOURS; ++f) {
-            const int d = f * 32 + t * 8, have = r < n ? p.dim - d : 0;
-            kr[h][f] = dc_load8<WIDE>(row + p.k_off + d, have);
-            qr[h][f] = dc_load8<WIDE>(row + p.q_off + d, have);
-        }
+    float decay = 0.f, beta = 0.f;                             // of the lane's token, the first head's
+    if (lane < n) {
+        decay = p.log_decay[(size_t)(first + lane) * p.heads + narrow * p.share];
+        beta = p.beta[(size_t)(first + lane) * p.heads + narrow * p.share];
     }
-    const int i = lane & 15;                                   // the lane's token (twice per warp)
-    float decay = 0.f, beta = 0.f;
-    if (i < n) {
-        decay = p.log_decay[(size_t)(first + i) * p.heads + narrow * p.share];
-        beta = p.beta[(size_t)(first + i) * p.heads + narrow * p.share];
-    }
-    // ---- lengths of q and k, a power of two that brings each below one, both in half precision
-    float kk[2], qq[2];
-    unsigned kh[PARTS][2][FOURS][4], qh[PARTS][2][FOURS][4];
-    float kf[2], qf[2];                                    // length and power of two as one factor
+    // ---- q and k: their lengths, a power of two that brings each below one, both in half precision.  16 tokens at a time, a
+    // quad per token; in bfloat16 all loads go out first
+    constexpr int PAIRS = sizeof(T) == 2 ? 2 : 1;              // of 16 tokens that are held at once
+    Raw8<T> kr[PAIRS][2][FOURS], qr[PAIRS][2][FOURS];
+    auto load = [&](int m, Raw8<T> (&k)[2][FOURS], Raw8<T> (&q)[2][FOURS]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        kk[h] = qq[h] = 0.f;
-        float x[8];
+        for (int h = 0; h < 2; ++h) {
+            const int r = 16 * m + g + 8 * h;
+            const T* row = qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + narrow * p.dim;
 #pragma unroll
-        for (int f = 0; f < FOURS; ++f) {
-            dc_widen(kr[h][f], x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) kk[h] = fmaf(x[i], x[i], kk[h]);
-            dc_widen(qr[h][f], x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) qq[h] = fmaf(x[i], x[i], qq[h]);
-        }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            kk[h] += __shfl_xor_sync(0xffffffffu, kk[h], o);
-            qq[h] += __shfl_xor_sync(0xffffffffu, qq[h], o);
-        }
-        const int ke = (((__float_as_int(kk[h]) >> 23) & 255) - 125) >> 1, qe = (((__float_as_int(qq[h]) >> 23) & 255) - 125) >> 1;
-        const float ks = dc_power(-ke), qs = dc_power(-qe);
-        kf[h] = dc_power(ke) / sqrtf(kk[h] + p.eps);
-        qf[h] = p.scale * (dc_power(qe) / sqrtf(qq[h] + p.eps));
-#pragma unroll
-        for (int f = 0; f < FOURS; ++f) {
-            dc_widen(kr[h][f], x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (PARTS == 2) dc_split(x[2 * i] * ks, x[2 * i + 1] * ks, kh[0][h][f][i], kh[PARTS - 1][h][f][i]);
-                else kh[0][h][f][i] = dc_bits(__floats2half2_rn(x[2 * i] * ks, x[2 * i + 1] * ks));
-            }
-            dc_widen(qr[h][f], x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (PARTS == 2) dc_split(x[2 * i] * qs, x[2 * i + 1] * qs, qh[0][h][f][i], qh[PARTS - 1][h][f][i]);
-                else qh[0][h][f][i] = dc_bits(__floats2half2_rn(x[2 * i] * qs, x[2 * i + 1] * qs));
+            for (int f = 0; f < FOURS; ++f) {
+                const int d = f * 32 + t * 8, have = r < n ? p.dim - d : 0;
+                k[h][f] = dc_load8<WIDE>(row + p.k_off + d, have);
+                q[h][f] = dc_load8<WIDE>(row + p.q_off + d, have);
             }
         }
-    }
-    // ---- K K^T and Q K^T: a lane's eight neighbouring values are operand registers as they are, because both operands
-    // take their inner index in the same order
-    float kkt[2][2][4], qkt[2][2][4];                      // [two chains][columns 0-7, 8-15]
+    };
+    // one of q and k of one token: into `to` (PARTS rows `part_step` apart), returns the scaled number's way back to a unit length
+    auto bring = [&](const Raw8<T> (&raw)[FOURS], __half* to) {
+        float sum = 0.f, x[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+        for (int f = 0; f < FOURS; ++f) {
+            dc_widen(raw[f], x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const int e = (((__float_as_int(sum) >> 23) & 255) - 125) >> 1;
+        const float scale = dc_power(-e);
+#pragma unroll
+        for (int f = 0; f < FOURS; ++f) {
+            dc_widen(raw[f], x);
+            unsigned high[4], low[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (PARTS == 2) dc_split(x[2 * i] * scale, x[2 * i + 1] * scale, high[i], low[i]);
+                else high[i] = dc_bits(__floats2half2_rn(x[2 * i] * scale, x[2 * i + 1] * scale));
+            }
+            *reinterpret_cast<uint4*>(to + f * 32 + t * 8) = make_uint4(high[0], high[1], high[2], high[3]);
+            if (PARTS == 2)
+                *reinterpret_cast<uint4*>(to + DC_TOKENS * Sh::KLD + f * 32 + t * 8) = make_uint4(low[0], low[1], low[2], low[3]);
+        }
+        return dc_power(e) / sqrtf(sum + p.eps);
+    };
+    auto bring_all = [&](int m, const Raw8<T> (&k)[2][FOURS], const Raw8<T> (&q)[2][FOURS]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = 16 * m + g + 8 * h;
+            const float kf = bring(k[h], own.keys.k[0][r]), qf = bring(q[h], own.keys.q[0][r]);
+            if (t == 0) { own.kf[r] = kf; own.qf[r] = p.scale * qf; }
+        }
+    };
+    if constexpr (PAIRS == 2) {
+        load(0, kr[0], qr[0]);
+        load(1, kr[PAIRS - 1], qr[PAIRS - 1]);
+        bring_all(0, kr[0], qr[0]);
+        bring_all(1, kr[PAIRS - 1], qr[PAIRS - 1]);
+    } else {
+#pragma unroll 1
+        for (int m = 0; m < 2; ++m) {
+            load(m, kr[0], qr[0]);
+            bring_all(m, kr[0], qr[0]);
+        }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // generic writes before async-proxy reads
+    __syncwarp();
+    if (lane == 0)
+        dc_copy_out(records.keys + ((size_t)chunk * narrow_heads + narrow) * sizeof(typename Sh::Keys), &own.keys, sizeof(typename Sh::Keys));
+    // ---- K K^T and Q K^T, blocks (0, 0), (1, 0) and (1, 1)
+    float kkt[3][2][4], qkt[3][2][4];
+#pragma unroll
+    for (int b = 0; b < 3; ++b)
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) kkt[i][j][e] = qkt[i][j][e] = 0.f;
+            for (int e = 0; e < 4; ++e) kkt[b][j][e] = qkt[b][j][e] = 0.f;
+    const int a_row = lane & 15, a_col = 8 * (lane >> 4);      // ldmatrix, 16-row operand; its registers 0, 2 and 1, 3 are an 8-column one's
+#pragma unroll 2
+    for (int d = 0; d < DK; d += 16) {
 #pragma unroll
-    for (int f = 0; f < FOURS; ++f) {
+        for (int pb = 0; pb < PARTS; ++pb) {
+            unsigned kb[2][4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {                      // inner 16 of the 32 columns
+            for (int m = 0; m < 2; ++m) dc_ldmatrix(kb[m], &own.keys.k[pb][16 * m + a_row][d + a_col]);
 #pragma unroll
-            for (int pa = 0; pa < PARTS; ++pa) {
+            for (int pa = 0; pa + pb < PARTS; ++pa) {
+                unsigned ka[2][4], qa[2][4];
 #pragma unroll
-                for (int pb = 0; pb + pa < PARTS; ++pb) {
-                    const unsigned ka[4] = {kh[pa][0][f][2 * i], kh[pa][1][f][2 * i], kh[pa][0][f][2 * i + 1], kh[pa][1][f][2 * i + 1]};
-                    const unsigned qa[4] = {qh[pa][0][f][2 * i], qh[pa][1][f][2 * i], qh[pa][0][f][2 * i + 1], qh[pa][1][f][2 * i + 1]};
+                for (int m = 0; m < 2; ++m) {
+                    if (pa == pb) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) ka[m][e] = kb[m][e];
+                    } else {
+                        dc_ldmatrix(ka[m], &own.keys.k[pa][16 * m + a_row][d + a_col]);
+                    }
+                    dc_ldmatrix(qa[m], &own.keys.q[pa][16 * m + a_row][d + a_col]);
+                }
+#pragma unroll
+                for (int b = 0; b < 3; ++b)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        dc_mma(kkt[i][j], ka, kh[pb][j][f][2 * i], kh[pb][j][f][2 * i + 1]);
-                        dc_mma(qkt[i][j], qa, kh[pb][j][f][2 * i], kh[pb][j][f][2 * i + 1]);
+                        dc_mma(kkt[b][j], ka[b > 0], kb[b == 2][j], kb[b == 2][2 + j]);
+                        dc_mma(qkt[b][j], qa[b > 0], kb[b == 2][j], kb[b == 2][2 + j]);
                     }
-                }
             }
         }
     }
-    auto* keys = reinterpret_cast<typename Sh::Keys*>(records.keys) + ((size_t)chunk * narrow_heads + narrow);
-#pragma unroll
-    for (int part = 0; part < PARTS; ++part)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int f = 0; f < FOURS; ++f) {
-                const unsigned(&a)[4] = kh[part][h][f];
-                const unsigned(&b)[4] = qh[part][h][f];
-                *reinterpret_cast<uint4*>(&keys->k[part][g + 8 * h][f * 32 + t * 8]) = make_uint4(a[0], a[1], a[2], a[3]);
-                *reinterpret_cast<uint4*>(&keys->q[part][g + 8 * h][f * 32 + t * 8]) = make_uint4(b[0], b[1], b[2], b[3]);
-            }
-    const int from = (lane & 7) * 4;                           // a lane of the quad that holds row lane & 7
-    const float kf0 = __shfl_sync(0xffffffffu, kf[0], from), kf1 = __shfl_sync(0xffffffffu, kf[1], from);
-    const float qf0 = __shfl_sync(0xffffffffu, qf[0], from), qf1 = __shfl_sync(0xffffffffu, qf[1], from);
-    const float kfi = (lane & 8) ? kf1 : kf0, qfi = (lane & 8) ? qf1 : qf0;        // of token i
-    if (lane < DC_TOKENS) own.f[lane] = kfi;
+    const float kf = own.kf[lane], qf = own.qf[lane];
+    const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);   // ldmatrix.trans, operand stored [k][n]
     // ---- the gates of every head that reads these q and k
 #pragma unroll 1
     for (int z = 0; z < p.share; ++z) {
         const int head = narrow * p.share + z;
-        auto* to = reinterpret_cast<typename Sh::Gates*>(records.gates) + ((size_t)chunk * p.heads + head);
         // sums of log_decay in 64 bits, so that a difference of two of them is as exact as its own terms
         double sum = decay < -1e4f ? -1e4 : (double)decay;     // (e^-10000 is zero)
 #pragma unroll
         for (int o = 1; o < DC_TOKENS; o <<= 1) {
-            const double left = __shfl_up_sync(0xffffffffu, sum, o, DC_TOKENS);
-            if (i >= o) sum += left;
+            const double left = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += left;
         }
-        const double all = __shfl_sync(0xffffffffu, sum, DC_TOKENS - 1, DC_TOKENS);
-        if (lane < DC_TOKENS) { own.g[lane] = sum; own.beta[lane] = beta; }
+        const double all = __shfl_sync(0xffffffffu, sum, DC_TOKENS - 1);
+        own.g[lane] = sum;
+        own.beta[lane] = beta;
+        if (z > 0) {                                           // the last head's record has left
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+            __syncwarp();
+        }
         const float fade = expf((float)sum);
-        if (lane < DC_TOKENS) {
-            to->before[lane] = fade * kfi; to->after[lane] = expf((float)(all - sum)) * kfi; to->query[lane] = qfi; to->fade[lane] = fade;
-        }
-        if (z + 1 < p.share && i < n) {                        // the next head's
-            decay = p.log_decay[(size_t)(first + i) * p.heads + head + 1];
-            beta = p.beta[(size_t)(first + i) * p.heads + head + 1];
+        own.gates.before[lane] = fade * kf;
+        own.gates.after[lane] = expf((float)(all - sum)) * kf;
+        own.gates.query[lane] = qf;
+        own.gates.fade[lane] = fade;
+        if (z + 1 < p.share && lane < n) {                     // the next head's
+            decay = p.log_decay[(size_t)(first + lane) * p.heads + head + 1];
+            beta = p.beta[(size_t)(first + lane) * p.heads + head + 1];
         }
         __syncwarp();
+        float below[2][4];                                     // block (1, 0) of A without beta
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int col = 8 * j + 2 * t;
-            const double g0 = own.g[col], g1 = own.g[col + 1];
-            const float f0 = own.f[col], f1 = own.f[col + 1];
+        for (int b = 0; b < 3; ++b)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = g + 8 * h;
-                const double gr = own.g[row];
-                const float mine = own.beta[row] * own.f[row];
-                const float e0 = expf((float)(gr - g0)) * f0, e1 = expf((float)(gr - g1)) * f1;
-                const float w0 = row >= col ? (qkt[0][j][2 * h] + qkt[1][j][2 * h]) * e0 : 0.f;
-                const float w1 = row > col ? (qkt[0][j][2 * h + 1] + qkt[1][j][2 * h + 1]) * e1 : 0.f;
-                unsigned high, low;
-                dc_split(w0, w1, high, low);
-                *reinterpret_cast<unsigned*>(&to->p[0][row][col]) = high;
-                *reinterpret_cast<unsigned*>(&to->p[1][row][col]) = low;
-                own.a[row][col] = row > col ? mine * (kkt[0][j][2 * h] + kkt[1][j][2 * h]) * e0 : 0.f;
-                own.a[row][col + 1] = row > col + 1 ? mine * (kkt[0][j][2 * h + 1] + kkt[1][j][2 * h + 1]) * e1 : 0.f;
+            for (int j = 0; j < 2; ++j) {
+                const int bc = 8 * j + 2 * t, col = 16 * (b == 2) + bc;
+                const double g0 = own.g[col], g1 = own.g[col + 1];
+                const float f0 = own.kf[col], f1 = own.kf[col + 1];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int br = g + 8 * h, row = 16 * (b > 0) + br;
+                    const double gr = own.g[row];
+                    const float e0 = expf((float)(gr - g0)) * f0, e1 = expf((float)(gr - g1)) * f1;
+                    unsigned high, low;
+                    dc_split(row >= col ? qkt[b][j][2 * h] * e0 : 0.f, row > col ? qkt[b][j][2 * h + 1] * e1 : 0.f, high, low);
+                    *reinterpret_cast<unsigned*>(&own.gates.p[0][b][br][bc]) = high;
+                    *reinterpret_cast<unsigned*>(&own.gates.p[1][b][br][bc]) = low;
+                    const float x = own.kf[row] * kkt[b][j][2 * h] * e0, y = own.kf[row] * kkt[b][j][2 * h + 1] * e1;
+                    if (b == 1) {
+                        below[j][2 * h] = x; below[j][2 * h + 1] = y;
+                    } else {
+                        own.a[b / 2][br][bc] = row > col ? own.beta[row] * x : 0.f;
+                        own.a[b / 2][br][bc + 1] = row > col + 1 ? own.beta[row] * y : 0.f;
+                    }
+                }
             }
-        }
         __syncwarp();
-        // row i of (I + A)^-1 in lane i (and again in lane i + 16): from x (I + A) = e_i, last column first
-        float x[DC_TOKENS];
+        // blocks (0, 0) and (1, 1) of T: row i of (I + A)^-1 in a lane, from x (I + A) = e_i, last column first
+        const int i = lane & 15, m = lane >> 4;
+        float x[16];
 #pragma unroll
-        for (int j = 0; j < DC_TOKENS; ++j) x[j] = i == j ? 1.f : 0.f;
+        for (int j = 0; j < 16; ++j) x[j] = i == j ? 1.f : 0.f;
 #pragma unroll
-        for (int l = DC_TOKENS - 1; l >= 1; --l) {
+        for (int l = 15; l >= 1; --l) {
             if (l <= i) {
 #pragma unroll
-                for (int j = 0; j < l; ++j) x[j] = fmaf(-x[l], own.a[l][j], x[j]);
+                for (int j = 0; j < l; ++j) x[j] = fmaf(-x[l], own.a[m][l][j], x[j]);
             }
         }
         bool finite = true;
 #pragma unroll
-        for (int j = 0; j < DC_TOKENS; ++j) {
-            x[j] = j <= i ? x[j] * own.beta[j] : 0.f;
+        for (int j = 0; j < 16; ++j) {
+            x[j] = j <= i ? x[j] * own.beta[16 * m + j] : 0.f;
             finite = finite && fabsf(x[j]) < INFINITY;
         }
         const bool odd = !__all_sync(0xffffffffu, finite);
-        if (lane == 0) to->odd[0] = odd ? __int_as_float(0x7fffffff) : 0.f;
-        unsigned high[DC_TOKENS / 2], low[DC_TOKENS / 2];
+        if (lane == 0) own.gates.odd[0] = odd ? __int_as_float(0x7fffffff) : 0.f;
+        {
+            unsigned high[8], low[8];
 #pragma unroll
-        for (int j = 0; j < DC_TOKENS / 2; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
-        // the two lanes that hold a row write one part each
-        uint4* row = reinterpret_cast<uint4*>(&to->t[lane >> 4][i][0]);
-        const bool second = lane >= 16;
-        row[0] = second ? make_uint4(low[0], low[1], low[2], low[3]) : make_uint4(high[0], high[1], high[2], high[3]);
-        row[1] = second ? make_uint4(low[4], low[5], low[6], low[7]) : make_uint4(high[4], high[5], high[6], high[7]);
+            for (int j = 0; j < 8; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
+            uint4* to = reinterpret_cast<uint4*>(&own.gates.t[0][2 * m][i][0]);
+            to[0] = make_uint4(high[0], high[1], high[2], high[3]);
+            to[1] = make_uint4(high[4], high[5], high[6], high[7]);
+            to = reinterpret_cast<uint4*>(&own.gates.t[1][2 * m][i][0]);
+            to[0] = make_uint4(low[0], low[1], low[2], low[3]);
+            to[1] = make_uint4(low[4], low[5], low[6], low[7]);
+        }
         __syncwarp();
+        // block (1, 0): -T_11 (A_10 / beta) T_00, beta being in T_11
+        {
+            unsigned ah[4], al[4], bh[4], bl[4];
+            float w[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j][e] = 0.f;
+            dc_split_tiles(below[0], below[1], ah, al);
+            dc_ldmatrix_trans(bh, &own.gates.t[0][0][bt_row][bt_col]);
+            dc_ldmatrix_trans(bl, &own.gates.t[1][0][bt_row][bt_col]);
+            dc_product(w, ah, al, bh, bl);
+            // a number that is not finite is in T's other blocks too, and must not reach rows above its own
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j][e] = fabsf(w[j][e]) < INFINITY ? -w[j][e] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unsigned high, low;
+                    dc_split(w[j][2 * h], w[j][2 * h + 1], high, low);
+                    *reinterpret_cast<unsigned*>(&own.w[0][g + 8 * h][8 * j + 2 * t]) = high;
+                    *reinterpret_cast<unsigned*>(&own.w[1][g + 8 * h][8 * j + 2 * t]) = low;
+                }
+            __syncwarp();
+            dc_ldmatrix(ah, &own.gates.t[0][2][a_row][a_col]);
+            dc_ldmatrix(al, &own.gates.t[1][2][a_row][a_col]);
+            dc_ldmatrix_trans(bh, &own.w[0][bt_row][bt_col]);
+            dc_ldmatrix_trans(bl, &own.w[1][bt_row][bt_col]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j][e] = 0.f;
+            dc_product(w, ah, al, bh, bl);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    unsigned high, low;
+                    dc_split(w[j][2 * h], w[j][2 * h + 1], high, low);
+                    *reinterpret_cast<unsigned*>(&own.gates.t[0][1][g + 8 * h][8 * j + 2 * t]) = high;
+                    *reinterpret_cast<unsigned*>(&own.gates.t[1][1][g + 8 * h][8 * j + 2 * t]) = low;
+                }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)
+            dc_copy_out(records.gates + ((size_t)chunk * p.heads + head) * sizeof(typename Sh::Gates), &own.gates, sizeof(typename Sh::Gates));
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
 }
 
 __device__ __forceinline__ void dc_copy16(void* dst, const void* src, bool there) {
@@ -436,7 +551,6 @@ template <typename T, int DK, bool WIDE>
 struct DcFetch {
     using Sh = DcShape<T, DK>;
     using Stage = typename Sh::Stage;
-    static constexpr int FETCHERS = 32 * DC_WALKERS;
     static constexpr int PER = 16 / sizeof(T), ACROSS = Sh::COLS / PER;          // 16-byte pieces of a row of v
     static constexpr int KEYS = sizeof(typename Sh::Keys) / 16, GATES = sizeof(typename Sh::Gates) / 16;
     const unsigned char* keys;
@@ -446,7 +560,7 @@ struct DcFetch {
     int left, row, have;                                       // tokens from the next chunk on; the thread's row of v, its columns there
 
     __device__ __forceinline__ DcFetch(const DeltaParams& p, const DcRecords& records, int head, int col0, int t0, int count, int chunk0) {
-        const int narrow_heads = p.heads / p.share, tid = threadIdx.x - FETCHERS;
+        const int narrow_heads = p.heads / p.share, tid = threadIdx.x - 32 * DC_WALKERS;
         keys_step = (size_t)narrow_heads * sizeof(typename Sh::Keys);
         gates_step = (size_t)p.heads * sizeof(typename Sh::Gates);
         v_step = (size_t)DC_TOKENS * p.ld;
@@ -459,18 +573,18 @@ struct DcFetch {
         left = count;
     }
     __device__ __forceinline__ void next(const DeltaParams& p, Stage& st) {
-        const int tid = threadIdx.x - FETCHERS;
+        const int tid = threadIdx.x - 32 * DC_WALKERS;
         if (left > 0) {
 #pragma unroll
-            for (int i = 0; i < (KEYS + FETCHERS - 1) / FETCHERS; ++i)
-                if ((i + 1) * FETCHERS <= KEYS || tid + i * FETCHERS < KEYS)
-                    dc_copy16(reinterpret_cast<uint4*>(&st.keys) + tid + i * FETCHERS, keys + i * FETCHERS * 16, true);
+            for (int i = 0; i < (KEYS + DC_FETCHERS - 1) / DC_FETCHERS; ++i)
+                if ((i + 1) * DC_FETCHERS <= KEYS || tid + i * DC_FETCHERS < KEYS)
+                    dc_copy16(reinterpret_cast<uint4*>(&st.keys) + tid + i * DC_FETCHERS, keys + i * DC_FETCHERS * 16, true);
 #pragma unroll
-            for (int i = 0; i < (GATES + FETCHERS - 1) / FETCHERS; ++i)
-                if ((i + 1) * FETCHERS <= GATES || tid + i * FETCHERS < GATES)
-                    dc_copy16(reinterpret_cast<uint4*>(&st.gates) + tid + i * FETCHERS, gates + i * FETCHERS * 16, true);
+            for (int i = 0; i < (GATES + DC_FETCHERS - 1) / DC_FETCHERS; ++i)
+                if ((i + 1) * DC_FETCHERS <= GATES || tid + i * DC_FETCHERS < GATES)
+                    dc_copy16(reinterpret_cast<uint4*>(&st.gates) + tid + i * DC_FETCHERS, gates + i * DC_FETCHERS * 16, true);
             if constexpr (WIDE) {
-                constexpr int ROWS = FETCHERS / ACROSS;     // rows of v that the block's threads copy at once
+                constexpr int ROWS = DC_FETCHERS / ACROSS;     // rows of v that the block's threads copy at once
 #pragma unroll
                 for (int r = 0; r < DC_TOKENS; r += ROWS) {
                     const bool there = r + row < left && have > 0;
@@ -478,7 +592,7 @@ struct DcFetch {
                         dc_copy16(&st.v[r + row][(tid % ACROSS) * PER], v + (there ? (size_t)(r + row) * p.ld : 0), there);
                 }
             } else {
-                for (int e = tid; e < DC_TOKENS * Sh::COLS; e += FETCHERS) {
+                for (int e = tid; e < DC_TOKENS * Sh::COLS; e += DC_FETCHERS) {
                     const int r = e / Sh::COLS, d = e % Sh::COLS;
                     st.v[r][d] = r < left && d < have ? v[(size_t)r * p.ld + d] : from_float<T>(0.f);
                 }
@@ -492,35 +606,13 @@ struct DcFetch {
     }
 };
 
-// S0^T times a chunk's keys or queries, the state in two parts (in sums of their own: low parts are lost beside high ones)
-template <int STEPS>
-__device__ __forceinline__ void dc_state_product(float (&sum)[2][4], const unsigned (&high)[STEPS][4], const unsigned (&low)[STEPS][4],
-                                                 const unsigned (&b)[STEPS][4]) {
-    float lows[2][4];
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sum[j][e] = lows[j][e] = 0.f;
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            dc_mma(sum[j], high[k], b[k][2 * j], b[k][2 * j + 1]);
-            dc_mma(lows[j], low[k], b[k][2 * j], b[k][2 * j + 1]);
-        }
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) dc_add2(sum[j][e], sum[j][e + 1], sum[j][e], sum[j][e + 1], lows[j][e], lows[j][e + 1]);
-}
-
 // a thread's v of one chunk as it is stored
 template <typename T> struct DcValues;
 template <> struct DcValues<bf16> {
-    unsigned x[4];
-    __device__ __forceinline__ void widen(float (&r)[2][4]) const {
+    unsigned x[2 * DC_TILES];
+    __device__ __forceinline__ void widen(float (&r)[DC_TILES][4]) const {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 r[j][2 * h] = __uint_as_float(x[2 * j + h] << 16);
@@ -529,34 +621,46 @@ template <> struct DcValues<bf16> {
     }
 };
 template <> struct DcValues<float> {
-    float x[8];
-    __device__ __forceinline__ void widen(float (&r)[2][4]) const {
+    float x[4 * DC_TILES];
+    __device__ __forceinline__ void widen(float (&r)[DC_TILES][4]) const {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) r[e >> 2][e & 3] = x[e];
+        for (int e = 0; e < 4 * DC_TILES; ++e) r[e >> 2][e & 3] = x[e];
     }
 };
 
-// U = T R (both in two parts): operands R (high, low), T's parts as they lie in the stage
-__device__ __forceinline__ void dc_solve(float (&u)[2][4], const unsigned (&rh)[4], const unsigned (&rl)[4], const unsigned (&th)[4],
-                                         const unsigned (&tl)[4]) {
+// U = T R, all in two parts; th, tl: T's blocks (0, 0), (1, 0), (1, 1)
+__device__ __forceinline__ void dc_solve(float (&u)[DC_TILES][4], const unsigned (&rh)[2][4], const unsigned (&rl)[2][4],
+                                         const unsigned (&th)[3][4], const unsigned (&tl)[3][4]) {
+    float low[DC_TILES][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-        dc_mma(b, rl, th[2 * j], th[2 * j + 1]);
-        dc_mma(a, rh, th[2 * j], th[2 * j + 1]);
-        dc_mma(b, rh, tl[2 * j], tl[2 * j + 1]);
+    for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) dc_add2(u[j][e], u[j][e + 1], a[e], a[e + 1], b[e], b[e + 1]);
+        for (int e = 0; e < 4; ++e) u[j][e] = low[j][e] = 0.f;
+    // (tile after tile, so that no sum waits for its own last instruction)
+#pragma unroll
+    for (int b = 0; b < 3; ++b) {
+        const int block = b == 0 ? 1 : b == 1 ? 0 : 2, in = block == 2, to = 2 * (block > 0);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            dc_mma(low[to + j], rl[in], th[block][2 * j], th[block][2 * j + 1]);
+            dc_mma(u[to + j], rh[in], th[block][2 * j], th[block][2 * j + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) dc_mma(low[to + j], rh[in], tl[block][2 * j], tl[block][2 * j + 1]);
     }
+#pragma unroll
+    for (int j = 0; j < DC_TILES; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) dc_add2(u[j][e], u[j][e + 1], u[j][e], u[j][e + 1], low[j][e], low[j][e + 1]);
 }
 
 // the first token of each of the thread's two rows whose value is not finite (DC_TOKENS: none), over the row's four lanes
-__device__ __forceinline__ void dc_first_bad(const float (&x)[2][4], int t, int (&first)[2]) {
+__device__ __forceinline__ void dc_first_bad(const float (&x)[DC_TILES][4], int t, int (&first)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         int at = DC_TOKENS;
 #pragma unroll
-        for (int j = 1; j >= 0; --j)
+        for (int j = DC_TILES - 1; j >= 0; --j)
 #pragma unroll
             for (int e = 1; e >= 0; --e)
                 if (!(fabsf(x[j][2 * h + e]) < INFINITY)) at = 8 * j + 2 * t + e;
@@ -565,19 +669,19 @@ __device__ __forceinline__ void dc_first_bad(const float (&x)[2][4], int t, int 
         first[h] = min(first[h], at);
     }
 }
-__device__ __forceinline__ void dc_leave_out(float (&x)[2][4], int t, const int (&first)[2]) {
+__device__ __forceinline__ void dc_leave_out(float (&x)[DC_TILES][4], int t, const int (&first)[2]) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             if (8 * j + 2 * t + (e & 1) >= first[e >> 1]) x[j][e] = 0.f;
 }
 
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(2 * 32 * DC_WALKERS, 2)
+__global__ void __launch_bounds__(32 * DC_WALKERS + DC_FETCHERS, 2)
 delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     using Sh = DcShape<T, DK>;
-    constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16;
+    constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16, FINISH = Sh::FINISH;
     extern __shared__ __align__(16) unsigned char dc_raw[];
     auto& sm = *reinterpret_cast<typename Sh::Shared*>(dc_raw);
     const int head = blockIdx.y, item = blockIdx.z, col0 = blockIdx.x * Sh::COLS;
@@ -587,7 +691,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     const int chunks = (count + DC_TOKENS - 1) / DC_TOKENS;
     const int chunk0 = dc_chunks_before(p.item_qlen, item, lane);
     if (chunk0 + chunks > records.chunks) return;              // lists that name more tokens than there are
-    // registers: two blocks of 256 threads have 128 each; the walkers' four warps take over most of the fetchers' (216 + 40)
+    // registers: two blocks of 256 threads have 128 each; the walking warps take over most of the fetching ones' (216 + 40)
     if (warp >= DC_WALKERS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
         grid_dependency_wait();
@@ -595,11 +699,14 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         DcFetch<T, DK, WIDE> fetch(p, records, head, col0, t0, count, chunk0);
         fetch.next(p, sm.stage[0]);
         fetch.next(p, sm.stage[1]);
-        for (int c = 0; c <= chunks; ++c) {                    // (the last meeting is for a chunk that is not there)
-            asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+        asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+        dc_sync(DC_MEET, Sh::THREADS);                         // chunk 0 is there
+        for (int c = 1; c <= chunks + 1; ++c) {                // (the last meetings are for chunks that are not there)
+            asm volatile("cp.async.wait_group 0;\n" ::: "memory");
             dc_sync(DC_MEET, Sh::THREADS);                     // chunk c is there, and everybody is through with chunk c - 2:
-            fetch.next(p, sm.stage[(c + 2) % DC_STAGES]);      // its stage takes chunk c + 2
+            fetch.next(p, sm.stage[(c + 1) % DC_STAGES]);      // its stage takes chunk c + 1
         }
+        asm volatile("cp.async.wait_group 0;\n" ::: "memory");
         return;
     }
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
@@ -620,29 +727,60 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     grid_dependency_wait();
     grid_dependents_go();
     float sigma[2] = {1.f, 1.f}, back[2] = {1.f, 1.f};         // of columns col and col + 8, and one over it
-    unsigned sh[STEPS][4], sl[STEPS][4];
-#pragma unroll
-    for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
     const int b_row = (lane & 7) + 8 * (lane >> 4), b_col = 8 * ((lane >> 3) & 1);      // ldmatrix, operand stored [n][k]
     const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);    // ... and [k][n]
-    // two warps per 16 columns: each finishes the outputs of eight of the chunk's tokens
-    constexpr int FINISH = SLICES > 1 ? 1 : 2;                 // tiles of eight tokens that a warp finishes
-    const int tile0 = SLICES > 1 ? slice : 0;
-    float* out = p.out + (size_t)t0 * p.heads * p.vdim + (size_t)head * p.vdim + col;
     const size_t width = (size_t)p.heads * p.vdim;
     const int left = p.vdim - col;                             // columns col and col + 8 are there
+    const bool whole = col0 + group * 16 + 16 <= p.vdim;       // all of the warp's columns are there
+    float* out = p.out + (size_t)t0 * width + (size_t)head * p.vdim + col;      // the first token of the chunk that is written next
+    // Two warps per 16 columns: the first finishes the outputs of token tiles 0 and 3, the second of 1 and 2 (tiles 2 and 3 have
+    // two blocks of weights).  One warp: all four.
+    auto tile_of = [&](int j) { return SLICES > 1 ? (j == 0 ? slice : 3 - slice) : j; };
+    // outputs of the last chunk, without the other warp's S0^T q, and the factors on those
+    float kept[FINISH][4], factor_kept[FINISH][4];
+    auto write = [&](const float (&o)[4], int tile, int tokens) {
+        const int token = 8 * tile + 2 * t;
+        float* to = out + (size_t)token * width;
+        if (whole && tokens >= DC_TOKENS) {
+            to[0] = o[0]; to[8] = o[2]; to[width] = o[1]; to[width + 8] = o[3];
+        } else {
+            if (token < tokens && left > 0) to[0] = o[0];
+            if (token < tokens && left > 8) to[8] = o[2];
+            if (token + 1 < tokens && left > 0) to[width] = o[1];
+            if (token + 1 < tokens && left > 8) to[width + 8] = o[3];
+        }
+    };
+    auto finish = [&](const float4 (&x)[FINISH], int tokens) {
+#pragma unroll
+        for (int j = 0; j < FINISH; ++j) {
+            float o[4];
+            dc_fma2(o[0], o[1], factor_kept[j][0], factor_kept[j][1], x[j].x, x[j].y, kept[j][0], kept[j][1]);
+            dc_fma2(o[2], o[3], factor_kept[j][2], factor_kept[j][3], x[j].z, x[j].w, kept[j][2], kept[j][3]);
+            write(o, tile_of(j), tokens);
+        }
+        out += DC_TOKENS * width;
+    };
     // Operands of the next products are read well ahead of them, and sums that do not depend on one another are asked for
     // together: a warp has its scheduler nearly to itself, so what one instruction waits for, all wait for.
-    unsigned bk[STEPS][4];                                     // K of the chunk (the first part), operand of S0^T k
-    DcValues<T> v;                                             // its v, laid out as a tile of U
-    auto ask = [&](const typename Sh::Stage& st) {
+    unsigned bk[2][2][4];                                      // K, operand of S0^T k, 16 rows of S and two times 16 tokens each; two in turn
+    DcValues<T> v;                                             // the chunk's v, laid out as a tile of U
+    auto ask_keys = [&](const typename Sh::Stage& st, int k) {
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) dc_ldmatrix(bk[k], &st.keys.k[0][b_row][row0 + 16 * k + b_col]);
+        for (int m = 0; m < 2; ++m) dc_ldmatrix(bk[k & 1][m], &st.keys.k[0][16 * m + b_row][row0 + 16 * k + b_col]);
+    };
+    auto ask = [&](const typename Sh::Stage& st) {
+        ask_keys(st, 0);
         if constexpr (sizeof(T) == 2) {                        // tokens 0-7 of col, col + 8; tokens 8-15 of both
-            dc_ldmatrix_trans(v.x, &st.v[(lane & 7) + 8 * (lane >> 4)][group * 16 + 8 * ((lane >> 3) & 1)]);
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                unsigned x[4];
+                dc_ldmatrix_trans(x, &st.v[16 * m + b_row][group * 16 + b_col]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v.x[4 * m + e] = x[e];
+            }
         } else {
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v.x[4 * j + e] = st.v[8 * j + 2 * t + (e & 1)][group * 16 + g + 8 * (e >> 1)];
         }
@@ -652,14 +790,36 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 
     for (int c = 0; c < chunks; ++c) {
         const auto& st = sm.stage[c % DC_STAGES];
-        const int here = count - c * DC_TOKENS;                // tokens from the chunk's first on
         bool look = c % DC_REFRESH == 0, spoiled = false;
         int bad[2] = {DC_TOKENS, DC_TOKENS};
-        float u[2][4], wq[FINISH][4];
-        unsigned kt[STEPS][4];                                 // K again, operand of the new state
+        float u[DC_TILES][4], wq[DC_TILES][4];                 // U, S0^T q
+        unsigned bq[2][4];                                     // Q
+        unsigned sh[STEPS][4], sl[STEPS][4];                   // the state in two parts
+        float4 late[FINISH];                                   // the other warp's S0^T q of the last chunk
+        auto ask_query = [&](int k) {
+#pragma unroll
+            for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][16 * m + b_row][row0 + 16 * k + b_col]);
+        };
+        // a quarter of the instructions of S0^T q: they stand where the chain of R, U and the new state has to wait
+        auto query_step = [&](int k) {
+#pragma unroll
+            for (int j = 0; j < DC_TILES; ++j) dc_mma(wq[j], sl[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+            if (PARTS == 2) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    unsigned b[4];
+                    dc_ldmatrix(b, &st.keys.q[PARTS - 1][16 * m + b_row][row0 + 16 * k + b_col]);
+                    dc_mma(wq[2 * m], sh[k], b[0], b[1]);
+                    dc_mma(wq[2 * m + 1], sh[k], b[2], b[3]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < DC_TILES; ++j) dc_mma(wq[j], sh[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+            if (k + 1 < STEPS) ask_query(k + 1);
+        };
         for (int tries = 0;; ++tries) {
-            if (look) {                                        // the columns' powers of two from the columns themselves
-                float most[2], raw[2][4];
+            if (__builtin_expect(look, 0)) {                   // the columns' powers of two from the columns themselves
+                float most[2], raw[DC_TILES][4];
                 v.widen(raw);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -668,7 +828,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                     for (int n = 0; n < TILES; ++n) most[h] = fmaxf(most[h], fmaxf(fabsf(s[n][2 * h]), fabsf(s[n][2 * h + 1])));
                     most[h] *= back[h];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
                         for (int e = 2 * h; e < 2 * h + 2; ++e)        // (an infinite value must not move its column's power)
                             if (fabsf(raw[j][e]) < INFINITY) most[h] = fmaxf(most[h], fabsf(raw[j][e]));
@@ -691,196 +851,217 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                     for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= factor; s[n][2 * h + 1] *= factor; }
                 }
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
             }
-            // ---- S0^T k and S0^T q of the warp's rows: 16 columns x 16 tokens
-            unsigned bq[STEPS][4], th[4], tl[4];
-            float wk[2][4], both[2][4];
+            // ---- S0^T k of the warp's rows: 16 columns x 32 tokens; the next rows are taken apart meanwhile
+            float wk[DC_TILES][4], lk[DC_TILES][4];
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) dc_ldmatrix(bq[k], &st.keys.q[0][b_row][row0 + 16 * k + b_col]);
-            dc_state_product<STEPS>(wk, sh, sl, bk);
-            if (PARTS == 2) {
+            for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    dc_ldmatrix(kt[k], &st.keys.k[PARTS - 1][b_row][row0 + 16 * k + b_col]);
+                for (int e = 0; e < 4; ++e) wk[j][e] = lk[j][e] = wq[j][e] = 0.f;
+            dc_split_tiles(s[0], s[1], sh[0], sl[0]);
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) dc_mma(wk[j], sh[k], kt[k][2 * j], kt[k][2 * j + 1]);
+            for (int k = 0; k < STEPS; ++k) {
+                if (k + 1 < STEPS) ask_keys(st, k + 1);
+#pragma unroll
+                for (int j = 0; j < DC_TILES; ++j) {
+                    dc_mma(wk[j], sh[k], bk[k & 1][j >> 1][2 * (j & 1)], bk[k & 1][j >> 1][2 * (j & 1) + 1]);
+                    dc_mma(lk[j], sl[k], bk[k & 1][j >> 1][2 * (j & 1)], bk[k & 1][j >> 1][2 * (j & 1) + 1]);
+                }
+                if (k + 1 < STEPS) dc_split_tiles(s[2 * k + 2], s[2 * k + 3], sh[(k + 1) % STEPS], sl[(k + 1) % STEPS]);
+                if (PARTS == 2) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        unsigned b[4];
+                        dc_ldmatrix(b, &st.keys.k[PARTS - 1][16 * m + b_row][row0 + 16 * k + b_col]);
+                        dc_mma(lk[2 * m], sh[k], b[0], b[1]);
+                        dc_mma(lk[2 * m + 1], sh[k], b[2], b[3]);
+                    }
                 }
             }
-            if (SLICES > 1) {
-                sm.swap[c & 1][warp][0][lane] = make_float4(wk[0][0], wk[0][1], wk[0][2], wk[0][3]);
-                sm.swap[c & 1][warp][1][lane] = make_float4(wk[1][0], wk[1][1], wk[1][2], wk[1][3]);
+            ask_query(0);
+#pragma unroll
+            for (int j = 0; j < DC_TILES; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) dc_add2(wk[j][e], wk[j][e + 1], wk[j][e], wk[j][e + 1], lk[j][e], lk[j][e + 1]);
+                if (SLICES > 1) sm.swap[c & 1][warp][j][lane] = make_float4(wk[j][0], wk[j][1], wk[j][2], wk[j][3]);
             }
-            dc_ldmatrix(th, &st.gates.t[0][b_row][b_col]);
-            dc_ldmatrix(tl, &st.gates.t[1][b_row][b_col]);
-            const float2 before0 = *reinterpret_cast<const float2*>(&st.gates.before[2 * t]);
-            const float2 before1 = *reinterpret_cast<const float2*>(&st.gates.before[8 + 2 * t]);
+            float2 before[DC_TILES];
+#pragma unroll
+            for (int j = 0; j < DC_TILES; ++j) before[j] = *reinterpret_cast<const float2*>(&st.gates.before[8 * j + 2 * t]);
             float size = st.gates.odd[0];                      // NaN where T is not finite
-            dc_state_product<STEPS>(both, sh, sl, bq);
-            if (PARTS == 2) {
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    dc_ldmatrix(kt[k], &st.keys.q[PARTS - 1][b_row][row0 + 16 * k + b_col]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) dc_mma(both[j], sh[k], kt[k][2 * j], kt[k][2 * j + 1]);
-                }
-            }
-            if constexpr (SLICES > 1) {
-                sm.swap[c & 1][warp][2][lane] = make_float4(slice ? both[0][0] : both[1][0], slice ? both[0][1] : both[1][1],
-                                                            slice ? both[0][2] : both[1][2], slice ? both[0][3] : both[1][3]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wq[0][e] = slice ? both[1][e] : both[0][e];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wq[j % FINISH][e] = both[j][e];
-            }
             // ---- one meeting per chunk: the halves' sums are there, and so is the next stage
             if (tries == 0) dc_sync(DC_MEET, Sh::THREADS);
             else if (SLICES > 1) dc_sync(DC_PAIR + group, 64);
-            if (SLICES > 1) {
-                float4 x[2];
+            if constexpr (SLICES > 1) {
+                float4 x[DC_TILES];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) x[j] = sm.swap[c & 1][warp ^ 1][j][lane];
+                for (int j = 0; j < DC_TILES; ++j) x[j] = sm.swap[c & 1][warp ^ 1][j][lane];
+                query_step(0);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < DC_TILES; ++j) {
                     dc_add2(wk[j][0], wk[j][1], wk[j][0], wk[j][1], x[j].x, x[j].y);
                     dc_add2(wk[j][2], wk[j][3], wk[j][2], wk[j][3], x[j].z, x[j].w);
                 }
+            } else {
+                query_step(0);
             }
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
             // ---- R, U
-            float r[2][4];
+            float r[DC_TILES][4];
             v.widen(r);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float2 before = j ? before1 : before0;
+            for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float x, y;
                     dc_mul2(x, y, r[j][2 * h], r[j][2 * h + 1], sigma[h], sigma[h]);
-                    dc_fma2(r[j][2 * h], r[j][2 * h + 1], -before.x, -before.y, wk[j][2 * h], wk[j][2 * h + 1], x, y);
+                    dc_fma2(r[j][2 * h], r[j][2 * h + 1], -before[j].x, -before[j].y, wk[j][2 * h], wk[j][2 * h + 1], x, y);
                     asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(size) : "f"(fabsf(r[j][2 * h])), "f"(fabsf(r[j][2 * h + 1])));
                 }
+            unsigned rh[2][4], rl[2][4], th[3][4], tl[3][4];
+#pragma unroll
+            for (int b = 0; b < 3; ++b) {
+                dc_ldmatrix(th[b], &st.gates.t[0][b][b_row][b_col]);
+                dc_ldmatrix(tl[b], &st.gates.t[1][b][b_row][b_col]);
             }
-            unsigned rh[4], rl[4];
-            dc_split_tiles(r[0], r[1], rh, rl);
+            dc_split_tiles(r[0], r[1], rh[0], rl[0]);
+            query_step(1);
+            dc_split_tiles(r[2], r[3], rh[1], rl[1]);
             dc_solve(u, rh, rl, th, tl);
-            if (!__any_sync(0xffffffffu, !(size < DC_MOST))) break;
-            if (tries == 0) {                                  // (both warps of a pair have the same R and T)
+            if (__builtin_expect(!__any_sync(0xffffffffu, !(size < DC_MOST)), 1)) break;
+            if (tries == 0) {                                  // (both warps of 16 columns have the same R and T)
                 look = true;
-                ask(st);
+                ask_keys(st, 0);
                 continue;
             }
             // not a matter of size: something is not finite
             spoiled = true;
             dc_first_bad(r, t, bad);
             dc_leave_out(r, t, bad);
-            dc_split_tiles(r[0], r[1], rh, rl);
+            dc_split_tiles(r[0], r[1], rh[0], rl[0]);
+            dc_split_tiles(r[2], r[3], rh[1], rl[1]);
             dc_solve(u, rh, rl, th, tl);
             dc_first_bad(u, t, bad);
             dc_leave_out(u, t, bad);
             break;
         }
         // ---- the new state
-        unsigned uh[4], ul[4], zh[4], zl[4];
-        const float2 after0 = *reinterpret_cast<const float2*>(&st.gates.after[2 * t]);
-        const float2 after1 = *reinterpret_cast<const float2*>(&st.gates.after[8 + 2 * t]);
         const float decay = st.gates.fade[DC_TOKENS - 1];
-        float faded[2][4];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float2 after = j ? after1 : after0;
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) dc_mul2(faded[j][e], faded[j][e + 1], u[j][e], u[j][e + 1], after.x, after.y);
-        }
-        dc_split_tiles(faded[0], faded[1], uh, ul);
+        unsigned uh[2][4], ul[2][4], zh[2][4], zl[2][4], kt[STEPS][4];
         float add[TILES][4];
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) {
+        for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            float faded[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float2 after = *reinterpret_cast<const float2*>(&st.gates.after[16 * m + 8 * j + 2 * t]);
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    dc_mul2(faded[j][e], faded[j][e + 1], u[2 * m + j][e], u[2 * m + j][e + 1], after.x, after.y);
+            }
+            dc_split_tiles(faded[0], faded[1], uh[m], ul[m]);
+        }
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) add[n][e] = 0.f;
-            dc_mma(add[n], ul, kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
-        }
-        if (PARTS == 2) {
 #pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-                unsigned b[4];
-                dc_ldmatrix_trans(b, &st.keys.k[PARTS - 1][bt_row][row0 + 16 * k + bt_col]);
-                dc_mma(add[2 * k], uh, b[0], b[1]);
-                dc_mma(add[2 * k + 1], uh, b[2], b[3]);
+        for (int m = 0; m < 2; ++m) {                          // tokens 16 m on
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) dc_mma(add[n], ul[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+            if (PARTS == 2) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    unsigned b[4];
+                    dc_ldmatrix_trans(b, &st.keys.k[PARTS - 1][16 * m + bt_row][row0 + 16 * k + bt_col]);
+                    dc_mma(add[2 * k], uh[m], b[0], b[1]);
+                    dc_mma(add[2 * k + 1], uh[m], b[2], b[3]);
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) dc_mma(add[n], uh[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+            dc_split_tiles(u[2 * m], u[2 * m + 1], zh[m], zl[m]);
+            if (m == 0) {
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][16 + bt_row][row0 + 16 * k + bt_col]);
+                query_step(2);
+            }
+        }
+        query_step(3);
+        if (c + 1 < chunks) ask(sm.stage[(c + 1) % DC_STAGES]);
+#pragma unroll
+        for (int n = 0; n < TILES; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2)
+                dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
+        // ---- outputs: the chunk's start and its own tokens.  What the other warp has of S0^T q comes with the next meeting: the
+        // chunk before, which was a full one, is finished first
+        if constexpr (SLICES > 1) {
+            if (c > 0) {
+#pragma unroll
+                for (int j = 0; j < FINISH; ++j) late[j] = sm.swap[(c - 1) & 1][warp ^ 1][Sh::SWAPS - FINISH + j][lane];
+                finish(late, DC_TOKENS);
+            }
+#pragma unroll
+            for (int j = 0; j < FINISH; ++j) {                 // the other warp's tiles
+                const float(&x)[4] = j == 0 ? wq[0] : wq[3], (&y)[4] = j == 0 ? wq[1] : wq[2];
+                sm.swap[c & 1][warp][Sh::SWAPS - FINISH + j][lane] =
+                    make_float4(slice ? x[0] : y[0], slice ? x[1] : y[1], slice ? x[2] : y[2], slice ? x[3] : y[3]);
             }
         }
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) dc_mma(add[n], uh, kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
-        dc_split_tiles(u[0], u[1], zh, zl);
-        unsigned ph[4], pl[4];
-        if constexpr (SLICES > 1) {                            // the eight tokens' rows: both inner halves, both parts
-            dc_ldmatrix(ph, &st.gates.p[lane >> 4][8 * slice + (lane & 7)][b_col]);
-            pl[0] = ph[2]; pl[1] = ph[3];
-        } else {
-            dc_ldmatrix(ph, &st.gates.p[0][b_row][b_col]);
-            dc_ldmatrix(pl, &st.gates.p[1][b_row][b_col]);
-        }
-        if (SLICES > 1) {
-            const float4 x = sm.swap[c & 1][warp ^ 1][2][lane];
-            dc_add2(wq[0][0], wq[0][1], wq[0][0], wq[0][1], x.x, x.y);
-            dc_add2(wq[0][2], wq[0][3], wq[0][2], wq[0][3], x.z, x.w);
-        }
-        float oa[FINISH][4], ob[FINISH][4];
-#pragma unroll
         for (int j = 0; j < FINISH; ++j) {
+            const int tile = tile_of(j);
+            const bool second = SLICES > 1 ? j == 1 : j >= 2;  // the tile's tokens are in the chunk's second half
+            float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) oa[j][e] = ob[j][e] = 0.f;
-            dc_mma(ob[j], zl, ph[2 * j], ph[2 * j + 1]);
-            dc_mma(oa[j], zh, ph[2 * j], ph[2 * j + 1]);
-            dc_mma(ob[j], zh, pl[2 * j], pl[2 * j + 1]);
-        }
-        if (c + 1 < chunks) ask(sm.stage[(c + 1) % DC_STAGES]);
+            for (int m = 0; m <= (second ? 1 : 0); ++m) {
+                unsigned w[4];                                 // high and low part, two inner halves each
+                dc_ldmatrix(w, &st.gates.p[lane >> 4][second ? 1 + m : 0][8 * (tile & 1) + (lane & 7)][b_col]);
+                dc_mma(b, zl[m], w[0], w[1]);
+                dc_mma(a, zh[m], w[0], w[1]);
+                dc_mma(b, zh[m], w[2], w[3]);
+            }
+            float mine[4];
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) {
-#pragma unroll
-            for (int n = 2 * k; n < 2 * k + 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
-            dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
-        }
-        // ---- outputs: the chunk's start and its own tokens
-#pragma unroll
-        for (int j = 0; j < FINISH; ++j) {
-            const int first = 8 * (tile0 + j) + 2 * t;
+            for (int e = 0; e < 4; ++e)
+                mine[e] = SLICES == 1 ? wq[j][e] : j == 0 ? (slice ? wq[1][e] : wq[0][e]) : (slice ? wq[2][e] : wq[3][e]);
+            const int first = 8 * tile + 2 * t;
             const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[first]);
             const float2 query = *reinterpret_cast<const float2*>(&st.gates.query[first]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float x, y, fx, fy;
-                dc_add2(x, y, oa[j][2 * h], oa[j][2 * h + 1], ob[j][2 * h], ob[j][2 * h + 1]);
-                dc_fma2(x, y, fade.x, fade.y, wq[j][2 * h], wq[j][2 * h + 1], x, y);
+                dc_add2(x, y, a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]);
+                dc_fma2(x, y, fade.x, fade.y, mine[2 * h], mine[2 * h + 1], x, y);
                 dc_mul2(fx, fy, query.x, query.y, back[h], back[h]);
                 dc_mul2(x, y, x, y, fx, fy);
-                if (spoiled) {
+                if (__builtin_expect(spoiled, 0)) {
                     if (first >= bad[h]) x = __int_as_float(0x7fffffff);
                     if (first + 1 >= bad[h]) y = __int_as_float(0x7fffffff);
                 }
-                if (first < here && 8 * h < left) out[(size_t)first * width + 8 * h] = x;
-                if (first + 1 < here && 8 * h < left) out[(size_t)(first + 1) * width + 8 * h] = y;
+                kept[j][2 * h] = x; kept[j][2 * h + 1] = y;
+                dc_mul2(factor_kept[j][2 * h], factor_kept[j][2 * h + 1], fx, fy, fade.x, fade.y);
             }
+            if (SLICES == 1) write(kept[j], tile, count - c * DC_TOKENS);
         }
-        out += (size_t)DC_TOKENS * width;
-        if (spoiled) {
+        if (SLICES == 1) out += DC_TOKENS * width;
+        if (__builtin_expect(spoiled, 0)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 if (bad[h] < DC_TOKENS) {
 #pragma unroll
                     for (int n = 0; n < TILES; ++n) s[n][2 * h] = s[n][2 * h + 1] = __int_as_float(0x7fffffff);
                 }
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) dc_split_tiles(s[2 * k], s[2 * k + 1], sh[k], sl[k]);
         }
+    }
+    dc_sync(DC_MEET, Sh::THREADS);
+    if constexpr (SLICES > 1) {
+        float4 late[FINISH];
+#pragma unroll
+        for (int j = 0; j < FINISH; ++j) late[j] = sm.swap[(chunks - 1) & 1][warp ^ 1][Sh::SWAPS - FINISH + j][lane];
+        finish(late, count - (chunks - 1) * DC_TOKENS);
     }
 #pragma unroll
     for (int n = 0; n < TILES; ++n)
@@ -891,41 +1072,42 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
 }
 
-constexpr int DC_ALONE_BYTES = 120 * 1024;     // more than half of an SM's shared memory
+// An SM for each block: asks for more than half of the SM's shared memory.
+constexpr int DC_ALONE_BYTES = 180 * 1024;
 static_assert(sizeof(DcShape<float, 128>::Shared) <= DC_ALONE_BYTES, "the largest shape");
 
 template <typename T, int DK, bool WIDE>
 static int launch_chunk(const DeltaParams& p, const DcRecords& records, int early, cudaStream_t stream) {
     using Sh = DcShape<T, DK>;
-    auto kernel = delta_walk_kernel<T, DK, WIDE>;
-    static int sms = 0;                        // per process and kernel; harmless if repeated
+    auto maker = delta_records_kernel<T, DK, WIDE>;
+    auto walker = delta_walk_kernel<T, DK, WIDE>;
+    static int sms = 0;                        // per process and kernels; harmless if repeated
     if (sms == 0) {
         int device = 0, count = 0;
         cudaError_t e = cudaGetDevice(&device);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_ALONE_BYTES);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(maker, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DcMaker<T, DK>));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(walker, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_ALONE_BYTES);
         if (e != cudaSuccess) return (int)e;
         sms = count;
     }
     const long long units = (long long)records.chunks * (p.heads / p.share);
     const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.items);
-    if (grid.y > 65535 || grid.z > 65535 || units > 0x7fffffffLL) return ERR_UNSUPPORTED;
-    const int rc = launch_dependent_if(early, delta_records_kernel<T, DK, WIDE>, dim3((unsigned)((units + DC_MAKERS - 1) / DC_MAKERS)),
-                                       dim3(32 * DC_MAKERS), 0, stream, p, records);
+    if (units > 0x7fffffffLL || grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
+    const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32), sizeof(DcMaker<T, DK>), stream, p, records);
     if (rc != 0) return rc;
-    // Two blocks on an SM take 2,200 cycles for a chunk of each, one alone 1,530: as many blocks as SMs had better not share any,
-    // which they do if they start while the records' blocks still hold some (ask for more than half of the shared memory).
-    const size_t smem = (long long)grid.x * grid.y * grid.z <= sms ? DC_ALONE_BYTES : sizeof(typename Sh::Shared);
-    // the state is older than the records' kernel, which waits for whatever may have written it
-    return launch_dependent(kernel, grid, dim3(Sh::THREADS), smem, stream, p, records);
+    // As many blocks as SMs had better not share any (DC_ALONE), which they do if they start while the records' blocks still
+    // hold some.  The state is older than the records' kernel, which waits for whatever may have written it.
+    const bool alone = (long long)grid.x * grid.y * grid.z <= sms;
+    return launch_dependent(walker, grid, dim3(Sh::THREADS), alone ? (size_t)DC_ALONE_BYTES : sizeof(typename Sh::Shared), stream, p,
+                            records);
 }
 
 template <typename T, int DK>
 static int launch_chunk_any(const DeltaParams& p, int items, long long chunks, unsigned char* room, int early, cudaStream_t stream) {
-    using Sh = DcShape<T, DK>;
     DcRecords records;
     records.keys = room;
-    records.gates = room + (size_t)chunks * (p.heads / p.share) * sizeof(typename Sh::Keys);
+    records.gates = room + (size_t)chunks * (p.heads / p.share) * sizeof(typename DcRecord<T, DK>::Keys);
     records.items = items;
     records.chunks = (int)chunks;
     const bool wide = p.ld % 8 == 0 && p.q_off % 8 == 0 && p.k_off % 8 == 0 && p.v_off % 8 == 0 && p.dim % 8 == 0 &&
@@ -934,9 +1116,9 @@ static int launch_chunk_any(const DeltaParams& p, int items, long long chunks, u
 }
 
 static long long chunk_bytes(int heads, int share, int dim, int dtype) {
-    const long long gates = (long long)heads * sizeof(DcShape<bf16, 64>::Gates), narrow = heads / share;
-    if (dtype == DTYPE_F32) return gates + narrow * (dim <= 64 ? sizeof(DcShape<float, 64>::Keys) : sizeof(DcShape<float, 128>::Keys));
-    return gates + narrow * (dim <= 64 ? sizeof(DcShape<bf16, 64>::Keys) : sizeof(DcShape<bf16, 128>::Keys));
+    const long long gates = (long long)heads * sizeof(DcRecord<bf16, 64>::Gates), narrow = heads / share;
+    if (dtype == DTYPE_F32) return gates + narrow * (dim <= 64 ? sizeof(DcRecord<float, 64>::Keys) : sizeof(DcRecord<float, 128>::Keys));
+    return gates + narrow * (dim <= 64 ? sizeof(DcRecord<bf16, 64>::Keys) : sizeof(DcRecord<bf16, 128>::Keys));
 }
 
 // The chunked form; ERR_UNSUPPORTED where a head has more rows than it holds.  `room`: 16-byte aligned memory.
