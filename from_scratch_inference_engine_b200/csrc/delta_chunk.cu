@@ -232,7 +232,7 @@ __device__ __forceinline__ void dc_product(float (&sum)[2][4], const unsigned (&
 }
 
 template <typename T, int DK>
-struct DcMaker {                           // a preparing warp's shared memory: the records as they go out, and scratch
+struct DcMaker {                           // a preparing block's shared memory: the records as they go out, and scratch
     typename DcRecord<T, DK>::Keys keys;
     typename DcRecord<T, DK>::Gates gates;
     float a[2][16][16 + 4];                // A's blocks on the diagonal
@@ -246,15 +246,19 @@ __device__ __forceinline__ void dc_copy_out(void* to, const void* from, int byte
     asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
 }
 
-// a block of one warp per chunk and q/k head
+// A block of four warps per chunk and q/k head: they take eight tokens' q and k each, then three of them one block of the
+// products and weights each, the fourth the gates' sums.  (One warp for all of it held as much shared memory and left seven warps
+// on an SM: 60 us for 8,192 tokens of 16 q/k and 32 heads.)
+constexpr int DC_MAKERS = 4;
+
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(32)
+__global__ void __launch_bounds__(32 * DC_MAKERS, sizeof(T) == 2 ? 6 : 4)
 delta_records_kernel(const DeltaParams p, const DcRecords records) {
     using Sh = DcRecord<T, DK>;
     constexpr int PARTS = Sh::PARTS, FOURS = DK / 32;          // 32 columns are a quad's eight each
     extern __shared__ __align__(16) unsigned char dc_raw[];
     auto& own = *reinterpret_cast<DcMaker<T, DK>*>(dc_raw);
-    const int lane = threadIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int narrow_heads = p.heads / p.share;
     const int chunk = blockIdx.x / narrow_heads, narrow = blockIdx.x - chunk * narrow_heads;
@@ -281,198 +285,164 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
     grid_dependency_wait();
     grid_dependents_go();
     if (slot < 0 || chunk >= records.chunks) return;           // beyond the step's chunks, or a padding entry
-    const T* qkv = (const T*)p.qkv;
     float decay = 0.f, beta = 0.f;                             // of the lane's token, the first head's
-    if (lane < n) {
+    if (warp == 3 && lane < n) {
         decay = p.log_decay[(size_t)(first + lane) * p.heads + narrow * p.share];
         beta = p.beta[(size_t)(first + lane) * p.heads + narrow * p.share];
     }
-    // ---- q and k: their lengths, a power of two that brings each below one, both in half precision.  16 tokens at a time, a
-    // quad per token; in bfloat16 all loads go out first
-    constexpr int PAIRS = sizeof(T) == 2 ? 2 : 1;              // of 16 tokens that are held at once
-    Raw8<T> kr[PAIRS][2][FOURS], qr[PAIRS][2][FOURS];
-    auto load = [&](int m, Raw8<T> (&k)[2][FOURS], Raw8<T> (&q)[2][FOURS]) {
+    // ---- q and k, a quad per token: their lengths, a power of two that brings each below one, both in half precision
+    {
+        const int r = 8 * warp + g;
+        const T* row = (const T*)p.qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + narrow * p.dim;
+        Raw8<T> raw[2][FOURS];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = 16 * m + g + 8 * h;
-            const T* row = qkv + (size_t)(first + (r < n ? r : 0)) * p.ld + narrow * p.dim;
+        for (int f = 0; f < FOURS; ++f) {
+            const int d = f * 32 + t * 8, have = r < n ? p.dim - d : 0;
+            raw[0][f] = dc_load8<WIDE>(row + p.k_off + d, have);
+            raw[1][f] = dc_load8<WIDE>(row + p.q_off + d, have);
+        }
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __half* to = which ? own.keys.q[0][r] : own.keys.k[0][r];          // the second part's row comes DC_TOKENS later
+            float sum = 0.f, x[8];
 #pragma unroll
             for (int f = 0; f < FOURS; ++f) {
-                const int d = f * 32 + t * 8, have = r < n ? p.dim - d : 0;
-                k[h][f] = dc_load8<WIDE>(row + p.k_off + d, have);
-                q[h][f] = dc_load8<WIDE>(row + p.q_off + d, have);
+                dc_widen(raw[which][f], x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
             }
-        }
-    };
-    // one of q and k of one token: into `to` (PARTS rows `part_step` apart), returns the scaled number's way back to a unit length
-    auto bring = [&](const Raw8<T> (&raw)[FOURS], __half* to) {
-        float sum = 0.f, x[8];
 #pragma unroll
-        for (int f = 0; f < FOURS; ++f) {
-            dc_widen(raw[f], x);
+            for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int e = (((__float_as_int(sum) >> 23) & 255) - 125) >> 1;
+            const float scale = dc_power(-e);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-        }
+            for (int f = 0; f < FOURS; ++f) {
+                dc_widen(raw[which][f], x);
+                unsigned high[4], low[4];
 #pragma unroll
-        for (int o = 1; o < 4; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const int e = (((__float_as_int(sum) >> 23) & 255) - 125) >> 1;
-        const float scale = dc_power(-e);
-#pragma unroll
-        for (int f = 0; f < FOURS; ++f) {
-            dc_widen(raw[f], x);
-            unsigned high[4], low[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (PARTS == 2) dc_split(x[2 * i] * scale, x[2 * i + 1] * scale, high[i], low[i]);
-                else high[i] = dc_bits(__floats2half2_rn(x[2 * i] * scale, x[2 * i + 1] * scale));
+                for (int i = 0; i < 4; ++i) {
+                    if (PARTS == 2) dc_split(x[2 * i] * scale, x[2 * i + 1] * scale, high[i], low[i]);
+                    else high[i] = dc_bits(__floats2half2_rn(x[2 * i] * scale, x[2 * i + 1] * scale));
+                }
+                *reinterpret_cast<uint4*>(to + f * 32 + t * 8) = make_uint4(high[0], high[1], high[2], high[3]);
+                if (PARTS == 2)
+                    *reinterpret_cast<uint4*>(to + DC_TOKENS * Sh::KLD + f * 32 + t * 8) = make_uint4(low[0], low[1], low[2], low[3]);
             }
-            *reinterpret_cast<uint4*>(to + f * 32 + t * 8) = make_uint4(high[0], high[1], high[2], high[3]);
-            if (PARTS == 2)
-                *reinterpret_cast<uint4*>(to + DC_TOKENS * Sh::KLD + f * 32 + t * 8) = make_uint4(low[0], low[1], low[2], low[3]);
-        }
-        return dc_power(e) / sqrtf(sum + p.eps);
-    };
-    auto bring_all = [&](int m, const Raw8<T> (&k)[2][FOURS], const Raw8<T> (&q)[2][FOURS]) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = 16 * m + g + 8 * h;
-            const float kf = bring(k[h], own.keys.k[0][r]), qf = bring(q[h], own.keys.q[0][r]);
-            if (t == 0) { own.kf[r] = kf; own.qf[r] = p.scale * qf; }
-        }
-    };
-    if constexpr (PAIRS == 2) {
-        load(0, kr[0], qr[0]);
-        load(1, kr[PAIRS - 1], qr[PAIRS - 1]);
-        bring_all(0, kr[0], qr[0]);
-        bring_all(1, kr[PAIRS - 1], qr[PAIRS - 1]);
-    } else {
-#pragma unroll 1
-        for (int m = 0; m < 2; ++m) {
-            load(m, kr[0], qr[0]);
-            bring_all(m, kr[0], qr[0]);
+            if (t == 0) (which ? own.qf : own.kf)[r] = (which ? p.scale : 1.f) * (dc_power(e) / sqrtf(sum + p.eps));
         }
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // generic writes before async-proxy reads
-    __syncwarp();
-    if (lane == 0)
+    __syncthreads();
+    if (threadIdx.x == 96)
         dc_copy_out(records.keys + ((size_t)chunk * narrow_heads + narrow) * sizeof(typename Sh::Keys), &own.keys, sizeof(typename Sh::Keys));
-    // ---- K K^T and Q K^T, blocks (0, 0), (1, 0) and (1, 1)
-    float kkt[3][2][4], qkt[3][2][4];
+    // ---- K K^T and Q K^T: warp 0 block (0, 0), warp 1 block (1, 0), warp 2 block (1, 1)
+    const int rows = warp == 0 ? 0 : 16, cols = warp == 2 ? 16 : 0;
+    float kkt[2][4], qkt[2][4];
 #pragma unroll
-    for (int b = 0; b < 3; ++b)
+    for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) kkt[b][j][e] = qkt[b][j][e] = 0.f;
+        for (int e = 0; e < 4; ++e) kkt[j][e] = qkt[j][e] = 0.f;
     const int a_row = lane & 15, a_col = 8 * (lane >> 4);      // ldmatrix, 16-row operand; its registers 0, 2 and 1, 3 are an 8-column one's
-#pragma unroll 2
-    for (int d = 0; d < DK; d += 16) {
+    const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);   // ldmatrix.trans, operand stored [k][n]
+    if (warp < 3) {
+#pragma unroll 4
+        for (int d = 0; d < DK; d += 16) {
 #pragma unroll
-        for (int pb = 0; pb < PARTS; ++pb) {
-            unsigned kb[2][4];
+            for (int pb = 0; pb < PARTS; ++pb) {
+                unsigned kb[4];
+                dc_ldmatrix(kb, &own.keys.k[pb][cols + a_row][d + a_col]);
 #pragma unroll
-            for (int m = 0; m < 2; ++m) dc_ldmatrix(kb[m], &own.keys.k[pb][16 * m + a_row][d + a_col]);
-#pragma unroll
-            for (int pa = 0; pa + pb < PARTS; ++pa) {
-                unsigned ka[2][4], qa[2][4];
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    if (pa == pb) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) ka[m][e] = kb[m][e];
-                    } else {
-                        dc_ldmatrix(ka[m], &own.keys.k[pa][16 * m + a_row][d + a_col]);
-                    }
-                    dc_ldmatrix(qa[m], &own.keys.q[pa][16 * m + a_row][d + a_col]);
-                }
-#pragma unroll
-                for (int b = 0; b < 3; ++b)
+                for (int pa = 0; pa + pb < PARTS; ++pa) {
+                    unsigned ka[4], qa[4];
+                    dc_ldmatrix(ka, &own.keys.k[pa][rows + a_row][d + a_col]);
+                    dc_ldmatrix(qa, &own.keys.q[pa][rows + a_row][d + a_col]);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        dc_mma(kkt[b][j], ka[b > 0], kb[b == 2][j], kb[b == 2][2 + j]);
-                        dc_mma(qkt[b][j], qa[b > 0], kb[b == 2][j], kb[b == 2][2 + j]);
+                        dc_mma(kkt[j], ka, kb[j], kb[2 + j]);
+                        dc_mma(qkt[j], qa, kb[j], kb[2 + j]);
                     }
+                }
             }
         }
     }
-    const float kf = own.kf[lane], qf = own.qf[lane];
-    const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);   // ldmatrix.trans, operand stored [k][n]
     // ---- the gates of every head that reads these q and k
 #pragma unroll 1
     for (int z = 0; z < p.share; ++z) {
         const int head = narrow * p.share + z;
-        // sums of log_decay in 64 bits, so that a difference of two of them is as exact as its own terms
-        double sum = decay < -1e4f ? -1e4 : (double)decay;     // (e^-10000 is zero)
+        if (warp == 3) {
+            // sums of log_decay in 64 bits, so that a difference of two of them is as exact as its own terms
+            double sum = decay < -1e4f ? -1e4 : (double)decay;       // (e^-10000 is zero)
 #pragma unroll
-        for (int o = 1; o < DC_TOKENS; o <<= 1) {
-            const double left = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += left;
+            for (int o = 1; o < DC_TOKENS; o <<= 1) {
+                const double left = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += left;
+            }
+            const double all = __shfl_sync(0xffffffffu, sum, DC_TOKENS - 1);
+            const float kf = own.kf[lane], fade = expf((float)sum);
+            own.g[lane] = sum;
+            own.beta[lane] = beta;
+            if (z > 0) {                                       // the last head's record has left
+                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+                __syncwarp();
+            }
+            own.gates.before[lane] = fade * kf;
+            own.gates.after[lane] = expf((float)(all - sum)) * kf;
+            own.gates.query[lane] = own.qf[lane];
+            own.gates.fade[lane] = fade;
+            if (z + 1 < p.share && lane < n) {                 // the next head's
+                decay = p.log_decay[(size_t)(first + lane) * p.heads + head + 1];
+                beta = p.beta[(size_t)(first + lane) * p.heads + head + 1];
+            }
         }
-        const double all = __shfl_sync(0xffffffffu, sum, DC_TOKENS - 1);
-        own.g[lane] = sum;
-        own.beta[lane] = beta;
-        if (z > 0) {                                           // the last head's record has left
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
-            __syncwarp();
-        }
-        const float fade = expf((float)sum);
-        own.gates.before[lane] = fade * kf;
-        own.gates.after[lane] = expf((float)(all - sum)) * kf;
-        own.gates.query[lane] = qf;
-        own.gates.fade[lane] = fade;
-        if (z + 1 < p.share && lane < n) {                     // the next head's
-            decay = p.log_decay[(size_t)(first + lane) * p.heads + head + 1];
-            beta = p.beta[(size_t)(first + lane) * p.heads + head + 1];
-        }
-        __syncwarp();
-        float below[2][4];                                     // block (1, 0) of A without beta
-#pragma unroll
-        for (int b = 0; b < 3; ++b)
+        __syncthreads();
+        float below[2][4];                                     // warp 1: block (1, 0) of A without beta
+        if (warp < 3) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int bc = 8 * j + 2 * t, col = 16 * (b == 2) + bc;
+                const int bc = 8 * j + 2 * t, col = cols + bc;
                 const double g0 = own.g[col], g1 = own.g[col + 1];
                 const float f0 = own.kf[col], f1 = own.kf[col + 1];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int br = g + 8 * h, row = 16 * (b > 0) + br;
+                    const int br = g + 8 * h, row = rows + br;
                     const double gr = own.g[row];
                     const float e0 = expf((float)(gr - g0)) * f0, e1 = expf((float)(gr - g1)) * f1;
                     unsigned high, low;
-                    dc_split(row >= col ? qkt[b][j][2 * h] * e0 : 0.f, row > col ? qkt[b][j][2 * h + 1] * e1 : 0.f, high, low);
-                    *reinterpret_cast<unsigned*>(&own.gates.p[0][b][br][bc]) = high;
-                    *reinterpret_cast<unsigned*>(&own.gates.p[1][b][br][bc]) = low;
-                    const float x = own.kf[row] * kkt[b][j][2 * h] * e0, y = own.kf[row] * kkt[b][j][2 * h + 1] * e1;
-                    if (b == 1) {
-                        below[j][2 * h] = x; below[j][2 * h + 1] = y;
-                    } else {
-                        own.a[b / 2][br][bc] = row > col ? own.beta[row] * x : 0.f;
-                        own.a[b / 2][br][bc + 1] = row > col + 1 ? own.beta[row] * y : 0.f;
+                    dc_split(row >= col ? qkt[j][2 * h] * e0 : 0.f, row > col ? qkt[j][2 * h + 1] * e1 : 0.f, high, low);
+                    *reinterpret_cast<unsigned*>(&own.gates.p[0][warp][br][bc]) = high;
+                    *reinterpret_cast<unsigned*>(&own.gates.p[1][warp][br][bc]) = low;
+                    const float x = own.kf[row] * kkt[j][2 * h] * e0, y = own.kf[row] * kkt[j][2 * h + 1] * e1;
+                    below[j][2 * h] = x; below[j][2 * h + 1] = y;
+                    if (warp != 1) {
+                        // (one that is not finite is left out: its token's R or beta is not finite either, and T has that)
+                        const float bx = own.beta[row] * x, by = own.beta[row] * y;
+                        own.a[warp / 2][br][bc] = row > col && fabsf(bx) < INFINITY ? bx : 0.f;
+                        own.a[warp / 2][br][bc + 1] = row > col + 1 && fabsf(by) < INFINITY ? by : 0.f;
                     }
                 }
             }
-        __syncwarp();
-        // blocks (0, 0) and (1, 1) of T: row i of (I + A)^-1 in a lane, from x (I + A) = e_i, last column first
-        const int i = lane & 15, m = lane >> 4;
-        float x[16];
+        }
+        __syncthreads();
+        if (warp == 0) {
+            // blocks (0, 0) and (1, 1) of T: row i of (I + A)^-1 in a lane, from x (I + A) = e_i, last column first
+            const int i = lane & 15, m = lane >> 4;
+            float x[16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = i == j ? 1.f : 0.f;
+            for (int j = 0; j < 16; ++j) x[j] = i == j ? 1.f : 0.f;
 #pragma unroll
-        for (int l = 15; l >= 1; --l) {
-            if (l <= i) {
+            for (int l = 15; l >= 1; --l) {
+                const float xl = l <= i ? -x[l] : 0.f;
 #pragma unroll
-                for (int j = 0; j < l; ++j) x[j] = fmaf(-x[l], own.a[m][l][j], x[j]);
+                for (int j = 0; j < l; ++j) x[j] = fmaf(xl, own.a[m][l][j], x[j]);
             }
-        }
-        bool finite = true;
+            bool finite = true;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            x[j] = j <= i ? x[j] * own.beta[16 * m + j] : 0.f;
-            finite = finite && fabsf(x[j]) < INFINITY;
-        }
-        const bool odd = !__all_sync(0xffffffffu, finite);
-        if (lane == 0) own.gates.odd[0] = odd ? __int_as_float(0x7fffffff) : 0.f;
-        {
+            for (int j = 0; j < 16; ++j) {
+                x[j] = j <= i ? x[j] * own.beta[16 * m + j] : 0.f;
+                finite = finite && fabsf(x[j]) < INFINITY;
+            }
+            const bool odd = !__all_sync(0xffffffffu, finite);
+            if (lane == 0) own.gates.odd[0] = odd ? __int_as_float(0x7fffffff) : 0.f;
             unsigned high[8], low[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
@@ -483,9 +453,9 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
             to[0] = make_uint4(low[0], low[1], low[2], low[3]);
             to[1] = make_uint4(low[4], low[5], low[6], low[7]);
         }
-        __syncwarp();
-        // block (1, 0): -T_11 (A_10 / beta) T_00, beta being in T_11
-        {
+        __syncthreads();
+        if (warp == 1) {
+            // block (1, 0): -T_11 (A_10 / beta) T_00, beta being in T_11
             unsigned ah[4], al[4], bh[4], bl[4];
             float w[2][4];
 #pragma unroll
@@ -496,17 +466,14 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
             dc_ldmatrix_trans(bh, &own.gates.t[0][0][bt_row][bt_col]);
             dc_ldmatrix_trans(bl, &own.gates.t[1][0][bt_row][bt_col]);
             dc_product(w, ah, al, bh, bl);
-            // a number that is not finite is in T's other blocks too, and must not reach rows above its own
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[j][e] = fabsf(w[j][e]) < INFINITY ? -w[j][e] : 0.f;
+            // (one that is not finite must not reach rows above its own)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    const float x = w[j][2 * h], y = w[j][2 * h + 1];
                     unsigned high, low;
-                    dc_split(w[j][2 * h], w[j][2 * h + 1], high, low);
+                    dc_split(fabsf(x) < INFINITY ? -x : 0.f, fabsf(y) < INFINITY ? -y : 0.f, high, low);
                     *reinterpret_cast<unsigned*>(&own.w[0][g + 8 * h][8 * j + 2 * t]) = high;
                     *reinterpret_cast<unsigned*>(&own.w[1][g + 8 * h][8 * j + 2 * t]) = low;
                 }
@@ -531,11 +498,11 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                 }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0)
+        __syncthreads();
+        if (threadIdx.x == 96)
             dc_copy_out(records.gates + ((size_t)chunk * p.heads + head) * sizeof(typename Sh::Gates), &own.gates, sizeof(typename Sh::Gates));
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+    if (threadIdx.x == 96) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
 }
 
 __device__ __forceinline__ void dc_copy16(void* dst, const void* src, bool there) {
@@ -788,8 +755,8 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     dc_sync(DC_MEET, Sh::THREADS);                             // stage 0 is there
     ask(sm.stage[0]);
 
-    for (int c = 0; c < chunks; ++c) {
-        const auto& st = sm.stage[c % DC_STAGES];
+    for (int c = 0, stage = 0, next = 1; c < chunks; ++c, stage = next, next = next + 1 < DC_STAGES ? next + 1 : 0) {
+        const auto& st = sm.stage[stage];
         bool look = c % DC_REFRESH == 0, spoiled = false;
         int bad[2] = {DC_TOKENS, DC_TOKENS};
         float u[DC_TILES][4], wq[DC_TILES][4];                 // U, S0^T q
@@ -988,8 +955,20 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 query_step(2);
             }
         }
+        unsigned w[FINISH][2][4];                              // weights: high and low part, two inner halves each
+        float2 fade[FINISH], query[FINISH];
+#pragma unroll
+        for (int j = 0; j < FINISH; ++j) {
+            const bool second = SLICES > 1 ? j == 1 : j >= 2;  // the tile's tokens are in the chunk's second half
+#pragma unroll
+            for (int m = 0; m <= (second ? 1 : 0); ++m)
+                dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_col]);
+            fade[j] = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile_of(j) + 2 * t]);
+            query[j] = *reinterpret_cast<const float2*>(&st.gates.query[8 * tile_of(j) + 2 * t]);
+            if (SLICES > 1) late[j] = sm.swap[(c + 1) & 1][warp ^ 1][Sh::SWAPS - FINISH + j][lane];     // (first chunk: not used)
+        }
         query_step(3);
-        if (c + 1 < chunks) ask(sm.stage[(c + 1) % DC_STAGES]);
+        if (c + 1 < chunks) ask(sm.stage[next]);
 #pragma unroll
         for (int n = 0; n < TILES; ++n)
 #pragma unroll
@@ -998,11 +977,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         // ---- outputs: the chunk's start and its own tokens.  What the other warp has of S0^T q comes with the next meeting: the
         // chunk before, which was a full one, is finished first
         if constexpr (SLICES > 1) {
-            if (c > 0) {
-#pragma unroll
-                for (int j = 0; j < FINISH; ++j) late[j] = sm.swap[(c - 1) & 1][warp ^ 1][Sh::SWAPS - FINISH + j][lane];
-                finish(late, DC_TOKENS);
-            }
+            if (c > 0) finish(late, DC_TOKENS);
 #pragma unroll
             for (int j = 0; j < FINISH; ++j) {                 // the other warp's tiles
                 const float(&x)[4] = j == 0 ? wq[0] : wq[3], (&y)[4] = j == 0 ? wq[1] : wq[2];
@@ -1013,36 +988,33 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
             const int tile = tile_of(j);
-            const bool second = SLICES > 1 ? j == 1 : j >= 2;  // the tile's tokens are in the chunk's second half
-            float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
+            const bool second = SLICES > 1 ? j == 1 : j >= 2;
+            float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m <= (second ? 1 : 0); ++m) {
-                unsigned w[4];                                 // high and low part, two inner halves each
-                dc_ldmatrix(w, &st.gates.p[lane >> 4][second ? 1 + m : 0][8 * (tile & 1) + (lane & 7)][b_col]);
-                dc_mma(b, zl[m], w[0], w[1]);
-                dc_mma(a, zh[m], w[0], w[1]);
-                dc_mma(b, zh[m], w[2], w[3]);
+                dc_mma(b, zl[m], w[j][m][0], w[j][m][1]);
+                dc_mma(d, zh[m], w[j][m][2], w[j][m][3]);
+                dc_mma(a, zh[m], w[j][m][0], w[j][m][1]);
             }
             float mine[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 mine[e] = SLICES == 1 ? wq[j][e] : j == 0 ? (slice ? wq[1][e] : wq[0][e]) : (slice ? wq[2][e] : wq[3][e]);
             const int first = 8 * tile + 2 * t;
-            const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[first]);
-            const float2 query = *reinterpret_cast<const float2*>(&st.gates.query[first]);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float x, y, fx, fy;
-                dc_add2(x, y, a[2 * h], a[2 * h + 1], b[2 * h], b[2 * h + 1]);
-                dc_fma2(x, y, fade.x, fade.y, mine[2 * h], mine[2 * h + 1], x, y);
-                dc_mul2(fx, fy, query.x, query.y, back[h], back[h]);
+                dc_add2(x, y, b[2 * h], b[2 * h + 1], d[2 * h], d[2 * h + 1]);
+                dc_add2(x, y, a[2 * h], a[2 * h + 1], x, y);
+                dc_fma2(x, y, fade[j].x, fade[j].y, mine[2 * h], mine[2 * h + 1], x, y);
+                dc_mul2(fx, fy, query[j].x, query[j].y, back[h], back[h]);
                 dc_mul2(x, y, x, y, fx, fy);
                 if (__builtin_expect(spoiled, 0)) {
                     if (first >= bad[h]) x = __int_as_float(0x7fffffff);
                     if (first + 1 >= bad[h]) y = __int_as_float(0x7fffffff);
                 }
                 kept[j][2 * h] = x; kept[j][2 * h + 1] = y;
-                dc_mul2(factor_kept[j][2 * h], factor_kept[j][2 * h + 1], fx, fy, fade.x, fade.y);
+                dc_mul2(factor_kept[j][2 * h], factor_kept[j][2 * h + 1], fx, fy, fade[j].x, fade[j].y);
             }
             if (SLICES == 1) write(kept[j], tile, count - c * DC_TOKENS);
         }
@@ -1094,7 +1066,7 @@ static int launch_chunk(const DeltaParams& p, const DcRecords& records, int earl
     const long long units = (long long)records.chunks * (p.heads / p.share);
     const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.items);
     if (units > 0x7fffffffLL || grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
-    const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32), sizeof(DcMaker<T, DK>), stream, p, records);
+    const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32 * DC_MAKERS), sizeof(DcMaker<T, DK>), stream, p, records);
     if (rc != 0) return rc;
     // As many blocks as SMs had better not share any (DC_ALONE), which they do if they start while the records' blocks still
     // hold some.  The state is older than the records' kernel, which waits for whatever may have written it.
