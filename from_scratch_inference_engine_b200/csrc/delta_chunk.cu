@@ -32,7 +32,7 @@
 // Layout.  A warp of the second kernel owns 16 value columns x 64 rows of S, transposed: S^T is the 16-row operand of S0^T k
 // and S0^T q, the accumulator of S0^T k is (after R) the operand of the next product in the registers where it lies, and the
 // new sums end up where S lies.  Heads of more than 64 rows take two warps per 16 columns, which swap their halves' sums
-// through shared memory: of S0^T k in the chunk's one meeting, of S0^T q in the next chunk's.
+// of S0^T k through shared memory, in the chunk's one meeting; those of S0^T q the fetching warps add up.
 //
 // Values that are not finite: they spoil their column from their token on and nothing else, as in the recurrence - a product
 // with a zero of T would spoil the tokens before.  Such chunks are noticed by R and by a mark in their record, redone with those
@@ -53,7 +53,7 @@ constexpr int DC_SLICE = 64;               // rows of S (columns of k) per warp
 constexpr int DC_MAX_DIM = 128;
 constexpr int DC_REFRESH = 16;             // chunks between two looks at the state's size
 constexpr int DC_SIZE = 3;                 // ... which brings the largest number of a column to 2^3 .. 2^4
-constexpr int DC_TLD = 16 + 8;             // padded rows of a 16 x 16 block: ldmatrix without bank conflicts
+constexpr int DC_TLD = 16 + 8;             // padded rows of a 16 x 16 block in scratch
 // A number of R, times sigma, is below this: right behind a look it is at most 2^4 (1 + sqrt(128)).  A row of T has 32 numbers
 // of at most beta^2 <= 4 (what a token's value still does to a later token's u passes through contractions), so that u, and
 // u with a factor of at most 2, fit half precision.
@@ -167,6 +167,9 @@ __device__ __forceinline__ void dc_store8(float* p, const Raw8<float>& r) {
     *reinterpret_cast<float4*>(p) = r.x; *reinterpret_cast<float4*>(p + 4) = r.y;
 }
 
+// A row of a 16 x 16 block is two pieces of 16 bytes, in the other order in every second four rows: ldmatrix without bank conflicts.
+__device__ __forceinline__ int dc_piece(int row, int piece) { return 8 * (piece ^ ((row >> 2) & 1)); }
+
 // T and the weights of u_j are lower triangular: of their four 16 x 16 blocks those at (0, 0), (1, 0) and (1, 1) are kept.
 template <typename T, int DK>
 struct DcRecord {
@@ -174,7 +177,7 @@ struct DcRecord {
     static constexpr int KLD = DK + 8;                         // padded row of q and k
     struct alignas(16) Keys { __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD]; };
     struct alignas(16) Gates {
-        __half t[2][3][16][DC_TLD], p[2][3][16][DC_TLD];       // T and the weights of u_j, two parts each
+        __half t[2][3][16][16], p[2][3][16][16];               // T and the weights of u_j, two parts each; dc_piece()
         float before[DC_TOKENS];          // on S0^T k: e^(G_i), the key's length, the power of two
         float after[DC_TOKENS];           // on u_j in the new state: e^(G_31 - G_j), ...
         float query[DC_TOKENS];           // on an output: scale, the query's length, the power of two
@@ -188,14 +191,17 @@ struct DcShape : DcRecord<T, DK> {
     static constexpr int SLICES = DK / DC_SLICE;               // warps that share 16 value columns
     static constexpr int GROUPS = DC_WALKERS / SLICES;         // groups of 16 value columns
     static constexpr int COLS = 16 * GROUPS;                   // value columns of a block
-    static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 8);
+    static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 0);         // row of v; bfloat16: v_piece()
+    static constexpr int OLD = COLS + 4;                       // padded row of outputs
     static constexpr int THREADS = 32 * DC_WALKERS + DC_FETCHERS;
     static constexpr int FINISH = SLICES > 1 ? DC_TILES / 2 : DC_TILES;     // tiles of eight tokens whose outputs a warp finishes
-    static constexpr int SWAPS = SLICES > 1 ? DC_TILES + FINISH : 1;        // pieces of 16 bytes that a thread hands over
+    // Place of a row's 16-byte piece of bfloat16 v: in another order in every row, ldmatrix without bank conflicts.
+    static __device__ __forceinline__ int v_piece(int row, int piece) { return piece ^ (COLS == 32 ? (row >> 1) & 3 : row & 7); }
     struct alignas(16) Stage { typename DcRecord<T, DK>::Keys keys; typename DcRecord<T, DK>::Gates gates; T v[DC_TOKENS][VLD]; };
     struct Shared {
         Stage stage[DC_STAGES];
-        float4 swap[2][DC_WALKERS][SWAPS][32];
+        float4 swap[2][SLICES > 1 ? DC_WALKERS : 1][DC_TILES][32];      // S0^T k of a warp's rows
+        float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs, of two warps per 16 columns two summands
         float most[DC_WALKERS][16];
     };
 };
@@ -409,8 +415,8 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                     const float e0 = expf((float)(gr - g0)) * f0, e1 = expf((float)(gr - g1)) * f1;
                     unsigned high, low;
                     dc_split(row >= col ? qkt[j][2 * h] * e0 : 0.f, row > col ? qkt[j][2 * h + 1] * e1 : 0.f, high, low);
-                    *reinterpret_cast<unsigned*>(&own.gates.p[0][warp][br][bc]) = high;
-                    *reinterpret_cast<unsigned*>(&own.gates.p[1][warp][br][bc]) = low;
+                    *reinterpret_cast<unsigned*>(&own.gates.p[0][warp][br][dc_piece(br, j) + 2 * t]) = high;
+                    *reinterpret_cast<unsigned*>(&own.gates.p[1][warp][br][dc_piece(br, j) + 2 * t]) = low;
                     const float x = own.kf[row] * kkt[j][2 * h] * e0, y = own.kf[row] * kkt[j][2 * h + 1] * e1;
                     below[j][2 * h] = x; below[j][2 * h + 1] = y;
                     if (warp != 1) {
@@ -446,12 +452,11 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
             unsigned high[8], low[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
-            uint4* to = reinterpret_cast<uint4*>(&own.gates.t[0][2 * m][i][0]);
-            to[0] = make_uint4(high[0], high[1], high[2], high[3]);
-            to[1] = make_uint4(high[4], high[5], high[6], high[7]);
-            to = reinterpret_cast<uint4*>(&own.gates.t[1][2 * m][i][0]);
-            to[0] = make_uint4(low[0], low[1], low[2], low[3]);
-            to[1] = make_uint4(low[4], low[5], low[6], low[7]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                *reinterpret_cast<uint4*>(&own.gates.t[0][2 * m][i][dc_piece(i, j)]) = make_uint4(high[4 * j], high[4 * j + 1], high[4 * j + 2], high[4 * j + 3]);
+                *reinterpret_cast<uint4*>(&own.gates.t[1][2 * m][i][dc_piece(i, j)]) = make_uint4(low[4 * j], low[4 * j + 1], low[4 * j + 2], low[4 * j + 3]);
+            }
         }
         __syncthreads();
         if (warp == 1) {
@@ -463,8 +468,8 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[j][e] = 0.f;
             dc_split_tiles(below[0], below[1], ah, al);
-            dc_ldmatrix_trans(bh, &own.gates.t[0][0][bt_row][bt_col]);
-            dc_ldmatrix_trans(bl, &own.gates.t[1][0][bt_row][bt_col]);
+            dc_ldmatrix_trans(bh, &own.gates.t[0][0][bt_row][dc_piece(bt_row, lane >> 4)]);
+            dc_ldmatrix_trans(bl, &own.gates.t[1][0][bt_row][dc_piece(bt_row, lane >> 4)]);
             dc_product(w, ah, al, bh, bl);
             // (one that is not finite must not reach rows above its own)
 #pragma unroll
@@ -478,8 +483,8 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                     *reinterpret_cast<unsigned*>(&own.w[1][g + 8 * h][8 * j + 2 * t]) = low;
                 }
             __syncwarp();
-            dc_ldmatrix(ah, &own.gates.t[0][2][a_row][a_col]);
-            dc_ldmatrix(al, &own.gates.t[1][2][a_row][a_col]);
+            dc_ldmatrix(ah, &own.gates.t[0][2][a_row][dc_piece(a_row, lane >> 4)]);
+            dc_ldmatrix(al, &own.gates.t[1][2][a_row][dc_piece(a_row, lane >> 4)]);
             dc_ldmatrix_trans(bh, &own.w[0][bt_row][bt_col]);
             dc_ldmatrix_trans(bl, &own.w[1][bt_row][bt_col]);
 #pragma unroll
@@ -493,8 +498,8 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                 for (int h = 0; h < 2; ++h) {
                     unsigned high, low;
                     dc_split(w[j][2 * h], w[j][2 * h + 1], high, low);
-                    *reinterpret_cast<unsigned*>(&own.gates.t[0][1][g + 8 * h][8 * j + 2 * t]) = high;
-                    *reinterpret_cast<unsigned*>(&own.gates.t[1][1][g + 8 * h][8 * j + 2 * t]) = low;
+                    *reinterpret_cast<unsigned*>(&own.gates.t[0][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = high;
+                    *reinterpret_cast<unsigned*>(&own.gates.t[1][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = low;
                 }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -510,7 +515,7 @@ __device__ __forceinline__ void dc_copy16(void* dst, const void* src, bool there
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dc_smem(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
-enum { DC_MEET = 1, DC_PAIR = 2 };         // named barriers: all warps, and from DC_PAIR on the pairs'
+enum { DC_MEET = 1, DC_GO = 2, DC_PAIR = 3 };        // named barriers; from DC_PAIR on the pairs'
 
 // A fetching thread's share of the copies into the ring, chunk after chunk: the addresses move on by a chunk with every call.
 // (Copied by the walkers themselves a chunk takes them 800 cycles more: their own reads of shared memory queue behind.)
@@ -556,12 +561,12 @@ struct DcFetch {
                 for (int r = 0; r < DC_TOKENS; r += ROWS) {
                     const bool there = r + row < left && have > 0;
                     if (r + row < DC_TOKENS)
-                        dc_copy16(&st.v[r + row][(tid % ACROSS) * PER], v + (there ? (size_t)(r + row) * p.ld : 0), there);
+                        dc_copy16(&st.v[r + row][(sizeof(T) == 2 ? Sh::v_piece(r + row, tid % ACROSS) : tid % ACROSS) * PER], v + (there ? (size_t)(r + row) * p.ld : 0), there);
                 }
             } else {
                 for (int e = tid; e < DC_TOKENS * Sh::COLS; e += DC_FETCHERS) {
                     const int r = e / Sh::COLS, d = e % Sh::COLS;
-                    st.v[r][d] = r < left && d < have ? v[(size_t)r * p.ld + d] : from_float<T>(0.f);
+                    st.v[r][sizeof(T) == 2 ? Sh::v_piece(r, d / 8) * 8 + d % 8 : d] = r < left && d < have ? v[(size_t)r * p.ld + d] : from_float<T>(0.f);
                 }
             }
             keys += keys_step;
@@ -572,6 +577,34 @@ struct DcFetch {
         asm volatile("cp.async.commit_group;\n" ::: "memory");
     }
 };
+
+// The fetching threads also write outputs: `tokens` rows of a chunk's, from `to` on, whole lines side by side.
+template <typename T, int DK>
+__device__ __forceinline__ void dc_write(const float (&from)[DcShape<T, DK>::SLICES][DC_TOKENS][DcShape<T, DK>::OLD], float* to,
+                                         size_t width, int tokens, int columns, bool wide) {
+    using Sh = DcShape<T, DK>;
+    constexpr int FOURS = Sh::COLS / 4, AT_ONCE = DC_FETCHERS / FOURS;
+    const int tid = threadIdx.x - 32 * DC_WALKERS, d = (tid % FOURS) * 4;
+#pragma unroll
+    for (int i = 0; i < DC_TOKENS / AT_ONCE; ++i) {
+        const int r = tid / FOURS + i * AT_ONCE;
+        if (r >= tokens || d >= columns) continue;
+        float4 o = *reinterpret_cast<const float4*>(&from[0][r][d]);
+        if (Sh::SLICES > 1) {
+            const float4 x = *reinterpret_cast<const float4*>(&from[Sh::SLICES - 1][r][d]);
+            o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+        }
+        float* at = to + (size_t)r * width + d;
+        if (wide && d + 4 <= columns) {
+            *reinterpret_cast<float4*>(at) = o;
+        } else {
+            at[0] = o.x;
+            if (d + 1 < columns) at[1] = o.y;
+            if (d + 2 < columns) at[2] = o.z;
+            if (d + 3 < columns) at[3] = o.w;
+        }
+    }
+}
 
 // a thread's v of one chunk as it is stored
 template <typename T> struct DcValues;
@@ -645,7 +678,7 @@ __device__ __forceinline__ void dc_leave_out(float (&x)[DC_TILES][4], int t, con
 }
 
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(32 * DC_WALKERS + DC_FETCHERS, 2)
+__global__ void __launch_bounds__(32 * DC_WALKERS + DC_FETCHERS, sizeof(T) == 2 ? 2 : 1)
 delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     using Sh = DcShape<T, DK>;
     constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16, FINISH = Sh::FINISH;
@@ -658,12 +691,15 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     const int chunks = (count + DC_TOKENS - 1) / DC_TOKENS;
     const int chunk0 = dc_chunks_before(p.item_qlen, item, lane);
     if (chunk0 + chunks > records.chunks) return;              // lists that name more tokens than there are
-    // registers: two blocks of 256 threads have 128 each; the walking warps take over most of the fetching ones' (216 + 40)
+    // registers (bfloat16): two blocks of 256 threads have 128 each; the walking warps take over some of the fetching ones' (216 + 40)
     if (warp >= DC_WALKERS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
+        if (sizeof(T) == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
         grid_dependency_wait();
         grid_dependents_go();
         DcFetch<T, DK, WIDE> fetch(p, records, head, col0, t0, count, chunk0);
+        const size_t width = (size_t)p.heads * p.vdim;
+        float* out = p.out + (size_t)t0 * width + (size_t)head * p.vdim + col0;
+        const bool wide = p.vdim % 4 == 0 && (uintptr_t)p.out % 16 == 0;
         fetch.next(p, sm.stage[0]);
         fetch.next(p, sm.stage[1]);
         asm volatile("cp.async.wait_group 1;\n" ::: "memory");
@@ -671,12 +707,17 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         for (int c = 1; c <= chunks + 1; ++c) {                // (the last meetings are for chunks that are not there)
             asm volatile("cp.async.wait_group 0;\n" ::: "memory");
             dc_sync(DC_MEET, Sh::THREADS);                     // chunk c is there, and everybody is through with chunk c - 2:
+            if (c <= chunks) dc_sync(DC_GO, Sh::THREADS);      // (copies asked for at once would delay what the walkers swap)
             fetch.next(p, sm.stage[(c + 1) % DC_STAGES]);      // its stage takes chunk c + 1
+            if (c >= 2) {
+                dc_write<T, DK>(sm.out[c & 1], out, width, count - (c - 2) * DC_TOKENS, p.vdim - col0, wide);
+                out += DC_TOKENS * width;
+            }
         }
         asm volatile("cp.async.wait_group 0;\n" ::: "memory");
         return;
     }
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
+    if (sizeof(T) == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
     const int g = lane >> 2, t = lane & 3;
     const int group = warp / SLICES, slice = warp % SLICES;
     const int row0 = slice * DC_SLICE;                         // the warp's rows of S
@@ -696,37 +737,10 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     float sigma[2] = {1.f, 1.f}, back[2] = {1.f, 1.f};         // of columns col and col + 8, and one over it
     const int b_row = (lane & 7) + 8 * (lane >> 4), b_col = 8 * ((lane >> 3) & 1);      // ldmatrix, operand stored [n][k]
     const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);    // ... and [k][n]
-    const size_t width = (size_t)p.heads * p.vdim;
-    const int left = p.vdim - col;                             // columns col and col + 8 are there
-    const bool whole = col0 + group * 16 + 16 <= p.vdim;       // all of the warp's columns are there
-    float* out = p.out + (size_t)t0 * width + (size_t)head * p.vdim + col;      // the first token of the chunk that is written next
+    const int b_piece = dc_piece(lane & 7, (lane >> 3) & 1);   // ... of a 16 x 16 block
     // Two warps per 16 columns: the first finishes the outputs of token tiles 0 and 3, the second of 1 and 2 (tiles 2 and 3 have
     // two blocks of weights).  One warp: all four.
     auto tile_of = [&](int j) { return SLICES > 1 ? (j == 0 ? slice : 3 - slice) : j; };
-    // outputs of the last chunk, without the other warp's S0^T q, and the factors on those
-    float kept[FINISH][4], factor_kept[FINISH][4];
-    auto write = [&](const float (&o)[4], int tile, int tokens) {
-        const int token = 8 * tile + 2 * t;
-        float* to = out + (size_t)token * width;
-        if (whole && tokens >= DC_TOKENS) {
-            to[0] = o[0]; to[8] = o[2]; to[width] = o[1]; to[width + 8] = o[3];
-        } else {
-            if (token < tokens && left > 0) to[0] = o[0];
-            if (token < tokens && left > 8) to[8] = o[2];
-            if (token + 1 < tokens && left > 0) to[width] = o[1];
-            if (token + 1 < tokens && left > 8) to[width + 8] = o[3];
-        }
-    };
-    auto finish = [&](const float4 (&x)[FINISH], int tokens) {
-#pragma unroll
-        for (int j = 0; j < FINISH; ++j) {
-            float o[4];
-            dc_fma2(o[0], o[1], factor_kept[j][0], factor_kept[j][1], x[j].x, x[j].y, kept[j][0], kept[j][1]);
-            dc_fma2(o[2], o[3], factor_kept[j][2], factor_kept[j][3], x[j].z, x[j].w, kept[j][2], kept[j][3]);
-            write(o, tile_of(j), tokens);
-        }
-        out += DC_TOKENS * width;
-    };
     // Operands of the next products are read well ahead of them, and sums that do not depend on one another are asked for
     // together: a warp has its scheduler nearly to itself, so what one instruction waits for, all wait for.
     unsigned bk[2][2][4];                                      // K, operand of S0^T k, 16 rows of S and two times 16 tokens each; two in turn
@@ -741,7 +755,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
                 unsigned x[4];
-                dc_ldmatrix_trans(x, &st.v[16 * m + b_row][group * 16 + b_col]);
+                dc_ldmatrix_trans(x, &st.v[16 * m + b_row][Sh::v_piece(b_row, group * 2 + ((lane >> 3) & 1)) * 8]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) v.x[4 * m + e] = x[e];
             }
@@ -762,7 +776,6 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         float u[DC_TILES][4], wq[DC_TILES][4];                 // U, S0^T q
         unsigned bq[2][4];                                     // Q
         unsigned sh[STEPS][4], sl[STEPS][4];                   // the state in two parts
-        float4 late[FINISH];                                   // the other warp's S0^T q of the last chunk
         auto ask_query = [&](int k) {
 #pragma unroll
             for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][16 * m + b_row][row0 + 16 * k + b_col]);
@@ -887,13 +900,15 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             unsigned rh[2][4], rl[2][4], th[3][4], tl[3][4];
 #pragma unroll
             for (int b = 0; b < 3; ++b) {
-                dc_ldmatrix(th[b], &st.gates.t[0][b][b_row][b_col]);
-                dc_ldmatrix(tl[b], &st.gates.t[1][b][b_row][b_col]);
+                dc_ldmatrix(th[b], &st.gates.t[0][b][b_row][b_piece]);
+                dc_ldmatrix(tl[b], &st.gates.t[1][b][b_row][b_piece]);
             }
             dc_split_tiles(r[0], r[1], rh[0], rl[0]);
+            if (tries == 0) asm volatile("bar.arrive %0, %1;" ::"r"((int)DC_GO), "r"(Sh::THREADS) : "memory");
             query_step(1);
             dc_split_tiles(r[2], r[3], rh[1], rl[1]);
             dc_solve(u, rh, rl, th, tl);
+            query_step(2);
             if (__builtin_expect(!__any_sync(0xffffffffu, !(size < DC_MOST)), 1)) break;
             if (tries == 0) {                                  // (both warps of 16 columns have the same R and T)
                 look = true;
@@ -913,10 +928,11 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
         // ---- the new state
         const float decay = st.gates.fade[DC_TOKENS - 1];
-        unsigned uh[2][4], ul[2][4], zh[2][4], zl[2][4], kt[STEPS][4];
+        unsigned uh[2][4], ul[2][4], kt[STEPS][4];
         float add[TILES][4];
 #pragma unroll
         for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
+        query_step(3);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             float faded[2][4];
@@ -948,77 +964,85 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             }
 #pragma unroll
             for (int n = 0; n < TILES; ++n) dc_mma(add[n], uh[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
-            dc_split_tiles(u[2 * m], u[2 * m + 1], zh[m], zl[m]);
             if (m == 0) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][16 + bt_row][row0 + 16 * k + bt_col]);
-                query_step(2);
             }
         }
-        unsigned w[FINISH][2][4];                              // weights: high and low part, two inner halves each
-        float2 fade[FINISH], query[FINISH];
+        // ---- outputs: the chunk's start and its own tokens; the fetching warps add up what two warps have of S0^T q and write them
+        unsigned zh[2][4], zl[2][4], w[FINISH][2][4];          // U again, weights: high and low part, two inner halves each
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
             const bool second = SLICES > 1 ? j == 1 : j >= 2;  // the tile's tokens are in the chunk's second half
 #pragma unroll
             for (int m = 0; m <= (second ? 1 : 0); ++m)
-                dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_col]);
-            fade[j] = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile_of(j) + 2 * t]);
-            query[j] = *reinterpret_cast<const float2*>(&st.gates.query[8 * tile_of(j) + 2 * t]);
-            if (SLICES > 1) late[j] = sm.swap[(c + 1) & 1][warp ^ 1][Sh::SWAPS - FINISH + j][lane];     // (first chunk: not used)
+                dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_piece]);
         }
-        query_step(3);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) dc_split_tiles(u[2 * m], u[2 * m + 1], zh[m], zl[m]);
+        float oa[FINISH][4], ob[FINISH][4];
+#pragma unroll
+        for (int j = 0; j < FINISH; ++j) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) oa[j][e] = ob[j][e] = 0.f;
+#pragma unroll
+            for (int m = 0; m <= ((SLICES > 1 ? j == 1 : j >= 2) ? 1 : 0); ++m) {
+                dc_mma(ob[j], zl[m], w[j][m][0], w[j][m][1]);
+                dc_mma(oa[j], zh[m], w[j][m][0], w[j][m][1]);
+                dc_mma(ob[j], zh[m], w[j][m][2], w[j][m][3]);
+            }
+        }
         if (c + 1 < chunks) ask(sm.stage[next]);
 #pragma unroll
         for (int n = 0; n < TILES; ++n)
 #pragma unroll
             for (int e = 0; e < 4; e += 2)
                 dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
-        // ---- outputs: the chunk's start and its own tokens.  What the other warp has of S0^T q comes with the next meeting: the
-        // chunk before, which was a full one, is finished first
+        auto leave = [&](int which, int tile, const float4& o) {
+            float* to = &sm.out[c & 1][which][8 * tile + 2 * t][group * 16 + g];
+            to[0] = o.x; to[8] = o.z; to[Sh::OLD] = o.y; to[Sh::OLD + 8] = o.w;
+        };
+        // all that belongs to a token is multiplied by its factors, also what the other warp adds up
+        auto scaled = [&](const float (&x)[4], int tile, float2& query) {
+            const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile + 2 * t]);
+            query = *reinterpret_cast<const float2*>(&st.gates.query[8 * tile + 2 * t]);
+            float fx, fy;
+            float4 o;
+            dc_mul2(fx, fy, query.x, query.y, fade.x, fade.y);
+            dc_mul2(o.x, o.y, x[0], x[1], fx * back[0], fy * back[0]);
+            dc_mul2(o.z, o.w, x[2], x[3], fx * back[1], fy * back[1]);
+            return o;
+        };
         if constexpr (SLICES > 1) {
-            if (c > 0) finish(late, DC_TOKENS);
 #pragma unroll
             for (int j = 0; j < FINISH; ++j) {                 // the other warp's tiles
                 const float(&x)[4] = j == 0 ? wq[0] : wq[3], (&y)[4] = j == 0 ? wq[1] : wq[2];
-                sm.swap[c & 1][warp][Sh::SWAPS - FINISH + j][lane] =
-                    make_float4(slice ? x[0] : y[0], slice ? x[1] : y[1], slice ? x[2] : y[2], slice ? x[3] : y[3]);
+                const float z[4] = {slice ? x[0] : y[0], slice ? x[1] : y[1], slice ? x[2] : y[2], slice ? x[3] : y[3]};
+                float2 query;
+                const int tile = j == 0 ? 1 - slice : 2 + slice;
+                leave(SLICES - 1, tile, scaled(z, tile, query));
             }
         }
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
-            const int tile = tile_of(j);
-            const bool second = SLICES > 1 ? j == 1 : j >= 2;
-            float a[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int m = 0; m <= (second ? 1 : 0); ++m) {
-                dc_mma(b, zl[m], w[j][m][0], w[j][m][1]);
-                dc_mma(d, zh[m], w[j][m][2], w[j][m][3]);
-                dc_mma(a, zh[m], w[j][m][0], w[j][m][1]);
-            }
-            float mine[4];
+            const int tile = tile_of(j), first = 8 * tile + 2 * t;
+            float x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                mine[e] = SLICES == 1 ? wq[j][e] : j == 0 ? (slice ? wq[1][e] : wq[0][e]) : (slice ? wq[2][e] : wq[3][e]);
-            const int first = 8 * tile + 2 * t;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                float x, y, fx, fy;
-                dc_add2(x, y, b[2 * h], b[2 * h + 1], d[2 * h], d[2 * h + 1]);
-                dc_add2(x, y, a[2 * h], a[2 * h + 1], x, y);
-                dc_fma2(x, y, fade[j].x, fade[j].y, mine[2 * h], mine[2 * h + 1], x, y);
-                dc_mul2(fx, fy, query[j].x, query[j].y, back[h], back[h]);
-                dc_mul2(x, y, x, y, fx, fy);
-                if (__builtin_expect(spoiled, 0)) {
-                    if (first >= bad[h]) x = __int_as_float(0x7fffffff);
-                    if (first + 1 >= bad[h]) y = __int_as_float(0x7fffffff);
-                }
-                kept[j][2 * h] = x; kept[j][2 * h + 1] = y;
-                dc_mul2(factor_kept[j][2 * h], factor_kept[j][2 * h + 1], fx, fy, fade[j].x, fade[j].y);
+                x[e] = SLICES == 1 ? wq[j][e] : j == 0 ? (slice ? wq[1][e] : wq[0][e]) : (slice ? wq[2][e] : wq[3][e]);
+            float2 query;
+            float4 o = scaled(x, tile, query);
+            dc_fma2(o.x, o.y, oa[j][0] + ob[j][0], oa[j][1] + ob[j][1], query.x * back[0], query.y * back[0], o.x, o.y);
+            dc_fma2(o.z, o.w, oa[j][2] + ob[j][2], oa[j][3] + ob[j][3], query.x * back[1], query.y * back[1], o.z, o.w);
+            if (__builtin_expect(spoiled, 0)) {
+                const float nan = __int_as_float(0x7fffffff);
+                if (first >= bad[0]) o.x = nan;
+                if (first + 1 >= bad[0]) o.y = nan;
+                if (first >= bad[1]) o.z = nan;
+                if (first + 1 >= bad[1]) o.w = nan;
             }
-            if (SLICES == 1) write(kept[j], tile, count - c * DC_TOKENS);
+            leave(0, tile, o);
         }
-        if (SLICES == 1) out += DC_TOKENS * width;
         if (__builtin_expect(spoiled, 0)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -1029,12 +1053,6 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
     }
     dc_sync(DC_MEET, Sh::THREADS);
-    if constexpr (SLICES > 1) {
-        float4 late[FINISH];
-#pragma unroll
-        for (int j = 0; j < FINISH; ++j) late[j] = sm.swap[(chunks - 1) & 1][warp ^ 1][Sh::SWAPS - FINISH + j][lane];
-        finish(late, count - (chunks - 1) * DC_TOKENS);
-    }
 #pragma unroll
     for (int n = 0; n < TILES; ++n)
 #pragma unroll
