@@ -197,6 +197,58 @@ class CacheManager:
         handle.closed = True
         del self.live[handle.request_id]
 
+    def fork(self, handle: RequestCache, request_ids: Sequence) -> Tuple[List[RequestCache], List[List[Tuple[int, int]]]]:
+        """New requests that continue where `handle` stands: its full pages become shared (under reference counts), each
+        gets a page of its own for a begun one, and a state slot.  Returns them, and per group the (page, page) pairs
+        whose contents the owner of the device memory has to copy (as it has to copy the state slots, from the parent's
+        to the new ones).  OutOfPages, with nothing changed, when slots or pages do not suffice."""
+        if handle.closed:
+            raise RuntimeError(f"request {handle.request_id!r} is closed")
+        request_ids = list(request_ids)
+        for index, request_id in enumerate(request_ids):
+            if request_id in self.live or request_id in request_ids[:index]:
+                raise RuntimeError(f"request {request_id!r} is already open")
+        count = len(request_ids)
+        if count > self.slots.num_free:
+            raise OutOfPages(f"{count} state slots are needed, {self.slots.num_free} are free")
+        full = handle.length // self.page_size
+        begun = handle.length % self.page_size != 0
+        needed = [count if begun and table[full] >= 0 else 0 for table in handle.tables]
+        if any(n > have for n, have in zip(needed, self.free_pages())):
+            raise OutOfPages(f"{needed} pages are needed, free are {self.free_pages()}")
+        children, moves = [], [[] for _ in self.groups]
+        for request_id in request_ids:
+            child = RequestCache(request_id, self.slots.acquire(), [[] for _ in self.groups], handle.length,
+                                 handle.shared_tokens, fresh_state=handle.fresh_state)
+            for g, table in enumerate(handle.tables):
+                for page in table[:full]:
+                    if page >= 0:
+                        self._incref(g, page)
+                    child.tables[g].append(page)
+                if begun and table[full] >= 0:
+                    page = self._allocate(g)
+                    moves[g].append((table[full], page))
+                    child.tables[g].append(page)
+                elif begun:
+                    child.tables[g].append(-1)
+            self.live[request_id] = child
+            children.append(child)
+        return children, moves
+
+    def compact(self) -> List[List[Tuple[int, int]]]:
+        """Renumber every group's pages in use so that they are its first ones (the rest of the pool is then one piece);
+        tables, reference counts and cached prefixes follow.  Returns per group the (old, new) pairs whose contents the
+        owner of the device memory has to copy; no new page is an old one of the list."""
+        moves = [pool.compact() for pool in self.pools]
+        for handle in self.live.values():
+            for table, moved in zip(handle.tables, moves):
+                table[:] = [moved.get(page, page) for page in table]
+            handle._arrays = None
+        for entry in self._lru.values():
+            entry.pages = tuple(moved.get(page, page) for page, moved in zip(entry.pages, moves))
+        self._cached_page = {entry.pages[0]: entry for entry in self._lru.values()}
+        return [list(moved.items()) for moved in moves]
+
     def can_open(self) -> bool:
         return self.slots.num_free > 0
 

@@ -7,7 +7,7 @@ error on exhaustion, on a second free and on a reference to a free page.
 
 from __future__ import annotations
 
-from typing import List
+from typing import Dict, List
 
 
 class OutOfPages(RuntimeError):
@@ -47,6 +47,17 @@ class PagePool:
         self._refs[page] -= 1
         if self._refs[page] == 0:
             self._free.append(page)
+
+    def compact(self) -> Dict[int, int]:
+        """Renumber the pages in use so that they are the first ones: {old id: new id} of those that move, whose
+        old ids are all beyond the new ones."""
+        used = [page for page, refs in enumerate(self._refs) if refs]
+        moved = [page for page in used if page >= len(used)]
+        moves = dict(zip(moved, (page for page in range(len(used)) if not self._refs[page])))
+        for old, new in moves.items():
+            self._refs[new], self._refs[old] = self._refs[old], 0
+        self._free = list(range(len(self._refs) - 1, len(used) - 1, -1))
+        return moves
 
     def ref_count(self, page: int) -> int:
         return self._refs[page]

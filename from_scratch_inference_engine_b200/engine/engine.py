@@ -17,11 +17,13 @@ nothing, which is dropped.
 from __future__ import annotations
 
 import json
+from dataclasses import replace
 from pathlib import Path
 from typing import List, Optional, Sequence
 
 import torch
 
+from ..cache.pool import OutOfPages
 from ..config.registry import load_config
 from ..parts.model import DecoderModel
 from ..sampling.sampler import Sampler, SamplingParams, request_seed
@@ -114,6 +116,60 @@ class Engine:
         rid = self.scheduler.next_id
         seed = params.seed if params.seed is not None else request_seed(self.seed, rid)
         return self.scheduler.add(prompt, params, max_tokens, eos_id, seed)
+
+    def fork(self, request_id: int, count: int = 1, params: Optional[Sequence[SamplingParams]] = None) -> List[int]:
+        """Continue a running request `count` more times from where it stands: prompt and output so far are shared, not run
+        again (full pages under reference counts; the begun page and every layer's state are copied), and each
+        continuation samples by its own seed (`params`: one per continuation, the request's options otherwise).  Returns
+        their ids.  A request that is not running is refused; RuntimeError (OutOfPages where the cache's room is what lacks)
+        when there is no room now."""
+        if self._in_flight is not None:
+            self._settle()
+        seq = self.scheduler.sequences[request_id]
+        if seq.status is not SeqStatus.Running or seq.handle is None:
+            raise ValueError(f"Engine: request {request_id} is not running and cannot be continued another time")
+        if count < 0 or (params is not None and len(params) != count):
+            raise ValueError("Engine: one SamplingParams per continuation is needed")
+        if len(self.scheduler.running) + count > self.scheduler.max_batch:
+            raise RuntimeError(f"Engine: {count} more running requests exceed max_batch {self.scheduler.max_batch}")
+        if params is None:                  # a seed of its own each, whatever the request's is
+            params = [replace(seq.params, seed=None)] * count
+        ids = self.scheduler.next_ids(count)
+        handles = self.runner.fork(seq.handle, ids)
+        seeds = [p.seed if p.seed is not None else request_seed(self.seed, rid) for p, rid in zip(params, ids)]
+        return self.scheduler.fork(seq, handles, params, seeds)
+
+    def compact(self) -> List[int]:
+        """Bring the pages in use to the front of their pools; returns how many those are per group."""
+        if self._in_flight is not None:
+            self._settle()
+        return self.runner.compact()
+
+    def add_samples(self, prompt: Sequence[int], params: Sequence[SamplingParams], max_tokens: int = 16,
+                    eos_id: int = -1) -> List[int]:
+        """One request per element of `params` with the same prompt, which is run once: up to its last token by the first
+        request, which is then continued (`fork`) as often as needed.  Runs steps until then (of other requests too).
+        Continuations for which there is no room then run the prompt by themselves.  Returns the ids, in order."""
+        if not params:
+            return []
+        first = self.add_request(prompt, params[0], max_tokens, eos_id)
+        seq = self.scheduler.sequences[first]
+        ids, rest = [first], list(params[1:])
+        if len(prompt) > 1 and rest:
+            seq.hold = len(prompt) - 1
+            while seq.handle is None or seq.handle.length < seq.hold:
+                if self.step() == 0:
+                    break
+            if seq.handle is not None and seq.handle.length == seq.hold:
+                count = max(0, min(len(rest), self.scheduler.max_batch - len(self.scheduler.running),
+                                   self.runner.cache.slots.num_free))
+                try:
+                    ids += self.fork(first, count, rest[:count])
+                    rest = rest[count:]
+                except OutOfPages:
+                    pass
+            seq.hold = 0
+        return ids + [self.add_request(prompt, p, max_tokens, eos_id) for p in rest]
 
     def warm_up(self, max_context: int = 0) -> int:
         """Before serving starts: run one step of the largest size (its working memory then

@@ -10,7 +10,7 @@ engine.  Added: `dtype`, `device`, `max_step_tokens`.
 from __future__ import annotations
 
 import json
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from pathlib import Path
 from typing import List, Optional, Sequence
 
@@ -72,6 +72,17 @@ class LLM:
         config = config or GenerationConfig()
         ids = [self.engine.add_request(list(p), self._params(config), config.max_tokens,
                                        self.eos_id) for p in prompts]
+        self.engine.run_until_done()
+        return [list(self.engine.output(i)) for i in ids]
+
+    def generate_samples(self, prompt_ids: Sequence[int], count: int,
+                         config: Optional[GenerationConfig] = None) -> List[List[int]]:
+        """`count` answers to one prompt, which is run once (`Engine.add_samples`).  With a seed in `config` answer i
+        draws by seed + i, otherwise each by a seed of its own."""
+        config = config or GenerationConfig()
+        base = self._params(config)
+        params = [base if config.seed is None else replace(base, seed=config.seed + i) for i in range(count)]
+        ids = self.engine.add_samples(list(prompt_ids), params, config.max_tokens, self.eos_id)
         self.engine.run_until_done()
         return [list(self.engine.output(i)) for i in ids]
 

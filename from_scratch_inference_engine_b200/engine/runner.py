@@ -321,6 +321,38 @@ class ModelRunner:
             cache.commit(entry.handle, len(entry.tokens))
         return logits
 
+    # -------------------------------------------------------------- copies of what requests hold
+    def _copy_blocks(self, buffers: Sequence[torch.Tensor], moves) -> None:
+        from ..kernels import ops
+        host = np.asarray(moves, dtype=np.int32).reshape(-1)
+        ops.copy_blocks(buffers, self._ring.stage(host, self.runtime.device).view(-1, 2), self.error)
+
+    def fork(self, handle: RequestCache, request_ids: Sequence) -> List[RequestCache]:
+        """New requests that continue where `handle` stands (between two steps): full pages are shared, a begun page and
+        the state of every layer are copied.  OutOfPages, with nothing changed, when slots or pages do not suffice."""
+        children, moves = self.cache.fork(handle, request_ids)
+        for pages, pairs in zip(self.pages, moves):
+            if pairs:
+                self._copy_blocks([pages], pairs)
+        if children and not handle.fresh_state:
+            slots = [(handle.slot, child.slot) for child in children]
+            by_size: Dict[int, List[torch.Tensor]] = {}
+            for state in self.states:
+                if state is not None:
+                    by_size.setdefault(state[0].numel() * state.element_size(), []).append(state)
+            for states in by_size.values():
+                self._copy_blocks(states, slots)
+        return children
+
+    def compact(self) -> List[int]:
+        """Bring every group's pages in use to the front of its pool (between two steps): returns how many those are, so that
+        pages[g][:n] holds them in one piece."""
+        moves = self.cache.compact()
+        for pages, pairs in zip(self.pages, moves):
+            if pairs:
+                self._copy_blocks([pages], pairs)
+        return [pool.num_pages - pool.num_free for pool in self.cache.pools]
+
     def raise_on_device_error(self) -> None:
         code = int(self.error.item())
         if code:
@@ -346,5 +378,6 @@ class ModelRunner:
                     41: "tiled float32 product: the copy engine's stage never became free",
                     42: "tiled float32 product: a stage never arrived",
                     43: "tiled float32 product: a stage was never multiplied",
+                    4: "copy of blocks: a block outside its pool",
                     3: "attention: a visible key lies in a page that was given back"}
             raise DeviceFault(what.get(code, f"device error flag {code}"))

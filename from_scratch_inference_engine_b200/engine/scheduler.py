@@ -59,6 +59,7 @@ class Sequence_:
     preempted: int = 0
     pending: int = 0          # 1 while a sampled token has not been read from the GPU yet
     pending_row: int = -1     # ... and the row of that step's samples it will be found in
+    hold: int = 0             # > 0: no token from this place of the context on is run yet
 
     def context(self) -> List[int]:
         return self.prompt + self.output
@@ -140,6 +141,23 @@ class Scheduler:
         self.next_id += 1
         return seq.id
 
+    def fork(self, seq: Sequence_, handles: Sequence[RequestCache], params: Sequence[SamplingParams],
+             seeds: Sequence[int]) -> List[int]:
+        """Running requests of their own that continue where `seq` stands, one per handle (whose request ids are the ids
+        that `next_ids` named)."""
+        ids = []
+        for handle, own, seed in zip(handles, params, seeds):
+            child = Sequence_(self.next_id, list(seq.prompt), own, seq.max_tokens, seq.eos_id, seed, list(seq.output),
+                              SeqStatus.Running, seq.prefilled, handle)
+            self.sequences[child.id] = child
+            self.running.append(child.id)
+            self.next_id += 1
+            ids.append(child.id)
+        return ids
+
+    def next_ids(self, count: int) -> List[int]:
+        return list(range(self.next_id, self.next_id + count))
+
     def has_work(self) -> bool:
         return bool(self.waiting or self.running)
 
@@ -218,7 +236,7 @@ class Scheduler:
                             continue
                         pages_left = left
                 remaining = total - handle.length
-                chunk = min(remaining, tokens_left)
+                chunk = min(remaining, tokens_left, seq.hold - handle.length if seq.hold else remaining)
                 # shrink the portion to the pages that are left
                 room = min((len(t) + left) * cache.page_size - handle.length
                            for t, left in zip(handle.tables, pages_left)) if handle.tables \

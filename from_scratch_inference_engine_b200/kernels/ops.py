@@ -2303,6 +2303,11 @@ def delta():
     return _delta
 
 
+def delta_max_dim() -> int:
+    """State rows per head that the gated delta rule holds."""
+    return int(delta().fsie_delta_max_dim())
+
+
 def delta_prep_max_taps() -> int:
     return int(delta().fsie_delta_prep_max_taps())
 
@@ -2385,8 +2390,8 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
         raise KernelError("gated_delta_rule: the lists are shorter than the requests")
     if not eps > 0:
         raise KernelError("gated_delta_rule: eps must be positive")
-    if dim > delta().fsie_delta_max_dim():
-        raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {delta().fsie_delta_max_dim()}")
+    if dim > delta_max_dim():
+        raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {delta_max_dim()}")
     lib, tag, room = delta(), _tag(qkv.dtype), None
     chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= lib.fsie_delta_chunk_max_dim()
     if chunked:
