@@ -9,9 +9,10 @@
 // token - writes its new ones.  Sums, activation and gates are 32-bit; c is rounded once, to the storage type, as all
 // activations between kernels are.
 //
-// Bound by memory: the projection's columns are read and c is written once.  A thread owns eight neighbouring channels
-// (16-byte accesses in bfloat16) and walks the tile's tokens with the last taps - 1 inputs in registers, so that no input
-// is read for every tap again; the loads of PREP_AHEAD tokens go out together.
+// Bound by memory: the projection's columns are read and c is written once.  A thread owns four neighbouring channels
+// (8-byte accesses in bfloat16) of up to PREP_AHEAD tokens and asks for all their inputs, and the taps - 1 in front of
+// them, before it does anything else; what stands in front of another thread's tokens comes from L2 a second time.
+// PREP_MEASURED
 #include "common.cuh"
 #include <math.h>
 
@@ -22,7 +23,70 @@ constexpr int PREP_AHEAD = 8;
 constexpr int PREP_MAX_TAPS = 16;
 
 __device__ __forceinline__ float prep_silu(float z) { return z / (1.0f + expf(-z)); }
+// two floats in one register pair: the packed instructions of sm_100 work on both at once
+__device__ __forceinline__ unsigned long long prep_pair(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void prep_unpair(unsigned long long p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+__device__ __forceinline__ unsigned long long prep_fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long prep_mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float prep_exp2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ float prep_rcp(float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+// silu of four numbers.  Stored in 8 bits it needs no more than the approximate exponential and reciprocal (2^-22): the kernel is
+// bound by its instructions with the exact ones.
+template <typename T> __device__ __forceinline__ void prep_silu4(const unsigned long long (&z)[2], float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float x, y;
+        prep_unpair(z[i], x, y);
+        if (sizeof(T) == 2) {
+            constexpr float L = -1.4426950408889634f;
+            float ex, ey;
+            prep_unpair(prep_mul2(z[i], prep_pair(L, L)), ex, ey);
+            prep_unpair(prep_mul2(z[i], prep_pair(prep_rcp(1.0f + prep_exp2(ex)), prep_rcp(1.0f + prep_exp2(ey)))), v[2 * i], v[2 * i + 1]);
+        } else {
+            v[2 * i] = prep_silu(x);
+            v[2 * i + 1] = prep_silu(y);
+        }
+    }
+}
 __device__ __forceinline__ float prep_softplus(float z) { return z > 20.f ? z : log1pf(expf(z)); }
+// four neighbouring values
+template <typename T> struct Stored4;
+template <> struct Stored4<bf16> {
+    uint2 x;
+    __device__ __forceinline__ void load(const bf16* p) { x = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ void widen(float (&v)[4]) const {
+        v[0] = __uint_as_float(x.x << 16); v[1] = __uint_as_float(x.x & 0xffff0000u);
+        v[2] = __uint_as_float(x.y << 16); v[3] = __uint_as_float(x.y & 0xffff0000u);
+    }
+};
+template <> struct Stored4<float> {
+    float4 x;
+    __device__ __forceinline__ void load(const float* p) { x = *reinterpret_cast<const float4*>(p); }
+    __device__ __forceinline__ void widen(float (&v)[4]) const { v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; }
+};
+__device__ __forceinline__ void prep_load(const float* p, float (&v)[4]) {
+    const float4 x = *reinterpret_cast<const float4*>(p);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+}
+__device__ __forceinline__ void prep_store(float* p, const float (&v)[4]) { *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+__device__ __forceinline__ void prep_store(bf16* p, const float (&v)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b));
+}
 
 struct PrepParams {
     int ld, conv_off, a_off, b_off;
@@ -46,20 +110,24 @@ __device__ __forceinline__ void prep_gates(const PrepParams& p, const T* __restr
     }
 }
 
-// grid (tiles, slices of channels and one more for the gates)
+// grid (tiles, slices of channels and one more for the gates, parts of PREP_AHEAD tokens of a tile)
 template <typename T, int TAPS>
-__global__ void __launch_bounds__(PREP_THREADS)
+__global__ void __launch_bounds__(PREP_THREADS, 8)
 delta_prep_kernel(const T* __restrict__ proj, T* __restrict__ act, const PrepParams p) {
     const int tile = blockIdx.x;
-    const int item = p.seg_item[tile], row0 = p.seg_row0[tile];
+    const int item = p.seg_item[tile], row0 = p.seg_row0[tile] + blockIdx.z * PREP_AHEAD;
     const int qlen = p.item_qlen[item], slot = p.item_slots[item];
-    const int count = min(p.seg_tokens, qlen - row0), t0 = p.item_qstart[item] + row0;
-    const int c = (blockIdx.y * PREP_THREADS + threadIdx.x) * 8;
+    const int count = min(min(PREP_AHEAD, p.seg_tokens - (int)blockIdx.z * PREP_AHEAD), qlen - row0), t0 = p.item_qstart[item] + row0;
+    const int c = (blockIdx.y * PREP_THREADS + threadIdx.x) * 4;
     const bool gates = blockIdx.y == gridDim.y - 1, mine = !gates && c < p.channels;
-    float w[TAPS][8];
+    unsigned long long w[TAPS][2];
     if (mine) {
 #pragma unroll
-        for (int j = 0; j < TAPS; ++j) load8(p.conv + (size_t)j * p.channels + c, w[j]);
+        for (int j = 0; j < TAPS; ++j) {
+            const float4 x = *reinterpret_cast<const float4*>(p.conv + (size_t)j * p.channels + c);
+            w[j][0] = prep_pair(x.x, x.y);
+            w[j][1] = prep_pair(x.z, x.w);
+        }
     }
     grid_dependency_wait();
     grid_dependents_go();
@@ -69,46 +137,59 @@ delta_prep_kernel(const T* __restrict__ proj, T* __restrict__ act, const PrepPar
     const T* from = proj + (size_t)t0 * p.ld + p.conv_off + c;
     T* to = act + (size_t)t0 * p.channels + c;
     float* tail = p.state + (size_t)slot * p.state_stride + p.tail_off + c;
-    float last[TAPS - 1][8];                               // the inputs before the next token, oldest first
+    Stored4<T> u[PREP_AHEAD];
+#pragma unroll
+    for (int r = 0; r < PREP_AHEAD; ++r)
+        if (r < count) u[r].load(from + (size_t)r * p.ld);
+    // The inputs in front of the thread's first token, oldest first: in front of the request's first token the slot's.  Only the
+    // part with that token looks at the slot, and the same thread writes there behind it.
+    float last[TAPS - 1][4];
+    Stored4<T> ahead[TAPS - 1];
 #pragma unroll
     for (int j = 0; j < TAPS - 1; ++j) {
-        if (row0 == 0) load8(tail + (size_t)j * p.channels, last[j]);
-        else load8(from - (ptrdiff_t)(TAPS - 1 - j) * p.ld, last[j]);     // row0 >= taps - 1
+        const int back = TAPS - 1 - j;
+        if (row0 == 0) prep_load(tail + (size_t)j * p.channels, last[j]);
+        else ahead[j].load(from - (ptrdiff_t)back * p.ld);                    // row0 >= taps - 1
     }
-    for (int r0 = 0; r0 < count; r0 += PREP_AHEAD) {
-        float u[PREP_AHEAD][8];
+    if (row0 != 0) {
 #pragma unroll
-        for (int r = 0; r < PREP_AHEAD; ++r)
-            if (r0 + r < count) load8(from + (size_t)(r0 + r) * p.ld, u[r]);
+        for (int j = 0; j < TAPS - 1; ++j) ahead[j].widen(last[j]);
+    }
 #pragma unroll
-        for (int r = 0; r < PREP_AHEAD; ++r) {
-            if (r0 + r < count) {
-                float sum[8];
+    for (int r = 0; r < PREP_AHEAD; ++r) {
+        if (r < count) {
+            float sum[4], x[4];
+            unsigned long long z[2];
+            u[r].widen(x);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum[i] = w[0][i] * last[0][i];
+            for (int i = 0; i < 2; ++i) {
+                z[i] = prep_mul2(w[0][i], prep_pair(last[0][2 * i], last[0][2 * i + 1]));
 #pragma unroll
-                    for (int j = 1; j < TAPS - 1; ++j) sum[i] = fmaf(w[j][i], last[j][i], sum[i]);
-                    sum[i] = prep_silu(fmaf(w[TAPS - 1][i], u[r][i], sum[i]));
-                }
-                store8(to + (size_t)(r0 + r) * p.channels, sum);
+                for (int j = 1; j < TAPS - 1; ++j) z[i] = prep_fma2(w[j][i], prep_pair(last[j][2 * i], last[j][2 * i + 1]), z[i]);
+                z[i] = prep_fma2(w[TAPS - 1][i], prep_pair(x[2 * i], x[2 * i + 1]), z[i]);
+            }
+            prep_silu4<T>(z, sum);
+            prep_store(to, sum);
+            to += p.channels;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                    for (int j = 0; j + 1 < TAPS - 1; ++j) last[j][i] = last[j + 1][i];
-                    last[TAPS - 2][i] = u[r][i];
-                }
+                for (int j = 0; j + 1 < TAPS - 1; ++j) last[j][i] = last[j + 1][i];
+                last[TAPS - 2][i] = x[i];
             }
         }
     }
     if (row0 == 0) {
-        if (count < qlen) {                                // the request's last tokens are another tile's
+        if (count < qlen) {                                // the request's last tokens are another thread's
             const T* end = from + (size_t)qlen * p.ld;
 #pragma unroll
-            for (int j = 0; j < TAPS - 1; ++j) load8(end - (ptrdiff_t)(TAPS - 1 - j) * p.ld, last[j]);
+            for (int j = 0; j < TAPS - 1; ++j) {
+                const int back = TAPS - 1 - j;
+                if (back <= qlen) { ahead[j].load(end - (ptrdiff_t)back * p.ld); ahead[j].widen(last[j]); }
+            }
         }
 #pragma unroll
-        for (int j = 0; j < TAPS - 1; ++j) store8(tail + (size_t)j * p.channels, last[j]);
+        for (int j = 0; j < TAPS - 1; ++j) prep_store(tail + (size_t)j * p.channels, last[j]);
     }
 }
 
@@ -144,12 +225,15 @@ delta_prep_any_kernel(const T* __restrict__ proj, T* __restrict__ act, const Pre
 }
 
 template <typename T>
-static int launch_prep(const void* proj, void* act, const PrepParams& p, int tiles, int early, cudaStream_t stream) {
-    const bool wide = p.channels % 8 == 0 && p.ld % 8 == 0 && p.conv_off % 8 == 0 && (uintptr_t)proj % 16 == 0 &&
+static int launch_prep(const void* proj, void* act, const PrepParams& p, int tokens, int tiles, int early, cudaStream_t stream) {
+    const bool wide = p.channels % 4 == 0 && p.ld % 4 == 0 && p.conv_off % 4 == 0 && (uintptr_t)proj % 16 == 0 &&
                       (uintptr_t)act % 16 == 0 && (uintptr_t)p.conv % 16 == 0 && (uintptr_t)p.state % 16 == 0 &&
                       p.state_stride % 4 == 0 && p.tail_off % 4 == 0;
     if (wide && p.taps >= 2 && p.taps <= 4) {
-        const dim3 grid(tiles, (p.channels / 8 + PREP_THREADS - 1) / PREP_THREADS + 1);
+        // (no tile holds more tokens than there are)
+        const dim3 grid(tiles, (p.channels / 4 + PREP_THREADS - 1) / PREP_THREADS + 1,
+                        (min(p.seg_tokens, tokens) + PREP_AHEAD - 1) / PREP_AHEAD);
+        if (grid.z > 65535) return ERR_UNSUPPORTED;
         auto kernel = p.taps == 2 ? delta_prep_kernel<T, 2> : p.taps == 3 ? delta_prep_kernel<T, 3> : delta_prep_kernel<T, 4>;
         return launch_dependent_if(early, kernel, grid, dim3(PREP_THREADS), 0, stream, (const T*)proj, (T*)act, p);
     }
@@ -165,12 +249,12 @@ extern "C" {
 
 int fsie_delta_prep_max_taps() { return PREP_MAX_TAPS; }
 
-int fsie_delta_prep(const void* proj, int ld, int conv_off, int a_off, int b_off, const int* item_qstart, const int* item_qlen,
+int fsie_delta_prep(const void* proj, int tokens, int ld, int conv_off, int a_off, int b_off, const int* item_qstart, const int* item_qlen,
                     const int* item_slots, const int* seg_item, const int* seg_row0, int tiles, int seg_tokens, float* state,
                     long long state_stride, long long tail_off, const float* conv, int taps, int channels, const float* a_log,
                     const float* dt_bias, int heads, void* act, float* log_decay, float* beta, int dtype, int early,
                     cudaStream_t stream) {
-    if (tiles <= 0) return 0;
+    if (tiles <= 0 || tokens <= 0) return 0;
     if (taps < 1 || taps > PREP_MAX_TAPS || (channels + PREP_THREADS - 1) / PREP_THREADS > 65534) return ERR_UNSUPPORTED;
     // only the tile with a request's first token may look at the slot, which that tile also writes
     if (channels <= 0 || heads <= 0 || seg_tokens < 1 || seg_tokens < taps - 1 || (taps > 1 && !state)) return ERR_BAD_ARGUMENT;
@@ -181,8 +265,8 @@ int fsie_delta_prep(const void* proj, int ld, int conv_off, int a_off, int b_off
     p.state = state; p.state_stride = state_stride; p.tail_off = tail_off;
     p.conv = conv; p.taps = taps; p.channels = channels;
     p.a_log = a_log; p.dt_bias = dt_bias; p.heads = heads; p.log_decay = log_decay; p.beta = beta;
-    if (dtype == DTYPE_F32) return launch_prep<float>(proj, act, p, tiles, early, stream);
-    if (dtype == DTYPE_BF16) return launch_prep<bf16>(proj, act, p, tiles, early, stream);
+    if (dtype == DTYPE_F32) return launch_prep<float>(proj, act, p, tokens, tiles, early, stream);
+    if (dtype == DTYPE_BF16) return launch_prep<bf16>(proj, act, p, tokens, tiles, early, stream);
     return ERR_BAD_ARGUMENT;
 }
 

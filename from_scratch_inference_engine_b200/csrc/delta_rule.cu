@@ -22,7 +22,8 @@ namespace fsie {
 //
 // Bound by memory for one token per request: S is read and written once, nothing else is of that size.  The slices are
 // narrow (32 columns, a 128-byte line a row) so that one request's heads already give work to many SMs, and all of a
-// thread's loads of S are asked for before the kernel in front has finished (`early`).
+// thread's loads of S are asked for before the kernel in front has finished (`early`).  One request of 16 heads of 128 x 128
+// takes 5.0 us: a chain of list, S and two meetings, 2 MB being nothing.
 constexpr int STEP_COLS = 32;
 constexpr int STEP_THREADS = 256;
 constexpr int STEP_WARPS = STEP_THREADS / 32;
@@ -148,10 +149,135 @@ delta_step_kernel(const DeltaParams p) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------- many decoded tokens
+// The same for steps whose states are more than what the SMs work on at once.  What bounds the kernel above then is its
+// instructions: a thread has 16 numbers of S, and reading k and q, the sums over the warps and the lengths take it several times
+// what the S takes.  Here it has 64 or 32: a block of 2 DIM threads owns DIM rows (64 or 128) x 4 ACROSS columns, ACROSS threads
+// side by side in a row and groups of ACROSS / 2 rows.
+// 64 requests of 32 heads of 128 x 128 take 52 us (268 MB, 5.2 TB/s; the kernel above 61; a kernel that only reads and
+// writes such a state in place 43), 200 of 12 heads of 64 x 64 19 us (31), 16 of 16 heads 8.7 us (10.9).  What is left is the
+// block's own chain: lists, S, three meetings, S.  (One block per SM with the next two S on their way into its shared memory
+// took 70 us: its meetings hold up everything.)
+constexpr int HEAD_MAX_DIM = 128;
+constexpr int HEAD_FROM = 64;              // blocks
+
+template <typename T, int ACROSS, int DIM>
+__global__ void __launch_bounds__(2 * DIM, ACROSS == 16 ? (DIM == 128 ? 3 : 6) : DIM == 128 ? 2 : 4)
+delta_head_kernel(const DeltaParams p) {
+    constexpr int COLS = 4 * ACROSS, ROWS = ACROSS / 2, WARPS = 2 * DIM / 32;
+    __shared__ __align__(16) float ks[2][DIM], qs[2][DIM], sums[2][WARPS][COLS], us[2][COLS];
+    const int head = blockIdx.y, item = blockIdx.z, col0 = blockIdx.x * COLS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
+    if (slot < 0 || count <= 0) return;                    // a padding entry of a fixed-size batch
+    const int row0 = tid / ACROSS * ROWS, at = (tid % ACROSS) * 4;     // the thread's rows and columns
+    const bool in = col0 + at < p.vdim;
+    float* state = p.state + (size_t)slot * p.state_stride + ((size_t)head * p.dim + row0) * p.vdim + col0 + at;
+    float4 s[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        s[i] = in && row0 + i < p.dim ? *reinterpret_cast<const float4*>(state + (size_t)i * p.vdim) : make_float4(0.f, 0.f, 0.f, 0.f);
+    grid_dependency_wait();
+    grid_dependents_go();
+    // k by the first half of the threads, q by the other; v by the threads that sum up S^T k, later
+    const int d = tid & (DIM - 1), narrow = head / p.share * p.dim;
+    const T* row = (const T*)p.qkv + (size_t)t0 * p.ld;
+    auto part = [&](const T* from) { return d < p.dim ? to_float(from[(tid < DIM ? p.k_off : p.q_off) + narrow + d]) : 0.f; };
+    float mine = part(row);
+    for (int r = 0; r < count; ++r) {
+        const int turn = r & 1, t = t0 + r;
+        (tid < DIM ? ks : qs)[turn][d] = mine;
+        const float v = tid < COLS && col0 + tid < p.vdim ? to_float(row[p.v_off + head * p.vdim + col0 + tid]) : 0.f;
+        const float decay = expf(p.log_decay[(size_t)t * p.heads + head]), beta = p.beta[(size_t)t * p.heads + head];
+        row += p.ld;
+        __syncthreads();
+        if (r + 1 < count) mine = part(row);
+        float4 with_k = make_float4(0.f, 0.f, 0.f, 0.f), with_q = with_k;
+#pragma unroll
+        for (int i = 0; i < ROWS; i += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(&ks[turn][row0 + i]), q = *reinterpret_cast<const float4*>(&qs[turn][row0 + i]);
+            const float kx[4] = {k.x, k.y, k.z, k.w}, qx[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 x = s[i + j];
+                with_k.x = fmaf(x.x, kx[j], with_k.x); with_k.y = fmaf(x.y, kx[j], with_k.y);
+                with_k.z = fmaf(x.z, kx[j], with_k.z); with_k.w = fmaf(x.w, kx[j], with_k.w);
+                with_q.x = fmaf(x.x, qx[j], with_q.x); with_q.y = fmaf(x.y, qx[j], with_q.y);
+                with_q.z = fmaf(x.z, qx[j], with_q.z); with_q.w = fmaf(x.w, qx[j], with_q.w);
+            }
+        }
+        if (ACROSS == 16) {
+            with_k.x += __shfl_xor_sync(0xffffffffu, with_k.x, 16); with_k.y += __shfl_xor_sync(0xffffffffu, with_k.y, 16);
+            with_k.z += __shfl_xor_sync(0xffffffffu, with_k.z, 16); with_k.w += __shfl_xor_sync(0xffffffffu, with_k.w, 16);
+            with_q.x += __shfl_xor_sync(0xffffffffu, with_q.x, 16); with_q.y += __shfl_xor_sync(0xffffffffu, with_q.y, 16);
+            with_q.z += __shfl_xor_sync(0xffffffffu, with_q.z, 16); with_q.w += __shfl_xor_sync(0xffffffffu, with_q.w, 16);
+        }
+        if (lane < ACROSS) {
+            *reinterpret_cast<float4*>(&sums[0][warp][at]) = with_k;
+            *reinterpret_cast<float4*>(&sums[1][warp][at]) = with_q;
+        }
+        // lengths and product of q and k: every warp by itself, all in the same order (zeros beyond dim)
+        float kk = 0.f, qq = 0.f, kq = 0.f;
+        {
+#pragma unroll
+            for (int i = 0; i < DIM / 32; ++i) {
+                const float k = ks[turn][lane + 32 * i], q = qs[turn][lane + 32 * i];
+                kk = fmaf(k, k, kk); qq = fmaf(q, q, qq); kq = fmaf(k, q, kq);
+            }
+            kk = warp_sum(kk); qq = warp_sum(qq); kq = warp_sum(kq);
+        }
+        const float k_norm = 1.0f / sqrtf(kk + p.eps);
+        __syncthreads();
+        // S^T k in COLS threads, S^T q in as many others where there are that many
+        constexpr bool HALVES = 2 * DIM >= 2 * COLS;
+        float sum_k = 0.f, sum_q = 0.f;
+        const int c = tid & (COLS - 1);
+        if (tid < COLS) {
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sum_k += sums[0][w][c];
+            us[turn][c] = beta * (v - decay * k_norm * sum_k) * k_norm;          // u times one over the key's length
+        }
+        const bool writes = HALVES ? tid >= COLS && tid < 2 * COLS : tid < COLS;
+        if (writes) {
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) sum_q += sums[1][w][c];
+        }
+        __syncthreads();
+        if (writes && col0 + c < p.vdim)
+            p.out[(size_t)t * p.heads * p.vdim + head * p.vdim + col0 + c] =
+                p.scale / sqrtf(qq + p.eps) * (decay * sum_q + kq * us[turn][c]);
+        const float4 u = *reinterpret_cast<const float4*>(&us[turn][at]);
+#pragma unroll
+        for (int i = 0; i < ROWS; i += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(&ks[turn][row0 + i]);
+            const float kx[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float4& x = s[i + j];
+                x.x = fmaf(kx[j], u.x, decay * x.x); x.y = fmaf(kx[j], u.y, decay * x.y);
+                x.z = fmaf(kx[j], u.z, decay * x.z); x.w = fmaf(kx[j], u.w, decay * x.w);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i)
+        if (in && row0 + i < p.dim) *reinterpret_cast<float4*>(state + (size_t)i * p.vdim) = s[i];
+}
+
 template <typename T>
-static int launch_step(const DeltaParams& p, int items, int early, cudaStream_t stream) {
+static int launch_step(const DeltaParams& p, int items, bool few, int early, cudaStream_t stream) {
     if (p.dim > STEP_MAX_DIM) return ERR_UNSUPPORTED;
     const bool wide = p.vdim % 4 == 0 && p.state_stride % 4 == 0 && (uintptr_t)p.state % 16 == 0 && (uintptr_t)p.out % 16 == 0;
+    // Four requests of 16 heads (64 blocks) take both kernels 6.6 us; fewer blocks leave SMs idle (one request: 6.6 against 5.0).
+    if (few && wide && p.dim <= HEAD_MAX_DIM) {
+        const int across = p.vdim % 128 == 0 || p.vdim % 128 > 64 ? 32 : 16;
+        const dim3 grid((p.vdim + 4 * across - 1) / (4 * across), p.heads, items);
+        if ((long long)grid.x * grid.y * grid.z >= HEAD_FROM && grid.y <= 65535 && grid.z <= 65535)
+            return p.dim <= 64 ? launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 64> : delta_head_kernel<T, 16, 64>,
+                                                     grid, dim3(128), 0, stream, p)
+                               : launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 128> : delta_head_kernel<T, 16, 128>,
+                                                     grid, dim3(256), 0, stream, p);
+    }
     const dim3 grid((p.vdim + STEP_COLS - 1) / STEP_COLS, p.heads, items);
     if (grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
     void (*kernel)(const DeltaParams);
@@ -171,14 +297,14 @@ extern "C" {
 
 int fsie_delta_max_dim() { return STEP_MAX_DIM; }
 
-// `form`: 0 the recurrent form, 1 the chunked one, with a workspace `room` of fsie_delta_chunk_bytes() for every chunk
+// `form`: 0 the recurrent form, 2 the same for steps of about a token per request, 1 the chunked one, with a workspace `room` of fsie_delta_chunk_bytes() for every chunk
 // (of fsie_delta_chunk_tokens() tokens of a request, its last one begun)
 int fsie_delta_rule(int form, const void* qkv, int ld, int q_off, int k_off, int v_off, const float* log_decay, const float* beta,
                     const int* item_qstart, const int* item_qlen, const int* item_slots, int items, float* state,
                     long long state_stride, float* out, int heads, int dim, int vdim, int share, float scale, float eps,
                     int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (items <= 0) return 0;
-    if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 1) return ERR_BAD_ARGUMENT;
+    if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 2) return ERR_BAD_ARGUMENT;
     DeltaParams p;
     p.qkv = qkv; p.ld = ld; p.q_off = q_off; p.k_off = k_off; p.v_off = v_off; p.log_decay = log_decay; p.beta = beta;
     p.item_qstart = item_qstart; p.item_qlen = item_qlen; p.item_slots = item_slots;
@@ -186,7 +312,7 @@ int fsie_delta_rule(int form, const void* qkv, int ld, int q_off, int k_off, int
     p.heads = heads; p.dim = dim; p.vdim = vdim; p.share = share; p.scale = scale; p.eps = eps;
     if (dtype != DTYPE_F32 && dtype != DTYPE_BF16) return ERR_BAD_ARGUMENT;
     if (form == 1) return delta_chunk(p, items, dtype, room, room_bytes, early, stream);
-    return dtype == DTYPE_F32 ? launch_step<float>(p, items, early, stream) : launch_step<bf16>(p, items, early, stream);
+    return dtype == DTYPE_F32 ? launch_step<float>(p, items, form == 2, early, stream) : launch_step<bf16>(p, items, form == 2, early, stream);
 }
 
 }  // extern "C"

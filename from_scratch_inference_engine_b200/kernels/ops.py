@@ -17,6 +17,7 @@ run beside the kernel in front of it).  The functions without the argument (`gem
 from __future__ import annotations
 
 import ctypes
+from array import array
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -2282,7 +2283,7 @@ def stream_norm(x: torch.Tensor, start: Optional[torch.Tensor], delta: Optional[
 
 
 # ------------------------------------------------------------------ the gated delta rule
-_delta = None
+_delta = _delta_sizes = None
 
 
 def delta():
@@ -2291,7 +2292,7 @@ def delta():
     if _delta is None:
         lib = build.load_library("delta")
         i, f, ll, p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
-        lib.fsie_delta_prep.argtypes = [p, i, i, i, i, p, p, p, p, p, i, i, p, ll, ll, p, i, i, p, p, i, p, p, p, i, i, p]
+        lib.fsie_delta_prep.argtypes = [p, i, i, i, i, i, p, p, p, p, p, i, i, p, ll, ll, p, i, i, p, p, i, p, p, p, i, i, p]
         lib.fsie_delta_prep_max_taps.argtypes = []
         lib.fsie_delta_rule.argtypes = [i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, p, ll, i, p]
         lib.fsie_delta_max_dim.argtypes = lib.fsie_delta_chunk_max_dim.argtypes = lib.fsie_delta_chunk_tokens.argtypes = []
@@ -2305,7 +2306,16 @@ def delta():
 
 def delta_max_dim() -> int:
     """State rows per head that the gated delta rule holds."""
-    return int(delta().fsie_delta_max_dim())
+    return _delta_limits()[0]
+
+
+def _delta_limits():
+    """(state rows per head at most, of them in the chunked form, tokens of its chunks)."""
+    global _delta_sizes
+    if _delta_sizes is None:
+        lib = delta()
+        _delta_sizes = (int(lib.fsie_delta_max_dim()), int(lib.fsie_delta_chunk_max_dim()), int(lib.fsie_delta_chunk_tokens()))
+    return _delta_sizes
 
 
 def delta_prep_max_taps() -> int:
@@ -2324,13 +2334,18 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
     first live in the request's slot of `state` [slots, n] (float32) from float tail_off on, oldest first, and are moved on.
     seg_item / seg_row0 (int32): the tiles of `seg_tokens` tokens (at least taps - 1), listed request by request.
     `early`: see the module's first lines; the slots are read behind the wait."""
-    _need(proj, None, "proj")
-    _need(act, proj.dtype, "act")
-    for name, t in (("conv_wt", conv_wt), ("a_log", a_log), ("dt_bias", dt_bias), ("log_decay", log_decay), ("beta", beta)):
-        _need(t, torch.float32, name)
-    for name, t in (("item_qstart", item_qstart), ("item_qlen", item_qlen), ("item_slots", item_slots),
-                    ("seg_item", seg_item), ("seg_row0", seg_row0)):
-        _need(t, torch.int32, name)
+    f32, i32 = torch.float32, torch.int32
+    if not (_fits(proj, None, True) and _fits(act, proj.dtype, True) and _fits(conv_wt, f32, True) and _fits(a_log, f32, True)
+            and _fits(dt_bias, f32, True) and _fits(log_decay, f32, True) and _fits(beta, f32, True)
+            and _fits(item_qstart, i32, True) and _fits(item_qlen, i32, True) and _fits(item_slots, i32, True)
+            and _fits(seg_item, i32, True) and _fits(seg_row0, i32, True)):
+        _need(proj, None, "proj")
+        _need(act, proj.dtype, "act")
+        for name, t in (("conv_wt", conv_wt), ("a_log", a_log), ("dt_bias", dt_bias), ("log_decay", log_decay), ("beta", beta)):
+            _need(t, f32, name)
+        for name, t in (("item_qstart", item_qstart), ("item_qlen", item_qlen), ("item_slots", item_slots),
+                        ("seg_item", seg_item), ("seg_row0", seg_row0)):
+            _need(t, i32, name)
     tokens, ld = proj.shape
     taps, channels = conv_wt.shape
     heads = a_log.numel()
@@ -2345,7 +2360,7 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
         stride = state.stride(0)
         if tail_off + (taps - 1) * channels > stride:
             raise KernelError("delta_prep: the state slots do not hold the convolution's inputs")
-    _check(delta().fsie_delta_prep(proj, ld, conv_off, a_off, b_off, item_qstart, item_qlen, item_slots, seg_item, seg_row0,
+    _check(delta().fsie_delta_prep(proj, tokens, ld, conv_off, a_off, b_off, item_qstart, item_qlen, item_slots, seg_item, seg_row0,
                                    num_segs, seg_tokens, state, stride, tail_off, conv_wt, taps, channels, a_log, dt_bias,
                                    heads, act, log_decay, beta, _tag(proj.dtype), int(early), _stream()), "delta_prep")
 
@@ -2369,12 +2384,16 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     negative slot is passed over, its rows of `out` stay as they are.  `scale`: dim ** -0.5 unless given.  `longest`: the
     tokens of the step's longest request, which choose the kernel (0: not known to the caller).  dim is 256 at most.
     `early`: the state and the lists are older than the stream's last kernel, see the module's first lines."""
-    _need(qkv, None, "qkv")
-    for name, t in (("log_decay", log_decay), ("beta", beta), ("out", out)):
-        _need(t, torch.float32, name)
-    _need(state, torch.float32, "state", contiguous=False)
-    for name, t in (("item_qstart", item_qstart), ("item_qlen", item_qlen), ("item_slots", item_slots)):
-        _need(t, torch.int32, name)
+    f32, i32 = torch.float32, torch.int32
+    if not (_fits(qkv, None, True) and _fits(log_decay, f32, True) and _fits(beta, f32, True) and _fits(out, f32, True)
+            and _fits(state, f32, False) and _fits(item_qstart, i32, True) and _fits(item_qlen, i32, True)
+            and _fits(item_slots, i32, True)):
+        _need(qkv, None, "qkv")
+        for name, t in (("log_decay", log_decay), ("beta", beta), ("out", out)):
+            _need(t, f32, name)
+        _need(state, f32, "state", contiguous=False)
+        for name, t in (("item_qstart", item_qstart), ("item_qlen", item_qlen), ("item_slots", item_slots)):
+            _need(t, i32, name)
     tokens, ld = qkv.shape
     if min(heads, dim, vdim, share) <= 0 or heads % share:
         raise KernelError("gated_delta_rule: sizes must be positive and heads a multiple of share")
@@ -2384,20 +2403,22 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     if min(log_decay.numel(), beta.numel()) < tokens * heads or out.numel() < tokens * heads * vdim:
         raise KernelError("gated_delta_rule: log_decay, beta or out is too small")
     stride = state.stride(0)
-    if stride < heads * dim * vdim or state[0].numel() < heads * dim * vdim or not state[0].is_contiguous():
+    if stride < heads * dim * vdim or (not state.is_contiguous() and not (
+            state.shape[0] and state[0].is_contiguous() and state[0].numel() >= heads * dim * vdim)):
         raise KernelError("gated_delta_rule: the state slots do not hold the heads' matrices")
     if min(item_qstart.numel(), item_qlen.numel(), item_slots.numel()) < items:
         raise KernelError("gated_delta_rule: the lists are shorter than the requests")
     if not eps > 0:
         raise KernelError("gated_delta_rule: eps must be positive")
-    if dim > delta_max_dim():
-        raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {delta_max_dim()}")
+    most, chunked_most, chunk = _delta_limits()
+    if dim > most:
+        raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {most}")
     lib, tag, room = delta(), _tag(qkv.dtype), None
-    chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= lib.fsie_delta_chunk_max_dim()
+    chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= chunked_most
     if chunked:
-        chunks = tokens // lib.fsie_delta_chunk_tokens() + items
+        chunks = tokens // chunk + items
         room = torch.empty(chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag), dtype=torch.uint8, device=qkv.device)
-    _check(lib.fsie_delta_rule(int(chunked), qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
+    _check(lib.fsie_delta_rule(1 if chunked else 2 if longest == 1 or tokens == items else 0, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
                                items, state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
                                float(eps), tag, room, 0 if room is None else room.numel(), int(early), _stream()),
            "gated_delta_rule")
@@ -2406,6 +2427,9 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
 
 # ------------------------------------------------------------------ copies inside pools of blocks
 _blocks = None
+
+
+COPY_MAX_BUFFERS = 64      # buffers that one launch takes
 
 
 def blocks_lib():
@@ -2417,6 +2441,8 @@ def blocks_lib():
         lib.fsie_copy_blocks.argtypes = [p, i, ll, i, p, i, p, p]
         lib.fsie_copy_max_buffers.argtypes = []
         lib.fsie_copy_blocks.restype = lib.fsie_copy_max_buffers.restype = i
+        if lib.fsie_copy_max_buffers() != COPY_MAX_BUFFERS:
+            raise KernelError("copy_blocks: the library takes another number of buffers")
         _blocks = build.fast_calls(lib)
     return _blocks
 
@@ -2426,27 +2452,28 @@ def copy_blocks(buffers, moves: torch.Tensor, error: torch.Tensor) -> None:
     device).  The buffers are contiguous, of any types, with equally many blocks (their first dimension) of equally many
     bytes.  No block may be a destination twice, or a source and a destination: all pairs are copied side by side.  A pair
     outside the pool is left out and sets error[0] (int32)."""
-    _need(moves, torch.int32, "moves")
-    _need(error, torch.int32, "error")
+    if not (_fits(moves, torch.int32, True) and _fits(error, torch.int32, True)):
+        _need(moves, torch.int32, "moves")
+        _need(error, torch.int32, "error")
     if moves.dim() != 2 or moves.shape[1] != 2:
         raise KernelError("copy_blocks: moves must be [n, 2]")
-    buffers = list(buffers)
-    if not buffers:
-        return
-    blocks, size = None, None
+    bases = array("q")
+    blocks = size = None
     for buffer in buffers:
-        _need(buffer, None, "buffers")
+        if not _fits(buffer, None, True):
+            _need(buffer, None, "buffers")
         if buffer.dim() < 1:
             raise KernelError("copy_blocks: a buffer needs a dimension of blocks")
-        mine = (buffer.shape[0], buffer.numel() // max(1, buffer.shape[0]) * buffer.element_size())
+        count = buffer.shape[0]
+        mine = buffer.numel() // max(1, count) * buffer.element_size()
         if blocks is None:
-            blocks, size = mine
-        elif mine != (blocks, size):
+            blocks, size = count, mine
+        elif count != blocks or mine != size:
             raise KernelError("copy_blocks: the buffers differ in blocks or bytes per block")
-    lib = blocks_lib()
-    most = lib.fsie_copy_max_buffers()
-    for first in range(0, len(buffers), most):
-        part = buffers[first:first + most]
-        bases = (ctypes.c_longlong * len(part))(*[b.data_ptr() for b in part])
-        _check(lib.fsie_copy_blocks(ctypes.addressof(bases), len(part), size, blocks, moves, moves.shape[0], error, _stream()),
-               "copy_blocks")
+        bases.append(buffer.data_ptr())
+    if blocks is None:
+        return
+    lib, address, pairs = blocks_lib(), bases.buffer_info()[0], moves.shape[0]
+    for first in range(0, len(bases), COPY_MAX_BUFFERS):
+        _check(lib.fsie_copy_blocks(address + 8 * first, min(COPY_MAX_BUFFERS, len(bases) - first), size, blocks, moves, pairs,
+                                    error, _stream()), "copy_blocks")
