@@ -74,6 +74,16 @@ __device__ __forceinline__ void dc_mma(float (&d)[4], const unsigned (&a)[4], un
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d = a * b: the first of a sum
+__device__ __forceinline__ void dc_mma0(float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void dc_mma_if(bool first, float (&d)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
+    if (first) dc_mma0(d, a, b0, b1);
+    else dc_mma(d, a, b0, b1);
+}
 __device__ __forceinline__ void dc_sync(int barrier, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(barrier), "r"(threads) : "memory");
 }
@@ -194,6 +204,7 @@ struct DcShape : DcRecord<T, DK> {
     static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 0);         // row of v; bfloat16: v_piece()
     static constexpr int OLD = COLS + 4;                       // padded row of outputs
     static constexpr int THREADS = 32 * DC_WALKERS + DC_FETCHERS;
+    static constexpr int WRITES = DC_TOKENS * COLS / 4 / DC_FETCHERS;       // rows of four outputs that a fetching thread writes
     static constexpr int FINISH = SLICES > 1 ? DC_TILES / 2 : DC_TILES;     // tiles of eight tokens whose outputs a warp finishes
     // Place of a row's 16-byte piece of bfloat16 v: in another order in every row, ldmatrix without bank conflicts.
     static __device__ __forceinline__ int v_piece(int row, int piece) { return piece ^ (COLS == 32 ? (row >> 1) & 3 : row & 7); }
@@ -201,7 +212,8 @@ struct DcShape : DcRecord<T, DK> {
     struct Shared {
         Stage stage[DC_STAGES];
         float4 swap[2][SLICES > 1 ? DC_WALKERS : 1][DC_TILES][32];      // S0^T k of a warp's rows
-        float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs, of two warps per 16 columns two summands
+        float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs without the factors; of two warps per 16 columns two summands
+        float back[2][COLS];                       // what its columns are still to be multiplied by
         float most[DC_WALKERS][16];
     };
 };
@@ -578,22 +590,27 @@ struct DcFetch {
     }
 };
 
-// The fetching threads also write outputs: `tokens` rows of a chunk's, from `to` on, whole lines side by side.
+// The fetching threads also write outputs, whole lines side by side: `tokens` rows of a chunk's, from `to` on, the walkers' summands
+// times the column's and the token's factor (`queries`, from the chunk's record).
 template <typename T, int DK>
-__device__ __forceinline__ void dc_write(const float (&from)[DcShape<T, DK>::SLICES][DC_TOKENS][DcShape<T, DK>::OLD], float* to,
-                                         size_t width, int tokens, int columns, bool wide) {
+__device__ __forceinline__ void dc_write(const float (&from)[DcShape<T, DK>::SLICES][DC_TOKENS][DcShape<T, DK>::OLD], const float* back,
+                                         const float (&queries)[DcShape<T, DK>::WRITES], float* to, size_t width, int tokens, int columns, bool wide) {
     using Sh = DcShape<T, DK>;
     constexpr int FOURS = Sh::COLS / 4, AT_ONCE = DC_FETCHERS / FOURS;
     const int tid = threadIdx.x - 32 * DC_WALKERS, d = (tid % FOURS) * 4;
+    if (d >= columns) return;
+    const float4 b = *reinterpret_cast<const float4*>(back + d);
 #pragma unroll
     for (int i = 0; i < DC_TOKENS / AT_ONCE; ++i) {
         const int r = tid / FOURS + i * AT_ONCE;
-        if (r >= tokens || d >= columns) continue;
+        if (r >= tokens) continue;
+        const float query = queries[i];
         float4 o = *reinterpret_cast<const float4*>(&from[0][r][d]);
         if (Sh::SLICES > 1) {
             const float4 x = *reinterpret_cast<const float4*>(&from[Sh::SLICES - 1][r][d]);
             o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
         }
+        o = make_float4(o.x * b.x * query, o.y * b.y * query, o.z * b.z * query, o.w * b.w * query);
         float* at = to + (size_t)r * width + d;
         if (wide && d + 4 <= columns) {
             *reinterpret_cast<float4*>(at) = o;
@@ -632,18 +649,14 @@ template <> struct DcValues<float> {
 __device__ __forceinline__ void dc_solve(float (&u)[DC_TILES][4], const unsigned (&rh)[2][4], const unsigned (&rl)[2][4],
                                          const unsigned (&th)[3][4], const unsigned (&tl)[3][4]) {
     float low[DC_TILES][4];
-#pragma unroll
-    for (int j = 0; j < DC_TILES; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) u[j][e] = low[j][e] = 0.f;
     // (tile after tile, so that no sum waits for its own last instruction)
 #pragma unroll
     for (int b = 0; b < 3; ++b) {
         const int block = b == 0 ? 1 : b == 1 ? 0 : 2, in = block == 2, to = 2 * (block > 0);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            dc_mma(low[to + j], rl[in], th[block][2 * j], th[block][2 * j + 1]);
-            dc_mma(u[to + j], rh[in], th[block][2 * j], th[block][2 * j + 1]);
+            dc_mma_if(block < 2, low[to + j], rl[in], th[block][2 * j], th[block][2 * j + 1]);
+            dc_mma_if(block < 2, u[to + j], rh[in], th[block][2 * j], th[block][2 * j + 1]);
         }
 #pragma unroll
         for (int j = 0; j < 2; ++j) dc_mma(low[to + j], rh[in], tl[block][2 * j], tl[block][2 * j + 1]);
@@ -700,17 +713,24 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         const size_t width = (size_t)p.heads * p.vdim;
         float* out = p.out + (size_t)t0 * width + (size_t)head * p.vdim + col0;
         const bool wide = p.vdim % 4 == 0 && (uintptr_t)p.out % 16 == 0;
+        const float* queries = (reinterpret_cast<const typename Sh::Gates*>(records.gates) + (size_t)chunk0 * p.heads + head)->query;
         fetch.next(p, sm.stage[0]);
         fetch.next(p, sm.stage[1]);
         asm volatile("cp.async.wait_group 1;\n" ::: "memory");
         dc_sync(DC_MEET, Sh::THREADS);                         // chunk 0 is there
         for (int c = 1; c <= chunks + 1; ++c) {                // (the last meetings are for chunks that are not there)
+            float query[Sh::WRITES];                           // of the chunk that is written next
+            if (c >= 2) {
+#pragma unroll
+                for (int i = 0; i < Sh::WRITES; ++i) query[i] = queries[(threadIdx.x - 32 * DC_WALKERS) / (Sh::COLS / 4) + i * (DC_TOKENS / Sh::WRITES)];
+                queries += (size_t)p.heads * (sizeof(typename Sh::Gates) / sizeof(float));
+            }
             asm volatile("cp.async.wait_group 0;\n" ::: "memory");
             dc_sync(DC_MEET, Sh::THREADS);                     // chunk c is there, and everybody is through with chunk c - 2:
             if (c <= chunks) dc_sync(DC_GO, Sh::THREADS);      // (copies asked for at once would delay what the walkers swap)
             fetch.next(p, sm.stage[(c + 1) % DC_STAGES]);      // its stage takes chunk c + 1
             if (c >= 2) {
-                dc_write<T, DK>(sm.out[c & 1], out, width, count - (c - 2) * DC_TOKENS, p.vdim - col0, wide);
+                dc_write<T, DK>(sm.out[c & 1], sm.back[c & 1], query, out, width, count - (c - 2) * DC_TOKENS, p.vdim - col0, wide);
                 out += DC_TOKENS * width;
             }
         }
@@ -739,7 +759,9 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);    // ... and [k][n]
     const int b_piece = dc_piece(lane & 7, (lane >> 3) & 1);   // ... of a 16 x 16 block
     // Two warps per 16 columns: the first finishes the outputs of token tiles 0 and 3, the second of 1 and 2 (tiles 2 and 3 have
-    // two blocks of weights).  One warp: all four.
+    // two blocks of weights).  S0^T q has the second's tiles in the order 1, 0, 3, 2, so that a warp's own are its first and last.
+    // One warp: all four.
+    const int q_row = (lane & 7) + 8 * ((lane >> 4) ^ (SLICES > 1 ? slice : 0));
     auto tile_of = [&](int j) { return SLICES > 1 ? (j == 0 ? slice : 3 - slice) : j; };
     // Operands of the next products are read well ahead of them, and sums that do not depend on one another are asked for
     // together: a warp has its scheduler nearly to itself, so what one instruction waits for, all wait for.
@@ -773,22 +795,22 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         const auto& st = sm.stage[stage];
         bool look = c % DC_REFRESH == 0, spoiled = false;
         int bad[2] = {DC_TOKENS, DC_TOKENS};
-        float u[DC_TILES][4], wq[DC_TILES][4];                 // U, S0^T q
+        float u[DC_TILES][4], wq[DC_TILES][4];                 // U; S0^T q
         unsigned bq[2][4];                                     // Q
         unsigned sh[STEPS][4], sl[STEPS][4];                   // the state in two parts
         auto ask_query = [&](int k) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][16 * m + b_row][row0 + 16 * k + b_col]);
+            for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][16 * m + q_row][row0 + 16 * k + b_col]);
         };
         // a quarter of the instructions of S0^T q: they stand where the chain of R, U and the new state has to wait
         auto query_step = [&](int k) {
 #pragma unroll
-            for (int j = 0; j < DC_TILES; ++j) dc_mma(wq[j], sl[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+            for (int j = 0; j < DC_TILES; ++j) dc_mma_if(k == 0, wq[j], sl[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
             if (PARTS == 2) {
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     unsigned b[4];
-                    dc_ldmatrix(b, &st.keys.q[PARTS - 1][16 * m + b_row][row0 + 16 * k + b_col]);
+                    dc_ldmatrix(b, &st.keys.q[PARTS - 1][16 * m + q_row][row0 + 16 * k + b_col]);
                     dc_mma(wq[2 * m], sh[k], b[0], b[1]);
                     dc_mma(wq[2 * m + 1], sh[k], b[2], b[3]);
                 }
@@ -834,18 +856,14 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             }
             // ---- S0^T k of the warp's rows: 16 columns x 32 tokens; the next rows are taken apart meanwhile
             float wk[DC_TILES][4], lk[DC_TILES][4];
-#pragma unroll
-            for (int j = 0; j < DC_TILES; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) wk[j][e] = lk[j][e] = wq[j][e] = 0.f;
             dc_split_tiles(s[0], s[1], sh[0], sl[0]);
 #pragma unroll
             for (int k = 0; k < STEPS; ++k) {
                 if (k + 1 < STEPS) ask_keys(st, k + 1);
 #pragma unroll
                 for (int j = 0; j < DC_TILES; ++j) {
-                    dc_mma(wk[j], sh[k], bk[k & 1][j >> 1][2 * (j & 1)], bk[k & 1][j >> 1][2 * (j & 1) + 1]);
-                    dc_mma(lk[j], sl[k], bk[k & 1][j >> 1][2 * (j & 1)], bk[k & 1][j >> 1][2 * (j & 1) + 1]);
+                    dc_mma_if(k == 0, wk[j], sh[k], bk[k & 1][j >> 1][2 * (j & 1)], bk[k & 1][j >> 1][2 * (j & 1) + 1]);
+                    dc_mma_if(k == 0, lk[j], sl[k], bk[k & 1][j >> 1][2 * (j & 1)], bk[k & 1][j >> 1][2 * (j & 1) + 1]);
                 }
                 if (k + 1 < STEPS) dc_split_tiles(s[2 * k + 2], s[2 * k + 3], sh[(k + 1) % STEPS], sl[(k + 1) % STEPS]);
                 if (PARTS == 2) {
@@ -946,13 +964,9 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             dc_split_tiles(faded[0], faded[1], uh[m], ul[m]);
         }
 #pragma unroll
-        for (int n = 0; n < TILES; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) add[n][e] = 0.f;
-#pragma unroll
         for (int m = 0; m < 2; ++m) {                          // tokens 16 m on
 #pragma unroll
-            for (int n = 0; n < TILES; ++n) dc_mma(add[n], ul[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+            for (int n = 0; n < TILES; ++n) dc_mma_if(m == 0, add[n], ul[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
             if (PARTS == 2) {
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
@@ -971,8 +985,10 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
         // ---- outputs: the chunk's start and its own tokens; the fetching warps add up what two warps have of S0^T q and write them
         unsigned zh[2][4], zl[2][4], w[FINISH][2][4];          // U again, weights: high and low part, two inner halves each
+        float2 fade[FINISH];
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
+            fade[j] = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile_of(j) + 2 * t]);
             const bool second = SLICES > 1 ? j == 1 : j >= 2;  // the tile's tokens are in the chunk's second half
 #pragma unroll
             for (int m = 0; m <= (second ? 1 : 0); ++m)
@@ -983,11 +999,12 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         float oa[FINISH][4], ob[FINISH][4];
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
+            const float(&own)[4] = wq[SLICES > 1 ? 3 * j : j];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) oa[j][e] = ob[j][e] = 0.f;
+            for (int h = 0; h < 2; ++h) dc_mul2(oa[j][2 * h], oa[j][2 * h + 1], own[2 * h], own[2 * h + 1], fade[j].x, fade[j].y);
 #pragma unroll
             for (int m = 0; m <= ((SLICES > 1 ? j == 1 : j >= 2) ? 1 : 0); ++m) {
-                dc_mma(ob[j], zl[m], w[j][m][0], w[j][m][1]);
+                dc_mma_if(m == 0, ob[j], zl[m], w[j][m][0], w[j][m][1]);
                 dc_mma(oa[j], zh[m], w[j][m][0], w[j][m][1]);
                 dc_mma(ob[j], zh[m], w[j][m][2], w[j][m][3]);
             }
@@ -998,50 +1015,37 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
             for (int e = 0; e < 4; e += 2)
                 dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
-        auto leave = [&](int which, int tile, const float4& o) {
+        auto leave = [&](int which, int tile, const float (&o)[4]) {
             float* to = &sm.out[c & 1][which][8 * tile + 2 * t][group * 16 + g];
-            to[0] = o.x; to[8] = o.z; to[Sh::OLD] = o.y; to[Sh::OLD + 8] = o.w;
-        };
-        // all that belongs to a token is multiplied by its factors, also what the other warp adds up
-        auto scaled = [&](const float (&x)[4], int tile, float2& query) {
-            const float2 fade = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile + 2 * t]);
-            query = *reinterpret_cast<const float2*>(&st.gates.query[8 * tile + 2 * t]);
-            float fx, fy;
-            float4 o;
-            dc_mul2(fx, fy, query.x, query.y, fade.x, fade.y);
-            dc_mul2(o.x, o.y, x[0], x[1], fx * back[0], fy * back[0]);
-            dc_mul2(o.z, o.w, x[2], x[3], fx * back[1], fy * back[1]);
-            return o;
+            to[0] = o[0]; to[8] = o[2]; to[Sh::OLD] = o[1]; to[Sh::OLD + 8] = o[3];
         };
         if constexpr (SLICES > 1) {
 #pragma unroll
-            for (int j = 0; j < FINISH; ++j) {                 // the other warp's tiles
-                const float(&x)[4] = j == 0 ? wq[0] : wq[3], (&y)[4] = j == 0 ? wq[1] : wq[2];
-                const float z[4] = {slice ? x[0] : y[0], slice ? x[1] : y[1], slice ? x[2] : y[2], slice ? x[3] : y[3]};
-                float2 query;
-                const int tile = j == 0 ? 1 - slice : 2 + slice;
-                leave(SLICES - 1, tile, scaled(z, tile, query));
+            for (int j = 1; j < 3; ++j) {                      // the other warp's tiles
+                const int tile = j ^ slice;
+                const float2 f = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile + 2 * t]);
+                float o[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) dc_mul2(o[2 * h], o[2 * h + 1], wq[j][2 * h], wq[j][2 * h + 1], f.x, f.y);
+                leave(SLICES - 1, tile, o);
             }
         }
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
-            const int tile = tile_of(j), first = 8 * tile + 2 * t;
-            float x[4];
+            const int tile = tile_of(j);
+            float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                x[e] = SLICES == 1 ? wq[j][e] : j == 0 ? (slice ? wq[1][e] : wq[0][e]) : (slice ? wq[2][e] : wq[3][e]);
-            float2 query;
-            float4 o = scaled(x, tile, query);
-            dc_fma2(o.x, o.y, oa[j][0] + ob[j][0], oa[j][1] + ob[j][1], query.x * back[0], query.y * back[0], o.x, o.y);
-            dc_fma2(o.z, o.w, oa[j][2] + ob[j][2], oa[j][3] + ob[j][3], query.x * back[1], query.y * back[1], o.z, o.w);
+            for (int h = 0; h < 2; ++h) dc_add2(o[2 * h], o[2 * h + 1], oa[j][2 * h], oa[j][2 * h + 1], ob[j][2 * h], ob[j][2 * h + 1]);
             if (__builtin_expect(spoiled, 0)) {
-                const float nan = __int_as_float(0x7fffffff);
-                if (first >= bad[0]) o.x = nan;
-                if (first + 1 >= bad[0]) o.y = nan;
-                if (first >= bad[1]) o.z = nan;
-                if (first + 1 >= bad[1]) o.w = nan;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (8 * tile + 2 * t + (e & 1) >= bad[e >> 1]) o[e] = __int_as_float(0x7fffffff);
             }
             leave(0, tile, o);
+        }
+        if (slice == 0 && t == 0) {                            // (one over sigma as this chunk had it)
+            sm.back[c & 1][group * 16 + g] = back[0];
+            sm.back[c & 1][group * 16 + g + 8] = back[1];
         }
         if (__builtin_expect(spoiled, 0)) {
 #pragma unroll
