@@ -220,15 +220,24 @@ struct DcShape : DcRecord<T, DK> {
 
 // What the two kernels share beside the rule's arguments: the records, [chunk][q/k head] and [chunk][head].  Chunks are
 // numbered request after request, those of a request from its first token on; `chunks` is what the workspace has room for.
-struct DcRecords { unsigned char* keys; unsigned char* gates; int items, chunks; };
+struct DcRecords { unsigned char* keys; unsigned char* gates; int items, longer, chunks; };    // longer: a bound of the requests that have chunks
 
-// The number of chunks in front of request `item`, by all lanes of a warp.
-__device__ __forceinline__ int dc_chunks_before(const int* __restrict__ item_qlen, int item, int lane) {
-    int sum = 0;
-    for (int i = lane; i < item; i += 32) sum += (max(item_qlen[i], 0) + DC_TOKENS - 1) / DC_TOKENS;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    return sum;
+// A request's chunks; none for those of less than `least` tokens.
+__device__ __forceinline__ int dc_chunks(int tokens, int least) { return tokens < least ? 0 : (tokens + DC_TOKENS - 1) / DC_TOKENS; }
+
+// The request that is the `rank`-th with chunks, -1 if there are not so many, and the chunks in front of it; by all lanes of a warp.
+__device__ __forceinline__ int dc_find(const int* __restrict__ item_qlen, int items, int rank, int least, int lane, int& before) {
+    before = 0;
+    for (int i0 = 0; i0 < items; i0 += 32) {
+        const int have = i0 + lane < items ? dc_chunks(item_qlen[i0 + lane], least) : 0;
+        const unsigned with = __ballot_sync(0xffffffffu, have > 0);
+        const unsigned here = __ballot_sync(0xffffffffu, have > 0 && __popc(with & ((1u << lane) - 1)) == rank);
+        const int at = here ? __ffs(here) - 1 : 32;
+        before += __reduce_add_sync(0xffffffffu, lane < at ? have : 0);
+        if (here) return i0 + at;
+        rank -= __popc(with);
+    }
+    return -1;
 }
 
 // A product of two 16 x 16 matrices in two parts each: sum += a b, b's operand registers as ldmatrix gives them.
@@ -283,7 +292,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
     // the chunk's request and first token: 32 requests at a time
     int item = -1, place = 0;
     for (int i0 = 0, before = 0; i0 < records.items && item < 0; i0 += 32) {
-        const int i = i0 + lane, have = i < records.items ? (max(p.item_qlen[i], 0) + DC_TOKENS - 1) / DC_TOKENS : 0;
+        const int i = i0 + lane, have = i < records.items ? dc_chunks(p.item_qlen[i], p.least) : 0;
         int upto = have;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -697,13 +706,17 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16, FINISH = Sh::FINISH;
     extern __shared__ __align__(16) unsigned char dc_raw[];
     auto& sm = *reinterpret_cast<typename Sh::Shared*>(dc_raw);
-    const int head = blockIdx.y, item = blockIdx.z, col0 = blockIdx.x * Sh::COLS;
+    const int head = blockIdx.y, col0 = blockIdx.x * Sh::COLS;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
-    if (slot < 0 || count <= 0) return;                        // a padding entry of a fixed-size batch
-    const int chunks = (count + DC_TOKENS - 1) / DC_TOKENS;
-    const int chunk0 = dc_chunks_before(p.item_qlen, item, lane);
-    if (chunk0 + chunks > records.chunks) return;              // lists that name more tokens than there are
+    int chunk0;                                                // the request's first
+    const int item = dc_find(p.item_qlen, records.items, blockIdx.z, p.least, lane, chunk0);
+    const int slot = item < 0 ? -1 : p.item_slots[item], count = item < 0 ? 0 : p.item_qlen[item], t0 = item < 0 ? 0 : p.item_qstart[item];
+    const int chunks = dc_chunks(count, p.least);
+    // fewer requests than blocks, a padding entry of a fixed-size batch, or lists that name more tokens than there are
+    if (slot < 0 || chunk0 > records.chunks - chunks) {
+        grid_dependency_wait();
+        return;
+    }
     // registers (bfloat16): two blocks of 256 threads have 128 each; the walking warps take over some of the fetching ones' (216 + 40)
     if (warp >= DC_WALKERS) {
         if (sizeof(T) == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
@@ -1086,7 +1099,7 @@ static int launch_chunk(const DeltaParams& p, const DcRecords& records, int earl
         sms = count;
     }
     const long long units = (long long)records.chunks * (p.heads / p.share);
-    const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.items);
+    const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.longer);
     if (units > 0x7fffffffLL || grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
     const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32 * DC_MAKERS), sizeof(DcMaker<T, DK>), stream, p, records);
     if (rc != 0) return rc;
@@ -1098,11 +1111,12 @@ static int launch_chunk(const DeltaParams& p, const DcRecords& records, int earl
 }
 
 template <typename T, int DK>
-static int launch_chunk_any(const DeltaParams& p, int items, long long chunks, unsigned char* room, int early, cudaStream_t stream) {
+static int launch_chunk_any(const DeltaParams& p, int items, int longer, long long chunks, unsigned char* room, int early, cudaStream_t stream) {
     DcRecords records;
     records.keys = room;
     records.gates = room + (size_t)chunks * (p.heads / p.share) * sizeof(typename DcRecord<T, DK>::Keys);
     records.items = items;
+    records.longer = longer;
     records.chunks = (int)chunks;
     const bool wide = p.ld % 8 == 0 && p.q_off % 8 == 0 && p.k_off % 8 == 0 && p.v_off % 8 == 0 && p.dim % 8 == 0 &&
                       p.vdim % 8 == 0 && (uintptr_t)p.qkv % 16 == 0;
@@ -1115,17 +1129,18 @@ static long long chunk_bytes(int heads, int share, int dim, int dtype) {
     return gates + narrow * (dim <= 64 ? sizeof(DcRecord<bf16, 64>::Keys) : sizeof(DcRecord<bf16, 128>::Keys));
 }
 
-// The chunked form; ERR_UNSUPPORTED where a head has more rows than it holds.  `room`: 16-byte aligned memory.
-int delta_chunk(const DeltaParams& p, int items, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
+// The chunked form; ERR_UNSUPPORTED where a head has more rows than it holds.  `longer`: at most so many requests are of p.least tokens
+// or more; `room`: 16-byte aligned memory.
+int delta_chunk(const DeltaParams& p, int items, int longer, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (p.dim > DC_MAX_DIM) return ERR_UNSUPPORTED;
     const long long chunks = room_bytes / chunk_bytes(p.heads, p.share, p.dim, dtype);
     if (!room || (uintptr_t)room % 16 != 0 || chunks <= 0 || chunks > 0x7fffffffLL) return ERR_BAD_ARGUMENT;
     unsigned char* at = (unsigned char*)room;
     if (dtype == DTYPE_F32)
-        return p.dim <= 64 ? launch_chunk_any<float, 64>(p, items, chunks, at, early, stream)
-                           : launch_chunk_any<float, 128>(p, items, chunks, at, early, stream);
-    return p.dim <= 64 ? launch_chunk_any<bf16, 64>(p, items, chunks, at, early, stream)
-                       : launch_chunk_any<bf16, 128>(p, items, chunks, at, early, stream);
+        return p.dim <= 64 ? launch_chunk_any<float, 64>(p, items, longer, chunks, at, early, stream)
+                           : launch_chunk_any<float, 128>(p, items, longer, chunks, at, early, stream);
+    return p.dim <= 64 ? launch_chunk_any<bf16, 64>(p, items, longer, chunks, at, early, stream)
+                       : launch_chunk_any<bf16, 128>(p, items, longer, chunks, at, early, stream);
 }
 
 }  // namespace fsie

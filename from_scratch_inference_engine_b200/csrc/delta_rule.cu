@@ -11,6 +11,7 @@
 // This file: the recurrent form, for steps of few tokens per request and for any sizes.  delta_chunk.cu: the chunked form.
 #include "common.cuh"
 #include "delta_rule.cuh"
+#include <limits.h>
 #include <math.h>
 
 namespace fsie {
@@ -52,7 +53,10 @@ delta_step_kernel(const DeltaParams p) {
     const int head = blockIdx.y, item = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
-    if (slot < 0 || count <= 0) return;                    // a padding entry of a fixed-size batch
+    if (slot < 0 || count < p.least || count > p.most) {   // a padding entry of a fixed-size batch, or the other form's
+        grid_dependency_wait();
+        return;
+    }
     const int group = tid / ACROSS, at = (tid % ACROSS) * V, col = blockIdx.x * STEP_COLS + at;
     const bool in = col < p.vdim;
     float* state = p.state + (size_t)slot * p.state_stride + (size_t)head * p.dim * p.vdim + col;
@@ -64,8 +68,10 @@ delta_step_kernel(const DeltaParams p) {
         for (int x = 0; x < V; ++x) s[i].v[x] = 0.f;
         if (in && r < p.dim) s[i] = load_cols(state + (size_t)r * p.vdim, Cols<V>());
     }
-    grid_dependency_wait();
-    grid_dependents_go();
+    if (!p.beside) {
+        grid_dependency_wait();
+        grid_dependents_go();
+    }
     const T* row = (const T*)p.qkv + (size_t)t0 * p.ld;
     const int narrow = head / p.share * p.dim;
     // a thread's part of the next token's q and k (dim is 256 at most, one number of each per thread)
@@ -147,6 +153,7 @@ delta_step_kernel(const DeltaParams p) {
         const int r = group + i * GROUPS;
         if (in && r < p.dim) store_cols(state + (size_t)r * p.vdim, s[i]);
     }
+    if (p.beside) grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------------------------------------- many decoded tokens
@@ -169,7 +176,10 @@ delta_head_kernel(const DeltaParams p) {
     const int head = blockIdx.y, item = blockIdx.z, col0 = blockIdx.x * COLS;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
-    if (slot < 0 || count <= 0) return;                    // a padding entry of a fixed-size batch
+    if (slot < 0 || count < p.least || count > p.most) {   // a padding entry of a fixed-size batch, or the other form's
+        grid_dependency_wait();
+        return;
+    }
     const int row0 = tid / ACROSS * ROWS, at = (tid % ACROSS) * 4;     // the thread's rows and columns
     const bool in = col0 + at < p.vdim;
     float* state = p.state + (size_t)slot * p.state_stride + ((size_t)head * p.dim + row0) * p.vdim + col0 + at;
@@ -177,8 +187,10 @@ delta_head_kernel(const DeltaParams p) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
         s[i] = in && row0 + i < p.dim ? *reinterpret_cast<const float4*>(state + (size_t)i * p.vdim) : make_float4(0.f, 0.f, 0.f, 0.f);
-    grid_dependency_wait();
-    grid_dependents_go();
+    if (!p.beside) {
+        grid_dependency_wait();
+        grid_dependents_go();
+    }
     // k by the first half of the threads, q by the other; v by the threads that sum up S^T k, later
     const int d = tid & (DIM - 1), narrow = head / p.share * p.dim;
     const T* row = (const T*)p.qkv + (size_t)t0 * p.ld;
@@ -262,6 +274,7 @@ delta_head_kernel(const DeltaParams p) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
         if (in && row0 + i < p.dim) *reinterpret_cast<float4*>(state + (size_t)i * p.vdim) = s[i];
+    if (p.beside) grid_dependency_wait();
 }
 
 template <typename T>
@@ -287,7 +300,7 @@ static int launch_step(const DeltaParams& p, int items, bool few, int early, cud
 }
 
 // delta_chunk.cu
-int delta_chunk(const DeltaParams& p, int items, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream);
+int delta_chunk(const DeltaParams& p, int items, int longer, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream);
 
 }  // namespace fsie
 
@@ -297,22 +310,31 @@ extern "C" {
 
 int fsie_delta_max_dim() { return STEP_MAX_DIM; }
 
-// `form`: 0 the recurrent form, 2 the same for steps of about a token per request, 1 the chunked one, with a workspace `room` of fsie_delta_chunk_bytes() for every chunk
-// (of fsie_delta_chunk_tokens() tokens of a request, its last one begun)
-int fsie_delta_rule(int form, const void* qkv, int ld, int q_off, int k_off, int v_off, const float* log_decay, const float* beta,
+// `form`: 0 the recurrent form, 2 the same for steps of about a token per request, 1 the chunked one, with a workspace `room` of
+// fsie_delta_chunk_bytes() for every chunk (of fsie_delta_chunk_tokens() tokens of a request, its last one begun).  Form 1 with
+// `few` > 0: requests of up to `few` tokens, `ones` at least, in the recurrent form, beside the others.
+int fsie_delta_rule(int form, int few, int ones, const void* qkv, int ld, int q_off, int k_off, int v_off, const float* log_decay, const float* beta,
                     const int* item_qstart, const int* item_qlen, const int* item_slots, int items, float* state,
                     long long state_stride, float* out, int heads, int dim, int vdim, int share, float scale, float eps,
                     int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (items <= 0) return 0;
-    if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 2) return ERR_BAD_ARGUMENT;
+    if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 2 || ones < 0 || (form == 1 && ones >= items)) return ERR_BAD_ARGUMENT;
     DeltaParams p;
     p.qkv = qkv; p.ld = ld; p.q_off = q_off; p.k_off = k_off; p.v_off = v_off; p.log_decay = log_decay; p.beta = beta;
     p.item_qstart = item_qstart; p.item_qlen = item_qlen; p.item_slots = item_slots;
     p.state = state; p.state_stride = state_stride; p.out = out;
     p.heads = heads; p.dim = dim; p.vdim = vdim; p.share = share; p.scale = scale; p.eps = eps;
     if (dtype != DTYPE_F32 && dtype != DTYPE_BF16) return ERR_BAD_ARGUMENT;
-    if (form == 1) return delta_chunk(p, items, dtype, room, room_bytes, early, stream);
-    return dtype == DTYPE_F32 ? launch_step<float>(p, items, form == 2, early, stream) : launch_step<bf16>(p, items, form == 2, early, stream);
+    p.least = 1; p.most = INT_MAX; p.beside = false;
+    if (form == 1) {
+        p.least = few > 0 ? few + 1 : 1;
+        const int rc = delta_chunk(p, items, few > 0 ? items - ones : items, dtype, room, room_bytes, early, stream);
+        if (rc != 0 || few <= 0) return rc;
+        // Behind the walk in the stream, beside it on the GPU: its blocks need no wait, since the walk lets them go when its own
+        // is over, and wait for the walk's end at their own, so that whoever waits for them waits for both.
+        p.least = 1; p.most = few; p.beside = true; early = 1;
+    }
+    return dtype == DTYPE_F32 ? launch_step<float>(p, items, form != 0, early, stream) : launch_step<bf16>(p, items, form != 0, early, stream);
 }
 
 }  // extern "C"

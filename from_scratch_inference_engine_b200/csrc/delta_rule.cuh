@@ -10,6 +10,8 @@ struct DeltaParams {
     float* state; long long state_stride;                  // [slots], S [heads, dim, vdim] in front of each
     float* out;                                            // [tokens, heads * vdim]
     int heads, dim, vdim, share;
+    int least, most;                                       // tokens of a request that the launch takes; it leaves others alone
+    bool beside;                                           // the recurrent form runs beside the chunked one's launches
     float scale, eps;
 };
 

@@ -2294,7 +2294,7 @@ def delta():
         i, f, ll, p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
         lib.fsie_delta_prep.argtypes = [p, i, i, i, i, i, p, p, p, p, p, i, i, p, ll, ll, p, i, i, p, p, i, p, p, p, i, i, p]
         lib.fsie_delta_prep_max_taps.argtypes = []
-        lib.fsie_delta_rule.argtypes = [i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, p, ll, i, p]
+        lib.fsie_delta_rule.argtypes = [i, i, i, p, i, i, i, i, p, p, p, p, p, i, p, ll, p, i, i, i, i, f, f, i, p, ll, i, p]
         lib.fsie_delta_max_dim.argtypes = lib.fsie_delta_chunk_max_dim.argtypes = lib.fsie_delta_chunk_tokens.argtypes = []
         lib.fsie_delta_chunk_bytes.argtypes = [i, i, i, i]
         for name in ("fsie_delta_prep", "fsie_delta_prep_max_taps", "fsie_delta_rule", "fsie_delta_max_dim",
@@ -2365,13 +2365,20 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
                                    heads, act, log_decay, beta, _tag(proj.dtype), int(early), _stream()), "delta_prep")
 
 
-DELTA_FEW_TOKENS = 16      # up to so many tokens of a request the recurrent form walks them one by one
+# Up to so many tokens the recurrent form walks a request token by token; more go in chunks.  Recurrent against chunked, 64 requests
+# of 32 heads of 128 x 128: bfloat16 4 tokens 170 / 165 us, 6 240 / 167; float32 6 240 / 286, 8 312 / 290.  One request of 16 heads:
+# bfloat16 4 tokens 14 / 13 us, 8 20 / 13; float32 4 14 / 15, 8 20 / 15.
+# In a step of both kinds each request goes its way, the two forms beside one another: 63 decoded tokens and a prompt's 512 (32 heads
+# of 128 x 128) take 97 us, 85 with `ones` given, against 198 all in chunks and 948 all token by token.  A step without short requests
+# pays 2 to 4 us of 40 to 250 for the launch, so one whose requests are all of one length is spared it.
+DELTA_FEW_TOKENS = {DTYPE_F32: 6, DTYPE_BF16: 4}
 
 
 def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_decay: torch.Tensor, beta: torch.Tensor,
                      item_qstart: torch.Tensor, item_qlen: torch.Tensor, item_slots: torch.Tensor, items: int,
                      state: torch.Tensor, out: torch.Tensor, heads: int, dim: int, vdim: int, share: int = 1,
-                     scale: Optional[float] = None, eps: float = 1e-6, longest: int = 0, early: bool = False) -> torch.Tensor:
+                     scale: Optional[float] = None, eps: float = 1e-6, longest: int = 0, early: bool = False,
+                     ones: int = 0) -> torch.Tensor:
     """Per request and head, token by token, with q and k divided by sqrt(their squared length + eps) and
     a = exp(log_decay):
 
@@ -2382,7 +2389,8 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     (0 to 2) are float32 [tokens, heads]; state [slots, n] float32 with the heads' matrices [heads, dim, vdim] in the first
     heads * dim * vdim floats of a slot is read and left updated; out [tokens, heads * vdim] float32.  A request with a
     negative slot is passed over, its rows of `out` stay as they are.  `scale`: dim ** -0.5 unless given.  `longest`: the
-    tokens of the step's longest request, which choose the kernel (0: not known to the caller).  dim is 256 at most.
+    tokens of the step's longest request, which choose the kernel (0: not known to the caller); `ones`: at least so many of
+    the requests have one token, or none, and need no place among the longer ones (0 is always right).  dim is 256 at most.
     `early`: the state and the lists are older than the stream's last kernel, see the module's first lines."""
     f32, i32 = torch.float32, torch.int32
     if not (_fits(qkv, None, True) and _fits(log_decay, f32, True) and _fits(beta, f32, True) and _fits(out, f32, True)
@@ -2408,17 +2416,22 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
         raise KernelError("gated_delta_rule: the state slots do not hold the heads' matrices")
     if min(item_qstart.numel(), item_qlen.numel(), item_slots.numel()) < items:
         raise KernelError("gated_delta_rule: the lists are shorter than the requests")
+    if not 0 <= ones <= max(items, 0):
+        raise KernelError("gated_delta_rule: more requests of one token than requests")
     if not eps > 0:
         raise KernelError("gated_delta_rule: eps must be positive")
     most, chunked_most, chunk = _delta_limits()
     if dim > most:
         raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {most}")
     lib, tag, room = delta(), _tag(qkv.dtype), None
-    chunked = (longest or tokens) > DELTA_FEW_TOKENS and dim <= chunked_most
+    few = DELTA_FEW_TOKENS[tag]
+    chunked = (longest or tokens) > few and dim <= chunked_most and ones < items
+    form = 1 if chunked else 2 if longest == 1 or tokens == items or ones == items else 0
     if chunked:
+        few = few if items > 1 and tokens != items * longest else 0
         chunks = tokens // chunk + items
         room = torch.empty(chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag), dtype=torch.uint8, device=qkv.device)
-    _check(lib.fsie_delta_rule(1 if chunked else 2 if longest == 1 or tokens == items else 0, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
+    _check(lib.fsie_delta_rule(form, few, ones, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
                                items, state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
                                float(eps), tag, room, 0 if room is None else room.numel(), int(early), _stream()),
            "gated_delta_rule")

@@ -37,7 +37,7 @@ class Case:
         self.state = rand(self.items + 2, heads * dim * vdim + gap) * (0.1 * v_scale)
         self.starts = [sum(lengths[:i]) for i in range(self.items)]
 
-    def run(self, longest, portions=None, early=False, scale=None):
+    def run(self, longest, portions=None, early=False, scale=None, ones=0):
         """(out, state) of one call, or of one call per portion (lists of tokens per request)."""
         from from_scratch_inference_engine_b200.kernels import ops
         out = torch.full((self.tokens, self.heads * self.vdim), 7e7, device="cuda")
@@ -48,7 +48,7 @@ class Case:
             ops.gated_delta_rule(self.qkv, *self.offs, self.decay, self.beta,
                                  ints([s + d for s, d in zip(self.starts, done)]), ints(part), ints(self.slots), self.items,
                                  state, out, self.heads, self.dim, self.vdim, share=self.share, scale=scale, longest=longest,
-                                 early=early)
+                                 early=early, ones=ones)
             done = [d + n for d, n in zip(done, part)]
         return out, state
 
@@ -257,6 +257,34 @@ def test_on_another_stream(longest):
         assert torch.equal(have, want)
 
 
+MIXED = [[1] * 40 + [70], [90] + [1] * 33, [1, 5, 2, 40, 1, 0, 4, 7, 3, 6, 100, 1, 1], [1, 33], [6, 7, 5, 4, 1, 6], [0, 0, 50, 0, 1]]
+
+
+@pytest.mark.parametrize("told", [False, True])
+@pytest.mark.parametrize("dtype,dim,vdim", [(torch.bfloat16, 128, 128), (torch.bfloat16, 48, 20), (torch.float32, 64, 96),
+                                            (torch.float32, 40, 7)])
+@pytest.mark.parametrize("lengths", MIXED)
+def test_few_tokens_beside_long_requests(lengths, dtype, dim, vdim, told):
+    """Requests of few tokens go the recurrent way beside the others, wherever in the lists they stand."""
+    check(Case(lengths, 4, 2, dim, vdim, dtype), max(lengths), ones=sum(n <= 1 for n in lengths) if told else 0)
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_few_tokens_beside_long_requests_call_after_call(early):
+    """Each call reads the states that both launches of the one before left."""
+    case = Case([260] + [9] * 50, 8, 1, 64, 64, torch.bfloat16)
+    portions = [[100] + [1] * 50, [60] + [2] * 50, [1] + [1] * 50, [99] + [5] * 50]
+    for got, want in zip(case.run(MANY, portions=portions, early=early, ones=0), case.want()):
+        near(got, want)
+
+
+def test_few_tokens_beside_long_requests_without_slot():
+    case = Case([1, 40, 1, 64, 1, 2], 2, 1, 64, 64, torch.bfloat16)
+    case.slots[0] = case.slots[3] = case.slots[5] = -1
+    for got, want in zip(case.run(64, ones=3), case.want()):
+        near(got, want)
+
+
 def test_refusals():
     from from_scratch_inference_engine_b200.kernels import ops
     case = Case([4], 4, 2, 32, 32, torch.float32)
@@ -270,6 +298,6 @@ def test_refusals():
                   dict(offs=(-8, 72, 136)), dict(decay=case.decay[:, :2].contiguous()), dict(beta=case.beta.double()),
                   dict(lists=(lists[0].long(),) + lists[1:]), dict(items=2), dict(state=case.state[:, :100]),
                   dict(state=case.state.bfloat16()), dict(out=out[:3]), dict(out=out.bfloat16()), dict(heads=3), dict(share=3),
-                  dict(dim=0), dict(dim=257, heads=1, share=1), dict(eps=0.0)):
+                  dict(dim=0), dict(dim=257, heads=1, share=1), dict(eps=0.0), dict(ones=2), dict(ones=-1)):
         with pytest.raises(ops.KernelError):
             call(**wrong)
