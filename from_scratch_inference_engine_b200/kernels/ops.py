@@ -2365,13 +2365,14 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
                                    heads, act, log_decay, beta, _tag(proj.dtype), int(early), _stream()), "delta_prep")
 
 
-# Up to so many tokens the recurrent form walks a request token by token; more go in chunks.  Recurrent against chunked, 64 requests
-# of 32 heads of 128 x 128: bfloat16 4 tokens 170 / 165 us, 6 240 / 167; float32 6 240 / 286, 8 312 / 290.  One request of 16 heads:
-# bfloat16 4 tokens 14 / 13 us, 8 20 / 13; float32 4 14 / 15, 8 20 / 15.
+# Up to so many tokens the recurrent form walks a request token by token; more go in chunks.  In steps of less than 128 heads of
+# requests, and in others.  Recurrent against chunked, heads of 128 x 128, bfloat16 and float32: one request of 16 heads, 4 tokens
+# 14 / 13 and 13 / 15 us, 8 tokens 20 / 13 and 20 / 15; 8 of 32 heads, 8 tokens 25 / 32 and 25 / 42, 16 tokens 39 / 32 and 37 / 42;
+# 64 of 32 heads, 10 tokens 156 / 169 and 141 / 278, 16 tokens 221 / 173 and 201 / 290, 24 tokens 311 / 179 and 281 / 300.
 # In a step of both kinds each request goes its way, the two forms beside one another: 63 decoded tokens and a prompt's 512 (32 heads
 # of 128 x 128) take 97 us, 85 with `ones` given, against 198 all in chunks and 948 all token by token.  A step without short requests
 # pays 2 to 4 us of 40 to 250 for the launch, so one whose requests are all of one length is spared it.
-DELTA_FEW_TOKENS = {DTYPE_F32: 6, DTYPE_BF16: 4}
+DELTA_FEW_TOKENS = {DTYPE_F32: (6, 16), DTYPE_BF16: (4, 10)}
 
 
 def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_decay: torch.Tensor, beta: torch.Tensor,
@@ -2424,14 +2425,13 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     if dim > most:
         raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {most}")
     lib, tag, room = delta(), _tag(qkv.dtype), None
-    few = DELTA_FEW_TOKENS[tag]
+    few = DELTA_FEW_TOKENS[tag][items * heads >= 128]
     chunked = (longest or tokens) > few and dim <= chunked_most and ones < items
-    form = 1 if chunked else 2 if longest == 1 or tokens == items or ones == items else 0
     if chunked:
         few = few if items > 1 and tokens != items * longest else 0
         chunks = tokens // chunk + items
         room = torch.empty(chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag), dtype=torch.uint8, device=qkv.device)
-    _check(lib.fsie_delta_rule(form, few, ones, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
+    _check(lib.fsie_delta_rule(int(chunked), few, ones, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
                                items, state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
                                float(eps), tag, room, 0 if room is None else room.numel(), int(early), _stream()),
            "gated_delta_rule")

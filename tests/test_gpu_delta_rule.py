@@ -257,7 +257,7 @@ def test_on_another_stream(longest):
         assert torch.equal(have, want)
 
 
-MIXED = [[1] * 40 + [70], [90] + [1] * 33, [1, 5, 2, 40, 1, 0, 4, 7, 3, 6, 100, 1, 1], [1, 33], [6, 7, 5, 4, 1, 6], [0, 0, 50, 0, 1]]
+MIXED = [[1] * 40 + [70], [1] * 20 + [11, 10, 12, 9, 17, 16, 18, 15], [90] + [1] * 33, [1, 5, 2, 40, 1, 0, 4, 7, 3, 6, 100, 1, 1], [1, 33], [6, 7, 5, 4, 1, 6], [0, 0, 50, 0, 1]]
 
 
 @pytest.mark.parametrize("told", [False, True])
