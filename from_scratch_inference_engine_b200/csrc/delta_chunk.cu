@@ -54,6 +54,7 @@ constexpr int DC_MAX_DIM = 128;
 constexpr int DC_REFRESH = 16;             // chunks between two looks at the state's size
 constexpr int DC_SIZE = 3;                 // ... which brings the largest number of a column to 2^3 .. 2^4
 constexpr int DC_TLD = 16 + 8;             // padded rows of a 16 x 16 block in scratch
+constexpr int DC_ALD = 16 + 4;             // ... of floats
 // A number of R, times sigma, is below this: right behind a look it is at most 2^4 (1 + sqrt(128)).  A row of T has 32 numbers
 // of at most beta^2 <= 4 (what a token's value still does to a later token's u passes through contractions), so that u, and
 // u with a factor of at most 2, fit half precision.
@@ -262,7 +263,7 @@ template <typename T, int DK>
 struct DcMaker {                           // a preparing block's shared memory: the records as they go out, and scratch
     typename DcRecord<T, DK>::Keys keys;
     typename DcRecord<T, DK>::Gates gates;
-    float a[2][16][16 + 4];                // A's blocks on the diagonal
+    float a[2][16 * DC_ALD + 16];          // A's blocks on the diagonal; the two are read at once, from other banks
     __half w[2][16][DC_TLD];
     double g[DC_TOKENS];
     float kf[DC_TOKENS], qf[DC_TOKENS], beta[DC_TOKENS];
@@ -279,7 +280,7 @@ __device__ __forceinline__ void dc_copy_out(void* to, const void* from, int byte
 constexpr int DC_MAKERS = 4;
 
 template <typename T, int DK, bool WIDE>
-__global__ void __launch_bounds__(32 * DC_MAKERS, sizeof(T) == 2 ? 6 : 4)
+__global__ void __launch_bounds__(32 * DC_MAKERS, sizeof(T) == 2 ? 5 : 4)
 delta_records_kernel(const DeltaParams p, const DcRecords records) {
     using Sh = DcRecord<T, DK>;
     constexpr int PARTS = Sh::PARTS, FOURS = DK / 32;          // 32 columns are a quad's eight each
@@ -290,9 +291,11 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
     const int narrow_heads = p.heads / p.share;
     const int chunk = blockIdx.x / narrow_heads, narrow = blockIdx.x - chunk * narrow_heads;
     // the chunk's request and first token: 32 requests at a time
-    int item = -1, place = 0;
-    for (int i0 = 0, before = 0; i0 < records.items && item < 0; i0 += 32) {
-        const int i = i0 + lane, have = i < records.items ? dc_chunks(p.item_qlen[i], p.least) : 0;
+    int slot = -1, count = 0, first = 0, place = 0;
+    for (int i0 = 0, before = 0; i0 < records.items; i0 += 32) {
+        const int i = i0 + lane, last = records.items - 1;     // (read all at once: they come from far)
+        const int tokens = p.item_qlen[min(i, last)], its_slot = p.item_slots[min(i, last)], its_first = p.item_qstart[min(i, last)];
+        const int have = i <= last ? dc_chunks(tokens, p.least) : 0;
         int upto = have;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -302,13 +305,15 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
         const unsigned here = __ballot_sync(0xffffffffu, before + upto > chunk && before + upto - have <= chunk);
         if (here) {
             const int at = __ffs(here) - 1;
-            item = i0 + at;
             place = chunk - __shfl_sync(0xffffffffu, before + upto - have, at);
+            slot = __shfl_sync(0xffffffffu, its_slot, at);
+            count = __shfl_sync(0xffffffffu, tokens, at);
+            first = __shfl_sync(0xffffffffu, its_first, at) + place * DC_TOKENS;
+            break;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    const int slot = item >= 0 ? p.item_slots[item] : -1, count = item >= 0 ? p.item_qlen[item] : 0;
-    const int first = item >= 0 ? p.item_qstart[item] + place * DC_TOKENS : 0, n = min(DC_TOKENS, count - place * DC_TOKENS);
+    const int n = min(DC_TOKENS, count - place * DC_TOKENS);
     grid_dependency_wait();
     grid_dependents_go();
     if (slot < 0 || chunk >= records.chunks) return;           // beyond the step's chunks, or a padding entry
@@ -443,8 +448,8 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                     if (warp != 1) {
                         // (one that is not finite is left out: its token's R or beta is not finite either, and T has that)
                         const float bx = own.beta[row] * x, by = own.beta[row] * y;
-                        own.a[warp / 2][br][bc] = row > col && fabsf(bx) < INFINITY ? bx : 0.f;
-                        own.a[warp / 2][br][bc + 1] = row > col + 1 && fabsf(by) < INFINITY ? by : 0.f;
+                        own.a[warp / 2][br * DC_ALD + bc] = row > col && fabsf(bx) < INFINITY ? bx : 0.f;
+                        own.a[warp / 2][br * DC_ALD + bc + 1] = row > col + 1 && fabsf(by) < INFINITY ? by : 0.f;
                     }
                 }
             }
@@ -460,7 +465,11 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
             for (int l = 15; l >= 1; --l) {
                 const float xl = l <= i ? -x[l] : 0.f;
 #pragma unroll
-                for (int j = 0; j < l; ++j) x[j] = fmaf(xl, own.a[m][l][j], x[j]);
+                for (int j = 0; j < l; j += 4) {               // (A is zero on the diagonal and beyond)
+                    const float4 a = *reinterpret_cast<const float4*>(&own.a[m][l * DC_ALD + j]);
+                    x[j] = fmaf(xl, a.x, x[j]); x[j + 1] = fmaf(xl, a.y, x[j + 1]);
+                    x[j + 2] = fmaf(xl, a.z, x[j + 2]); x[j + 3] = fmaf(xl, a.w, x[j + 3]);
+                }
             }
             bool finite = true;
 #pragma unroll

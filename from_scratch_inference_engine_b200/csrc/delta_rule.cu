@@ -54,7 +54,7 @@ delta_step_kernel(const DeltaParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
     if (slot < 0 || count < p.least || count > p.most) {   // a padding entry of a fixed-size batch, or the other form's
-        grid_dependency_wait();
+        if (!p.beside || first_block()) grid_dependency_wait();
         return;
     }
     const int group = tid / ACROSS, at = (tid % ACROSS) * V, col = blockIdx.x * STEP_COLS + at;
@@ -153,7 +153,7 @@ delta_step_kernel(const DeltaParams p) {
         const int r = group + i * GROUPS;
         if (in && r < p.dim) store_cols(state + (size_t)r * p.vdim, s[i]);
     }
-    if (p.beside) grid_dependency_wait();
+    if (p.beside && first_block()) grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------------------------------------- many requests
@@ -177,7 +177,7 @@ delta_head_kernel(const DeltaParams p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];
     if (slot < 0 || count < p.least || count > p.most) {   // a padding entry of a fixed-size batch, or the other form's
-        grid_dependency_wait();
+        if (!p.beside || first_block()) grid_dependency_wait();
         return;
     }
     const int row0 = tid / ACROSS * ROWS, at = (tid % ACROSS) * 4;     // the thread's rows and columns
@@ -274,7 +274,7 @@ delta_head_kernel(const DeltaParams p) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
         if (in && row0 + i < p.dim) *reinterpret_cast<float4*>(state + (size_t)i * p.vdim) = s[i];
-    if (p.beside) grid_dependency_wait();
+    if (p.beside && first_block()) grid_dependency_wait();
 }
 
 template <typename T>
@@ -332,7 +332,7 @@ int fsie_delta_rule(int form, int few, int ones, const void* qkv, int ld, int q_
         const int rc = delta_chunk(p, items, few > 0 ? items - ones : items, dtype, room, room_bytes, early, stream);
         if (rc != 0 || few <= 0) return rc;
         // Behind the walk in the stream, beside it on the GPU: its blocks need no wait, since the walk lets them go when its own
-        // is over, and wait for the walk's end at their own, so that whoever waits for them waits for both.
+        // is over, and the first waits for the walk's end at its own, so that whoever waits for them all waits for both.
         p.least = 1; p.most = few; p.beside = true; early = 1;
     }
     return dtype == DTYPE_F32 ? launch_step<float>(p, items, early, stream) : launch_step<bf16>(p, items, early, stream);

@@ -3,6 +3,8 @@
 
 namespace fsie {
 
+__device__ __forceinline__ bool first_block() { return (blockIdx.x | blockIdx.y | blockIdx.z) == 0; }
+
 struct DeltaParams {
     const void* qkv; int ld, q_off, k_off, v_off;          // [tokens, ld]; heads / share q and k columns of dim, heads of vdim
     const float* log_decay; const float* beta;             // [tokens, heads]
