@@ -39,6 +39,7 @@
 // values left out, and what they reach is set to NaN.
 #include "common.cuh"
 #include "delta_rule.cuh"
+#include "tma.cuh"
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -216,6 +217,8 @@ struct DcShape : DcRecord<T, DK> {
         float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs without the factors; of two warps per 16 columns two summands
         float back[2][COLS];                       // what its columns are still to be multiplied by
         float most[DC_WALKERS][16];
+        uint64_t full[DC_STAGES];                  // a stage's records are there
+        int lost;                                  // ... or were waited for in vain
     };
 };
 
@@ -545,16 +548,22 @@ __device__ __forceinline__ void dc_copy16(void* dst, const void* src, bool there
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dc_smem(dst)), "l"(src), "r"(bytes) : "memory");
 }
 
-enum { DC_MEET = 1, DC_GO = 2, DC_PAIR = 3 };        // named barriers; from DC_PAIR on the pairs'
+__device__ __forceinline__ void dc_copy_in(void* to, const void* from, unsigned bytes, uint64_t* full) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n"
+                 ::"r"(dc_smem(to)), "l"(from), "r"(bytes), "r"(dc_smem(full)) : "memory");
+}
+
+enum { DC_MEET = 1, DC_PAIR = 2 };                   // named barriers; from DC_PAIR on the pairs'
 
 // A fetching thread's share of the copies into the ring, chunk after chunk: the addresses move on by a chunk with every call.
-// (Copied by the walkers themselves a chunk takes them 800 cycles more: their own reads of shared memory queue behind.)
+// (Copied by the walkers themselves a chunk took them 800 cycles more, their own reads of shared memory queueing behind.  The
+// records come as two bulk copies: 16-byte copies of all the threads queued before the walkers' reads as well, 8,192 tokens of
+// 16 q/k and 32 heads took 366 us against 343.)
 template <typename T, int DK, bool WIDE>
 struct DcFetch {
     using Sh = DcShape<T, DK>;
     using Stage = typename Sh::Stage;
     static constexpr int PER = 16 / sizeof(T), ACROSS = Sh::COLS / PER;          // 16-byte pieces of a row of v
-    static constexpr int KEYS = sizeof(typename Sh::Keys) / 16, GATES = sizeof(typename Sh::Gates) / 16;
     const unsigned char* keys;
     const unsigned char* gates;
     const T* v;
@@ -566,25 +575,22 @@ struct DcFetch {
         keys_step = (size_t)narrow_heads * sizeof(typename Sh::Keys);
         gates_step = (size_t)p.heads * sizeof(typename Sh::Gates);
         v_step = (size_t)DC_TOKENS * p.ld;
-        keys = records.keys + chunk0 * keys_step + (size_t)(head / p.share) * sizeof(typename Sh::Keys) + tid * 16;
-        gates = records.gates + chunk0 * gates_step + (size_t)head * sizeof(typename Sh::Gates) + tid * 16;
+        keys = records.keys + chunk0 * keys_step + (size_t)(head / p.share) * sizeof(typename Sh::Keys);
+        gates = records.gates + chunk0 * gates_step + (size_t)head * sizeof(typename Sh::Gates);
         row = WIDE ? tid / ACROSS : 0;
         const int d = WIDE ? (tid % ACROSS) * PER : 0;
         have = p.vdim - col0 - d;
         v = (const T*)p.qkv + (size_t)t0 * p.ld + p.v_off + (size_t)head * p.vdim + col0 + (WIDE && have > 0 ? d : 0);
         left = count;
     }
-    __device__ __forceinline__ void next(const DeltaParams& p, Stage& st) {
+    __device__ __forceinline__ void next(const DeltaParams& p, Stage& st, uint64_t* full) {
         const int tid = threadIdx.x - 32 * DC_WALKERS;
         if (left > 0) {
-#pragma unroll
-            for (int i = 0; i < (KEYS + DC_FETCHERS - 1) / DC_FETCHERS; ++i)
-                if ((i + 1) * DC_FETCHERS <= KEYS || tid + i * DC_FETCHERS < KEYS)
-                    dc_copy16(reinterpret_cast<uint4*>(&st.keys) + tid + i * DC_FETCHERS, keys + i * DC_FETCHERS * 16, true);
-#pragma unroll
-            for (int i = 0; i < (GATES + DC_FETCHERS - 1) / DC_FETCHERS; ++i)
-                if ((i + 1) * DC_FETCHERS <= GATES || tid + i * DC_FETCHERS < GATES)
-                    dc_copy16(reinterpret_cast<uint4*>(&st.gates) + tid + i * DC_FETCHERS, gates + i * DC_FETCHERS * 16, true);
+            if (tid == 0) {
+                mbar_expect_tx(full, sizeof(st.keys) + sizeof(st.gates));
+                dc_copy_in(&st.keys, keys, sizeof(st.keys), full);
+                dc_copy_in(&st.gates, gates, sizeof(st.gates), full);
+            }
             if constexpr (WIDE) {
                 constexpr int ROWS = DC_FETCHERS / ACROSS;     // rows of v that the block's threads copy at once
 #pragma unroll
@@ -736,9 +742,27 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         float* out = p.out + (size_t)t0 * width + (size_t)head * p.vdim + col0;
         const bool wide = p.vdim % 4 == 0 && (uintptr_t)p.out % 16 == 0;
         const float* queries = (reinterpret_cast<const typename Sh::Gates*>(records.gates) + (size_t)chunk0 * p.heads + head)->query;
-        fetch.next(p, sm.stage[0]);
-        fetch.next(p, sm.stage[1]);
+        const bool first = threadIdx.x == 32 * DC_WALKERS;
+        if (first) {
+            for (int i = 0; i < DC_STAGES; ++i) mbar_init(&sm.full[i], 1);
+            sm.lost = 0;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        fetch.next(p, sm.stage[0], &sm.full[0]);
+        fetch.next(p, sm.stage[1], &sm.full[1]);
         asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+        // (A copy between checked addresses ends; should one be waited for in vain, no more are asked for, the outputs and the state
+        // become NaN, and the copies on their way are waited for once more at the end.)
+        int lost = -1;                                         // the chunk that did not come
+        auto await_chunk = [&](int c) {
+            if (first && lost < 0 && !mbar_wait(&sm.full[c % DC_STAGES], (c / DC_STAGES) & 1)) {
+                sm.lost = 1;
+                lost = c;
+                fetch.left = 0;
+            }
+            __syncwarp();
+        };
+        await_chunk(0);
         dc_sync(DC_MEET, Sh::THREADS);                         // chunk 0 is there
         for (int c = 1; c <= chunks + 1; ++c) {                // (the last meetings are for chunks that are not there)
             float query[Sh::WRITES];                           // of the chunk that is written next
@@ -748,15 +772,21 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 queries += (size_t)p.heads * (sizeof(typename Sh::Gates) / sizeof(float));
             }
             asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+            if (c < chunks) await_chunk(c);
             dc_sync(DC_MEET, Sh::THREADS);                     // chunk c is there, and everybody is through with chunk c - 2:
-            if (c <= chunks) dc_sync(DC_GO, Sh::THREADS);      // (copies asked for at once would delay what the walkers swap)
-            fetch.next(p, sm.stage[(c + 1) % DC_STAGES]);      // its stage takes chunk c + 1
+            fetch.next(p, sm.stage[(c + 1) % DC_STAGES], &sm.full[(c + 1) % DC_STAGES]);       // its stage takes chunk c + 1
             if (c >= 2) {
+                if (__builtin_expect(sm.lost, 0)) {
+#pragma unroll
+                    for (int i = 0; i < Sh::WRITES; ++i) query[i] = __int_as_float(0x7fffffff);
+                }
                 dc_write<T, DK>(sm.out[c & 1], sm.back[c & 1], query, out, width, count - (c - 2) * DC_TOKENS, p.vdim - col0, wide);
                 out += DC_TOKENS * width;
             }
         }
         asm volatile("cp.async.wait_group 0;\n" ::: "memory");
+        if (lost >= 0)
+            for (int c = lost; c < min(chunks, max(lost + 1, 2)); ++c) mbar_wait(&sm.full[c % DC_STAGES], (c / DC_STAGES) & 1);
         return;
     }
     if (sizeof(T) == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
@@ -944,7 +974,6 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 dc_ldmatrix(tl[b], &st.gates.t[1][b][b_row][b_piece]);
             }
             dc_split_tiles(r[0], r[1], rh[0], rl[0]);
-            if (tries == 0) asm volatile("bar.arrive %0, %1;" ::"r"((int)DC_GO), "r"(Sh::THREADS) : "memory");
             query_step(1);
             dc_split_tiles(r[2], r[3], rh[1], rl[1]);
             dc_solve(u, rh, rl, th, tl);
@@ -1079,6 +1108,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         }
     }
     dc_sync(DC_MEET, Sh::THREADS);
+    if (__builtin_expect(sm.lost, 0)) back[0] = back[1] = __int_as_float(0x7fffffff);
 #pragma unroll
     for (int n = 0; n < TILES; ++n)
 #pragma unroll
@@ -1112,11 +1142,15 @@ static int launch_chunk(const DeltaParams& p, const DcRecords& records, int earl
     if (units > 0x7fffffffLL || grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
     const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32 * DC_MAKERS), sizeof(DcMaker<T, DK>), stream, p, records);
     if (rc != 0) return rc;
-    // As many blocks as SMs had better not share any (DC_ALONE), which they do if they start while the records' blocks still
-    // hold some.  The state is older than the records' kernel, which waits for whatever may have written it.
-    const bool alone = (long long)grid.x * grid.y * grid.z <= sms;
-    return launch_dependent(walker, grid, dim3(Sh::THREADS), alone ? (size_t)DC_ALONE_BYTES : sizeof(typename Sh::Shared), stream, p,
-                            records);
+    // As many blocks as SMs had better not share any, which they do if they start while the records' blocks still hold some:
+    // 8,192 tokens of 16 heads of 128 x 128 (64 blocks) take 366 us alone, 546 two to an SM.  More blocks, some of which may have
+    // nothing to do (p.least: requests of many lengths), start behind the records' end and spread: 13 requests of 1 to 700 tokens,
+    // 16 heads of 64 x 64 (208 blocks) 54 against 64 us; three of 256 to 1,024 of 16 heads of 128 x 128 (192) 89 against 85.
+    // The state is older than the records' kernel, which waits for whatever may have written it.
+    const long long blocks = (long long)grid.x * grid.y * grid.z;
+    const bool alone = blocks <= sms, spread = !alone && blocks <= 2 * sms && p.least > 1;
+    return launch_dependent_if(!spread, walker, grid, dim3(Sh::THREADS), alone ? (size_t)DC_ALONE_BYTES : sizeof(typename Sh::Shared),
+                               stream, p, records);
 }
 
 template <typename T, int DK>
