@@ -29,9 +29,9 @@
 // kernel in which four more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads: every block of
 // value columns prepared them again, and the two roles' code did not fit the instruction cache together.)
 //
-// Layout.  A warp of the second kernel owns 16 value columns x 64 rows of S, transposed: S^T is the 16-row operand of S0^T k
+// Layout.  A warp of the second kernel owns 16 value columns x 64 or 32 rows of S, transposed: S^T is the 16-row operand of S0^T k
 // and S0^T q, the accumulator of S0^T k is (after R) the operand of the next product in the registers where it lies, and the
-// new sums end up where S lies.  Heads of more than 64 rows take two warps per 16 columns, which swap their halves' sums
+// new sums end up where S lies.  Heads of more rows take two or four warps per 16 columns, which swap their rows' sums
 // of S0^T k through shared memory, in the chunk's one meeting; those of S0^T q the fetching warps add up.
 //
 // Values that are not finite: they spoil their column from their token on and nothing else, as in the recurrence - a product
@@ -50,7 +50,6 @@ constexpr int DC_TILES = DC_TOKENS / 8;    // ... in tiles of eight
 constexpr int DC_STAGES = 3;               // stages of the ring: the chunk's, the next one's and one on its way
 constexpr int DC_WALKERS = 4;              // warps that walk a block's chunks
 constexpr int DC_FETCHERS = 128;           // threads that copy
-constexpr int DC_SLICE = 64;               // rows of S (columns of k) per warp
 constexpr int DC_MAX_DIM = 128;
 constexpr int DC_REFRESH = 16;             // chunks between two looks at the state's size
 constexpr int DC_SIZE = 3;                 // ... which brings the largest number of a column to 2^3 .. 2^4
@@ -198,23 +197,24 @@ struct DcRecord {
     };
 };
 
-template <typename T, int DK>
+// SLICE: rows of S (columns of k) per warp
+template <typename T, int DK, int SLICE>
 struct DcShape : DcRecord<T, DK> {
-    static constexpr int SLICES = DK / DC_SLICE;               // warps that share 16 value columns
+    static constexpr int SLICES = DK / SLICE;                  // warps that share 16 value columns
     static constexpr int GROUPS = DC_WALKERS / SLICES;         // groups of 16 value columns
     static constexpr int COLS = 16 * GROUPS;                   // value columns of a block
     static constexpr int VLD = COLS + (sizeof(T) == 4 ? 4 : 0);         // row of v; bfloat16: v_piece()
     static constexpr int OLD = COLS + 4;                       // padded row of outputs
     static constexpr int THREADS = 32 * DC_WALKERS + DC_FETCHERS;
     static constexpr int WRITES = DC_TOKENS * COLS / 4 / DC_FETCHERS;       // rows of four outputs that a fetching thread writes
-    static constexpr int FINISH = SLICES > 1 ? DC_TILES / 2 : DC_TILES;     // tiles of eight tokens whose outputs a warp finishes
+    static constexpr int FINISH = DC_TILES / SLICES;           // tiles of eight tokens whose outputs a warp finishes
     // Place of a row's 16-byte piece of bfloat16 v: in another order in every row, ldmatrix without bank conflicts.
-    static __device__ __forceinline__ int v_piece(int row, int piece) { return piece ^ (COLS == 32 ? (row >> 1) & 3 : row & 7); }
+    static __device__ __forceinline__ int v_piece(int row, int piece) { return piece ^ (COLS == 16 ? (row >> 2) & 1 : COLS == 32 ? (row >> 1) & 3 : row & 7); }
     struct alignas(16) Stage { typename DcRecord<T, DK>::Keys keys; typename DcRecord<T, DK>::Gates gates; T v[DC_TOKENS][VLD]; };
     struct Shared {
         Stage stage[DC_STAGES];
         float4 swap[2][SLICES > 1 ? DC_WALKERS : 1][DC_TILES][32];      // S0^T k of a warp's rows
-        float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs without the factors; of two warps per 16 columns two summands
+        float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs without the factors, a summand per warp of the 16 columns
         float back[2][COLS];                       // what its columns are still to be multiplied by
         float most[DC_WALKERS][16];
         uint64_t full[DC_STAGES];                  // a stage's records are there
@@ -559,9 +559,9 @@ enum { DC_MEET = 1, DC_PAIR = 2 };                   // named barriers; from DC_
 // (Copied by the walkers themselves a chunk took them 800 cycles more, their own reads of shared memory queueing behind.  The
 // records come as two bulk copies: 16-byte copies of all the threads queued before the walkers' reads as well, 8,192 tokens of
 // 16 q/k and 32 heads took 366 us against 343.)
-template <typename T, int DK, bool WIDE>
+template <typename T, int DK, int SLICE, bool WIDE>
 struct DcFetch {
-    using Sh = DcShape<T, DK>;
+    using Sh = DcShape<T, DK, SLICE>;
     using Stage = typename Sh::Stage;
     static constexpr int PER = 16 / sizeof(T), ACROSS = Sh::COLS / PER;          // 16-byte pieces of a row of v
     const unsigned char* keys;
@@ -616,10 +616,9 @@ struct DcFetch {
 
 // The fetching threads also write outputs, whole lines side by side: `tokens` rows of a chunk's, from `to` on, the walkers' summands
 // times the column's and the token's factor (`queries`, from the chunk's record).
-template <typename T, int DK>
-__device__ __forceinline__ void dc_write(const float (&from)[DcShape<T, DK>::SLICES][DC_TOKENS][DcShape<T, DK>::OLD], const float* back,
-                                         const float (&queries)[DcShape<T, DK>::WRITES], float* to, size_t width, int tokens, int columns, bool wide) {
-    using Sh = DcShape<T, DK>;
+template <typename Sh>
+__device__ __forceinline__ void dc_write(const float (&from)[Sh::SLICES][DC_TOKENS][Sh::OLD], const float* back,
+                                         const float (&queries)[Sh::WRITES], float* to, size_t width, int tokens, int columns, bool wide) {
     constexpr int FOURS = Sh::COLS / 4, AT_ONCE = DC_FETCHERS / FOURS;
     const int tid = threadIdx.x - 32 * DC_WALKERS, d = (tid % FOURS) * 4;
     if (d >= columns) return;
@@ -630,8 +629,9 @@ __device__ __forceinline__ void dc_write(const float (&from)[DcShape<T, DK>::SLI
         if (r >= tokens) continue;
         const float query = queries[i];
         float4 o = *reinterpret_cast<const float4*>(&from[0][r][d]);
-        if (Sh::SLICES > 1) {
-            const float4 x = *reinterpret_cast<const float4*>(&from[Sh::SLICES - 1][r][d]);
+#pragma unroll
+        for (int s = 1; s < Sh::SLICES; ++s) {
+            const float4 x = *reinterpret_cast<const float4*>(&from[s][r][d]);
             o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
         }
         o = make_float4(o.x * b.x * query, o.y * b.y * query, o.z * b.z * query, o.w * b.w * query);
@@ -714,11 +714,11 @@ __device__ __forceinline__ void dc_leave_out(float (&x)[DC_TILES][4], int t, con
             if (8 * j + 2 * t + (e & 1) >= first[e >> 1]) x[j][e] = 0.f;
 }
 
-template <typename T, int DK, bool WIDE>
+template <typename T, int DK, int SLICE, bool WIDE>
 __global__ void __launch_bounds__(32 * DC_WALKERS + DC_FETCHERS, sizeof(T) == 2 ? 2 : 1)
 delta_walk_kernel(const DeltaParams p, const DcRecords records) {
-    using Sh = DcShape<T, DK>;
-    constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = DC_SLICE / 8, STEPS = DC_SLICE / 16, FINISH = Sh::FINISH;
+    using Sh = DcShape<T, DK, SLICE>;
+    constexpr int PARTS = Sh::PARTS, SLICES = Sh::SLICES, TILES = SLICE / 8, STEPS = SLICE / 16, FINISH = Sh::FINISH;
     extern __shared__ __align__(16) unsigned char dc_raw[];
     auto& sm = *reinterpret_cast<typename Sh::Shared*>(dc_raw);
     const int head = blockIdx.y, col0 = blockIdx.x * Sh::COLS;
@@ -737,7 +737,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         if (sizeof(T) == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
         grid_dependency_wait();
         grid_dependents_go();
-        DcFetch<T, DK, WIDE> fetch(p, records, head, col0, t0, count, chunk0);
+        DcFetch<T, DK, SLICE, WIDE> fetch(p, records, head, col0, t0, count, chunk0);
         const size_t width = (size_t)p.heads * p.vdim;
         float* out = p.out + (size_t)t0 * width + (size_t)head * p.vdim + col0;
         const bool wide = p.vdim % 4 == 0 && (uintptr_t)p.out % 16 == 0;
@@ -780,7 +780,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                     for (int i = 0; i < Sh::WRITES; ++i) query[i] = __int_as_float(0x7fffffff);
                 }
-                dc_write<T, DK>(sm.out[c & 1], sm.back[c & 1], query, out, width, count - (c - 2) * DC_TOKENS, p.vdim - col0, wide);
+                dc_write<Sh>(sm.out[c & 1], sm.back[c & 1], query, out, width, count - (c - 2) * DC_TOKENS, p.vdim - col0, wide);
                 out += DC_TOKENS * width;
             }
         }
@@ -792,7 +792,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     if (sizeof(T) == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;\n");
     const int g = lane >> 2, t = lane & 3;
     const int group = warp / SLICES, slice = warp % SLICES;
-    const int row0 = slice * DC_SLICE;                         // the warp's rows of S
+    const int row0 = slice * SLICE;                            // the warp's rows of S
     const int col = col0 + group * 16 + g;                     // the thread's value columns: col and col + 8
     float* state = p.state + (size_t)slot * p.state_stride + (size_t)head * p.dim * p.vdim;
     // S^T, tile n: rows (value columns) g and g + 8, columns (rows of S) 8 n + 2 t and the next; times sigma
@@ -810,11 +810,12 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     const int b_row = (lane & 7) + 8 * (lane >> 4), b_col = 8 * ((lane >> 3) & 1);      // ldmatrix, operand stored [n][k]
     const int bt_row = (lane & 7) + 8 * ((lane >> 3) & 1), bt_col = 8 * (lane >> 4);    // ... and [k][n]
     const int b_piece = dc_piece(lane & 7, (lane >> 3) & 1);   // ... of a 16 x 16 block
-    // Two warps per 16 columns: the first finishes the outputs of token tiles 0 and 3, the second of 1 and 2 (tiles 2 and 3 have
-    // two blocks of weights).  S0^T q has the second's tiles in the order 1, 0, 3, 2, so that a warp's own are its first and last.
-    // One warp: all four.
-    const int q_row = (lane & 7) + 8 * ((lane >> 4) ^ (SLICES > 1 ? slice : 0));
-    auto tile_of = [&](int j) { return SLICES > 1 ? (j == 0 ? slice : 3 - slice) : j; };
+    // Each of the warps of 16 columns finishes the outputs of some of the four token tiles: of two the first 0 and 3, the second 1 and 2
+    // (tiles 2 and 3 have two blocks of weights), of four each one.  S0^T q has tile `place ^ slice` at a place, so that a warp's own
+    // tiles are at the same places in every warp.
+    const int q_row = (lane & 7) + 8 * ((lane >> 4) ^ (slice & 1)), q_half = 16 * (slice >> 1);
+    constexpr int OWN = SLICES == 2 ? 3 : 1;                   // steps between the places of a warp's own tiles
+    auto tile_of = [&](int j) { return OWN * j ^ slice; };
     // Operands of the next products are read well ahead of them, and sums that do not depend on one another are asked for
     // together: a warp has its scheduler nearly to itself, so what one instruction waits for, all wait for.
     unsigned bk[2][2][4];                                      // K, operand of S0^T k, 16 rows of S and two times 16 tokens each; two in turn
@@ -852,17 +853,18 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         unsigned sh[STEPS][4], sl[STEPS][4];                   // the state in two parts
         auto ask_query = [&](int k) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][16 * m + q_row][row0 + 16 * k + b_col]);
+            for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][(16 * m ^ q_half) + q_row][row0 + 16 * k + b_col]);
         };
         // a quarter of the instructions of S0^T q: they stand where the chain of R, U and the new state has to wait
         auto query_step = [&](int k) {
+            if (k >= STEPS) return;
 #pragma unroll
             for (int j = 0; j < DC_TILES; ++j) dc_mma_if(k == 0, wq[j], sl[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
             if (PARTS == 2) {
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     unsigned b[4];
-                    dc_ldmatrix(b, &st.keys.q[PARTS - 1][16 * m + q_row][row0 + 16 * k + b_col]);
+                    dc_ldmatrix(b, &st.keys.q[PARTS - 1][(16 * m ^ q_half) + q_row][row0 + 16 * k + b_col]);
                     dc_mma(wq[2 * m], sh[k], b[0], b[1]);
                     dc_mma(wq[2 * m + 1], sh[k], b[2], b[3]);
                 }
@@ -891,9 +893,12 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 }
                 if (SLICES > 1) {
                     if (t == 0) { sm.most[warp][g] = most[0]; sm.most[warp][g + 8] = most[1]; }
-                    dc_sync(DC_PAIR + group, 64);
-                    most[0] = fmaxf(most[0], sm.most[warp ^ 1][g]);
-                    most[1] = fmaxf(most[1], sm.most[warp ^ 1][g + 8]);
+                    dc_sync(DC_PAIR + group, 32 * SLICES);
+#pragma unroll
+                    for (int s = 1; s < SLICES; ++s) {
+                        most[0] = fmaxf(most[0], sm.most[warp ^ s][g]);
+                        most[1] = fmaxf(most[1], sm.most[warp ^ s][g + 8]);
+                    }
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -941,16 +946,27 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             float size = st.gates.odd[0];                      // NaN where T is not finite
             // ---- one meeting per chunk: the halves' sums are there, and so is the next stage
             if (tries == 0) dc_sync(DC_MEET, Sh::THREADS);
-            else if (SLICES > 1) dc_sync(DC_PAIR + group, 64);
+            else if (SLICES > 1) dc_sync(DC_PAIR + group, 32 * SLICES);
             if constexpr (SLICES > 1) {
                 float4 x[DC_TILES];
 #pragma unroll
                 for (int j = 0; j < DC_TILES; ++j) x[j] = sm.swap[c & 1][warp ^ 1][j][lane];
+                float4 y[DC_TILES], z[DC_TILES];
+                if (SLICES > 2) {
+#pragma unroll
+                    for (int j = 0; j < DC_TILES; ++j) { y[j] = sm.swap[c & 1][warp ^ 2][j][lane]; z[j] = sm.swap[c & 1][warp ^ 3][j][lane]; }
+                }
                 query_step(0);
 #pragma unroll
                 for (int j = 0; j < DC_TILES; ++j) {
                     dc_add2(wk[j][0], wk[j][1], wk[j][0], wk[j][1], x[j].x, x[j].y);
                     dc_add2(wk[j][2], wk[j][3], wk[j][2], wk[j][3], x[j].z, x[j].w);
+                    if (SLICES > 2) {                          // (pairs first: the same sum in all four warps)
+                        dc_add2(y[j].x, y[j].y, y[j].x, y[j].y, z[j].x, z[j].y);
+                        dc_add2(y[j].z, y[j].w, y[j].z, y[j].w, z[j].z, z[j].w);
+                        dc_add2(wk[j][0], wk[j][1], wk[j][0], wk[j][1], y[j].x, y[j].y);
+                        dc_add2(wk[j][2], wk[j][3], wk[j][2], wk[j][3], y[j].z, y[j].w);
+                    }
                 }
             } else {
                 query_step(0);
@@ -1037,24 +1053,25 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         // ---- outputs: the chunk's start and its own tokens; the fetching warps add up what two warps have of S0^T q and write them
         unsigned zh[2][4], zl[2][4], w[FINISH][2][4];          // U again, weights: high and low part, two inner halves each
         float2 fade[FINISH];
+        auto second = [&](int j) { return SLICES == 4 ? slice >= 2 : OWN * j >= 2; };      // the tile's tokens are in the chunk's second half
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
             fade[j] = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile_of(j) + 2 * t]);
-            const bool second = SLICES > 1 ? j == 1 : j >= 2;  // the tile's tokens are in the chunk's second half
 #pragma unroll
-            for (int m = 0; m <= (second ? 1 : 0); ++m)
-                dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_piece]);
+            for (int m = 0; m < 2; ++m)
+                if (m == 0 || second(j)) dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second(j) ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_piece]);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) dc_split_tiles(u[2 * m], u[2 * m + 1], zh[m], zl[m]);
         float oa[FINISH][4], ob[FINISH][4];
 #pragma unroll
         for (int j = 0; j < FINISH; ++j) {
-            const float(&own)[4] = wq[SLICES > 1 ? 3 * j : j];
+            const float(&own)[4] = wq[OWN * j];
 #pragma unroll
             for (int h = 0; h < 2; ++h) dc_mul2(oa[j][2 * h], oa[j][2 * h + 1], own[2 * h], own[2 * h + 1], fade[j].x, fade[j].y);
 #pragma unroll
-            for (int m = 0; m <= ((SLICES > 1 ? j == 1 : j >= 2) ? 1 : 0); ++m) {
+            for (int m = 0; m < 2; ++m) {
+                if (m > 0 && !second(j)) continue;
                 dc_mma_if(m == 0, ob[j], zl[m], w[j][m][0], w[j][m][1]);
                 dc_mma(oa[j], zh[m], w[j][m][0], w[j][m][1]);
                 dc_mma(ob[j], zh[m], w[j][m][2], w[j][m][3]);
@@ -1072,13 +1089,13 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         };
         if constexpr (SLICES > 1) {
 #pragma unroll
-            for (int j = 1; j < 3; ++j) {                      // the other warp's tiles
+            for (int j = 1; j < (SLICES > 2 ? 4 : 3); ++j) {   // the other warps' tiles
                 const int tile = j ^ slice;
                 const float2 f = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile + 2 * t]);
                 float o[4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) dc_mul2(o[2 * h], o[2 * h + 1], wq[j][2 * h], wq[j][2 * h + 1], f.x, f.y);
-                leave(SLICES - 1, tile, o);
+                leave(SLICES > 2 ? j : 1, tile, o);
             }
         }
 #pragma unroll
@@ -1120,28 +1137,18 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 
 // An SM for each block: asks for more than half of the SM's shared memory.
 constexpr int DC_ALONE_BYTES = 180 * 1024;
-static_assert(sizeof(DcShape<float, 128>::Shared) <= DC_ALONE_BYTES, "the largest shape");
+static_assert(sizeof(DcShape<float, 128, 64>::Shared) <= DC_ALONE_BYTES && sizeof(DcShape<float, 128, 32>::Shared) <= DC_ALONE_BYTES, "the largest shapes");
 
-template <typename T, int DK, bool WIDE>
-static int launch_chunk(const DeltaParams& p, const DcRecords& records, int early, cudaStream_t stream) {
-    using Sh = DcShape<T, DK>;
-    auto maker = delta_records_kernel<T, DK, WIDE>;
-    auto walker = delta_walk_kernel<T, DK, WIDE>;
-    static int sms = 0;                        // per process and kernels; harmless if repeated
-    if (sms == 0) {
-        int device = 0, count = 0;
-        cudaError_t e = cudaGetDevice(&device);
-        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(maker, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DcMaker<T, DK>));
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(walker, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_ALONE_BYTES);
+template <typename T, int DK, int SLICE, bool WIDE>
+static int launch_walk(const DeltaParams& p, const DcRecords& records, dim3 grid, int sms, cudaStream_t stream) {
+    using Sh = DcShape<T, DK, SLICE>;
+    auto walker = delta_walk_kernel<T, DK, SLICE, WIDE>;
+    static bool ready = false;                 // per process and kernel; harmless if repeated
+    if (!ready) {
+        const cudaError_t e = cudaFuncSetAttribute(walker, cudaFuncAttributeMaxDynamicSharedMemorySize, DC_ALONE_BYTES);
         if (e != cudaSuccess) return (int)e;
-        sms = count;
+        ready = true;
     }
-    const long long units = (long long)records.chunks * (p.heads / p.share);
-    const dim3 grid((p.vdim + Sh::COLS - 1) / Sh::COLS, p.heads, records.longer);
-    if (units > 0x7fffffffLL || grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
-    const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32 * DC_MAKERS), sizeof(DcMaker<T, DK>), stream, p, records);
-    if (rc != 0) return rc;
     // As many blocks as SMs had better not share any, which they do if they start while the records' blocks still hold some:
     // 8,192 tokens of 16 heads of 128 x 128 (64 blocks) take 366 us alone, 546 two to an SM.  More blocks, some of which may have
     // nothing to do (p.least: requests of many lengths), start behind the records' end and spread: 13 requests of 1 to 700 tokens,
@@ -1151,6 +1158,31 @@ static int launch_chunk(const DeltaParams& p, const DcRecords& records, int earl
     const bool alone = blocks <= sms, spread = !alone && blocks <= 2 * sms && p.least > 1;
     return launch_dependent_if(!spread, walker, grid, dim3(Sh::THREADS), alone ? (size_t)DC_ALONE_BYTES : sizeof(typename Sh::Shared),
                                stream, p, records);
+}
+
+template <typename T, int DK, bool WIDE>
+static int launch_chunk(const DeltaParams& p, const DcRecords& records, int early, cudaStream_t stream) {
+    auto maker = delta_records_kernel<T, DK, WIDE>;
+    static int sms = 0;                        // per process and kernel; harmless if repeated
+    if (sms == 0) {
+        int device = 0, count = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(maker, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DcMaker<T, DK>));
+        if (e != cudaSuccess) return (int)e;
+        sms = count;
+    }
+    const long long units = (long long)records.chunks * (p.heads / p.share);
+    if (units > 0x7fffffffLL || p.heads > 65535 || records.longer > 65535) return ERR_UNSUPPORTED;
+    const int rc = launch_dependent_if(early, maker, dim3((unsigned)units), dim3(32 * DC_MAKERS), sizeof(DcMaker<T, DK>), stream, p, records);
+    if (rc != 0) return rc;
+    // Half the rows per warp shorten a chunk's chain, twice the blocks solve for U twice as often: where they have an SM each it pays.
+    // 8,192 tokens of 16 heads of 128 x 128 (128 blocks) 312 us against 349, 1,024 in float32 56 against 65; 2,048 tokens of 20
+    // heads (160 blocks) 124 against 101.
+    constexpr int NARROW = DcShape<T, DK, 32>::COLS, COLS = DcShape<T, DK, 64>::COLS;
+    const dim3 narrow((p.vdim + NARROW - 1) / NARROW, p.heads, records.longer), wide((p.vdim + COLS - 1) / COLS, p.heads, records.longer);
+    return (long long)narrow.x * narrow.y * narrow.z <= sms ? launch_walk<T, DK, 32, WIDE>(p, records, narrow, sms, stream)
+                                                            : launch_walk<T, DK, 64, WIDE>(p, records, wide, sms, stream);
 }
 
 template <typename T, int DK>
