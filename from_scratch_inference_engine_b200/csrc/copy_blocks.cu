@@ -5,6 +5,8 @@
 // Bound by memory: every source is read and every destination written once (a source with several destinations comes
 // from L2 after its first read).  A thread block owns PART bytes of one pair, all of a thread's loads go out before
 // its first store, and the buffers' addresses travel with the launch, so that a fork of all layers is one launch.
+// 600 pages of 458,752 bytes: 80 us (6.9 TB/s); one state of 1 MB in each of 24 layers for eight forks: 36 us (226 MB, 6.3 TB/s); one
+// page: 3.6 us, a chain of list, load and store.
 // Pairs outside the pool are skipped and reported.
 #include "common.cuh"
 

@@ -11,7 +11,13 @@
 // A chunk is a chain - S0^T k, R, U, S - whose steps wait for one another, and a request's heads give a warp of its own to every
 // 16 columns and 64 rows of S only, so what bounds a prompt is the chain's latency.  A longer chunk puts more independent
 // instructions into every step; it adds to the two products that grow with the chunk (T R and the sum over u_j), by halves only
-// where the blocks of T above the diagonal are left out.  DC_MEASURED
+// where the blocks of T above the diagonal are left out.
+//
+// Measured (bfloat16, heads of 128 x 128): 8,192 tokens of 16 q/k and 32 heads 361 us - records 56, walk 322, a part of it beside
+// the records -, against 42 for their bytes; 0.7 TB/s.  A chunk of a block that has its SM alone takes 2,470 cycles for 984 of tensor
+// instructions (123 of 8 cycles per warp), and no step of the chain stands out; with two blocks on an SM 3,400 for both, so that
+// four prompts of 2,048 tokens of 32 heads (512 blocks in 296 places) take 328 us: records 77, walk 266.  Chunks of 16 tokens took
+// 530 us for the 8,192 when those of 32, in their first form, took 443.
 //
 // Precision.  States and outputs are 32-bit results, so no operand may be rounded to 11 bits.  q and k (bfloat16, 8 bits)
 // scaled by a power of two to a length of about one are exact in half precision; what is 32-bit - the state, R, U, T and the
@@ -22,12 +28,12 @@
 // and the instructions only ever sum up one chunk (their running sums are truncated, not rounded).  float32 storage: q and k
 // are two parts as well.
 //
-// Two kernels.  The first prepares all chunks side by side, a warp per chunk and q/k head: q and k in half precision, T by
+// Two kernels.  The first prepares all chunks side by side, a block per chunk and q/k head: q and k in half precision, T by
 // substitution, the weights of u_j, the gates' factors, as records in the workspace that lie as the second kernel's shared
-// memory holds them.  The second walks a head's chunks, a block for every 16 GROUPS value columns, four more warps keeping
-// the records and v of the next chunks on their way into a ring of stages; all meet once per chunk and nothing spins.  (One
-// kernel in which four more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads: every block of
-// value columns prepared them again, and the two roles' code did not fit the instruction cache together.)
+// memory holds them.  The second walks a head's chunks, a block for every 16 to 64 value columns, four more warps keeping
+// the records and v of the next chunks on their way into a ring of stages; all meet once per chunk.  (One kernel in which four
+// more warps per block prepared the chunks took 951 us for 8,192 tokens of 32 heads, the first form of the two 691: every block
+// of value columns prepared them again, and the two roles' code did not fit the instruction cache together.)
 //
 // Layout.  A warp of the second kernel owns 16 value columns x 64 or 32 rows of S, transposed: S^T is the 16-row operand of S0^T k
 // and S0^T q, the accumulator of S0^T k is (after R) the operand of the next product in the registers where it lies, and the
@@ -279,7 +285,9 @@ __device__ __forceinline__ void dc_copy_out(void* to, const void* from, int byte
 
 // A block of four warps per chunk and q/k head: they take eight tokens' q and k each, then three of them one block of the
 // products and weights each, the fourth the gates' sums.  (One warp for all of it held as much shared memory and left seven warps
-// on an SM: 60 us for 8,192 tokens of 16 q/k and 32 heads.)
+// on an SM.)  8,192 tokens of 32 heads of 128 columns: 77 us, 330 MB read and written, 4.3 TB/s; 8,192 tokens of 16 q/k and 32 heads
+// 56 us.  A block is a chain of nine steps behind barriers (7,300 cycles alone, 20,000 among others), shared memory is busy 65 % of
+// the time, and five blocks to an SM beat six (80 us) and seven (96).
 constexpr int DC_MAKERS = 4;
 
 template <typename T, int DK, bool WIDE>
@@ -558,7 +566,7 @@ enum { DC_MEET = 1, DC_PAIR = 2 };                   // named barriers; from DC_
 // A fetching thread's share of the copies into the ring, chunk after chunk: the addresses move on by a chunk with every call.
 // (Copied by the walkers themselves a chunk took them 800 cycles more, their own reads of shared memory queueing behind.  The
 // records come as two bulk copies: 16-byte copies of all the threads queued before the walkers' reads as well, 8,192 tokens of
-// 16 q/k and 32 heads took 366 us against 343.)
+// 16 heads took 366 us against 343.)
 template <typename T, int DK, int SLICE, bool WIDE>
 struct DcFetch {
     using Sh = DcShape<T, DK, SLICE>;
