@@ -159,17 +159,18 @@ delta_step_kernel(const DeltaParams p) {
 // ---------------------------------------------------------------------------------------------- many requests
 // The same for steps whose states are more than what the SMs work on at once.  What bounds the kernel above then is its
 // instructions: a thread has 16 numbers of S, and reading k and q, the sums over the warps and the lengths take it several times
-// what the S takes.  Here it has 64 or 32: a block of 2 DIM threads owns DIM rows (64 or 128) x 4 ACROSS columns, ACROSS threads
-// side by side in a row and groups of ACROSS / 2 rows.
-// 64 requests of 32 heads of 128 x 128 take 52 us (268 MB, 5.2 TB/s; the kernel above 61; a kernel that only reads and
-// writes such a state in place 43), 200 of 12 heads of 64 x 64 19 us (31), 16 of 16 heads 8.7 us (10.9).  What is left is the
-// block's own chain: lists, S, three meetings, S.  (One block per SM with the next two S on their way into its shared memory
-// took 70 us: its meetings hold up everything.)
+// what the S takes.  Here it has 64 or 32: a block of 2 DIM threads owns DIM rows (64, 96 or 128) x 4 ACROSS columns, ACROSS
+// threads side by side in a row and groups of ACROSS / 2 rows.
+// 64 requests of 32 heads of 128 x 128 take 49 us (268 MB, 5.4 TB/s; the kernel above 61; a kernel that only reads and
+// writes such a state in place 43), 100 of 16 heads of 128 x 160 52 us (57 with a block less per SM), 33 of 6 heads of 96 x 160
+// 7.6 us (9.4 with 128 rows to a block), 200 of 12 heads of 64 x 64 15 us.  What is left is the block's own chain: lists, S,
+// three meetings, S.  (One block per SM with the next two S on their way into its shared memory took 70 us: its meetings hold up
+// everything.)
 constexpr int HEAD_MAX_DIM = 128;
 constexpr int HEAD_FROM = 64;              // blocks
 
 template <typename T, int ACROSS, int DIM>
-__global__ void __launch_bounds__(2 * DIM, ACROSS == 16 ? (DIM == 128 ? 3 : 6) : DIM == 128 ? 2 : 4)
+__global__ void __launch_bounds__(2 * DIM, ACROSS == 16 ? (DIM == 128 ? 4 : DIM == 96 ? 5 : 8) : DIM == 128 ? 2 : DIM == 96 ? 3 : 4)
 delta_head_kernel(const DeltaParams p) {
     constexpr int COLS = 4 * ACROSS, ROWS = ACROSS / 2, WARPS = 2 * DIM / 32;
     __shared__ __align__(16) float ks[2][DIM], qs[2][DIM], sums[2][WARPS][COLS], us[2][COLS];
@@ -192,7 +193,7 @@ delta_head_kernel(const DeltaParams p) {
         grid_dependents_go();
     }
     // k by the first half of the threads, q by the other; v by the threads that sum up S^T k, later
-    const int d = tid & (DIM - 1), narrow = head / p.share * p.dim;
+    const int d = tid < DIM ? tid : tid - DIM, narrow = head / p.share * p.dim;
     const T* row = (const T*)p.qkv + (size_t)t0 * p.ld;
     auto part = [&](const T* from) { return d < p.dim ? to_float(from[(tid < DIM ? p.k_off : p.q_off) + narrow + d]) : 0.f; };
     float mine = part(row);
@@ -287,10 +288,12 @@ static int launch_step(const DeltaParams& p, int items, int early, cudaStream_t 
         const int across = p.vdim % 128 == 0 || p.vdim % 128 > 64 ? 32 : 16;
         const dim3 grid((p.vdim + 4 * across - 1) / (4 * across), p.heads, items);
         if ((long long)grid.x * grid.y * grid.z >= HEAD_FROM && grid.y <= 65535 && grid.z <= 65535)
-            return p.dim <= 64 ? launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 64> : delta_head_kernel<T, 16, 64>,
-                                                     grid, dim3(128), 0, stream, p)
-                               : launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 128> : delta_head_kernel<T, 16, 128>,
-                                                     grid, dim3(256), 0, stream, p);
+            return p.dim <= 64   ? launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 64> : delta_head_kernel<T, 16, 64>,
+                                                       grid, dim3(128), 0, stream, p)
+                   : p.dim <= 96 ? launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 96> : delta_head_kernel<T, 16, 96>,
+                                                       grid, dim3(192), 0, stream, p)
+                                 : launch_dependent_if(early, across == 32 ? delta_head_kernel<T, 32, 128> : delta_head_kernel<T, 16, 128>,
+                                                       grid, dim3(256), 0, stream, p);
     }
     const dim3 grid((p.vdim + STEP_COLS - 1) / STEP_COLS, p.heads, items);
     if (grid.y > 65535 || grid.z > 65535) return ERR_UNSUPPORTED;
