@@ -9,6 +9,7 @@ reaches the device in one copy from pinned host memory.
 from __future__ import annotations
 
 from dataclasses import dataclass
+from functools import cached_property
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
@@ -138,6 +139,16 @@ class StepContext:
             tables = take(I * width).view(I, width)
             self.groups.append(GroupStep(page_size, tables, take(T)))
         self._tiles: Dict[Tuple[int, int], Tiles] = {}
+
+    @cached_property
+    def longest(self) -> int:
+        """Tokens of the step's longest request."""
+        return int(self.h_qlen.max()) if self.num_items else 0
+
+    @cached_property
+    def ones(self) -> int:
+        """Requests of one token, or none."""
+        return int((self.h_qlen <= 1).sum())
 
     def attention_tiles(self, group_size: int, rows_per_tile: int) -> Tiles:
         """Tiles of `rows_per_tile` query rows, a row being (token, head of the group):

@@ -106,7 +106,7 @@ class GatedDeltaRule(Mixer):
         o = rt.buffer("gated_delta.o", tokens, self.v_width, torch.float32)
         ops.gated_delta_rule(act, 0, self.qk_width, 2 * self.qk_width, log_decay, beta, *items, cache.state, o, self.heads,
                              self.dim, self.vdim, share=self.heads // self.qk_heads, eps=self.eps,
-                             longest=int(ctx.h_qlen.max()), early=True, ones=int((ctx.h_qlen <= 1).sum()))
+                             longest=ctx.longest, early=True, ones=ctx.ones)
         gated = rt.buffer("gated_delta.gated", tokens, self.v_width, proj.dtype)
         ops.head_norm_silu(o, proj, gate0, self.gain, self.eps, gated, self.heads)
         return rt.linear(gated, self.w_o, None, "gated_delta.out")
