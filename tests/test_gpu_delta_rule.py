@@ -12,6 +12,7 @@ import plain_delta as plain
 pytestmark = pytest.mark.gpu
 UNIT = 2.0 ** -24
 FEW, MANY = 1, 1 << 20           # what the caller says about the longest request: the recurrent form, the chunked one
+CROWD = 1 << 21                  # the chunked one as among 400 more requests (padding entries): blocks share the SMs
 
 
 def ints(values):
@@ -43,12 +44,13 @@ class Case:
         out = torch.full((self.tokens, self.heads * self.vdim), 7e7, device="cuda")
         state = self.state.clone()
         done = [0] * self.items
+        padding = 400 if longest == CROWD else 0
         for part in portions or [self.lengths]:
             torch.cuda.synchronize()
             ops.gated_delta_rule(self.qkv, *self.offs, self.decay, self.beta,
-                                 ints([s + d for s, d in zip(self.starts, done)]), ints(part), ints(self.slots), self.items,
-                                 state, out, self.heads, self.dim, self.vdim, share=self.share, scale=scale, longest=longest,
-                                 early=early, ones=ones)
+                                 ints([s + d for s, d in zip(self.starts, done)] + [0] * padding), ints(part + [0] * padding),
+                                 ints(self.slots + [-1] * padding), self.items + padding, state, out, self.heads, self.dim,
+                                 self.vdim, share=self.share, scale=scale, longest=longest, early=early, ones=ones)
             done = [d + n for d, n in zip(done, part)]
         return out, state
 
@@ -80,27 +82,28 @@ def check(case, longest, units=32, **given):
         near(got, want, units)
 
 
-SIZES = [  # lengths, heads, share, dim, vdim: chunks of 16 that are full, begun, one token over; heads that fill tiles and do not
+SIZES = [  # lengths, heads, share, dim, vdim: chunks that are full, begun, one token over; heads that fill tiles and do not
+    ([32, 31, 33], 2, 1, 128, 128), ([64, 96, 65, 63], 2, 1, 64, 64), ([32], 3, 3, 80, 17),
     ([16], 2, 1, 128, 128), ([1], 3, 1, 64, 64), ([17, 1, 33], 4, 2, 128, 128), ([5, 64, 100, 15], 6, 3, 64, 64),
     ([200], 2, 1, 96, 80), ([31, 2], 2, 2, 32, 160), ([20, 9], 2, 1, 48, 32), ([18], 1, 1, 36, 20), ([40], 2, 1, 33, 19),
     ([7, 19], 2, 1, 100, 1), ([35], 1, 1, 1, 5), ([12, 3], 2, 1, 200, 64), ([9], 1, 1, 256, 36), ([130], 1, 1, 112, 256)]
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lengths,heads,share,dim,vdim", SIZES)
 def test_against_the_formula(lengths, heads, share, dim, vdim, dtype, longest):
     check(Case(lengths, heads, share, dim, vdim, dtype), longest)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 @pytest.mark.parametrize("lead,gap", [(3, 1), (4, 2), (8, 3)])
 def test_rows_and_slots_off_the_16_bytes(lead, gap, longest):
     check(Case([21, 34], 2, 1, 64, 64, torch.bfloat16, lead=lead, gap=gap), longest)
     check(Case([21, 34], 2, 1, 64, 64, torch.float32, lead=lead, gap=gap), longest)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_gates_at_their_ends(longest):
     case = Case([50, 33], 3, 1, 64, 96, torch.bfloat16)
     case.decay[::3], case.decay[1::7], case.decay[5], case.decay[11] = 0.0, -1e4, -float("inf"), -40.0
@@ -108,7 +111,7 @@ def test_gates_at_their_ends(longest):
     check(case, longest)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 @pytest.mark.parametrize("beta", [1.0, 2.0])
 def test_the_same_key_again_and_again(beta, longest):
     """Nothing decays and every key is the first one: a chunk's triangular system is as far from the unit matrix as it gets.
@@ -122,7 +125,7 @@ def test_the_same_key_again_and_again(beta, longest):
     check(case, longest, units=32 if beta < 2 else 32 + 6 * 70)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_keys_and_queries_of_nothing_and_of_all_sizes(longest):
     case = Case([60], 2, 1, 64, 64, torch.float32)
     factor = torch.tensor([0.0, 1e-6, 1e-3, 1.0, 300.0, 1e9], device="cuda")[torch.arange(60, device="cuda") % 6]
@@ -130,7 +133,7 @@ def test_keys_and_queries_of_nothing_and_of_all_sizes(longest):
     check(case, longest)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 @pytest.mark.parametrize("v_scale", [1e-25, 1e-6, 1e4, 1e20])
 def test_values_of_all_sizes(v_scale, longest):
     check(Case([70], 2, 1, 64, 64, torch.float32, v_scale=v_scale), longest)
@@ -138,7 +141,7 @@ def test_values_of_all_sizes(v_scale, longest):
     check(case, longest, scale=1.0)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_columns_of_all_sizes_side_by_side(longest):
     """Every column of the state has its own size: a column's error is measured against that column."""
     case = Case([90], 1, 1, 64, 64, torch.float32, lead=8)
@@ -152,7 +155,7 @@ def test_columns_of_all_sizes_side_by_side(longest):
         near(state[1, col:64 * 64:64], want_state[1, col:64 * 64:64])
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_memories_that_fade_by_many_orders(longest):
     """A large state that a few tokens forget, and small values behind it."""
     case = Case([64], 2, 1, 64, 64, torch.float32)
@@ -165,7 +168,7 @@ def test_memories_that_fade_by_many_orders(longest):
     near(state[1], want_state[1])
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_a_value_that_is_not_finite_stays_in_its_column_and_behind_its_token(bad, longest):
     case = Case([45, 20], 2, 1, 64, 64, torch.bfloat16)
@@ -184,7 +187,7 @@ def test_a_value_that_is_not_finite_stays_in_its_column_and_behind_its_token(bad
     near(state[case.slots[1]], want_state[case.slots[1]])
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 @pytest.mark.parametrize("which", ["q", "k", "decay", "beta", "state"])
 def test_what_is_not_finite_reaches_no_token_before_it(which, longest):
     case = Case([45], 2, 1, 64, 64, torch.bfloat16)
@@ -211,7 +214,7 @@ def test_what_is_not_finite_reaches_no_token_before_it(which, longest):
     near(out[~hit], want_out[~hit])
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_requests_without_slot_or_tokens_change_nothing(longest):
     case = Case([20, 18, 0, 5], 2, 1, 64, 64, torch.bfloat16)
     case.slots = [3, -1, 1, 5]
@@ -227,13 +230,13 @@ def test_requests_without_slot_or_tokens_change_nothing(longest):
     assert torch.equal(state[:, 2 * 64 * 64:], case.state[:, 2 * 64 * 64:])      # what else the slots hold
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_cut_into_portions(longest):
     case = Case([50, 23], 2, 1, 128, 64, torch.bfloat16)
     check(case, longest, portions=[[17, 0], [1, 16], [32, 7]])
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_long_and_the_same_bits_again(longest):
     """More tokens than the chunked form walks between two looks at the state's size, twice, and behind an early launch."""
     case = Case([1100], 1, 1, 64, 32, torch.bfloat16)
@@ -245,7 +248,7 @@ def test_long_and_the_same_bits_again(longest):
         assert torch.equal(first, again) and torch.equal(state, other)
 
 
-@pytest.mark.parametrize("longest", [FEW, MANY])
+@pytest.mark.parametrize("longest", [FEW, MANY, CROWD])
 def test_on_another_stream(longest):
     case = Case([40], 2, 1, 64, 64, torch.bfloat16)
     stream = torch.cuda.Stream()
