@@ -322,7 +322,8 @@ int fsie_delta_rule(int form, int few, int ones, const void* qkv, int ld, int q_
                     long long state_stride, float* out, int heads, int dim, int vdim, int share, float scale, float eps,
                     int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (items <= 0) return 0;
-    if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 1 || ones < 0 || (form == 1 && ones >= items)) return ERR_BAD_ARGUMENT;
+    if (heads <= 0 || dim <= 0 || vdim <= 0 || share <= 0 || heads % share != 0 || form < 0 || form > 1) return ERR_BAD_ARGUMENT;
+    if (ones < 0 || (form == 1 && ones >= items)) return ERR_BAD_ARGUMENT;
     DeltaParams p;
     p.qkv = qkv; p.ld = ld; p.q_off = q_off; p.k_off = k_off; p.v_off = v_off; p.log_decay = log_decay; p.beta = beta;
     p.item_qstart = item_qstart; p.item_qlen = item_qlen; p.item_slots = item_slots;

@@ -2391,7 +2391,9 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     heads * dim * vdim floats of a slot is read and left updated; out [tokens, heads * vdim] float32.  A request with a
     negative slot is passed over, its rows of `out` stay as they are.  `scale`: dim ** -0.5 unless given.  `longest`: the
     tokens of the step's longest request, which choose the kernel (0: not known to the caller); `ones`: at least so many of
-    the requests have one token, or none, and need no place among the longer ones (0 is always right).  dim is 256 at most.
+    the requests have one token, or none, and need no place among the longer ones (0 is always right; a number above theirs
+    leaves long requests out).  dim is 256 at most.  Requests walked in chunks take a workspace for the call: some 24 kB
+    (bfloat16, dim 128; float32 41) per head and 32 tokens.
     `early`: the state and the lists are older than the stream's last kernel, see the module's first lines."""
     f32, i32 = torch.float32, torch.int32
     if not (_fits(qkv, None, True) and _fits(log_decay, f32, True) and _fits(beta, f32, True) and _fits(out, f32, True)
