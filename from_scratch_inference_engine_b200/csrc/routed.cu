@@ -211,14 +211,27 @@ __global__ void moe_align_kernel(const int* __restrict__ ids, int pairs, int exp
         for (int r = threadIdx.x; r < start[experts]; r += blockDim.x) sorted[r] = -1;
     __syncthreads();
     // a pair's place among its expert's rows: in the order the threads arrive.  Each row of a
-    // product is summed on its own, so the order of an expert's rows changes no result.
-    for (int p = threadIdx.x; p < pairs; p += blockDim.x) {
-        const int e = ids[p];
-        if (e < 0 || e >= experts) continue;
+    // product is summed on its own, so the order of an expert's rows changes no result.  Two warps take turns, so that
+    // the lists of a few pairs are the same every time.
+    auto put = [&](int p, int e) {
+        if (e < 0 || e >= experts) return;
         const int at = start[e] + atomicAdd(&count[e], 1);
         sorted[at] = p;
         if (place) place[p] = at;
+    };
+    if (blockDim.x == 64) {
+        int next = threadIdx.x < pairs ? ids[threadIdx.x] : -1;
+        for (int p0 = 0; p0 < pairs; p0 += 64) {
+            const int p = p0 + threadIdx.x, e = next;
+            next = p + 64 < pairs ? ids[p + 64] : -1;
+            if (threadIdx.x < 32) put(p, e);
+            __syncthreads();
+            if (threadIdx.x >= 32) put(p, e);
+            __syncthreads();
+        }
+        return;
     }
+    for (int p = threadIdx.x; p < pairs; p += blockDim.x) put(p, ids[p]);
 }
 
 // ------------------------------------------------- choice and lists of a step in one launch
