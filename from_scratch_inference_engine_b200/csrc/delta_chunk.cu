@@ -22,11 +22,17 @@
 // Precision.  States and outputs are 32-bit results, so no operand may be rounded to 11 bits.  q and k (bfloat16, 8 bits)
 // scaled by a power of two to a length of about one are exact in half precision; what is 32-bit - the state, R, U, T and the
 // weights of u_j - goes into the instructions as the sum of two half-precision numbers (22 bits), products of two low parts left
-// out.  Half precision has little range: every column of the state (a row of the transposed tiles below) has a power of
-// two, `sigma`, chosen from the column's and the chunk's own largest numbers every 16 chunks, and anew, with the chunk's
-// sums taken again, whenever a number of R leaves the range in between.  The state itself stays in 32-bit registers
-// and the instructions only ever sum up one chunk (their running sums are truncated, not rounded).  float32 storage: q and k
-// are two parts as well.
+// out.  The state itself stays in 32-bit registers and the instructions only ever sum up one chunk (their running sums are
+// truncated, not rounded).  float32 storage: q and k are two parts as well.
+//
+// Range.  Half precision has little of it: a pair ends at 2^-25, 22 bits below a number of 2^-3.  Where a sum of its own takes the low
+// parts' products they go in 2^11 times as large (DC_LOW), so that the pairs of R, U, T and the weights end at 2^-36; T and the weights
+// are stored 2^11 and 2^14 times as large besides.  Every column of the state (a row of the transposed tiles below) has a power of two,
+// `sigma`, chosen in a look at the column's and the first chunk's largest numbers, and anew, the chunk's sums taken again, when a chunk
+// is out of range: when a number of U is too large, when next to nothing of a column's is taken into the state, or when next to nothing is
+// stored at some token and the column holds no more (DC_LEAST...).  Where that is so even right behind a look - a large value that is
+// forgotten within its chunk, small ones in front of a large one -, where a state is small beside the values, or where something is not
+// finite, the warps of the 16 columns walk the chunk token by token in 32 bits, as the recurrence is written.
 //
 // Two kernels.  The first prepares all chunks side by side, a block per chunk and q/k head: q and k in half precision, T by
 // substitution, the weights of u_j, the gates' factors, as records in the workspace that lie as the second kernel's shared
@@ -40,9 +46,8 @@
 // new sums end up where S lies.  Heads of more rows take two or four warps per 16 columns, which swap their rows' sums
 // of S0^T k through shared memory, in the chunk's one meeting; those of S0^T q the fetching warps add up.
 //
-// Values that are not finite: they spoil their column from their token on and nothing else, as in the recurrence - a product
-// with a zero of T would spoil the tokens before.  Such chunks are noticed by R and by a mark in their record, redone with those
-// values left out, and what they reach is set to NaN.
+// Values that are not finite spoil their column from their token on and nothing else, as in the recurrence: a product with a zero
+// of T would spoil the tokens before, so such chunks, noticed by U, are walked token by token.
 #include "common.cuh"
 #include "delta_rule.cuh"
 #include "tma.cuh"
@@ -57,14 +62,22 @@ constexpr int DC_STAGES = 3;               // stages of the ring: the chunk's, t
 constexpr int DC_WALKERS = 4;              // warps that walk a block's chunks
 constexpr int DC_FETCHERS = 128;           // threads that copy
 constexpr int DC_MAX_DIM = 128;
-constexpr int DC_REFRESH = 16;             // chunks between two looks at the state's size
-constexpr int DC_SIZE = 3;                 // ... which brings the largest number of a column to 2^3 .. 2^4
+constexpr int DC_SIZE = 12;                // a look brings the largest number of a column to 2^12 .. 2^13
+constexpr int DC_DOWN = 3;                 // ... or, where R or U are then too large, to 2^-DC_DOWN of that
+constexpr float DC_LOW = 2048.f;           // on a low part whose products have a sum of their own
+constexpr float DC_T_SCALE = DC_LOW;       // on T, whose numbers are below beta^2 <= 4, as its record has it
+constexpr float DC_P_SCALE = 16384.f;      // ... and on the weights of u_j, which are below 1
 constexpr int DC_TLD = 16 + 8;             // padded rows of a 16 x 16 block in scratch
 constexpr int DC_ALD = 16 + 4;             // ... of floats
-// A number of R, times sigma, is below this: right behind a look it is at most 2^4 (1 + sqrt(128)).  A row of T has 32 numbers
-// of at most beta^2 <= 4 (what a token's value still does to a later token's u passes through contractions), so that u, and
-// u with a factor of at most 2, fit half precision.
-constexpr float DC_MOST = 250.f;
+// Numbers of U, times sigma, are below this: u with a factor of at most 2 then fits half precision.  (Those of R do if U is finite.)
+// Right behind a look R is at most 2^13 (1 + sqrt(128)), 12,300 with DC_DOWN.
+constexpr float DC_MOST = 32000.f;
+// What a column holds at a token, times sigma, is no less than this: R and U, as pairs, end at 2^-36, and what the weights' pairs leave
+// of a number of DC_MOST at 2^-32.
+constexpr float DC_LEAST = 1.f / 4096;
+// ... and the state, ahead of a chunk and behind it: its pairs, and those of what it takes in, end at 2^-25.  32 tokens' roundings there,
+// of either sign, are 2^-23.3 together, six units of 2^-24 beside this.
+constexpr float DC_LEAST_STATE = 1.f / 4;
 
 __device__ __forceinline__ unsigned dc_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void dc_ldmatrix(unsigned (&r)[4], const void* p) {
@@ -129,12 +142,28 @@ __device__ __forceinline__ void dc_split(float x, float y, unsigned& high, unsig
     dc_add2(lx, ly, x, y, -f.x, -f.y);
     low = dc_bits(__floats2half2_rn(lx, ly));
 }
+// the same from x and y times DC_LOW, the low part times DC_LOW
+__device__ __forceinline__ void dc_split_far(float x, float y, unsigned& high, unsigned& low) {
+    float hx, hy;
+    dc_mul2(hx, hy, x, y, 1.f / DC_LOW, 1.f / DC_LOW);
+    const __half2 h = __floats2half2_rn(hx, hy);
+    const float2 f = __half22float2(h);
+    high = dc_bits(h);
+    dc_fma2(hx, hy, f.x, f.y, -DC_LOW, -DC_LOW, x, y);
+    low = dc_bits(__floats2half2_rn(hx, hy));
+}
 // the 16 x 16 operand of two neighbouring accumulator tiles, in two parts
 __device__ __forceinline__ void dc_split_tiles(const float (&x)[4], const float (&y)[4], unsigned (&high)[4], unsigned (&low)[4]) {
     dc_split(x[0], x[1], high[0], low[0]);
     dc_split(x[2], x[3], high[1], low[1]);
     dc_split(y[0], y[1], high[2], low[2]);
     dc_split(y[2], y[3], high[3], low[3]);
+}
+__device__ __forceinline__ void dc_split_tiles_far(const float (&x)[4], const float (&y)[4], unsigned (&high)[4], unsigned (&low)[4]) {
+    dc_split_far(x[0], x[1], high[0], low[0]);
+    dc_split_far(x[2], x[3], high[1], low[1]);
+    dc_split_far(y[0], y[1], high[2], low[2]);
+    dc_split_far(y[2], y[3], high[3], low[3]);
 }
 __device__ __forceinline__ float dc_power(int e) { return __int_as_float((e + 127) << 23); }     // 2^e, e in -126..127
 
@@ -195,11 +224,11 @@ struct DcRecord {
     struct alignas(16) Keys { __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD]; };
     struct alignas(16) Gates {
         __half t[2][3][16][16], p[2][3][16][16];               // T and the weights of u_j, two parts each; dc_piece()
-        float before[DC_TOKENS];          // on S0^T k: e^(G_i), the key's length, the power of two
-        float after[DC_TOKENS];           // on u_j in the new state: e^(G_31 - G_j), ...
-        float query[DC_TOKENS];           // on an output: scale, the query's length, the power of two
-        float fade[DC_TOKENS];            // e^(G_i)
-        float odd[4];                     // NaN where T has a number that is not finite, else 0
+        float before[DC_TOKENS];          // on S0^T k: e^(G_i), the key's length, the power of two, DC_LOW
+        float after[DC_TOKENS];           // on u_j in the new state: e^(G_31 - G_j), ..., one over DC_T_SCALE
+        float query[DC_TOKENS];           // on an output: scale, the query's length, the power of two, one over DC_P_SCALE
+        float fade[DC_TOKENS];            // e^(G_i), times DC_P_SCALE, as the weights of u_j are
+        float key[DC_TOKENS], decay[DC_TOKENS], beta[DC_TOKENS];        // the key's length, the power of two; e^log_decay; beta
     };
 };
 
@@ -222,7 +251,7 @@ struct DcShape : DcRecord<T, DK> {
         float4 swap[2][SLICES > 1 ? DC_WALKERS : 1][DC_TILES][32];      // S0^T k of a warp's rows
         float out[2][SLICES][DC_TOKENS][OLD];      // a chunk's outputs without the factors, a summand per warp of the 16 columns
         float back[2][COLS];                       // what its columns are still to be multiplied by
-        float most[DC_WALKERS][16];
+        float most[2][DC_WALKERS][16];             // of looks; of the search for what is too small
         uint64_t full[DC_STAGES];                  // a stage's records are there
         int lost;                                  // ... or were waited for in vain
     };
@@ -250,7 +279,7 @@ __device__ __forceinline__ int dc_find(const int* __restrict__ item_qlen, int it
     return -1;
 }
 
-// A product of two 16 x 16 matrices in two parts each: sum += a b, b's operand registers as ldmatrix gives them.
+// A product of two 16 x 16 matrices in two parts each, low ones times DC_LOW: sum += a b, b's operand registers as ldmatrix gives them.
 __device__ __forceinline__ void dc_product(float (&sum)[2][4], const unsigned (&ah)[4], const unsigned (&al)[4], const unsigned (&bh)[4],
                                            const unsigned (&bl)[4]) {
     float low[2][4];
@@ -265,7 +294,7 @@ __device__ __forceinline__ void dc_product(float (&sum)[2][4], const unsigned (&
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum[j][e] += low[j][e];
+        for (int e = 0; e < 4; ++e) sum[j][e] = fmaf(low[j][e], 1.f / DC_LOW, sum[j][e]);
 }
 
 template <typename T, int DK>
@@ -428,10 +457,13 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
                 __syncwarp();
             }
-            own.gates.before[lane] = fade * kf;
-            own.gates.after[lane] = expf((float)(all - sum)) * kf;
-            own.gates.query[lane] = own.qf[lane];
-            own.gates.fade[lane] = fade;
+            own.gates.before[lane] = fade * kf * DC_LOW;
+            own.gates.after[lane] = expf((float)(all - sum)) * kf * (1.f / DC_T_SCALE);
+            own.gates.query[lane] = own.qf[lane] * (1.f / DC_P_SCALE);
+            own.gates.fade[lane] = fade * DC_P_SCALE;
+            own.gates.key[lane] = kf;
+            own.gates.decay[lane] = expf(decay);
+            own.gates.beta[lane] = beta;
             if (z + 1 < p.share && lane < n) {                 // the next head's
                 decay = p.log_decay[(size_t)(first + lane) * p.heads + head + 1];
                 beta = p.beta[(size_t)(first + lane) * p.heads + head + 1];
@@ -451,7 +483,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                     const double gr = own.g[row];
                     const float e0 = expf((float)(gr - g0)) * f0, e1 = expf((float)(gr - g1)) * f1;
                     unsigned high, low;
-                    dc_split(row >= col ? qkt[j][2 * h] * e0 : 0.f, row > col ? qkt[j][2 * h + 1] * e1 : 0.f, high, low);
+                    dc_split_far(row >= col ? qkt[j][2 * h] * e0 * (DC_P_SCALE * DC_LOW) : 0.f, row > col ? qkt[j][2 * h + 1] * e1 * (DC_P_SCALE * DC_LOW) : 0.f, high, low);
                     *reinterpret_cast<unsigned*>(&own.gates.p[0][warp][br][dc_piece(br, j) + 2 * t]) = high;
                     *reinterpret_cast<unsigned*>(&own.gates.p[1][warp][br][dc_piece(br, j) + 2 * t]) = low;
                     const float x = own.kf[row] * kkt[j][2 * h] * e0, y = own.kf[row] * kkt[j][2 * h + 1] * e1;
@@ -482,17 +514,11 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                     x[j + 2] = fmaf(xl, a.z, x[j + 2]); x[j + 3] = fmaf(xl, a.w, x[j + 3]);
                 }
             }
-            bool finite = true;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                x[j] = j <= i ? x[j] * own.beta[16 * m + j] : 0.f;
-                finite = finite && fabsf(x[j]) < INFINITY;
-            }
-            const bool odd = !__all_sync(0xffffffffu, finite);
-            if (lane == 0) own.gates.odd[0] = odd ? __int_as_float(0x7fffffff) : 0.f;
+            for (int j = 0; j < 16; ++j) x[j] = j <= i ? x[j] * own.beta[16 * m + j] : 0.f;
             unsigned high[8], low[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dc_split(x[2 * j], x[2 * j + 1], high[j], low[j]);
+            for (int j = 0; j < 8; ++j) dc_split_far(x[2 * j] * (DC_T_SCALE * DC_LOW), x[2 * j + 1] * (DC_T_SCALE * DC_LOW), high[j], low[j]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 *reinterpret_cast<uint4*>(&own.gates.t[0][2 * m][i][dc_piece(i, j)]) = make_uint4(high[4 * j], high[4 * j + 1], high[4 * j + 2], high[4 * j + 3]);
@@ -501,14 +527,20 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
         }
         __syncthreads();
         if (warp == 1) {
-            // block (1, 0): -T_11 (A_10 / beta) T_00, beta being in T_11
+            // block (1, 0): -T_11 (A_10 / beta) T_00, beta being in T_11; A's numbers are below 1 and those of the second product, 16
+            // summands, below 64: both go in DC_INNER times as large
+            constexpr float DC_INNER = 512.f;
             unsigned ah[4], al[4], bh[4], bl[4];
             float w[2][4];
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[j][e] = 0.f;
-            dc_split_tiles(below[0], below[1], ah, al);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) below[j][e] *= DC_INNER * DC_LOW;
+            dc_split_tiles_far(below[0], below[1], ah, al);
             dc_ldmatrix_trans(bh, &own.gates.t[0][0][bt_row][dc_piece(bt_row, lane >> 4)]);
             dc_ldmatrix_trans(bl, &own.gates.t[1][0][bt_row][dc_piece(bt_row, lane >> 4)]);
             dc_product(w, ah, al, bh, bl);
@@ -517,9 +549,9 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float x = w[j][2 * h], y = w[j][2 * h + 1];
+                    const float x = w[j][2 * h], y = w[j][2 * h + 1];      // (T has DC_T_SCALE, which is DC_LOW)
                     unsigned high, low;
-                    dc_split(fabsf(x) < INFINITY ? -x : 0.f, fabsf(y) < INFINITY ? -y : 0.f, high, low);
+                    dc_split_far(fabsf(x) < INFINITY ? -x : 0.f, fabsf(y) < INFINITY ? -y : 0.f, high, low);
                     *reinterpret_cast<unsigned*>(&own.w[0][g + 8 * h][8 * j + 2 * t]) = high;
                     *reinterpret_cast<unsigned*>(&own.w[1][g + 8 * h][8 * j + 2 * t]) = low;
                 }
@@ -538,7 +570,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     unsigned high, low;
-                    dc_split(w[j][2 * h], w[j][2 * h + 1], high, low);
+                    dc_split_far(w[j][2 * h] * (DC_LOW / DC_INNER), w[j][2 * h + 1] * (DC_LOW / DC_INNER), high, low);
                     *reinterpret_cast<unsigned*>(&own.gates.t[0][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = high;
                     *reinterpret_cast<unsigned*>(&own.gates.t[1][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = low;
                 }
@@ -677,7 +709,7 @@ template <> struct DcValues<float> {
     }
 };
 
-// U = T R, all in two parts; th, tl: T's blocks (0, 0), (1, 0), (1, 1)
+// U = T R, times DC_T_SCALE, all in two parts; th, tl: T's blocks (0, 0), (1, 0), (1, 1)
 __device__ __forceinline__ void dc_solve(float (&u)[DC_TILES][4], const unsigned (&rh)[2][4], const unsigned (&rl)[2][4],
                                          const unsigned (&th)[3][4], const unsigned (&tl)[3][4]) {
     float low[DC_TILES][4];
@@ -696,30 +728,7 @@ __device__ __forceinline__ void dc_solve(float (&u)[DC_TILES][4], const unsigned
 #pragma unroll
     for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) dc_add2(u[j][e], u[j][e + 1], u[j][e], u[j][e + 1], low[j][e], low[j][e + 1]);
-}
-
-// the first token of each of the thread's two rows whose value is not finite (DC_TOKENS: none), over the row's four lanes
-__device__ __forceinline__ void dc_first_bad(const float (&x)[DC_TILES][4], int t, int (&first)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        int at = DC_TOKENS;
-#pragma unroll
-        for (int j = DC_TILES - 1; j >= 0; --j)
-#pragma unroll
-            for (int e = 1; e >= 0; --e)
-                if (!(fabsf(x[j][2 * h + e]) < INFINITY)) at = 8 * j + 2 * t + e;
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) at = min(at, __shfl_xor_sync(0xffffffffu, at, o));
-        first[h] = min(first[h], at);
-    }
-}
-__device__ __forceinline__ void dc_leave_out(float (&x)[DC_TILES][4], int t, const int (&first)[2]) {
-#pragma unroll
-    for (int j = 0; j < DC_TILES; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (8 * j + 2 * t + (e & 1) >= first[e >> 1]) x[j][e] = 0.f;
+        for (int e = 0; e < 4; e += 2) dc_fma2(u[j][e], u[j][e + 1], low[j][e], low[j][e + 1], 1.f / DC_LOW, 1.f / DC_LOW, u[j][e], u[j][e + 1]);
 }
 
 template <typename T, int DK, int SLICE, bool WIDE>
@@ -849,76 +858,202 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 for (int e = 0; e < 4; ++e) v.x[4 * j + e] = st.v[8 * j + 2 * t + (e & 1)][group * 16 + g + 8 * (e >> 1)];
         }
     };
-    dc_sync(DC_MEET, Sh::THREADS);                             // stage 0 is there
-    ask(sm.stage[0]);
-
-    for (int c = 0, stage = 0, next = 1; c < chunks; ++c, stage = next, next = next + 1 < DC_STAGES ? next + 1 : 0) {
-        const auto& st = sm.stage[stage];
-        bool look = c % DC_REFRESH == 0, spoiled = false;
-        int bad[2] = {DC_TOKENS, DC_TOKENS};
-        float u[DC_TILES][4], wq[DC_TILES][4];                 // U; S0^T q
-        unsigned bq[2][4];                                     // Q
-        unsigned sh[STEPS][4], sl[STEPS][4];                   // the state in two parts
-        auto ask_query = [&](int k) {
+    // v of a token in the thread's columns
+    auto value = [&](const typename Sh::Stage& st, int i, int h) {
+        return to_float(st.v[i][sizeof(T) == 2 ? Sh::v_piece(i, group * 2 + h) * 8 + g : group * 16 + 8 * h + g]);
+    };
+    // the largest number of the thread's two columns of S, over all the warps that have rows of them, without sigma
+    auto largest = [&](float (&most)[2], float (&swap)[DC_WALKERS][16]) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][(16 * m ^ q_half) + q_row][row0 + 16 * k + b_col]);
-        };
-        // a quarter of the instructions of S0^T q: they stand where the chain of R, U and the new state has to wait
-        auto query_step = [&](int k) {
-            if (k >= STEPS) return;
+        for (int h = 0; h < 2; ++h) {
+            most[h] = 0.f;
 #pragma unroll
-            for (int j = 0; j < DC_TILES; ++j) dc_mma_if(k == 0, wq[j], sl[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
-            if (PARTS == 2) {
+            for (int n = 0; n < TILES; ++n) most[h] = fmaxf(most[h], fmaxf(fabsf(s[n][2 * h]), fabsf(s[n][2 * h + 1])));
+            most[h] *= back[h];
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    unsigned b[4];
-                    dc_ldmatrix(b, &st.keys.q[PARTS - 1][(16 * m ^ q_half) + q_row][row0 + 16 * k + b_col]);
-                    dc_mma(wq[2 * m], sh[k], b[0], b[1]);
-                    dc_mma(wq[2 * m + 1], sh[k], b[2], b[3]);
-                }
+            for (int o = 1; o < 4; o <<= 1) most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], o));
+        }
+        if (SLICES > 1) {
+            if (t == 0) { swap[warp][g] = most[0]; swap[warp][g + 8] = most[1]; }
+            dc_sync(DC_PAIR + group, 32 * SLICES);
+#pragma unroll
+            for (int s = 1; s < SLICES; ++s) {
+                most[0] = fmaxf(most[0], swap[warp ^ s][g]);
+                most[1] = fmaxf(most[1], swap[warp ^ s][g + 8]);
             }
+        }
+    };
+    const float least[2] = {col < p.vdim ? DC_LEAST * DC_T_SCALE : -1.f, col + 8 < p.vdim ? DC_LEAST * DC_T_SCALE : -1.f};
+    const float least_state[2] = {col < p.vdim ? DC_LEAST_STATE : -1.f, col + 8 < p.vdim ? DC_LEAST_STATE : -1.f};
+    enum { FRESH, LITTLE, MUCH };                              // why a chunk is not walked just so: no sigma yet, small numbers, large ones
+    int why = FRESH, down = 0, c = 0, stage = 0;
+    bool looked = false, met = false;                          // sigma is this chunk's own; the chunk's meeting has been
+    auto through = [&] {                                       // with chunk c
+        ++c;
+        stage = stage + 1 < DC_STAGES ? stage + 1 : 0;
+        looked = met = false;
+    };
+    dc_sync(DC_MEET, Sh::THREADS);                             // stage 0 is there
+
+    while (c < chunks) {
+        bool by_token = false, passed = false;
+        {
+            const auto& st = sm.stage[stage];
+            const int tokens = min(DC_TOKENS, count - c * DC_TOKENS);
+            ask(st);
+            if (why == LITTLE) {
+                // Nearly nothing is stored at a token, or taken in.  What the columns hold: the state's largest number and the values, faded.
+                float most[2];
+                largest(most, sm.most[1]);
+                bool small = false;
+                most[0] *= sigma[0]; most[1] *= sigma[1];
+#pragma unroll 2
+                for (int i = 0; i < tokens; ++i) {
+                    const float decay = st.gates.decay[i], beta = st.gates.beta[i], least = i + 1 < tokens ? DC_LEAST : DC_LEAST_STATE;
 #pragma unroll
-            for (int j = 0; j < DC_TILES; ++j) dc_mma(wq[j], sh[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
-            if (k + 1 < STEPS) ask_query(k + 1);
-        };
-        for (int tries = 0;; ++tries) {
-            if (__builtin_expect(look, 0)) {                   // the columns' powers of two from the columns themselves
-                float most[2], raw[DC_TILES][4];
+                    for (int h = 0; h < 2; ++h) {
+                        most[h] = fmaxf(most[h] * decay, fabsf(value(st, i, h)) * beta * sigma[h]);
+                        small = small || (most[h] > 0.f && most[h] < least);
+                    }
+                }
+                passed = !__any_sync(0xffffffffu, small);
+            }
+            if (!passed && looked && !(why == MUCH && down == 0)) {
+                by_token = true;                               // not a matter of sigma
+            } else if (!passed) {
+                // the columns' powers of two from the columns themselves; token by token where a state is small beside the values
+                down = looked ? DC_DOWN : 0;
+                looked = true;
+                float most[2], held[2], raw[DC_TILES][4];
                 v.widen(raw);
+                largest(most, sm.most[0]);
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    most[h] = 0.f;
-#pragma unroll
-                    for (int n = 0; n < TILES; ++n) most[h] = fmaxf(most[h], fmaxf(fabsf(s[n][2 * h]), fabsf(s[n][2 * h + 1])));
-                    most[h] *= back[h];
+                    float x = 0.f;
 #pragma unroll
                     for (int j = 0; j < DC_TILES; ++j)
 #pragma unroll
                         for (int e = 2 * h; e < 2 * h + 2; ++e)        // (an infinite value must not move its column's power)
-                            if (fabsf(raw[j][e]) < INFINITY) most[h] = fmaxf(most[h], fabsf(raw[j][e]));
+                            if (fabsf(raw[j][e]) < INFINITY) x = fmaxf(x, fabsf(raw[j][e]));
 #pragma unroll
-                    for (int o = 1; o < 4; o <<= 1) most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], o));
-                }
-                if (SLICES > 1) {
-                    if (t == 0) { sm.most[warp][g] = most[0]; sm.most[warp][g + 8] = most[1]; }
-                    dc_sync(DC_PAIR + group, 32 * SLICES);
-#pragma unroll
-                    for (int s = 1; s < SLICES; ++s) {
-                        most[0] = fmaxf(most[0], sm.most[warp ^ s][g]);
-                        most[1] = fmaxf(most[1], sm.most[warp ^ s][g + 8]);
-                    }
+                    for (int o = 1; o < 4; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+                    held[h] = most[h];
+                    most[h] = fmaxf(most[h], x);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int e = DC_SIZE - (((__float_as_int(most[h]) >> 23) & 255) - 127);
+                    const int e = DC_SIZE - down - (((__float_as_int(most[h]) >> 23) & 255) - 127);
                     const float next = most[h] > 0.f ? dc_power(min(max(e, -100), 100)) : sigma[h];
                     const float factor = next * back[h];
                     sigma[h] = next;
                     back[h] = 1.f / next;
+                    by_token = by_token || (held[h] > 0.f && held[h] * next < DC_LEAST_STATE);
 #pragma unroll
                     for (int n = 0; n < TILES; ++n) { s[n][2 * h] *= factor; s[n][2 * h + 1] *= factor; }
                 }
+                by_token = __any_sync(0xffffffffu, by_token);
             }
+            if (by_token) {
+                // ---- the recurrence, token by token
+                if (!met) dc_sync(DC_MEET, Sh::THREADS);
+                else if (SLICES > 1) dc_sync(DC_PAIR + group, 32 * SLICES);       // the swapped sums have been read
+#pragma unroll 1
+                for (int i = 0; i < tokens; ++i) {
+                    float with_k[2] = {0.f, 0.f}, with_q[2] = {0.f, 0.f}, kq = 0.f;
+                    auto both = [&](const __half (&rows)[PARTS][DC_TOKENS][Sh::KLD], int n) {
+                        float2 x = __half22float2(*reinterpret_cast<const __half2*>(&rows[0][i][row0 + 8 * n + 2 * t]));
+                        if (PARTS == 2) {
+                            const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&rows[PARTS - 1][i][row0 + 8 * n + 2 * t]));
+                            x.x += y.x; x.y += y.y;
+                        }
+                        return x;
+                    };
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) {
+                        const float2 k = both(st.keys.k, n), q = both(st.keys.q, n);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            with_k[h] = fmaf(s[n][2 * h + 1], k.y, fmaf(s[n][2 * h], k.x, with_k[h]));
+                            with_q[h] = fmaf(s[n][2 * h + 1], q.y, fmaf(s[n][2 * h], q.x, with_q[h]));
+                        }
+                        kq = fmaf(k.y, q.y, fmaf(k.x, q.x, kq));
+                    }
+#pragma unroll
+                    for (int o = 1; o < 4; o <<= 1) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            with_k[h] += __shfl_xor_sync(0xffffffffu, with_k[h], o);
+                            with_q[h] += __shfl_xor_sync(0xffffffffu, with_q[h], o);
+                        }
+                        kq += __shfl_xor_sync(0xffffffffu, kq, o);
+                    }
+                    if (SLICES > 1) {                          // (two places in turn: one meeting a token)
+                        if (t == 0) sm.swap[c & 1][warp][i & 1][g] = make_float4(with_k[0], with_k[1], 0.f, 0.f);
+                        dc_sync(DC_PAIR + group, 32 * SLICES);
+                        with_k[0] = with_k[1] = 0.f;
+#pragma unroll
+                        for (int x = 0; x < SLICES; ++x) {     // the same sum in all the warps
+                            const float4 part = sm.swap[c & 1][group * SLICES + x][i & 1][g];
+                            with_k[0] += part.x; with_k[1] += part.y;
+                        }
+                    }
+                    const float key = st.gates.key[i], decay = st.gates.decay[i], beta = st.gates.beta[i];
+                    float now[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        now[h] = beta * (value(st, i, h) * sigma[h] - decay * key * with_k[h]);
+                        // a warp's own rows' summand of the output
+                        if (t == 0) sm.out[c & 1][slice][i][group * 16 + 8 * h + g] = DC_P_SCALE * (decay * with_q[h] + kq * key * now[h]);
+                    }
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) {
+                        const float2 k = both(st.keys.k, n);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            s[n][2 * h] = fmaf(k.x * key, now[h], decay * s[n][2 * h]);
+                            s[n][2 * h + 1] = fmaf(k.y * key, now[h], decay * s[n][2 * h + 1]);
+                        }
+                    }
+                }
+                if (slice == 0 && t == 0) {
+                    sm.back[c & 1][group * 16 + g] = back[0];
+                    sm.back[c & 1][group * 16 + g + 8] = back[1];
+                }
+                why = FRESH;
+                through();
+                continue;
+            }
+        }
+        // ---- chunk after chunk, until one is out of range
+        for (;;) {
+            const auto& st = sm.stage[stage];
+            const int tokens = min(DC_TOKENS, count - c * DC_TOKENS);
+            float u[DC_TILES][4], wq[DC_TILES][4];             // U, times DC_T_SCALE; S0^T q
+            unsigned bq[2][4];                                 // Q
+            unsigned sh[STEPS][4], sl[STEPS][4];               // the state in two parts
+            auto ask_query = [&](int k) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) dc_ldmatrix(bq[m], &st.keys.q[0][(16 * m ^ q_half) + q_row][row0 + 16 * k + b_col]);
+            };
+            // a quarter of the instructions of S0^T q: they stand where the chain of R, U and the new state has to wait
+            auto query_step = [&](int k) {
+                if (k >= STEPS) return;
+#pragma unroll
+                for (int j = 0; j < DC_TILES; ++j) dc_mma_if(k == 0, wq[j], sl[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+                if (PARTS == 2) {
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        unsigned b[4];
+                        dc_ldmatrix(b, &st.keys.q[PARTS - 1][(16 * m ^ q_half) + q_row][row0 + 16 * k + b_col]);
+                        dc_mma(wq[2 * m], sh[k], b[0], b[1]);
+                        dc_mma(wq[2 * m + 1], sh[k], b[2], b[3]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < DC_TILES; ++j) dc_mma(wq[j], sh[k], bq[j >> 1][2 * (j & 1)], bq[j >> 1][2 * (j & 1) + 1]);
+                if (k + 1 < STEPS) ask_query(k + 1);
+            };
+            float add[TILES][4], oa[FINISH][4], ob[FINISH][4];     // what the new state takes in; outputs
             // ---- S0^T k of the warp's rows: 16 columns x 32 tokens; the next rows are taken apart meanwhile
             float wk[DC_TILES][4], lk[DC_TILES][4];
             dc_split_tiles(s[0], s[1], sh[0], sl[0]);
@@ -951,9 +1086,8 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             float2 before[DC_TILES];
 #pragma unroll
             for (int j = 0; j < DC_TILES; ++j) before[j] = *reinterpret_cast<const float2*>(&st.gates.before[8 * j + 2 * t]);
-            float size = st.gates.odd[0];                      // NaN where T is not finite
             // ---- one meeting per chunk: the halves' sums are there, and so is the next stage
-            if (tries == 0) dc_sync(DC_MEET, Sh::THREADS);
+            if (!met) dc_sync(DC_MEET, Sh::THREADS);
             else if (SLICES > 1) dc_sync(DC_PAIR + group, 32 * SLICES);
             if constexpr (SLICES > 1) {
                 float4 x[DC_TILES];
@@ -979,7 +1113,8 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             } else {
                 query_step(0);
             }
-            // ---- R, U
+            // ---- R, times DC_LOW, and U
+            const float sigma_far[2] = {sigma[0] * DC_LOW, sigma[1] * DC_LOW};
             float r[DC_TILES][4];
             v.widen(r);
 #pragma unroll
@@ -987,9 +1122,8 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float x, y;
-                    dc_mul2(x, y, r[j][2 * h], r[j][2 * h + 1], sigma[h], sigma[h]);
+                    dc_mul2(x, y, r[j][2 * h], r[j][2 * h + 1], sigma_far[h], sigma_far[h]);
                     dc_fma2(r[j][2 * h], r[j][2 * h + 1], -before[j].x, -before[j].y, wk[j][2 * h], wk[j][2 * h + 1], x, y);
-                    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(size) : "f"(fabsf(r[j][2 * h])), "f"(fabsf(r[j][2 * h + 1])));
                 }
             unsigned rh[2][4], rl[2][4], th[3][4], tl[3][4];
 #pragma unroll
@@ -997,139 +1131,153 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 dc_ldmatrix(th[b], &st.gates.t[0][b][b_row][b_piece]);
                 dc_ldmatrix(tl[b], &st.gates.t[1][b][b_row][b_piece]);
             }
-            dc_split_tiles(r[0], r[1], rh[0], rl[0]);
+            dc_split_tiles_far(r[0], r[1], rh[0], rl[0]);
             query_step(1);
-            dc_split_tiles(r[2], r[3], rh[1], rl[1]);
+            dc_split_tiles_far(r[2], r[3], rh[1], rl[1]);
             dc_solve(u, rh, rl, th, tl);
             query_step(2);
-            if (__builtin_expect(!__any_sync(0xffffffffu, !(size < DC_MOST)), 1)) break;
-            if (tries == 0) {                                  // (both warps of 16 columns have the same R and T)
-                look = true;
-                ask_keys(st, 0);
-                continue;
-            }
-            // not a matter of size: something is not finite
-            spoiled = true;
-            dc_first_bad(r, t, bad);
-            dc_leave_out(r, t, bad);
-            dc_split_tiles(r[0], r[1], rh[0], rl[0]);
-            dc_split_tiles(r[2], r[3], rh[1], rl[1]);
-            dc_solve(u, rh, rl, th, tl);
-            dc_first_bad(u, t, bad);
-            dc_leave_out(u, t, bad);
-            break;
-        }
-        // ---- the new state
-        const float decay = st.gates.fade[DC_TOKENS - 1];
-        unsigned uh[2][4], ul[2][4], kt[STEPS][4];
-        float add[TILES][4];
+            // ---- the new state
+            unsigned uh[2][4], ul[2][4], kt[STEPS][4];
+            float taken[2] = {0.f, 0.f};                       // the largest number that the new state takes in, of the thread's tokens
 #pragma unroll
-        for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
-        query_step(3);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            float faded[2][4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const float2 after = *reinterpret_cast<const float2*>(&st.gates.after[16 * m + 8 * j + 2 * t]);
-#pragma unroll
-                for (int e = 0; e < 4; e += 2)
-                    dc_mul2(faded[j][e], faded[j][e + 1], u[2 * m + j][e], u[2 * m + j][e + 1], after.x, after.y);
-            }
-            dc_split_tiles(faded[0], faded[1], uh[m], ul[m]);
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {                          // tokens 16 m on
-#pragma unroll
-            for (int n = 0; n < TILES; ++n) dc_mma_if(m == 0, add[n], ul[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
-            if (PARTS == 2) {
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    unsigned b[4];
-                    dc_ldmatrix_trans(b, &st.keys.k[PARTS - 1][16 * m + bt_row][row0 + 16 * k + bt_col]);
-                    dc_mma(add[2 * k], uh[m], b[0], b[1]);
-                    dc_mma(add[2 * k + 1], uh[m], b[2], b[3]);
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < TILES; ++n) dc_mma(add[n], uh[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
-            if (m == 0) {
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][16 + bt_row][row0 + 16 * k + bt_col]);
-            }
-        }
-        // ---- outputs: the chunk's start and its own tokens; the fetching warps add up what two warps have of S0^T q and write them
-        unsigned zh[2][4], zl[2][4], w[FINISH][2][4];          // U again, weights: high and low part, two inner halves each
-        float2 fade[FINISH];
-        auto second = [&](int j) { return SLICES == 4 ? slice >= 2 : OWN * j >= 2; };      // the tile's tokens are in the chunk's second half
-#pragma unroll
-        for (int j = 0; j < FINISH; ++j) {
-            fade[j] = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile_of(j) + 2 * t]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-                if (m == 0 || second(j)) dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second(j) ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_piece]);
-        }
-#pragma unroll
-        for (int m = 0; m < 2; ++m) dc_split_tiles(u[2 * m], u[2 * m + 1], zh[m], zl[m]);
-        float oa[FINISH][4], ob[FINISH][4];
-#pragma unroll
-        for (int j = 0; j < FINISH; ++j) {
-            const float(&own)[4] = wq[OWN * j];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) dc_mul2(oa[j][2 * h], oa[j][2 * h + 1], own[2 * h], own[2 * h + 1], fade[j].x, fade[j].y);
+            for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][bt_row][row0 + 16 * k + bt_col]);
+            query_step(3);
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                if (m > 0 && !second(j)) continue;
-                dc_mma_if(m == 0, ob[j], zl[m], w[j][m][0], w[j][m][1]);
-                dc_mma(oa[j], zh[m], w[j][m][0], w[j][m][1]);
-                dc_mma(ob[j], zh[m], w[j][m][2], w[j][m][3]);
+                float faded[2][4];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 after = *reinterpret_cast<const float2*>(&st.gates.after[16 * m + 8 * j + 2 * t]);
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2)
+                        dc_mul2(faded[j][e], faded[j][e + 1], u[2 * m + j][e], u[2 * m + j][e + 1], after.x, after.y);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        asm("max.f32 %0, %0, %1, %2;" : "+f"(taken[h]) : "f"(fabsf(faded[j][2 * h])), "f"(fabsf(faded[j][2 * h + 1])));
+                }
+                dc_split_tiles(faded[0], faded[1], uh[m], ul[m]);
             }
-        }
-        if (c + 1 < chunks) ask(sm.stage[next]);
 #pragma unroll
-        for (int n = 0; n < TILES; ++n)
+            for (int m = 0; m < 2; ++m) {                      // tokens 16 m on
 #pragma unroll
-            for (int e = 0; e < 4; e += 2)
-                dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
-        auto leave = [&](int which, int tile, const float (&o)[4]) {
-            float* to = &sm.out[c & 1][which][8 * tile + 2 * t][group * 16 + g];
-            to[0] = o[0]; to[8] = o[2]; to[Sh::OLD] = o[1]; to[Sh::OLD + 8] = o[3];
-        };
-        if constexpr (SLICES > 1) {
+                for (int n = 0; n < TILES; ++n) dc_mma_if(m == 0, add[n], ul[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+                if (PARTS == 2) {
 #pragma unroll
-            for (int j = 1; j < (SLICES > 2 ? 4 : 3); ++j) {   // the other warps' tiles
-                const int tile = j ^ slice;
-                const float2 f = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile + 2 * t]);
+                    for (int k = 0; k < STEPS; ++k) {
+                        unsigned b[4];
+                        dc_ldmatrix_trans(b, &st.keys.k[PARTS - 1][16 * m + bt_row][row0 + 16 * k + bt_col]);
+                        dc_mma(add[2 * k], uh[m], b[0], b[1]);
+                        dc_mma(add[2 * k + 1], uh[m], b[2], b[3]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) dc_mma(add[n], uh[m], kt[n >> 1][2 * (n & 1)], kt[n >> 1][2 * (n & 1) + 1]);
+                if (m == 0) {
+#pragma unroll
+                    for (int k = 0; k < STEPS; ++k) dc_ldmatrix_trans(kt[k], &st.keys.k[0][16 + bt_row][row0 + 16 * k + bt_col]);
+                }
+            }
+            // ---- is everything in range?  (all warps of 16 columns have the same U)
+            float size, low[2], most[DC_TILES], little[2][2];  // (short chains: three at a time)
+#pragma unroll
+            for (int j = 0; j < DC_TILES; ++j) {
+                asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(most[j]) : "f"(fabsf(u[j][0])), "f"(fabsf(u[j][1])), "f"(fabsf(u[j][2])));
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(most[j]) : "f"(fabsf(u[j][3])));
+            }
+            asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(size) : "f"(most[0]), "f"(most[1]), "f"(most[2]));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(size) : "f"(most[3]));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    asm("min.f32 %0, %1, %2, %3;" : "=f"(little[h][m])
+                        : "f"(fabsf(u[2 * m][2 * h])), "f"(fabsf(u[2 * m][2 * h + 1])), "f"(fabsf(u[2 * m + 1][2 * h])));
+                    little[h][m] = fminf(little[h][m], fabsf(u[2 * m + 1][2 * h + 1]));
+                }
+                low[h] = fminf(little[h][0], little[h][1]);
+            }
+            if (__builtin_expect(tokens < DC_TOKENS, 0)) {     // (nothing is stored for tokens that are not there)
+                low[0] = low[1] = INFINITY;
+#pragma unroll
+                for (int j = 0; j < DC_TILES; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (8 * j + 2 * t + (e & 1) < tokens) low[e >> 1] = fminf(low[e >> 1], fabsf(u[j][e]));
+            }
+            const bool high = !(size < DC_MOST * DC_T_SCALE);
+            // of a column's four lanes one at least has taken in enough, of both columns
+            unsigned enough = __ballot_sync(0xffffffffu, taken[0] >= least_state[0] && taken[1] >= least_state[1]);
+            enough |= enough >> 2;
+            enough |= enough >> 1;
+            if (__builtin_expect(!passed && ((enough & 0x11111111u) != 0x11111111u ||
+                                             __any_sync(0xffffffffu, high || low[0] < least[0] || low[1] < least[1])), 0)) {
+                why = __any_sync(0xffffffffu, high) ? MUCH : LITTLE;
+                met = true;
+                break;
+            }
+            // ---- outputs: the chunk's start and its own tokens; the fetching warps add up what two warps have of S0^T q and write them
+            unsigned zh[2][4], zl[2][4], w[FINISH][2][4];      // U again, weights: high and low part, two inner halves each
+            float2 fade[FINISH];
+            auto second = [&](int j) { return SLICES == 4 ? slice >= 2 : OWN * j >= 2; };      // the tile's tokens are in the chunk's second half
+#pragma unroll
+            for (int j = 0; j < FINISH; ++j) {
+                fade[j] = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile_of(j) + 2 * t]);
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+                    if (m == 0 || second(j)) dc_ldmatrix(w[j][m], &st.gates.p[lane >> 4][second(j) ? 1 + m : 0][8 * (tile_of(j) & 1) + (lane & 7)][b_piece]);
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m) dc_split_tiles_far(u[2 * m], u[2 * m + 1], zh[m], zl[m]);
+#pragma unroll
+            for (int j = 0; j < FINISH; ++j) {
+                const float(&own)[4] = wq[OWN * j];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) dc_mul2(oa[j][2 * h], oa[j][2 * h + 1], own[2 * h], own[2 * h + 1], fade[j].x, fade[j].y);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    if (m > 0 && !second(j)) continue;
+                    dc_mma_if(m == 0, ob[j], zl[m], w[j][m][0], w[j][m][1]);
+                    dc_mma(oa[j], zh[m], w[j][m][0], w[j][m][1]);
+                    dc_mma(ob[j], zh[m], w[j][m][2], w[j][m][3]);
+                }
+            }
+            const float decay = st.gates.fade[DC_TOKENS - 1] * (1.f / DC_P_SCALE);
+            if (c + 1 < chunks) ask(sm.stage[stage + 1 < DC_STAGES ? stage + 1 : 0]);
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; e += 2)
+                    dc_fma2(s[n][e], s[n][e + 1], s[n][e], s[n][e + 1], decay, decay, add[n][e], add[n][e + 1]);
+            auto leave = [&](int which, int tile, const float (&o)[4]) {
+                float* to = &sm.out[c & 1][which][8 * tile + 2 * t][group * 16 + g];
+                to[0] = o[0]; to[8] = o[2]; to[Sh::OLD] = o[1]; to[Sh::OLD + 8] = o[3];
+            };
+            if constexpr (SLICES > 1) {
+#pragma unroll
+                for (int j = 1; j < (SLICES > 2 ? 4 : 3); ++j) {   // the other warps' tiles
+                    const int tile = j ^ slice;
+                    const float2 f = *reinterpret_cast<const float2*>(&st.gates.fade[8 * tile + 2 * t]);
+                    float o[4];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) dc_mul2(o[2 * h], o[2 * h + 1], wq[j][2 * h], wq[j][2 * h + 1], f.x, f.y);
+                    leave(SLICES > 2 ? j : 1, tile, o);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < FINISH; ++j) {
+                const int tile = tile_of(j);
                 float o[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) dc_mul2(o[2 * h], o[2 * h + 1], wq[j][2 * h], wq[j][2 * h + 1], f.x, f.y);
-                leave(SLICES > 2 ? j : 1, tile, o);
+                for (int h = 0; h < 2; ++h) dc_fma2(o[2 * h], o[2 * h + 1], ob[j][2 * h], ob[j][2 * h + 1], 1.f / DC_LOW, 1.f / DC_LOW, oa[j][2 * h], oa[j][2 * h + 1]);
+                leave(0, tile, o);
             }
-        }
-#pragma unroll
-        for (int j = 0; j < FINISH; ++j) {
-            const int tile = tile_of(j);
-            float o[4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) dc_add2(o[2 * h], o[2 * h + 1], oa[j][2 * h], oa[j][2 * h + 1], ob[j][2 * h], ob[j][2 * h + 1]);
-            if (__builtin_expect(spoiled, 0)) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (8 * tile + 2 * t + (e & 1) >= bad[e >> 1]) o[e] = __int_as_float(0x7fffffff);
+            if (slice == 0 && t == 0) {                        // (one over sigma as this chunk had it)
+                sm.back[c & 1][group * 16 + g] = back[0];
+                sm.back[c & 1][group * 16 + g + 8] = back[1];
             }
-            leave(0, tile, o);
-        }
-        if (slice == 0 && t == 0) {                            // (one over sigma as this chunk had it)
-            sm.back[c & 1][group * 16 + g] = back[0];
-            sm.back[c & 1][group * 16 + g + 8] = back[1];
-        }
-        if (__builtin_expect(spoiled, 0)) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (bad[h] < DC_TOKENS) {
-#pragma unroll
-                    for (int n = 0; n < TILES; ++n) s[n][2 * h] = s[n][2 * h + 1] = __int_as_float(0x7fffffff);
-                }
+            passed = false;
+            through();
+            if (c >= chunks) break;
         }
     }
     dc_sync(DC_MEET, Sh::THREADS);
