@@ -220,13 +220,15 @@ class ModelRunner:
         """Run one step of `tokens` tokens (default: the cap) of a scratch request, so that the
         allocator holds the working memory of the largest step before serving starts and no
         later step has to ask the driver for memory; the request's pages and slot are given
-        back.  Skipped (returns 0) when the pool cannot hold that many tokens right now."""
+        back.  What depends on how many requests share the tokens is taken for as many as the runner
+        takes.  Skipped (returns 0) when the pool cannot hold that many tokens right now."""
         tokens = min(tokens or self.max_step_tokens, self.max_step_tokens, self.max_positions)
         cache = self.cache
         if not cache.can_open() or any(cache.blocks_for(tokens) > free for free in cache.free_pages()):
             return 0
         handle = cache.open(("reserve_step_memory", id(self)))
         try:
+            self.model.reserve(tokens, self.max_step_items)
             self.step([StepEntry(handle, [0] * tokens, [tokens - 1])])
             torch.cuda.current_stream().synchronize()
         finally:

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 from array import array
+from functools import lru_cache
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -2375,11 +2376,28 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
 DELTA_FEW_TOKENS = {DTYPE_F32: (6, 16), DTYPE_BF16: (4, 10)}
 
 
+def _delta_chunks(tokens: int, items: int, ones: int, few: int, chunk: int) -> int:
+    """At most so many chunks of `chunk` tokens, the last of a request begun, do the requests of more than `few` tokens have."""
+    return tokens // chunk + min(items - ones if few else items, tokens // (few + 1))
+
+
+@lru_cache(maxsize=1024)
+def gated_delta_room(tokens: int, items: int, heads: int, dim: int, dtype: torch.dtype, share: int = 1) -> int:
+    """Bytes of `room` that no call of `gated_delta_rule` with up to so many tokens and requests exceeds."""
+    _, chunked_most, chunk = _delta_limits()
+    if dim > chunked_most or tokens <= 0 or items <= 0:
+        return 0
+    tag = _tag(dtype)
+    most = max(_delta_chunks(tokens, min(items, 127 // heads) if small else items, 0, few, chunk)
+               for few, small in zip(DELTA_FEW_TOKENS[tag], (True, False)))
+    return most * delta().fsie_delta_chunk_bytes(heads, share, dim, tag)
+
+
 def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_decay: torch.Tensor, beta: torch.Tensor,
                      item_qstart: torch.Tensor, item_qlen: torch.Tensor, item_slots: torch.Tensor, items: int,
                      state: torch.Tensor, out: torch.Tensor, heads: int, dim: int, vdim: int, share: int = 1,
                      scale: Optional[float] = None, eps: float = 1e-6, longest: int = 0, early: bool = False,
-                     ones: int = 0) -> torch.Tensor:
+                     ones: int = 0, room: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Per request and head, token by token, with q and k divided by sqrt(their squared length + eps) and
     a = exp(log_decay):
 
@@ -2392,8 +2410,9 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     negative slot is passed over, its rows of `out` stay as they are.  `scale`: dim ** -0.5 unless given.  `longest`: the
     tokens of the step's longest request, which choose the kernel (0: not known to the caller); `ones`: at least so many of
     the requests have one token, or none, and need no place among the longer ones (0 is always right; a number above theirs
-    leaves long requests out).  dim is 256 at most.  Requests walked in chunks take a workspace for the call: some 24 kB
-    (bfloat16, dim 128; float32 41) per head and 32 tokens.
+    leaves long requests out).  dim is 256 at most.  Requests walked in chunks take a workspace: some 24 kB (bfloat16, dim
+    128; float32 42) per head and 32 tokens of theirs, the last 32 of each begun.  It is allocated for the call unless `room`
+    (uint8, on 16 bytes; `gated_delta_room` says how large) is given.
     `early`: the state and the lists are older than the stream's last kernel, see the module's first lines."""
     f32, i32 = torch.float32, torch.int32
     if not (_fits(qkv, None, True) and _fits(log_decay, f32, True) and _fits(beta, f32, True) and _fits(out, f32, True)
@@ -2426,14 +2445,23 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
     most, chunked_most, chunk = _delta_limits()
     if dim > most:
         raise KernelError(f"gated_delta_rule: {dim} state rows per head, the kernels hold {most}")
-    lib, tag, room = delta(), _tag(qkv.dtype), None
-    few = DELTA_FEW_TOKENS[tag][items * heads >= 128]
-    chunked = (longest or tokens) > few and dim <= chunked_most and ones < items
-    if chunked:
+    lib, tag = delta(), _tag(qkv.dtype)
+    few, chunks = DELTA_FEW_TOKENS[tag][items * heads >= 128], 0
+    if (longest or tokens) > few and dim <= chunked_most and ones < items:
         few = few if items > 1 and tokens != items * longest else 0
-        chunks = tokens // chunk + items
-        room = torch.empty(chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag), dtype=torch.uint8, device=qkv.device)
-    _check(lib.fsie_delta_rule(int(chunked), few, ones, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
+        chunks = _delta_chunks(tokens, items, ones, few, chunk)
+    if chunks:
+        size = chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag)
+        if room is None:
+            room = torch.empty(size, dtype=torch.uint8, device=qkv.device)
+        else:
+            _need(room, torch.uint8, "room")
+            if room.numel() < size or room.data_ptr() % 16:
+                raise KernelError(f"gated_delta_rule: room must have {size} bytes, on 16 bytes")
+            room = room.view(-1)[:size]
+    else:
+        room = None
+    _check(lib.fsie_delta_rule(int(chunks > 0), few, ones, qkv, ld, q_off, k_off, v_off, log_decay, beta, item_qstart, item_qlen, item_slots,
                                items, state, stride, out, heads, dim, vdim, share, float(dim ** -0.5 if scale is None else scale),
                                float(eps), tag, room, 0 if room is None else room.numel(), int(early), _stream()),
            "gated_delta_rule")

@@ -122,3 +122,7 @@ class Mixer(Part):
 
     def state_need(self) -> Optional[StateNeed]:
         return None
+
+    def reserve(self, tokens: int, requests: int) -> None:
+        """Take from the runtime what working memory a step of up to so many tokens may need beyond what it needs when they are
+        one request's: steps of up to `requests` requests follow."""

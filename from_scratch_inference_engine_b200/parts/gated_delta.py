@@ -89,6 +89,13 @@ class GatedDeltaRule(Mixer):
         runtime.prepare_weight(self.w_in)
         runtime.prepare_weight(self.w_o)
 
+    def _room(self, tokens: int, requests: int) -> Optional[torch.Tensor]:
+        size = ops.gated_delta_room(tokens, requests, self.heads, self.dim, self.runtime.dtype, self.heads // self.qk_heads)
+        return self.runtime.buffer("gated_delta.room", 1, size, torch.uint8) if size else None
+
+    def reserve(self, tokens: int, requests: int) -> None:
+        self._room(tokens, requests)
+
     def forward(self, ctx, y: torch.Tensor, cache: LayerCache) -> torch.Tensor:
         rt = self.runtime
         tokens = y.shape[0]
@@ -106,7 +113,8 @@ class GatedDeltaRule(Mixer):
         o = rt.buffer("gated_delta.o", tokens, self.v_width, torch.float32)
         ops.gated_delta_rule(act, 0, self.qk_width, 2 * self.qk_width, log_decay, beta, *items, cache.state, o, self.heads,
                              self.dim, self.vdim, share=self.heads // self.qk_heads, eps=self.eps,
-                             longest=ctx.longest, early=True, ones=ctx.ones)
+                             longest=ctx.longest, early=True, ones=ctx.ones,
+                             room=self._room(tokens, ctx.num_items) if ctx.longest > 1 else None)
         gated = rt.buffer("gated_delta.gated", tokens, self.v_width, proj.dtype)
         ops.head_norm_silu(o, proj, gate0, self.gain, self.eps, gated, self.heads)
         return rt.linear(gated, self.w_o, None, "gated_delta.out")

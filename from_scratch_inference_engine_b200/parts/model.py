@@ -123,6 +123,11 @@ class DecoderModel:
         """State each call of the run order keeps per request (None for most mixers)."""
         return [self.blocks[layer].mixer.state_need() for layer, _, _ in self.schedule]
 
+    def reserve(self, tokens: int, requests: int) -> None:
+        """Working memory that depends on how many requests share a step's tokens (see `Mixer.reserve`)."""
+        for block in self.blocks:
+            block.mixer.reserve(tokens, requests)
+
     # ------------------------------------------------------------------ forward
     def forward(self, ctx, caches: List[LayerCache], want_rows: Optional[torch.Tensor]):
         """Run the step's tokens; returns float32 logits [len(want_rows), vocab] (None if

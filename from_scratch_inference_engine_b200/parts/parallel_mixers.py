@@ -53,6 +53,10 @@ class ParallelMixers(Mixer):
     def state_need(self) -> Optional[StateNeed]:
         return self.left.state_need() or self.right.state_need()
 
+    def reserve(self, tokens: int, requests: int) -> None:
+        self.left.reserve(tokens, requests)
+        self.right.reserve(tokens, requests)
+
     def bind(self, tensors: Dict[str, torch.Tensor], runtime) -> None:
         self.runtime = runtime
         self.left.bind(tensors, runtime)
