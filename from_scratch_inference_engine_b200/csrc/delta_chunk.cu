@@ -355,6 +355,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
     }
     const int n = min(DC_TOKENS, count - place * DC_TOKENS);
     grid_dependency_wait();
+    if (p.go && first_block() && threadIdx.x == 0) delta_release(p.go, 0);
     grid_dependents_go();
     if (slot < 0 || chunk >= records.chunks) return;           // beyond the step's chunks, or a padding entry
     float decay = 0.f, beta = 0.f;                             // of the lane's token, the first head's
@@ -745,14 +746,17 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
     const int slot = item < 0 ? -1 : p.item_slots[item], count = item < 0 ? 0 : p.item_qlen[item], t0 = item < 0 ? 0 : p.item_qstart[item];
     const int chunks = dc_chunks(count, p.least);
     // fewer requests than blocks, a padding entry of a fixed-size batch, or lists that name more tokens than there are
+    const bool tells = p.go && first_block() && threadIdx.x == 32 * DC_WALKERS;
     if (slot < 0 || chunk0 > records.chunks - chunks) {
         grid_dependency_wait();
+        if (tells) delta_release(p.go, DELTA_GO);
         return;
     }
     // registers (bfloat16): two blocks of 256 threads have 128 each; the walking warps take over some of the fetching ones' (216 + 40)
     if (warp >= DC_WALKERS) {
         if (sizeof(T) == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;\n");
         grid_dependency_wait();
+        if (tells) delta_release(p.go, DELTA_GO);
         grid_dependents_go();
         DcFetch<T, DK, SLICE, WIDE> fetch(p, records, head, col0, t0, count, chunk0);
         const size_t width = (size_t)p.heads * p.vdim;
@@ -1361,12 +1365,12 @@ static long long chunk_bytes(int heads, int share, int dim, int dtype) {
 }
 
 // The chunked form; ERR_UNSUPPORTED where a head has more rows than it holds.  `longer`: at most so many requests are of p.least tokens
-// or more; `room`: 16-byte aligned memory.
+// or more; `room`: 16-byte aligned memory, 16 bytes and the records.
 int delta_chunk(const DeltaParams& p, int items, int longer, int dtype, void* room, long long room_bytes, int early, cudaStream_t stream) {
     if (p.dim > DC_MAX_DIM) return ERR_UNSUPPORTED;
-    const long long chunks = room_bytes / chunk_bytes(p.heads, p.share, p.dim, dtype);
+    const long long chunks = (room_bytes - 16) / chunk_bytes(p.heads, p.share, p.dim, dtype);        // (behind p.go's word)
     if (!room || (uintptr_t)room % 16 != 0 || chunks <= 0 || chunks > 0x7fffffffLL) return ERR_BAD_ARGUMENT;
-    unsigned char* at = (unsigned char*)room;
+    unsigned char* at = (unsigned char*)room + 16;
     if (dtype == DTYPE_F32)
         return p.dim <= 64 ? launch_chunk_any<float, 64>(p, items, longer, chunks, at, early, stream)
                            : launch_chunk_any<float, 128>(p, items, longer, chunks, at, early, stream);

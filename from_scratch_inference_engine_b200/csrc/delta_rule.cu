@@ -68,7 +68,9 @@ delta_step_kernel(const DeltaParams p) {
         for (int x = 0; x < V; ++x) s[i].v[x] = 0.f;
         if (in && r < p.dim) s[i] = load_cols(state + (size_t)r * p.vdim, Cols<V>());
     }
-    if (!p.beside) {
+    if (p.beside) {
+        delta_await(p.go);
+    } else {
         grid_dependency_wait();
         grid_dependents_go();
     }
@@ -188,7 +190,9 @@ delta_head_kernel(const DeltaParams p) {
 #pragma unroll
     for (int i = 0; i < ROWS; ++i)
         s[i] = in && row0 + i < p.dim ? *reinterpret_cast<const float4*>(state + (size_t)i * p.vdim) : make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!p.beside) {
+    if (p.beside) {
+        delta_await(p.go);
+    } else {
         grid_dependency_wait();
         grid_dependents_go();
     }
@@ -314,7 +318,7 @@ extern "C" {
 
 int fsie_delta_max_dim() { return STEP_MAX_DIM; }
 
-// `form`: 0 the recurrent form, 1 the chunked one, with a workspace `room` of
+// `form`: 0 the recurrent form, 1 the chunked one, with a workspace `room` of 16 bytes and
 // fsie_delta_chunk_bytes() for every chunk (of fsie_delta_chunk_tokens() tokens of a request, its last one begun).  Form 1 with
 // `few` > 0: requests of up to `few` tokens, `ones` at least, in the recurrent form, beside the others.
 int fsie_delta_rule(int form, int few, int ones, const void* qkv, int ld, int q_off, int k_off, int v_off, const float* log_decay, const float* beta,
@@ -330,13 +334,14 @@ int fsie_delta_rule(int form, int few, int ones, const void* qkv, int ld, int q_
     p.state = state; p.state_stride = state_stride; p.out = out;
     p.heads = heads; p.dim = dim; p.vdim = vdim; p.share = share; p.scale = scale; p.eps = eps;
     if (dtype != DTYPE_F32 && dtype != DTYPE_BF16) return ERR_BAD_ARGUMENT;
-    p.least = 1; p.most = INT_MAX; p.beside = false;
+    p.least = 1; p.most = INT_MAX; p.beside = false; p.go = nullptr;
     if (form == 1) {
         p.least = few > 0 ? few + 1 : 1;
+        if (few > 0) p.go = (unsigned*)room;
         const int rc = delta_chunk(p, items, few > 0 ? items - ones : items, dtype, room, room_bytes, early, stream);
         if (rc != 0 || few <= 0) return rc;
-        // Behind the walk in the stream, beside it on the GPU: its blocks need no wait, since the walk lets them go when its own
-        // is over, and the first waits for the walk's end at its own, so that whoever waits for them all waits for both.
+        // Behind the walk in the stream, beside it on the GPU: its blocks start when the walk's have, and the first waits for the
+        // walk's end at its own, so that whoever waits for them all waits for both.
         p.least = 1; p.most = few; p.beside = true; early = 1;
     }
     return dtype == DTYPE_F32 ? launch_step<float>(p, items, early, stream) : launch_step<bf16>(p, items, early, stream);

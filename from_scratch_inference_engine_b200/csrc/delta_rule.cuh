@@ -14,7 +14,27 @@ struct DeltaParams {
     int heads, dim, vdim, share;
     int least, most;                                       // tokens of a request that the launch takes; it leaves others alone
     bool beside;                                           // the recurrent form runs beside the chunked one's launches
+    unsigned* go;                                          // ... and its inputs are there when this is 1 (delta_await)
     float scale, eps;
 };
+
+// The recurrent launch beside the walk starts when every block of the walk has, whose wait for the records' kernel is over, whose own
+// wait made visible to it what stands in front of the rule.  No wait of the launch's own is among these: it would be one for the walk's end.
+// So the order is handed on: the records' kernel clears the word behind its wait, the walk's first block, behind its own, releases it
+// as 1, and a block here acquires that before it reads what the kernels in front may have written.  The poll's first answer is
+// 1 but for a few hundred cycles; a block that is not answered waits for the walk's end.
+constexpr unsigned DELTA_GO = 1;
+__device__ __forceinline__ void delta_release(unsigned* word, unsigned value) {
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(word), "r"(value) : "memory");
+}
+__device__ __forceinline__ void delta_await(const unsigned* word) {
+    if (threadIdx.x == 0) {
+        unsigned seen = 0;
+        for (int i = 0; i < 1000 && seen != DELTA_GO; ++i)
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(word) : "memory");
+        if (seen != DELTA_GO) grid_dependency_wait();
+    }
+    __syncthreads();
+}
 
 }  // namespace fsie

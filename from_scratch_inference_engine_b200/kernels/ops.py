@@ -2390,7 +2390,7 @@ def gated_delta_room(tokens: int, items: int, heads: int, dim: int, dtype: torch
     tag = _tag(dtype)
     most = max(_delta_chunks(tokens, min(items, 127 // heads) if small else items, 0, few, chunk)
                for few, small in zip(DELTA_FEW_TOKENS[tag], (True, False)))
-    return most * delta().fsie_delta_chunk_bytes(heads, share, dim, tag)
+    return most * delta().fsie_delta_chunk_bytes(heads, share, dim, tag) + 16
 
 
 def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_decay: torch.Tensor, beta: torch.Tensor,
@@ -2451,7 +2451,7 @@ def gated_delta_rule(qkv: torch.Tensor, q_off: int, k_off: int, v_off: int, log_
         few = few if items > 1 and tokens != items * longest else 0
         chunks = _delta_chunks(tokens, items, ones, few, chunk)
     if chunks:
-        size = chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag)
+        size = chunks * lib.fsie_delta_chunk_bytes(heads, share, dim, tag) + 16
         if room is None:
             room = torch.empty(size, dtype=torch.uint8, device=qkv.device)
         else:
