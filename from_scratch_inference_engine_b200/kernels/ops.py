@@ -2073,7 +2073,8 @@ def moe_align(ids: torch.Tensor, pairs: int, experts: int, lists: torch.Tensor,
     sorted, tile_expert, tile_row0, meta [1], place).  Compact layout: sorted [pairs] holds the pairs
     expert after expert, place is None.  `padded`: every expert's rows start on a multiple of `tile`,
     sorted [(pairs // tile + experts) * tile] holds -1 where no pair owns the row, place [pairs] is
-    each pair's row."""
+    each pair's row.  The pairs of an expert stand in their own order in lists of fewer than 512 pairs (of up to 500
+    experts or so, a bit per expert and pair being kept), else in any."""
     _need(ids, torch.int32, "ids")
     _need(lists, torch.int32, "lists")
     tile = tile or moe_tile_rows()
