@@ -49,7 +49,7 @@ delta_step_kernel(const DeltaParams p) {
     constexpr int GROUPS = STEP_THREADS / ACROSS;          // row groups of the block
     constexpr int IN_WARP = 32 / ACROSS;                   // ... of a warp
     __shared__ float ks[2][STEP_MAX_DIM], qs[2][STEP_MAX_DIM];
-    __shared__ float sums[2][STEP_WARPS][2][STEP_COLS];
+    __shared__ __align__(16) float sums[2][STEP_WARPS][2][STEP_COLS];
     const int head = blockIdx.y, item = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int slot = p.item_slots[item], count = p.item_qlen[item], t0 = p.item_qstart[item];

@@ -92,8 +92,8 @@ __global__ void __launch_bounds__(256) head_product_kernel(const T* __restrict__
                                                            const T* __restrict__ w, T* __restrict__ out,
                                                            long long out_ld, int out_head, int tokens,
                                                            int n, int k) {
-    __shared__ float xs[HP_K][HP_TILE + 4];
-    __shared__ float ws[HP_K][HP_TILE + 4];
+    __shared__ __align__(16) float xs[HP_K][HP_TILE + 4];
+    __shared__ __align__(16) float ws[HP_K][HP_TILE + 4];
     const int h = blockIdx.z, t0 = blockIdx.x * HP_TILE, n0 = blockIdx.y * HP_TILE;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     grid_dependency_wait();

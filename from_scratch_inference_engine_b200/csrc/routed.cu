@@ -486,8 +486,8 @@ __global__ void __launch_bounds__(256) moe_product_kernel(
         const int* __restrict__ offsets, const int* __restrict__ sorted, const int* __restrict__ tile_expert,
         const int* __restrict__ tile_row0, const int* __restrict__ meta, int top, int n, int k, int gate_kind) {
     constexpr bool GATED = MODE == 1, FIRST = MODE != 0;
-    __shared__ float xs[16][MOE_TILE + 4];
-    __shared__ float ws[16][MOE_TILE + 4];
+    __shared__ __align__(16) float xs[16][MOE_TILE + 4];
+    __shared__ __align__(16) float ws[16][MOE_TILE + 4];
     __shared__ int src[MOE_TILE], dst[MOE_TILE];
     grid_dependency_wait();
     grid_dependents_go();
