@@ -235,6 +235,16 @@ class CacheManager:
             children.append(child)
         return children, moves
 
+    def fork_room(self, handle: RequestCache) -> int:
+        """How many requests `fork` can make of this one now."""
+        full = handle.length // self.page_size
+        room = self.slots.num_free
+        if handle.length % self.page_size:
+            for table, free in zip(handle.tables, self.free_pages()):
+                if table[full] >= 0:
+                    room = min(room, free)
+        return room
+
     def compact(self) -> List[List[Tuple[int, int]]]:
         """Renumber every group's pages in use so that they are its first ones (the rest of the pool is then one piece);
         tables, reference counts and cached prefixes follow.  Returns per group the (old, new) pairs whose contents the

@@ -23,7 +23,6 @@ from typing import List, Optional, Sequence
 
 import torch
 
-from ..cache.pool import OutOfPages
 from ..config.registry import load_config
 from ..parts.model import DecoderModel
 from ..sampling.sampler import Sampler, SamplingParams, request_seed
@@ -148,8 +147,9 @@ class Engine:
     def add_samples(self, prompt: Sequence[int], params: Sequence[SamplingParams], max_tokens: int = 16,
                     eos_id: int = -1) -> List[int]:
         """One request per element of `params` with the same prompt, which is run once: up to its last token by the first
-        request, which is then continued (`fork`) as often as needed.  Runs steps until then (of other requests too).
-        Continuations for which there is no room then run the prompt by themselves.  Returns the ids, in order."""
+        request, which is then continued (`fork`) as often as needed.  Runs steps until then (of other requests too).  The
+        continuations run at once, in front of requests that wait; those for which there is no running place, state slot or
+        page then wait and run the prompt by themselves.  Returns the ids, in order."""
         if not params:
             return []
         first = self.add_request(prompt, params[0], max_tokens, eos_id)
@@ -162,12 +162,9 @@ class Engine:
                     break
             if seq.handle is not None and seq.handle.length == seq.hold:
                 count = max(0, min(len(rest), self.scheduler.max_batch - len(self.scheduler.running),
-                                   self.runner.cache.slots.num_free))
-                try:
-                    ids += self.fork(first, count, rest[:count])
-                    rest = rest[count:]
-                except OutOfPages:
-                    pass
+                                   self.runner.cache.fork_room(seq.handle)))
+                ids += self.fork(first, count, rest[:count])
+                rest = rest[count:]
             seq.hold = 0
         return ids + [self.add_request(prompt, p, max_tokens, eos_id) for p in rest]
 
