@@ -157,15 +157,17 @@ class Engine:
         ids, rest = [first], list(params[1:])
         if len(prompt) > 1 and rest:
             seq.hold = len(prompt) - 1
-            while seq.handle is None or seq.handle.length < seq.hold:
-                if self.step() == 0:
-                    break
-            if seq.handle is not None and seq.handle.length == seq.hold:
-                count = max(0, min(len(rest), self.scheduler.max_batch - len(self.scheduler.running),
-                                   self.runner.cache.fork_room(seq.handle)))
-                ids += self.fork(first, count, rest[:count])
-                rest = rest[count:]
-            seq.hold = 0
+            try:
+                while seq.handle is None or seq.handle.length < seq.hold:
+                    if self.step() == 0:
+                        break
+                if seq.handle is not None and seq.handle.length == seq.hold:
+                    count = max(0, min(len(rest), self.scheduler.max_batch - len(self.scheduler.running),
+                                       self.runner.cache.fork_room(seq.handle)))
+                    ids += self.fork(first, count, rest[:count])
+                    rest = rest[count:]
+            finally:                        # whatever happened, the request may go on
+                seq.hold = 0
         return ids + [self.add_request(prompt, p, max_tokens, eos_id) for p in rest]
 
     def warm_up(self, max_context: int = 0) -> int:

@@ -1,4 +1,4 @@
-"""How often a request can be continued, and answers to one prompt where room lacks."""
+"""How often a request can be continued, and answers to one prompt where room lacks or a step fails."""
 import random
 import sys
 from pathlib import Path
@@ -73,3 +73,24 @@ def test_as_many_answers_share_the_prompt_as_pages_allow(folder, pipeline):
     alone = engine_of(folder, 200)
     assert [engine.output(i) for i in ids] == [alone.generate(prompt, p, 3) for p in params]
     assert engine.stats()["tokens_prefilled"] == 29 + 4 + 30 and engine.preemptions() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("pipeline", [True, False])
+def test_a_step_that_fails_holds_nothing_back(folder, pipeline, monkeypatch):
+    prompt, params = helpers.random_ids(VOCAB, 37, 11), params_of(3)
+    engine = engine_of(folder, 200, pipeline=pipeline)
+    step, calls = engine.step, []
+
+    def failing():
+        calls.append(1)
+        if len(calls) == 2:
+            raise RuntimeError("lost")
+        return step()
+    monkeypatch.setattr(engine, "step", failing)
+    with pytest.raises(RuntimeError, match="lost"):
+        engine.add_samples(prompt, params, 5)
+    monkeypatch.undo()
+    engine.run_until_done()
+    assert engine.output(0) == engine_of(folder, 200).generate(prompt, params[0], 5)
+    engine.runner.cache.check()
