@@ -576,6 +576,20 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                     *reinterpret_cast<unsigned*>(&own.gates.t[1][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = low;
                 }
         }
+        if (n < DC_TOKENS) {
+            // Tokens that are not there have the last one's row of T, so that U repeats its value: nothing is out of range for their sake.
+            // (Their keys are zero and no output reads them.)
+            __syncthreads();
+            const int last = n - 1;
+            for (int x = threadIdx.x; x < 8 * (DC_TOKENS - n); x += 32 * DC_MAKERS) {
+                const int row = n + (x >> 3), part = (x >> 2) & 1, right = (x >> 1) & 1, piece = x & 1;       // columns 0 to 15, 16 to 31
+                if (row < 16 && right) continue;
+                uint4 from = make_uint4(0, 0, 0, 0);
+                if (last >= 16 || !right)
+                    from = *reinterpret_cast<const uint4*>(&own.gates.t[part][last < 16 ? 0 : 1 + right][last & 15][dc_piece(last & 15, piece)]);
+                *reinterpret_cast<uint4*>(&own.gates.t[part][row < 16 ? 0 : 1 + right][row & 15][dc_piece(row & 15, piece)]) = from;
+            }
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 96)
@@ -1031,7 +1045,6 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
         // ---- chunk after chunk, until one is out of range
         for (;;) {
             const auto& st = sm.stage[stage];
-            const int tokens = min(DC_TOKENS, count - c * DC_TOKENS);
             float u[DC_TILES][4], wq[DC_TILES][4];             // U, times DC_T_SCALE; S0^T q
             unsigned bq[2][4];                                 // Q
             unsigned sh[STEPS][4], sl[STEPS][4];               // the state in two parts
@@ -1199,14 +1212,6 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                     little[h][m] = fminf(little[h][m], fabsf(u[2 * m + 1][2 * h + 1]));
                 }
                 low[h] = fminf(little[h][0], little[h][1]);
-            }
-            if (__builtin_expect(tokens < DC_TOKENS, 0)) {     // (nothing is stored for tokens that are not there)
-                low[0] = low[1] = INFINITY;
-#pragma unroll
-                for (int j = 0; j < DC_TILES; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (8 * j + 2 * t + (e & 1) < tokens) low[e >> 1] = fminf(low[e >> 1], fabsf(u[j][e]));
             }
             const bool high = !(size < DC_MOST * DC_T_SCALE);
             // of a column's four lanes one at least has taken in enough, of both columns
