@@ -3,8 +3,8 @@
 // Inside a chunk that starts from state S0, with G_i = sum of log_decay over the chunk's tokens up to i and k, q divided by
 // their lengths,
 //
-//   R_i = v_i - e^(G_i) S0^T k_i                      what the chunk's start leaves to be stored
-//   U   = T R,  T = (I + A)^-1 diag(beta)             A_ij = beta_i (k_i.k_j) e^(G_i - G_j) for j < i, else 0
+//   R_i = b (v_i - e^(G_i) S0^T k_i)                  what the chunk's start leaves to be stored; b: a power of two, above every beta
+//   U   = T R,  T = (I + A)^-1 diag(beta) / b         A_ij = beta_i (k_i.k_j) e^(G_i - G_j) for j < i, else 0
 //   o_i = scale (e^(G_i) S0^T q_i + sum_(j <= i) (q_i.k_j) e^(G_i - G_j) u_j)
 //   S   = e^(G_31) S0 + sum_j e^(G_31 - G_j) k_j u_j^T
 //
@@ -28,11 +28,13 @@
 // Range.  Half precision has little of it: a pair ends at 2^-25, 22 bits below a number of 2^-3.  Where a sum of its own takes the low
 // parts' products they go in 2^11 times as large (DC_LOW), so that the pairs of R, U, T and the weights end at 2^-36; T and the weights
 // are stored 2^11 and 2^14 times as large besides.  Every column of the state (a row of the transposed tiles below) has a power of two,
-// `sigma`, chosen in a look at the column's and the first chunk's largest numbers, and anew, the chunk's sums taken again, when a chunk
-// is out of range: when a number of U is too large, when next to nothing of a column's is taken into the state, or when next to nothing is
-// stored at some token and the column holds no more (DC_LEAST...).  Where that is so even right behind a look - a large value that is
-// forgotten within its chunk, small ones in front of a large one -, where a state is small beside the values, or where something is not
-// finite, the warps of the 16 columns walk the chunk token by token in 32 bits, as the recurrence is written.
+// `sigma`, chosen in a look at the largest numbers of the column and of the first chunk's b v, and anew, the chunk's sums taken again,
+// when a chunk is out of range: when a number of U is too large, when next to nothing of a column's is taken into the state, or when next
+// to nothing is stored at some token and the column holds no more (DC_LEAST...).  Where that is so even right behind a look - a large
+// value that is forgotten within its chunk, small ones in front of a large one -, where a state is small beside the values, or where
+// something is not finite, the warps of the 16 columns walk the chunk token by token in 32 bits, as the recurrence is written.  Such a
+// chunk takes some nine times as long (8,192 tokens of 16 q/k and 32 heads, all so, 3.0 ms; values with e^(2 N(0, 1)) for a token's size 460
+// us, half of them zeros 460, a column of zeros, decays of e^-4 or steps of 0.001 take nothing more).
 //
 // Two kernels.  The first prepares all chunks side by side, a block per chunk and q/k head: q and k in half precision, T by
 // substitution, the weights of u_j, the gates' factors, as records in the workspace that lie as the second kernel's shared
@@ -63,9 +65,10 @@ constexpr int DC_WALKERS = 4;              // warps that walk a block's chunks
 constexpr int DC_FETCHERS = 128;           // threads that copy
 constexpr int DC_MAX_DIM = 128;
 constexpr int DC_SIZE = 12;                // a look brings the largest number of a column to 2^12 .. 2^13
+constexpr int DC_FIRST = -100, DC_LAST = 115;        // ... with powers of two from the one to the other
 constexpr int DC_DOWN = 3;                 // ... or, where R or U are then too large, to 2^-DC_DOWN of that
 constexpr float DC_LOW = 2048.f;           // on a low part whose products have a sum of their own
-constexpr float DC_T_SCALE = DC_LOW;       // on T, whose numbers are below beta^2 <= 4, as its record has it
+constexpr float DC_T_SCALE = DC_LOW;       // on T, whose numbers are below beta <= 2, as its record has it
 constexpr float DC_P_SCALE = 16384.f;      // ... and on the weights of u_j, which are below 1
 constexpr int DC_TLD = 16 + 8;             // padded rows of a 16 x 16 block in scratch
 constexpr int DC_ALD = 16 + 4;             // ... of floats
@@ -74,10 +77,12 @@ constexpr int DC_ALD = 16 + 4;             // ... of floats
 constexpr float DC_MOST = 32000.f;
 // What a column holds at a token, times sigma, is no less than this: R and U, as pairs, end at 2^-36, and what the weights' pairs leave
 // of a number of DC_MOST at 2^-32.
-constexpr float DC_LEAST = 1.f / 4096;
-// ... and the state, ahead of a chunk and behind it: its pairs, and those of what it takes in, end at 2^-25.  32 tokens' roundings there,
-// of either sign, are 2^-23.3 together, six units of 2^-24 beside this.
-constexpr float DC_LEAST_STATE = 1.f / 4;
+constexpr float DC_LEAST = 1.f / 8192;
+// ... and the state in front of a chunk no less than this: its pairs end at 2^-25, a rounding there (2^-25.8, the mean square) is nine
+// units of 2^-24.  What the chunk leaves: this times the root of the number of tokens that have not faded by then, whose pairs
+// end at 2^-25 as well; six for 32, and DC_ENOUGH is enough in any case.
+constexpr float DC_LEAST_STATE = 1.f / 32, DC_ENOUGH = 1.f / 4;
+static_assert(DC_ENOUGH == DC_LEAST * DC_T_SCALE, "one register for both");
 
 __device__ __forceinline__ unsigned dc_smem(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void dc_ldmatrix(unsigned (&r)[4], const void* p) {
@@ -224,11 +229,12 @@ struct DcRecord {
     struct alignas(16) Keys { __half k[PARTS][DC_TOKENS][KLD], q[PARTS][DC_TOKENS][KLD]; };
     struct alignas(16) Gates {
         __half t[2][3][16][16], p[2][3][16][16];               // T and the weights of u_j, two parts each; dc_piece()
-        float before[DC_TOKENS];          // on S0^T k: e^(G_i), the key's length, the power of two, DC_LOW
+        float before[DC_TOKENS];          // on S0^T k: b, e^(G_i), the key's length, the power of two, DC_LOW
         float after[DC_TOKENS];           // on u_j in the new state: e^(G_31 - G_j), ..., one over DC_T_SCALE
         float query[DC_TOKENS];           // on an output: scale, the query's length, the power of two, one over DC_P_SCALE
         float fade[DC_TOKENS];            // e^(G_i), times DC_P_SCALE, as the weights of u_j are
         float key[DC_TOKENS], decay[DC_TOKENS], beta[DC_TOKENS];        // the key's length, the power of two; e^log_decay; beta
+        float above[4];                   // b
     };
 };
 
@@ -304,7 +310,7 @@ struct DcMaker {                           // a preparing block's shared memory:
     float a[2][16 * DC_ALD + 16];          // A's blocks on the diagonal; the two are read at once, from other banks
     __half w[2][16][DC_TLD];
     double g[DC_TOKENS];
-    float kf[DC_TOKENS], qf[DC_TOKENS], beta[DC_TOKENS];
+    float kf[DC_TOKENS], qf[DC_TOKENS], beta[DC_TOKENS], share[DC_TOKENS], above;     // share: beta / b
 };
 
 __device__ __forceinline__ void dc_copy_out(void* to, const void* from, int bytes) {
@@ -452,19 +458,25 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
             }
             const double all = __shfl_sync(0xffffffffu, sum, DC_TOKENS - 1);
             const float kf = own.kf[lane], fade = expf((float)sum);
+            // b: 2^(n + 1) for a largest beta from 2^n on; 1 where that is nothing or not finite
+            const unsigned largest = __reduce_max_sync(0xffffffffu, __float_as_uint(beta) & 0x7fffffffu) >> 23;
+            const float above = largest > 0 && largest < 253 ? dc_power((int)largest - 126) : 1.f;
+            if (lane == 0) own.above = above;
             own.g[lane] = sum;
+            own.share[lane] = beta / above;
             own.beta[lane] = beta;
             if (z > 0) {                                       // the last head's record has left
                 if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
                 __syncwarp();
             }
-            own.gates.before[lane] = fade * kf * DC_LOW;
+            own.gates.before[lane] = fade * kf * (above * DC_LOW);
             own.gates.after[lane] = expf((float)(all - sum)) * kf * (1.f / DC_T_SCALE);
             own.gates.query[lane] = own.qf[lane] * (1.f / DC_P_SCALE);
             own.gates.fade[lane] = fade * DC_P_SCALE;
             own.gates.key[lane] = kf;
             own.gates.decay[lane] = expf(decay);
             own.gates.beta[lane] = beta;
+            if (lane < 4) own.gates.above[lane] = above;
             if (z + 1 < p.share && lane < n) {                 // the next head's
                 decay = p.log_decay[(size_t)(first + lane) * p.heads + head + 1];
                 beta = p.beta[(size_t)(first + lane) * p.heads + head + 1];
@@ -516,7 +528,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = j <= i ? x[j] * own.beta[16 * m + j] : 0.f;
+            for (int j = 0; j < 16; ++j) x[j] = j <= i ? x[j] * own.share[16 * m + j] : 0.f;
             unsigned high[8], low[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) dc_split_far(x[2 * j] * (DC_T_SCALE * DC_LOW), x[2 * j + 1] * (DC_T_SCALE * DC_LOW), high[j], low[j]);
@@ -528,7 +540,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
         }
         __syncthreads();
         if (warp == 1) {
-            // block (1, 0): -T_11 (A_10 / beta) T_00, beta being in T_11; A's numbers are below 1 and those of the second product, 16
+            // block (1, 0): -T_11 b (A_10 / beta) T_00, beta / b being in T_11; A / beta is below 1 and the second product's numbers, 16
             // summands, below 64: both go in DC_INNER times as large
             constexpr float DC_INNER = 512.f;
             unsigned ah[4], al[4], bh[4], bl[4];
@@ -571,7 +583,7 @@ delta_records_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     unsigned high, low;
-                    dc_split_far(w[j][2 * h] * (DC_LOW / DC_INNER), w[j][2 * h + 1] * (DC_LOW / DC_INNER), high, low);
+                    dc_split_far(w[j][2 * h] * (own.above * (DC_LOW / DC_INNER)), w[j][2 * h + 1] * (own.above * (DC_LOW / DC_INNER)), high, low);
                     *reinterpret_cast<unsigned*>(&own.gates.t[0][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = high;
                     *reinterpret_cast<unsigned*>(&own.gates.t[1][1][g + 8 * h][dc_piece(g, j) + 2 * t]) = low;
                 }
@@ -901,8 +913,10 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             }
         }
     };
-    const float least[2] = {col < p.vdim ? DC_LEAST * DC_T_SCALE : -1.f, col + 8 < p.vdim ? DC_LEAST * DC_T_SCALE : -1.f};
-    const float least_state[2] = {col < p.vdim ? DC_LEAST_STATE : -1.f, col + 8 < p.vdim ? DC_LEAST_STATE : -1.f};
+    // What the two columns' numbers are held against.  A column of zeros (S and v; those beyond the last among them) is out of the check
+    // and gets the largest power of two, so that the first number that is not zero is too large for it.
+    float least[2];
+    auto arm = [&](int h, bool there) { least[h] = there ? DC_ENOUGH : -1.f; };
     enum { FRESH, LITTLE, MUCH };                              // why a chunk is not walked just so: no sigma yet, small numbers, large ones
     int why = FRESH, down = 0, c = 0, stage = 0;
     bool looked = false, met = false;                          // sigma is this chunk's own; the chunk's meeting has been
@@ -921,19 +935,32 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             ask(st);
             if (why == LITTLE) {
                 // Nearly nothing is stored at a token, or taken in.  What the columns hold: the state's largest number and the values, faded.
-                float most[2];
+                float most[2], all[2];                         // faded; not faded, and as a look counts them
                 largest(most, sm.most[1]);
                 bool small = false;
-                most[0] *= sigma[0]; most[1] *= sigma[1];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) all[h] = most[h] *= sigma[h];
 #pragma unroll 2
                 for (int i = 0; i < tokens; ++i) {
-                    const float decay = st.gates.decay[i], beta = st.gates.beta[i], least = i + 1 < tokens ? DC_LEAST : DC_LEAST_STATE;
+                    const float decay = st.gates.decay[i], beta = st.gates.beta[i];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        most[h] = fmaxf(most[h] * decay, fabsf(value(st, i, h)) * beta * sigma[h]);
-                        small = small || (most[h] > 0.f && most[h] < least);
+                        const float x = fabsf(value(st, i, h));
+                        all[h] = fmaxf(all[h], x);
+                        most[h] = fmaxf(most[h] * decay, x * beta * sigma[h]);
+                        small = small || (most[h] > 0.f && most[h] < DC_LEAST);
                     }
                 }
+                float fade = 1.f, there = 0.f;                 // of the tokens behind; tokens that are still there
+                for (int i = tokens - 1; i >= 0 && fade >= 1.f / (1 << 21); --i) {
+                    there += 1.f;
+                    fade *= st.gates.decay[i];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) small = small || (most[h] > 0.f && most[h] * most[h] < there * (DC_LEAST_STATE * DC_LEAST_STATE));
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (all[h] == 0.f) { sigma[h] = dc_power(DC_LAST); back[h] = dc_power(-DC_LAST); arm(h, false); }
                 passed = !__any_sync(0xffffffffu, small);
             }
             if (!passed && looked && !(why == MUCH && down == 0)) {
@@ -956,12 +983,13 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
 #pragma unroll
                     for (int o = 1; o < 4; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
                     held[h] = most[h];
-                    most[h] = fmaxf(most[h], x);
+                    most[h] = fmaxf(most[h], x * st.gates.above[0]);
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int e = DC_SIZE - down - (((__float_as_int(most[h]) >> 23) & 255) - 127);
-                    const float next = most[h] > 0.f ? dc_power(min(max(e, -100), 100)) : sigma[h];
+                    const float next = dc_power(most[h] > 0.f ? min(max(e, DC_FIRST), DC_LAST) : DC_LAST);
+                    arm(h, most[h] > 0.f);
                     const float factor = next * back[h];
                     sigma[h] = next;
                     back[h] = 1.f / next;
@@ -1019,7 +1047,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                     float now[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        now[h] = beta * (value(st, i, h) * sigma[h] - decay * key * with_k[h]);
+                        now[h] = value(st, i, h) * beta * sigma[h] - beta * (decay * key * with_k[h]);
                         // a warp's own rows' summand of the output
                         if (t == 0) sm.out[c & 1][slice][i][group * 16 + 8 * h + g] = DC_P_SCALE * (decay * with_q[h] + kq * key * now[h]);
                     }
@@ -1131,7 +1159,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
                 query_step(0);
             }
             // ---- R, times DC_LOW, and U
-            const float sigma_far[2] = {sigma[0] * DC_LOW, sigma[1] * DC_LOW};
+            const float above = st.gates.above[0] * DC_LOW, sigma_far[2] = {sigma[0] * above, sigma[1] * above};
             float r[DC_TILES][4];
             v.widen(r);
 #pragma unroll
@@ -1215,7 +1243,7 @@ delta_walk_kernel(const DeltaParams p, const DcRecords records) {
             }
             const bool high = !(size < DC_MOST * DC_T_SCALE);
             // of a column's four lanes one at least has taken in enough, of both columns
-            unsigned enough = __ballot_sync(0xffffffffu, taken[0] >= least_state[0] && taken[1] >= least_state[1]);
+            unsigned enough = __ballot_sync(0xffffffffu, taken[0] >= least[0] && taken[1] >= least[1]);
             enough |= enough >> 2;
             enough |= enough >> 1;
             if (__builtin_expect(!passed && ((enough & 0x11111111u) != 0x11111111u ||

@@ -130,3 +130,38 @@ def test_one_column_among_others(longest):
     values(case)[0, 13] *= 1e7
     case.decay[3] = -1e4
     check_parts(case, longest, [3])
+
+
+@FORMS
+@TYPES
+def test_columns_of_zeros(dtype, dim, vdim, longest):
+    """Columns whose values are zero for a while, over a state of zeros: zero outputs as long as both are, and right ones when
+    values come, of whatever size."""
+    case = Case([300], 2, 1, dim, vdim, dtype)
+    v = values(case)
+    case.state.zero_()
+    v[:, 5] = 0.0
+    v[:150, 9] = 0.0
+    v[:100, 16:19] = 0.0
+    v[100:, 16], v[100:, 17] = v[100:, 16] * 1e-28, v[100:, 17] * 1e9
+    v[40:260] *= (torch.arange(case.heads * vdim, device="cuda") != 20)      # zeros in between
+    v[:64, vdim:] = 0.0                                        # the second head's first chunks
+    case.beta[130:140] = 0.0
+    check_parts(case, longest, [32, 64])
+    out, state = case.run(longest)
+    assert (out[:, 5] == 0).all() and (out[:100, 16:19] == 0).all() and (out[:64, vdim:] == 0).all()
+
+
+@FORMS
+def test_values_that_come_to_columns_of_zeros_without_a_step(longest):
+    """Nothing is stored (beta = 0) of values over a state of zeros: the outputs are zero."""
+    case = Case([200], 2, 1, 64, 48, torch.float32)
+    case.state.zero_()
+    v = values(case)
+    v[:64] = 0.0
+    case.beta[:130] = 0.0
+    out, state = case.run(longest)
+    want_out, want_state = case.want()
+    assert (out[:130] == 0).all()
+    near(out, want_out)
+    near(state, want_state)
