@@ -5,8 +5,9 @@
 // Bound by memory: every source is read and every destination written once (a source with several destinations comes
 // from L2 after its first read).  A thread block owns PART bytes of one pair, all of a thread's loads go out before
 // its first store, and the buffers' addresses travel with the launch, so that a fork of all layers is one launch.
-// 600 pages of 458,752 bytes: 80 us (6.9 TB/s); one state of 1 MB in each of 24 layers for eight forks: 36 us (226 MB, 6.3 TB/s); one
-// page: 3.6 us, a chain of list, load and store.
+// 600 pages of 458,752 bytes: 84.6 us a call (6.5 TB/s, the rate of a plain copy; the kernel ends after 80, its last writes still in
+// L2); one state of 1 MB in each of 24 layers for eight forks: 38 us (226 MB, 6.0 TB/s; the kernel 36); one page: 3.6 us, a chain of
+// list, load and store.
 // Pairs outside the pool are skipped and reported.
 #include "common.cuh"
 

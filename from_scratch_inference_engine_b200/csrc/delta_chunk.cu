@@ -13,14 +13,15 @@
 // instructions into every step; it adds to the two products that grow with the chunk (T R and the sum over u_j), by halves only
 // where the blocks of T above the diagonal are left out.
 //
-// Measured (bfloat16, heads of 128 x 128): 8,192 tokens of 16 q/k and 32 heads 361 us - records 56, walk 322, a part of it beside
-// the records -, against 42 for their bytes; 0.7 TB/s.  A chunk of a block that has its SM alone takes 2,470 cycles for 984 of tensor
-// instructions (123 of 8 cycles per warp), and no step of the chain stands out; with two blocks on an SM 3,400 for both, so that
-// four prompts of 2,048 tokens of 32 heads (512 blocks in 296 places) take 328 us: records 77, walk 266.  Chunks of 16 tokens took
+// Measured (bfloat16, heads of 128 x 128): 8,192 tokens of 16 q/k and 32 heads 358 us - records 61, walk 313, a part of it beside
+// the records -, against 42 for their bytes; 0.7 TB/s.  A chunk of a block that has its SM alone takes 2,400 cycles for 984 of tensor
+// instructions (123 of 8 cycles per warp), and no step of the chain stands out; with two blocks on an SM 3,500 for both, so that
+// four prompts of 2,048 tokens of 32 heads (512 blocks in 296 places) take 335 us: records 83, walk 273.  Chunks of 16 tokens took
 // 530 us for the 8,192 when those of 32, in their first form, took 443.
 //
 // Precision.  States and outputs are 32-bit results, so no operand may be rounded to 11 bits.  q and k (bfloat16, 8 bits)
-// scaled by a power of two to a length of about one are exact in half precision; what is 32-bit - the state, R, U, T and the
+// scaled by a power of two to a length of about one are exact in half precision (down to 2^-17 of the length; what is smaller is cut
+// at 2^-24 of it); what is 32-bit - the state, R, U, T and the
 // weights of u_j - goes into the instructions as the sum of two half-precision numbers (22 bits), products of two low parts left
 // out.  The state itself stays in 32-bit registers and the instructions only ever sum up one chunk (their running sums are
 // truncated, not rounded).  float32 storage: q and k are two parts as well.
@@ -320,9 +321,9 @@ __device__ __forceinline__ void dc_copy_out(void* to, const void* from, int byte
 
 // A block of four warps per chunk and q/k head: they take eight tokens' q and k each, then three of them one block of the
 // products and weights each, the fourth the gates' sums.  (One warp for all of it held as much shared memory and left seven warps
-// on an SM.)  8,192 tokens of 32 heads of 128 columns: 77 us, 330 MB read and written, 4.3 TB/s; 8,192 tokens of 16 q/k and 32 heads
-// 56 us.  A block is a chain of nine steps behind barriers (7,300 cycles alone, 20,000 among others), shared memory is busy 65 % of
-// the time, and five blocks to an SM beat six (80 us) and seven (96).
+// on an SM.)  8,192 tokens of 32 heads of 128 columns: 83 us, 336 MB read and written, 4.0 TB/s; 8,192 tokens of 16 q/k and 32 heads
+// 61 us.  A block is a chain of nine steps behind barriers (7,300 cycles alone, 20,000 among others), shared memory is busy 63 % of
+// the time, and five blocks to an SM beat six and seven (77 us against 80 and 96, before the low parts had a range of their own).
 constexpr int DC_MAKERS = 4;
 
 template <typename T, int DK, bool WIDE>

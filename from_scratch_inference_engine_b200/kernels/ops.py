@@ -2369,10 +2369,10 @@ def delta_prep(proj: torch.Tensor, conv_off: int, a_off: int, b_off: int, item_q
 
 # Up to so many tokens the recurrent form walks a request token by token; more go in chunks.  In steps of less than 128 heads of
 # requests, and in others.  Recurrent against chunked, heads of 128 x 128, bfloat16 and float32: one request of 16 heads, 4 tokens
-# 14 / 13 and 13 / 15 us, 8 tokens 20 / 13 and 20 / 15; 8 of 32 heads, 8 tokens 25 / 32 and 25 / 42, 16 tokens 39 / 32 and 37 / 42;
-# 64 of 32 heads, 10 tokens 156 / 169 and 141 / 278, 16 tokens 221 / 173 and 201 / 290, 24 tokens 311 / 179 and 281 / 300.
+# 14 / 13 and 12 / 15 us, 8 tokens 20 / 13 and 20 / 15; 8 of 32 heads, 8 tokens 22 / 34 and 22 / 42, 16 tokens 35 / 34 and 35 / 44;
+# 64 of 32 heads, 10 tokens 141 / 177 and 131 / 284, 16 tokens 199 / 181 and 188 / 288, 24 tokens 279 / 187 and 268 / 294.
 # In a step of both kinds each request goes its way, the two forms beside one another: 63 decoded tokens and a prompt's 512 (32 heads
-# of 128 x 128) take 95 us, 79 with `ones` given, against 198 all in chunks and 948 all token by token.  A step without short requests
+# of 128 x 128) take 99 us, 77 with `ones` given, against 210 all in chunks and 948 all token by token.  A step without short requests
 # pays 2 to 4 us of 40 to 250 for the launch, so one whose requests are all of one length is spared it.
 DELTA_FEW_TOKENS = {DTYPE_F32: (6, 16), DTYPE_BF16: (4, 10)}
 
