@@ -10,6 +10,7 @@ and the cache come from the context.
     class PositionEncoding: prepare(runtime, capacity); fields rotary_dim, table
     class Mixer:          cache_need() -> CacheNeed | None
                           state_need() -> StateNeed | None
+                          reserve(tokens, requests)        (working memory; may do nothing)
                           forward(ctx, y, cache: LayerCache) -> [tokens, hidden]
     class FeedForward:    forward(ctx, y) -> [tokens, hidden]
     class Arrangement:    forward(ctx, x, delta, cache) -> delta'
