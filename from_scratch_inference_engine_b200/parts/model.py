@@ -126,7 +126,8 @@ class DecoderModel:
     def reserve(self, tokens: int, requests: int) -> None:
         """Working memory that depends on how many requests share a step's tokens (see `Mixer.reserve`)."""
         for block in self.blocks:
-            block.mixer.reserve(tokens, requests)
+            if hasattr(block.mixer, "reserve"):           # (a registered mixer need not be a `Mixer`)
+                block.mixer.reserve(tokens, requests)
 
     # ------------------------------------------------------------------ forward
     def forward(self, ctx, caches: List[LayerCache], want_rows: Optional[torch.Tensor]):

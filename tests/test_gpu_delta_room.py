@@ -31,6 +31,16 @@ def test_the_chunks_of_any_step_fit():
     assert tight > 0
 
 
+def test_mixers_that_know_nothing_of_reserving():
+    """A registered mixer of the older interface, beside one that takes memory (host only)."""
+    from types import SimpleNamespace
+    from from_scratch_inference_engine_b200.parts.model import DecoderModel
+    seen = []
+    mixers = [object(), SimpleNamespace(reserve=lambda tokens, requests: seen.append((tokens, requests)))]
+    DecoderModel.reserve(SimpleNamespace(blocks=[SimpleNamespace(mixer=m) for m in mixers]), 7, 3)
+    assert seen == [(7, 3)]
+
+
 def chunk_bytes(case):
     from from_scratch_inference_engine_b200.kernels import ops
     return ops.delta().fsie_delta_chunk_bytes(case.heads, case.share, case.dim, ops._tag(case.qkv.dtype))
