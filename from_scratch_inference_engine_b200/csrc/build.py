@@ -69,6 +69,8 @@ LIBRARIES: Dict[str, Sequence[str]] = {
     "delta": ("delta_rule.cu", "delta_chunk.cu", "delta_prep.cu"),
     # blocks copied inside pools of pages and of states: forked requests, compaction
     "blocks": ("copy_blocks.cu",),
+    # penalties, biases and masks on logits, and the histories of tokens that the penalties go by
+    "logits": ("logits.cu",),
 }
 # specialisations compiled by build_all() beside the default form of every library
 DEFAULT_SPECIALISATIONS = {"attn_mma": [("-DHEAD_DIM=128",)],

@@ -2521,3 +2521,105 @@ def copy_blocks(buffers, moves: torch.Tensor, error: torch.Tensor) -> None:
     for first in range(0, len(bases), COPY_MAX_BUFFERS):
         _check(lib.fsie_copy_blocks(address + 8 * first, min(COPY_MAX_BUFFERS, len(bases) - first), size, blocks, moves, pairs,
                                     error, _stream()), "copy_blocks")
+
+
+# --------------------------------------------------- logits changed before a token is chosen
+_logits = None
+
+
+def logits_lib():
+    """Penalties, biases and masks on logits, and the histories of tokens behind the penalties."""
+    global _logits
+    if _logits is None:
+        lib = build.load_library("logits")
+        i, p = ctypes.c_int, ctypes.c_void_p
+        lib.fsie_adjust_logits.argtypes = [p, i, i, p, p, p, p, i, p, p, p, i, p, p, i, p, p]
+        lib.fsie_count_tokens.argtypes = [p, p, i, i, i, p, p, i, p, p]
+        lib.fsie_adjust_logits.restype = lib.fsie_count_tokens.restype = i
+        _logits = build.fast_calls(lib)
+    return _logits
+
+
+def bit_words(vocab: int) -> int:
+    """Words of 32 bits that a row of one bit per token takes: token v is bit v % 32 of word v // 32."""
+    return -(-vocab // 32)
+
+
+def count_tokens(tokens: torch.Tensor, slots: torch.Tensor, counts: torch.Tensor, seen: torch.Tensor, error: torch.Tensor,
+                 generated: bool = True) -> None:
+    """Take tokens[i] into the history slots[i] (int32 [n]; -1: into none): its bit of seen (int32 [histories, bit_words(vocab)])
+    is set and, if the tokens were generated, its place in counts (int32 [histories, vocab]) goes up by one.  A token
+    outside the vocabulary or a history that does not exist is left out and sets error[0] (int32)."""
+    if not (_fits(tokens, torch.int32, True) and _fits(slots, torch.int32, True) and _fits(counts, torch.int32, True)
+            and _fits(seen, torch.int32, True) and _fits(error, torch.int32, True)):
+        for tensor, name in ((tokens, "tokens"), (slots, "slots"), (counts, "counts"), (seen, "seen"), (error, "error")):
+            _need(tensor, torch.int32, name)
+    _history_shapes("count_tokens", counts, seen)
+    if tokens.shape != slots.shape or tokens.dim() != 1:
+        raise KernelError("count_tokens: tokens and slots must be [n]")
+    _check(logits_lib().fsie_count_tokens(tokens, slots, tokens.shape[0], counts.shape[1], counts.shape[0], counts, seen,
+                                          int(generated), error, _stream()), "count_tokens")
+
+
+def _history_shapes(what: str, counts: torch.Tensor, seen: torch.Tensor) -> None:
+    if counts.dim() != 2 or seen.dim() != 2 or seen.shape != (counts.shape[0], bit_words(counts.shape[1])):
+        raise KernelError(f"{what}: counts must be [histories, vocab] and seen [histories, words of 32 bits]")
+
+
+def adjust_logits(logits: torch.Tensor, error: torch.Tensor, slots: Optional[torch.Tensor] = None,
+                  penalties: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                  seen: Optional[torch.Tensor] = None, bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None,
+                  masks: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> torch.Tensor:
+    """Change logits (float32 [rows, vocab]) in place; returns them.  In this order, each where it is given:
+
+    slots (int32 [rows], the row's history or -1), penalties (float32 [rows, 3]: theta > 0, presence, frequency), counts and
+    seen (see `count_tokens`): a token that the history holds gets z / theta where z > 0, else z * theta, less presence if
+    it was generated, less frequency for every time it was;
+    bias (int32 [rows + 1], int32 [n], float32 [n]): row r adds the values bias[2][i] to the tokens bias[1][i] for i from
+    bias[0][r] on and in front of bias[0][r + 1], tokens in rising order;
+    masks (int32 [rows], int32 [m, bit_words(vocab)]): row r may take what mask row masks[0][r] allows (-1: everything); the
+    others become -inf.  A mask without a bit leaves a row of -inf.
+
+    A history or a mask that does not exist counts as none, a token of a bias outside the vocabulary or out of order is
+    left out; each sets error[0] (int32)."""
+    if not (_fits(logits, torch.float32, True) and _fits(error, torch.int32, True)):
+        _need(logits, torch.float32, "logits")
+        _need(error, torch.int32, "error")
+    if logits.dim() != 2:
+        raise KernelError("adjust_logits: logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    histories = biases = mask_count = 0
+    if slots is not None:
+        if penalties is None or counts is None or seen is None:
+            raise KernelError("adjust_logits: slots go with penalties, counts and seen")
+        for tensor, dtype, name in ((slots, torch.int32, "slots"), (penalties, torch.float32, "penalties"),
+                                    (counts, torch.int32, "counts"), (seen, torch.int32, "seen")):
+            if not _fits(tensor, dtype, True):
+                _need(tensor, dtype, name)
+        _history_shapes("adjust_logits", counts, seen)
+        if slots.shape != (rows,) or penalties.shape != (rows, 3) or counts.shape[1] != vocab:
+            raise KernelError("adjust_logits: a slot, three penalties and counts of the vocabulary are needed for every row")
+        histories = counts.shape[0]
+    start = token = value = None
+    if bias is not None:
+        start, token, value = bias
+        for tensor, dtype in ((start, torch.int32), (token, torch.int32), (value, torch.float32)):
+            if not _fits(tensor, dtype, True):
+                _need(tensor, dtype, "bias")
+        if start.shape != (rows + 1,) or token.dim() != 1 or token.shape != value.shape:
+            raise KernelError("adjust_logits: a bias is [rows + 1] starts, [n] tokens and [n] values")
+        biases = token.shape[0]
+    mask_of = bits = None
+    if masks is not None:
+        mask_of, bits = masks
+        if not (_fits(mask_of, torch.int32, True) and _fits(bits, torch.int32, True)):
+            _need(mask_of, torch.int32, "masks")
+            _need(bits, torch.int32, "masks")
+        if mask_of.shape != (rows,) or bits.dim() != 2 or bits.shape[1] != bit_words(vocab):
+            raise KernelError("adjust_logits: masks are [rows] indices and [m, words of 32 bits]")
+        mask_count = bits.shape[0]
+    _check(logits_lib().fsie_adjust_logits(logits, rows, vocab, slots, penalties if slots is not None else None,
+                                           counts if slots is not None else None, seen if slots is not None else None,
+                                           histories, start, token, value, biases, mask_of, bits, mask_count, error, _stream()),
+           "adjust_logits")
+    return logits
