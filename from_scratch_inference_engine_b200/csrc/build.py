@@ -69,12 +69,15 @@ LIBRARIES: Dict[str, Sequence[str]] = {
     "delta": ("delta_rule.cu", "delta_chunk.cu", "delta_prep.cu"),
     # blocks copied inside pools of pages and of states: forked requests, compaction
     "blocks": ("copy_blocks.cu",),
+    # attention over pages that several requests share, one build per head size: defines=("-DHEAD_DIM=128",)
+    "attn_shared": ("shared_attention.cu",),
     # penalties, biases and masks on logits, and the histories of tokens that the penalties go by
     "logits": ("logits.cu",),
 }
 # specialisations compiled by build_all() beside the default form of every library
 DEFAULT_SPECIALISATIONS = {"attn_mma": [("-DHEAD_DIM=128",)],
-                           "attn_tc": [("-DHEAD_DIM=128",)]}
+                           "attn_tc": [("-DHEAD_DIM=128",)],
+                           "attn_shared": [("-DHEAD_DIM=128",), ("-DHEAD_DIM=64",)]}
 
 _loaded: Dict[Tuple[str, Tuple[str, ...]], ctypes.CDLL] = {}
 _lock = threading.Lock()

@@ -2523,6 +2523,103 @@ def copy_blocks(buffers, moves: torch.Tensor, error: torch.Tensor) -> None:
                                     error, _stream()), "copy_blocks")
 
 
+# ----------------------------------------------------- attention over pages that requests share
+_attn_shared: Dict[int, object] = {}
+SHARED_ATTENTION_MAX_RUNS = 1024
+
+
+def attn_shared(head_dim: int):
+    """The library of the attention over shared pages for a head size, compiled at first use."""
+    if head_dim not in _attn_shared:
+        lib = build.load_library("attn_shared", (f"-DHEAD_DIM={head_dim}",))
+        i, f, ll, p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
+        lib.fsie_shared_attention_head_dim.argtypes = lib.fsie_shared_attention_max_runs.argtypes = []
+        lib.fsie_shared_attention_head_dim.restype = lib.fsie_shared_attention_max_runs.restype = i
+        lib.fsie_shared_attention_room.argtypes = [i, i, i, i, i, i]
+        lib.fsie_shared_attention_room.restype = ll
+        lib.fsie_shared_attention.argtypes = [p, i, p, p, ll, i, i, p, i, i, p, i, p, i, p, i, p, p, i, i, i, i, f, p, ll, i, i,
+                                              p, p]
+        lib.fsie_shared_attention.restype = i
+        if lib.fsie_shared_attention_head_dim() != head_dim or lib.fsie_shared_attention_max_runs() != SHARED_ATTENTION_MAX_RUNS:
+            raise KernelError("shared_attention: the library was built for other sizes")
+        _attn_shared[head_dim] = build.fast_calls(lib)
+    return _attn_shared[head_dim]
+
+
+def shared_attention_takes(dtype: torch.dtype, head_dim: int) -> bool:
+    return dtype in (torch.bfloat16, torch.float32) and head_dim % 16 == 0 and 16 <= head_dim <= 256
+
+
+def shared_attention_room(tokens: int, runs: int, levels: int, heads: int, kv_heads: int, head_dim: int,
+                          dtype: torch.dtype) -> int:
+    """Bytes of working memory that `shared_attention` needs for so many places in `order` and runs, with at most `levels`
+    runs around an innermost one."""
+    size = attn_shared(head_dim).fsie_shared_attention_room(tokens, runs, levels, heads, kv_heads, _tag(dtype))
+    if size < 0:
+        raise KernelError(f"shared_attention_room: refused ({size})")
+    return size
+
+
+def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages: torch.Tensor, page_stride: int,
+                     page_size: int, block_tables: torch.Tensor, positions: torch.Tensor, order: torch.Tensor,
+                     runs: torch.Tensor, own_run: torch.Tensor, out: torch.Tensor, heads: int, kv_heads: int, head_dim: int,
+                     scale: float, room: torch.Tensor, error: torch.Tensor, early: bool = False) -> torch.Tensor:
+    """Causal grouped-query attention of new tokens over a paged cache in which requests hold the same leading pages: keys
+    and values that several requests share are read once for all of them.
+
+    q [tokens, ..] (float32 or bfloat16; head h of token t at t * q_ld + h * head_dim), k_pages and v_pages [pages, kv_heads,
+    page_size, head_dim] (views; page p begins p * page_stride elements further), block_tables int32 [requests, width],
+    positions int32 [tokens].  Every key that a token sees lies in one run:
+
+    order    int32 [n], the tokens to work on, so arranged that the tokens of every run are neighbours
+    runs     int32 [r, 6]: first place in order, number of places, first key, end of the keys, row of block_tables that has
+             their pages, index of the run around it or -1 (a run comes behind the run around it).  Its keys are behind those
+             of the run around it
+    own_run  int32 [n]: the innermost run of the token at each place.  It belongs to one request, whose tokens see its keys up
+             to their positions.  The runs around it end in front of all of their tokens
+
+    out [tokens, ..] gets the rows of the tokens in `order` (zeros for a token without keys); other rows stay as they are.
+    `room`: uint8, `shared_attention_room` bytes.  A run or token outside of what there is, or a shared run that reaches
+    beyond one of its tokens, sets error[0] to 7, a page outside the pool to 3 (its keys are left out), runs that nest
+    deeper than `room` was made for to 8; the rows concerned hold no result.  `early`: the lists, tables and positions are
+    older than the stream's last kernel."""
+    if not (_fits(block_tables, torch.int32, True) and _fits(positions, torch.int32, True) and _fits(order, torch.int32, True)
+            and _fits(runs, torch.int32, True) and _fits(own_run, torch.int32, True) and _fits(error, torch.int32, True)
+            and _fits(room, torch.uint8, True)):
+        for tensor, name in ((block_tables, "block_tables"), (positions, "positions"), (order, "order"), (runs, "runs"),
+                             (own_run, "own_run"), (error, "error")):
+            _need(tensor, torch.int32, name)
+        _need(room, torch.uint8, "room")
+    dtype = q.dtype
+    for tensor, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (out, "out")):
+        if not _fits(tensor, dtype, False):
+            _need(tensor, dtype, name, contiguous=False)
+    if not shared_attention_takes(dtype, head_dim):
+        raise KernelError(f"shared_attention: {dtype} with heads of {head_dim} is not taken")
+    if block_tables.dim() != 2 or runs.dim() != 2 or runs.shape[1] != 6 or order.dim() != 1 or own_run.shape != order.shape \
+            or positions.dim() != 1:
+        raise KernelError("shared_attention: block_tables [requests, width], positions [tokens], order and own_run [n] and runs "
+                          "[r, 6] are needed")
+    if runs.shape[0] > SHARED_ATTENTION_MAX_RUNS:
+        raise KernelError(f"shared_attention: {runs.shape[0]} runs, the kernels take {SHARED_ATTENTION_MAX_RUNS}")
+    if kv_heads <= 0 or heads <= 0 or heads % kv_heads or page_size <= 0 or not 0 < scale < float("inf"):
+        raise KernelError("shared_attention: heads must be a multiple of kv_heads, page_size and scale positive")
+    tokens = positions.shape[0]
+    if q.dim() != 2 or out.dim() != 2 or min(q.shape[0], out.shape[0]) < tokens or q.stride(0) != q_ld or q.stride(1) != 1 \
+            or min(q.shape[1], out.shape[1]) < heads * head_dim or out.stride(1) != 1:
+        raise KernelError("shared_attention: q and out must hold a row of all heads for every token")
+    layout = (kv_heads, page_size, head_dim)
+    strides = (page_stride, page_size * head_dim, head_dim, 1)
+    if k_pages.shape[1:] != layout or v_pages.shape != k_pages.shape or k_pages.stride() != strides or v_pages.stride() != strides:
+        raise KernelError("shared_attention: pages of keys and of values must be [pages, kv_heads, page_size, head_dim], "
+                          "page_stride apart")
+    _check(attn_shared(head_dim).fsie_shared_attention(
+        q, q_ld, k_pages, v_pages, page_stride, page_size, k_pages.shape[0], block_tables, block_tables.shape[0],
+        block_tables.shape[1], positions, tokens, order, order.shape[0], runs, runs.shape[0], own_run, out, out.stride(0), heads,
+        kv_heads, head_dim, float(scale), room, room.numel(), _tag(dtype), int(early), error, _stream()), "shared_attention")
+    return out
+
+
 # --------------------------------------------------- logits changed before a token is chosen
 _logits = None
 
