@@ -311,7 +311,8 @@ def test_replayed_with_other_lists_and_on_another_stream():
     rows = max(len(p.found.runs), len(other.found.runs))
     order, own_run = p.lists[0].clone(), p.lists[2].clone()
     runs, tables = torch.zeros(rows, 6, dtype=torch.int32, device="cuda"), ints(p.tables)
-    rooms = [torch.empty(1 << 24, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    size = ops().shared_attention_room(len(order), rows, max(p.found.levels, other.found.levels), 12, 2, 64, torch.bfloat16)
+    rooms = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(2)]
     graphs = []
     side = torch.cuda.Stream()
     for room in rooms:
