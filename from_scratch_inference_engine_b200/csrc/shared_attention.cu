@@ -15,23 +15,25 @@
 // tokens see, so their rows - a row is a (token, head of the group) pair - fill tiles whatever request they are of, and no
 // row of any tile sees other keys than the tile's other rows.
 //
-// Four launches.  What the runs are is known on the device only (a captured graph replays with others):
+// Two launches.  What the runs are is known on the device only (a captured graph replays with others), so every block works
+// the plan out by itself: all (tile, kv head) lines of the runs laid end to end, in steps of keys, cut into equal pieces, one
+// per worker; runs of few rows (a token's own keys) and of many (shared ones) are two such rows of lines.  The first launch
+// walks through both, a worker from line to line with the next steps' keys on their way, and leaves the triple of every
+// stretch of a line that it has worked on in `room`:
 //
-//   plan    lays all (tile, kv head) lines of the runs end to end, in steps of keys, cuts them into equal pieces, one per
-//           worker, and writes down every worker's stretches of lines; runs of few rows (a token's own keys) and of many
-//           (shared ones) are two such rows of lines, for different kernels
-//   many    tcgen05 (head sizes 64 and 128), mma.sync or FFMA: a worker is a block
-//   few     beside it: a worker is a warp (bfloat16) or a block (float32)
-//   merge   joins the triples of a row, in a fixed order
+//   many rows   tcgen05 (head sizes 64 and 128), mma.sync or FFMA: a worker is a block
+//   few rows    a worker is a warp (bfloat16) or a block (float32)
 //
-// What a small call waits for is instructions: they come at 7 to 10 cycles each the first time a multiprocessor runs them,
-// and 750 cycles pass for each read of what another kernel has written.  With every block working out its own stretches, and
-// the merge looking up its runs, 8 requests of a 4,096-token prompt (28 heads over 4 of 128) took 23.8 us, with the plan XX.
+// The second joins the triples of a row, in a fixed order; it makes its plan while the first still runs.
+//
+// What a small call waits for is a chain of reads of what other multiprocessors hold, 750 cycles each, and instructions that
+// run for the first time.  8 requests of a 4,096-token prompt, 28 heads over 4 of 128: 23.9 us with a launch for the plan in
+// front, one each for many and few rows and one for the merge; 31.5 in one cooperative launch whose blocks meet twice
+// (6 of them between two such launches); 20.7 as it is.
 #include "common.cuh"
 #include "tma.cuh"
 #include "attention_tc.cuh"
 #include <math.h>
-#include <string.h>
 
 #ifndef HEAD_DIM
 #error "compile with -DHEAD_DIM=<head size>"
@@ -42,25 +44,16 @@ namespace fsie {
 
 constexpr int HD = HEAD_DIM;
 constexpr int FEW = 16;                  // rows that count as few: those of a tile
-constexpr int MMA_FEW_KEYS = 16, MMA_MANY_KEYS = 64, F32_KEYS = 32;       // keys of a step
-constexpr int MAX_RUNS = 1024;
-constexpr int MAX_LEVELS = 32;           // one more than runs may lie around each other, the innermost among them
+constexpr int MMA_FEW_KEYS = 16, MMA_MANY_KEYS = HD <= 128 ? 64 : 32, F32_KEYS = 32;       // keys of a step
+constexpr int MAX_RUNS = 768;
+constexpr int MAX_LEVELS = 32;           // runs that lie around each other, the innermost among them
 constexpr int RUN_INTS = 6;
 constexpr int LINE_PIECES = 32;          // a line is cut into no more pieces than this: what joins them reads them all
 constexpr int FEW_LEAST = 2, MANY_LEAST = 1;                              // steps of a piece, at least
 enum { ERR_PAGE = 3, ERR_RUNS = 7, ERR_ROOM = 8 };
 
-// A worker's stretch of a line.
-struct __align__(16) Stretch {
-    int worker, steps, k0, kend;         // whose it is; steps of keys, the first's first key, end of the keys
-    int table, kvh, place, row0;         // row of the block tables; the tile's rows are rows row0 .. of the tokens from `place` on
-    int rows, begin, token, spare;       // (begin: the run's first key: steps may begin in front of it; token: that of a tile of one)
-};
-// One launch's side of the plan.
+// One side of the plan: the runs of few rows or of many.
 struct Side {
-    int* first;                          // [workers] the worker's first stretch, -1: none
-    int2* lines;                         // [line_room] a line's first stretch, and how many it has
-    Stretch* stretches;                  // [line_room + workers + 1]; those of a worker follow each other
     int workers, line_room, tile, keys, align, least;         // (align: where steps begin, a power of two)
     long long row0;                      // the triples of stretch s are rows row0 + s * tile ..
 };
@@ -76,7 +69,6 @@ struct SharedArgs {
     void* out; int out_ld;
     int heads, kv_heads, group; float scale;
     Side few, many;
-    int4* levels;                                             // [places][MAX_LEVELS]: see Level
     float* part_ml; float* part_o;                            // the triples: [rows, 2], [rows, HD]
     int early;                                                // the lists are older than the stream's last kernel
     int* error;
@@ -95,25 +87,34 @@ __device__ __forceinline__ Tiling tiling(const SharedArgs& a, int kind, int most
     return {kind & RUN_INNERMOST ? 1 : most / a.group, 1};
 }
 
-constexpr int PLAN_THREADS = 256, PLAN_BLOCKS = 32;
-struct PlanShared {
-    Run runs[MAX_RUNS];                  // count 0 where a run has no keys or places, or points outside of what there is
-    int line0[2][MAX_RUNS + 1], step0[2][MAX_RUNS + 1];       // lines and steps in front of each run, few and many
-    unsigned char kind[MAX_RUNS];
-    int sums[4][PLAN_THREADS / 32], longest[2][PLAN_THREADS / 32];
+// What every block keeps in shared memory.
+struct Plan {
+    Run* runs;                           // [run_count]; count 0 where a run has no keys or places, or points outside of what there is
+    int *sums, stride;                   // see line0 and step0
+    unsigned char* kind;
+    int few_piece, many_piece, few_total, many_total, few_lines, many_lines;      // steps of a piece, steps and lines in all
+    // [run_count + 1] lines and steps in front of each run, few (0) and many (1)
+    __device__ __forceinline__ int* line0(int many) const { return sums + many * stride; }
+    __device__ __forceinline__ int* step0(int many) const { return sums + (2 + many) * stride; }
 };
+__host__ __device__ __forceinline__ size_t plan_bytes(int runs) { return ((size_t)runs * (sizeof(Run) + 1) + 4 * ((size_t)runs + 1) * 4 + 15) / 16 * 16; }
+constexpr int MAX_WARPS = 10;            // of a block
+struct PlanSums { int sums[4][MAX_WARPS], longest[2][MAX_WARPS]; };
 
 __device__ __forceinline__ int run_kind(const SharedArgs& a, const Run& run, int r) {
     const int innermost = a.own_run[run.first] == r ? RUN_INNERMOST : 0;
     return innermost | ((innermost ? a.group : run.count * a.group) <= FEW ? RUN_FEW : 0);
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS)
-shared_plan_kernel(const __grid_constant__ SharedArgs a) {
-    __shared__ PlanShared s;
+// All PLAN_THREADS threads of a block; false (and *error): it does not fit the room.
+template <int PLAN_THREADS>
+__device__ __forceinline__ bool make_plan(const SharedArgs& a, unsigned char* smem, PlanSums& s, Plan& plan) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    if (!a.early) grid_dependency_wait();
-    for (int e = tid; e < a.run_count * RUN_INTS; e += PLAN_THREADS) reinterpret_cast<int*>(s.runs)[e] = a.runs[e];
+    plan.runs = reinterpret_cast<Run*>(smem);
+    plan.sums = reinterpret_cast<int*>(plan.runs + a.run_count);
+    plan.stride = a.run_count + 1;
+    plan.kind = reinterpret_cast<unsigned char*>(plan.sums + 4 * plan.stride);
+    for (int e = tid; e < a.run_count * RUN_INTS; e += PLAN_THREADS) reinterpret_cast<int*>(plan.runs)[e] = a.runs[e];
     __syncthreads();
     // ---- runs: checked, sorted into few and many, summed up
     int before[4] = {0, 0, 0, 0}, longest[2] = {0, 0};                    // lines of few and many, steps of few and many
@@ -122,7 +123,7 @@ shared_plan_kernel(const __grid_constant__ SharedArgs a) {
         const int r = base + tid;
         int mine[4] = {0, 0, 0, 0};
         if (r < a.run_count) {
-            Run run = s.runs[r];
+            Run run = plan.runs[r];
             int kind = 0;
             if (run.count <= 0 || run.end <= run.begin) {
                 run.count = 0;
@@ -143,8 +144,8 @@ shared_plan_kernel(const __grid_constant__ SharedArgs a) {
                 mine[many] = lines; mine[2 + many] = (int)steps;
                 longest[many] = max(longest[many], of_line);
             }
-            s.runs[r].count = run.count;
-            s.kind[r] = (unsigned char)kind;
+            plan.runs[r].count = run.count;
+            plan.kind[r] = (unsigned char)kind;
         }
         int upto[4];
 #pragma unroll
@@ -165,8 +166,8 @@ shared_plan_kernel(const __grid_constant__ SharedArgs a) {
             before[i] += (int)__reduce_add_sync(0xffffffffu, (unsigned)of_warp);
         }
         if (r < a.run_count) {
-            s.line0[0][r] = upto[0] - mine[0]; s.line0[1][r] = upto[1] - mine[1];
-            s.step0[0][r] = upto[2] - mine[2]; s.step0[1][r] = upto[3] - mine[3];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) plan.sums[i * plan.stride + r] = upto[i] - mine[i];
         }
         __syncthreads();
     }
@@ -174,95 +175,83 @@ shared_plan_kernel(const __grid_constant__ SharedArgs a) {
     for (int i = 0; i < 2; ++i) {
         longest[i] = __reduce_max_sync(0xffffffffu, longest[i]);
         if (lane == 0) s.longest[i][warp] = longest[i];
-        if (tid == 0) { s.line0[i][a.run_count] = before[i]; s.step0[i][a.run_count] = before[2 + i]; }
+        if (tid == 0) { plan.line0(i)[a.run_count] = before[i]; plan.step0(i)[a.run_count] = before[2 + i]; }
     }
     overflow = __syncthreads_or(overflow);
-    int piece[2];
     bool fits = !overflow;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const Side& side = i ? a.many : a.few;
         const int l = __reduce_max_sync(0xffffffffu, lane < PLAN_THREADS / 32 ? s.longest[i][lane] : 0);
-        piece[i] = max((before[2 + i] + side.workers - 1) / side.workers, max(side.least, (l + LINE_PIECES - 1) / LINE_PIECES));
+        (i ? plan.many_lines : plan.few_lines) = before[i];
+        (i ? plan.many_total : plan.few_total) = before[2 + i];
+        (i ? plan.many_piece : plan.few_piece) = max((before[2 + i] + side.workers - 1) / side.workers, max(side.least, (l + LINE_PIECES - 1) / LINE_PIECES));
         fits = fits && before[i] <= side.line_room;
     }
-    if (!fits && tid == 0 && blockIdx.x == 0) atomicExch(a.error, ERR_ROOM);
-    if (a.early) grid_dependency_wait();                  // (the kernel in front may still read the last plan)
-    grid_dependents_go();
+    if (!fits && tid == 0) atomicExch(a.error, ERR_ROOM);
+    return fits;
+}
 
-    // ---- workers without a piece, lines, places
-    const int lines = fits ? before[0] + before[1] : 0, workers = a.few.workers + a.many.workers;
-    const int tasks = workers + lines + a.places;
-    for (int task = blockIdx.x * PLAN_THREADS + tid; task < tasks; task += gridDim.x * PLAN_THREADS) {
-        if (task < workers) {
-            const int many = task >= a.few.workers, worker = many ? task - a.few.workers : task;
-            if (!fits || (long long)worker * piece[many] >= before[2 + many]) (many ? a.many : a.few).first[worker] = -1;
-        } else if (task < workers + lines) {
-            int number = task - workers;
-            const int many = number >= before[0];
-            if (many) number -= before[0];
-            const Side& side = many ? a.many : a.few;
-            const int* line0 = s.line0[many];
-            int low = 0, high = a.run_count;              // line0[low] <= number < line0[low + 1]
-            while (high - low > 1) {
-                const int middle = (low + high) >> 1;
-                if (line0[middle] <= number) low = middle; else high = middle;
-            }
-            const Run run = s.runs[low];
-            const int kind = s.kind[low], line = number - line0[low], aligned = run.begin & ~(side.align - 1);
-            const int of_line = (run.end - aligned - 1) / side.keys + 1, from = s.step0[many][low] + line * of_line;
-            const Tiling t = tiling(a, kind, side.tile);
-            const int tile = line / a.kv_heads;
-            Stretch n;
-            n.kvh = line - tile * a.kv_heads;
-            const int token = t.parts > 1 ? tile / t.parts : tile * t.tokens;
-            n.place = run.first + token;
-            n.row0 = t.parts > 1 ? (tile - token * t.parts) * side.tile : 0;
-            n.rows = min(side.tile, t.parts > 1 ? a.group - n.row0 : min(t.tokens, run.count - token) * a.group);
-            n.begin = run.begin; n.kend = run.end; n.table = run.table; n.spare = 0;
-            n.token = t.tokens == 1 ? a.order[n.place] : -1;
-            if (kind & RUN_INNERMOST) {
-                const int position = (unsigned)n.token < (unsigned)a.tokens ? a.positions[n.token] : -1;
-                if (position < run.end) n.kend = position + 1;
-            }
-            const int worker0 = from / piece[many], last = from + of_line;
-            int at = from, worker = worker0;
-            for (; at < last; ++worker) {
-                const int until = min((worker + 1) * piece[many], last);
-                n.worker = worker; n.steps = until - at; n.k0 = aligned + (at - from) * side.keys;
-                const int slot = number + worker;
-                side.stretches[slot] = n;
-                if (at == worker * piece[many]) side.first[worker] = slot;
-                at = until;
-            }
-            side.lines[number] = make_int2(number + worker0, worker - worker0);
-            if (last == worker * piece[many] || last == before[2 + many]) side.stretches[number + worker].worker = -1;       // a gap, or the end
-        } else {
-            // the token's runs, from the innermost on: its first row in the first of its tiles' lines
-            const int place = task - workers - lines, token = a.order[place];
-            int4* levels = a.levels + (size_t)place * MAX_LEVELS;
-            const bool there = (unsigned)token < (unsigned)a.tokens;
-            const int position = there ? a.positions[token] : -1;
-            int r = a.own_run[place], count = 0, depth = 0;
-            if (!there || !fits || r >= a.run_count) r = -1;
-            for (; r >= 0 && depth < MAX_LEVELS - 1; ++depth) {
-                const Run run = s.runs[r];
-                if (run.count > 0 && place >= run.first && place < run.first + run.count) {
-                    const int kind = s.kind[r], many = kind & RUN_FEW ? 0 : 1;
-                    const Tiling t = tiling(a, kind, (many ? a.many : a.few).tile);
-                    const int token_in = place - run.first, tile = t.parts > 1 ? token_in * t.parts : token_in / t.tokens;
-                    levels[1 + count] = make_int4(s.line0[many][r] + tile * a.kv_heads, many, (token_in - tile * t.tokens) * a.group, 0);
-                    if (t.parts > 1) levels[1 + count].z = 0;
-                    ++count;
-                    // (a shared run ends in front of its tokens)
-                    if (!(kind & RUN_INNERMOST) && run.end - 1 > position) atomicExch(a.error, ERR_RUNS);
-                }
-                r = run.parent < r ? run.parent : -1;
-            }
-            if (r >= 0 || !there) atomicExch(a.error, ERR_RUNS);
-            levels[0] = make_int4(count, there ? token : -1, 0, 0);
-        }
+// ---- a worker's piece, as stretches: the part of a line that lies in it.  The lines of a side are numbered through, so the
+// k-th stretch of a worker belongs to the k-th line behind its first, and any thread can work out any stretch by itself.
+struct __align__(16) Stretch {
+    int steps, k0, kend, slot;           // 0: there is none; first step's first key, end of the keys; where the triple goes, in tiles
+    int table, kvh, place, row0;         // row of the block tables; the tile's rows are rows row0 .. of the tokens from `place` on
+    int rows, begin, token, spare;       // (begin: the run's first key: steps may begin in front of it; token: that of a tile of one)
+};
+struct Piece { int from, end, first_line, worker; };          // steps, and the line in which the piece starts; from = end: no piece
+
+// largest r with at[r] <= value, for at[0] <= value < at[count]
+__device__ __forceinline__ int find_run(const int* at, int count, int value) {
+    int low = 0, high = count;
+    while (high - low > 1) {
+        const int middle = (low + high) >> 1;
+        if (at[middle] <= value) low = middle; else high = middle;
     }
+    return low;
+}
+__device__ __forceinline__ int line_steps(const Run& run, const Side& side) { return (run.end - (run.begin & ~(side.align - 1)) - 1) / side.keys + 1; }
+
+template <int MANY>
+__device__ __forceinline__ Piece piece_of(const SharedArgs& a, const Plan& plan, int worker) {
+    const Side& side = MANY ? a.many : a.few;
+    const int step_piece = MANY ? plan.many_piece : plan.few_piece, total = MANY ? plan.many_total : plan.few_total;
+    Piece piece = {0, 0, 0, worker};
+    const long long from = (long long)worker * step_piece;
+    if (from >= total) return piece;
+    piece.from = (int)from;
+    piece.end = piece.from + min(step_piece, total - piece.from);
+    const int r = find_run(plan.step0(MANY), a.run_count, piece.from);
+    piece.first_line = plan.line0(MANY)[r] + (piece.from - plan.step0(MANY)[r]) / line_steps(plan.runs[r], side);
+    return piece;
+}
+template <int MANY>
+__device__ __forceinline__ void stretch_of(const SharedArgs& a, const Plan& plan, const Piece& piece, int k, Stretch& n) {
+    const Side& side = MANY ? a.many : a.few;
+    n.steps = 0;
+    const int number = piece.first_line + k;
+    if (piece.from == piece.end || number >= (MANY ? plan.many_lines : plan.few_lines)) return;
+    const int r = find_run(plan.line0(MANY), a.run_count, number);
+    const Run run = plan.runs[r];
+    const int kind = plan.kind[r], line = number - plan.line0(MANY)[r], of_line = line_steps(run, side), begin = plan.step0(MANY)[r] + line * of_line;
+    const int first = max(begin, piece.from), last = min(begin + of_line, piece.end);
+    if (first >= last) return;
+    const Tiling t = tiling(a, kind, side.tile);
+    const int tile = line / a.kv_heads;
+    n.kvh = line - tile * a.kv_heads;
+    const int token = t.parts > 1 ? tile / t.parts : tile * t.tokens;
+    n.place = run.first + token;
+    n.row0 = t.parts > 1 ? (tile - token * t.parts) * side.tile : 0;
+    n.rows = min(side.tile, t.parts > 1 ? a.group - n.row0 : min(t.tokens, run.count - token) * a.group);
+    n.k0 = (run.begin & ~(side.align - 1)) + (first - begin) * side.keys;
+    n.begin = run.begin; n.kend = run.end; n.table = run.table;
+    n.slot = number + piece.worker;
+    n.token = t.tokens == 1 ? a.order[n.place] : -1;
+    if (kind & RUN_INNERMOST) {
+        const int position = (unsigned)n.token < (unsigned)a.tokens ? a.positions[n.token] : -1;
+        if (position < run.end) n.kend = position + 1;
+    }
+    n.steps = last - first;
 }
 
 __device__ __forceinline__ unsigned smem_u32(const void* p) { return (unsigned)__cvta_generic_to_shared(p); }
@@ -309,7 +298,7 @@ constexpr int THREADS = 128;
 struct Step {
     Stretch of;
     int valid, k0, first, last;          // whether there is one; its first key; first or last of its stretch
-    int stretch, slot;                   // how many stretches the worker has begun before; this one's number in all
+    int stretch;                         // how many stretches the worker has begun before
 };
 template <typename T, int ROWS, bool IS_FEW, int KEYS, int STAGES, int K_LD, int V_LD, int Q_LD>
 struct Feed {
@@ -322,26 +311,25 @@ struct Feed {
         Step steps[RECORDS];
     };
     const SharedArgs& a;
-    const Side& side;
+    const Plan& plan;
     Shared& sh;
     T *ks, *vs, *qs;
-    int slot, stretches, at;                                              // thread 0's: the stretch, and the step of it
+    Piece piece;
+    int stretches, at;                                                    // thread 0's: the stretch, and the step of it
 
-    __device__ Feed(const SharedArgs& args, Shared& shared, T* k, T* v, T* q)
-        : a(args), side(IS_FEW ? args.few : args.many), sh(shared), ks(k), vs(v), qs(q) {}
+    __device__ Feed(const SharedArgs& args, const Plan& p, Shared& shared, T* k, T* v, T* q) : a(args), plan(p), sh(shared), ks(k), vs(v), qs(q) {}
 
     __device__ void next(Step& out) {                                     // (thread 0)
-        out.valid = sh.stretch.worker == (int)blockIdx.x;
+        out.valid = sh.stretch.steps != 0;
         if (!out.valid) return;
         out.of = sh.stretch;
         out.k0 = sh.stretch.k0 + at * KEYS;
         out.first = at == 0;
         out.last = at + 1 == sh.stretch.steps;
-        out.stretch = stretches; out.slot = slot;
+        out.stretch = stretches;
         if (++at < sh.stretch.steps) return;
         at = 0;
-        ++stretches;
-        sh.stretch = side.stretches[++slot];
+        stretch_of<!IS_FEW>(a, plan, piece, ++stretches, sh.stretch);
     }
     __device__ void find(int n) {                                         // where the keys of step n lie
         const Step& st = sh.steps[n % RECORDS];
@@ -387,17 +375,13 @@ struct Feed {
         }
         copies_commit();
     }
-    // First steps; false: nothing to do.  The launch of the many rows comes first and waits for the plan.  That of the few rows
-    // reads nothing that the many's wrote, and starts when all of its blocks have waited: it works beside it and waits when
-    // it is done, so that the merge behind it finds both done.
+    // first steps; false: nothing to do
     __device__ bool start() {
-        if (!IS_FEW) grid_dependency_wait();
-        grid_dependents_go();
-        const int first = side.first[blockIdx.x];
-        if (first < 0) { finish(); return false; }
+        piece = piece_of<!IS_FEW>(a, plan, blockIdx.x);
+        if (piece.from == piece.end) return false;
         if (threadIdx.x == 0) {
-            slot = first; stretches = at = 0;
-            sh.stretch = side.stretches[slot];
+            stretches = at = 0;
+            stretch_of<!IS_FEW>(a, plan, piece, 0, sh.stretch);
 #pragma unroll 1
             for (int n = 0; n <= STAGES; ++n) next(sh.steps[n]);
         }
@@ -409,9 +393,9 @@ struct Feed {
         for (int n = 0; n < STAGES - 1; ++n) fetch(n);
         return true;
     }
-    __device__ void finish() {
+    __device__ void finish() {                                            // (the shared memory may serve for something else)
         copies_wait<0>();
-        if (IS_FEW) grid_dependency_wait();
+        __syncthreads();
     }
     // step n has landed: on with the steps behind it
     __device__ void advance(int n) {
@@ -428,49 +412,58 @@ struct Feed {
 // Every warp is a worker of its own: one tile of 16 rows, steps of 16 keys, its own ring of STAGES steps in shared memory, and
 // no meeting of warps on the way.  What a step costs is its chain of dependent instructions, so what counts is how many warps
 // an SM has at it and how few instructions they take: four warps that shared a step of 32 keys took 442 instructions each,
-// and 62 us where these take XX (200 requests, 40 heads over 8 of 128, 32 to 512 keys of their own each).
+// and 62 us where these take 40 (200 requests, 40 heads over 8 of 128, 32 to 512 keys of their own each).
+template <int MOST_WARPS, int ROOM>
 struct FewShape {
     static constexpr int KEYS = MMA_FEW_KEYS, STAGES = 3;
     static constexpr int LD = HD + 8;                    // padded rows: ldmatrix without bank conflicts
     static constexpr bool Q_IN_REGS = HD <= 128;
     static constexpr int Q_SLOTS = Q_IN_REGS ? 2 : 3;
-    static constexpr size_t WORKER = ((size_t)STAGES * 2 * KEYS + (size_t)Q_SLOTS * FEW) * LD * sizeof(bf16);
-    static constexpr int FIT = (int)(226 * 1024 / WORKER);
-    static constexpr int WORKERS = FIT < 8 ? FIT : 8;
-    static constexpr int THREADS = 32 * WORKERS;
+    static constexpr int AT_ONCE = 8;                    // stretches that a worker works out at once
+    static constexpr size_t WORKER = ((size_t)STAGES * 2 * KEYS + (size_t)Q_SLOTS * FEW) * LD * sizeof(bf16) + FEW * 8 + AT_ONCE * sizeof(Stretch);
+    static constexpr int FIT = (int)(ROOM / WORKER);
+    static constexpr int WORKERS = FIT < MOST_WARPS ? FIT : MOST_WARPS;
     static constexpr size_t SMEM = WORKERS * WORKER;
 };
 
-__global__ void __launch_bounds__(FewShape::THREADS, 1)
-shared_few_kernel(const __grid_constant__ SharedArgs a) {
-    using S = FewShape;
+template <typename S>
+__device__ __forceinline__ void few_phase(const SharedArgs& a, const Plan& plan, unsigned char* smem, int workers) {
     constexpr int KEYS = S::KEYS, STAGES = S::STAGES, LD = S::LD, PIECES = HD / 8, ROUNDS = KEYS * PIECES / 32;
     static_assert(KEYS == FEW, "keys and queries are copied alike");
-    extern __shared__ __align__(16) unsigned char smem[];
+    if (threadIdx.x >= 32 * workers) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     bf16* ring = reinterpret_cast<bf16*>(smem + warp * S::WORKER);        // [stage][K, V][KEYS][LD]
     bf16* qs = ring + STAGES * 2 * KEYS * LD;                             // [slot][FEW][LD]
-    const int worker = blockIdx.x * S::WORKERS + warp;
-    grid_dependents_go();
-    int slot = a.few.first[worker];
-    if (slot < 0) { grid_dependency_wait(); return; }
-
-    // ---- the walk: the step that comes next, and its keys' pages, asked for a turn before its keys and values are; the
-    // stretch behind the one that is walked through is asked for with it
+    long long* row_at = reinterpret_cast<long long*>(qs + S::Q_SLOTS * FEW * LD);       // where the rows to copy begin
+    Stretch* stretches = reinterpret_cast<Stretch*>(row_at + FEW);
+    // the blocks that have the fewest pieces of many rows come first
+    const Piece piece = piece_of<0>(a, plan, (gridDim.x - 1 - blockIdx.x) * workers + warp);
+    if (piece.from == piece.end) return;
+    // (held in registers: a parameter is read from where it lies, again and again, otherwise)
+    const bf16 *kp = (const bf16*)a.k_pages, *vp = (const bf16*)a.v_pages, *qp = (const bf16*)a.q;
+    long long page_stride = a.page_stride;
+    int page_size = a.page_size, num_pages = a.num_pages, q_ld = a.q_ld, group = a.group, table_width = a.table_width, tokens = a.tokens;
+    const int* block_tables = a.block_tables;
+    asm volatile("" : "+l"(kp), "+l"(vp), "+l"(qp), "+l"(page_stride), "+l"(block_tables), "+r"(page_size), "+r"(num_pages), "+r"(q_ld), "+r"(group), "+r"(table_width), "+r"(tokens));
+    // ---- the walk: the step that comes next, and its keys' pages, asked for a turn before its keys and values are
     int k = -1, left = 0, k0 = 0;                         // stretch, steps left of it, the step's first key
     bool first = false, more = true;
-    Stretch at, ahead = a.few.stretches[slot];
+    Stretch at = {};
     int page = 0, inside = -1;                            // of key `lane % 16`: its page, and its place there (-1: no key)
     auto look_up = [&]() {
         inside = -1;
         if (!more) return;
         first = left == 0;
         if (first) {
-            at = ahead;
-            more = at.worker == worker;
-            if (!more) return;
-            ahead = a.few.stretches[slot + ++k + 1];
+            if (++k % S::AT_ONCE == 0) {
+                __syncwarp();
+                if (lane < S::AT_ONCE) stretch_of<0>(a, plan, piece, k + lane, stretches[lane]);
+                __syncwarp();
+            }
+            at = stretches[k % S::AT_ONCE];
             left = at.steps;
+            more = left > 0;
+            if (!more) return;
             k0 = at.k0;
         } else {
             k0 += KEYS;
@@ -478,9 +471,9 @@ shared_few_kernel(const __grid_constant__ SharedArgs a) {
         --left;
         const int key = k0 + (lane & 15);
         if (key < at.kend) {
-            const int block = key / a.page_size;
-            inside = key - block * a.page_size;
-            page = a.block_tables[(size_t)at.table * a.table_width + block];
+            const int block = key / page_size;
+            inside = key - block * page_size;
+            page = block_tables[(size_t)at.table * table_width + block];
         }
     };
     // what a step needs when it has landed: bits 0 .. 15 its keys, 16 .. 18 first, last and valid; rows and slot
@@ -488,41 +481,41 @@ shared_few_kernel(const __grid_constant__ SharedArgs a) {
     auto fetch = [&](int n) {
         Landing landing = {0u, 0, 0};
         if (more) {
-            const bool there = inside >= 0 && (unsigned)page < (unsigned)a.num_pages;
+            const bool there = inside >= 0 && (unsigned)page < (unsigned)num_pages;
             if (inside >= 0 && !there) atomicExch(a.error, ERR_PAGE);
             landing.bits = (__ballot_sync(0xffffffffu, there) & 0xffffu) | (first ? 1u << 16 : 0u) | (left == 0 ? 1u << 17 : 0u) | 1u << 18;
-            landing.rows = at.rows; landing.slot = slot + k;
-            const long long base = there ? (long long)page * a.page_stride + ((long long)at.kvh * a.page_size + inside) * HD : 0;
+            landing.rows = at.rows; landing.slot = at.slot;
+            const long long base = there ? (long long)page * page_stride + ((long long)at.kvh * page_size + inside) * HD : 0;
             bf16* kd = ring + (n % STAGES) * 2 * KEYS * LD;
-            const bf16* kp = (const bf16*)a.k_pages;
-            const bf16* vp = (const bf16*)a.v_pages;
-            long long from[ROUNDS];
-#pragma unroll
-            for (int i = 0; i < ROUNDS; ++i) from[i] = __shfl_sync(0xffffffffu, base, (i * 32 + lane) / PIECES);
+            __syncwarp();
+            if (lane < KEYS) row_at[lane] = base;
+            __syncwarp();
 #pragma unroll
             for (int i = 0; i < ROUNDS; ++i) {
                 const int e = i * 32 + lane, j = e / PIECES, c = (e - j * PIECES) * 8;
                 const bool ok = landing.bits >> j & 1;
-                copy16(kd + j * LD + c, kp + from[i] + c, ok);
-                copy16(kd + (KEYS + j) * LD + c, vp + from[i] + c, ok);
+                const long long from = row_at[j] + c;
+                copy16(kd + j * LD + c, kp + from, ok);
+                copy16(kd + (KEYS + j) * LD + c, vp + from, ok);
             }
             if (first) {
-                long long row_at = 0;                     // of row `lane`
+                long long query_at = 0;                   // of row `lane`
                 bool row_there = false;
                 if (lane < at.rows) {
-                    const int row = at.row0 + lane, further = row < a.group ? 0 : row / a.group;
+                    const int row = at.row0 + lane, further = row < group ? 0 : row / group;
                     const int token = at.token >= 0 ? at.token : a.order[at.place + further];
-                    row_there = (unsigned)token < (unsigned)a.tokens;
-                    if (row_there) row_at = (long long)token * a.q_ld + (at.kvh * a.group + row - further * a.group) * HD;
+                    row_there = (unsigned)token < (unsigned)tokens;
+                    if (row_there) query_at = (long long)token * q_ld + (at.kvh * group + row - further * group) * HD;
                 }
                 const unsigned rows = __ballot_sync(0xffffffffu, row_there);
                 bf16* qd = qs + (k % S::Q_SLOTS) * FEW * LD;
-#pragma unroll
-                for (int i = 0; i < ROUNDS; ++i) from[i] = __shfl_sync(0xffffffffu, row_at, (i * 32 + lane) / PIECES);
+                __syncwarp();
+                if (lane < FEW) row_at[lane] = query_at;
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < ROUNDS; ++i) {
                     const int e = i * 32 + lane, r = e / PIECES, c = (e - r * PIECES) * 8;
-                    copy16(qd + r * LD + c, (const bf16*)a.q + from[i] + c, rows >> r & 1);
+                    copy16(qd + r * LD + c, qp + row_at[r] + c, rows >> r & 1);
                 }
             }
         }
@@ -655,7 +648,6 @@ shared_few_kernel(const __grid_constant__ SharedArgs a) {
         now = next; next = behind;
     }
     copies_wait<0>();
-    grid_dependency_wait();                               // (beside the many's kernel: see Feed::start)
 }
 
 // ------------------------------------------------------------------------------------- bfloat16, many rows
@@ -667,16 +659,14 @@ struct ManyShape {
     static constexpr size_t SMEM = (size_t)STAGES * (2 * KEYS + ROWS) * LD * sizeof(bf16) + (sizeof(F::Shared) + 15) / 16 * 16;
 };
 
-__global__ void __launch_bounds__(THREADS)
-shared_many_kernel(const __grid_constant__ SharedArgs a) {
+__device__ __forceinline__ void many_phase(const SharedArgs& a, const Plan& plan, unsigned char* smem) {
     using S = ManyShape;
     constexpr int KEYS = S::KEYS, NT = KEYS / 8;
-    extern __shared__ __align__(16) unsigned char smem[];
     bf16* ks = reinterpret_cast<bf16*>(smem);
     bf16* vs = ks + (size_t)S::STAGES * KEYS * S::LD;
     bf16* qs = vs + (size_t)S::STAGES * KEYS * S::LD;
     S::F::Shared& sh = *reinterpret_cast<S::F::Shared*>(qs + (size_t)S::STAGES * S::ROWS * S::LD);
-    S::F feed(a, sh, ks, vs, qs);
+    S::F feed(a, plan, sh, ks, vs, qs);
     if (!feed.start()) return;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -763,7 +753,7 @@ shared_many_kernel(const __grid_constant__ SharedArgs a) {
         // ---- the stretch's triples
         l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 1); l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 2);
         l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 1); l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 2);
-        const size_t row = (size_t)a.many.row0 + (size_t)st.slot * S::ROWS;
+        const size_t row = (size_t)a.many.row0 + (size_t)st.of.slot * S::ROWS;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             const int r = half ? r_hi : r_lo;
@@ -798,11 +788,9 @@ struct F32Shape {
 };
 
 template <int WARPS_M, int WARPS_K, bool FEW_ROWS>
-__global__ void __launch_bounds__(THREADS)
-shared_f32_kernel(const __grid_constant__ SharedArgs a) {
+__device__ __forceinline__ void f32_phase(const SharedArgs& a, const Plan& plan, unsigned char* smem) {
     using S = F32Shape<WARPS_M, WARPS_K, FEW_ROWS>;
     constexpr int STAGES = S::STAGES, VEC = S::VEC, KEYS = S::KEYS;
-    extern __shared__ __align__(16) unsigned char smem[];
     float* ks = reinterpret_cast<float*>(smem);
     float* vs = ks + STAGES * KEYS * S::K_LD;
     float* qs = vs + STAGES * KEYS * HD;
@@ -810,7 +798,7 @@ shared_f32_kernel(const __grid_constant__ SharedArgs a) {
     float* row_max = ps + S::ROWS * S::P_LD;
     float* row_sum = row_max + WARPS_K * S::ROWS;
     typename S::F::Shared& sh = *reinterpret_cast<typename S::F::Shared*>(row_sum + WARPS_K * S::ROWS);
-    typename S::F feed(a, sh, ks, vs, qs);
+    typename S::F feed(a, plan, sh, ks, vs, qs);
     if (!feed.start()) return;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, wm = warp / WARPS_K, wk = warp % WARPS_K;
@@ -936,7 +924,7 @@ shared_f32_kernel(const __grid_constant__ SharedArgs a) {
                 for (int w = 0; w < WARPS_K; ++w) l[i] += row_sum[w * S::ROWS + r0 + i];
             }
         }
-        const size_t row = (size_t)feed.side.row0 + (size_t)st.slot * S::ROWS;
+        const size_t row = (S::IS_FEW ? 0 : (size_t)a.many.row0) + (size_t)st.of.slot * S::ROWS;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (r0 + i >= st.of.rows) continue;
@@ -989,18 +977,17 @@ constexpr int CONTROL_BYTES = 2048;
 static_assert(sizeof(Control) <= CONTROL_BYTES, "control block");
 constexpr size_t SMEM = CONTROL_BYTES + STREAMS * Q_BYTES + SLOTS * KV_BYTES;
 
-__global__ void __launch_bounds__(THREADS, 1)
-shared_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ SharedArgs a) {
-    extern __shared__ __align__(1024) unsigned char smem_all[];
+__device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtensorMap& v_map, const SharedArgs& a, const Plan& plan, unsigned char* smem_all) {
     Control& ctl = *reinterpret_cast<Control*>(smem_all);
     unsigned char* q_s = smem_all + CONTROL_BYTES;       // [stream][HALVES][128 rows][128 B]
     unsigned char* ring = q_s + STREAMS * Q_BYTES;       // [slot][HALVES][128 keys][128 B]
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const Piece piece = piece_of<1>(a, plan, blockIdx.x);
+    if (piece.from == piece.end) return;
     if ((smem_addr(smem_all) & 1023) != 0) {             // the swizzle goes by addresses
-        if (threadIdx.x == 0) atomicExch(a.error, ERR_TC_LAYOUT);
-        grid_dependency_wait();
+        if (tid == 0) atomicExch(a.error, ERR_TC_LAYOUT);
         return;
     }
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int s = 0; s < SLOTS; ++s) { mbar_init(&ctl.ring_full[s], 1); mbar_init(&ctl.ring_empty[s], 1); }
         for (int st = 0; st < STREAMS; ++st) {
@@ -1010,6 +997,8 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
         ctl.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    static_assert(STRETCHES == 32, "a lane each");
+    if (warp == 2) stretch_of<1>(a, plan, piece, lane, ctl.stretches[lane]);
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&ctl.tmem_slot)), "r"(TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -1018,15 +1007,7 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = ctl.tmem_slot;
-    grid_dependency_wait();
-    grid_dependents_go();
-    int slot = a.many.first[blockIdx.x];
-    auto read_stretches = [&]() {                         // those from `slot` on
-        static_assert(STRETCHES == 32, "a lane each");
-        if (warp == 2) ctl.stretches[lane] = a.many.stretches[min(slot + lane, a.many.line_room + a.many.workers)];
-    };
-    if (slot >= 0) read_stretches();
-    __syncthreads();
+    int done = 0;                                         // stretches of the rounds before
     auto give_up = [&](int code) { atomicExch(a.error, code); atomicExch(&ctl.abort_flag, 1); };
 
     // what the roles count on from stretch to stretch
@@ -1039,10 +1020,10 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
     const uint32_t s_addr = lane_base + COL_S + st_own * KEYS, o_addr = lane_base + COL_O + st_own * KEYS;
     const float sc = a.scale * LOG2E;
 
-    while (slot >= 0) {
+    for (;;) {
         for (int k = 0; k < STRETCHES && ok; ++k) {
             const Stretch sr = ctl.stretches[k];
-            if (sr.worker != (int)blockIdx.x) break;
+            if (sr.steps == 0) break;
             const int tiles = sr.steps, streams = sr.rows > BM ? 2 : 1;
             if (warp == 0) {
                 // -------------------------------------------------------------- producer: lane j has page j of a tile
@@ -1233,15 +1214,16 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
                 if (ok) {
                     // ---- the row's triple
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const size_t row = (size_t)a.many.row0 + (size_t)(slot + k) * ROWS + st_own * BM + r;
+                    const size_t row = (size_t)a.many.row0 + (size_t)sr.slot * ROWS + st_own * BM + r;
 #pragma unroll 1
                     for (int c = 0; c < HD; c += 32) {
                         float v[32];
                         tmem_ld32(o_addr + c, v);         // (all lanes take part)
-                        if (valid) {
+                        if (valid) {                      // (whole sectors: a warp's rows lie 4 * HD bytes apart)
 #pragma unroll
-                            for (int j = 0; j < 32; j += 4)
-                                *reinterpret_cast<float4*>(a.part_o + row * HD + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                            for (int j = 0; j < 32; j += 8)
+                                asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(a.part_o + row * HD + c + j), "f"(v[j]),
+                                             "f"(v[j + 1]), "f"(v[j + 2]), "f"(v[j + 3]), "f"(v[j + 4]), "f"(v[j + 5]), "f"(v[j + 6]), "f"(v[j + 7]) : "memory");
                         }
                     }
                     if (valid) *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m_run == -INFINITY ? m_run : m_run * a.scale, l_run);
@@ -1249,13 +1231,12 @@ shared_tc_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constan
                 }
             }
         }
-        // all roles are done with these stretches; there may be more where all of them were this block's
-        const bool all = __syncthreads_and(ctl.stretches[lane].worker == (int)blockIdx.x);
-        const bool aborted = ctl.abort_flag;
+        __syncthreads();                                  // all roles are done with these stretches
+        const bool more = ctl.stretches[STRETCHES - 1].steps != 0 && !ctl.abort_flag;
         __syncthreads();
-        if (aborted || !all) break;
-        slot += STRETCHES;
-        read_stretches();
+        if (!more) break;
+        done += STRETCHES;
+        if (warp == 2) stretch_of<1>(a, plan, piece, done + lane, ctl.stretches[lane]);
         __syncthreads();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1289,43 +1270,68 @@ static int pages_map(CUtensorMap& map, const void* pages, long long rows, int pa
 // place into a list in shared memory, each lane has the maxima and sums of one of the rows and of every (32 / ROWS)-th
 // triple, the weights go into shared memory, and the columns are summed four per lane, in the order of the triples.  SPLIT
 // warps have a share of a unit's triples each and join through shared memory, in order.
-constexpr int MERGE_WARPS = 4;
-constexpr long long MERGE_SPLIT_ROWS = 2048;
+template <int ROWS, int SPLIT>
+struct MergeShared {
+    static constexpr int WARPS = SPLIT > 1 ? SPLIT : 1;
+    int listed[32];                                       // of each warp: a turn's triples, their first rows
+    float weights[32][ROWS];
+    float4 joined[SPLIT > 1 ? ROWS : 1][SPLIT > 1 ? HD / 4 : 1];
+    float2 joined_ml[ROWS];
+};
 
-template <typename T, int ROWS, int SPLIT>
-__global__ void __launch_bounds__(32 * MERGE_WARPS)
-shared_merge_kernel(const __grid_constant__ SharedArgs a) {
-    constexpr int UNITS = MERGE_WARPS / SPLIT;                            // units of a block
+template <typename T, int ROWS, int SPLIT, int WARPS>
+__device__ __forceinline__ void merge_units(const SharedArgs& a, const Plan& plan, unsigned char* smem) {
     constexpr int CHUNKS = (HD / 4 + 31) / 32;
     constexpr int PARTS = 32 / ROWS, AHEAD = ROWS * CHUNKS >= 16 ? 1 : 16 / (ROWS * CHUNKS) < 8 ? 16 / (ROWS * CHUNKS) : 8;
+    constexpr int TEAMS = WARPS / SPLIT;                                  // units that a block works on at once
+    static_assert(sizeof(MergeShared<ROWS, SPLIT>) % 16 == 0 && sizeof(PlanSums) % 16 == 0, "what follows starts on 16 bytes");
     static_assert(FEW % ROWS == 0, "a unit lies in one tile");
-    __shared__ int listed[MERGE_WARPS][32];                               // a turn's triples: first row
-    __shared__ float weights[MERGE_WARPS][32][ROWS];
-    __shared__ float4 joined[SPLIT > 1 ? MERGE_WARPS : 1][ROWS][SPLIT > 1 ? HD / 4 : 1];
-    __shared__ float2 joined_ml[SPLIT > 1 ? MERGE_WARPS : 1][ROWS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SPLIT;
+    MergeShared<ROWS, SPLIT>* mine = reinterpret_cast<MergeShared<ROWS, SPLIT>*>(smem);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SPLIT, team = warp / SPLIT;
+    MergeShared<ROWS, SPLIT>& own = mine[warp];
+    if (team >= TEAMS) return;
     const int chunks = (a.group + ROWS - 1) / ROWS;                       // units of a token and kv head
-    const int unit = blockIdx.x * UNITS + warp / SPLIT, per_place = a.kv_heads * chunks;
+    const int per_place = a.kv_heads * chunks, units = a.places * per_place;
+    bool waited = false;
+    for (int unit = blockIdx.x * TEAMS + team; unit < units; unit += gridDim.x * TEAMS) {
     const int place = unit / per_place, in_place = unit - place * per_place, kvh = in_place / chunks, g0 = (in_place - kvh * chunks) * ROWS;
     const int rows = min(ROWS, a.group - g0);
-    grid_dependency_wait();
-    grid_dependents_go();
-    if (place >= a.places) return;                        // (all warps of a unit)
+    const int token = a.order[place];
+    int r = a.own_run[place], levels = 0, own_level = -1;
+    if (r >= a.run_count) r = -1;
     // ---- lane d: the d-th run around the token; its triples of row g0 are rows first_at, first_at + tile, ..
-    const int4* of_place = a.levels + (size_t)place * MAX_LEVELS;
-    const int4 head = of_place[0], level = of_place[lane];
-    const int levels = head.x, token = head.y;
-    if (token < 0) return;
-    int first_at = 0, count = 0, tile_rows = FEW;
-    const int4 run = make_int4(__shfl_down_sync(0xffffffffu, level.x, 1), __shfl_down_sync(0xffffffffu, level.y, 1), __shfl_down_sync(0xffffffffu, level.z, 1), 0);
-    if (lane < levels) {
-        const Side& side = run.y ? a.many : a.few;
-        tile_rows = side.tile;
-        const int part = g0 / tile_rows;                  // (0 but for groups that are larger than a tile)
-        const int2 line = side.lines[run.x + part * a.kv_heads + kvh];
-        count = line.y;
-        first_at = (int)side.row0 + line.x * tile_rows + run.z + g0 - part * tile_rows;
+    for (; r >= 0 && levels < MAX_LEVELS; ++levels) {
+        if (lane == levels) own_level = r;
+        const int parent = plan.runs[r].parent;
+        r = parent < r ? parent : -1;
     }
+    const bool there = (unsigned)token < (unsigned)a.tokens;
+    const int position = there ? a.positions[token] : -1;
+    if ((r >= 0 || !there) && lane == 0) atomicExch(a.error, ERR_RUNS);
+    int first_at = 0, count = 0, tile_rows = FEW;
+    if (own_level >= 0) {
+        const Run run = plan.runs[own_level];
+        if (run.count > 0 && place >= run.first && place < run.first + run.count) {
+            const int kind = plan.kind[own_level], many = kind & RUN_FEW ? 0 : 1;
+            const Side& side = many ? a.many : a.few;
+            tile_rows = side.tile;
+            const Tiling t = tiling(a, kind, tile_rows);
+            const int token_in = place - run.first, part = t.parts > 1 ? g0 / tile_rows : 0, tile = t.parts > 1 ? token_in * t.parts + part : token_in / t.tokens;
+            const int row = t.parts > 1 ? g0 - part * tile_rows : (token_in - tile * t.tokens) * a.group + g0;
+            const int line = tile * a.kv_heads + kvh, of_line = line_steps(run, side), from = plan.step0(many)[own_level] + line * of_line;
+            const int steps = many ? plan.many_piece : plan.few_piece, b0 = from / steps;
+            count = (from + of_line - 1) / steps - b0 + 1;
+            first_at = (int)side.row0 + (plan.line0(many)[own_level] + line + b0) * tile_rows + row;
+            // (a shared run ends in front of its tokens)
+            if (!(kind & RUN_INNERMOST) && run.end - 1 > position) atomicExch(a.error, ERR_RUNS);
+        }
+    }
+    if (!waited) {                                        // (all of the above is older than the kernel in front)
+        grid_dependency_wait();
+        grid_dependents_go();
+        waited = true;
+    }
+    if (!there) continue;                                 // (all warps of a unit)
     int upto = count;
 #pragma unroll
     for (int o = 1; o < MAX_LEVELS; o *= 2) {
@@ -1341,7 +1347,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs a) {
         for (int c = 0; c < CHUNKS; ++c) sum[g][c] = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = -INFINITY, denom = 0.f;                   // of row x
     const int x = lane % ROWS, part = lane / ROWS;
-    int* list = listed[warp];
+    int* list = own.listed;
     const int each = (triples + SPLIT - 1) / SPLIT, last = min(triples, (share + 1) * each);
     for (int t0 = share * each; t0 < last; t0 += 32) {
         const int have = min(32, last - t0);
@@ -1373,7 +1379,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs a) {
 #pragma unroll
         for (int i = 0; i < ROWS; ++i) {
             const float w = m[i] == -INFINITY ? 0.f : expf(m[i] - top_new);
-            weights[warp][part + PARTS * i][x] = w;
+            own.weights[part + PARTS * i][x] = w;
             sum_l += l[i] * w;
         }
 #pragma unroll
@@ -1408,7 +1414,7 @@ shared_merge_kernel(const __grid_constant__ SharedArgs a) {
 #pragma unroll
                 for (int g = 0; g < ROWS; ++g)
                     if (g < rows) {
-                        const float w = weights[warp][j0 + j][g];
+                        const float w = own.weights[j0 + j][g];
                         const bool counts = w != 0.f;     // (a stretch without a key may hold anything)
 #pragma unroll
                         for (int c = 0; c < CHUNKS; ++c) {
@@ -1422,23 +1428,24 @@ shared_merge_kernel(const __grid_constant__ SharedArgs a) {
     }
     // (lane g has row g's denominator)
     if constexpr (SPLIT > 1) {
-        static_assert(SPLIT == MERGE_WARPS, "a unit is a block");
 #pragma unroll
         for (int g = 0; g < ROWS; ++g)
 #pragma unroll
             for (int c = 0; c < CHUNKS; ++c)
-                if (HD / 4 % 32 == 0 || lane + 32 * c < HD / 4) joined[warp][g][lane + 32 * c] = sum[g][c];
-        if (lane < ROWS) joined_ml[warp][lane] = make_float2(top, denom);
-        __syncthreads();
-        if (warp > 0) return;
+                if (HD / 4 % 32 == 0 || lane + 32 * c < HD / 4) own.joined[g][lane + 32 * c] = sum[g][c];
+        if (lane < ROWS) own.joined_ml[lane] = make_float2(top, denom);
+        // (a unit's warps meet; behind the join again, since the next unit's sums go to the same place)
+        auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * SPLIT) : "memory"); };
+        meet();
+        const MergeShared<ROWS, SPLIT>* of = mine + team * SPLIT;
         float f[SPLIT];
         float top_all = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < SPLIT; ++w) top_all = fmaxf(top_all, joined_ml[w][x].x);
+        for (int w = 0; w < SPLIT; ++w) top_all = fmaxf(top_all, of[w].joined_ml[x].x);
         denom = 0.f;
 #pragma unroll
         for (int w = 0; w < SPLIT; ++w) {
-            const float2 ml = joined_ml[w][x];
+            const float2 ml = of[w].joined_ml[x];
             f[w] = ml.x == -INFINITY ? 0.f : expf(ml.x - top_all);
             denom += ml.y * f[w];
         }
@@ -1450,11 +1457,13 @@ shared_merge_kernel(const __grid_constant__ SharedArgs a) {
 #pragma unroll
                 for (int w = 0; w < SPLIT; ++w) {
                     const float fw = __shfl_sync(0xffffffffu, f[w], g);
-                    const float4 v = joined[w][g][HD / 4 % 32 == 0 ? lane + 32 * c : min(lane + 32 * c, HD / 4 - 1)];
+                    const float4 v = of[w].joined[g][HD / 4 % 32 == 0 ? lane + 32 * c : min(lane + 32 * c, HD / 4 - 1)];
                     if (fw != 0.f) { all.x = fmaf(fw, v.x, all.x); all.y = fmaf(fw, v.y, all.y); all.z = fmaf(fw, v.z, all.z); all.w = fmaf(fw, v.w, all.w); }
                 }
                 sum[g][c] = all;
             }
+        meet();
+        if (share > 0) continue;
     }
     const float inverse = denom > 0.f ? 1.0f / denom : denom == denom ? 0.f : denom;     // no key: zeros; NaN stays NaN
 #pragma unroll
@@ -1471,25 +1480,85 @@ shared_merge_kernel(const __grid_constant__ SharedArgs a) {
             }
         }
     }
+    }
 }
+
+// Few rows in all: a row to a unit and four warps on it, since what such a call waits for is one warp's chain of loads.  More:
+// what counts are instructions, and a warp takes several heads of a kv head together.
+constexpr int MERGE_WARPS = 4;
+template <typename T, int ROWS, int SPLIT>
+__global__ void __launch_bounds__(32 * MERGE_WARPS)
+shared_merge_kernel(const __grid_constant__ SharedArgs a) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    MergeShared<ROWS, SPLIT>* shared = reinterpret_cast<MergeShared<ROWS, SPLIT>*>(smem);
+    PlanSums& sums = *reinterpret_cast<PlanSums*>(shared + MERGE_WARPS);
+    Plan plan;
+    const bool fits = make_plan<32 * MERGE_WARPS>(a, reinterpret_cast<unsigned char*>(&sums + 1), sums, plan);
+    if (fits) merge_units<T, ROWS, SPLIT, MERGE_WARPS>(a, plan, smem);
+    grid_dependency_wait();
+    grid_dependents_go();
+}
+template <int ROWS, int SPLIT> constexpr size_t merge_smem() { return MERGE_WARPS * sizeof(MergeShared<ROWS, SPLIT>) + sizeof(PlanSums); }
 
 using F32Few = F32Shape<2, 2, true>;
-using F32Many = F32Shape<4, 1, false>;
+using F32Many = F32Shape<HD <= 128 ? 4 : 2, HD <= 128 ? 1 : 2, false>;
 static_assert(F32Few::ROWS == FEW, "tiles of few rows");
 
-// blocks of `kernel` that the current device runs at once
-template <typename K>
-static int blocks_at_once(K kernel, int threads, size_t smem, int& blocks) {
-    int device = 0, sms = 0, per_sm = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem);
-    blocks = sms * per_sm;
-    return e != cudaSuccess ? (int)e : blocks > 0 ? 0 : (int)ERR_UNSUPPORTED;
+// ----------------------------------------------------------------------------------------- the first launch
+enum { ON_F32, ON_MMA, ON_TC };
+constexpr size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
+constexpr size_t MOST_SMEM = 227 * 1024;
+// WORKER_SMEM: shared memory of a worker of few rows where a block has several, 0 where it is one
+template <int FORM> struct Form;
+template <> struct Form<ON_F32> {
+    static constexpr int THREADS = 128, FEW_WORKERS = 1, FEW_KEYS = F32Few::KEYS, MANY_TILE = F32Many::ROWS, MANY_KEYS = F32Many::KEYS;
+    static constexpr size_t SMEM = most_of(F32Few::SMEM, F32Many::SMEM), FEW_AT = 0, WORKER_SMEM = 0;
+};
+template <> struct Form<ON_MMA> {
+    using Few = FewShape<4, 190 * 1024>;
+    static constexpr int THREADS = 128, FEW_WORKERS = Few::WORKERS, FEW_KEYS = Few::KEYS, MANY_TILE = ManyShape::ROWS, MANY_KEYS = ManyShape::KEYS;
+    static constexpr size_t SMEM = most_of(Few::SMEM, ManyShape::SMEM), FEW_AT = 0, WORKER_SMEM = 0;
+};
+#ifdef FSIE_SHARED_TC
+template <> struct Form<ON_TC> {
+    using Few = FewShape<tc::THREADS / 32, (int)MOST_SMEM - tc::CONTROL_BYTES>;
+    static constexpr int THREADS = tc::THREADS, FEW_WORKERS = Few::WORKERS, FEW_KEYS = Few::KEYS, MANY_TILE = tc::ROWS, MANY_KEYS = tc::KEYS;
+    static constexpr size_t SMEM = tc::SMEM, FEW_AT = tc::CONTROL_BYTES, WORKER_SMEM = Few::WORKER;
+};
+#endif
+template <int FORM> constexpr size_t plan_at(int few_workers) {
+    return (most_of(Form<FORM>::SMEM, Form<FORM>::FEW_AT + few_workers * Form<FORM>::WORKER_SMEM) + 15) / 16 * 16;
 }
 
-struct Shape { int few_blocks, few_workers, few_keys, many_blocks, many_tile, many_keys, on_tcgen05; };      // (a worker: a block, or a warp of one)
+template <int FORM>
+__global__ void __launch_bounds__(Form<FORM>::THREADS, 1)
+shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const __grid_constant__ SharedArgs a,
+                        int few_workers, int plan_offset) {
+    extern __shared__ __align__(1024) unsigned char smem[];
+    if (!a.early) grid_dependency_wait();
+    PlanSums& sums = *reinterpret_cast<PlanSums*>(smem + plan_offset);
+    Plan plan;
+    const bool fits = make_plan<Form<FORM>::THREADS>(a, smem + plan_offset + sizeof(PlanSums), sums, plan);
+    if (a.early) grid_dependency_wait();
+    grid_dependents_go();
+    if (!fits) return;
+    if constexpr (FORM == ON_F32) {
+        f32_phase<HD <= 128 ? 4 : 2, HD <= 128 ? 1 : 2, false>(a, plan, smem);
+        f32_phase<2, 2, true>(a, plan, smem);
+    } else if constexpr (FORM == ON_MMA) {
+        many_phase(a, plan, smem);
+        few_phase<typename Form<FORM>::Few>(a, plan, smem, few_workers);
+    }
+#ifdef FSIE_SHARED_TC
+    else {
+        tc::tc_phase(k_map, v_map, a, plan, smem);
+        __syncthreads();
+        few_phase<typename Form<FORM>::Few>(a, plan, smem + tc::CONTROL_BYTES, few_workers);
+    }
+#endif
+}
+
+struct Shape { int blocks, few_workers, few_keys, many_tile, many_keys; };       // (few_workers: of a block)
 constexpr int MAX_DEVICES = 64;
 
 static bool tcgen05_takes(int page_size, long long page_stride) {
@@ -1500,64 +1569,75 @@ static bool tcgen05_takes(int page_size, long long page_stride) {
 #endif
 }
 
-// How the launches of a storage type look on the current device.
-static int shape_of(int dtype, bool on_tcgen05, Shape& shape) {
-    static Shape known[3][MAX_DEVICES] = {};             // per process; the same whoever writes it
-    int device = 0;
-    const cudaError_t e = cudaGetDevice(&device);
+// How a form's launch looks on the current device: as many blocks as run at once beside plans of middling size.
+template <int FORM>
+static int shape_of(Shape& shape) {
+    static Shape known[MAX_DEVICES] = {};                // per process; the same whoever writes it
+    using F = Form<FORM>;
+    int device = 0, sms = 0, per_sm = 0;
+    cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
     if (device < 0 || device >= MAX_DEVICES) return ERR_UNSUPPORTED;
-    Shape& have = known[dtype == DTYPE_F32 ? 0 : on_tcgen05 ? 2 : 1][device];
-    if (have.many_blocks == 0) {
-        Shape found = {};
-        int rc;
-        if (dtype == DTYPE_F32) {
-            rc = blocks_at_once(shared_f32_kernel<2, 2, true>, THREADS, F32Few::SMEM, found.few_blocks);
-            if (rc == 0) rc = blocks_at_once(shared_f32_kernel<4, 1, false>, THREADS, F32Many::SMEM, found.many_blocks);
-            found.few_workers = found.few_blocks; found.few_keys = F32Few::KEYS;
-            found.many_tile = F32Many::ROWS; found.many_keys = F32Many::KEYS;
-        } else {
-            rc = blocks_at_once(shared_few_kernel, FewShape::THREADS, FewShape::SMEM, found.few_blocks);
-            found.few_workers = found.few_blocks * FewShape::WORKERS; found.few_keys = FewShape::KEYS;
-#ifdef FSIE_SHARED_TC
-            if (rc == 0 && on_tcgen05) {
-                rc = blocks_at_once(tc::shared_tc_kernel, tc::THREADS, tc::SMEM, found.many_blocks);
-                found.many_tile = tc::ROWS; found.many_keys = tc::KEYS; found.on_tcgen05 = 1;
-            }
-#endif
-            if (rc == 0 && !found.on_tcgen05) {
-                rc = blocks_at_once(shared_many_kernel, THREADS, ManyShape::SMEM, found.many_blocks);
-                found.many_tile = ManyShape::ROWS; found.many_keys = ManyShape::KEYS;
-            }
-        }
-        if (rc != 0) return rc;
-        have = found;
+    if (known[device].blocks == 0) {
+        e = cudaFuncSetAttribute(shared_attention_kernel<FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_SMEM);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+        if (e == cudaSuccess)
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, shared_attention_kernel<FORM>, F::THREADS,
+                                                              most_of(F::SMEM, F::FEW_AT + F::FEW_WORKERS * F::WORKER_SMEM) + plan_bytes(100));
+        if (e != cudaSuccess) return (int)e;
+        if (sms * per_sm <= 0) return ERR_UNSUPPORTED;
+        known[device] = {sms * per_sm, F::FEW_WORKERS, F::FEW_KEYS, F::MANY_TILE, F::MANY_KEYS};
     }
-    shape = have;
+    shape = known[device];
     return 0;
+}
+static int shape_of(int dtype, bool on_tcgen05, Shape& shape) {
+    if (dtype == DTYPE_F32) return shape_of<ON_F32>(shape);
+#ifdef FSIE_SHARED_TC
+    if (on_tcgen05) return shape_of<ON_TC>(shape);
+#endif
+    return shape_of<ON_MMA>(shape);
+}
+
+template <int FORM>
+static int launch(const Shape& shape, const CUtensorMap& k_map, const CUtensorMap& v_map, SharedArgs& a, cudaStream_t stream) {
+    // a large plan takes the place of workers of few rows
+    const size_t plan = sizeof(PlanSums) + plan_bytes(a.run_count);
+    int workers = shape.few_workers;
+    while (Form<FORM>::WORKER_SMEM && workers > 1 && plan_at<FORM>(workers) + plan > MOST_SMEM) --workers;
+    const size_t at = plan_at<FORM>(workers);
+    if (at + plan > MOST_SMEM) return ERR_UNSUPPORTED;
+    a.few.workers = shape.blocks * workers;
+    return launch_dependent(shared_attention_kernel<FORM>, dim3(shape.blocks), dim3(Form<FORM>::THREADS), at + plan, stream, k_map, v_map, a, workers, (int)at);
+}
+
+// Few rows in all: a row to a unit and four warps on it, since what such a call waits for is one warp's chain of loads.  More:
+// what counts are instructions, and a warp takes several heads of a kv head together.  One block per multiprocessor finds
+// room beside the first launch's.
+template <typename T, int ROWS, int SPLIT>
+static int launch_merge_as(const SharedArgs& a, int blocks, cudaStream_t stream) {
+    const size_t smem = merge_smem<ROWS, SPLIT>() + plan_bytes(a.run_count);
+    if (smem > 48 * 1024) return ERR_UNSUPPORTED;
+    const long long units = (long long)a.places * a.kv_heads * ((a.group + ROWS - 1) / ROWS), teams = MERGE_WARPS / SPLIT;
+    return launch_dependent(shared_merge_kernel<T, ROWS, SPLIT>, dim3((unsigned)min((units + teams - 1) / teams, (long long)blocks)), dim3(32 * MERGE_WARPS),
+                            smem, stream, a);
+}
+template <typename T>
+static int launch_merge(const SharedArgs& a, int blocks, cudaStream_t stream) {
+    const long long rows = (long long)a.places * a.heads;
+    if (rows <= 2 * blocks) return launch_merge_as<T, 1, 4>(a, 2 * blocks, stream);
+    if (rows <= 16 * blocks) return launch_merge_as<T, 2, 1>(a, 2 * blocks, stream);
+    return launch_merge_as<T, 8, 1>(a, 2 * blocks, stream);
 }
 
 // Where everything lies in the room, for `lines` lines of many rows; returns the bytes.
 static long long lay_out(const Shape& shape, long long places, long long runs, int kv_heads, long long lines, unsigned char* room, SharedArgs& a) {
-    long long at = 0;
-    auto take = [&](long long bytes) { unsigned char* here = room + at; at += (bytes + 15) / 16 * 16; return here; };
-    Side few = {}, many = {};
-    few.workers = shape.few_workers; few.line_room = (int)((places + runs) * kv_heads); few.tile = FEW; few.keys = shape.few_keys;
-    few.align = 1; few.least = FEW_LEAST;
-    many.workers = shape.many_blocks; many.line_room = (int)lines; many.tile = shape.many_tile; many.keys = shape.many_keys;
-    many.align = 1; many.least = MANY_LEAST;
-    for (Side* side : {&few, &many}) {
-        side->first = (int*)take(4ll * side->workers);
-        side->lines = (int2*)take(8ll * side->line_room);
-        side->stretches = (Stretch*)take((long long)sizeof(Stretch) * (side->line_room + side->workers + 1));
-    }
-    const long long few_rows = (long long)(few.line_room + few.workers) * few.tile, many_rows = (long long)(many.line_room + many.workers) * many.tile;
-    many.row0 = few_rows;
-    a.few = few; a.many = many;
-    a.levels = (int4*)take(16ll * MAX_LEVELS * places);
-    a.part_ml = (float*)take(8 * (few_rows + many_rows));
-    a.part_o = (float*)take(4ll * HD * (few_rows + many_rows));
-    return few_rows + many_rows > 0x7fffffffLL ? -1 : at;
+    a.few = {shape.blocks * shape.few_workers, (int)((places + runs) * kv_heads), FEW, shape.few_keys, 1, FEW_LEAST, 0};
+    const long long few_rows = (long long)(a.few.line_room + a.few.workers) * FEW, many_rows = (lines + shape.blocks) * shape.many_tile;
+    a.many = {shape.blocks, (int)lines, shape.many_tile, shape.many_keys, 1, MANY_LEAST, few_rows};
+    a.part_o = (float*)room;                             // (stores of 32 bytes: it starts on 128)
+    a.part_ml = a.part_o + (few_rows + many_rows) * HD;
+    return few_rows + many_rows > 0x7fffffffLL ? -1 : (few_rows + many_rows) * (HD + 2) * 4 + 128;
 }
 
 // Lines of many rows: the tiles of the runs around a token are at most `levels` deep, a run has one begun tile; with a group
@@ -1566,16 +1646,6 @@ static long long many_lines(const Shape& shape, long long places, long long runs
     const long long group = heads / kv_heads, most = shape.many_tile;
     const long long of_all = group > most ? places * ((group + most - 1) / most) : (places + most / group - 1) / (most / group);
     return (levels * of_all + runs + (group > FEW ? places * ((group + most - 1) / most) : 0)) * kv_heads;
-}
-
-template <typename T>
-static int launch_merge(const SharedArgs& a, cudaStream_t stream) {
-    const long long rows = (long long)a.places * a.heads;
-    if (rows <= MERGE_SPLIT_ROWS)
-        return launch_dependent(shared_merge_kernel<T, 1, MERGE_WARPS>, dim3((unsigned)rows), dim3(32 * MERGE_WARPS), 0, stream, a);
-    const long long units = (long long)a.places * a.kv_heads * ((a.group + 7) / 8);
-    return launch_dependent(shared_merge_kernel<T, 8, 1>, dim3((unsigned)((units + MERGE_WARPS - 1) / MERGE_WARPS)),
-                            dim3(32 * MERGE_WARPS), 0, stream, a);
 }
 
 }  // namespace fsie
@@ -1628,42 +1698,37 @@ int fsie_shared_attention(const void* q, int q_ld, const void* k_pages, const vo
     Shape shape;
     int rc = shape_of(dtype, on_tcgen05, shape);
     if (rc != 0) return rc;
-    // as many lines of many rows as the room has place for
+    // as many lines of many rows as the room has place for (its last 128 bytes are for a start on 128)
+    room = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(room) + 127) & ~uintptr_t(127));
     SharedArgs a;
-    const long long least = lay_out(shape, places, run_count, kv_heads, many_lines(shape, places, run_count, heads, kv_heads, 0), (unsigned char*)room, a);
-    if (least < 0) return ERR_UNSUPPORTED;
-    if (least > room_bytes) return ERR_BAD_ARGUMENT;
-    const long long a_line = (long long)shape.many_tile * (HD + 2) * 4 + 8 + (long long)sizeof(Stretch);
-    long long lines = min(a.many.line_room + (room_bytes - least) / a_line + 1, 0x7fffffffLL / 2 / shape.many_tile);
-    long long bytes = 0;
-    while ((bytes = lay_out(shape, places, run_count, kv_heads, lines, (unsigned char*)room, a)) > room_bytes) --lines;
-    if (bytes < 0) return ERR_UNSUPPORTED;
+    const long long at_least = many_lines(shape, places, run_count, heads, kv_heads, 0);
+    const long long needed = lay_out(shape, places, run_count, kv_heads, at_least, (unsigned char*)room, a);
+    if (needed < 0) return ERR_UNSUPPORTED;
+    if (needed > room_bytes) return ERR_BAD_ARGUMENT;
+    const long long of_line = (long long)shape.many_tile * (HD + 2) * 4;
+    const long long lines = min(at_least + (room_bytes - needed) / of_line, 0x7fffffffLL / shape.many_tile - shape.blocks - (a.many.row0 + shape.many_tile) / shape.many_tile);
+    if (lay_out(shape, places, run_count, kv_heads, lines, (unsigned char*)room, a) < 0) return ERR_UNSUPPORTED;
     a.many.align = on_tcgen05 ? page_size : 1;
     a.q = q; a.q_ld = q_ld; a.k_pages = k_pages; a.v_pages = v_pages; a.page_stride = page_stride; a.page_size = page_size;
     a.num_pages = num_pages; a.block_tables = block_tables; a.table_rows = table_rows; a.table_width = table_width;
     a.positions = positions; a.tokens = tokens; a.order = order; a.places = places; a.runs = runs; a.run_count = run_count;
     a.own_run = own_run; a.out = out; a.out_ld = out_ld; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
     a.scale = scale; a.early = early; a.error = error;
-    rc = launch_dependent(shared_plan_kernel, dim3(PLAN_BLOCKS), dim3(PLAN_THREADS), 0, stream, a);
-    if (rc != 0) return rc;
-    const dim3 few_grid(shape.few_blocks), many_grid(shape.many_blocks);
+    CUtensorMap k_map = {}, v_map = {};
     if (dtype == DTYPE_F32) {
-        rc = launch_dependent(shared_f32_kernel<4, 1, false>, many_grid, dim3(THREADS), F32Many::SMEM, stream, a);
-        if (rc == 0) rc = launch_dependent(shared_f32_kernel<2, 2, true>, few_grid, dim3(THREADS), F32Few::SMEM, stream, a);
-    } else {
-#ifdef FSIE_SHARED_TC
-        if (on_tcgen05) {
-            CUtensorMap k_map, v_map;
-            rc = tc::pages_map(k_map, k_pages, page_rows, page_size);
-            if (rc == 0) rc = tc::pages_map(v_map, v_pages, page_rows, page_size);
-            if (rc == 0) rc = launch_dependent(tc::shared_tc_kernel, many_grid, dim3(tc::THREADS), tc::SMEM, stream, k_map, v_map, a);
-        } else
-#endif
-            rc = launch_dependent(shared_many_kernel, many_grid, dim3(THREADS), ManyShape::SMEM, stream, a);
-        if (rc == 0) rc = launch_dependent(shared_few_kernel, few_grid, dim3(FewShape::THREADS), FewShape::SMEM, stream, a);
+        rc = launch<ON_F32>(shape, k_map, v_map, a, stream);
+        return rc != 0 ? rc : launch_merge<float>(a, shape.blocks, stream);
     }
-    if (rc != 0) return rc;
-    return dtype == DTYPE_F32 ? launch_merge<float>(a, stream) : launch_merge<bf16>(a, stream);
+#ifdef FSIE_SHARED_TC
+    if (on_tcgen05) {
+        rc = tc::pages_map(k_map, k_pages, page_rows, page_size);
+        if (rc == 0) rc = tc::pages_map(v_map, v_pages, page_rows, page_size);
+        if (rc == 0) rc = launch<ON_TC>(shape, k_map, v_map, a, stream);
+        return rc != 0 ? rc : launch_merge<bf16>(a, shape.blocks, stream);
+    }
+#endif
+    rc = launch<ON_MMA>(shape, k_map, v_map, a, stream);
+    return rc != 0 ? rc : launch_merge<bf16>(a, shape.blocks, stream);
 }
 
 }  // extern "C"

@@ -2525,7 +2525,7 @@ def copy_blocks(buffers, moves: torch.Tensor, error: torch.Tensor) -> None:
 
 # ----------------------------------------------------- attention over pages that requests share
 _attn_shared: Dict[int, object] = {}
-SHARED_ATTENTION_MAX_RUNS = 1024
+SHARED_ATTENTION_MAX_RUNS = 768
 
 
 def attn_shared(head_dim: int):
