@@ -27,39 +27,43 @@ class SharedRuns:
 
 
 def find_shared_runs(tables: np.ndarray, page_size: int, q_start: np.ndarray, q_len: np.ndarray, pos0: np.ndarray,
-                     least_saved: int = 64) -> SharedRuns:
+                     least_saved: int = 64, most_shared: int = 1 << 30, most_levels: int = 31) -> SharedRuns:
     """tables int32 [requests, width] (page ids, below 0 where there is none), and per request where its tokens start in the
-    step, how many they are and the position of the first.  Only full pages in front of that position count as shared, and
-    only where sharing them saves reading `least_saved` keys."""
+    step, how many they are and the position of the first.  Only full pages in front of that position count as shared, only
+    where sharing them saves reading `least_saved` keys, in at most `most_shared` runs and `most_levels` around a token."""
     full = np.asarray(pos0, dtype=np.int64) // page_size
     shared: List[Tuple[int, int, int, int, int, int]] = []       # runs, places counted in requests
     items: List[np.ndarray] = []
     begins: List[np.ndarray] = []
     parents: List[np.ndarray] = []
     placed = levels = saved = 0
-
-    def leave(members: np.ndarray, begin: int, parent: int) -> None:
-        nonlocal placed
-        items.append(members)
-        begins.append(np.full(len(members), begin * page_size, dtype=np.int64))
-        parents.append(np.full(len(members), parent, dtype=np.int64))
-        placed += len(members)
-
-    def visit(members: np.ndarray, column: int, begin: int, parent: int, depth: int) -> None:
-        """`members` (two at least) hold the same pages in front of `column`; those from `begin` on are in no run yet."""
-        nonlocal levels, saved
+    everyone = np.arange(len(q_len))
+    # Still to do, the next one last: requests that hold the same pages in front of `column` (those from `begin` on are in no
+    # run yet), the run around them and how many lie around each other there.  column -1: they are done and take their places.
+    todo: List[Tuple[np.ndarray, int, int, int, int]] = []
+    if len(everyone):
+        todo.append((everyone, 0 if len(everyone) > 1 else -1, 0, -1, 0))
+    while todo:
+        members, column, begin, parent, depth = todo.pop()
+        if column < 0:
+            items.append(members)
+            begins.append(np.full(len(members), begin * page_size, dtype=np.int64))
+            parents.append(np.full(len(members), parent, dtype=np.int64))
+            placed += len(members)
+            continue
         upto = int(full[members].min())
         if upto > column:
             pages = tables[members, column:upto]
             same = (pages == pages[0]).all(axis=0) & (pages[0] >= 0)
             column = upto if same.all() else column + int(np.argmin(same))
         keys = (column - begin) * page_size
-        if keys * (len(members) - 1) >= max(least_saved, 1):
+        if keys * (len(members) - 1) >= max(least_saved, 1) and len(shared) < most_shared and depth < most_levels:
             shared.append((placed, len(members), begin * page_size, column * page_size, int(members[0]), parent))
             begin, parent, depth = column, len(shared) - 1, depth + 1
             levels = max(levels, depth)
             saved += keys * (len(members) - 1)
         # those that go on with the same page stay together
+        parts = []
         going = members[full[members] > column]
         if len(going) > 1:
             page = tables[going, column]
@@ -67,18 +71,11 @@ def find_shared_runs(tables: np.ndarray, page_size: int, q_start: np.ndarray, q_
             values, which, counts = np.unique(tables[going, column], return_inverse=True, return_counts=True)
             together = np.nonzero(counts > 1)[0]
             if len(together):
-                apart = np.setdiff1d(members, going[counts[which] > 1], assume_unique=True)
-                for value in together:
-                    visit(going[which == value], column, begin, parent, depth)
-                members = apart
+                parts = [going[which == value] for value in together]
+                members = np.setdiff1d(members, going[counts[which] > 1], assume_unique=True)
         if len(members):
-            leave(members, begin, parent)
-
-    everyone = np.arange(len(q_len))
-    if len(everyone) > 1:
-        visit(everyone, 0, 0, -1, 0)
-    elif len(everyone):
-        leave(everyone, 0, -1)
+            todo.append((members, -1, begin, parent, depth))
+        todo += [(part, column, begin, parent, depth) for part in reversed(parts)]
     q_start, q_len = np.asarray(q_start, dtype=np.int64), np.asarray(q_len, dtype=np.int64)
     member = np.concatenate(items) if items else everyone
     lengths = q_len[member]

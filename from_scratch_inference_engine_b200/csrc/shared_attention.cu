@@ -48,7 +48,7 @@ constexpr int MMA_FEW_KEYS = 16, MMA_MANY_KEYS = HD <= 128 ? 64 : 32, F32_KEYS =
 constexpr int MAX_RUNS = 768;
 constexpr int MAX_LEVELS = 32;           // runs that lie around each other, the innermost among them
 constexpr int RUN_INTS = 6;
-constexpr int LINE_PIECES = 32;          // a line is cut into no more pieces than this: what joins them reads them all
+constexpr int LINE_PIECES = 128;         // a line is cut into no more pieces than this: what joins them reads them all
 constexpr int FEW_LEAST = 2, MANY_LEAST = 1;                              // steps of a piece, at least
 enum { ERR_PAGE = 3, ERR_RUNS = 7, ERR_ROOM = 8 };
 
@@ -1640,12 +1640,12 @@ static long long lay_out(const Shape& shape, long long places, long long runs, i
     return few_rows + many_rows > 0x7fffffffLL ? -1 : (few_rows + many_rows) * (HD + 2) * 4 + 128;
 }
 
-// Lines of many rows: the tiles of the runs around a token are at most `levels` deep, a run has one begun tile; with a group
-// of more than few rows a token's own keys are among them.
-static long long many_lines(const Shape& shape, long long places, long long runs, int heads, int kv_heads, int levels) {
+// Lines of many rows: the tiles of the runs around a token are at most `levels` deep, a shared run has one begun tile; with a
+// group of more than few rows a token's own keys are among them.
+static long long many_lines(const Shape& shape, long long places, long long shared, int heads, int kv_heads, int levels) {
     const long long group = heads / kv_heads, most = shape.many_tile;
     const long long of_all = group > most ? places * ((group + most - 1) / most) : (places + most / group - 1) / (most / group);
-    return (levels * of_all + runs + (group > FEW ? places * ((group + most - 1) / most) : 0)) * kv_heads;
+    return (levels * of_all + shared + (group > FEW ? places * ((group + most - 1) / most) : 0)) * kv_heads;
 }
 
 }  // namespace fsie
@@ -1657,9 +1657,10 @@ extern "C" {
 int fsie_shared_attention_head_dim() { return HD; }
 int fsie_shared_attention_max_runs() { return MAX_RUNS; }
 
-// Bytes of room for `places` tokens in `runs` runs that are at most `levels` deep around a token; negative: an error.
-long long fsie_shared_attention_room(int places, int runs, int levels, int heads, int kv_heads, int dtype) {
-    if (places < 0 || runs < 0 || runs > MAX_RUNS || levels < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads ||
+// Bytes of room for `places` tokens in `runs` runs, `shared` of which are no token's innermost and lie at most `levels` deep
+// around a token; negative: an error.
+long long fsie_shared_attention_room(int places, int runs, int shared, int levels, int heads, int kv_heads, int dtype) {
+    if (places < 0 || runs < 0 || runs > MAX_RUNS || shared < 0 || shared > runs || levels < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads ||
         (dtype != DTYPE_F32 && dtype != DTYPE_BF16))
         return ERR_BAD_ARGUMENT;
     long long most = 0;
@@ -1669,7 +1670,7 @@ long long fsie_shared_attention_room(int places, int runs, int levels, int heads
         const int rc = shape_of(dtype, on_tcgen05, shape);
         if (rc != 0) return rc > 0 ? -1000 - rc : rc;
         SharedArgs a;
-        const long long bytes = lay_out(shape, places, runs, kv_heads, many_lines(shape, places, runs, heads, kv_heads, levels), nullptr, a);
+        const long long bytes = lay_out(shape, places, runs, kv_heads, many_lines(shape, places, shared, heads, kv_heads, levels), nullptr, a);
         if (bytes < 0) return ERR_UNSUPPORTED;
         most = max(most, bytes);
     }
@@ -1701,12 +1702,11 @@ int fsie_shared_attention(const void* q, int q_ld, const void* k_pages, const vo
     // as many lines of many rows as the room has place for (its last 128 bytes are for a start on 128)
     room = reinterpret_cast<void*>((reinterpret_cast<uintptr_t>(room) + 127) & ~uintptr_t(127));
     SharedArgs a;
-    const long long at_least = many_lines(shape, places, run_count, heads, kv_heads, 0);
-    const long long needed = lay_out(shape, places, run_count, kv_heads, at_least, (unsigned char*)room, a);
+    const long long needed = lay_out(shape, places, run_count, kv_heads, 0, (unsigned char*)room, a);
     if (needed < 0) return ERR_UNSUPPORTED;
     if (needed > room_bytes) return ERR_BAD_ARGUMENT;
     const long long of_line = (long long)shape.many_tile * (HD + 2) * 4;
-    const long long lines = min(at_least + (room_bytes - needed) / of_line, 0x7fffffffLL / shape.many_tile - shape.blocks - (a.many.row0 + shape.many_tile) / shape.many_tile);
+    const long long lines = min((room_bytes - needed) / of_line, 0x7fffffffLL / shape.many_tile - shape.blocks - (a.many.row0 + shape.many_tile) / shape.many_tile);
     if (lay_out(shape, places, run_count, kv_heads, lines, (unsigned char*)room, a) < 0) return ERR_UNSUPPORTED;
     a.many.align = on_tcgen05 ? page_size : 1;
     a.q = q; a.q_ld = q_ld; a.k_pages = k_pages; a.v_pages = v_pages; a.page_stride = page_stride; a.page_size = page_size;

@@ -24,6 +24,18 @@ class GroupStep:
 
 
 @dataclass
+class SharedLists:
+    """The tokens of a group's requests of one token each, their keys cut into runs (see `ops.shared_attention`).  `shared` and
+    `levels`: at most so many runs are shared and lie around a token, whatever a captured graph is replayed with."""
+
+    order: torch.Tensor             # int32 [places]
+    own_run: torch.Tensor           # int32 [places]
+    runs: torch.Tensor              # int32 [runs, 6]
+    shared: int
+    levels: int
+
+
+@dataclass
 class Tiles:
     item: torch.Tensor              # int32 [count]
     row0: torch.Tensor              # int32 [count]
@@ -82,11 +94,14 @@ class StepContext:
                  q_len: Sequence[int], pos0: Sequence[int], slots: Sequence[int],
                  group_tables: Sequence[Tuple[int, List[List[int]]]],
                  table_width: int = 0, out: Optional[torch.Tensor] = None,
-                 max_context: int = 0):
+                 max_context: int = 0, shared: Sequence = (), shared_room: Tuple[int, int] = (0, 0)):
         """group_tables: per cache group (page_size, block table of each item).
         table_width forces the width of the device block tables, `out` is a fixed device
         buffer to fill instead of fresh memory, max_context overrides the longest context
-        (all three serve captured graphs, whose shapes and launch choices must not vary)."""
+        (all three serve captured graphs, whose shapes and launch choices must not vary).
+        shared: per cache group the `SharedRuns` of the requests of one token, or None where every request reads its keys by
+        itself; shared_room (runs, levels): their lists are padded to so many runs (for captured graphs as well), and to
+        places for all tokens."""
         self.runtime = runtime
         self._ring, self._scratch, self.error = ring, scratch, error
         # what one part leaves for a later part of the same step (values of the step's tokens that
@@ -121,6 +136,18 @@ class StepContext:
             slot_of = np.where(page >= 0, page * page_size + positions % page_size, -1)
             parts += [table.reshape(-1), slot_of.astype(np.int32)]
             shapes.append((page_size, width))
+        lists = []
+        for runs in shared:
+            if runs is None:
+                lists.append(None)
+                continue
+            order, own_run, table = runs.order, runs.own_run, runs.runs
+            if shared_room[0]:                        # tokens behind the requests see no key; runs without places
+                order = np.concatenate([order, np.arange(len(order), T, dtype=np.int32)])
+                own_run = np.concatenate([own_run, np.full(T - len(own_run), -1, dtype=np.int32)])
+                table = np.concatenate([table, np.zeros((shared_room[0] - len(table), 6), dtype=np.int32)])
+            parts += [order, own_run, table.reshape(-1)]
+            lists.append((len(order), len(table), shared_room if shared_room[0] else (runs.shared, runs.levels)))
         flat = np.concatenate(parts) if parts else np.zeros(0, np.int32)
         dev = ring.stage(flat, runtime.device, out)
         self.staged_ints = flat.size
@@ -138,6 +165,11 @@ class StepContext:
         for page_size, width in shapes:
             tables = take(I * width).view(I, width)
             self.groups.append(GroupStep(page_size, tables, take(T)))
+        self.shared_lists: List[Optional[SharedLists]] = [None] * len(self.groups)
+        for group, sizes in enumerate(lists):
+            if sizes is not None:
+                places, count, (most, levels) = sizes
+                self.shared_lists[group] = SharedLists(take(places), take(places), take(6 * count).view(count, 6), most, levels)
         self._tiles: Dict[Tuple[int, int], Tiles] = {}
 
     @cached_property
@@ -150,12 +182,15 @@ class StepContext:
         """Requests of one token, or none."""
         return int((self.h_qlen <= 1).sum())
 
-    def attention_tiles(self, group_size: int, rows_per_tile: int) -> Tiles:
+    def attention_tiles(self, group_size: int, rows_per_tile: int, skip_ones: bool = False) -> Tiles:
         """Tiles of `rows_per_tile` query rows, a row being (token, head of the group):
-        row = token_in_item * group_size + head_in_group.  No tile spans two items."""
-        key = (group_size, rows_per_tile)
+        row = token_in_item * group_size + head_in_group.  No tile spans two items.  `skip_ones`: requests of one token
+        have none."""
+        key = (group_size, rows_per_tile, skip_ones)
         if key not in self._tiles:
             counts = (self.h_qlen.astype(np.int64) * group_size + rows_per_tile - 1) // rows_per_tile
+            if skip_ones:
+                counts[self.h_qlen == 1] = 0
             item = np.repeat(np.arange(self.num_items, dtype=np.int32), counts)
             first = np.cumsum(counts) - counts
             row0 = (np.arange(int(counts.sum())) - np.repeat(first, counts)) * rows_per_tile
@@ -165,13 +200,13 @@ class StepContext:
             self._tiles[key] = Tiles(dev[:n], dev[n:2 * n], n)
         return self._tiles[key]
 
-    def attention_row_classes(self, group_size: int, class_rows):
+    def attention_row_classes(self, group_size: int, class_rows, skip_ones: bool = False):
         """Requests sorted into row classes by their number of query rows (new tokens x
         group size): class c takes those that fit one tile of class_rows[c] rows, the last
         class takes the rest in as many tiles as needed.  Returns, per non-empty class,
         (class index, Tiles, int32 device list of the class's tokens, their count, the
-        longest context in the class)."""
-        key = ("classes", group_size, tuple(class_rows))
+        longest context in the class).  `skip_ones`: requests of one token are in no class."""
+        key = ("classes", group_size, tuple(class_rows), skip_ones)
         if key in self._tiles:
             return self._tiles[key]
         rows = self.h_qlen.astype(np.int64) * group_size
@@ -179,6 +214,8 @@ class StepContext:
         which = np.full(self.num_items, last, dtype=np.int64)
         for c in range(last - 1, -1, -1):
             which[rows <= class_rows[c]] = c
+        if skip_ones:
+            which[self.h_qlen == 1] = -1
         host, layout = [], []
         for c, per_tile in enumerate(class_rows):
             members = np.nonzero(which == c)[0]
@@ -200,6 +237,8 @@ class StepContext:
             longest = self.fixed_context or int((self.h_pos0[members] + self.h_qlen[members]).max())
             layout.append((c, item.size, tokens.size, longest))
             host += [item, row0.astype(np.int32), tokens]
+        if not host:
+            return []
         dev = self._ring.stage(np.concatenate(host), self.runtime.device)
         out, cut = [], 0
         for c, n_tiles, n_tokens, longest in layout:

@@ -89,12 +89,15 @@ class LoadedModel:
 class Engine:
     def __init__(self, model: LoadedModel, block_size: int = 16, num_blocks: int = 2048,
                  seed: int = 0, max_batch: int = 256, enable_prefix_cache: bool = False,
-                 max_step_tokens: int = 2048, pipeline: bool = True):
+                 max_step_tokens: int = 2048, pipeline: bool = True, shared_attention: bool = False):
+        """`shared_attention`: keys that several running requests hold (answers to one prompt, prompts with a common
+        beginning under the prefix cache) are read once for all of them in the steps where that pays, which rounds a little
+        differently than when each reads for itself."""
         self.model = model
         self.runner = ModelRunner(model.model, model.runtime, page_size=block_size,
                                   num_pages=num_blocks, max_requests=max_batch,
                                   enable_prefix_cache=enable_prefix_cache,
-                                  max_step_tokens=max_step_tokens)
+                                  max_step_tokens=max_step_tokens, shared_attention=shared_attention)
         self.scheduler = Scheduler(self.runner.cache, max_batch, max_step_tokens,
                                    self.runner.max_positions)
         self.sampler = Sampler(model.runtime.device)

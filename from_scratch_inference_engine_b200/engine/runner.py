@@ -17,6 +17,8 @@ import numpy as np
 import torch
 
 from ..cache.manager import CacheManager, RequestCache
+from ..cache.shared_runs import SharedRuns, find_shared_runs
+from ..kernels import ops
 from ..parts.base import LayerCache
 from ..parts.model import DecoderModel
 from .context import PinnedRing, StepContext
@@ -42,32 +44,38 @@ class DeviceFault(RuntimeError):
 
 DECODE_BATCHES = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512)
 TABLE_STEP = 64          # block tables of captured steps grow in steps of this many pages
+MOST_SHARED_RUNS, MOST_SHARED_LEVELS = 128, 4    # of a step; what working memory is sized by
+NO_RUNS = SharedRuns(np.zeros(0, np.int32), np.zeros((0, 6), np.int32), np.zeros(0, np.int32), 0, 0, 0)
 
 
 class _DecodeGraph:
     """One decode step (a single token per request) of a fixed batch size and block-table
     width, captured in a CUDA graph.  Its inputs live in one fixed int32 device buffer that
     every step refills with one copy from pinned host memory; requests fewer than the batch
-    size are padded with entries that store nothing and see no key."""
+    size are padded with entries that store nothing and see no key.  `shared`: of the groups whose
+    layers can, keys that several requests hold are read once for all of them."""
 
-    def __init__(self, runner: "ModelRunner", batch: int, width: int):
-        self.runner, self.batch, self.width = runner, batch, width
+    def __init__(self, runner: "ModelRunner", batch: int, width: int, shared: bool = False):
+        self.runner, self.batch, self.width, self.shared = runner, batch, width, shared
         groups = len(runner.cache.groups)
         ints = 6 * batch + groups * (batch * width + batch)
+        if shared:
+            self.shared_room = (batch + min(batch - 1, MOST_SHARED_RUNS), MOST_SHARED_LEVELS)
+            ints += sum(runner.shareable) * (2 * batch + 6 * self.shared_room[0])
         device = runner.runtime.device
         self.buffer = torch.zeros(ints, dtype=torch.int32, device=device)
         self.rows = torch.arange(batch, dtype=torch.int32, device=device)
         # scratch of its own: the graph holds raw addresses, so what it uses must never be
         # freed or regrown by later steps
         self.scratch: Dict[str, torch.Tensor] = {}
-        self.context = self.fill([], [], [], [[] for _ in range(groups)])
+        self.context = self.fill([], [], [], [[] for _ in range(groups)],
+                                 [NO_RUNS if takes else None for takes in runner.shareable])
         # one plain run first: libraries initialise, tile lists and scratch get allocated
         stream = torch.cuda.Stream(device=device)
         stream.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(stream):
             runner.model.forward(self.context, runner.layer_caches, self.rows)
         torch.cuda.current_stream().wait_stream(stream)
-        from ..kernels import ops
         self.graph = torch.cuda.CUDAGraph()
         before = ops.launches
         # Nothing may free pinned or device memory while the stream is capturing; the garbage
@@ -84,7 +92,7 @@ class _DecodeGraph:
                 gc.enable()
         self.launches = ops.launches - before
 
-    def fill(self, token_ids, pos0, slots, tables) -> StepContext:
+    def fill(self, token_ids, pos0, slots, tables, shared=()) -> StepContext:
         """Write one step's inputs into the fixed buffer (padded to the batch size)."""
         runner, pad = self.runner, self.batch - len(token_ids)
         page = runner.cache.page_size
@@ -93,10 +101,10 @@ class _DecodeGraph:
                            list(token_ids) + [0] * pad, list(range(self.batch)),
                            [1] * self.batch, list(pos0) + [0] * pad, list(slots) + [-1] * pad,
                            group_tables, table_width=self.width, out=self.buffer,
-                           max_context=self.width * page)
+                           max_context=self.width * page, shared=shared if self.shared else (),
+                           shared_room=self.shared_room if self.shared else (0, 0))
 
     def replay(self) -> torch.Tensor:
-        from ..kernels import ops
         self.graph.replay()
         ops.launches += self.launches
         return self.logits
@@ -105,10 +113,13 @@ class _DecodeGraph:
 class ModelRunner:
     def __init__(self, model: DecoderModel, runtime: Runtime, page_size: int = 16,
                  num_pages=2048, max_requests: int = 256, enable_prefix_cache: bool = False,
-                 cuda_graphs: bool = True, max_step_tokens: int = 8192):
+                 cuda_graphs: bool = True, max_step_tokens: int = 8192, shared_attention: bool = False):
         """`max_step_tokens` and `max_requests` cap what one step may bring (tokens; requests):
         a step beyond them is refused before anything runs, so that the working memory of a
-        step is bounded by what `reserve_step_memory` has seen."""
+        step is bounded by what `reserve_step_memory` has seen.  `shared_attention`: where requests
+        of one token hold the same pages (after `fork`, or by the prefix cache) and it pays, layers
+        that keep every key read those once for all of them; refused for a model without such a
+        layer."""
         if max_step_tokens <= 0 or max_requests <= 0:
             raise ValueError("max_step_tokens and max_requests must be positive")
         self.model, self.runtime = model, runtime
@@ -149,6 +160,19 @@ class ModelRunner:
                                      else pages[:, position, keys:])
                 cache.page_stride = pages.stride(0)
             self.layer_caches.append(cache)
+        # cache groups some layer of which can read keys once for all requests that hold them
+        self.shareable = [False] * len(self.cache.groups)
+        for (layer, _, _), cache in zip(model.schedule, self.layer_caches):
+            takes = getattr(model.blocks[layer].mixer, "takes_shared_lists", None)
+            if shared_attention and cache.pages is not None and takes is not None and takes(dtype):
+                self.shareable[cache.group] = True
+        if shared_attention and not any(self.shareable):
+            raise ValueError("shared_attention: no layer of this model can read keys for several requests at once")
+        # It pays where at least so many bytes of keys and values of a layer, and at least this part of what its requests
+        # see, need not be read again.
+        self.shared_min_bytes = 64 << 20
+        self.shared_min_part = 0.5
+        self.shared_least_keys = 64          # ... and of every single run so many keys
         self.error = runtime.error
         self._ring = PinnedRing()
         self._scratch: Dict[str, torch.Tensor] = {}
@@ -213,7 +237,6 @@ class ModelRunner:
         if device_tokens is None:
             raise ValueError("step: entries take tokens from the device, but none were given")
         host = np.asarray([d for d, _ in pairs] + [r for _, r in pairs], dtype=np.int32)
-        from ..kernels import ops
         ops.place_tokens(ctx.token_ids, self._ring.stage(host, self.runtime.device), device_tokens)
 
     def reserve_step_memory(self, tokens: int = 0) -> int:
@@ -246,11 +269,53 @@ class ModelRunner:
         widths = range(TABLE_STEP, -(-pages // TABLE_STEP) * TABLE_STEP + 1, TABLE_STEP)
         for batch in DECODE_BATCHES:
             for width in widths:
-                if (batch, width) not in self._graphs:
-                    self._graphs[batch, width] = _DecodeGraph(self, batch, width)
+                for shared in ((False, True) if any(self.shareable) and batch > 1 else (False,)):
+                    self._graph(batch, width, shared)
             if batch >= limit:
                 break
         return len(self._graphs)
+
+    def _graph(self, batch: int, width: int, shared: bool) -> _DecodeGraph:
+        key = (batch, width, shared)
+        if key not in self._graphs:
+            self._graphs[key] = _DecodeGraph(self, *key)
+        return self._graphs[key]
+
+    @staticmethod
+    def _alone(count: int, pos0: Sequence[int]) -> SharedRuns:
+        """Requests of one token that share nothing."""
+        places = np.arange(count, dtype=np.int32)
+        zeros = np.zeros(count, dtype=np.int32)
+        runs = np.stack([places, zeros + 1, zeros, np.asarray(pos0, dtype=np.int32) + 1, places, zeros - 1], axis=1)
+        return SharedRuns(places, runs, places, 0, 0, 0)
+
+    def _find_shared(self, tables: Sequence[Sequence[np.ndarray]], q_start, q_len, pos0) -> List[Optional[SharedRuns]]:
+        """Per cache group how its requests of one token share their keys, or None where each had better read for itself.
+        tables[g][i]: the pages that request i holds in group g."""
+        found: List[Optional[SharedRuns]] = [None] * len(tables)
+        if not any(self.shareable):
+            return found
+        lengths = np.asarray(q_len)
+        ones = np.nonzero(lengths == 1)[0]
+        if not 2 <= len(ones) <= ops.SHARED_ATTENTION_MAX_RUNS - MOST_SHARED_RUNS:
+            return found
+        at = np.asarray(pos0, dtype=np.int64)[ones]
+        for g, takes in enumerate(self.shareable):
+            if not takes:
+                continue
+            rows = [tables[g][i] for i in ones]
+            table = np.full((len(rows), max(1, max(len(row) for row in rows))), -1, dtype=np.int32)
+            for i, row in enumerate(rows):
+                table[i, :len(row)] = row
+            runs = find_shared_runs(table, self.cache.page_size, np.asarray(q_start)[ones], lengths[ones], at,
+                                    self.shared_least_keys, MOST_SHARED_RUNS, MOST_SHARED_LEVELS)
+            need = self.cache.groups[g].need
+            key_bytes = 2 * need.kv_heads * need.head_dim * self.pages[g].element_size()
+            if runs.saved and runs.saved * key_bytes >= self.shared_min_bytes \
+                    and runs.saved >= self.shared_min_part * int((at + 1).sum()):
+                runs.runs[:, 4] = ones[runs.runs[:, 4]]        # rows of the step's block tables
+                found[g] = runs
+        return found
 
     def _decode_step(self, entries: Sequence[StepEntry], device_tokens: Optional[torch.Tensor]):
         """A step of single tokens through a captured graph: (whether it ran, logits)."""
@@ -261,13 +326,15 @@ class ModelRunner:
             return False, None
         blocks = max((len(t) for e in entries for t in e.handle.tables), default=1)
         width = -(-max(blocks, 1) // TABLE_STEP) * TABLE_STEP
-        key = (batch, width)
-        graph = self._graphs.get(key)
-        if graph is None:
-            graph = self._graphs[key] = _DecodeGraph(self, batch, width)
-        ctx = graph.fill([max(0, e.tokens[0]) for e in entries], [e.handle.length for e in entries],
-                         [e.handle.slot for e in entries],
-                         [[e.handle.table_array(g) for e in entries] for g in range(len(cache.groups))])
+        tables = [[e.handle.table_array(g) for e in entries] for g in range(len(cache.groups))]
+        pos0 = [e.handle.length for e in entries]
+        shared = self._find_shared(tables, range(count), [1] * count, pos0)
+        if any(runs is not None for runs in shared):      # (then all of its groups that can, by whatever they share)
+            shared = [runs or (self._alone(count, pos0) if takes else None) for runs, takes in zip(shared, self.shareable)]
+            graph = self._graph(batch, width, True)
+        else:
+            graph = self._graph(batch, width, False)
+        ctx = graph.fill([max(0, e.tokens[0]) for e in entries], pos0, [e.handle.slot for e in entries], tables, shared)
         self._place_device_tokens(ctx, entries, range(count), device_tokens)
         logits = graph.replay()
         wanted = [i for i, e in enumerate(entries) if len(e.want)]
@@ -312,8 +379,9 @@ class ModelRunner:
             token_ids += [0] if entry.source_row >= 0 else list(entry.tokens)
         tables = [(cache.page_size, [e.handle.table_array(g) for e in entries])
                   for g in range(len(cache.groups))]
+        shared = self._find_shared([t for _, t in tables], q_start, q_len, pos0)
         ctx = StepContext(self.runtime, self._ring, self._scratch, self.error, token_ids, q_start,
-                          q_len, pos0, slots, tables)
+                          q_len, pos0, slots, tables, shared=shared)
         self._place_device_tokens(ctx, entries, q_start, device_tokens)
         rows = None
         if want_rows:
@@ -325,7 +393,6 @@ class ModelRunner:
 
     # -------------------------------------------------------------- copies of what requests hold
     def _copy_blocks(self, buffers: Sequence[torch.Tensor], moves) -> None:
-        from ..kernels import ops
         host = np.asarray(moves, dtype=np.int32).reshape(-1)
         ops.copy_blocks(buffers, self._ring.stage(host, self.runtime.device).view(-1, 2), self.error)
 
@@ -381,5 +448,9 @@ class ModelRunner:
                     42: "tiled float32 product: a stage never arrived",
                     43: "tiled float32 product: a stage was never multiplied",
                     4: "copy of blocks: a block outside its pool",
-                    3: "attention: a visible key lies in a page that was given back"}
+                    3: "attention: a visible key lies in a page that was given back",
+                    5: "biases of logits: a token outside the vocabulary or out of order",
+                    6: "logits: a history or a mask that does not exist",
+                    7: "shared attention: a run outside of what there is, or beyond one of its tokens",
+                    8: "shared attention: more runs than its working memory is for"}
             raise DeviceFault(what.get(code, f"device error flag {code}"))

@@ -2535,7 +2535,7 @@ def attn_shared(head_dim: int):
         i, f, ll, p = ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_void_p
         lib.fsie_shared_attention_head_dim.argtypes = lib.fsie_shared_attention_max_runs.argtypes = []
         lib.fsie_shared_attention_head_dim.restype = lib.fsie_shared_attention_max_runs.restype = i
-        lib.fsie_shared_attention_room.argtypes = [i, i, i, i, i, i]
+        lib.fsie_shared_attention_room.argtypes = [i, i, i, i, i, i, i]
         lib.fsie_shared_attention_room.restype = ll
         lib.fsie_shared_attention.argtypes = [p, i, p, p, ll, i, i, p, i, i, p, i, p, i, p, i, p, p, i, i, i, i, f, p, ll, i, i,
                                               p, p]
@@ -2551,10 +2551,11 @@ def shared_attention_takes(dtype: torch.dtype, head_dim: int) -> bool:
 
 
 def shared_attention_room(tokens: int, runs: int, levels: int, heads: int, kv_heads: int, head_dim: int,
-                          dtype: torch.dtype) -> int:
-    """Bytes of working memory that `shared_attention` needs for so many places in `order` and runs, with at most `levels`
-    runs around an innermost one."""
-    size = attn_shared(head_dim).fsie_shared_attention_room(tokens, runs, levels, heads, kv_heads, _tag(dtype))
+                          dtype: torch.dtype, shared: Optional[int] = None) -> int:
+    """Bytes of working memory that `shared_attention` needs for so many places in `order` and runs, `shared` of them
+    (None: all) no token's innermost, at most `levels` around an innermost one."""
+    size = attn_shared(head_dim).fsie_shared_attention_room(tokens, runs, runs if shared is None else shared, levels, heads,
+                                                            kv_heads, _tag(dtype))
     if size < 0:
         raise KernelError(f"shared_attention_room: refused ({size})")
     return size

@@ -102,6 +102,9 @@ class GqaAttention(Mixer):
     def cache_need(self) -> Optional[CacheNeed]:
         return CacheNeed(self.num_kv_heads, self.head_dim, self.window)
 
+    def takes_shared_lists(self, dtype: torch.dtype) -> bool:
+        return self.window == 0 and ops.shared_attention_takes(dtype, self.head_dim)
+
     def bind(self, tensors: Dict[str, torch.Tensor], runtime) -> None:
         self.runtime = runtime
         p = self.prefix
@@ -130,15 +133,33 @@ class GqaAttention(Mixer):
         # working memory shared by all attention layers of a model: a layer's q, k, v and its
         # attention output are dead when the next attention layer runs
         out = rt.buffer("attention.out", tokens, self.q_width, qkv.dtype)
-        self._attend(ctx, qkv, group, cache, out)
+        lists = ctx.shared_lists[cache.group] if self.takes_shared_lists(qkv.dtype) else None
+        if lists is None:
+            self._attend(ctx, qkv, group, cache, out)
+        else:
+            if not ctx.one_each:
+                self._attend(ctx, qkv, group, cache, out, skip_ones=True)
+            self._attend_shared(ctx, qkv, group, cache, out, lists)
         return rt.linear(out, self.w_o, None, "attention.o")
 
-    def _attend(self, ctx, qkv: torch.Tensor, group, cache: LayerCache, out: torch.Tensor) -> None:
+    def _attend_shared(self, ctx, qkv: torch.Tensor, group, cache: LayerCache, out: torch.Tensor, lists) -> None:
+        """Attention of the requests of one token, with keys that several of them hold read once for all.  Behind `_attend`,
+        whose 32-bit form may leave anything in these tokens' rows."""
+        room = ctx.runtime.buffer("attention.shared_room", 1, ops.shared_attention_room(
+            lists.order.shape[0], lists.runs.shape[0], lists.levels, self.num_heads, self.num_kv_heads, self.head_dim,
+            qkv.dtype, lists.shared), torch.uint8)
+        ops.shared_attention(qkv, qkv.stride(0), cache.k_pages, cache.v_pages, cache.page_stride, group.page_size,
+                             group.block_tables, ctx.positions, lists.order, lists.runs, lists.own_run, out, self.num_heads,
+                             self.num_kv_heads, self.head_dim, self.scale, room, ctx.error, early=True)
+
+    def _attend(self, ctx, qkv: torch.Tensor, group, cache: LayerCache, out: torch.Tensor,
+                skip_ones: bool = False) -> None:
         """Attention of the step's tokens over the pages.  Work is cut into tiles of query
         rows, a row being a (token, head of the group) pair; a tile's key range is split
         over several blocks when the batch alone would not fill the GPU.  bfloat16 runs on
         the tensor cores (one launch per row class present in the batch: single decoded
-        tokens, short portions, long portions); float32 runs the 32-bit kernel."""
+        tokens, short portions, long portions); float32 runs the 32-bit kernel.  `skip_ones`:
+        requests of one token are left out."""
         tokens = qkv.shape[0]
         group_size = self.num_heads // self.num_kv_heads
         sms = ctx.runtime.sm_count
@@ -156,7 +177,7 @@ class GqaAttention(Mixer):
             if pages_map is not None:
                 class_rows = class_rows[:-1] + (ops.ATTENTION_TC_ROWS,)
             for row_class, tiles, class_tokens, count, longest in \
-                    ctx.attention_row_classes(group_size, class_rows):
+                    ctx.attention_row_classes(group_size, class_rows, skip_ones):
                 on_tcgen05 = pages_map is not None and row_class == len(class_rows) - 1
                 # decoded tokens: from about 1.6 blocks per SM before any split the tcgen05 kernel
                 # (a tile's keys as the M side) is ahead of the mma.sync one, below that behind
@@ -202,10 +223,10 @@ class GqaAttention(Mixer):
         # kernel for tiles of 32 rows; one choice of key splits and one merge for both
         if ops.attention_rows16_fits(qkv.dtype, self.head_dim, cache.page_stride):
             classes = ctx.attention_row_classes(group_size, (ops.attention_rows16_rows(),
-                                                             ops.attention_rows_per_tile()))
+                                                             ops.attention_rows_per_tile()), skip_ones)
             launches = [(row_class == 0, tiles) for row_class, tiles, _, _, _ in classes]
         else:
-            launches = [(False, ctx.attention_tiles(group_size, ops.attention_rows_per_tile()))]
+            launches = [(False, ctx.attention_tiles(group_size, ops.attention_rows_per_tile(), skip_ones))]
         blocks = sum(tiles.count for _, tiles in launches) * self.num_kv_heads
         decoding = all(rows16 for rows16, _ in launches)
         nsplit = splits(blocks, ctx.max_context, even_work=decoding, blocks_per_sm=2)

@@ -124,6 +124,10 @@ class Mixer(Part):
     def state_need(self) -> Optional[StateNeed]:
         return None
 
+    def takes_shared_lists(self, dtype: torch.dtype) -> bool:
+        """Whether forward reads keys that several requests hold once for all of them where `ctx.shared_lists` says so."""
+        return False
+
     def reserve(self, tokens: int, requests: int) -> None:
         """Take from the runtime what working memory a step of up to so many tokens may need beyond what it needs when they are
         one request's: steps of up to `requests` requests follow."""

@@ -8,7 +8,7 @@ from from_scratch_inference_engine_b200.cache.manager import CacheManager, Cache
 from from_scratch_inference_engine_b200.cache.shared_runs import find_shared_runs
 
 
-def runs_of(tables, page, lengths, new=None, least=1):
+def runs_of(tables, page, lengths, new=None, least=1, *most):
     width = max([len(t) for t in tables] + [1])
     array = np.full((len(tables), width), -1, dtype=np.int32)
     for i, t in enumerate(tables):
@@ -16,7 +16,7 @@ def runs_of(tables, page, lengths, new=None, least=1):
     new = new or [1] * len(tables)
     start = np.cumsum([0] + new[:-1]) if tables else []
     return find_shared_runs(array, page, np.asarray(start, dtype=np.int32), np.asarray(new, dtype=np.int32),
-                            np.asarray([n - k for n, k in zip(lengths, new)], dtype=np.int32), least)
+                            np.asarray([n - k for n, k in zip(lengths, new)], dtype=np.int32), least, *most)
 
 
 def check(found, tables, page, lengths, new):
@@ -120,3 +120,14 @@ def test_forked_requests_of_the_cache_manager():
     found = runs_of(tables, 4, lengths)
     check(found, tables, 4, lengths, [1] * 4)
     assert found.shared == 2 and found.levels == 2 and found.saved == 3 * 8 + 8
+
+
+@pytest.mark.parametrize("most,levels", [(0, 31), (1, 31), (5, 31), (700, 3), (1000, 31), (1000, 1), (1000, 0)])
+def test_no_more_runs_and_levels_than_asked_for(most, levels):
+    """Request i holds the first i pages of one chain: without a limit a run around a run around a run.."""
+    count, page = 300, 4
+    tables = [list(range(i)) + [1000 + i] for i in range(count)]
+    lengths = [i * page + 1 for i in range(count)]
+    found = runs_of(tables, page, lengths, None, 1, most, levels)
+    check(found, tables, page, lengths, [1] * count)
+    assert found.shared == min(most, levels, count - 2) and found.levels == found.shared
