@@ -6,7 +6,9 @@ Options follow the reference's harness (benchmarks/harness/bench_engine.py:118-1
 up front, drives `Engine.step` and reports TTFT mean/p50/p90, TPOT, tokens/s and
 requests/s (bench_engine.py:48-98).  Added: --prompt-ids / --prompt-len (token ids need
 no tokenizer), --top-k, --top-p, --seed, --dtype, --max-batch, --max-step-tokens,
---prefix-cache, and --random-weights CONFIG.json with --weights-seed / --std, which
+--prefix-cache, --shared-attention (keys that several requests hold are read once),
+--repetition-penalty, --presence-penalty, --frequency-penalty, --logit-bias ID:VALUE,..
+and --allowed-ids ID,.. (of every token's choice), and --random-weights CONFIG.json with --weights-seed / --std, which
 writes a random model folder to --model-dir first.
 """
 
@@ -44,10 +46,16 @@ def main(argv=None) -> int:
     parser.add_argument("--top-k", type=int, default=0)
     parser.add_argument("--top-p", type=float, default=1.0)
     parser.add_argument("--seed", type=int, default=0)
+    parser.add_argument("--repetition-penalty", type=float, default=1.0)
+    parser.add_argument("--presence-penalty", type=float, default=0.0)
+    parser.add_argument("--frequency-penalty", type=float, default=0.0)
+    parser.add_argument("--logit-bias", default=None, help="comma-separated ID:VALUE, added to these tokens' logits")
+    parser.add_argument("--allowed-ids", default=None, help="comma-separated token ids that may be chosen")
     parser.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     parser.add_argument("--max-batch", type=int, default=256)
     parser.add_argument("--max-step-tokens", type=int, default=2048)
     parser.add_argument("--prefix-cache", type=int, default=1, choices=[0, 1])
+    parser.add_argument("--shared-attention", type=int, default=0, choices=[0, 1])
     parser.add_argument("--random-weights", default=None, metavar="CONFIG.json")
     parser.add_argument("--weights-seed", type=int, default=0)
     parser.add_argument("--std", type=float, default=0.02)
@@ -55,6 +63,16 @@ def main(argv=None) -> int:
     args = parser.parse_args(argv)
     if not args.model_dir:
         parser.error("--model-dir (or ENGINE_MODEL_DIR) is required")
+    logit_bias = allowed = None
+    try:
+        if args.logit_bias:
+            pairs = [pair.split(":") for pair in args.logit_bias.split(",")]
+            logit_bias = {int(token): float(value) for token, value in pairs}
+        if args.allowed_ids:
+            allowed_ids = [int(t) for t in args.allowed_ids.split(",")]
+            allowed = lambda output: allowed_ids
+    except ValueError:
+        parser.error("--logit-bias takes ID:VALUE,.. and --allowed-ids takes ID,..")
 
     from . import LLM, SamplingParams, SeqStatus, write_random_model
     from .config import config_from_dict
@@ -64,7 +82,8 @@ def main(argv=None) -> int:
         write_random_model(args.model_dir, config, args.weights_seed, args.std)
     llm = LLM(args.model_dir, block_size=args.block_size, num_blocks=args.num_blocks,
               seed=args.seed, max_batch=args.max_batch, dtype=args.dtype,
-              enable_prefix_cache=bool(args.prefix_cache), max_step_tokens=args.max_step_tokens)
+              enable_prefix_cache=bool(args.prefix_cache), max_step_tokens=args.max_step_tokens,
+              shared_attention=bool(args.shared_attention))
     vocab = llm.model.model.spec.vocab_size
     if args.prompt_ids:
         prompts = [[int(t) for t in args.prompt_ids.split(",")]] * args.num_requests
@@ -78,7 +97,8 @@ def main(argv=None) -> int:
         parser.error("one of --prompt, --prompt-ids, --prompt-len is required")
 
     engine = llm.engine
-    params = SamplingParams(args.temperature, args.top_k, args.top_p)
+    params = SamplingParams(args.temperature, args.top_k, args.top_p, None, args.repetition_penalty,
+                            args.presence_penalty, args.frequency_penalty, logit_bias, allowed)
     start = perf_counter()
     ids = [engine.add_request(list(p), params, args.max_tokens, llm.eos_id) for p in prompts]
     first, finished = {}, {}

@@ -25,7 +25,8 @@ import torch
 
 from ..config.registry import load_config
 from ..parts.model import DecoderModel
-from ..sampling.sampler import Sampler, SamplingParams, request_seed
+from ..sampling.history import TokenHistory
+from ..sampling.sampler import Sampler, SamplingParams, pack_allowed, request_seed, sorted_bias
 from ..weights.loader import load_checkpoint
 from .runner import ModelRunner, StepEntry
 from .runtime import Runtime, parse_dtype
@@ -101,9 +102,11 @@ class Engine:
         self.scheduler = Scheduler(self.runner.cache, max_batch, max_step_tokens,
                                    self.runner.max_positions)
         self.sampler = Sampler(model.runtime.device)
+        self.history = TokenHistory(model.runtime.device, self.runner.vocab_size)
         self.seed = int(seed)
         self.pipeline = bool(pipeline)
         self._in_flight = None          # (items, Picked) of a launched step whose tokens are not read yet
+        self._raised = None             # what a request's `allowed` raised
         self.steps = 0
         self.tokens_prefilled = 0
         self.tokens_decoded = 0
@@ -115,9 +118,12 @@ class Engine:
         vocab = self.runner.vocab_size
         if any(t < 0 or t >= vocab for t in prompt):
             raise IndexError(f"Engine: token id out of range [0, {vocab})")
+        params.check(vocab)
         rid = self.scheduler.next_id
         seed = params.seed if params.seed is not None else request_seed(self.seed, rid)
-        return self.scheduler.add(prompt, params, max_tokens, eos_id, seed)
+        self.scheduler.add(prompt, params, max_tokens, eos_id, seed)
+        self.scheduler.sequences[rid].bias = sorted_bias(params.logit_bias, vocab)
+        return rid
 
     def fork(self, request_id: int, count: int = 1, params: Optional[Sequence[SamplingParams]] = None) -> List[int]:
         """Continue a running request `count` more times from where it stands: prompt and output so far are shared, not run
@@ -136,10 +142,15 @@ class Engine:
             raise RuntimeError(f"Engine: {count} more running requests exceed max_batch {self.scheduler.max_batch}")
         if params is None:                  # a seed of its own each, whatever the request's is
             params = [replace(seq.params, seed=None)] * count
+        for p in params:
+            p.check(self.runner.vocab_size)
         ids = self.scheduler.next_ids(count)
         handles = self.runner.fork(seq.handle, ids)
         seeds = [p.seed if p.seed is not None else request_seed(self.seed, rid) for p, rid in zip(params, ids)]
-        return self.scheduler.fork(seq, handles, params, seeds)
+        self.scheduler.fork(seq, handles, params, seeds)
+        for rid, p in zip(ids, params):
+            self.scheduler.sequences[rid].bias = sorted_bias(p.logit_bias, self.runner.vocab_size)
+        return ids
 
     def compact(self) -> List[int]:
         """Bring the pages in use to the front of their pools; returns how many those are per group."""
@@ -155,6 +166,8 @@ class Engine:
         page then wait and run the prompt by themselves.  Returns the ids, in order."""
         if not params:
             return []
+        for p in params:
+            p.check(self.runner.vocab_size)
         first = self.add_request(prompt, params[0], max_tokens, eos_id)
         seq = self.scheduler.sequences[first]
         ids, rest = [first], list(params[1:])
@@ -199,14 +212,23 @@ class Engine:
 
     # ---------------------------------------------------------------------- step
     def step(self) -> int:
-        """One batched step; returns the number of tokens it ran (0 = nothing could run)."""
+        """One batched step; returns the number of tokens it ran (0 = nothing could run).  What a request's `allowed`
+        raised is raised here, once the step is recorded; that request has ended."""
+        ran = self._step()
+        if self._raised is not None:
+            raised, self._raised = self._raised, None
+            raise raised
+        return ran
+
+    def _step(self) -> int:
         if not self.pipeline:
             items = self.scheduler.plan()
             if not items:
                 return 0
             picked = self._launch(items)
             tokens = self._tokens_of(items, picked)
-            self.scheduler.finish_step(items, tokens)
+            self.scheduler.begin_step(items)
+            self._resolve(items, tokens)
             return self._count(items)
         # plan and launch the next step before the one in flight is read; a plan that would
         # have to preempt (or finds nothing to do) waits until the pending tokens are settled
@@ -222,7 +244,7 @@ class Engine:
             self._settle()
         self.scheduler.begin_step(items)
         if picked is None:                     # nothing sampled: nothing to wait for
-            self.scheduler.resolve_step(items, [None] * len(items))
+            self._resolve(items, [None] * len(items))
         else:
             self._in_flight = (items, picked)
         return self._count(items)
@@ -237,10 +259,40 @@ class Engine:
         sampling = [item for item in items if item.samples]
         if not sampling:
             return None
-        return self.sampler.sample_async(logits, [i.seq.params for i in sampling],
-                                         [i.seq.seed for i in sampling],
+        params = [i.seq.params for i in sampling]
+        slots = masks = biases = None
+        if any(p.penalised for p in params):
+            known = iter(self.history.slots([(i.seq.id, i.seq.prompt, i.seq.output) for i in sampling
+                                             if i.seq.params.penalised], self.runner.error))
+            slots = [next(known) if p.penalised else -1 for p in params]
+        if any(p.allowed is not None for p in params):
+            if self._in_flight is not None:        # the answers so far are needed; the GPU runs this step meanwhile
+                self._settle()
+            masks = [self._mask_of(item) for item in sampling]
+        if any(i.seq.bias is not None for i in sampling):
+            biases = [i.seq.bias for i in sampling]
+        return self.sampler.sample_async(logits, params, [i.seq.seed for i in sampling],
                                          [len(i.seq.output) + i.seq.pending for i in sampling],
-                                         self.runner.error)
+                                         self.runner.error, slots, self.history if slots else None, biases, masks)
+
+    def _mask_of(self, item):
+        """The tokens that may come next in the item's answer, as bits (None: all).  Marks the item where there is none."""
+        seq = item.seq
+        if seq.params.allowed is None or seq.status is not SeqStatus.Running:
+            return None
+        try:
+            tokens = seq.params.allowed(seq.output)
+            mask = None if tokens is None else pack_allowed(tokens, self.runner.vocab_size)
+            item.ends = mask is not None and not mask.any()
+        except Exception as raised:                # the step is under way: it is recorded first
+            self._raised, item.ends = raised, True
+        return None if item.ends else mask
+
+    def _resolve(self, items, tokens) -> None:
+        self.scheduler.resolve_step(items, tokens)
+        for item in items:
+            if item.seq.status is SeqStatus.Finished:
+                self.history.release(item.seq.id)
 
     def _tokens_of(self, items, picked) -> List[Optional[int]]:
         if picked is None:
@@ -254,7 +306,7 @@ class Engine:
         """Wait for the tokens of the step in flight and record them."""
         items, picked = self._in_flight
         self._in_flight = None
-        self.scheduler.resolve_step(items, self._tokens_of(items, picked))
+        self._resolve(items, self._tokens_of(items, picked))
         return sum(len(item.tokens) for item in items)
 
     def _count(self, items) -> int:

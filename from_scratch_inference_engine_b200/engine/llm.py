@@ -4,7 +4,8 @@ Names and defaults as the reference wrapper (python/engine/llm.py:33-76): `LLM(m
 block_size=16, num_blocks=2048, seed=0, max_batch=256, eos_id=None, enable_prefix_cache=
 True)`, `GenerationConfig(max_tokens=64, temperature=0.0, top_k=0, top_p=1.0)`,
 `generate_ids`, `generate`.  `quantize` is not taken: quantised weights are outside this
-engine.  Added: `dtype`, `device`, `max_step_tokens`.
+engine.  Added: `dtype`, `device`, `max_step_tokens`, `shared_attention` (see `Engine`), and in `GenerationConfig` what
+changes logits before a token is chosen (see `SamplingParams`).
 """
 
 from __future__ import annotations
@@ -12,7 +13,7 @@ from __future__ import annotations
 import json
 from dataclasses import dataclass, replace
 from pathlib import Path
-from typing import List, Optional, Sequence
+from typing import Callable, List, Mapping, Optional, Sequence
 
 from ..sampling.sampler import SamplingParams
 from .engine import Engine, LoadedModel
@@ -40,24 +41,30 @@ class GenerationConfig:
     top_k: int = 0
     top_p: float = 1.0
     seed: Optional[int] = None
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Optional[Mapping[int, float]] = None
+    allowed: Optional[Callable[[Sequence[int]], Optional[Sequence[int]]]] = None
 
 
 class LLM:
     def __init__(self, model_dir, *, block_size: int = 16, num_blocks: int = 2048, seed: int = 0,
                  max_batch: int = 256, eos_id: Optional[int] = None,
                  enable_prefix_cache: bool = True, dtype="bfloat16", device="cuda:0",
-                 max_step_tokens: int = 2048):
+                 max_step_tokens: int = 2048, shared_attention: bool = False):
         self.model_dir = Path(model_dir)
         self.model = LoadedModel.from_pretrained(model_dir, dtype=dtype, device=device,
                                                  max_positions=block_size * num_blocks)
         self.engine = Engine(self.model, block_size, num_blocks, seed, max_batch,
-                             enable_prefix_cache, max_step_tokens)
+                             enable_prefix_cache, max_step_tokens, shared_attention=shared_attention)
         self.eos_id = read_eos_id(model_dir) if eos_id is None else eos_id
         self._tokenizer = None
 
     @staticmethod
     def _params(config: GenerationConfig) -> SamplingParams:
-        return SamplingParams(config.temperature, config.top_k, config.top_p, config.seed)
+        return SamplingParams(config.temperature, config.top_k, config.top_p, config.seed, config.repetition_penalty,
+                              config.presence_penalty, config.frequency_penalty, config.logit_bias, config.allowed)
 
     def generate_ids(self, prompt_ids: Sequence[int],
                      config: Optional[GenerationConfig] = None) -> List[int]:

@@ -60,6 +60,7 @@ class Sequence_:
     pending: int = 0          # 1 while a sampled token has not been read from the GPU yet
     pending_row: int = -1     # ... and the row of that step's samples it will be found in
     hold: int = 0             # > 0: no token from this place of the context on is run yet
+    bias: Optional[tuple] = None   # params.logit_bias as the sampler takes it
 
     def context(self) -> List[int]:
         return self.prompt + self.output
@@ -87,6 +88,7 @@ class PlanItem:
     samples: bool          # the portion ends the context: logits of its last token are wanted
     was_prefill: bool
     source_row: int = -1   # >= 0: the single token is row source_row of the previous step's samples
+    ends: bool = False     # no token may come next: the request ends without the one that was sampled
 
 
 def cache_too_small_for_window(cache: CacheManager) -> str:
@@ -296,9 +298,10 @@ class Scheduler:
                     or not seq.pending:
                 continue
             seq.pending, seq.pending_row = 0, -1
-            seq.output.append(int(token))
+            if not item.ends:
+                seq.output.append(int(token))
             hit_eos = seq.eos_id >= 0 and token == seq.eos_id
-            if hit_eos or len(seq.output) >= seq.max_tokens:
+            if item.ends or hit_eos or len(seq.output) >= seq.max_tokens:
                 seq.status = SeqStatus.Finished
                 self.cache.close(seq.handle)
                 seq.handle = None

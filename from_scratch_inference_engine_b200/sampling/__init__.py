@@ -1,3 +1,4 @@
-from .sampler import Sampler, SamplingParams, request_seed, uniform_draw
+from .history import TokenHistory
+from .sampler import Sampler, SamplingParams, pack_allowed, request_seed, sorted_bias, uniform_draw
 
-__all__ = ["Sampler", "SamplingParams", "request_seed", "uniform_draw"]
+__all__ = ["Sampler", "SamplingParams", "TokenHistory", "pack_allowed", "request_seed", "sorted_bias", "uniform_draw"]
