@@ -409,6 +409,105 @@ struct Feed {
 };
 
 // ------------------------------------------------------------------------------------- bfloat16, few rows
+// A tile of 16 rows in one warp, steps of 16 keys: lane 4 g + t has of rows g and g + 8 keys and columns 2 t, 2 t + 1 of every eight.
+struct FewState {
+    float m_lo, m_hi, l_lo, l_hi, o[HD / 8][4];
+    __device__ __forceinline__ void begin() {
+        m_lo = m_hi = -INFINITY; l_lo = l_hi = 0.f;
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c) { o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f; }
+    }
+    // k_at(i), v_at(c): where this lane's row of the i-th (c-th) 16 columns of keys (values) lies; q_of(i, f): the queries' fragment;
+    // bit j of `keys`: key j counts
+    template <typename KeysAt, typename ValuesAt, typename QueryOf>
+    __device__ __forceinline__ void step(KeysAt k_at, ValuesAt v_at, QueryOf q_of, unsigned keys, int t, float sc) {
+        // ---- scores: two chains of products for each eight keys
+        float s[2][4], s2[2][4];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[c][e] = s2[c][e] = 0.f;
+        constexpr int TOGETHER = HD / 16 < 8 ? HD / 16 : 8;               // fragments asked for before the first is used
+#pragma unroll
+        for (int i0 = 0; i0 < HD / 16; i0 += TOGETHER) {
+            unsigned b[TOGETHER][4], q4[4];
+#pragma unroll
+            for (int i = 0; i < TOGETHER; ++i)
+                if (i0 + i < HD / 16) ldmatrix_x4(b[i], k_at(i0 + i));
+#pragma unroll
+            for (int i = 0; i < TOGETHER; ++i) {
+                if (i0 + i >= HD / 16) break;
+                q_of(i0 + i, q4);
+                mma_bf16(i & 1 ? s2[0] : s[0], q4, b[i][0], b[i][1]);
+                mma_bf16(i & 1 ? s2[1] : s[1], q4, b[i][2], b[i][3]);
+            }
+        }
+        float mx_lo = -INFINITY, mx_hi = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const bool there = keys >> (c * 8 + 2 * t + e) & 1;
+                s[c][e] = there ? s[c][e] + s2[c][e] : -INFINITY;
+                s[c][2 + e] = there ? s[c][2 + e] + s2[c][2 + e] : -INFINITY;
+                mx_lo = fmaxf(mx_lo, s[c][e]);
+                mx_hi = fmaxf(mx_hi, s[c][2 + e]);
+            }
+        mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 1));
+        mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 1));
+        mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 2));
+        mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 2));
+        const float mn_lo = fmaxf(m_lo, mx_lo), mn_hi = fmaxf(m_hi, mx_hi);
+        const float base_lo = mn_lo == -INFINITY ? 0.f : mn_lo * sc, base_hi = mn_hi == -INFINITY ? 0.f : mn_hi * sc;
+        const float corr_lo = fast_exp2(m_lo * sc - base_lo), corr_hi = fast_exp2(m_hi * sc - base_hi);
+        m_lo = mn_lo; m_hi = mn_hi;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            s[c][0] = fast_exp2(fmaf(s[c][0], sc, -base_lo)); s[c][1] = fast_exp2(fmaf(s[c][1], sc, -base_lo));
+            s[c][2] = fast_exp2(fmaf(s[c][2], sc, -base_hi)); s[c][3] = fast_exp2(fmaf(s[c][3], sc, -base_hi));
+        }
+        l_lo = l_lo * corr_lo + ((s[0][0] + s[0][1]) + (s[1][0] + s[1][1]));       // of this thread's keys
+        l_hi = l_hi * corr_hi + ((s[0][2] + s[0][3]) + (s[1][2] + s[1][3]));
+        if (__any_sync(0xffffffffu, corr_lo != 1.f || corr_hi != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) { o[c][0] *= corr_lo; o[c][1] *= corr_lo; o[c][2] *= corr_hi; o[c][3] *= corr_hi; }
+        }
+        // ---- weighted values: the weights are rounded to bfloat16, as the values are; the sums l hold them unrounded
+        const unsigned p4[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
+#pragma unroll
+        for (int c0 = 0; c0 < HD / 16; c0 += TOGETHER) {
+            unsigned b[TOGETHER][4];
+#pragma unroll
+            for (int c = 0; c < TOGETHER; ++c)
+                if (c0 + c < HD / 16) ldmatrix_x4_trans(b[c], v_at(c0 + c));
+#pragma unroll
+            for (int c = 0; c < TOGETHER; ++c) {
+                if (c0 + c >= HD / 16) break;
+                mma_bf16(o[2 * (c0 + c)], p4, b[c][0], b[c][1]);
+                mma_bf16(o[2 * (c0 + c) + 1], p4, b[c][2], b[c][3]);
+            }
+        }
+    }
+    __device__ __forceinline__ void leave(const SharedArgs& a, int rows, int slot, int g, int t) {
+        l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 1); l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 2);
+        l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 1); l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 2);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = g + 8 * half;
+            if (r >= rows) continue;
+            const size_t row = (size_t)slot * FEW + r;
+            float* dst = a.part_o + row * HD;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c)
+                *reinterpret_cast<float2*>(dst + c * 8 + 2 * t) = make_float2(o[c][2 * half], o[c][2 * half + 1]);
+            if (t == 0) {
+                const float m = half ? m_hi : m_lo;
+                *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m == -INFINITY ? m : m * a.scale, half ? l_hi : l_lo);
+            }
+        }
+    }
+};
+
 // Every warp is a worker of its own: one tile of 16 rows, steps of 16 keys, its own ring of STAGES steps in shared memory, and
 // no meeting of warps on the way.  What a step costs is its chain of dependent instructions, so what counts is how many warps
 // an SM has at it and how few instructions they take: four warps that shared a step of 32 keys took 442 instructions each,
@@ -525,8 +624,7 @@ __device__ __forceinline__ void few_phase(const SharedArgs& a, const Plan& plan,
 
     const int g = lane >> 2, t = lane & 3;
     const float sc = a.scale * LOG2E;                     // scores in base-2 units
-    float m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.f, l_hi = 0.f;
-    float o[HD / 8][4];
+    FewState state;
     unsigned qf[S::Q_IN_REGS ? HD / 16 : 1][4];
     int stretch = -1;
     Landing now = {0u, 0, 0}, next = {0u, 0, 0};
@@ -543,9 +641,7 @@ __device__ __forceinline__ void few_phase(const SharedArgs& a, const Plan& plan,
         const bf16* q_at = qs + (stretch & (S::Q_IN_REGS ? 1 : 0)) * FEW * LD + ((lane & 7) + 8 * ((lane >> 3) & 1)) * LD + 8 * (lane >> 4);
         if (!S::Q_IN_REGS) q_at += (stretch % 3) * FEW * LD;
         if (begins) {
-            m_lo = m_hi = -INFINITY; l_lo = l_hi = 0.f;
-#pragma unroll
-            for (int c = 0; c < HD / 8; ++c) { o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f; }
+            state.begin();
             if (S::Q_IN_REGS) {
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i) ldmatrix_x4(qf[i], q_at + i * 16);
@@ -557,92 +653,13 @@ __device__ __forceinline__ void few_phase(const SharedArgs& a, const Plan& plan,
         if (n >= 0) {
             const bf16* kt = ring + (n % STAGES) * 2 * KEYS * LD;
             const bf16* vt = kt + KEYS * LD;
-            // ---- scores: two chains of products for each eight keys
-            float s[2][4], s2[2][4];
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[c][e] = s2[c][e] = 0.f;
-            constexpr int TOGETHER = HD / 16 < 8 ? HD / 16 : 8;               // fragments asked for before the first is used
-#pragma unroll
-            for (int i0 = 0; i0 < HD / 16; i0 += TOGETHER) {
-                unsigned b[TOGETHER][4], q4[4];
-#pragma unroll
-                for (int i = 0; i < TOGETHER; ++i)
-                    if (i0 + i < HD / 16) ldmatrix_x4(b[i], kt + ((lane & 7) + 8 * (lane >> 4)) * LD + (i0 + i) * 16 + 8 * ((lane >> 3) & 1));
-#pragma unroll
-                for (int i = 0; i < TOGETHER; ++i) {
-                    if (i0 + i >= HD / 16) break;
-                    if (S::Q_IN_REGS) { q4[0] = qf[i0 + i][0]; q4[1] = qf[i0 + i][1]; q4[2] = qf[i0 + i][2]; q4[3] = qf[i0 + i][3]; }
-                    else ldmatrix_x4(q4, q_at + (i0 + i) * 16);
-                    mma_bf16(i & 1 ? s2[0] : s[0], q4, b[i][0], b[i][1]);
-                    mma_bf16(i & 1 ? s2[1] : s[1], q4, b[i][2], b[i][3]);
-                }
-            }
-            float mx_lo = -INFINITY, mx_hi = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const bool there = now.bits >> (c * 8 + 2 * t + e) & 1;
-                    s[c][e] = there ? s[c][e] + s2[c][e] : -INFINITY;
-                    s[c][2 + e] = there ? s[c][2 + e] + s2[c][2 + e] : -INFINITY;
-                    mx_lo = fmaxf(mx_lo, s[c][e]);
-                    mx_hi = fmaxf(mx_hi, s[c][2 + e]);
-                }
-            mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 1));
-            mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 1));
-            mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 2));
-            mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 2));
-            const float mn_lo = fmaxf(m_lo, mx_lo), mn_hi = fmaxf(m_hi, mx_hi);
-            const float base_lo = mn_lo == -INFINITY ? 0.f : mn_lo * sc, base_hi = mn_hi == -INFINITY ? 0.f : mn_hi * sc;
-            const float corr_lo = fast_exp2(m_lo * sc - base_lo), corr_hi = fast_exp2(m_hi * sc - base_hi);
-            m_lo = mn_lo; m_hi = mn_hi;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                s[c][0] = fast_exp2(fmaf(s[c][0], sc, -base_lo)); s[c][1] = fast_exp2(fmaf(s[c][1], sc, -base_lo));
-                s[c][2] = fast_exp2(fmaf(s[c][2], sc, -base_hi)); s[c][3] = fast_exp2(fmaf(s[c][3], sc, -base_hi));
-            }
-            l_lo = l_lo * corr_lo + ((s[0][0] + s[0][1]) + (s[1][0] + s[1][1]));       // of this thread's keys
-            l_hi = l_hi * corr_hi + ((s[0][2] + s[0][3]) + (s[1][2] + s[1][3]));
-            if (__any_sync(0xffffffffu, corr_lo != 1.f || corr_hi != 1.f)) {
-#pragma unroll
-                for (int c = 0; c < HD / 8; ++c) { o[c][0] *= corr_lo; o[c][1] *= corr_lo; o[c][2] *= corr_hi; o[c][3] *= corr_hi; }
-            }
-            // ---- weighted values: the weights are rounded to bfloat16, as the values are; the sums l hold them unrounded
-            const unsigned p4[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
-#pragma unroll
-            for (int c0 = 0; c0 < HD / 16; c0 += TOGETHER) {
-                unsigned b[TOGETHER][4];
-#pragma unroll
-                for (int c = 0; c < TOGETHER; ++c)
-                    if (c0 + c < HD / 16) ldmatrix_x4_trans(b[c], vt + ((lane & 7) + 8 * ((lane >> 3) & 1)) * LD + (c0 + c) * 16 + 8 * (lane >> 4));
-#pragma unroll
-                for (int c = 0; c < TOGETHER; ++c) {
-                    if (c0 + c >= HD / 16) break;
-                    mma_bf16(o[2 * (c0 + c)], p4, b[c][0], b[c][1]);
-                    mma_bf16(o[2 * (c0 + c) + 1], p4, b[c][2], b[c][3]);
-                }
-            }
-            if (now.bits >> 17 & 1) {
-                // ---- the stretch's triples
-                l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 1); l_lo += __shfl_xor_sync(0xffffffffu, l_lo, 2);
-                l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 1); l_hi += __shfl_xor_sync(0xffffffffu, l_hi, 2);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int r = g + 8 * half;
-                    if (r >= now.rows) continue;
-                    const size_t row = (size_t)now.slot * FEW + r;
-                    float* dst = a.part_o + row * HD;
-#pragma unroll
-                    for (int c = 0; c < HD / 8; ++c)
-                        *reinterpret_cast<float2*>(dst + c * 8 + 2 * t) = make_float2(o[c][2 * half], o[c][2 * half + 1]);
-                    if (t == 0) {
-                        const float m = half ? m_hi : m_lo;
-                        *reinterpret_cast<float2*>(a.part_ml + row * 2) = make_float2(m == -INFINITY ? m : m * a.scale, half ? l_hi : l_lo);
-                    }
-                }
-            }
+            state.step([&](int i) { return kt + ((lane & 7) + 8 * (lane >> 4)) * LD + i * 16 + 8 * ((lane >> 3) & 1); },
+                       [&](int c) { return vt + ((lane & 7) + 8 * ((lane >> 3) & 1)) * LD + c * 16 + 8 * (lane >> 4); },
+                       [&](int i, unsigned (&q4)[4]) {
+                           if constexpr (S::Q_IN_REGS) { q4[0] = qf[i][0]; q4[1] = qf[i][1]; q4[2] = qf[i][2]; q4[3] = qf[i][3]; }
+                           else ldmatrix_x4(q4, q_at + i * 16);
+                       }, now.bits, t, sc);
+            if (now.bits >> 17 & 1) state.leave(a, now.rows, now.slot, g, t);
             __syncwarp();                                 // the step's place in the ring may be filled again
         }
         now = next; next = behind;
@@ -965,7 +982,8 @@ constexpr int HALVES = HD / 64, ATOM = 128 * 128;        // 128-byte column halv
 constexpr int Q_BYTES = HALVES * ATOM, KV_BYTES = HALVES * ATOM;
 constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = STREAMS * KEYS;
 constexpr int STRETCHES = 32;                            // of a block's piece, worked out at once
-enum { ERR_TC_PRODUCER = 31, ERR_TC_MMA = 32, ERR_TC_SOFTMAX = 33, ERR_TC_LAYOUT = 34 };
+constexpr int BOX = 16;                                  // keys that a copy brings, where a page has as many
+enum { ERR_TC_PRODUCER = 31, ERR_TC_MMA = 32, ERR_TC_SOFTMAX = 33, ERR_TC_LAYOUT = 34, ERR_FEW = 39 };
 
 struct Control {
     uint64_t ring_full[SLOTS], ring_empty[SLOTS], s_full[STREAMS], p_ready[STREAMS], o_done[STREAMS], q_ready[STREAMS];
@@ -977,17 +995,25 @@ constexpr int CONTROL_BYTES = 2048;
 static_assert(sizeof(Control) <= CONTROL_BYTES, "control block");
 constexpr size_t SMEM = CONTROL_BYTES + STREAMS * Q_BYTES + SLOTS * KV_BYTES;
 
+// Two 32-bit numbers to an instruction, and the largest of three: the softmax warps wait for their turn to issue.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float x, float y) { Pair p; asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y)); return p; }
+__device__ __forceinline__ float2 apart(Pair p) { float2 v; asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(p)); return v; }
+__device__ __forceinline__ Pair fma2(Pair x, Pair y, Pair z) { Pair p; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p) : "l"(x), "l"(y), "l"(z)); return p; }
+__device__ __forceinline__ Pair add2(Pair x, Pair y) { Pair p; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y)); return p; }
+__device__ __forceinline__ float max3(float x, float y, float z) { float v; asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z)); return v; }
+
 __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtensorMap& v_map, const SharedArgs& a, const Plan& plan, unsigned char* smem_all) {
     Control& ctl = *reinterpret_cast<Control*>(smem_all);
     unsigned char* q_s = smem_all + CONTROL_BYTES;       // [stream][HALVES][128 rows][128 B]
     unsigned char* ring = q_s + STREAMS * Q_BYTES;       // [slot][HALVES][128 keys][128 B]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const Piece piece = piece_of<1>(a, plan, blockIdx.x);
-    if (piece.from == piece.end) return;
     if ((smem_addr(smem_all) & 1023) != 0) {             // the swizzle goes by addresses
         if (tid == 0) atomicExch(a.error, ERR_TC_LAYOUT);
         return;
     }
+    if (piece.from == piece.end) return;
     if (tid == 0) {
         for (int s = 0; s < SLOTS; ++s) { mbar_init(&ctl.ring_full[s], 1); mbar_init(&ctl.ring_empty[s], 1); }
         for (int st = 0; st < STREAMS; ++st) {
@@ -1026,13 +1052,13 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
             if (sr.steps == 0) break;
             const int tiles = sr.steps, streams = sr.rows > BM ? 2 : 1;
             if (warp == 0) {
-                // -------------------------------------------------------------- producer: lane j has page j of a tile
-                const int ps = a.page_size, pages_per_tile = KEYS / ps;
+                // -------------------------------------------------------------- producer: lane j has box j of a tile
+                const int ps = a.page_size, shift = __ffs(ps) - 1, box = min(ps, BOX), boxes = KEYS / box;
                 const long long rows_per_page = a.page_stride / HD;
                 const int* table = a.block_tables + (size_t)sr.table * a.table_width;
                 auto look_up = [&](int i) {               // beyond the keys any page will do: they count for nothing
-                    const int key = sr.k0 + i * KEYS + lane * ps;
-                    return lane < pages_per_tile && i < tiles && key < sr.kend ? table[key / ps] : 0;
+                    const int key = sr.k0 + i * KEYS + lane * box;
+                    return lane < boxes && i < tiles && key < sr.kend ? table[key >> shift] : 0;
                 };
                 int ahead = look_up(0);
                 for (int i = 0; i < tiles && ok; ++i) {
@@ -1051,9 +1077,9 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
                         if (!ok) break;
                         if (lane == 0) mbar_expect_tx(&ctl.ring_full[s], (uint32_t)KV_BYTES);
                         __syncwarp();
-                        if (lane < pages_per_tile) {
-                            unsigned char* dst = ring + (size_t)s * KV_BYTES + lane * ps * 128;
-                            const int row = (int)(page * rows_per_page + (long long)sr.kvh * ps);
+                        if (lane < boxes) {
+                            unsigned char* dst = ring + (size_t)s * KV_BYTES + lane * box * 128;
+                            const int row = (int)(page * rows_per_page + (long long)sr.kvh * ps) + (sr.k0 + lane * box & (ps - 1));
 #pragma unroll
                             for (int h = 0; h < HALVES; ++h) tma_load_2d(dst + h * ATOM, kv ? &v_map : &k_map, h * 64, row, &ctl.ring_full[s]);
                         }
@@ -1159,18 +1185,26 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const int from = sr.k0 + i * KEYS;
-                    uint32_t sv[KEYS];
+                    // (32 keys at a time, twice: a step alone, as a short prompt has it, waits for its instructions, which all
+                    // 128 in registers are four times as many of)
+                    const bool part = from < sr.begin || from + KEYS > sr.kend;
+                    auto scores = [&](int c, uint32_t (&sv)[32]) {
+                        tmem_ld32_issue(s_addr + c, sv);
+                        tmem_wait_ld();
+                        if (part) {
 #pragma unroll
-                    for (int c = 0; c < KEYS; c += 32) tmem_ld32_issue(s_addr + c, sv + c);
-                    tmem_wait_ld();
-                    if (from < sr.begin || from + KEYS > sr.kend) {
-#pragma unroll
-                        for (int j = 0; j < KEYS; ++j)
-                            if (from + j < sr.begin || from + j >= sr.kend) sv[j] = 0xff800000u;        // -inf
-                    }
+                            for (int j = 0; j < 32; ++j)
+                                if (from + c + j < sr.begin || from + c + j >= sr.kend) sv[j] = 0xff800000u;        // -inf
+                        }
+                    };
                     float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                    for (int c = 0; c < KEYS; c += 32) {
+                        uint32_t sv[32];
+                        scores(c, sv);
 #pragma unroll
-                    for (int j = 0; j < KEYS; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(sv[j]));
+                        for (int j = 0; j < 32; j += 2) mx4[j / 2 & 3] = max3(mx4[j / 2 & 3], __uint_as_float(sv[j]), __uint_as_float(sv[j + 1]));
+                    }
                     const float mx = valid ? fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) : -INFINITY;
                     // the reference point of the exponentials moves only when the maximum has grown by more than 2^8 since it was
                     // set: until then a weight may exceed 1, by at most that, and O and the row sum stay as they are
@@ -1190,19 +1224,24 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
                             tmem_wait_st();
                         }
                     }
-                    float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+                    Pair sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                    const Pair sc2 = pair(sc, sc), base2 = pair(-base, -base);
+#pragma unroll 1
+                    for (int c = 0; c < KEYS; c += 32) {  // (weights go over scores that are done with)
+                        uint32_t sv[32];
+                        scores(c, sv);
 #pragma unroll
-                    for (int j = 0; j < KEYS; j += 2) {
-                        const float p0 = fast_exp2(fmaf(__uint_as_float(sv[j]), sc, -base));
-                        const float p1 = fast_exp2(fmaf(__uint_as_float(sv[j + 1]), sc, -base));
-                        sum4[(j >> 1) & 1] += p0;
-                        sum4[2 + ((j >> 1) & 1)] += p1;
-                        sv[j >> 1] = pack_bf16(p0, p1);
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 x = apart(fma2(pair(__uint_as_float(sv[j]), __uint_as_float(sv[j + 1])), sc2, base2));
+                            const float p0 = fast_exp2(x.x), p1 = fast_exp2(x.y);
+                            sum2[(j >> 1) & 1] = add2(sum2[(j >> 1) & 1], pair(p0, p1));
+                            sv[j >> 1] = pack_bf16(p0, p1);
+                        }
+                        tmem_st16_issue(s_addr + c / 2, sv);
                     }
-#pragma unroll
-                    for (int c = 0; c < KEYS / 2; c += 32) tmem_st32_issue(s_addr + c, sv + c);
                     tmem_wait_st();
-                    l_run = l_run * corr + (valid ? (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]) : 0.f);
+                    const float2 sum = apart(add2(sum2[0], sum2[1]));
+                    l_run = l_run * corr + (valid ? sum.x + sum.y : 0.f);
                     m_run = m_new;
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     mbar_arrive(&ctl.p_ready[st_own]);
@@ -1247,13 +1286,166 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
     }
 }
 
-// Pages of keys or values as a matrix of HD columns, boxes of page_size rows x 64 columns, 128-byte swizzle.
+// Few rows: as few_phase, a warp a worker, but the copy engine brings a step's keys and values, so that a step costs neither 32
+// addresses nor copies of 16 bytes, and the queries come straight into registers, which leaves room for more workers.
+// 200 requests, 40 heads over 8 of 128, 32 to 512 keys of their own each: 34 us by copies of 16 bytes and as much
+// here, but 63 requests of 1,024 to 2,048 keys, 28 heads over 4, 50.6 and 45.9 in all (193 MB: 5.4 TB/s behind what such a call
+// takes with few keys).
+struct TmaFew {
+    static constexpr int KEYS = MMA_FEW_KEYS, STAGES = 3, AT_ONCE = 8;
+    static constexpr int HALF = KEYS * 128, STAGE = 2 * HALVES * HALF;                  // bytes: 64 columns of a step's keys; a stage
+    struct Worker { uint64_t full[STAGES]; Stretch stretches[AT_ONCE]; };
+    static constexpr int CONTROL = (sizeof(Worker) + 15) / 16 * 16;
+    static constexpr size_t WORKER = STAGES * STAGE + CONTROL;
+    static constexpr int FIT = (int)((227 * 1024 - CONTROL_BYTES) / WORKER);
+    // (a ninth leaves the second launch's blocks no room beside the first's: 8 requests of a 300-token prompt 13.0 us for 12.0 with
+    // seven; 64 requests with 512 keys in common 25.1 us with nine, 20.4 with eight, 25.8 with seven)
+    static constexpr int WORKERS = FIT < 8 ? FIT : 8;
+};
+
+__device__ __forceinline__ void few_phase(const CUtensorMap& k_map, const CUtensorMap& v_map, const SharedArgs& a, const Plan& plan, unsigned char* smem, int workers) {
+    using S = TmaFew;
+    constexpr int KEYS = S::KEYS, STAGES = S::STAGES;
+    if (threadIdx.x >= 32 * workers) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned char* ring = smem + warp * STAGES * S::STAGE;                // [stage][K, V][HALVES][KEYS][128 B], swizzled
+    S::Worker& own = *reinterpret_cast<S::Worker*>(smem + workers * STAGES * S::STAGE + warp * S::CONTROL);
+    // the blocks that have the fewest pieces of many rows come first
+    const Piece piece = piece_of<0>(a, plan, (gridDim.x - 1 - blockIdx.x) * workers + warp);
+    if (piece.from == piece.end) return;
+    if (lane == 0) {
+        for (int i = 0; i < STAGES; ++i) mbar_init(&own.full[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    const int group = a.group, tokens = a.tokens, num_pages = a.num_pages, page_size = a.page_size, shift = __ffs(page_size) - 1;
+    const int box = min(page_size, KEYS), boxes = KEYS / box, rows_per_page = (int)(a.page_stride / HD);
+    // ---- the walk: the step that comes next, and its pages, asked for a turn before its keys and values are
+    int k = -1, left = 0, k0 = 0;                         // stretch, steps left of it, the step's first key
+    bool first = false, more = true;
+    Stretch at = {};
+    int page = 0;                                         // lane j < boxes: of the step's j-th box
+    const int* table = a.block_tables;
+    auto look_up = [&]() {
+        if (!more) return;
+        first = left == 0;
+        if (first) {
+            if (++k % S::AT_ONCE == 0) {
+                __syncwarp();
+                if (lane < S::AT_ONCE) stretch_of<0>(a, plan, piece, k + lane, own.stretches[lane]);
+                __syncwarp();
+            }
+            at = own.stretches[k % S::AT_ONCE];
+            left = at.steps;
+            more = left > 0;
+            if (!more) return;
+            k0 = at.k0;
+            table = a.block_tables + (size_t)at.table * a.table_width;
+        } else {
+            k0 += KEYS;
+        }
+        --left;
+        const int key = k0 + lane * box;
+        page = lane < boxes && key < at.kend ? table[key >> shift] : -1;
+    };
+    // what a step needs when it has landed: bits 0 .. 15 its keys, 16 .. 18 first, last and valid; rows and slot; lane r: where
+    // row r of the queries lies
+    struct Landing { unsigned bits; int rows, slot; long long query; };
+    auto fetch = [&](int stage) {
+        Landing landing = {0u, 0, 0, 0};
+        if (!more) return landing;
+        const int key = k0 + lane * box;
+        const bool asked = lane < boxes && key < at.kend, there = asked && (unsigned)page < (unsigned)num_pages;
+        if (asked && !there) atomicExch(a.error, ERR_PAGE);
+        const unsigned missing = __ballot_sync(0xffffffffu, asked && !there);
+        unsigned keys = (0xffffu >> min(max(KEYS - (at.kend - k0), 0), KEYS)) & (0xffffu << max(at.begin - k0, 0));
+        if (missing) keys &= missing & 1 ? (missing & 2 ? 0u : 0xff00u) : 0x00ffu;
+        if (missing && boxes == 1) keys = 0u;
+        landing.bits = (keys & 0xffffu) | (first ? 1u << 16 : 0u) | (left == 0 ? 1u << 17 : 0u) | 1u << 18;
+        landing.rows = at.rows; landing.slot = at.slot;
+        if (lane == 0) mbar_expect_tx(&own.full[stage], (uint32_t)S::STAGE);
+        __syncwarp();
+        if (lane < boxes) {
+            // (a box that is not there: rows behind all pages, which arrive as zeros)
+            const int row = there ? page * rows_per_page + (at.kvh << shift) + (key & (page_size - 1)) : 0x7fffff00;
+            unsigned char* dst = ring + stage * S::STAGE + lane * box * 128;
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h) {
+                tma_load_2d(dst + h * S::HALF, &k_map, h * 64, row, &own.full[stage]);
+                tma_load_2d(dst + (HALVES + h) * S::HALF, &v_map, h * 64, row, &own.full[stage]);
+            }
+        }
+        if (first && lane < at.rows) {
+            const int row = at.row0 + lane, further = row < group ? 0 : row / group;
+            const int token = at.token >= 0 ? at.token : a.order[at.place + further];
+            if ((unsigned)token < (unsigned)tokens) landing.query = (long long)token * a.q_ld + (at.kvh * group + row - further * group) * HD;
+        }
+        return landing;
+    };
+
+    const int g = lane >> 2, t = lane & 3;
+    const float sc = a.scale * LOG2E;                     // scores in base-2 units
+    FewState state;
+    state.begin();
+    unsigned qf[HD / 16][4];
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) qf[i][0] = qf[i][1] = qf[i][2] = qf[i][3] = 0u;
+    // ldmatrix: this lane's row of 16 keys, and its 16-byte piece c of a row at 16 * (c ^ row % 8)
+    const int k_row = ((lane & 7) + 8 * (lane >> 4)) * 128, k_piece = ((lane >> 3) & 1) ^ (lane & 7);
+    const int v_row = ((lane & 7) + 8 * ((lane >> 3) & 1)) * 128, v_piece = (lane >> 4) ^ (lane & 7);
+    Landing now = {0u, 0, 0, 0}, next = {0u, 0, 0, 0};
+    static_assert(STAGES == 3, "landings held: this step's and the next two");
+    int stage = 1, parity = 0;                            // of the step n (in front of the first: those of step -2)
+    look_up();
+    for (int n = 1 - STAGES;; ++n) {                      // (the first turns only fetch)
+        if (n >= 0) {
+            if (!(now.bits >> 18)) break;
+            if (now.bits >> 16 & 1) {                     // a stretch begins: its queries, on their way beside the wait
+                state.begin();
+                const long long lo = __shfl_sync(0xffffffffu, now.query, g), hi = __shfl_sync(0xffffffffu, now.query, g + 8);
+                const unsigned *q_lo = reinterpret_cast<const unsigned*>((const bf16*)a.q + lo) + t, *q_hi = reinterpret_cast<const unsigned*>((const bf16*)a.q + hi) + t;
+#pragma unroll
+                for (int i = 0; i < HD / 16; ++i) { qf[i][0] = q_lo[8 * i]; qf[i][1] = q_hi[8 * i]; qf[i][2] = q_lo[8 * i + 4]; qf[i][3] = q_hi[8 * i + 4]; }
+            }
+            if (!__all_sync(0xffffffffu, mbar_wait(&own.full[stage], parity))) {
+                if (lane == 0) atomicExch(a.error, ERR_FEW);
+                for (int i = 1; i < STAGES; ++i) {        // copies on the way
+                    if (++stage == STAGES) { stage = 0; parity ^= 1; }
+                    if ((i == 1 ? next.bits : 0u) >> 18) mbar_wait(&own.full[stage], parity);
+                }
+                return;
+            }
+        }
+        const int ahead = stage == 0 ? STAGES - 1 : stage - 1;            // of step n + STAGES - 1
+        const Landing behind = fetch(ahead);
+        look_up();
+        if (n >= 0) {
+            unsigned char* kt = ring + stage * S::STAGE;
+            unsigned char* vt = kt + HALVES * S::HALF;
+            if ((now.bits & 0xffffu) != 0xffffu) {        // whatever lies behind the keys is multiplied with nothing
+                for (int e = lane; e < HALVES * KEYS * 8; e += 32)
+                    if (!(now.bits >> ((e >> 3) % KEYS) & 1)) *reinterpret_cast<uint4*>(vt + e * 16) = make_uint4(0, 0, 0, 0);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            }
+            state.step([&](int i) { return kt + (i >> 2) * S::HALF + k_row + ((k_piece ^ (2 * (i & 3))) << 4); },
+                       [&](int c) { return vt + (c >> 2) * S::HALF + v_row + ((v_piece ^ (2 * (c & 3))) << 4); },
+                       [&](int i, unsigned (&q4)[4]) { q4[0] = qf[i][0]; q4[1] = qf[i][1]; q4[2] = qf[i][2]; q4[3] = qf[i][3]; }, now.bits, t, sc);
+            if (now.bits >> 17 & 1) state.leave(a, now.rows, now.slot, g, t);
+            __syncwarp();                                 // the step's place in the ring may be filled again
+        }
+        if (++stage == STAGES) { stage = 0; if (n >= 0) parity ^= 1; }
+        now = next; next = behind;
+    }
+}
+
+// Pages of keys or values as a matrix of HD columns, boxes of up to 16 rows x 64 columns, 128-byte swizzle.
 static int pages_map(CUtensorMap& map, const void* pages, long long rows, int page_size) {
     EncodeTiled encode = encode_tiled();
     if (!encode) return ERR_UNSUPPORTED;
     const cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)rows};
     const cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)page_size};
+    const cuuint32_t box[2] = {64, (cuuint32_t)min(page_size, BOX)};
     const cuuint32_t elem[2] = {1, 1};
     const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(pages), dims, strides, box, elem,
                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1483,8 +1675,6 @@ __device__ __forceinline__ void merge_units(const SharedArgs& a, const Plan& pla
     }
 }
 
-// Few rows in all: a row to a unit and four warps on it, since what such a call waits for is one warp's chain of loads.  More:
-// what counts are instructions, and a warp takes several heads of a kv head together.
 constexpr int MERGE_WARPS = 4;
 template <typename T, int ROWS, int SPLIT>
 __global__ void __launch_bounds__(32 * MERGE_WARPS)
@@ -1521,7 +1711,7 @@ template <> struct Form<ON_MMA> {
 };
 #ifdef FSIE_SHARED_TC
 template <> struct Form<ON_TC> {
-    using Few = FewShape<tc::THREADS / 32, (int)MOST_SMEM - tc::CONTROL_BYTES>;
+    using Few = tc::TmaFew;
     static constexpr int THREADS = tc::THREADS, FEW_WORKERS = Few::WORKERS, FEW_KEYS = Few::KEYS, MANY_TILE = tc::ROWS, MANY_KEYS = tc::KEYS;
     static constexpr size_t SMEM = tc::SMEM, FEW_AT = tc::CONTROL_BYTES, WORKER_SMEM = Few::WORKER;
 };
@@ -1552,8 +1742,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 #ifdef FSIE_SHARED_TC
     else {
         tc::tc_phase(k_map, v_map, a, plan, smem);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // what was written there comes before the copies of the few
         __syncthreads();
-        few_phase<typename Form<FORM>::Few>(a, plan, smem + tc::CONTROL_BYTES, few_workers);
+        tc::few_phase(k_map, v_map, a, plan, smem + tc::CONTROL_BYTES, few_workers);
     }
 #endif
 }
@@ -1611,9 +1802,16 @@ static int launch(const Shape& shape, const CUtensorMap& k_map, const CUtensorMa
     return launch_dependent(shared_attention_kernel<FORM>, dim3(shape.blocks), dim3(Form<FORM>::THREADS), at + plan, stream, k_map, v_map, a, workers, (int)at);
 }
 
-// Few rows in all: a row to a unit and four warps on it, since what such a call waits for is one warp's chain of loads.  More:
-// what counts are instructions, and a warp takes several heads of a kv head together.  One block per multiprocessor finds
-// room beside the first launch's.
+// Few rows in all: a row to a unit and several warps on it, since what such a call waits for is one warp's chain of loads.
+// More: what counts are instructions, and a warp takes several heads of a kv head together.  The whole call in us, 28 heads over
+// 4 of 128, for <rows of a unit, warps on it>:
+//   requests x keys in common    rows    <1,4>  <1,2>  <2,2>  <8,1>
+//   8 x 4,096                     224     19.2   20.0   22.4   40.3
+//   16 x 1,024                    448     16.1   13.2   13.6   20.9
+//   32 x 1,024                    896     24.1   16.0   16.5   23.3
+//   64 x 2,048                  1,792     52.8   40.6   39.1   52.9
+//   128 x 128                   3,584     52.1   34.4   27.9   19.4
+// Up to four blocks to a multiprocessor.
 template <typename T, int ROWS, int SPLIT>
 static int launch_merge_as(const SharedArgs& a, int blocks, cudaStream_t stream) {
     const size_t smem = merge_smem<ROWS, SPLIT>() + plan_bytes(a.run_count);
@@ -1625,9 +1823,10 @@ static int launch_merge_as(const SharedArgs& a, int blocks, cudaStream_t stream)
 template <typename T>
 static int launch_merge(const SharedArgs& a, int blocks, cudaStream_t stream) {
     const long long rows = (long long)a.places * a.heads;
-    if (rows <= 2 * blocks) return launch_merge_as<T, 1, 4>(a, 2 * blocks, stream);
-    if (rows <= 16 * blocks) return launch_merge_as<T, 2, 1>(a, 2 * blocks, stream);
-    return launch_merge_as<T, 8, 1>(a, 2 * blocks, stream);
+    if (rows <= 2 * blocks) return launch_merge_as<T, 1, 4>(a, 4 * blocks, stream);
+    if (rows <= 6 * blocks) return launch_merge_as<T, 1, 2>(a, 4 * blocks, stream);
+    if (rows <= 16 * blocks) return launch_merge_as<T, 2, 2>(a, 4 * blocks, stream);
+    return launch_merge_as<T, 8, 1>(a, 4 * blocks, stream);
 }
 
 // Where everything lies in the room, for `lines` lines of many rows; returns the bytes.
@@ -1708,7 +1907,7 @@ int fsie_shared_attention(const void* q, int q_ld, const void* k_pages, const vo
     const long long of_line = (long long)shape.many_tile * (HD + 2) * 4;
     const long long lines = min((room_bytes - needed) / of_line, 0x7fffffffLL / shape.many_tile - shape.blocks - (a.many.row0 + shape.many_tile) / shape.many_tile);
     if (lay_out(shape, places, run_count, kv_heads, lines, (unsigned char*)room, a) < 0) return ERR_UNSUPPORTED;
-    a.many.align = on_tcgen05 ? page_size : 1;
+    a.many.align = a.few.align = on_tcgen05 ? min(page_size, 16) : 1;     // (a box of the copy engine)
     a.q = q; a.q_ld = q_ld; a.k_pages = k_pages; a.v_pages = v_pages; a.page_stride = page_stride; a.page_size = page_size;
     a.num_pages = num_pages; a.block_tables = block_tables; a.table_rows = table_rows; a.table_width = table_width;
     a.positions = positions; a.tokens = tokens; a.order = order; a.places = places; a.runs = runs; a.run_count = run_count;

@@ -162,9 +162,9 @@ class ModelRunner:
             self.layer_caches.append(cache)
         # cache groups some layer of which can read keys once for all requests that hold them
         self.shareable = [False] * len(self.cache.groups)
-        for (layer, _, _), cache in zip(model.schedule, self.layer_caches):
+        for (layer, _, _), cache in zip(model.schedule if shared_attention else (), self.layer_caches):
             takes = getattr(model.blocks[layer].mixer, "takes_shared_lists", None)
-            if shared_attention and cache.pages is not None and takes is not None and takes(dtype):
+            if cache.pages is not None and takes is not None and takes(dtype):
                 self.shareable[cache.group] = True
         if shared_attention and not any(self.shareable):
             raise ValueError("shared_attention: no layer of this model can read keys for several requests at once")
@@ -444,6 +444,7 @@ class ModelRunner:
                     37: "tcgen05 decode attention: scores or outputs never completed",
                     38: "tcgen05 decode attention: shared memory does not start on a 1,024-byte "
                         "boundary",
+                    39: "shared attention: keys of a few rows never arrived",
                     41: "tiled float32 product: the copy engine's stage never became free",
                     42: "tiled float32 product: a stage never arrived",
                     43: "tiled float32 product: a stage was never multiplied",

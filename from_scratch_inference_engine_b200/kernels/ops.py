@@ -2597,27 +2597,30 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
             _need(tensor, dtype, name, contiguous=False)
     if not shared_attention_takes(dtype, head_dim):
         raise KernelError(f"shared_attention: {dtype} with heads of {head_dim} is not taken")
-    if block_tables.dim() != 2 or runs.dim() != 2 or runs.shape[1] != 6 or order.dim() != 1 or own_run.shape != order.shape \
-            or positions.dim() != 1:
+    # (a shape or a stride asked for costs the host 0.13 us: each once)
+    table_shape, run_shape, places, token_shape = block_tables.shape, runs.shape, order.shape, positions.shape
+    if len(table_shape) != 2 or len(run_shape) != 2 or run_shape[1] != 6 or len(places) != 1 or own_run.shape != places \
+            or len(token_shape) != 1:
         raise KernelError("shared_attention: block_tables [requests, width], positions [tokens], order and own_run [n] and runs "
                           "[r, 6] are needed")
-    if runs.shape[0] > SHARED_ATTENTION_MAX_RUNS:
-        raise KernelError(f"shared_attention: {runs.shape[0]} runs, the kernels take {SHARED_ATTENTION_MAX_RUNS}")
+    if run_shape[0] > SHARED_ATTENTION_MAX_RUNS:
+        raise KernelError(f"shared_attention: {run_shape[0]} runs, the kernels take {SHARED_ATTENTION_MAX_RUNS}")
     if kv_heads <= 0 or heads <= 0 or heads % kv_heads or page_size <= 0 or not 0 < scale < float("inf"):
         raise KernelError("shared_attention: heads must be a multiple of kv_heads, page_size and scale positive")
-    tokens = positions.shape[0]
-    if q.dim() != 2 or out.dim() != 2 or min(q.shape[0], out.shape[0]) < tokens or q.stride(0) != q_ld or q.stride(1) != 1 \
-            or min(q.shape[1], out.shape[1]) < heads * head_dim or out.stride(1) != 1:
+    tokens, width = token_shape[0], heads * head_dim
+    q_shape, out_shape, out_stride = q.shape, out.shape, out.stride()
+    if len(q_shape) != 2 or len(out_shape) != 2 or q_shape[0] < tokens or out_shape[0] < tokens or q.stride() != (q_ld, 1) \
+            or q_shape[1] < width or out_shape[1] < width or out_stride[1] != 1:
         raise KernelError("shared_attention: q and out must hold a row of all heads for every token")
-    layout = (kv_heads, page_size, head_dim)
-    strides = (page_stride, page_size * head_dim, head_dim, 1)
-    if k_pages.shape[1:] != layout or v_pages.shape != k_pages.shape or k_pages.stride() != strides or v_pages.stride() != strides:
+    pages, strides = k_pages.shape, (page_stride, page_size * head_dim, head_dim, 1)
+    if len(pages) != 4 or pages != (pages[0], kv_heads, page_size, head_dim) or v_pages.shape != pages \
+            or k_pages.stride() != strides or v_pages.stride() != strides:
         raise KernelError("shared_attention: pages of keys and of values must be [pages, kv_heads, page_size, head_dim], "
                           "page_stride apart")
     _check(attn_shared(head_dim).fsie_shared_attention(
-        q, q_ld, k_pages, v_pages, page_stride, page_size, k_pages.shape[0], block_tables, block_tables.shape[0],
-        block_tables.shape[1], positions, tokens, order, order.shape[0], runs, runs.shape[0], own_run, out, out.stride(0), heads,
-        kv_heads, head_dim, float(scale), room, room.numel(), _tag(dtype), int(early), error, _stream()), "shared_attention")
+        q, q_ld, k_pages, v_pages, page_stride, page_size, pages[0], block_tables, table_shape[0], table_shape[1], positions,
+        tokens, order, places[0], runs, run_shape[0], own_run, out, out_stride[0], heads, kv_heads, head_dim, float(scale), room,
+        room.numel(), _tag(dtype), int(early), error, _stream()), "shared_attention")
     return out
 
 
