@@ -48,7 +48,9 @@ constexpr int MMA_FEW_KEYS = 16, MMA_MANY_KEYS = HD <= 128 ? 64 : 32, F32_KEYS =
 constexpr int MAX_RUNS = 768;
 constexpr int MAX_LEVELS = 32;           // runs that lie around each other, the innermost among them
 constexpr int RUN_INTS = 6;
-constexpr int LINE_PIECES = 128;         // a line is cut into no more pieces than this: what joins them reads them all
+// A line is cut into no more pieces than this: what joins them reads them all.  Two requests with 32,768 keys in common: 32 pieces
+// 97 us, 128 35, 256 29, 512 28; with 8,192 in common 128 19, 256 21.
+constexpr int LINE_PIECES = 256;
 constexpr int FEW_LEAST = 2, MANY_LEAST = 1;                              // steps of a piece, at least
 enum { ERR_PAGE = 3, ERR_RUNS = 7, ERR_ROOM = 8 };
 
