@@ -211,6 +211,10 @@ class _PlainCalls:
     def fits(tensor, dtype, contiguous) -> bool:
         return tensor.is_cuda and (dtype is None or tensor.dtype is dtype) and (not contiguous or tensor.is_contiguous())
 
+    @staticmethod
+    def on(device, *tensors) -> bool:
+        return all(tensor is None or tensor.get_device() == device for tensor in tensors)
+
 
 def host_call():
     """The extension module host_call.cpp, compiled at first use; `_PlainCalls` where that fails."""

@@ -9,7 +9,7 @@
 // integers and 8 floats (those that fit the registers: a ninth would take a place among the integers on the stack).
 //
 // fits(tensor, dtype, contiguous): whether a tensor lives on the GPU, has that dtype (None: any) and is contiguous
-// (False: need not be).
+// (False: need not be).  on(device, tensors...): whether all of them live on that GPU (None is passed over).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stddef.h>
@@ -35,7 +35,7 @@ struct Function {
     PyObject* name;
 };
 
-static PyObject *s_data_ptr, *s_is_cuda, *s_dtype, *s_is_contiguous;
+static PyObject *s_data_ptr, *s_is_cuda, *s_dtype, *s_is_contiguous, *s_get_device;
 
 // The integer an argument stands for; -1 with an exception set where it stands for none.
 static i64 integer_of(PyObject* arg) {
@@ -145,7 +145,26 @@ static PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyBool_FromLong(ok);
 }
 
-static PyMethodDef methods[] = {{"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+static PyObject* on(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    const long device = n > 0 ? PyLong_AsLong(args[0]) : -1;
+    if (n < 1 || (device == -1 && PyErr_Occurred())) {
+        if (n < 1) PyErr_SetString(PyExc_TypeError, "on takes a device's number and tensors");
+        return nullptr;
+    }
+    bool ok = true;
+    for (Py_ssize_t i = 1; ok && i < n; ++i) {
+        if (args[i] == Py_None) continue;
+        PyObject* number = PyObject_CallMethodNoArgs(args[i], s_get_device);
+        if (!number) return nullptr;
+        ok = PyLong_AsLong(number) == device;
+        Py_DECREF(number);
+        if (PyErr_Occurred()) return nullptr;
+    }
+    return PyBool_FromLong(ok);
+}
+
+static PyMethodDef methods[] = {{"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL, nullptr},
+                                {"on", (PyCFunction)(void (*)(void))on, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "host_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 PyMODINIT_FUNC PyInit_host_call(void) {
@@ -161,7 +180,8 @@ PyMODINIT_FUNC PyInit_host_call(void) {
     s_is_cuda = PyUnicode_InternFromString("is_cuda");
     s_dtype = PyUnicode_InternFromString("dtype");
     s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
-    if (!s_data_ptr || !s_is_cuda || !s_dtype || !s_is_contiguous) return nullptr;
+    s_get_device = PyUnicode_InternFromString("get_device");
+    if (!s_data_ptr || !s_is_cuda || !s_dtype || !s_is_contiguous || !s_get_device) return nullptr;
     PyObject* m = PyModule_Create(&module);
     if (!m) return nullptr;
     Py_INCREF(&FunctionType);

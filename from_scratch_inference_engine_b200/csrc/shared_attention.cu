@@ -22,14 +22,15 @@
 // stretch of a line that it has worked on in `room`:
 //
 //   many rows   tcgen05 (head sizes 64 and 128), mma.sync or FFMA: a worker is a block
-//   few rows    a worker is a warp (bfloat16) or a block (float32)
+//   few rows    a worker is a warp (bfloat16; fed by the copy engine beside tcgen05, by copies of 16 bytes beside mma.sync) or a
+//               block (float32)
 //
 // The second joins the triples of a row, in a fixed order; it makes its plan while the first still runs.
 //
 // What a small call waits for is a chain of reads of what other multiprocessors hold, 750 cycles each, and instructions that
 // run for the first time.  8 requests of a 4,096-token prompt, 28 heads over 4 of 128: 23.9 us with a launch for the plan in
 // front, one each for many and few rows and one for the merge; 31.5 in one cooperative launch whose blocks meet twice
-// (6 of them between two such launches); 20.7 as it is.
+// (6 of them between two such launches); 20.7 in two, and 16.0 since their code is shorter and more of their warps join.
 #include "common.cuh"
 #include "tma.cuh"
 #include "attention_tc.cuh"
@@ -985,6 +986,7 @@ constexpr int Q_BYTES = HALVES * ATOM, KV_BYTES = HALVES * ATOM;
 constexpr uint32_t TMEM_COLS = 512, COL_S = 0, COL_O = STREAMS * KEYS;
 constexpr int STRETCHES = 32;                            // of a block's piece, worked out at once
 constexpr int BOX = 16;                                  // keys that a copy brings, where a page has as many
+constexpr int NO_ROW = 0x7fffff00;                       // behind the rows of all pages
 enum { ERR_TC_PRODUCER = 31, ERR_TC_MMA = 32, ERR_TC_SOFTMAX = 33, ERR_TC_LAYOUT = 34, ERR_FEW = 39 };
 
 struct Control {
@@ -1369,7 +1371,7 @@ __device__ __forceinline__ void few_phase(const CUtensorMap& k_map, const CUtens
         __syncwarp();
         if (lane < boxes) {
             // (a box that is not there: rows behind all pages, which arrive as zeros)
-            const int row = there ? page * rows_per_page + (at.kvh << shift) + (key & (page_size - 1)) : 0x7fffff00;
+            const int row = there ? page * rows_per_page + (at.kvh << shift) + (key & (page_size - 1)) : NO_ROW;
             unsigned char* dst = ring + stage * S::STAGE + lane * box * 128;
 #pragma unroll
             for (int h = 0; h < HALVES; ++h) {
@@ -1754,9 +1756,9 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 struct Shape { int blocks, few_workers, few_keys, many_tile, many_keys; };       // (few_workers: of a block)
 constexpr int MAX_DEVICES = 64;
 
-static bool tcgen05_takes(int page_size, long long page_stride) {
+static bool tcgen05_takes(int page_size, long long page_stride, long long page_rows) {
 #ifdef FSIE_SHARED_TC
-    return (page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && page_stride % HD == 0;
+    return (page_size == 8 || page_size == 16 || page_size == 32 || page_size == 64 || page_size == 128) && page_stride % HD == 0 && page_rows <= tc::NO_ROW;
 #else
     return false;
 #endif
@@ -1866,7 +1868,7 @@ long long fsie_shared_attention_room(int places, int runs, int shared, int level
         return ERR_BAD_ARGUMENT;
     long long most = 0;
     for (int on_tcgen05 = 0; on_tcgen05 < 2; ++on_tcgen05) {        // (which of the two takes the call the pages decide)
-        if (on_tcgen05 && (dtype != DTYPE_BF16 || !tcgen05_takes(16, HD))) continue;
+        if (on_tcgen05 && (dtype != DTYPE_BF16 || !tcgen05_takes(16, HD, 0))) continue;
         Shape shape;
         const int rc = shape_of(dtype, on_tcgen05, shape);
         if (rc != 0) return rc > 0 ? -1000 - rc : rc;
@@ -1896,7 +1898,7 @@ int fsie_shared_attention(const void* q, int q_ld, const void* k_pages, const vo
         return ERR_BAD_ARGUMENT;
     if ((long long)places * heads > 0x7fffffffLL / 2) return ERR_UNSUPPORTED;
     const long long page_rows = num_pages > 0 ? (num_pages - 1) * (page_stride / HD) + (long long)kv_heads * page_size : 0;
-    const bool on_tcgen05 = dtype == DTYPE_BF16 && page_rows > 0 && page_rows < (1ll << 31) && run_count > 0 && tcgen05_takes(page_size, page_stride);
+    const bool on_tcgen05 = dtype == DTYPE_BF16 && page_rows > 0 && run_count > 0 && tcgen05_takes(page_size, page_stride, page_rows);
     Shape shape;
     int rc = shape_of(dtype, on_tcgen05, shape);
     if (rc != 0) return rc;

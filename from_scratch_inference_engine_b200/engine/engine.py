@@ -175,7 +175,7 @@ class Engine:
             seq.hold = len(prompt) - 1
             try:
                 while seq.handle is None or seq.handle.length < seq.hold:
-                    if self.step() == 0:
+                    if self._step() == 0:         # (what an `allowed` raises waits for the next `step`)
                         break
                 if seq.handle is not None and seq.handle.length == seq.hold:
                     count = max(0, min(len(rest), self.scheduler.max_batch - len(self.scheduler.running),
@@ -285,7 +285,7 @@ class Engine:
             mask = None if tokens is None else pack_allowed(tokens, self.runner.vocab_size)
             item.ends = mask is not None and not mask.any()
         except Exception as raised:                # the step is under way: it is recorded first
-            self._raised, item.ends = raised, True
+            self._raised, item.ends = self._raised or raised, True
         return None if item.ends else mask
 
     def _resolve(self, items, tokens) -> None:

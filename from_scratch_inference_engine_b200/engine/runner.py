@@ -45,6 +45,7 @@ class DeviceFault(RuntimeError):
 DECODE_BATCHES = (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512)
 TABLE_STEP = 64          # block tables of captured steps grow in steps of this many pages
 MOST_SHARED_RUNS, MOST_SHARED_LEVELS = 128, 4    # of a step; what working memory is sized by
+MOST_SHARED_PLACES = ops.SHARED_ATTENTION_MAX_RUNS - MOST_SHARED_RUNS
 NO_RUNS = SharedRuns(np.zeros(0, np.int32), np.zeros((0, 6), np.int32), np.zeros(0, np.int32), 0, 0, 0)
 
 
@@ -257,6 +258,11 @@ class ModelRunner:
         handle = cache.open(("reserve_step_memory", id(self)))
         try:
             self.model.reserve(tokens, self.max_step_items)
+            if any(self.shareable):
+                places = min(self.max_step_items, self.max_step_tokens, MOST_SHARED_PLACES)
+                for block in self.model.blocks:
+                    if hasattr(block.mixer, "reserve_shared_lists"):
+                        block.mixer.reserve_shared_lists(places, places + MOST_SHARED_RUNS, MOST_SHARED_RUNS, MOST_SHARED_LEVELS)
             self.step([StepEntry(handle, [0] * tokens, [tokens - 1])])
             torch.cuda.current_stream().synchronize()
         finally:
@@ -302,7 +308,7 @@ class ModelRunner:
             return found
         lengths = np.asarray(q_len)
         ones = np.nonzero(lengths == 1)[0]
-        if not 2 <= len(ones) <= ops.SHARED_ATTENTION_MAX_RUNS - MOST_SHARED_RUNS:
+        if not 2 <= len(ones) <= MOST_SHARED_PLACES:
             return found
         at = np.asarray(pos0, dtype=np.int64)[ones]
         for g, takes in enumerate(self.shareable):

@@ -56,7 +56,18 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _device() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
 _fits = build.host_call().fits
+_on = build.host_call().on
+
+
+def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A launch goes to the current device: its tensors must live there."""
+    if not _on(_device(), *tensors):
+        raise KernelError(f"{what}: the tensors must live on the current device, cuda:{_device()}")
 
 
 def _need(tensor: torch.Tensor, dtype, name: str, contiguous: bool = True) -> None:
@@ -2580,7 +2591,7 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
              to their positions.  The runs around it end in front of all of their tokens
 
     out [tokens, ..] gets the rows of the tokens in `order` (zeros for a token without keys); other rows stay as they are.
-    `room`: uint8, `shared_attention_room` bytes.  A run or token outside of what there is, or a shared run that reaches
+    `room`: uint8, `shared_attention_room` bytes, of no other call that may run at the same time.  A run or token outside of what there is, or a shared run that reaches
     beyond one of its tokens, sets error[0] to 7, a page outside the pool to 3 (its keys are left out), runs that nest
     deeper than `room` was made for to 8; the rows concerned hold no result.  `early`: the lists, tables and positions are
     older than the stream's last kernel."""
@@ -2595,6 +2606,7 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
     for tensor, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (out, "out")):
         if not _fits(tensor, dtype, False):
             _need(tensor, dtype, name, contiguous=False)
+    _here("shared_attention", q, k_pages, v_pages, block_tables, positions, order, runs, own_run, out, room, error)
     if not shared_attention_takes(dtype, head_dim):
         raise KernelError(f"shared_attention: {dtype} with heads of {head_dim} is not taken")
     # (a shape or a stride asked for costs the host 0.13 us: each once)
@@ -2655,6 +2667,7 @@ def count_tokens(tokens: torch.Tensor, slots: torch.Tensor, counts: torch.Tensor
             and _fits(seen, torch.int32, True) and _fits(error, torch.int32, True)):
         for tensor, name in ((tokens, "tokens"), (slots, "slots"), (counts, "counts"), (seen, "seen"), (error, "error")):
             _need(tensor, torch.int32, name)
+    _here("count_tokens", tokens, slots, counts, seen, error)
     _history_shapes("count_tokens", counts, seen)
     if tokens.shape != slots.shape or tokens.dim() != 1:
         raise KernelError("count_tokens: tokens and slots must be [n]")
@@ -2688,6 +2701,7 @@ def adjust_logits(logits: torch.Tensor, error: torch.Tensor, slots: Optional[tor
         _need(error, torch.int32, "error")
     if logits.dim() != 2:
         raise KernelError("adjust_logits: logits must be [rows, vocab]")
+    _here("adjust_logits", logits, error, slots, penalties, counts, seen, *(bias or ()), *(masks or ()))
     rows, vocab = logits.shape
     histories = biases = mask_count = 0
     if slots is not None:

@@ -142,12 +142,19 @@ class GqaAttention(Mixer):
             self._attend_shared(ctx, qkv, group, cache, out, lists)
         return rt.linear(out, self.w_o, None, "attention.o")
 
+    def reserve_shared_lists(self, places: int, runs: int, shared: int, levels: int) -> None:
+        """Take the working memory of steps with so many requests of one token, runs, shared ones and levels of them."""
+        if self.takes_shared_lists(self.runtime.dtype):
+            self._shared_room(places, runs, shared, levels)
+
+    def _shared_room(self, places: int, runs: int, shared: int, levels: int) -> torch.Tensor:
+        return self.runtime.buffer("attention.shared_room", 1, ops.shared_attention_room(
+            places, runs, levels, self.num_heads, self.num_kv_heads, self.head_dim, self.runtime.dtype, shared), torch.uint8).view(-1)
+
     def _attend_shared(self, ctx, qkv: torch.Tensor, group, cache: LayerCache, out: torch.Tensor, lists) -> None:
         """Attention of the requests of one token, with keys that several of them hold read once for all.  Behind `_attend`,
         whose 32-bit form may leave anything in these tokens' rows."""
-        room = ctx.runtime.buffer("attention.shared_room", 1, ops.shared_attention_room(
-            lists.order.shape[0], lists.runs.shape[0], lists.levels, self.num_heads, self.num_kv_heads, self.head_dim,
-            qkv.dtype, lists.shared), torch.uint8)
+        room = self._shared_room(lists.order.shape[0], lists.runs.shape[0], lists.shared, lists.levels)
         ops.shared_attention(qkv, qkv.stride(0), cache.k_pages, cache.v_pages, cache.page_stride, group.page_size,
                              group.block_tables, ctx.positions, lists.order, lists.runs, lists.own_run, out, self.num_heads,
                              self.num_kv_heads, self.head_dim, self.scale, room, ctx.error, early=True)

@@ -53,6 +53,14 @@ class ParallelMixers(Mixer):
     def state_need(self) -> Optional[StateNeed]:
         return self.left.state_need() or self.right.state_need()
 
+    def takes_shared_lists(self, dtype: torch.dtype) -> bool:
+        return self.left.takes_shared_lists(dtype) or self.right.takes_shared_lists(dtype)
+
+    def reserve_shared_lists(self, *sizes: int) -> None:
+        for mixer in (self.left, self.right):
+            if hasattr(mixer, "reserve_shared_lists"):
+                mixer.reserve_shared_lists(*sizes)
+
     def reserve(self, tokens: int, requests: int) -> None:
         self.left.reserve(tokens, requests)
         self.right.reserve(tokens, requests)

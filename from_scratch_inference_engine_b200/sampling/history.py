@@ -50,7 +50,7 @@ class TokenHistory:
             if len({request[0] for request in fresh}) != len(fresh):
                 raise ValueError("history: a request appears twice")
             self._grow(len(fresh))
-            taken = [self._free.pop() for _ in fresh]
+            taken = self._free[-len(fresh):][::-1]
             for slot in taken:                            # (what the last owner left)
                 self.counts[slot].zero_()
                 self.seen[slot].zero_()
@@ -63,6 +63,7 @@ class TokenHistory:
                     host[1] = np.repeat(np.asarray(taken, dtype=np.int32), lengths)
                     staged = self._ring.stage(host.reshape(-1), self.device).view(2, total)
                     ops.count_tokens(staged[0], staged[1], self.counts, self.seen, error, generated=generated)
+            del self._free[-len(fresh):]
             for (request, _, _), slot in zip(fresh, taken):
                 self._slot_of[request] = slot
         return [self._slot_of[request[0]] for request in requests]

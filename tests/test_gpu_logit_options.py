@@ -108,8 +108,11 @@ def test_the_sampler_refuses_what_it_cannot_do():
                           ([masked] * 2, dict(masks=[pack_allowed([1], 40)])), ([SamplingParams()] * 2, dict(slots=[0, 1], biases=[None]))):
         with pytest.raises(ValueError):
             sampler.sample_async(logits, params, [0, 0], [0, 0], error, **given)
+    with pytest.raises(ValueError, match="no token is allowed"):
+        sampler.sample_async(logits, [masked] * 2, [0, 0], [0, 0], error, masks=[pack_allowed([1], 40), pack_allowed([], 40)])
     with pytest.raises(ValueError):
         history.slots([(1, [2], []), (1, [2], [])], error)
+    assert len(history) == 0
     # a history of another vocabulary
     history.slots([(1, [2], []), (2, [], [])], error)
     with pytest.raises(Exception, match="vocabulary"):
@@ -232,6 +235,25 @@ def test_what_a_callback_raises(folders, pipeline):
         assert engine.output(rid) == alone.generate(prompt, params[0], 9)[:len(engine.output(rid))]
     engine.runner.cache.check()
     assert engine.runner.cache.slots.num_free == 8
+
+
+def test_what_a_callback_raises_while_another_request_is_sampled(folders):
+    """`add_samples` runs steps of other requests: it returns its ids, the next step raises.  Of two that raise in one step the
+    first comes out, both requests have ended."""
+    from from_scratch_inference_engine_b200 import SamplingParams, SeqStatus
+    engine = engine_for(folders["A"])
+
+    def breaks(output):
+        raise KeyError(f"after {len(output)}")
+    broken = [engine.add_request([5, 6, 7 + i], SamplingParams(temperature=0.0, allowed=breaks), 5) for i in range(2)]
+    prompt = helpers.random_ids(256, 40, 3)
+    ids = engine.add_samples(prompt, [SamplingParams(temperature=0.9, seed=i) for i in range(3)], 4)
+    assert len(ids) == 3
+    with pytest.raises(KeyError, match="after 0"):
+        engine.step()
+    engine.run_until_done()
+    assert [len(engine.output(i)) for i in ids] == [4, 4, 4]
+    assert all(engine.status(i) is SeqStatus.Finished and not engine.output(i) for i in broken)
 
 
 def test_options_are_refused_before_anything_is_kept(folders):

@@ -182,3 +182,15 @@ def test_answers_are_those_of_requests_alone(folders, blocks, pipeline, calls):
     alone = Engine(model, block_size=4, num_blocks=200, max_batch=8, max_step_tokens=16)
     for index, (rid, own) in enumerate(zip(ids, params)):
         assert engine.output(rid) == alone.generate(prompts[index >= 4], own, 9)
+
+
+def test_working_memory_is_taken_before_serving(folders, calls):
+    """A runner that has reserved its memory has that of steps outside of graphs, whose requests share and prompts run beside."""
+    runner = runner_of(folders["E"], "bfloat16", 16, graphs=False)
+    runner.reserve_step_memory(100)
+    room = runner.runtime._buffers["attention.shared_room", torch.uint8]
+    parent = runner.cache.open("parent")
+    step(runner, (parent, [3] * 70))
+    handles = [parent] + runner.fork(parent, list("bcdefg"))
+    step(runner, *[(handle, [5]) for handle in handles], (runner.cache.open("other"), [1, 2, 3]))
+    assert calls and runner.runtime._buffers["attention.shared_room", torch.uint8] is room

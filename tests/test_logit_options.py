@@ -27,8 +27,10 @@ def test_allowed_tokens_as_bits(vocab, kind):
 
 def test_allowed_tokens_that_are_none():
     assert not pack_allowed([], 50).any() and not pack_allowed(np.zeros(0, np.int64), 50).any()
+    assert pack_allowed(np.arange(50) % 7 == 3, 50).tolist() == pack_allowed(range(3, 50, 7), 50).tolist()
+    assert not pack_allowed(np.zeros(50, bool), 50).any()
     assert pack_allowed([7, 7, 7], 50).tolist() == [128, 0]              # twice is once
-    for wrong in ([50], [-1], [1.5], [[1, 2]], [True, False], ["a"], np.ones(50, bool)):
+    for wrong in ([50], [-1], [1.5], [[1, 2]], [True, False], ["a"], np.ones(49, bool), np.ones((1, 50), bool)):
         with pytest.raises(ValueError):
             pack_allowed(wrong, 50)
 
