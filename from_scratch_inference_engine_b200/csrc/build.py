@@ -212,8 +212,9 @@ class _PlainCalls:
         return tensor.is_cuda and (dtype is None or tensor.dtype is dtype) and (not contiguous or tensor.is_contiguous())
 
     @staticmethod
-    def on(device, *tensors) -> bool:
-        return all(tensor is None or tensor.get_device() == device for tensor in tensors)
+    def all_fit(device, dtype, contiguous, *tensors) -> bool:
+        return all(tensor is None or (tensor.get_device() == device and (dtype is None or tensor.dtype is dtype)
+                                      and (not contiguous or tensor.is_contiguous())) for tensor in tensors)
 
 
 def host_call():

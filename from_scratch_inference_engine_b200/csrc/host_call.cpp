@@ -9,7 +9,8 @@
 // integers and 8 floats (those that fit the registers: a ninth would take a place among the integers on the stack).
 //
 // fits(tensor, dtype, contiguous): whether a tensor lives on the GPU, has that dtype (None: any) and is contiguous
-// (False: need not be).  on(device, tensors...): whether all of them live on that GPU (None is passed over).
+// (False: need not be).  all_fit(device, dtype, contiguous, tensors...): the same of several in one call, on that GPU (None is passed
+// over).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stddef.h>
@@ -120,6 +121,24 @@ static void function_dealloc(PyObject* self) {
 
 static PyTypeObject FunctionType = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
+// Whether a tensor has that dtype and is contiguous where it is to be; -1 with an exception set.
+static int holds_and_lies(PyObject* tensor, PyObject* wanted, PyObject* is_to_be) {
+    bool ok = true;
+    if (wanted != Py_None) {
+        PyObject* dtype = PyObject_GetAttr(tensor, s_dtype);
+        if (!dtype) return -1;
+        ok = dtype == wanted;
+        Py_DECREF(dtype);
+    }
+    if (ok && is_to_be == Py_True) {
+        PyObject* contiguous = PyObject_CallMethodNoArgs(tensor, s_is_contiguous);
+        if (!contiguous) return -1;
+        ok = contiguous == Py_True;
+        Py_DECREF(contiguous);
+    }
+    return ok;
+}
+
 static PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 3) {
         PyErr_SetString(PyExc_TypeError, "fits takes a tensor, a dtype or None, and whether it is to be contiguous");
@@ -128,43 +147,35 @@ static PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyObject* tensor = args[0];
     PyObject* cuda = PyObject_GetAttr(tensor, s_is_cuda);
     if (!cuda) return nullptr;
-    bool ok = cuda == Py_True;
+    const bool ok = cuda == Py_True;
     Py_DECREF(cuda);
-    if (ok && args[1] != Py_None) {
-        PyObject* dtype = PyObject_GetAttr(tensor, s_dtype);
-        if (!dtype) return nullptr;
-        ok = dtype == args[1];
-        Py_DECREF(dtype);
-    }
-    if (ok && args[2] == Py_True) {
-        PyObject* contiguous = PyObject_CallMethodNoArgs(tensor, s_is_contiguous);
-        if (!contiguous) return nullptr;
-        ok = contiguous == Py_True;
-        Py_DECREF(contiguous);
-    }
-    return PyBool_FromLong(ok);
+    const int holds = ok ? holds_and_lies(tensor, args[1], args[2]) : 0;
+    return holds < 0 ? nullptr : PyBool_FromLong(holds);
 }
 
-static PyObject* on(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    const long device = n > 0 ? PyLong_AsLong(args[0]) : -1;
-    if (n < 1 || (device == -1 && PyErr_Occurred())) {
-        if (n < 1) PyErr_SetString(PyExc_TypeError, "on takes a device's number and tensors");
+static PyObject* all_fit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n < 3) {
+        PyErr_SetString(PyExc_TypeError, "all_fit takes a device's number, a dtype or None, whether they are to be contiguous, and tensors");
         return nullptr;
     }
-    bool ok = true;
-    for (Py_ssize_t i = 1; ok && i < n; ++i) {
+    const long device = PyLong_AsLong(args[0]);
+    if (device == -1 && PyErr_Occurred()) return nullptr;
+    int ok = 1;
+    for (Py_ssize_t i = 3; ok && i < n; ++i) {
         if (args[i] == Py_None) continue;
         PyObject* number = PyObject_CallMethodNoArgs(args[i], s_get_device);
         if (!number) return nullptr;
-        ok = PyLong_AsLong(number) == device;
+        const long lives_on = PyLong_AsLong(number);
         Py_DECREF(number);
-        if (PyErr_Occurred()) return nullptr;
+        if (lives_on == -1 && PyErr_Occurred()) return nullptr;
+        ok = lives_on == device ? holds_and_lies(args[i], args[1], args[2]) : 0;
+        if (ok < 0) return nullptr;
     }
     return PyBool_FromLong(ok);
 }
 
 static PyMethodDef methods[] = {{"fits", (PyCFunction)(void (*)(void))fits, METH_FASTCALL, nullptr},
-                                {"on", (PyCFunction)(void (*)(void))on, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+                                {"all_fit", (PyCFunction)(void (*)(void))all_fit, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef module = {PyModuleDef_HEAD_INIT, "host_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 PyMODINIT_FUNC PyInit_host_call(void) {

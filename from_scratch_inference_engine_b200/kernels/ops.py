@@ -61,12 +61,16 @@ def _device() -> int:
 
 
 _fits = build.host_call().fits
-_on = build.host_call().on
+_all_fit = build.host_call().all_fit
 
 
-def _here(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """A launch goes to the current device: its tensors must live there."""
-    if not _on(_device(), *tensors):
+def _need_all(what: str, dtype, contiguous: bool, **tensors: Optional[torch.Tensor]) -> None:
+    """Raise for the first of them that does not fit (None is passed over), or because one lives on another device than the
+    current one, which a launch goes to."""
+    for name, tensor in tensors.items():
+        if tensor is not None:
+            _need(tensor, dtype, name, contiguous)
+    if not _all_fit(_device(), dtype, contiguous, *tensors.values()):
         raise KernelError(f"{what}: the tensors must live on the current device, cuda:{_device()}")
 
 
@@ -2595,18 +2599,13 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
     beyond one of its tokens, sets error[0] to 7, a page outside the pool to 3 (its keys are left out), runs that nest
     deeper than `room` was made for to 8; the rows concerned hold no result.  `early`: the lists, tables and positions are
     older than the stream's last kernel."""
-    if not (_fits(block_tables, torch.int32, True) and _fits(positions, torch.int32, True) and _fits(order, torch.int32, True)
-            and _fits(runs, torch.int32, True) and _fits(own_run, torch.int32, True) and _fits(error, torch.int32, True)
-            and _fits(room, torch.uint8, True)):
-        for tensor, name in ((block_tables, "block_tables"), (positions, "positions"), (order, "order"), (runs, "runs"),
-                             (own_run, "own_run"), (error, "error")):
-            _need(tensor, torch.int32, name)
-        _need(room, torch.uint8, "room")
-    dtype = q.dtype
-    for tensor, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (out, "out")):
-        if not _fits(tensor, dtype, False):
-            _need(tensor, dtype, name, contiguous=False)
-    _here("shared_attention", q, k_pages, v_pages, block_tables, positions, order, runs, own_run, out, room, error)
+    dtype, device = q.dtype, _device()
+    if not (_all_fit(device, torch.int32, True, block_tables, positions, order, runs, own_run, error)
+            and _all_fit(device, dtype, False, q, k_pages, v_pages, out) and _all_fit(device, torch.uint8, True, room)):
+        _need_all("shared_attention", torch.int32, True, block_tables=block_tables, positions=positions, order=order, runs=runs,
+                  own_run=own_run, error=error)
+        _need_all("shared_attention", dtype, False, q=q, k_pages=k_pages, v_pages=v_pages, out=out)
+        _need_all("shared_attention", torch.uint8, True, room=room)
     if not shared_attention_takes(dtype, head_dim):
         raise KernelError(f"shared_attention: {dtype} with heads of {head_dim} is not taken")
     # (a shape or a stride asked for costs the host 0.13 us: each once)
@@ -2663,21 +2662,21 @@ def count_tokens(tokens: torch.Tensor, slots: torch.Tensor, counts: torch.Tensor
     """Take tokens[i] into the history slots[i] (int32 [n]; -1: into none): its bit of seen (int32 [histories, bit_words(vocab)])
     is set and, if the tokens were generated, its place in counts (int32 [histories, vocab]) goes up by one.  A token
     outside the vocabulary or a history that does not exist is left out and sets error[0] (int32)."""
-    if not (_fits(tokens, torch.int32, True) and _fits(slots, torch.int32, True) and _fits(counts, torch.int32, True)
-            and _fits(seen, torch.int32, True) and _fits(error, torch.int32, True)):
-        for tensor, name in ((tokens, "tokens"), (slots, "slots"), (counts, "counts"), (seen, "seen"), (error, "error")):
-            _need(tensor, torch.int32, name)
-    _here("count_tokens", tokens, slots, counts, seen, error)
-    _history_shapes("count_tokens", counts, seen)
-    if tokens.shape != slots.shape or tokens.dim() != 1:
+    if not _all_fit(_device(), torch.int32, True, tokens, slots, counts, seen, error):
+        _need_all("count_tokens", torch.int32, True, tokens=tokens, slots=slots, counts=counts, seen=seen, error=error)
+    histories, vocab = _history_shapes("count_tokens", counts, seen)
+    shape = tokens.shape
+    if slots.shape != shape or len(shape) != 1:
         raise KernelError("count_tokens: tokens and slots must be [n]")
-    _check(logits_lib().fsie_count_tokens(tokens, slots, tokens.shape[0], counts.shape[1], counts.shape[0], counts, seen,
-                                          int(generated), error, _stream()), "count_tokens")
+    _check(logits_lib().fsie_count_tokens(tokens, slots, shape[0], vocab, histories, counts, seen, int(generated), error, _stream()),
+           "count_tokens")
 
 
-def _history_shapes(what: str, counts: torch.Tensor, seen: torch.Tensor) -> None:
-    if counts.dim() != 2 or seen.dim() != 2 or seen.shape != (counts.shape[0], bit_words(counts.shape[1])):
+def _history_shapes(what: str, counts: torch.Tensor, seen: torch.Tensor) -> Tuple[int, int]:
+    shape = counts.shape
+    if len(shape) != 2 or seen.shape != (shape[0], bit_words(shape[1])):
         raise KernelError(f"{what}: counts must be [histories, vocab] and seen [histories, words of 32 bits]")
+    return shape
 
 
 def adjust_logits(logits: torch.Tensor, error: torch.Tensor, slots: Optional[torch.Tensor] = None,
@@ -2696,40 +2695,35 @@ def adjust_logits(logits: torch.Tensor, error: torch.Tensor, slots: Optional[tor
 
     A history or a mask that does not exist counts as none, a token of a bias outside the vocabulary or out of order is
     left out; each sets error[0] (int32)."""
-    if not (_fits(logits, torch.float32, True) and _fits(error, torch.int32, True)):
-        _need(logits, torch.float32, "logits")
-        _need(error, torch.int32, "error")
-    if logits.dim() != 2:
+    device = _device()
+    if not (_all_fit(device, torch.float32, True, logits, penalties) and _all_fit(device, torch.int32, True, error, slots, counts, seen)):
+        _need_all("adjust_logits", torch.float32, True, logits=logits, penalties=penalties)
+        _need_all("adjust_logits", torch.int32, True, error=error, slots=slots, counts=counts, seen=seen)
+    shape = logits.shape
+    if len(shape) != 2:
         raise KernelError("adjust_logits: logits must be [rows, vocab]")
-    _here("adjust_logits", logits, error, slots, penalties, counts, seen, *(bias or ()), *(masks or ()))
-    rows, vocab = logits.shape
+    rows, vocab = shape
     histories = biases = mask_count = 0
     if slots is not None:
         if penalties is None or counts is None or seen is None:
             raise KernelError("adjust_logits: slots go with penalties, counts and seen")
-        for tensor, dtype, name in ((slots, torch.int32, "slots"), (penalties, torch.float32, "penalties"),
-                                    (counts, torch.int32, "counts"), (seen, torch.int32, "seen")):
-            if not _fits(tensor, dtype, True):
-                _need(tensor, dtype, name)
-        _history_shapes("adjust_logits", counts, seen)
-        if slots.shape != (rows,) or penalties.shape != (rows, 3) or counts.shape[1] != vocab:
+        histories, counted = _history_shapes("adjust_logits", counts, seen)
+        if slots.shape != (rows,) or penalties.shape != (rows, 3) or counted != vocab:
             raise KernelError("adjust_logits: a slot, three penalties and counts of the vocabulary are needed for every row")
-        histories = counts.shape[0]
     start = token = value = None
     if bias is not None:
         start, token, value = bias
-        for tensor, dtype in ((start, torch.int32), (token, torch.int32), (value, torch.float32)):
-            if not _fits(tensor, dtype, True):
-                _need(tensor, dtype, "bias")
+        if not (_all_fit(device, torch.int32, True, start, token) and _all_fit(device, torch.float32, True, value)):
+            _need_all("adjust_logits", torch.int32, True, bias_start=start, bias_token=token)
+            _need_all("adjust_logits", torch.float32, True, bias_value=value)
         if start.shape != (rows + 1,) or token.dim() != 1 or token.shape != value.shape:
             raise KernelError("adjust_logits: a bias is [rows + 1] starts, [n] tokens and [n] values")
         biases = token.shape[0]
     mask_of = bits = None
     if masks is not None:
         mask_of, bits = masks
-        if not (_fits(mask_of, torch.int32, True) and _fits(bits, torch.int32, True)):
-            _need(mask_of, torch.int32, "masks")
-            _need(bits, torch.int32, "masks")
+        if not _all_fit(device, torch.int32, True, mask_of, bits):
+            _need_all("adjust_logits", torch.int32, True, mask_of=mask_of, masks=bits)
         if mask_of.shape != (rows,) or bits.dim() != 2 or bits.shape[1] != bit_words(vocab):
             raise KernelError("adjust_logits: masks are [rows] indices and [m, words of 32 bits]")
         mask_count = bits.shape[0]
