@@ -380,7 +380,8 @@ struct Feed {
     }
     // first steps; false: nothing to do
     __device__ bool start() {
-        piece = piece_of<!IS_FEW>(a, plan, blockIdx.x);
+        // few rows from the last block on: it has the fewest pieces of many rows
+        piece = piece_of<!IS_FEW>(a, plan, IS_FEW ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         if (piece.from == piece.end) return false;
         if (threadIdx.x == 0) {
             stretches = at = 0;
