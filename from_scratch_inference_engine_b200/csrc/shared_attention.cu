@@ -55,9 +55,28 @@ constexpr int LINE_PIECES = 256;
 constexpr int FEW_LEAST = 2, MANY_LEAST = 1;                              // steps of a piece, at least
 enum { ERR_PAGE = 3, ERR_RUNS = 7, ERR_ROOM = 8 };
 
+// Division by a number that the host knows, for dividends below 2^31: a product's upper half, a sum and a shift (Granlund and
+// Montgomery, Division by invariant integers using multiplication, 1994).  A division by any number is some forty instructions,
+// and a call of few steps waits for every one of them, which runs for the first time.
+struct Div {
+    unsigned factor; int shift;
+    __device__ __forceinline__ int of(int n) const { return (int)((__umulhi(factor, (unsigned)n) + (unsigned)n) >> shift); }
+};
+static int log2_of(int n) { int shift = 0; while (1 << shift < n) ++shift; return shift; }
+static Div div_by(long long d) {
+    int shift = 0;
+    while ((1LL << shift) < d) ++shift;
+    return {(unsigned)(((1ULL << 32) * ((1ULL << shift) - (unsigned long long)d)) / (unsigned long long)d + 1), shift};
+}
+
 // One side of the plan: the runs of few rows or of many.
 struct Side {
-    int workers, line_room, tile, keys, align, least;         // (align: where steps begin, a power of two)
+    int workers, line_room, tile, keys, align, least;         // (align: where steps begin; it, tile and keys are powers of two)
+    int tile_shift, key_shift;
+    int tokens, parts;                   // tokens of a shared run's tile; tiles of a token, where there are several
+    Div by_tokens, by_parts, by_workers;
+    int of_block;                        // (few) workers of a block
+    int fixed, of_step;                  // (few) tenths of steps in whose time a worker's block does a piece of many rows: to begin, per step
     long long row0;                      // the triples of stretch s are rows row0 + s * tile ..
 };
 
@@ -74,6 +93,8 @@ struct SharedArgs {
     Side few, many;
     float* part_ml; float* part_o;                            // the triples: [rows, 2], [rows, HD]
     int early;                                                // the lists are older than the stream's last kernel
+    int most_steps;                                           // of a run, so that no sum of all passes 2^31
+    Div by_kv_heads, by_group, by_chunks, by_place;           // (the last two: see the join)
     int* error;
 };
 
@@ -84,11 +105,8 @@ enum { RUN_INNERMOST = 1, RUN_FEW = 2 };
 // Tiles of up to `most` rows.  One holds whole tokens (in an innermost run a single one), or, of a group that is larger, a
 // part of one token: so all rows of a token and kv head that lie in one tile lie side by side, here and in what is left for
 // the merge.
-struct Tiling { int tokens, parts; };    // tokens of a tile; tiles of a token, where there are several
-__device__ __forceinline__ Tiling tiling(const SharedArgs& a, int kind, int most) {
-    if (a.group > most) return {1, (a.group + most - 1) / most};
-    return {kind & RUN_INNERMOST ? 1 : most / a.group, 1};
-}
+__device__ __forceinline__ int line_steps(const Run& run, const Side& side) { return ((run.end - (run.begin & ~(side.align - 1)) - 1) >> side.key_shift) + 1; }
+__device__ __forceinline__ int tile_tokens(const Side& side, int kind) { return kind & RUN_INNERMOST ? 1 : side.tokens; }
 
 // What every block keeps in shared memory.
 struct Plan {
@@ -96,6 +114,7 @@ struct Plan {
     int *sums, stride;                   // see line0 and step0
     unsigned char* kind;
     int few_piece, many_piece, few_total, many_total, few_lines, many_lines;      // steps of a piece, steps and lines in all
+    int free_workers, free_piece;        // few: the first workers, whose blocks have no piece of many, and the steps of their pieces
     // [run_count + 1] lines and steps in front of each run, few (0) and many (1)
     __device__ __forceinline__ int* line0(int many) const { return sums + many * stride; }
     __device__ __forceinline__ int* step0(int many) const { return sums + (2 + many) * stride; }
@@ -139,11 +158,10 @@ __device__ __forceinline__ bool make_plan(const SharedArgs& a, unsigned char* sm
                 kind = run_kind(a, run, r);
                 const int many = kind & RUN_FEW ? 0 : 1;
                 const Side& side = many ? a.many : a.few;
-                const Tiling t = tiling(a, kind, side.tile);
-                const int of_line = (run.end - (run.begin & ~(side.align - 1)) - 1) / side.keys + 1;
-                const int lines = (t.tokens == 1 ? run.count * t.parts : (run.count - 1) / t.tokens + 1) * a.kv_heads;
+                const int of_line = line_steps(run, side);
+                const int lines = (tile_tokens(side, kind) == 1 ? run.count * side.parts : side.by_tokens.of(run.count - 1) + 1) * a.kv_heads;
                 const long long steps = (long long)lines * of_line;
-                overflow = overflow || max(steps, (long long)lines) > 0x7fffffff / a.run_count;       // (so no sum does)
+                overflow = overflow || max(steps, (long long)lines) > a.most_steps;
                 mine[many] = lines; mine[2 + many] = (int)steps;
                 longest[many] = max(longest[many], of_line);
             }
@@ -188,10 +206,39 @@ __device__ __forceinline__ bool make_plan(const SharedArgs& a, unsigned char* sm
         const int l = __reduce_max_sync(0xffffffffu, lane < PLAN_THREADS / 32 ? s.longest[i][lane] : 0);
         (i ? plan.many_lines : plan.few_lines) = before[i];
         (i ? plan.many_total : plan.few_total) = before[2 + i];
-        (i ? plan.many_piece : plan.few_piece) = max((before[2 + i] + side.workers - 1) / side.workers, max(side.least, (l + LINE_PIECES - 1) / LINE_PIECES));
+        const int least = max(side.least, (l + LINE_PIECES - 1) / LINE_PIECES);
+        (i ? plan.many_piece : plan.few_piece) = max(side.by_workers.of(max(before[2 + i] - 1, 0)) + 1, least);
+        if (i == 0) plan.free_piece = least;
         fits = fits && before[i] <= side.line_room;
     }
     if (!fits && tid == 0) atomicExch(a.error, ERR_ROOM);
+    // ---- blocks without a piece of many rows take more of the few, so that all are done at about the same time.  (Whole numbers:
+    // every block of both launches comes to the same.)
+    plan.free_workers = 0;
+    const int least = plan.free_piece, blocks = a.many.workers, of_block = a.few.of_block;
+    if (plan.many_total == 0 || plan.many_piece > 4096 || plan.few_total > 1 << 30) return fits;
+    // (the few go to the last blocks first: where the least pieces of them find room on blocks without many, all is well)
+    if (plan.many_piece == 1 && plan.few_total <= (blocks - plan.many_total) * of_block * least) return fits;
+    if (plan.many_piece <= 2) {                           // pieces of 2 or 4 steps on fewer blocks: what it takes to begin weighs less
+        long long best = 0x7fffffffffffffffLL;
+        int piece = 0;
+#pragma unroll
+        for (int shift = 0; shift < 3; ++shift) {
+            const int later = a.few.fixed + (a.few.of_step << shift), busy = ((plan.many_total - 1) >> shift) + 1;
+            const long long until = max((long long)later * a.few.workers, 10LL * plan.few_total + (long long)busy * of_block * later);
+            if (1 << shift >= plan.many_piece && until < best) { best = until; piece = 1 << shift; }
+        }
+        plan.many_piece = piece;
+    }
+    const int busy = (plan.many_total - 1) / plan.many_piece + 1, free_workers = (blocks - busy) * of_block;
+    if (free_workers > 0) {
+        const int later = (a.few.fixed + a.few.of_step * plan.many_piece + 9) / 10;
+        const int alone = max((plan.few_total + free_workers - 1) / free_workers, least);
+        const int all = a.few.by_workers.of(plan.few_total + busy * of_block * later - 1) + 1;
+        plan.free_workers = free_workers;
+        plan.few_piece = alone <= later + least ? 0 : max(all - later, least);           // (0: the others have none)
+        plan.free_piece = plan.few_piece == 0 ? alone : plan.few_piece + later;
+    }
     return fits;
 }
 
@@ -213,20 +260,32 @@ __device__ __forceinline__ int find_run(const int* at, int count, int value) {
     }
     return low;
 }
-__device__ __forceinline__ int line_steps(const Run& run, const Side& side) { return (run.end - (run.begin & ~(side.align - 1)) - 1) / side.keys + 1; }
 
 template <int MANY>
 __device__ __forceinline__ Piece piece_of(const SharedArgs& a, const Plan& plan, int worker) {
     const Side& side = MANY ? a.many : a.few;
     const int step_piece = MANY ? plan.many_piece : plan.few_piece, total = MANY ? plan.many_total : plan.few_total;
     Piece piece = {0, 0, 0, worker};
-    const long long from = (long long)worker * step_piece;
-    if (from >= total) return piece;
+    long long from = (long long)worker * step_piece;
+    int size = step_piece;
+    if (!MANY && plan.free_workers > 0) {
+        const int further = max(worker - plan.free_workers, 0);
+        from = (long long)(worker - further) * plan.free_piece + (long long)further * step_piece;
+        if (worker < plan.free_workers) size = plan.free_piece;
+    }
+    if (from >= total || size == 0) return piece;
     piece.from = (int)from;
-    piece.end = piece.from + min(step_piece, total - piece.from);
+    piece.end = piece.from + min(size, total - piece.from);
     const int r = find_run(plan.step0(MANY), a.run_count, piece.from);
     piece.first_line = plan.line0(MANY)[r] + (piece.from - plan.step0(MANY)[r]) / line_steps(plan.runs[r], side);
     return piece;
+}
+// the worker whose piece a step lies in
+__device__ __forceinline__ int piece_at(const Plan& plan, int many, int step) {
+    if (many) return step / plan.many_piece;
+    const long long free_steps = (long long)plan.free_workers * plan.free_piece;
+    if (step < free_steps) return step / plan.free_piece;
+    return plan.free_workers + (int)(step - free_steps) / plan.few_piece;
 }
 template <int MANY>
 __device__ __forceinline__ void stretch_of(const SharedArgs& a, const Plan& plan, const Piece& piece, int k, Stretch& n) {
@@ -239,17 +298,16 @@ __device__ __forceinline__ void stretch_of(const SharedArgs& a, const Plan& plan
     const int kind = plan.kind[r], line = number - plan.line0(MANY)[r], of_line = line_steps(run, side), begin = plan.step0(MANY)[r] + line * of_line;
     const int first = max(begin, piece.from), last = min(begin + of_line, piece.end);
     if (first >= last) return;
-    const Tiling t = tiling(a, kind, side.tile);
-    const int tile = line / a.kv_heads;
+    const int tokens = tile_tokens(side, kind), tile = a.by_kv_heads.of(line);
     n.kvh = line - tile * a.kv_heads;
-    const int token = t.parts > 1 ? tile / t.parts : tile * t.tokens;
+    const int token = side.parts > 1 ? side.by_parts.of(tile) : tile * tokens;
     n.place = run.first + token;
-    n.row0 = t.parts > 1 ? (tile - token * t.parts) * side.tile : 0;
-    n.rows = min(side.tile, t.parts > 1 ? a.group - n.row0 : min(t.tokens, run.count - token) * a.group);
+    n.row0 = side.parts > 1 ? (tile - token * side.parts) * side.tile : 0;
+    n.rows = min(side.tile, side.parts > 1 ? a.group - n.row0 : min(tokens, run.count - token) * a.group);
     n.k0 = (run.begin & ~(side.align - 1)) + (first - begin) * side.keys;
     n.begin = run.begin; n.kend = run.end; n.table = run.table;
     n.slot = number + piece.worker;
-    n.token = t.tokens == 1 ? a.order[n.place] : -1;
+    n.token = tokens == 1 ? a.order[n.place] : -1;
     if (kind & RUN_INNERMOST) {
         const int position = (unsigned)n.token < (unsigned)a.tokens ? a.positions[n.token] : -1;
         if (position < run.end) n.kend = position + 1;
@@ -369,7 +427,7 @@ struct Feed {
                 const T* q = (const T*)a.q;
 #pragma unroll 1
                 for (int e = threadIdx.x; e < ROWS * PIECES; e += THREADS) {
-                    const int r = e / PIECES, c = (e - r * PIECES) * EACH, row = st.of.row0 + r, further = row / a.group;
+                    const int r = e / PIECES, c = (e - r * PIECES) * EACH, row = st.of.row0 + r, further = a.by_group.of(row);
                     const int token = r < st.of.rows ? a.order[st.of.place + further] : -1;
                     const bool ok = (unsigned)token < (unsigned)a.tokens;
                     copy16(qd + r * Q_LD + c, q + (ok ? (long long)token * a.q_ld + (st.of.kvh * a.group + row - further * a.group) * HD + c : 0), ok);
@@ -1166,7 +1224,7 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
                 // ---- the queries, K-major and swizzled (zero beyond the tile's rows); all S of the stretch before are done
                 long long mine = -1;
                 if (valid) {
-                    const int row = sr.row0 + st_own * BM + r, further = row / a.group, token = a.order[sr.place + further];
+                    const int row = sr.row0 + st_own * BM + r, further = a.by_group.of(row), token = a.order[sr.place + further];
                     if ((unsigned)token < (unsigned)a.tokens) mine = (long long)token * a.q_ld + (sr.kvh * a.group + row - further * a.group) * HD;
                 }
                 constexpr int CHUNKS = HD / 8, AT_ONCE = 32 / CHUNKS;     // 16-byte pieces of a row; rows that a warp copies at once
@@ -1491,7 +1549,7 @@ __device__ __forceinline__ void merge_units(const SharedArgs& a, const Plan& pla
     const int per_place = a.kv_heads * chunks, units = a.places * per_place;
     bool waited = false;
     for (int unit = blockIdx.x * TEAMS + team; unit < units; unit += gridDim.x * TEAMS) {
-    const int place = unit / per_place, in_place = unit - place * per_place, kvh = in_place / chunks, g0 = (in_place - kvh * chunks) * ROWS;
+    const int place = a.by_place.of(unit), in_place = unit - place * per_place, kvh = a.by_chunks.of(in_place), g0 = (in_place - kvh * chunks) * ROWS;
     const int rows = min(ROWS, a.group - g0);
     const int token = a.order[place];
     int r = a.own_run[place], levels = 0, own_level = -1;
@@ -1512,12 +1570,12 @@ __device__ __forceinline__ void merge_units(const SharedArgs& a, const Plan& pla
             const int kind = plan.kind[own_level], many = kind & RUN_FEW ? 0 : 1;
             const Side& side = many ? a.many : a.few;
             tile_rows = side.tile;
-            const Tiling t = tiling(a, kind, tile_rows);
-            const int token_in = place - run.first, part = t.parts > 1 ? g0 / tile_rows : 0, tile = t.parts > 1 ? token_in * t.parts + part : token_in / t.tokens;
-            const int row = t.parts > 1 ? g0 - part * tile_rows : (token_in - tile * t.tokens) * a.group + g0;
+            const int token_in = place - run.first, tokens = tile_tokens(side, kind), part = side.parts > 1 ? g0 >> side.tile_shift : 0;
+            const int tile = side.parts > 1 ? token_in * side.parts + part : tokens == 1 ? token_in : side.by_tokens.of(token_in);
+            const int row = side.parts > 1 ? g0 - part * tile_rows : (token_in - tile * tokens) * a.group + g0;
             const int line = tile * a.kv_heads + kvh, of_line = line_steps(run, side), from = plan.step0(many)[own_level] + line * of_line;
-            const int steps = many ? plan.many_piece : plan.few_piece, b0 = from / steps;
-            count = (from + of_line - 1) / steps - b0 + 1;
+            const int b0 = piece_at(plan, many, from);
+            count = piece_at(plan, many, from + of_line - 1) - b0 + 1;
             first_at = (int)side.row0 + (plan.line0(many)[own_level] + line + b0) * tile_rows + row;
             // (a shared run ends in front of its tokens)
             if (!(kind & RUN_INNERMOST) && run.end - 1 > position) atomicExch(a.error, ERR_RUNS);
@@ -1703,22 +1761,30 @@ static_assert(F32Few::ROWS == FEW, "tiles of few rows");
 enum { ON_F32, ON_MMA, ON_TC };
 constexpr size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
 constexpr size_t MOST_SMEM = 227 * 1024;
+// FIXED, OF_STEP: see Side.  Equal pieces for all / these, us in a graph, 28 heads over 4, requests x keys in common and of their own:
+//   tcgen05   32 x 1,024 + 1,024  28.5 / 22.2   64 x 1,024 + 1,024  40.3 / 32.1   128 x 512 + 200  32.8 / 26.9   8 x 4,096 + 200  16.0 / 15.1
+//   mma.sync  (pages of 24)       29.3 / 27.8                       46.6 / 45.0                    34.8 / 32.5                    18.9 / 14.9
+//   FFMA                          84.4 / 78.9                      145.7 / 144.5                    104 / 102                     42.9 / 33.9
+// (Half of them or twice as much: tcgen05 within 3 %, mma.sync and FFMA up to 40 % slower with twice as much.)
 // WORKER_SMEM: shared memory of a worker of few rows where a block has several, 0 where it is one
 template <int FORM> struct Form;
 template <> struct Form<ON_F32> {
     static constexpr int THREADS = 128, FEW_WORKERS = 1, FEW_KEYS = F32Few::KEYS, MANY_TILE = F32Many::ROWS, MANY_KEYS = F32Many::KEYS;
     static constexpr size_t SMEM = most_of(F32Few::SMEM, F32Many::SMEM), FEW_AT = 0, WORKER_SMEM = 0;
+    static constexpr int FIXED = 10, OF_STEP = 10;
 };
 template <> struct Form<ON_MMA> {
     using Few = FewShape<4, 190 * 1024>;
     static constexpr int THREADS = 128, FEW_WORKERS = Few::WORKERS, FEW_KEYS = Few::KEYS, MANY_TILE = ManyShape::ROWS, MANY_KEYS = ManyShape::KEYS;
     static constexpr size_t SMEM = most_of(Few::SMEM, ManyShape::SMEM), FEW_AT = 0, WORKER_SMEM = 0;
+    static constexpr int FIXED = 20, OF_STEP = 10;
 };
 #ifdef FSIE_SHARED_TC
 template <> struct Form<ON_TC> {
     using Few = tc::TmaFew;
     static constexpr int THREADS = tc::THREADS, FEW_WORKERS = Few::WORKERS, FEW_KEYS = Few::KEYS, MANY_TILE = tc::ROWS, MANY_KEYS = tc::KEYS;
     static constexpr size_t SMEM = tc::SMEM, FEW_AT = tc::CONTROL_BYTES, WORKER_SMEM = Few::WORKER;
+    static constexpr int FIXED = 40, OF_STEP = 21;
 };
 #endif
 template <int FORM> constexpr size_t plan_at(int few_workers) {
@@ -1754,7 +1820,7 @@ shared_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_
 #endif
 }
 
-struct Shape { int blocks, few_workers, few_keys, many_tile, many_keys; };       // (few_workers: of a block)
+struct Shape { int blocks, few_workers, few_keys, many_tile, many_keys, fixed, of_step; };       // (few_workers: of a block)
 constexpr int MAX_DEVICES = 64;
 
 static bool tcgen05_takes(int page_size, long long page_stride, long long page_rows) {
@@ -1782,7 +1848,7 @@ static int shape_of(Shape& shape) {
                                                               most_of(F::SMEM, F::FEW_AT + F::FEW_WORKERS * F::WORKER_SMEM) + plan_bytes(100));
         if (e != cudaSuccess) return (int)e;
         if (sms * per_sm <= 0) return ERR_UNSUPPORTED;
-        known[device] = {sms * per_sm, F::FEW_WORKERS, F::FEW_KEYS, F::MANY_TILE, F::MANY_KEYS};
+        known[device] = {sms * per_sm, F::FEW_WORKERS, F::FEW_KEYS, F::MANY_TILE, F::MANY_KEYS, F::FIXED, F::OF_STEP};
     }
     shape = known[device];
     return 0;
@@ -1803,7 +1869,9 @@ static int launch(const Shape& shape, const CUtensorMap& k_map, const CUtensorMa
     while (Form<FORM>::WORKER_SMEM && workers > 1 && plan_at<FORM>(workers) + plan > MOST_SMEM) --workers;
     const size_t at = plan_at<FORM>(workers);
     if (at + plan > MOST_SMEM) return ERR_UNSUPPORTED;
+    a.few.of_block = workers;
     a.few.workers = shape.blocks * workers;
+    a.few.by_workers = div_by(a.few.workers);
     return launch_dependent(shared_attention_kernel<FORM>, dim3(shape.blocks), dim3(Form<FORM>::THREADS), at + plan, stream, k_map, v_map, a, workers, (int)at);
 }
 
@@ -1818,7 +1886,9 @@ static int launch(const Shape& shape, const CUtensorMap& k_map, const CUtensorMa
 //   128 x 128                   3,584     52.1   34.4   27.9   19.4
 // Up to four blocks to a multiprocessor.
 template <typename T, int ROWS, int SPLIT>
-static int launch_merge_as(const SharedArgs& a, int blocks, cudaStream_t stream) {
+static int launch_merge_as(SharedArgs& a, int blocks, cudaStream_t stream) {
+    a.by_chunks = div_by((a.group + ROWS - 1) / ROWS);
+    a.by_place = div_by((long long)a.kv_heads * ((a.group + ROWS - 1) / ROWS));
     const size_t smem = merge_smem<ROWS, SPLIT>() + plan_bytes(a.run_count);
     if (smem > 48 * 1024) return ERR_UNSUPPORTED;
     const long long units = (long long)a.places * a.kv_heads * ((a.group + ROWS - 1) / ROWS), teams = MERGE_WARPS / SPLIT;
@@ -1826,7 +1896,7 @@ static int launch_merge_as(const SharedArgs& a, int blocks, cudaStream_t stream)
                             smem, stream, a);
 }
 template <typename T>
-static int launch_merge(const SharedArgs& a, int blocks, cudaStream_t stream) {
+static int launch_merge(SharedArgs& a, int blocks, cudaStream_t stream) {
     const long long rows = (long long)a.places * a.heads;
     if (rows <= 2 * blocks) return launch_merge_as<T, 1, 4>(a, 4 * blocks, stream);
     if (rows <= 6 * blocks) return launch_merge_as<T, 1, 2>(a, 4 * blocks, stream);
@@ -1836,9 +1906,11 @@ static int launch_merge(const SharedArgs& a, int blocks, cudaStream_t stream) {
 
 // Where everything lies in the room, for `lines` lines of many rows; returns the bytes.
 static long long lay_out(const Shape& shape, long long places, long long runs, int kv_heads, long long lines, unsigned char* room, SharedArgs& a) {
-    a.few = {shape.blocks * shape.few_workers, (int)((places + runs) * kv_heads), FEW, shape.few_keys, 1, FEW_LEAST, 0};
+    a.few = {shape.blocks * shape.few_workers, (int)((places + runs) * kv_heads), FEW, shape.few_keys, 1, FEW_LEAST};
+    a.few.fixed = shape.fixed; a.few.of_step = shape.of_step;
     const long long few_rows = (long long)(a.few.line_room + a.few.workers) * FEW, many_rows = (lines + shape.blocks) * shape.many_tile;
-    a.many = {shape.blocks, (int)lines, shape.many_tile, shape.many_keys, 1, MANY_LEAST, few_rows};
+    a.many = {shape.blocks, (int)lines, shape.many_tile, shape.many_keys, 1, MANY_LEAST};
+    a.many.row0 = few_rows;
     a.part_o = (float*)room;                             // (stores of 32 bytes: it starts on 128)
     a.part_ml = a.part_o + (few_rows + many_rows) * HD;
     return few_rows + many_rows > 0x7fffffffLL ? -1 : (few_rows + many_rows) * (HD + 2) * 4 + 128;
@@ -1918,6 +1990,13 @@ int fsie_shared_attention(const void* q, int q_ld, const void* k_pages, const vo
     a.positions = positions; a.tokens = tokens; a.order = order; a.places = places; a.runs = runs; a.run_count = run_count;
     a.own_run = own_run; a.out = out; a.out_ld = out_ld; a.heads = heads; a.kv_heads = kv_heads; a.group = heads / kv_heads;
     a.scale = scale; a.early = early; a.error = error;
+    a.most_steps = 0x7fffffff / max(run_count, 1);
+    a.by_kv_heads = div_by(kv_heads); a.by_group = div_by(a.group);
+    for (Side* side : {&a.few, &a.many}) {
+        side->tile_shift = log2_of(side->tile); side->key_shift = log2_of(side->keys);
+        side->tokens = max(side->tile / a.group, 1); side->parts = (a.group + side->tile - 1) / side->tile;
+        side->by_tokens = div_by(side->tokens); side->by_parts = div_by(side->parts); side->by_workers = div_by(side->workers);
+    }
     CUtensorMap k_map = {}, v_map = {};
     if (dtype == DTYPE_F32) {
         rc = launch<ON_F32>(shape, k_map, v_map, a, stream);

@@ -171,13 +171,13 @@ class ModelRunner:
             raise ValueError("shared_attention: no layer of this model can read keys for several requests at once")
         # It pays where at least so many bytes of keys and values of a layer, and at least this part of what its requests see,
         # need not be read again.  A layer's attention, keys read by each request / once, us (bfloat16, 28 heads over 4 of 128;
-        # requests x keys in common, with 16 to 256 of their own): 16 x 512 (16 MB need not be read) 11.1 / 13.0, 32 x 512 (33 MB)
-        # 15.3 / 16.0, 4 x 8,192 (50 MB) 18.1 / 17.3, 8 x 4,096 (59 MB) 18.7 / 15.9, 64 x 512 (66 MB) 19.7 / 19.4, 128 x 512
-        # (133 MB) 37.3 / 30.8; float32 8 x 2,048 of 12 heads over 2 (29 MB) 21.0 / 26.7, 8 x 4,096 (59 MB) 43 / 32.  By the part:
-        # 64 x 512 beside 1,024 to 2,048 keys of each one's own (a quarter) 52.8 / 55.4, 32 x 1,024 and 32 requests that share
-        # nothing (0.4) 38.8 / 39.4, 16 x 4,096 and 16 (0.39) 77.9 / 58.8.
+        # requests x keys in common, with 16 to 256 of their own): 16 x 512 (16 MB need not be read) 11.0 / 12.4, 32 x 512 (33 MB)
+        # 15.1 / 15.4, 4 x 8,192 (50 MB) 18.0 / 17.1, 8 x 4,096 (59 MB) 18.8 / 15.0, 64 x 512 (66 MB) 19.7 / 18.4, 128 x 512
+        # (133 MB) 37.2 / 23.8; float32 8 x 2,048 of 12 heads over 2 (29 MB) 20.8 / 18.8, 8 x 4,096 (59 MB) 43 / 22.  By the part:
+        # 64 requests that share 16 keys (nothing) beside 1,024 to 2,048 of their own 44.1 / 45.2, 8 x 2,048 and 56 such requests
+        # (0.13) 69.3 / 46.4, 64 x 512 beside as many of their own (a quarter) 52.8 / 45.9.
         self.shared_min_bytes = 40 << 20
-        self.shared_min_part = 0.3
+        self.shared_min_part = 0.1
         self.shared_least_keys = 64          # ... and of every single run so many keys
         self.error = runtime.error
         self._ring = PinnedRing()
