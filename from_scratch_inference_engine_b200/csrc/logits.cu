@@ -13,10 +13,11 @@
 // Bound by latency and by little memory: the bits tell which logits and counts have to be read at all (a row of 151,936 tokens:
 // 19 KB of bits per history and mask, against 608 KB of logits and as much of counts).  A warp owns 1,024 tokens, a word of 32
 // bits to a lane.  The tokens that the history holds and the mask allows go into a list, so that a lane has one of them and all
-// of a warp's logits and counts are asked for at once; what the mask forbids is written without a read, 16 bytes at a time
-// where it forbids four tokens in a row.  64 rows of 152,064 tokens with 1,500 in every history, 22 of them masked: 9.2 us, where
-// threads that walked four groups of four tokens each, with a wait at each, took 12.0; 200 rows with 800 in every history 9.1
-// for 21.7.  Blocks of 2, 4, 8 warps: 8.3, 9.2, 10.2 us for those 64 rows, 16.1, 9.1, 8.0 for those 200.
+// of a warp's logits and counts are asked for at once; what the mask forbids is written without a read, a word's 32 tokens side
+// by side.  64 rows of 152,064 tokens with 1,500 in every history, 22 of them masked: 6.4 us, where 16 bytes were written at a
+// time and single tokens where a word is mixed 9.2, and threads that walked four groups of four tokens each, with a wait at each,
+// took 12.0; 200 rows with 800 in every history 8.7, those threads 21.7.  Blocks of 2, 4, 8 warps (of the form before): 8.3, 9.2,
+// 10.2 us for those 64 rows, 16.1, 9.1, 8.0 for those 200.
 #include "common.cuh"
 #include <math.h>
 
@@ -34,8 +35,6 @@ struct AdjustArgs {
     int* error;
 };
 
-// VEC: rows of logits start on 16 bytes
-template <bool VEC>
 __global__ void __launch_bounds__(ADJUST_THREADS)
 adjust_logits_kernel(const AdjustArgs a) {
     __shared__ unsigned short lists[ADJUST_WARPS][WARP_TOKENS];
@@ -76,20 +75,13 @@ adjust_logits_kernel(const AdjustArgs a) {
             const float repeated = z > 0.f ? z / theta : z * theta;
             logits[v] = repeated - (n > 0 ? presence : 0.f) - frequency * (float)n;
         }
-        // ---- forbidden: four tokens to a lane and turn
+        // ---- forbidden: a word's tokens side by side
         if (mask) {
-#pragma unroll 2
-            for (int turn = 0; turn < 8; ++turn) {
-                const unsigned bits = __shfl_sync(0xffffffffu, allowed, 4 * turn + (lane >> 3)) >> 4 * (lane & 7) & 15u;
-                const int v = base + 128 * turn + 4 * lane, there = min(a.vocab - v, 4);
-                if (there <= 0 || bits == 15u) continue;
-                if (VEC && bits == 0) {                   // (the vocabulary is a multiple of 4)
-                    *reinterpret_cast<float4*>(logits + v) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < there && !(bits >> e & 1)) logits[v + e] = -INFINITY;
-                }
+            for (int w = 0; w < 32; ++w) {
+                const unsigned bits = __shfl_sync(0xffffffffu, allowed, w);
+                const int v = base + 32 * w + lane;
+                if (!(bits >> lane & 1) && v < a.vocab) logits[v] = -INFINITY;
             }
         }
     }
@@ -152,10 +144,8 @@ int fsie_adjust_logits(float* logits, int rows, int vocab, const int* slots, con
     a.bias_start = bias_start; a.bias_token = bias_token; a.bias_value = bias_value; a.bias_count = bias_count;
     a.mask_of = mask_of; a.masks = (const unsigned*)masks; a.mask_count = mask_count;
     a.error = error;
-    const bool vec = vocab % 4 == 0 && ((uintptr_t)logits & 15) == 0;
     const dim3 grid((vocab - 1) / ADJUST_SPAN + 1, rows);
-    return launch_dependent(vec ? adjust_logits_kernel<true> : adjust_logits_kernel<false>, grid, dim3(ADJUST_THREADS), 0,
-                            stream, a);
+    return launch_dependent(adjust_logits_kernel, grid, dim3(ADJUST_THREADS), 0, stream, a);
 }
 
 int fsie_count_tokens(const int* tokens, const int* slots, int n, int vocab, int slot_count, int* counts, int* seen,
