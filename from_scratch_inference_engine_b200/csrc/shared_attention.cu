@@ -209,6 +209,12 @@ __device__ __forceinline__ bool make_plan(const SharedArgs& a, unsigned char* sm
         const int least = max(side.least, (l + LINE_PIECES - 1) / LINE_PIECES);
         (i ? plan.many_piece : plan.few_piece) = max(side.by_workers.of(max(before[2 + i] - 1, 0)) + 1, least);
         if (i == 0) plan.free_piece = least;
+        // pieces that end where long lines do: a piece in two lines loads two sets of queries and leaves two sets of triples
+        // (100 requests with 16,384 keys in common 67.8 -> 55.1 us)
+        if (i == 1 && plan.many_piece > 4 && plan.many_piece < l) {
+            const int pieces = l / plan.many_piece, even = (l - 1) / pieces + 1;
+            if (4 * even <= 5 * plan.many_piece) plan.many_piece = even;
+        }
         fits = fits && before[i] <= side.line_room;
     }
     if (!fits && tid == 0) atomicExch(a.error, ERR_ROOM);
@@ -1066,6 +1072,13 @@ __device__ __forceinline__ Pair fma2(Pair x, Pair y, Pair z) { Pair p; asm("fma.
 __device__ __forceinline__ Pair add2(Pair x, Pair y) { Pair p; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p) : "l"(x), "l"(y)); return p; }
 __device__ __forceinline__ float max3(float x, float y, float z) { float v; asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z)); return v; }
 
+__device__ __forceinline__ bool mbar_done(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+    return done;
+}
+
 __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtensorMap& v_map, const SharedArgs& a, const Plan& plan, unsigned char* smem_all) {
     Control& ctl = *reinterpret_cast<Control*>(smem_all);
     unsigned char* q_s = smem_all + CONTROL_BYTES;       // [stream][HALVES][128 rows][128 B]
@@ -1154,69 +1167,71 @@ __device__ __forceinline__ void tc_phase(const CUtensorMap& k_map, const CUtenso
                 }
             } else if (warp == 1) {
                 // -------------------------------------------------------------- MMA: one lane issues, all take part in the waits
+                // The streams by turns, each one's product with V and its next scores together, so that one stream's products run
+                // beside the other's softmax (a warp for each stream: both fall into step, 5,000 cycles a step).  Little else stands
+                // between a stream's weights and its next scores: what the copy engine brings is waited for beside the softmax,
+                // whether all lanes are well is asked once a tile.  3,950 cycles a step of 256 rows; with a vote and a fence at
+                // every wait, and the waits where their data is used, 4,890.
                 const uint32_t idesc_s = idesc_bf16(BM, KEYS, 0), idesc_o = idesc_bf16(BM, HD, 1);
                 const uint64_t q_base = desc_k_major(q_s), k_base = desc_k_major(ring), v_base = desc_mn_major(ring, ATOM);
-                auto wait = [&](uint64_t* bar, int parity) {
-                    if (!__all_sync(0xffffffffu, mbar_wait(bar, parity & 1))) {
-                        if (lane == 0) give_up(ERR_TC_MMA);
-                        ok = false;
+                auto wait = [&](uint64_t* bar, int parity) { if (!mbar_done(bar, parity & 1)) ok = mbar_wait(bar, parity & 1) && ok; };
+                auto scores = [&](int st, int entry) {    // S_st = Q_st K^T
+                    const uint64_t qd = q_base + (uint64_t)(st * (Q_BYTES >> 4)), kd = k_base + (uint64_t)((entry % SLOTS) * (KV_BYTES >> 4));
+#pragma unroll
+                    for (int c = 0; c < HD / 16; ++c) {
+                        const uint32_t step = (c >> 2) * (ATOM >> 4) + 2 * (c & 3);
+                        mma_ss(tmem + COL_S + st * KEYS, qd + step, kd + step, idesc_s, c > 0);
                     }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    mma_commit(&ctl.s_full[st]);
                 };
-                auto ring_wait = [&](int entry) { wait(&ctl.ring_full[entry % SLOTS], entry / SLOTS); };
-                // tile -1: only the first scores
-                for (int i = -1; i < tiles && ok; ++i) {
+                wait(&ctl.ring_full[e % SLOTS], e / SLOTS);
 #pragma unroll 1
-                    for (int st = 0; st < streams && ok; ++st) {
-                        if (i < 0) {
-                            wait(&ctl.q_ready[st], stretches_of[st]++);
-                        } else {
-                            wait(&ctl.p_ready[st], tiles_of[st]++);
-                            if (!ok) break;
-                            if (st == 0) {
-                                ring_wait(e + 1);
-                                if (!ok) break;
-                                const int from = sr.k0 + i * KEYS;
-                                if (from < sr.begin || from + KEYS > sr.kend) {        // rows of V that are none of the run's keys
-                                    unsigned char* v = ring + (size_t)((e + 1) % SLOTS) * KV_BYTES;
-                                    for (int at = lane; at < KEYS * 8 * HALVES; at += 32) {
-                                        const int key = from + (at >> 3) % KEYS;
-                                        if (key < sr.begin || key >= sr.kend) *reinterpret_cast<uint4*>(v + (size_t)at * 16) = make_uint4(0, 0, 0, 0);
-                                    }
-                                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                                    __syncwarp();
-                                }
-                            }
-                            if (lane == 0) {              // O_st += P_st V: 16 keys are 8 columns of P, 16 rows of V
-                                const uint64_t vd = v_base + (uint64_t)(((e + 1) % SLOTS) * (KV_BYTES >> 4));
-#pragma unroll
-                                for (int c = 0; c < KEYS / 16; ++c)
-                                    mma_ts(tmem + COL_O + st * KEYS, tmem + COL_S + st * KEYS + c * 8, vd + (uint64_t)(c * (16 * 128 >> 4)),
-                                           idesc_o, (i > 0 || c > 0) ? 1u : 0u);
-                                if (i + 1 == tiles) mma_commit(&ctl.o_done[st]);
-                                if (st == streams - 1) mma_commit(&ctl.ring_empty[(e + 1) % SLOTS]);
-                            }
-                            __syncwarp();
+                for (int st = 0; st < streams; ++st) {
+                    wait(&ctl.q_ready[st], stretches_of[st]++);
+                    if (lane == 0 && ok) {
+                        scores(st, e);
+                        if (st == streams - 1) mma_commit(&ctl.ring_empty[e % SLOTS]);
+                    }
+                    __syncwarp();
+                }
+                for (int i = 0; i < tiles; ++i, e += 2) {
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const bool on = i + 1 < tiles;
+                    wait(&ctl.ring_full[(e + 1) % SLOTS], (e + 1) / SLOTS);            // V of this tile, K of the next
+                    if (on) wait(&ctl.ring_full[(e + 2) % SLOTS], (e + 2) / SLOTS);
+                    const int from = sr.k0 + i * KEYS;
+                    if (from < sr.begin || from + KEYS > sr.kend) {        // rows of V that are none of the run's keys
+                        unsigned char* v = ring + (size_t)((e + 1) % SLOTS) * KV_BYTES;
+                        for (int at = lane; at < KEYS * 8 * HALVES; at += 32) {
+                            const int key = from + (at >> 3) % KEYS;
+                            if (key < sr.begin || key >= sr.kend) *reinterpret_cast<uint4*>(v + (size_t)at * 16) = make_uint4(0, 0, 0, 0);
                         }
-                        if (i + 1 == tiles) continue;
-                        const int next = i < 0 ? e : e + 2;               // the stream's next scores, beside the other's softmax
-                        if (st == 0) ring_wait(next);
-                        if (!ok) break;
-                        if (lane == 0) {                  // S_st = Q_st K^T
-                            const uint64_t qd = q_base + (uint64_t)(st * (Q_BYTES >> 4));
-                            const uint64_t kd = k_base + (uint64_t)((next % SLOTS) * (KV_BYTES >> 4));
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+#pragma unroll 1
+                    for (int st = 0; st < streams; ++st) {
+                        wait(&ctl.p_ready[st], tiles_of[st]++);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        if (lane == 0 && ok) {            // O_st += P_st V: 16 keys are 8 columns of P, 16 rows of V
+                            const uint64_t vd = v_base + (uint64_t)(((e + 1) % SLOTS) * (KV_BYTES >> 4));
 #pragma unroll
-                            for (int c = 0; c < HD / 16; ++c) {
-                                const uint32_t step = (c >> 2) * (ATOM >> 4) + 2 * (c & 3);
-                                mma_ss(tmem + COL_S + st * KEYS, qd + step, kd + step, idesc_s, c > 0);
+                            for (int c = 0; c < KEYS / 16; ++c)
+                                mma_ts(tmem + COL_O + st * KEYS, tmem + COL_S + st * KEYS + c * 8, vd + (uint64_t)(c * (16 * 128 >> 4)), idesc_o,
+                                       (i > 0 || c > 0) ? 1u : 0u);
+                            if (on) scores(st, e + 2);
+                            else mma_commit(&ctl.o_done[st]);
+                            if (st == streams - 1) {
+                                mma_commit(&ctl.ring_empty[(e + 1) % SLOTS]);
+                                if (on) mma_commit(&ctl.ring_empty[(e + 2) % SLOTS]);
                             }
-                            mma_commit(&ctl.s_full[st]);
-                            if (st == streams - 1) mma_commit(&ctl.ring_empty[next % SLOTS]);
                         }
                         __syncwarp();
                     }
-                    if (i >= 0) e += 2;
                 }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok && lane == 0) give_up(ERR_TC_MMA);
             } else if (st_own < streams) {
                 // -------------------------------------------------------------- softmax, a thread per row of a stream
                 const int rows = sr.rows - st_own * BM;
@@ -1762,10 +1777,11 @@ enum { ON_F32, ON_MMA, ON_TC };
 constexpr size_t most_of(size_t a, size_t b) { return a > b ? a : b; }
 constexpr size_t MOST_SMEM = 227 * 1024;
 // FIXED, OF_STEP: see Side.  Equal pieces for all / these, us in a graph, 28 heads over 4, requests x keys in common and of their own:
-//   tcgen05   32 x 1,024 + 1,024  28.5 / 22.2   64 x 1,024 + 1,024  40.3 / 32.1   128 x 512 + 200  32.8 / 26.9   8 x 4,096 + 200  16.0 / 15.1
+//   tcgen05   32 x 1,024 + 1,024  28.5 / 22.2   64 x 1,024 + 1,024  40.3 / 31.2   128 x 512 + 200  32.8 / 26.9   8 x 4,096 + 200  16.0 / 15.1
 //   mma.sync  (pages of 24)       29.3 / 27.8                       46.6 / 45.0                    34.8 / 32.5                    18.9 / 14.9
 //   FFMA                          84.4 / 78.9                      145.7 / 144.5                    104 / 102                     42.9 / 33.9
-// (Half of them or twice as much: tcgen05 within 3 %, mma.sync and FFMA up to 40 % slower with twice as much.)
+// (200 x 8,192 + 512, 40 heads over 8: FIXED, OF_STEP 40, 21 99.3, 60, 16 92.2, 60, 12 86.7; the others within 4 %.  mma.sync and FFMA
+// up to 40 % slower with twice as much.)
 // WORKER_SMEM: shared memory of a worker of few rows where a block has several, 0 where it is one
 template <int FORM> struct Form;
 template <> struct Form<ON_F32> {
@@ -1784,7 +1800,7 @@ template <> struct Form<ON_TC> {
     using Few = tc::TmaFew;
     static constexpr int THREADS = tc::THREADS, FEW_WORKERS = Few::WORKERS, FEW_KEYS = Few::KEYS, MANY_TILE = tc::ROWS, MANY_KEYS = tc::KEYS;
     static constexpr size_t SMEM = tc::SMEM, FEW_AT = tc::CONTROL_BYTES, WORKER_SMEM = Few::WORKER;
-    static constexpr int FIXED = 40, OF_STEP = 21;
+    static constexpr int FIXED = 60, OF_STEP = 12;
 };
 #endif
 template <int FORM> constexpr size_t plan_at(int few_workers) {
