@@ -107,6 +107,7 @@ class Engine:
         self.pipeline = bool(pipeline)
         self._in_flight = None          # (items, Picked) of a launched step whose tokens are not read yet
         self._raised = None             # what a request's `allowed` raised
+        self._raises_later = False
         self.steps = 0
         self.tokens_prefilled = 0
         self.tokens_decoded = 0
@@ -173,9 +174,10 @@ class Engine:
         ids, rest = [first], list(params[1:])
         if len(prompt) > 1 and rest:
             seq.hold = len(prompt) - 1
+            self._raises_later = True       # (what another request's `allowed` raises: behind the answers' ids)
             try:
                 while seq.handle is None or seq.handle.length < seq.hold:
-                    if self._step() == 0:         # (what an `allowed` raises waits for the next `step`)
+                    if self.step() == 0:
                         break
                 if seq.handle is not None and seq.handle.length == seq.hold:
                     count = max(0, min(len(rest), self.scheduler.max_batch - len(self.scheduler.running),
@@ -184,6 +186,7 @@ class Engine:
                     rest = rest[count:]
             finally:                        # whatever happened, the request may go on
                 seq.hold = 0
+                self._raises_later = False
         return ids + [self.add_request(prompt, p, max_tokens, eos_id) for p in rest]
 
     def warm_up(self, max_context: int = 0) -> int:
@@ -215,7 +218,7 @@ class Engine:
         """One batched step; returns the number of tokens it ran (0 = nothing could run).  What a request's `allowed`
         raised is raised here, once the step is recorded; that request has ended."""
         ran = self._step()
-        if self._raised is not None:
+        if self._raised is not None and not self._raises_later:
             raised, self._raised = self._raised, None
             raise raised
         return ran
