@@ -75,3 +75,27 @@ def test_calls_beside_one_another():
     torch.cuda.synchronize()
     for p, want in zip(problems, alone):
         assert torch.equal(p.out, want) and not p.error.item()
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,dtype", [(14, 2, 128, 16, "bf16"), (12, 2, 64, 8, "bf16"), (8, 1, 128, 64, "bf16"), (28, 4, 128, 128, "bf16"),
+                                                     (6, 2, 64, 24, "bf16"), (6, 2, 48, 4, "bf16"), (6, 2, 64, 16, "f32"), (40, 1, 64, 16, "bf16")])
+@pytest.mark.parametrize("count", [2, 9, 60])
+@pytest.mark.parametrize("cuts", [(1,), (5, 77, 130), (15, 16, 17, 18), (127, 128, 129, 255, 256), (300,)])
+def test_runs_that_begin_and_end_anywhere(cuts, count, heads, kv, dim, page, dtype):
+    """Shared keys in several runs around one another, cut inside of pages, tiles and steps; own keys from inside a page on."""
+    p = Problem(answers(count, 512 // page + 1, lambda i: 1 + 7 * i), heads, kv, dim, page, dtype, seed=sum(cuts))
+    runs, begin = [], 0
+    for end in cuts:
+        runs.append([0, count, begin, end, count - 1, len(runs) - 1])
+        begin = end
+    runs += [[i, 1, begin, n, i, len(cuts) - 1] for i, n in enumerate(p.lengths)]
+    room = torch.empty(ops_module().shared_attention_room(count, len(runs), len(cuts), heads, kv, dim, p.dtype, shared=len(cuts)),
+                       dtype=torch.uint8, device="cuda").fill_(255)
+    p.run([torch.arange(count, dtype=torch.int32, device="cuda"), torch.tensor(runs, dtype=torch.int32, device="cuda"),
+           torch.arange(len(cuts), len(cuts) + count, dtype=torch.int32, device="cuda")], room=room)
+    p.check()
+
+
+def ops_module():
+    from from_scratch_inference_engine_b200.kernels import ops
+    return ops
