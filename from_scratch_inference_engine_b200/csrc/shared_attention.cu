@@ -35,6 +35,7 @@
 #include "tma.cuh"
 #include "attention_tc.cuh"
 #include <math.h>
+#include <atomic>
 
 #ifndef HEAD_DIM
 #error "compile with -DHEAD_DIM=<head size>"
@@ -1850,23 +1851,27 @@ static bool tcgen05_takes(int page_size, long long page_stride, long long page_r
 // How a form's launch looks on the current device: as many blocks as run at once beside plans of middling size.
 template <int FORM>
 static int shape_of(Shape& shape) {
-    static Shape known[MAX_DEVICES] = {};                // per process; the same whoever writes it
+    // Per process.  Calls come from several threads at once: one number is all that is kept, and whoever sees it sees the
+    // kernel's attribute set as well; two that find none work out the same.
+    static std::atomic<int> known[MAX_DEVICES];
     using F = Form<FORM>;
     int device = 0, sms = 0, per_sm = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return (int)e;
     if (device < 0 || device >= MAX_DEVICES) return ERR_UNSUPPORTED;
-    if (known[device].blocks == 0) {
+    int blocks = known[device].load(std::memory_order_acquire);
+    if (blocks == 0) {
         e = cudaFuncSetAttribute(shared_attention_kernel<FORM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_SMEM);
         if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
         if (e == cudaSuccess)
             e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, shared_attention_kernel<FORM>, F::THREADS,
                                                               most_of(F::SMEM, F::FEW_AT + F::FEW_WORKERS * F::WORKER_SMEM) + plan_bytes(100));
         if (e != cudaSuccess) return (int)e;
-        if (sms * per_sm <= 0) return ERR_UNSUPPORTED;
-        known[device] = {sms * per_sm, F::FEW_WORKERS, F::FEW_KEYS, F::MANY_TILE, F::MANY_KEYS, F::FIXED, F::OF_STEP};
+        blocks = sms * per_sm;
+        if (blocks <= 0) return ERR_UNSUPPORTED;
+        known[device].store(blocks, std::memory_order_release);
     }
-    shape = known[device];
+    shape = {blocks, F::FEW_WORKERS, F::FEW_KEYS, F::MANY_TILE, F::MANY_KEYS, F::FIXED, F::OF_STEP};
     return 0;
 }
 static int shape_of(int dtype, bool on_tcgen05, Shape& shape) {

@@ -1,5 +1,8 @@
 """Attention over pages that several requests share, against the formula in 64 bits."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -367,3 +370,47 @@ def test_refusals():
                  (1, 1, 1, 12, 2, 64, torch.float16), (1, 1, -1, 12, 2, 64, torch.float32)):
         with pytest.raises(o.KernelError):
             o.shared_attention_room(*args)
+
+
+FIRST_CALLS = """
+import sys, threading
+import torch
+sys.path[:0] = sys.argv[1:]
+import test_gpu_shared_attention as t
+forms = [(16, "bf16"), (24, "bf16"), (16, "f32")]               # on tcgen05, on mma.sync, FFMA
+problems = [t.Problem(t.TREES["tree"], 28, 4, 128, *forms[i % 3]) for i in range(12)]
+tables = [t.ints(p.tables) for p in problems]
+rooms = [torch.empty(64 << 20, dtype=torch.uint8, device="cuda") for _ in problems]
+torch.cuda.synchronize()
+sizes, raised, start = [0] * 12, [], threading.Barrier(12)
+
+def call(i):
+    p, f = problems[i], problems[i].found
+    size = lambda: t.ops().shared_attention_room(len(f.order), len(f.runs), f.levels, 28, 4, 128, p.dtype)
+    try:
+        start.wait()
+        if i < 6:
+            sizes[i] = size()
+        p.run(tables=tables[i], room=rooms[i])
+        sizes[i] = sizes[i] or size()
+    except Exception as e:
+        raised.append(e)
+
+threads = [threading.Thread(target=call, args=(i,)) for i in range(12)]
+for thread in threads:
+    thread.start()
+for thread in threads:
+    thread.join()
+assert not raised, raised
+assert max(sizes) <= 64 << 20 and all(sizes[i] == sizes[i % 3] for i in range(12)), sizes
+for p in problems:
+    p.check()
+print("well")
+"""
+
+
+def test_first_calls_of_several_threads_at_once():
+    """In a process of its own, where nothing is known yet of how the launches look."""
+    here = Path(__file__).resolve().parent
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(here), str(here.parent)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "well", done.stderr[-2000:]
