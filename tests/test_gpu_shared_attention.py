@@ -372,6 +372,51 @@ def test_refusals():
             o.shared_attention_room(*args)
 
 
+def formula_without(p, tables):
+    """`Problem.expected` over the keys whose pages `tables` has inside the pool; zeros where none is left."""
+    group, step, unit = p.heads // p.kv, 2.0 ** -23, torch.finfo(p.dtype).eps / 2
+    want = torch.zeros(p.tokens, p.heads * p.dim, dtype=torch.float64)
+    bound = torch.zeros_like(want)
+    k, v = p.k.double().cpu(), p.v.double().cpu()
+    q = p.qkv[:, :p.heads * p.dim].double().cpu().view(p.tokens, p.kv, group, p.dim)
+    for i, table in enumerate(tables.tolist()):
+        for t in range(p.start[i], p.start[i] + p.new[i]):
+            keys = [(table[j // p.page], j % p.page) for j in range(int(p.positions[t]) + 1) if 0 <= table[j // p.page] < len(p.pages)]
+            if not keys:
+                continue
+            pages, places = (torch.tensor(x) for x in zip(*keys))
+            ki, vi = (x[pages, :, places].transpose(0, 1) for x in (k, v))
+            weights = torch.softmax(torch.einsum("kgd,knd->kgn", q[t], ki) * p.scale, -1)
+            o, size = torch.einsum("kgn,knd->kgd", weights, vi), torch.einsum("kgn,knd->kgd", weights, vi.abs())
+            off = torch.einsum("kgd,knd->kgn", q[t].abs(), ki.abs()).amax(-1, keepdim=True) * p.scale
+            b = (2 * (p.dim + 4) * step * off + 2 * (len(keys) + 64) * step + 2.0 ** -19) * size + unit * o.abs() * 1.01
+            want[t], bound[t] = o.reshape(-1), (b + (2.0 ** -8 * 1.01 * size if p.dtype is torch.bfloat16 else 0)).reshape(-1)
+    return want, bound
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,page", [("bf16", 28, 4, 128, 16), ("bf16", 28, 4, 64, 8), ("bf16", 14, 2, 128, 64), ("bf16", 14, 2, 128, 24),
+                                                     ("bf16", 8, 2, 256, 16), ("f32", 14, 2, 128, 16), ("f32", 6, 2, 48, 8)])
+@pytest.mark.parametrize("tree", ["many rows", "long", "tree"])
+def test_keys_of_pages_outside_the_pool_are_left_out(tree, dtype, heads, kv, dim, page):
+    """In every form alike, of shared runs and of a request's own keys: a page here and there, all shared ones, all."""
+    p = Problem(TREES[tree], heads, kv, dim, page, dtype, seed=dim + page)
+    held = p.tables >= 0
+    shared = np.zeros_like(held)
+    for first, count, begin, end, row, _ in p.found.runs[:p.found.shared]:
+        pages = p.tables[row, begin // page:end // page]
+        shared |= np.isin(p.tables, pages)
+    for turn, gone in enumerate((held & (p.tables % 5 == 2), shared & held, held)):
+        tables = p.tables.copy()
+        tables[gone] = np.resize([-1, len(p.pages), 2 ** 31 - 1, -2 ** 31], gone.sum())
+        p.error.zero_()
+        p.out.fill_(9)
+        p.run(tables=ints(tables))
+        assert int(p.error) == 3
+        want, bound = formula_without(p, tables)
+        got = p.out.double().cpu()
+        assert bool(((got - want).abs() <= bound).all()), (turn, float((got - want).abs().max()))
+
+
 FIRST_CALLS = """
 import sys, threading
 import torch
