@@ -1594,7 +1594,8 @@ __device__ __forceinline__ void merge_units(const SharedArgs& a, const Plan& pla
     const int rows = min(ROWS, a.group - g0);
     const int token = a.order[place];
     int r = a.own_run[place], levels = 0, own_level = -1;
-    if (r >= a.run_count) r = -1;
+    const bool no_such_run = r < -1 || r >= a.run_count;
+    if (no_such_run) r = -1;
     // ---- lane d: the d-th run around the token; its triples of row g0 are rows first_at, first_at + tile, ..
     for (; r >= 0 && levels < MAX_LEVELS; ++levels) {
         if (lane == levels) own_level = r;
@@ -1603,11 +1604,13 @@ __device__ __forceinline__ void merge_units(const SharedArgs& a, const Plan& pla
     }
     const bool there = (unsigned)token < (unsigned)a.tokens;
     const int position = there ? a.positions[token] : -1;
-    if ((r >= 0 || !there) && lane == 0) atomicExch(a.error, ERR_RUNS);
+    if ((no_such_run || r >= 0 || !there) && lane == 0) atomicExch(a.error, ERR_RUNS);
     int first_at = 0, count = 0, tile_rows = FEW;
     if (own_level >= 0) {
         const Run run = plan.runs[own_level];
-        if (run.count > 0 && place >= run.first && place < run.first + run.count) {
+        if (run.count > 0 && (place < run.first || place >= run.first + run.count)) {
+            atomicExch(a.error, ERR_RUNS);                // a run that the token is not in
+        } else if (run.count > 0) {
             const int kind = plan.kind[own_level], many = kind & RUN_FEW ? 0 : 1;
             const Side& side = many ? a.many : a.few;
             tile_rows = side.tile;

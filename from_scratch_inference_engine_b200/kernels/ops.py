@@ -2591,14 +2591,15 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
     runs     int32 [r, 6]: first place in order, number of places, first key, end of the keys, row of block_tables that has
              their pages, index of the run around it or -1 (a run comes behind the run around it).  Its keys are behind those
              of the run around it
-    own_run  int32 [n]: the innermost run of the token at each place.  It belongs to one request, whose tokens see its keys up
-             to their positions.  The runs around it end in front of all of their tokens
+    own_run  int32 [n]: the innermost run of the token at each place (-1: it sees no key).  It belongs to one request, whose
+             tokens see its keys up to their positions.  The runs around it end in front of all of their tokens
 
     out [tokens, ..] gets the rows of the tokens in `order` (zeros for a token without keys); other rows stay as they are.
-    `room`: uint8, `shared_attention_room` bytes, of no other call that may run at the same time.  A run or token outside of what there is, or a shared run that reaches
-    beyond one of its tokens, sets error[0] to 7, a page outside the pool to 3 (its keys are left out), runs that nest
-    deeper than `room` was made for to 8; the rows concerned hold no result.  `early`: the lists, tables and positions are
-    older than the stream's last kernel."""
+    `room`: uint8, `shared_attention_room` bytes, of no other call that may run at the same time.  A run or token outside of
+    what there is, a token whose innermost run or one around that does not hold its place (a run of no places does no harm),
+    or a shared run that reaches beyond one of its tokens, sets error[0] to 7, a page outside the pool to 3 (its keys are left
+    out), runs that nest deeper than `room` was made for to 8; the rows concerned hold no result.  `early`: the lists, tables
+    and positions are older than the stream's last kernel."""
     dtype, device = q.dtype, _device()
     if not (_all_fit(device, torch.int32, True, block_tables, positions, order, runs, own_run, error)
             and _all_fit(device, dtype, False, q, k_pages, v_pages, out) and _all_fit(device, torch.uint8, True, room)):

@@ -417,6 +417,43 @@ def test_keys_of_pages_outside_the_pool_are_left_out(tree, dtype, heads, kv, dim
         assert bool(((got - want).abs() <= bound).all()), (turn, float((got - want).abs().max()))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_runs_that_a_token_is_not_in(dtype):
+    """An innermost run that there is none of, or one of another token, and a run around it that lies elsewhere are reported;
+    -1 and runs without places are not."""
+    p = Problem(TREES["tree"], 12, 2, 64, 16, dtype)
+    want, bound = p.expected()
+    order, runs, own_run = p.lists
+    place = order.tolist().index(18)                                     # the request of 33 tokens that shares nothing
+    run, elsewhere = int(own_run[place]), p.found.shared - 1
+    assert runs[run].tolist()[1] == 1 and runs[run].tolist()[5] == -1
+    first, count = runs[elsewhere].tolist()[:2]
+    assert count > 1 and not first <= place < first + count
+    others = [t for t in range(p.tokens) if t != 18]
+
+    def reports(code, lists):
+        p.error.zero_()
+        p.out.fill_(9)
+        p.run(lists)
+        assert int(p.error) == code
+        assert ((p.out.double().cpu() - want).abs() <= bound)[others].all()
+    for value in (len(runs), 2 ** 31 - 1, -2, -2 ** 31, int(own_run[(place + 1) % p.tokens]), elsewhere):
+        broken = own_run.clone()
+        broken[place] = value
+        reports(7, [order, runs, broken])
+    broken = runs.clone()
+    broken[run, 5] = elsewhere
+    reports(7, [order, broken, own_run])
+    broken = own_run.clone()
+    broken[place] = -1
+    reports(0, [order, runs, broken])
+    assert (p.out[18] == 0).all()
+    emptied = runs.clone()
+    emptied[run, 1] = 0
+    reports(0, [order, emptied, own_run])
+    assert (p.out[18] == 0).all()
+
+
 FIRST_CALLS = """
 import sys, threading
 import torch
