@@ -86,21 +86,29 @@ adjust_logits_kernel(const AdjustArgs a) {
         }
     }
     if (!a.bias_start) return;
-    // biases come behind the penalties: this block's tokens have them now
-    __syncthreads();
     const int begin = max(a.bias_start[row], 0), end = min(a.bias_start[row + 1], a.bias_count);
+    auto add = [&](int i, int v) {
+        if ((unsigned)v >= (unsigned)a.vocab) atomicExch(a.error, ERR_TOKEN_ID);
+        else if (i > begin && a.bias_token[i - 1] >= v) atomicExch(a.error, ERR_BIAS_ORDER);
+        else if (!mask || (mask[v >> 5] >> (v & 31) & 1)) logits[v] += a.bias_value[i];
+    };
+    // what this block has to do with (whatever is outside the vocabulary is the first block's)
+    auto is_mine = [&](int v) { return (unsigned)v < (unsigned)a.vocab ? v >= first && v - first < ADJUST_SPAN : first == 0; };
+    int mine = 0, at = 0, token = 0;                             // of the thread's share of the list; the last of them
+    bool disordered = false;                                     // somewhere in the row's list
     for (int i = begin + (int)threadIdx.x; i < end; i += ADJUST_THREADS) {
         const int v = a.bias_token[i];
-        if ((unsigned)v >= (unsigned)a.vocab) {
-            atomicExch(a.error, ERR_TOKEN_ID);
-            continue;
-        }
-        if (v < first || v - first >= ADJUST_SPAN) continue;
-        if (i > begin && a.bias_token[i - 1] >= v) {             // a token twice: which of the two would come first is open
-            atomicExch(a.error, ERR_BIAS_ORDER);
-            continue;
-        }
-        if (!mask || (mask[v >> 5] >> (v & 31) & 1)) logits[v] += a.bias_value[i];
+        disordered |= i > begin && a.bias_token[i - 1] >= v;
+        if (is_mine(v)) { ++mine; at = i; token = v; }
+    }
+    // biases come behind the penalties: this block's tokens have them now
+    if (__syncthreads_or(disordered)) {                          // a token may be there twice: one after the other
+        if (threadIdx.x == 0)
+            for (int i = begin; i < end; ++i) { const int v = a.bias_token[i]; if (is_mine(v)) add(i, v); }
+    } else if (mine == 1) {
+        add(at, token);
+    } else if (mine) {
+        for (int i = begin + (int)threadIdx.x; i < end; i += ADJUST_THREADS) { const int v = a.bias_token[i]; if (is_mine(v)) add(i, v); }
     }
 }
 

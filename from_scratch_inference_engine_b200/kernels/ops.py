@@ -2694,8 +2694,8 @@ def adjust_logits(logits: torch.Tensor, error: torch.Tensor, slots: Optional[tor
     masks (int32 [rows], int32 [m, bit_words(vocab)]): row r may take what mask row masks[0][r] allows (-1: everything); the
     others become -inf.  A mask without a bit leaves a row of -inf.
 
-    A history or a mask that does not exist counts as none, a token of a bias outside the vocabulary or out of order is
-    left out; each sets error[0] (int32)."""
+    A history or a mask that does not exist counts as none, a token of a bias outside the vocabulary or not above the one in
+    front of it is left out; each sets error[0] (int32)."""
     device = _device()
     if not (_all_fit(device, torch.float32, True, logits, penalties) and _all_fit(device, torch.int32, True, error, slots, counts, seen)):
         _need_all("adjust_logits", torch.float32, True, logits=logits, penalties=penalties)

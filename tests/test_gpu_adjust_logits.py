@@ -169,6 +169,23 @@ def test_what_does_not_fit_is_left_out_and_reported():
     assert none
 
 
+def test_a_token_twice_in_a_bias_that_is_out_of_order():
+    """What is above the one in front of it counts, one after the other: 32-bit sums in the order of the list."""
+    vocab, low, high = 9000, 3, 8500
+    values = torch.randn(1001, generator=torch.Generator().manual_seed(4))
+    for tokens in ([high, low] * 500 + [high], [low, high] * 500 + [low], [low, high, low + 1] * 333, [high, low, high]):
+        bias = [[(t, float(v)) for t, v in zip(tokens, values)], [(t, 1.0) for t in range(0, vocab, 10)]]
+        want = torch.zeros(2, vocab)
+        for i, (token, value) in enumerate(bias[0]):
+            if i == 0 or tokens[i - 1] < token:
+                want[0, token] += value                        # (a 32-bit sum)
+        want[1, ::10] = 1
+        for _ in range(5):
+            got, error = torch.zeros(2, vocab, device="cuda"), flag()
+            ops().adjust_logits(got, error, bias=device_bias(bias))
+            assert int(error) == 5 and torch.equal(got.cpu(), want)
+
+
 def test_nothing_around_the_rows_is_written():
     around = torch.full((5, 101), 7.0, device="cuda")
     held, counts = torch.ones(1, 101, dtype=torch.bool), torch.full((1, 101), 2, dtype=torch.int32)
