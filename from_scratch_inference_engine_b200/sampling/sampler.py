@@ -14,7 +14,6 @@ tokens that the request's context holds, by a bias per token, and by the set of 
 
 from __future__ import annotations
 
-import math
 import operator
 from dataclasses import dataclass
 from typing import Callable, List, Mapping, Optional, Sequence, Tuple
@@ -24,6 +23,7 @@ import torch
 
 from ..kernels import ops
 
+LEAST32, MOST32 = float(np.finfo(np.float32).tiny), float(np.finfo(np.float32).max)
 _MASK = 0xFFFFFFFFFFFFFFFF
 
 
@@ -52,12 +52,13 @@ class SamplingParams:
         return self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
 
     def check(self, vocab: int) -> None:
-        """ValueError where the options that change logits make no sense for this vocabulary."""
-        if not (math.isfinite(self.repetition_penalty) and self.repetition_penalty > 0.0):
-            raise ValueError(f"repetition_penalty must be positive and finite, not {self.repetition_penalty}")
+        """ValueError where the options that change logits make no sense for this vocabulary, as the 32-bit numbers that they
+        are applied as: a penalty that becomes infinite turns a count of zero into NaN, one that becomes zero a logit into inf."""
+        if not LEAST32 <= self.repetition_penalty <= MOST32:
+            raise ValueError(f"repetition_penalty must be positive and finite in 32 bits, not {self.repetition_penalty}")
         for name in ("presence_penalty", "frequency_penalty"):
-            if not math.isfinite(getattr(self, name)):
-                raise ValueError(f"{name} must be finite, not {getattr(self, name)}")
+            if not abs(getattr(self, name)) <= MOST32:
+                raise ValueError(f"{name} must be finite in 32 bits, not {getattr(self, name)}")
         sorted_bias(self.logit_bias, vocab)
         if self.allowed is not None and not callable(self.allowed):
             raise ValueError("allowed must be a function of the answer so far")

@@ -54,6 +54,23 @@ def test_options_that_make_no_sense(options):
     SamplingParams(repetition_penalty=1.2, presence_penalty=-0.5, frequency_penalty=2, logit_bias={99: -1e9}, allowed=lambda o: None).check(100)
 
 
+@pytest.mark.parametrize("name", ["repetition_penalty", "presence_penalty", "frequency_penalty"])
+def test_penalties_are_checked_as_the_numbers_they_are_applied_as(name):
+    """What is finite, or positive, in 64 bits only is refused; the ends of the range of 32 bits are taken."""
+    top, low = float(np.finfo(np.float32).max), float(np.finfo(np.float32).tiny)
+    wrong = [1e39, top * (1 + 2.0 ** -24), np.inf, np.nan, -np.inf]
+    wrong += [1e-50, low / 2, 0.0, -0.0, -1.0] if name == "repetition_penalty" else [-1e39]
+    for value in wrong:
+        with pytest.raises(ValueError, match=name):
+            SamplingParams(**{name: value}).check(100)
+    for value in [top, 1] + ([low, np.float32(1.5)] if name == "repetition_penalty" else [-top, 1e-50, 0, np.float32(-2)]):
+        params = SamplingParams(**{name: value})
+        params.check(100)
+        host, histories, _, _ = stage_changes([params], [0], [None], None)
+        staged = host[histories[1]].view(np.float32)
+        assert np.isfinite(staged).all() and staged[0] >= low
+
+
 def test_what_is_staged_for_the_rows():
     params = [SamplingParams(), SamplingParams(repetition_penalty=1.5, frequency_penalty=0.25), SamplingParams(presence_penalty=2.0)]
     biases = [sorted_bias({5: 1.0, 2: 3.0}, 40), None, sorted_bias({39: -4.0}, 40)]
