@@ -94,14 +94,15 @@ class StepContext:
                  q_len: Sequence[int], pos0: Sequence[int], slots: Sequence[int],
                  group_tables: Sequence[Tuple[int, List[List[int]]]],
                  table_width: int = 0, out: Optional[torch.Tensor] = None,
-                 max_context: int = 0, shared: Sequence = (), shared_room: Tuple[int, int] = (0, 0)):
+                 max_context: int = 0, shared: Sequence = (), shared_room: Tuple[int, int] = (0, 0),
+                 most_shared: Optional[int] = None):
         """group_tables: per cache group (page_size, block table of each item).
         table_width forces the width of the device block tables, `out` is a fixed device
         buffer to fill instead of fresh memory, max_context overrides the longest context
         (all three serve captured graphs, whose shapes and launch choices must not vary).
         shared: per cache group the `SharedRuns` of the requests of one token, or None where every request reads its keys by
         itself; shared_room (runs, levels): their lists are padded to so many runs (for captured graphs as well), and to
-        places for all tokens."""
+        places for all tokens; most_shared of those runs (None: all) may be shared ones in some step that is filled in."""
         self.runtime = runtime
         self._ring, self._scratch, self.error = ring, scratch, error
         # what one part leaves for a later part of the same step (values of the step's tokens that
@@ -147,7 +148,8 @@ class StepContext:
                 own_run = np.concatenate([own_run, np.full(T - len(own_run), -1, dtype=np.int32)])
                 table = np.concatenate([table, np.zeros((shared_room[0] - len(table), 6), dtype=np.int32)])
             parts += [order, own_run, table.reshape(-1)]
-            lists.append((len(order), len(table), shared_room if shared_room[0] else (runs.shared, runs.levels)))
+            most = shared_room[0] if most_shared is None else most_shared
+            lists.append((len(order), len(table), (most, shared_room[1]) if shared_room[0] else (runs.shared, runs.levels)))
         flat = np.concatenate(parts) if parts else np.zeros(0, np.int32)
         dev = ring.stage(flat, runtime.device, out)
         self.staged_ints = flat.size

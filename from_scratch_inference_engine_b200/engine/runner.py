@@ -61,7 +61,8 @@ class _DecodeGraph:
         groups = len(runner.cache.groups)
         ints = 6 * batch + groups * (batch * width + batch)
         if shared:
-            self.shared_room = (batch + min(batch - 1, MOST_SHARED_RUNS), MOST_SHARED_LEVELS)
+            self.most_shared = min(batch - 1, MOST_SHARED_RUNS)       # (each of two branches at least)
+            self.shared_room = (batch + self.most_shared, MOST_SHARED_LEVELS)
             ints += sum(runner.shareable) * (2 * batch + 6 * self.shared_room[0])
         device = runner.runtime.device
         self.buffer = torch.zeros(ints, dtype=torch.int32, device=device)
@@ -103,7 +104,8 @@ class _DecodeGraph:
                            [1] * self.batch, list(pos0) + [0] * pad, list(slots) + [-1] * pad,
                            group_tables, table_width=self.width, out=self.buffer,
                            max_context=self.width * page, shared=shared if self.shared else (),
-                           shared_room=self.shared_room if self.shared else (0, 0))
+                           shared_room=self.shared_room if self.shared else (0, 0),
+                           most_shared=self.most_shared if self.shared else None)
 
     def replay(self) -> torch.Tensor:
         self.graph.replay()
@@ -260,6 +262,8 @@ class ModelRunner:
             self.model.reserve(tokens, self.max_step_items)
             if any(self.shareable):
                 places = min(self.max_step_items, self.max_step_tokens, MOST_SHARED_PLACES)
+                if self.cuda_graphs:                      # (captured batches are padded)
+                    places = next((b for b in DECODE_BATCHES if b >= places), places)
                 for block in self.model.blocks:
                     if hasattr(block.mixer, "reserve_shared_lists"):
                         block.mixer.reserve_shared_lists(places, places + MOST_SHARED_RUNS, MOST_SHARED_RUNS, MOST_SHARED_LEVELS)

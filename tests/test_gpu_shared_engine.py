@@ -194,3 +194,27 @@ def test_working_memory_is_taken_before_serving(folders, calls):
     handles = [parent] + runner.fork(parent, list("bcdefg"))
     step(runner, *[(handle, [5]) for handle in handles], (runner.cache.open("other"), [1, 2, 3]))
     assert calls and runner.runtime._buffers["attention.shared_room", torch.uint8] is room
+
+
+@pytest.mark.parametrize("requests", [7, 40, 200])
+def test_captured_steps_find_the_working_memory_that_was_taken(folders, calls, requests):
+    """Graphs of padded batches (8, 48, 256), captured ahead or while serving: none is given more than was reserved, and what a
+    step of as many requests as there may be needs is what was reserved."""
+    from from_scratch_inference_engine_b200.engine import runner as module
+    runner = runner_of(folders["E"], "bfloat16", 16, pages=500, max_requests=requests)
+    runner.reserve_step_memory(300)
+    room = runner.runtime._buffers["attention.shared_room", torch.uint8]
+    runner.capture_decode_graphs(100)
+    assert calls and runner.runtime._buffers["attention.shared_room", torch.uint8] is room
+    graphs = {batch: graph for (batch, _, shared), graph in runner._graphs.items() if shared}
+    largest = max(graphs)
+    assert largest >= requests
+    for batch, graph in graphs.items():
+        lists = graph.context.shared_lists[runner.shareable.index(True)]
+        assert lists.shared == min(batch - 1, module.MOST_SHARED_RUNS) and lists.runs.shape[0] == batch + lists.shared
+    parent = runner.cache.open("parent")
+    step(runner, (parent, [3] * 70))
+    handles = [parent] + runner.fork(parent, list(range(requests - 1)))
+    step(runner, *[(handle, [5]) for handle in handles])
+    assert len(runner._graphs) == 2 * len(graphs) + 1
+    assert runner.runtime._buffers["attention.shared_room", torch.uint8] is room

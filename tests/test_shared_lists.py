@@ -29,6 +29,18 @@ def test_lists_of_shared_runs():
         assert ctx.groups[0].slot_of.tolist() == [11, 13, -1]
 
 
+def test_how_many_runs_of_a_captured_step_may_be_shared():
+    """Working memory goes by it: of the runs that a list is padded to most are requests' own."""
+    from from_scratch_inference_engine_b200.cache.shared_runs import SharedRuns
+    runs = SharedRuns(np.array([0, 1], np.int32), np.array([[0, 2, 0, 8, 0, -1], [0, 1, 8, 10, 0, 0], [1, 1, 8, 12, 1, 0]], np.int32),
+                      np.array([1, 2], np.int32), 1, 1, 8)
+    for most in (1, 3):
+        ctx = StepContext(types.SimpleNamespace(device="cpu"), Ring(), {}, None, [7] * 4, [0, 1, 2, 3], [1] * 4, [9, 11, 0, 0],
+                          [0, 1, -1, -1], [(4, [[0, 1, 2], [0, 1, 3], [], []])], shared=[runs], shared_room=(7, 4), most_shared=most)
+        lists = ctx.shared_lists[0]
+        assert (lists.shared, lists.levels, lists.runs.shape[0], lists.order.shape[0]) == (most, 4, 7, 4)
+
+
 def test_requests_of_one_token_can_be_left_out_of_the_tiles():
     ctx = StepContext(types.SimpleNamespace(device="cpu"), Ring(), {}, None, [0] * 24, [0, 1, 21, 22], [1, 20, 1, 2], [3, 0, 8, 5],
                       [0, 1, 2, 3], [(4, [list(range(8)) for _ in range(4)])])
