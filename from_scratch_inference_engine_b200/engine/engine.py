@@ -216,7 +216,8 @@ class Engine:
     # ---------------------------------------------------------------------- step
     def step(self) -> int:
         """One batched step; returns the number of tokens it ran (0 = nothing could run).  What a request's `allowed`
-        raised is raised here, once the step is recorded; that request has ended."""
+        raised is raised here, once the step is recorded; that request has ended.  Its notes (`__notes__`) say which request
+        it was, and what others' raised by then: those have ended too."""
         ran = self._step()
         if self._raised is not None and not self._raises_later:
             raised, self._raised = self._raised, None
@@ -288,7 +289,12 @@ class Engine:
             mask = None if tokens is None else pack_allowed(tokens, self.runner.vocab_size)
             item.ends = mask is not None and not mask.any()
         except Exception as raised:                # the step is under way: it is recorded first
-            self._raised, item.ends = self._raised or raised, True
+            if self._raised is None:
+                self._raised = raised
+                raised.add_note(f"raised by `allowed` of request {seq.id}, which has ended")
+            else:
+                self._raised.add_note(f"request {seq.id} has ended too, its `allowed` raised {raised!r}")
+            item.ends = True
         return None if item.ends else mask
 
     def _resolve(self, items, tokens) -> None:

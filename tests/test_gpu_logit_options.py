@@ -256,6 +256,35 @@ def test_what_a_callback_raises_while_another_request_is_sampled(folders):
     assert all(engine.status(i) is SeqStatus.Finished and not engine.output(i) for i in broken)
 
 
+@pytest.mark.parametrize("pipeline", [True, False])
+def test_what_several_callbacks_raise(folders, pipeline):
+    """The first comes out; its notes say whose it was, and what the others raised, in the same step and in later ones of
+    `add_samples`."""
+    from from_scratch_inference_engine_b200 import SamplingParams, SeqStatus
+    engine = engine_for(folders["A"], pipeline=pipeline)
+
+    def breaks_after(count, error):
+        def allowed(output):
+            if len(output) == count:
+                raise error
+        return allowed
+    errors = [KeyError("one"), ValueError("two"), KeyError("three")]
+    broken = [engine.add_request([5, 6, 7 + i], SamplingParams(temperature=0.0, allowed=breaks_after(i // 2, error)), 5)
+              for i, error in enumerate(errors)]
+    ids = engine.add_samples(helpers.random_ids(256, 40, 3), [SamplingParams(temperature=0.9, seed=i) for i in range(3)], 4)
+    assert len(ids) == 3
+    with pytest.raises(KeyError, match="one") as caught:
+        engine.step()
+    assert caught.value is errors[0]
+    notes = caught.value.__notes__
+    assert len(notes) == 3
+    for rid, note, text in zip(broken, notes, ("request", "ValueError('two')", "KeyError('three')")):
+        assert f"request {rid}" in note and text in note
+    engine.run_until_done()
+    assert [len(engine.output(i)) for i in broken + ids] == [0, 0, 1, 4, 4, 4]
+    assert all(engine.status(i) is SeqStatus.Finished for i in broken)
+
+
 def test_options_are_refused_before_anything_is_kept(folders):
     from from_scratch_inference_engine_b200 import SamplingParams
     engine = engine_for(folders["A"])
