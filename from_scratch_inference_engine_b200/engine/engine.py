@@ -19,7 +19,7 @@ from __future__ import annotations
 import json
 from dataclasses import replace
 from pathlib import Path
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -106,7 +106,7 @@ class Engine:
         self.seed = int(seed)
         self.pipeline = bool(pipeline)
         self._in_flight = None          # (items, Picked) of a launched step whose tokens are not read yet
-        self._raised = None             # what a request's `allowed` raised
+        self._raised: List[Tuple[int, BaseException]] = []      # requests whose `allowed` raised, and what
         self._raises_later = False
         self.steps = 0
         self.tokens_prefilled = 0
@@ -219,9 +219,15 @@ class Engine:
         raised is raised here, once the step is recorded; that request has ended.  Its notes (`__notes__`) say which request
         it was, and what others' raised by then: those have ended too."""
         ran = self._step()
-        if self._raised is not None and not self._raises_later:
-            raised, self._raised = self._raised, None
-            raise raised
+        # (an interrupt, or whatever else is no Exception, comes first and is not kept for later)
+        first = next((i for i, (_, raised) in enumerate(self._raised) if not isinstance(raised, Exception)), -1)
+        if first >= 0 or (self._raised and not self._raises_later):
+            others, self._raised = self._raised, []
+            request, error = others.pop(max(first, 0))
+            error.add_note(f"raised by `allowed` of request {request}, which has ended")
+            for request, raised in others:
+                error.add_note(f"request {request} has ended too, its `allowed` raised {raised!r}")
+            raise error
         return ran
 
     def _step(self) -> int:
@@ -288,12 +294,8 @@ class Engine:
             tokens = seq.params.allowed(seq.output)
             mask = None if tokens is None else pack_allowed(tokens, self.runner.vocab_size)
             item.ends = mask is not None and not mask.any()
-        except Exception as raised:                # the step is under way: it is recorded first
-            if self._raised is None:
-                self._raised = raised
-                raised.add_note(f"raised by `allowed` of request {seq.id}, which has ended")
-            else:
-                self._raised.add_note(f"request {seq.id} has ended too, its `allowed` raised {raised!r}")
+        except BaseException as raised:            # the step is under way: it is recorded first
+            self._raised.append((seq.id, raised))
             item.ends = True
         return None if item.ends else mask
 

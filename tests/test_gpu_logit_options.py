@@ -285,6 +285,45 @@ def test_what_several_callbacks_raise(folders, pipeline):
     assert all(engine.status(i) is SeqStatus.Finished for i in broken)
 
 
+@pytest.mark.parametrize("pipeline", [True, False])
+def test_a_callback_that_is_interrupted(folders, pipeline):
+    """What is no Exception comes out of `step` as well once the step is recorded, in front of what others raised, and of
+    `add_samples` at once; the others lose nothing."""
+    from from_scratch_inference_engine_b200 import SamplingParams, SeqStatus
+
+    class Stop(BaseException):
+        pass
+    engine = engine_for(folders["A"], pipeline=pipeline)
+    prompts = [helpers.random_ids(256, n, n) for n in (6, 5, 4)]      # one step's tokens
+
+    def breaks_after(count, error):
+        def allowed(output):
+            if len(output) == count:
+                raise error
+        return allowed
+    greedy = SamplingParams(temperature=0.0)
+    params = [greedy, SamplingParams(temperature=0.0, allowed=breaks_after(3, KeyError("other"))),
+              SamplingParams(temperature=0.0, allowed=breaks_after(3, Stop("now")))]
+    ids = [engine.add_request(p, q, 9) for p, q in zip(prompts, params)]
+    with pytest.raises(Stop, match="now") as caught:
+        engine.run_until_done()
+    assert [f"request {i}" in note for i, note in zip((ids[2], ids[1]), caught.value.__notes__)] == [True, True]
+    engine.run_until_done()
+    assert [len(engine.output(i)) for i in ids] == [9, 3, 3]
+    alone = engine_for(folders["A"])
+    for rid, prompt in zip(ids, prompts):
+        assert engine.output(rid) == alone.generate(prompt, greedy, 9)[:len(engine.output(rid))]
+    stopping = engine.add_request(prompts[0], params[2], 9)
+    prompt = helpers.random_ids(256, 100, 3)
+    with pytest.raises(Stop, match="now"):
+        engine.add_samples(prompt, [greedy] * 2, 4)
+    engine.run_until_done()
+    assert engine.status(stopping) is SeqStatus.Finished and len(engine.output(stopping)) == 3
+    assert engine.output(stopping + 1) == alone.generate(prompt, greedy, 4)
+    engine.runner.cache.check()
+    assert engine.runner.cache.slots.num_free == 8 and len(engine.history) == 0
+
+
 def test_options_are_refused_before_anything_is_kept(folders):
     from from_scratch_inference_engine_b200 import SamplingParams
     engine = engine_for(folders["A"])
