@@ -192,7 +192,9 @@ class Engine:
     def warm_up(self, max_context: int = 0) -> int:
         """Before serving starts: run one step of the largest size (its working memory then
         stays with the allocator) and capture the decode graphs for contexts of up to
-        `max_context` tokens (default: what one request may hold); returns their number."""
+        `max_context` tokens (default: what one request may hold); returns their number.
+        Histories of tokens are not among it: `history.reserve` takes their memory, or the steps
+        in which requests with penalties choose their first token."""
         if not self.has_work():
             self.runner.reserve_step_memory()
         limit = max_context or min(self.runner.cache.max_tokens_per_request(), self.runner.max_positions)
@@ -265,15 +267,17 @@ class Engine:
                              [len(item.tokens) - 1] if item.samples else [], item.source_row)
                    for item in items]
         before = self._in_flight[1].device if self._in_flight is not None else None
-        logits = self.runner.step(entries, before)
         sampling = [item for item in items if item.samples]
+        penalised = [item.seq for item in sampling if item.seq.params.penalised]
+        # (without room for a history nothing has run: the step can be tried again)
+        self.history.reserve([seq.id for seq in penalised])
+        logits = self.runner.step(entries, before)
         if not sampling:
             return None
         params = [i.seq.params for i in sampling]
         slots = masks = biases = None
-        if any(p.penalised for p in params):
-            known = iter(self.history.slots([(i.seq.id, i.seq.prompt, i.seq.output) for i in sampling
-                                             if i.seq.params.penalised], self.runner.error))
+        if penalised:
+            known = iter(self.history.slots([(seq.id, seq.prompt, seq.output) for seq in penalised], self.runner.error))
             slots = [next(known) if p.penalised else -1 for p in params]
         if any(p.allowed is not None for p in params):
             if self._in_flight is not None:        # the answers so far are needed; the GPU runs this step meanwhile

@@ -324,6 +324,38 @@ def test_a_callback_that_is_interrupted(folders, pipeline):
     assert engine.runner.cache.slots.num_free == 8 and len(engine.history) == 0
 
 
+@pytest.mark.parametrize("pipeline", [True, False])
+def test_no_memory_for_a_history(folders, pipeline, monkeypatch):
+    """It comes out of `step` before anything of the step has run: tried again, every request gives the tokens that it gives alone."""
+    from from_scratch_inference_engine_b200 import SamplingParams
+    from from_scratch_inference_engine_b200.sampling import TokenHistory
+    engine = engine_for(folders["A"], pipeline=pipeline, num_blocks=200, max_batch=20, max_step_tokens=40)
+    params = [SamplingParams(temperature=0.0, **PARAMS[i % 4]) for i in range(18)]
+    prompts = [helpers.random_ids(256, 3 + i, i) for i in range(18)]
+    grow, fails = TokenHistory._grow, [0]
+
+    def scarce(self, slots):
+        if len(self._free) < slots and fails[0] < 6:               # three times for the first slots, twice for more
+            fails[0] += 1
+            if fails[0] % 4:
+                raise torch.OutOfMemoryError("CUDA out of memory")
+        return grow(self, slots)
+    monkeypatch.setattr(TokenHistory, "_grow", scarce)
+    ids = [engine.add_request(p, q, 7) for p, q in zip(prompts, params)]
+    raised = 0
+    while engine.has_work():
+        try:
+            assert engine.step() > 0
+        except torch.OutOfMemoryError:
+            raised += 1
+    assert raised == 5 and fails[0] == 6
+    engine.runner.cache.check()
+    assert engine.runner.cache.slots.num_free == 20 and len(engine.history) == 0
+    alone = engine_for(folders["A"], num_blocks=200)
+    for rid, prompt, own in zip(ids, prompts, params):
+        assert engine.output(rid) == alone.generate(prompt, own, 7)
+
+
 def test_options_are_refused_before_anything_is_kept(folders):
     from from_scratch_inference_engine_b200 import SamplingParams
     engine = engine_for(folders["A"])
