@@ -9,8 +9,8 @@ Most kernels are launched while the kernel before them on the stream still runs,
 wait what a step does not change: weights, gains, biases, scales and tables, the request lists and block tables, a
 recurrence's state, the keys and values in front of the requests' new tokens.  Where the stream's last kernel may have
 made one of these, the function has an argument `early`: False, the default, and its kernel starts behind that one; True
-says that all of them are older than the stream's last kernel (and that this is not `attention_tc_decode`, which may still
-run beside the kernel in front of it).  The functions without the argument (`gemm_skinny` and its forms, `gemm_decode`,
+says that all of them are older than the stream's last kernel, and where that is `attention_tc_decode`, which may still
+run beside the kernel in front of it, older than that one as well.  The functions without the argument (`gemm_skinny` and its forms, `gemm_decode`,
 `add_rmsnorm`, `row_decay`, and those that read no more than positions and lists early) always need them that old.
 """
 
@@ -2599,7 +2599,8 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
     what there is, a token whose innermost run or one around that does not hold its place (a run of no places does no harm),
     or a shared run that reaches beyond one of its tokens, sets error[0] to 7, a page outside the pool to 3 (its keys are left
     out), runs that nest deeper than `room` was made for to 8; the rows concerned hold no result.  `early`: the lists, tables
-    and positions are older than the stream's last kernel."""
+    and positions are older than the stream's last kernel, and behind `attention_tc_decode` older than the kernel in front
+    of that (as what is staged before a step's first kernel is)."""
     dtype, device = q.dtype, _device()
     if not (_all_fit(device, torch.int32, True, block_tables, positions, order, runs, own_run, error)
             and _all_fit(device, dtype, False, q, k_pages, v_pages, out) and _all_fit(device, torch.uint8, True, room)):

@@ -153,7 +153,8 @@ class GqaAttention(Mixer):
 
     def _attend_shared(self, ctx, qkv: torch.Tensor, group, cache: LayerCache, out: torch.Tensor, lists) -> None:
         """Attention of the requests of one token, with keys that several of them hold read once for all.  Behind `_attend`,
-        whose 32-bit form may leave anything in these tokens' rows."""
+        whose 32-bit form may leave anything in these tokens' rows, and which may end with `ops.attention_tc_decode`: the lists
+        are staged before the step's first kernel, so they are read early all the same."""
         room = self._shared_room(lists.order.shape[0], lists.runs.shape[0], lists.shared, lists.levels)
         ops.shared_attention(qkv, qkv.stride(0), cache.k_pages, cache.v_pages, cache.page_stride, group.page_size,
                              group.block_tables, ctx.positions, lists.order, lists.runs, lists.own_run, out, self.num_heads,

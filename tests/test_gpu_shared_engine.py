@@ -218,3 +218,29 @@ def test_captured_steps_find_the_working_memory_that_was_taken(folders, calls, r
     step(runner, *[(handle, [5]) for handle in handles])
     assert len(runner._graphs) == 2 * len(graphs) + 1
     assert runner.runtime._buffers["attention.shared_room", torch.uint8] is room
+
+
+def test_behind_the_attention_that_lets_its_successor_go_early(folders, monkeypatch):
+    """Requests of two tokens on `attention_tc_decode` in front of those of one that share keys, step after step."""
+    from from_scratch_inference_engine_b200.kernels import ops
+    runner = runner_of(folders["F"], "bfloat16", 16)
+    runner.runtime.decode_tcgen05_min_blocks = 1
+    order = []
+    for name in ("attention_tc_decode", "shared_attention"):
+        monkeypatch.setattr(ops, name, lambda *args, real=getattr(ops, name), name=name, **kwargs: (order.append(name), real(*args, **kwargs))[1])
+    prompt = helpers.random_ids(300, 100, 1)
+    parent = runner.cache.open("parent")
+    step(runner, (parent, prompt))
+    handles = [parent] + runner.fork(parent, list("bcdefg"))
+    seqs = [list(prompt) for _ in handles]
+    apart = [runner.cache.open(f"apart {i}") for i in range(9)]
+    handles += apart
+    seqs += [[] for _ in apart]
+    for turn in range(6):
+        order.clear()
+        fresh = [helpers.random_ids(300, 1 if i < 7 else 2, 100 * turn + i) for i in range(len(handles))]
+        rows = step(runner, *zip(handles, fresh))
+        assert order == ["attention_tc_decode", "shared_attention"] * 2
+        for seq, more in zip(seqs, fresh):
+            seq += more
+        check("F", folders["F"], "bfloat16", seqs, rows)
