@@ -14,7 +14,7 @@
 // 19 KB of bits per history and mask, against 608 KB of logits and as much of counts).  A warp owns 1,024 tokens, a word of 32
 // bits to a lane.  The tokens that the history holds and the mask allows go into a list, so that a lane has one of them and all
 // of a warp's logits and counts are asked for at once; what the mask forbids is written without a read, a word's 32 tokens side
-// by side.  64 rows of 152,064 tokens with 1,500 in every history, 22 of them masked: 6.4 us, where 16 bytes were written at a
+// by side.  64 rows of 152,064 tokens with 1,500 in every history, 22 of them masked, 40 biases: 6.6 us, where 16 bytes were written at a
 // time and single tokens where a word is mixed 9.2, and threads that walked four groups of four tokens each, with a wait at each,
 // took 12.0; 200 rows with 800 in every history 8.7, those threads 21.7.  Blocks of 2, 4, 8 warps (of the form before): 8.3, 9.2,
 // 10.2 us for those 64 rows, 16.1, 9.1, 8.0 for those 200.

@@ -30,7 +30,7 @@
 // What a small call waits for is a chain of reads of what other multiprocessors hold, 750 cycles each, and instructions that
 // run for the first time.  8 requests of a 4,096-token prompt, 28 heads over 4 of 128: 23.9 us with a launch for the plan in
 // front, one each for many and few rows and one for the merge; 31.5 in one cooperative launch whose blocks meet twice
-// (6 of them between two such launches); 20.7 in two, and 16.0 since their code is shorter and more of their warps join.
+// (6 of them between two such launches); 20.7 in two, and 15.2 since their code is shorter and more of their warps join.
 #include "common.cuh"
 #include "tma.cuh"
 #include "attention_tc.cuh"
@@ -1925,14 +1925,14 @@ static int launch(const Shape& shape, const CUtensorMap& k_map, const CUtensorMa
 }
 
 // Few rows in all: a row to a unit and several warps on it, since what such a call waits for is one warp's chain of loads.
-// More: what counts are instructions, and a warp takes several heads of a kv head together.  The whole call in us, 28 heads over
-// 4 of 128, for <rows of a unit, warps on it>:
+// More: what counts are instructions, and a warp takes several heads of a kv head together.  The whole call in a graph in us,
+// 28 heads over 4 of 128, 16 to 256 keys of their own, for <rows of a unit, warps on it>:
 //   requests x keys in common    rows    <1,4>  <1,2>  <2,2>  <8,1>
-//   8 x 4,096                     224     19.2   20.0   22.4   40.3
-//   16 x 1,024                    448     16.1   13.2   13.6   20.9
-//   32 x 1,024                    896     24.1   16.0   16.5   23.3
-//   64 x 2,048                  1,792     52.8   40.6   39.1   52.9
-//   128 x 128                   3,584     52.1   34.4   27.9   19.4
+//   8 x 4,096                     224     15.0   15.6   17.8   32.5
+//   16 x 1,024                    448     14.0   12.6   13.1   20.3
+//   32 x 1,024                    896     18.2   15.3   15.8   22.6
+//   64 x 2,048                  1,792     35.4   31.1   28.7   37.0
+//   128 x 128                   3,584     34.8   25.9   23.0   20.3
 // Up to four blocks to a multiprocessor.
 template <typename T, int ROWS, int SPLIT>
 static int launch_merge_as(SharedArgs& a, int blocks, cudaStream_t stream) {

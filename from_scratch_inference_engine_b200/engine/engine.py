@@ -92,8 +92,9 @@ class Engine:
                  seed: int = 0, max_batch: int = 256, enable_prefix_cache: bool = False,
                  max_step_tokens: int = 2048, pipeline: bool = True, shared_attention: bool = False):
         """`shared_attention`: keys that several running requests hold (answers to one prompt, prompts with a common
-        beginning under the prefix cache) are read once for all of them in the steps where that pays, which rounds a little
-        differently than when each reads for itself."""
+        beginning under the prefix cache) are read once for all of them in the steps where that pays on the GPU, which rounds
+        a little differently than when each reads for itself.  The host looks for them every step: 0.1 ms for 200 answers to
+        one prompt, 1 ms for 32 prompts of 8 answers each, 3.5 ms for 128 of 2."""
         self.model = model
         self.runner = ModelRunner(model.model, model.runtime, page_size=block_size,
                                   num_pages=num_blocks, max_requests=max_batch,

@@ -177,7 +177,8 @@ class ModelRunner:
         # 15.1 / 15.4, 4 x 8,192 (50 MB) 18.0 / 17.1, 8 x 4,096 (59 MB) 18.8 / 15.0, 64 x 512 (66 MB) 19.7 / 18.4, 128 x 512
         # (133 MB) 37.2 / 23.8; float32 8 x 2,048 of 12 heads over 2 (29 MB) 20.8 / 18.8, 8 x 4,096 (59 MB) 43 / 22.  By the part:
         # 64 requests that share 16 keys (nothing) beside 1,024 to 2,048 of their own 44.1 / 45.2, 8 x 2,048 and 56 such requests
-        # (0.13) 69.3 / 46.4, 64 x 512 beside as many of their own (a quarter) 52.8 / 45.9.
+        # (0.13) 69.3 / 46.4, 64 x 512 beside as many of their own (a quarter) 52.8 / 45.9.  (The forms on mma.sync, of other head
+        # sizes and pages, go by the same two numbers and were not measured for it; float32 would pay from less on.)
         self.shared_min_bytes = 40 << 20
         self.shared_min_part = 0.1
         self.shared_least_keys = 64          # ... and of every single run so many keys

@@ -2587,7 +2587,7 @@ def shared_attention(q: torch.Tensor, q_ld: int, k_pages: torch.Tensor, v_pages:
     page_size, head_dim] (views; page p begins p * page_stride elements further), block_tables int32 [requests, width],
     positions int32 [tokens].  Every key that a token sees lies in one run:
 
-    order    int32 [n], the tokens to work on, so arranged that the tokens of every run are neighbours
+    order    int32 [n], the tokens to work on, each once, so arranged that the tokens of every run are neighbours
     runs     int32 [r, 6]: first place in order, number of places, first key, end of the keys, row of block_tables that has
              their pages, index of the run around it or -1 (a run comes behind the run around it).  Its keys are behind those
              of the run around it
